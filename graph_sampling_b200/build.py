@@ -61,14 +61,16 @@ def build(force: bool = False, verbose: bool = False) -> str:
 
 GLUE_SRC = os.path.join(CSRC, "glue", "gs_glue.cc")
 GLUE_LIB = os.path.join(LIBDIR, "libgs.so")
-NATIVE_SRC = os.path.join(CSRC, "glue", "gs_native.cc")
+NATIVE_SRCS = [os.path.join(CSRC, "glue", "gs_native.cc"), os.path.join(CSRC, "glue", "gs_rows.cc")]
 NATIVE_LIB = os.path.join(LIBDIR, "_gsb_native.so")
 
 
-def _build_against_torch(src, lib, extra_libs, force):
+def _build_against_torch(srcs, lib, extra_libs, force):
     """g++ over the C ABI and the torch headers; links against libgsb200.so (found next to it through $ORIGIN)."""
     build(force=False)
-    deps = [src, os.path.join(os.path.dirname(PKG), "include", "gsb200.h")]
+    glue = os.path.join(CSRC, "glue")
+    deps = srcs + [os.path.join(glue, f) for f in os.listdir(glue) if f.endswith(".h")]
+    deps.append(os.path.join(os.path.dirname(PKG), "include", "gsb200.h"))
     if not force and os.path.exists(lib) and all(os.path.getmtime(lib) >= os.path.getmtime(d) for d in deps):
         return lib
     import sysconfig
@@ -77,7 +79,7 @@ def _build_against_torch(src, lib, extra_libs, force):
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-w",
            "-I", os.path.join(tdir, "include"), "-I", os.path.join(tdir, "include", "torch", "csrc", "api", "include"),
-           "-I", sysconfig.get_paths()["include"], "-I", "/usr/local/cuda/include", src, "-o", lib,
+           "-I", sysconfig.get_paths()["include"], "-I", "/usr/local/cuda/include", *srcs, "-o", lib,
            "-L", LIBDIR, "-lgsb200", "-Wl,-rpath,$ORIGIN", "-L", os.path.join(tdir, "lib"), *extra_libs, "-ltorch",
            "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", "-Wl,-rpath," + os.path.join(tdir, "lib"),
            "-L", "/usr/local/cuda/lib64", "-lcudart"]
@@ -87,12 +89,12 @@ def _build_against_torch(src, lib, extra_libs, force):
 
 def build_glue(force: bool = False) -> str:
     """Builds lib/libgs.so: the TorchScript front end (gs_classes.Graph, gs_ops.*)."""
-    return _build_against_torch(GLUE_SRC, GLUE_LIB, [], force)
+    return _build_against_torch([GLUE_SRC], GLUE_LIB, [], force)
 
 
 def build_native(force: bool = False) -> str:
     """Builds lib/_gsb_native.so: the extension module behind graph_sampling_b200.ops."""
-    return _build_against_torch(NATIVE_SRC, NATIVE_LIB, ["-ltorch_python"], force)
+    return _build_against_torch(NATIVE_SRCS, NATIVE_LIB, ["-ltorch_python"], force)
 
 
 if __name__ == "__main__":

@@ -88,6 +88,10 @@ enum KernelId {
   KID_PART_RESOLVE,
   KID_FIRST_BITS,
   KID_RANK_EMIT,
+  KID_KEY_SORT,
+  KID_EMBED_LOOKUP,
+  KID_EMBED_GRAD,
+  KID_EXPERT_ROWS,
   KID_OTHER,
   KID_NUM
 };

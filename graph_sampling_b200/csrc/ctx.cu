@@ -608,7 +608,8 @@ const char* gsb_profile_kernel_name(int kid) {
       "count_scan",     "slice_fill",   "sample_uniform", "sample_keepdim", "sample_weighted", "table_clear",
       "table_insert",   "first_compact", "relabel",       "random_walk",    "sddmm_dot",       "sddmm_generic",
       "segment",        "row_filter",   "list_sample",    "sort",           "format",          "partition_count",
-      "partition_scatter", "bucket_resolve", "first_bits",  "rank_emit",      "other"};
+      "partition_scatter", "bucket_resolve", "first_bits",  "rank_emit",      "key_sort",        "embed_lookup",
+      "embed_grad",     "expert_rows",  "other"};
   return (kid >= 0 && kid < gsb::KID_NUM) ? names[kid] : "";
 }
 

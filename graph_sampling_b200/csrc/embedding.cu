@@ -1,0 +1,385 @@
+// Embedding rows: lookup by id with scaling, and the gradient of the table.
+//
+// Lookup: out[i, :] = scale * table[ids[i], :], one rounding.
+// Gradient: total[v, :] = scale * (sum of grad[i, :] over the positions i with ids[i] == v), summed in float in the order of the
+// positions within pieces that depend on sizes alone, so the same inputs give the same bits; one rounding.  The positions are
+// sorted by id (key_sort.cuh); the sorted list is cut into chunks of equal length whoever the ids are, so a frequent id is
+// shared by many groups of lanes.  A sum that begins and ends inside a chunk is written at once; what reaches over a chunk's
+// ends goes to `part` and is added up by k_join_rows.
+#include <type_traits>
+
+#include "key_sort.cuh"
+#include "row_values.cuh"
+#include "scan.cuh"
+
+namespace gsb {
+
+constexpr int kLookupThreads = 256;
+constexpr u32 kNoRow = 0xffffffffu;
+
+template <class T, int BYTES>
+__global__ void __launch_bounds__(kLookupThreads) k_lookup_rows(const Unit<T, BYTES>* __restrict__ table, i64 num_rows,
+                                                                i64 stride, i64 units, const i64* __restrict__ ids, i64 n,
+                                                                float scale, bool has_padding, i64 padding, int lanes,
+                                                                Unit<T, BYTES>* __restrict__ out, i64* counters) {
+  const int lane = threadIdx.x & (lanes - 1);
+  const i64 groups = (i64)gridDim.x * (kLookupThreads / lanes);
+  for (i64 i = ((i64)blockIdx.x * kLookupThreads + threadIdx.x) / lanes; i < n; i += groups) {
+    i64 row = __ldg(ids + i);
+    if ((u64)row >= (u64)num_rows || (has_padding && row == padding)) {
+      if (lane == 0 && !(has_padding && row == padding)) raise_error(counters, GSB_ERR_INDEX_RANGE, i);
+      row = -1;
+    }
+    for (i64 j = lane; j < units; j += lanes) {
+      Unit<T, BYTES> v;
+      if (row >= 0) {
+        v = load_unit(table + row * stride + j);
+#pragma unroll
+        for (int q = 0; q < v.N; ++q) v.v[q] = from_float<T>(to_float(v.v[q]) * scale);
+      } else {
+#pragma unroll
+        for (int q = 0; q < v.N; ++q) v.v[q] = from_float<T>(0.f);
+      }
+      store_unit(out + i * units + j, v);
+    }
+  }
+}
+
+// N values of `to`, 16 bytes at a time where they are that many.
+template <class O, int N>
+__device__ __forceinline__ void store_values(O* to, const float* v, float scale) {
+  constexpr int kBytes = N * (int)sizeof(O), kUnit = kBytes > 16 ? 16 : kBytes, kPer = kUnit / (int)sizeof(O);
+#pragma unroll
+  for (int p = 0; p < N / kPer; ++p) {
+    Unit<O, kUnit> u;
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) u.v[q] = from_float<O>(v[p * kPer + q] * scale);
+    store_unit((Unit<O, kUnit>*)(to + p * kPer), u);
+  }
+}
+
+constexpr int kSumThreads = 128;
+
+struct SumArgs {
+  i64 n;          // sorted positions
+  int chunk;      // positions per group of lanes
+  int lanes;      // per group, a power of two
+  u32 num_rows;   // of the result: a position whose row is not below that belongs to no sum
+  i64 units;      // per row
+  i64 stride;     // of `grad`, in units
+  float scale;
+};
+
+// One group of lanes per chunk and column tile (blockIdx.y) of lanes * STEPS units.
+template <class T, class O, int BYTES, int STEPS>
+__global__ void __launch_bounds__(kSumThreads) k_sum_rows(const SumArgs a, const Unit<T, BYTES>* __restrict__ grad,
+                                                          const u32* __restrict__ at, const u32* __restrict__ row,
+                                                          O* __restrict__ out, float* __restrict__ part) {
+  constexpr int N = Unit<T, BYTES>::N, kAhead = STEPS >= 4 ? 2 : 4;
+  const i64 chunk = ((i64)blockIdx.x * kSumThreads + threadIdx.x) / a.lanes;
+  const i64 begin = chunk * a.chunk, end = min(begin + a.chunk, a.n);
+  const i64 first = (i64)blockIdx.y * a.lanes * STEPS + (threadIdx.x & (a.lanes - 1));
+  if (begin >= a.n) return;
+  const i64 width = a.units * N;
+  float sum[STEPS][N] = {};
+  bool head = begin > 0 && row[begin - 1] == row[begin];
+  auto put = [&](auto* to, float scale) {
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      const i64 unit = first + s * a.lanes;
+      if (unit < a.units) store_values<std::remove_pointer_t<decltype(to)>, N>(to + unit * N, sum[s], scale);
+#pragma unroll
+      for (int q = 0; q < N; ++q) sum[s][q] = 0.f;
+    }
+  };
+  for (i64 j = begin; j < end; j += kAhead) {
+    u32 r[kAhead + 1];
+    Unit<T, BYTES> v[kAhead][STEPS];
+#pragma unroll
+    for (int u = 0; u <= kAhead; ++u) r[u] = j + u < a.n ? row[j + u] : kNoRow;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (j + u >= end || r[u] >= a.num_rows) continue;
+      const Unit<T, BYTES>* from = grad + (i64)at[j + u] * a.stride;
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s)
+        if (first + s * a.lanes < a.units) v[u][s] = load_unit_once(from + first + s * a.lanes);
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (j + u >= end || r[u] >= a.num_rows) return;  // the sorted list ends with the positions that belong to no row
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s)
+        if (first + s * a.lanes < a.units)
+#pragma unroll
+          for (int q = 0; q < N; ++q) sum[s][q] += to_float(v[u][s].v[q]);
+      const bool ends = r[u + 1] != r[u];
+      if (ends && !head) put(out + (i64)r[u] * width, a.scale);
+      else if (ends || j + u + 1 == end) put(part + (2 * chunk + (head ? 0 : 1)) * width, 1.f);
+      if (ends) head = false;
+    }
+  }
+}
+
+// Where the last sum of a chunk began there and goes on: its part and those of the chunks behind, in their order.
+template <class O>
+__global__ void __launch_bounds__(kSumThreads) k_join_rows(const SumArgs a, i64 width, i64 chunks, const u32* __restrict__ row,
+                                                           const float* __restrict__ part, O* __restrict__ out) {
+  const i64 column = (i64)blockIdx.y * kSumThreads + threadIdx.x;
+  for (i64 c = blockIdx.x; c + 1 < chunks; c += gridDim.x) {
+    const i64 begin = c * a.chunk, end = begin + a.chunk;
+    const u32 r = row[end - 1];
+    if (r >= a.num_rows || row[end] != r || (begin > 0 && row[begin - 1] == r)) continue;
+    if (column >= width) continue;
+    float sum = part[(2 * c + 1) * width + column];
+    for (i64 next = c + 1; next < chunks && row[next * a.chunk] == r; ++next) sum += part[2 * next * width + column];
+    out[(i64)r * width + column] = from_float<O>(sum * a.scale);
+  }
+}
+
+// The sorted keys' ranks among the distinct ones.
+constexpr int kHeadThreads = 1024;
+
+__device__ __forceinline__ bool is_head(const u32* key, i64 i, i64 n, u32 num_keys) {
+  return i < n && key[i] < num_keys && (i == 0 || key[i - 1] != key[i]);
+}
+
+__global__ void __launch_bounds__(kHeadThreads) k_head_count(const u32* __restrict__ key, i64 n, u32 num_keys,
+                                                             u32* __restrict__ count) {
+  const i64 i = (i64)blockIdx.x * kHeadThreads + threadIdx.x;
+  const int heads = __syncthreads_count(is_head(key, i, n, num_keys));
+  if (threadIdx.x == 0) count[blockIdx.x] = heads;
+}
+
+__global__ void __launch_bounds__(kHeadThreads) k_head_rank(const u32* __restrict__ key, i64 n, u32 num_keys,
+                                                            const u32* __restrict__ count, u32* __restrict__ rank,
+                                                            i64* __restrict__ ids, i64* __restrict__ total, Mail mail,
+                                                            const i64* counters) {
+  __shared__ i64 s_scan[33];
+  i64 before = 0;
+  for (int t = threadIdx.x; t < (int)blockIdx.x; t += kHeadThreads) before += count[t];
+  i64 base;
+  block_exclusive_scan<kHeadThreads>(before, s_scan, &base);
+  const i64 i = (i64)blockIdx.x * kHeadThreads + threadIdx.x;
+  const bool head = is_head(key, i, n, num_keys);
+  i64 heads;
+  const i64 excl = block_exclusive_scan<kHeadThreads>((i64)head, s_scan, &heads);
+  const i64 mine = base + excl + (head ? 1 : 0) - 1;  // of the latest head up to here
+  if (i < n) rank[i] = key[i] < num_keys ? (u32)mine : kNoRow;
+  if (head) ids[mine] = key[i];
+  if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) {
+    total[0] = base + heads;
+    mail_post(mail, 0, base + heads, counters);
+  }
+}
+
+// Chunks: long enough that their ends are few beside what is read, short enough that there are many of them.
+static int sum_chunk(i64 n) {
+  i64 c = (n / 16384 + 31) / 32 * 32;
+  return (int)(c < 32 ? 32 : c);
+}
+
+struct GradPlan {
+  size_t sort_bytes, total_bytes;
+  i64 chunks;
+  int chunk;
+};
+
+static GradPlan grad_plan(i64 n, i64 num_rows, i64 row_len) {
+  GradPlan g;
+  g.chunk = sum_chunk(n);
+  g.chunks = (n + g.chunk - 1) / g.chunk;
+  g.sort_bytes = key_sort_bytes(n, num_rows);
+  Pieces p(nullptr);
+  p.take<char>(g.sort_bytes);
+  p.take<float>((size_t)g.chunks * 2 * (size_t)row_len);
+  p.take<u32>((size_t)(n + kHeadThreads - 1) / kHeadThreads);
+  p.take<i64>(1);
+  g.total_bytes = p.used;
+  return g;
+}
+
+template <class T, class O, int BYTES>
+static void launch_sum(cudaStream_t stream, SumArgs a, i64 chunks, const void* grad, i64 stride_bytes, i64 row_bytes,
+                       const SortedKeys& sorted, const u32* row, void* out, float* part) {
+  a.units = row_bytes / BYTES;
+  a.stride = stride_bytes / BYTES;
+  a.lanes = 1;
+  while (a.lanes < 32 && a.lanes < a.units) a.lanes *= 2;
+  auto go = [&](auto steps) {
+    constexpr int S = decltype(steps)::value;
+    const dim3 grid(grid_for(chunks * a.lanes, kSumThreads), grid_for(a.units, a.lanes * S));
+    k_sum_rows<T, O, BYTES, S><<<grid, kSumThreads, 0, stream>>>(a, (const Unit<T, BYTES>*)grad, sorted.at, row, (O*)out, part);
+  };
+  if (a.units <= 32) go(std::integral_constant<int, 1>{});
+  else if (a.units <= 64) go(std::integral_constant<int, 2>{});
+  else go(std::integral_constant<int, 4>{});
+}
+
+struct GradCall {
+  const void* grad;
+  int dtype;
+  i64 row_len, grad_stride;
+  float scale;
+  void* out;
+  int out_dtype;
+};
+
+// Sums of the sorted rows into out[row[j], :].
+static int sum_sorted(gsb_ctx* ctx, cudaStream_t stream, const GradCall& c, const GradPlan& plan, const SortedKeys& sorted,
+                      const u32* row, i64 n, i64 num_rows, float* part) {
+  const int size = value_bytes(c.dtype), out_size = value_bytes(c.out_dtype);
+  const i64 row_bytes = c.row_len * size, stride_bytes = c.grad_stride * size;
+  int unit = unit_bytes(row_bytes, (u64)(uintptr_t)c.grad | (u64)stride_bytes);
+  while (unit > size && (uintptr_t)c.out % min(16, unit / size * out_size) != 0) unit /= 2;
+  SumArgs a{n, plan.chunk, 32, (u32)num_rows, 0, 0, c.scale};
+  ScopedKernelTimer timer(ctx, KID_EMBED_GRAD, stream);
+  with_unit(c.dtype, unit, [&](auto value, auto bytes) {
+    typedef decltype(value) T;
+    constexpr int kBytes = decltype(bytes)::value;
+    if (c.out_dtype == c.dtype)
+      launch_sum<T, T, kBytes>(stream, a, plan.chunks, c.grad, stride_bytes, row_bytes, sorted, row, c.out, part);
+    else
+      launch_sum<T, float, kBytes>(stream, a, plan.chunks, c.grad, stride_bytes, row_bytes, sorted, row, c.out, part);
+  });
+  GSB_LAUNCH_OK();
+  if (plan.chunks > 1) {
+    const dim3 grid((unsigned)min(plan.chunks - 1, (i64)kNumSMs * 16), grid_for(c.row_len, kSumThreads));
+    if (c.out_dtype == GSB_F32) k_join_rows<float><<<grid, kSumThreads, 0, stream>>>(a, c.row_len, plan.chunks, row, part, (float*)c.out);
+    else if (c.out_dtype == GSB_F16) k_join_rows<__half><<<grid, kSumThreads, 0, stream>>>(a, c.row_len, plan.chunks, row, part, (__half*)c.out);
+    else k_join_rows<__nv_bfloat16><<<grid, kSumThreads, 0, stream>>>(a, c.row_len, plan.chunks, row, part, (__nv_bfloat16*)c.out);
+    GSB_LAUNCH_OK();
+    ctx_count_launches(ctx, 1);
+  }
+  return GSB_OK;
+}
+
+// What the calls that sum gradients ask of their arguments.
+static int check_grad(i64 n, i64 num_rows, i64 row_len, i64 grad_stride, int dtype, int out_dtype) {
+  GSB_REQUIRE(n >= 0 && n < ((i64)1 << 31) && num_rows >= 0 && num_rows < 0xffffffffll, GSB_ERR_INVALID_ARGUMENT);
+  GSB_REQUIRE(row_len >= 1 && row_len <= ((i64)1 << 31) && grad_stride >= 0, GSB_ERR_INVALID_ARGUMENT);
+  GSB_REQUIRE(value_bytes(dtype) != 0 && (out_dtype == dtype || out_dtype == GSB_F32), GSB_ERR_INVALID_ARGUMENT);
+  return GSB_OK;
+}
+
+}  // namespace gsb
+
+using namespace gsb;
+
+extern "C" int gsb_embedding_lookup(gsb_ctx* ctx, void* stream_, const void* table, int dtype, int64_t num_rows,
+                                    int64_t row_len, int64_t row_stride, const int64_t* ids, int64_t n, float scale,
+                                    int has_padding, int64_t padding_id, void* out) {
+  GSB_ENTER(ctx);
+  GSB_REQUIRE(num_rows >= 0 && row_len >= 1 && row_stride >= 0 && n >= 0 && value_bytes(dtype) != 0, GSB_ERR_INVALID_ARGUMENT);
+  if (n == 0) return GSB_OK;
+  GSB_REQUIRE((table || num_rows == 0) && ids && out, GSB_ERR_INVALID_ARGUMENT);
+  const void* from = nullptr;
+  if (num_rows > 0) {  // device memory, or page-locked host memory by the address that the device uses for it
+    cudaPointerAttributes attr;
+    GSB_CUDA_OK(cudaPointerGetAttributes(&attr, table));
+    GSB_REQUIRE(attr.devicePointer != nullptr && (attr.type == cudaMemoryTypeDevice || attr.type == cudaMemoryTypeHost ||
+                                                  attr.type == cudaMemoryTypeManaged),
+                GSB_ERR_INVALID_ARGUMENT);
+    from = attr.devicePointer;
+  }
+  cudaStream_t stream = (cudaStream_t)stream_;
+  const int size = value_bytes(dtype);
+  const int unit = unit_bytes(row_len * size, (u64)(uintptr_t)from | (u64)(uintptr_t)out | (u64)(row_stride * size));
+  {
+    ScopedKernelTimer timer(ctx, KID_EMBED_LOOKUP, stream);
+    with_unit(dtype, unit, [&](auto value, auto bytes) {
+      typedef decltype(value) T;
+      constexpr int kBytes = decltype(bytes)::value;
+      const i64 units = row_len * size / kBytes;
+      int lanes = 1;
+      while (lanes < 32 && lanes < units) lanes *= 2;
+      const int grid = (int)min((i64)kNumSMs * 32, (i64)grid_for(n * lanes, kLookupThreads));
+      k_lookup_rows<T, kBytes><<<grid, kLookupThreads, 0, stream>>>((const Unit<T, kBytes>*)from, num_rows,
+                                                                   row_stride * size / kBytes, units, ids, n, scale,
+                                                                   has_padding != 0, padding_id, lanes,
+                                                                   (Unit<T, kBytes>*)out, ctx_counters(ctx));
+    });
+  }
+  GSB_LAUNCH_OK();
+  return GSB_OK;
+}
+
+extern "C" int64_t gsb_embedding_grad_workspace(int64_t n, int64_t num_rows, int64_t row_len) {
+  const int st = check_grad(n, num_rows, row_len, row_len, GSB_F32, GSB_F32);
+  return st != GSB_OK ? st : (int64_t)grad_plan(n, num_rows, row_len).total_bytes;
+}
+
+extern "C" int gsb_embedding_grad(gsb_ctx* ctx, void* stream_, const void* grad, int dtype, int64_t row_len,
+                                  int64_t grad_stride, const int64_t* ids, int64_t n, int64_t num_rows, float scale,
+                                  int has_padding, int64_t padding_id, void* out, int out_dtype, void* workspace,
+                                  int64_t workspace_bytes) {
+  GSB_ENTER(ctx);
+  int st = check_grad(n, num_rows, row_len, grad_stride, dtype, out_dtype);
+  if (st != GSB_OK) return st;
+  if (num_rows == 0 && n == 0) return GSB_OK;
+  GSB_REQUIRE(out || num_rows == 0, GSB_ERR_INVALID_ARGUMENT);
+  cudaStream_t stream = (cudaStream_t)stream_;
+  if (num_rows > 0)
+    GSB_CUDA_OK(cudaMemsetAsync(out, 0, (size_t)num_rows * (size_t)row_len * value_bytes(out_dtype), stream));
+  if (n == 0) return GSB_OK;
+  const GradPlan plan = grad_plan(n, num_rows, row_len);
+  GSB_REQUIRE(grad && ids && workspace, GSB_ERR_INVALID_ARGUMENT);
+  GSB_REQUIRE(workspace_bytes >= (int64_t)plan.total_bytes, GSB_ERR_CAPACITY);
+  SortedKeys sorted;
+  {
+    ScopedKernelTimer timer(ctx, KID_KEY_SORT, stream);
+    st = key_sort(ctx, stream, KeySource{ids, n, num_rows, has_padding != 0, padding_id, ctx_counters(ctx)}, workspace, &sorted);
+  }
+  if (st != GSB_OK) return st;
+  Pieces p(workspace);
+  p.take<char>(plan.sort_bytes);
+  float* part = p.take<float>((size_t)plan.chunks * 2 * (size_t)row_len);
+  return sum_sorted(ctx, stream, GradCall{grad, dtype, row_len, grad_stride, scale, out, out_dtype}, plan, sorted, sorted.key, n,
+                    num_rows, part);
+}
+
+extern "C" int gsb_embedding_grad_rows(gsb_ctx* ctx, void* stream_, const void* grad, int dtype, int64_t row_len,
+                                       int64_t grad_stride, const int64_t* ids, int64_t n, int64_t num_rows, float scale,
+                                       int has_padding, int64_t padding_id, int64_t* out_ids, void* out_rows, int out_dtype,
+                                       int64_t* out_count, void* workspace, int64_t workspace_bytes, int64_t* count_host) {
+  GSB_ENTER(ctx);
+  int st = check_grad(n, num_rows, row_len, grad_stride, dtype, out_dtype);
+  if (st != GSB_OK) return st;
+  cudaStream_t stream = (cudaStream_t)stream_;
+  if (count_host) {
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    GSB_CUDA_OK(cudaStreamIsCapturing(stream, &capture));
+    GSB_REQUIRE(capture == cudaStreamCaptureStatusNone, GSB_ERR_UNSUPPORTED);
+    *count_host = 0;
+  }
+  GSB_REQUIRE(out_count, GSB_ERR_INVALID_ARGUMENT);
+  if (n == 0) {
+    GSB_CUDA_OK(cudaMemsetAsync(out_count, 0, sizeof(int64_t), stream));
+    return GSB_OK;
+  }
+  const GradPlan plan = grad_plan(n, num_rows, row_len);
+  GSB_REQUIRE(grad && ids && out_ids && out_rows && workspace, GSB_ERR_INVALID_ARGUMENT);
+  GSB_REQUIRE(workspace_bytes >= (int64_t)plan.total_bytes, GSB_ERR_CAPACITY);
+  SortedKeys sorted;
+  const Mail mail = count_host ? ctx_mail(ctx) : Mail{nullptr, 0};
+  const int tiles = grid_for(n, kHeadThreads);
+  Pieces p(workspace);
+  p.take<char>(plan.sort_bytes);
+  float* part = p.take<float>((size_t)plan.chunks * 2 * (size_t)row_len);
+  u32* count = p.take<u32>((size_t)tiles);
+  {
+    ScopedKernelTimer timer(ctx, KID_KEY_SORT, stream);
+    st = key_sort(ctx, stream, KeySource{ids, n, num_rows, has_padding != 0, padding_id, ctx_counters(ctx)}, workspace, &sorted);
+    if (st != GSB_OK) return st;
+    k_head_count<<<tiles, kHeadThreads, 0, stream>>>(sorted.key, n, (u32)num_rows, count);
+    GSB_LAUNCH_OK();
+    k_head_rank<<<tiles, kHeadThreads, 0, stream>>>(sorted.key, n, (u32)num_rows, count, sorted.spare, out_ids, out_count, mail,
+                                                    ctx_counters(ctx));
+    GSB_LAUNCH_OK();
+    ctx_count_launches(ctx, 2);
+  }
+  st = sum_sorted(ctx, stream, GradCall{grad, dtype, row_len, grad_stride, scale, out_rows, out_dtype}, plan, sorted,
+                  sorted.spare, n, n, part);
+  if (st != GSB_OK || !count_host) return st;
+  return ctx_mail_result(ctx, stream, mail, 1, count_host);
+}

@@ -417,6 +417,63 @@ def take(src, index):
     return gather_rows(src, index)
 
 
+# ---- rows that are learned -------------------------------------------------------------------
+# Rows of float32, float16 or bfloat16 values on the GPU, arithmetic in float32, every result rounded once.  These operators
+# take no gradients themselves (graph_sampling_b200.gs.nn does); they may be captured into a CUDA graph.
+def embedding_lookup(table, ids, scale=1.0, padding_id=None, ctx=None):
+    """out[..., :] = scale * table[ids[...], :] → a tensor of the shape of `ids` and the rows' width, in the table's dtype.
+    Positions that hold `padding_id` (any number, -1 for instance) get zeros; so do ids outside the table, which are
+    recorded as an error that the next call that waits for a size reports.  `table` lives on the GPU, its rows at any
+    stride, or in pinned host memory."""
+    ctx = _context_for(ids, ctx)
+    return ctx.native.embedding_lookup(ctx.address, table, ids, scale, padding_id)
+
+
+def embedding_grad(grad, ids, num_rows, scale=1.0, padding_id=None, dtype=None, ctx=None):
+    """Gradient of a table of num_rows rows from that of `embedding_lookup`'s result → [num_rows, width], in grad's dtype or,
+    with dtype=torch.float32, in float32: row v is scale * the sum of grad over the positions that hold v, zeros where there
+    is none.  The same inputs give the same bits."""
+    ctx = _context_for(ids, ctx)
+    return ctx.native.embedding_grad(ctx.address, grad, ids, num_rows, scale, padding_id, dtype)
+
+
+def embedding_grad_rows(grad, ids, num_rows, scale=1.0, padding_id=None, dtype=None, sync=True, ctx=None):
+    """The rows of `embedding_grad` that occur → (row_ids, rows), row_ids ascending.  With sync=False the call does not wait
+    for their number and returns (row_ids, rows, number): what lies behind the first `number` (a tensor on the GPU) is
+    left as it was."""
+    ctx = _context_for(ids, ctx)
+    return ctx.native.embedding_grad_rows(ctx.address, grad, ids, num_rows, scale, padding_id, dtype, sync)
+
+
+def expert_order(expert_ids, num_experts, ctx=None):
+    """Slots sorted by expert (or node type, or relation), stably → (offsets, source, place).  expert_ids: [tokens] or
+    [tokens, per token], -1 for a slot that wants none.  Rows offsets[e] .. offsets[e + 1] are expert e's, rows from
+    offsets[num_experts] on those of the slots without one; source[row] is the slot t * per_token + k of a row, and place,
+    of the shape of expert_ids, the row of a slot, or -1 - row for a slot without an expert."""
+    ctx = _context_for(expert_ids, ctx)
+    return ctx.native.expert_order(ctx.address, expert_ids, num_experts)
+
+
+def expert_dispatch(x, place, weights=None, ctx=None):
+    """rows[place[t, k], :] = x[t, :], times weights[t, k] where given → one row per slot; zeros in the rows of slots without
+    an expert.  `place` as expert_order gives it."""
+    ctx = _context_for(place, ctx)
+    return ctx.native.expert_dispatch(ctx.address, x, place, weights)
+
+
+def expert_combine(rows, place, weights=None, ctx=None):
+    """out[t, :] = sum over k of weights[t, k] * rows[place[t, k], :] (weights float32 or of the rows' dtype, None: all 1);
+    slots without an expert are left out.  `rows` may end with the last row that an expert has."""
+    ctx = _context_for(place, ctx)
+    return ctx.native.expert_combine(ctx.address, rows, place, weights)
+
+
+def expert_combine_grad(grad, rows, place, weights=None, ctx=None):
+    """Gradients of `expert_combine` → (of rows, of weights or None)."""
+    ctx = _context_for(place, ctx)
+    return ctx.native.expert_combine_grad(ctx.address, grad, rows, place, weights)
+
+
 def index_search(origin_data, keys, ctx=None):
     """gs::IndexSearch (src/tensor_ops.cc:23-31): position of every key in origin_data, -1 if absent."""
     origin_data, keys = _i64(origin_data, "origin_data"), _i64(keys, "keys")

@@ -21,7 +21,7 @@
  *    calls sharing a context must be ordered on one stream (use one context per stream/thread).  A call of the
  *    context's thread on another stream than the last one's is ordered behind it by waiting for the whole device;
  *    calls through a context are not for capture into a CUDA graph (scratch may move, and a launch carries numbers
- *    that the next one may not repeat): gsb_unique_relabel_static is;
+ *    that the next one may not repeat): gsb_unique_relabel_static is, and so are the calls on learned rows;
  *    Scratch grows on demand with cudaMalloc the first time a size is seen (this synchronises the
  *    device once); steady-state calls allocate nothing;
  *  - a context belongs to the CUDA device it was created on: every entry point checks that this device is
@@ -567,6 +567,61 @@ GSB_API int gsb_sage_hop_sized(gsb_ctx* ctx, void* stream, const int64_t* indptr
                                int64_t* out_select, int64_t* out_indices_ptr, int64_t* out_unique,
                                int64_t* out_unique_ptr, int64_t* out_relabeled, int64_t* unique_total_host,
                                int64_t* edges_total_host);
+
+/* ---- rows that are learned ---------------------------------------------------------------------------------------
+ * No counterpart in the reference, which ends at the loaded features.  Rows of float, half or bfloat16 values (gsb_dtype),
+ * one after the other with `*_stride` values from one row's start to the next (values of a row are contiguous); arithmetic
+ * in float, every result rounded once.  These calls use no scratch of the context: the caller provides it (at least the
+ * bytes that the *_workspace function of the same sizes names, 256-byte aligned), so they may be captured into a CUDA graph
+ * and queued on several streams at once, each call with a workspace of its own.  Ids, experts and places out of range are
+ * never followed and record GSB_ERR_INDEX_RANGE. */
+enum gsb_dtype { GSB_F32 = 0, GSB_F16 = 1, GSB_BF16 = 2 };
+
+/* out[i, :] = scale * table[ids[i], :]; zeros where ids[i] == padding_id (with has_padding; it may be any number, -1 for
+ * instance) or ids[i] is outside [0, num_rows).  table: device memory, or page-locked host memory read in place. */
+GSB_API int gsb_embedding_lookup(gsb_ctx* ctx, void* stream, const void* table, int dtype, int64_t num_rows,
+                                 int64_t row_len, int64_t row_stride, const int64_t* ids, int64_t n, float scale,
+                                 int has_padding, int64_t padding_id, void* out);
+/* Gradient of the table: out[v, :] = scale * sum of grad[i, :] over ids[i] == v (not the padding), zeros for rows that do
+ * not occur; the same inputs give the same bits.  out_dtype: dtype or GSB_F32.  n below 2^31, num_rows below 2^32 - 1. */
+GSB_API int64_t gsb_embedding_grad_workspace(int64_t n, int64_t num_rows, int64_t row_len);
+GSB_API int gsb_embedding_grad(gsb_ctx* ctx, void* stream, const void* grad, int dtype, int64_t row_len,
+                               int64_t grad_stride, const int64_t* ids, int64_t n, int64_t num_rows, float scale,
+                               int has_padding, int64_t padding_id, void* out, int out_dtype, void* workspace,
+                               int64_t workspace_bytes);
+/* The rows of it that occur: out_ids[0 .. U) ascending, out_rows[j, :] the gradient of row out_ids[j]; both hold n entries, the
+ * ones from U on are left as they are.  U is left in out_count (DEVICE); with count_host the call waits for it (and cannot be
+ * captured: GSB_ERR_UNSUPPORTED). */
+GSB_API int gsb_embedding_grad_rows(gsb_ctx* ctx, void* stream, const void* grad, int dtype, int64_t row_len,
+                                    int64_t grad_stride, const int64_t* ids, int64_t n, int64_t num_rows, float scale,
+                                    int has_padding, int64_t padding_id, int64_t* out_ids, void* out_rows, int out_dtype,
+                                    int64_t* out_count, void* workspace, int64_t workspace_bytes, int64_t* count_host);
+
+/* Slots sorted by expert (or node type), stably: experts[s] in [0, num_experts), or -1 for a slot that wants none; those come
+ * last.  out_offsets[num_experts + 1]: the rows of expert e are out_offsets[e] .. out_offsets[e + 1]; out_source[row] = slot;
+ * out_place[slot] = row, or ~row (-1 - row) for a slot without an expert.  num_experts <= GSB_MAX_EXPERTS, n below 2^31. */
+#define GSB_MAX_EXPERTS 65536
+GSB_API int64_t gsb_expert_order_workspace(int64_t n, int64_t num_experts);
+GSB_API int gsb_expert_order(gsb_ctx* ctx, void* stream, const int64_t* experts, int64_t n, int64_t num_experts,
+                             int64_t* out_offsets, int64_t* out_source, int64_t* out_place, void* workspace,
+                             int64_t workspace_bytes);
+/* Slot t * per_token + k is the k-th of token t.  Spread: out_rows[place[t, k], :] = weights[t, k] * x[t, :], zeros in the rows of
+ * slots without an expert; tokens * per_token rows.  Combine: out[t, :] = sum over k of weights[t, k] * rows[place[t, k], :],
+ * slots without an expert left out; place as gsb_expert_order gives it, num_rows at most tokens * per_token (fewer where the
+ * caller leaves rows of slots without an expert away).  weights: NULL (all 1), of type dtype or GSB_F32.  The gradient of spread without weights
+ * is combine without weights; that of combine is out_grad_rows = spread of grad (NULL: not wanted) and
+ * out_grad_weights[t, k] = <grad[t, :], rows[place[t, k], :]> (NULL: not wanted; else of the weights' type), 0 for slots without
+ * an expert. */
+GSB_API int gsb_expert_spread(gsb_ctx* ctx, void* stream, const void* x, int dtype, int64_t tokens, int64_t per_token,
+                              int64_t row_len, int64_t x_stride, const int64_t* place, const void* weights,
+                              int weights_dtype, void* out_rows);
+GSB_API int gsb_expert_combine(gsb_ctx* ctx, void* stream, const void* rows, int dtype, int64_t num_rows, int64_t tokens,
+                               int64_t per_token, int64_t row_len, int64_t rows_stride, const int64_t* place,
+                               const void* weights, int weights_dtype, void* out);
+GSB_API int gsb_expert_combine_grad(gsb_ctx* ctx, void* stream, const void* grad, int dtype, int64_t tokens,
+                                    int64_t per_token, int64_t row_len, int64_t grad_stride, const void* rows,
+                                    int64_t num_rows, int64_t rows_stride, const int64_t* place, const void* weights,
+                                    int weights_dtype, void* out_grad_rows, void* out_grad_weights);
 
 /* ---- unique + relabel without any allocation ----------------------------------------------------------
  * No counterpart in the reference.  For callers that must not allocate device memory while they
