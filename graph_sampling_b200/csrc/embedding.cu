@@ -15,7 +15,6 @@
 namespace gsb {
 
 constexpr int kLookupThreads = 256;
-constexpr u32 kNoRow = 0xffffffffu;
 
 template <class T, int BYTES>
 __global__ void __launch_bounds__(kLookupThreads) k_lookup_rows(const Unit<T, BYTES>* __restrict__ table, i64 num_rows,
@@ -69,12 +68,15 @@ struct SumArgs {
   i64 stride;     // of `grad`, in units
   float scale;
 };
+__device__ __forceinline__ bool usable(const SumArgs& a, u64 pair) {
+  return pair_key(pair) < a.num_rows && pair_at(pair) < (u32)a.n;
+}
 
 // One group of lanes per chunk and column tile (blockIdx.y) of lanes * STEPS units.
 template <class T, class O, int BYTES, int STEPS>
 __global__ void __launch_bounds__(kSumThreads) k_sum_rows(const SumArgs a, const Unit<T, BYTES>* __restrict__ grad,
-                                                          const u32* __restrict__ at, const u32* __restrict__ row,
-                                                          O* __restrict__ out, float* __restrict__ part) {
+                                                          const u64* __restrict__ sorted, O* __restrict__ out,
+                                                          float* __restrict__ part) {
   constexpr int N = Unit<T, BYTES>::N, kAhead = STEPS >= 4 ? 2 : 4;
   const i64 chunk = ((i64)blockIdx.x * kSumThreads + threadIdx.x) / a.lanes;
   const i64 begin = chunk * a.chunk, end = min(begin + a.chunk, a.n);
@@ -82,7 +84,7 @@ __global__ void __launch_bounds__(kSumThreads) k_sum_rows(const SumArgs a, const
   if (begin >= a.n) return;
   const i64 width = a.units * N;
   float sum[STEPS][N] = {};
-  bool head = begin > 0 && row[begin - 1] == row[begin];
+  bool head = begin > 0 && pair_key(sorted[begin - 1]) == pair_key(sorted[begin]);
   auto put = [&](auto* to, float scale) {
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
@@ -93,28 +95,29 @@ __global__ void __launch_bounds__(kSumThreads) k_sum_rows(const SumArgs a, const
     }
   };
   for (i64 j = begin; j < end; j += kAhead) {
-    u32 r[kAhead + 1];
+    u64 p[kAhead + 1];
     Unit<T, BYTES> v[kAhead][STEPS];
 #pragma unroll
-    for (int u = 0; u <= kAhead; ++u) r[u] = j + u < a.n ? row[j + u] : kNoRow;
+    for (int u = 0; u <= kAhead; ++u) p[u] = j + u < a.n ? sorted[j + u] : ~0ull;
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      if (j + u >= end || r[u] >= a.num_rows) continue;
-      const Unit<T, BYTES>* from = grad + (i64)at[j + u] * a.stride;
+      if (j + u >= end || !usable(a, p[u])) continue;
+      const Unit<T, BYTES>* from = grad + (i64)pair_at(p[u]) * a.stride;
 #pragma unroll
       for (int s = 0; s < STEPS; ++s)
         if (first + s * a.lanes < a.units) v[u][s] = load_unit_once(from + first + s * a.lanes);
     }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      if (j + u >= end || r[u] >= a.num_rows) return;  // the sorted list ends with the positions that belong to no row
+      if (j + u >= end || !usable(a, p[u])) return;  // the sorted list ends with the positions that belong to no row
 #pragma unroll
       for (int s = 0; s < STEPS; ++s)
         if (first + s * a.lanes < a.units)
 #pragma unroll
           for (int q = 0; q < N; ++q) sum[s][q] += to_float(v[u][s].v[q]);
-      const bool ends = r[u + 1] != r[u];
-      if (ends && !head) put(out + (i64)r[u] * width, a.scale);
+      const u32 row = pair_key(p[u]);
+      const bool ends = pair_key(p[u + 1]) != row;
+      if (ends && !head) put(out + (i64)row * width, a.scale);
       else if (ends || j + u + 1 == end) put(part + (2 * chunk + (head ? 0 : 1)) * width, 1.f);
       if (ends) head = false;
     }
@@ -123,53 +126,19 @@ __global__ void __launch_bounds__(kSumThreads) k_sum_rows(const SumArgs a, const
 
 // Where the last sum of a chunk began there and goes on: its part and those of the chunks behind, in their order.
 template <class O>
-__global__ void __launch_bounds__(kSumThreads) k_join_rows(const SumArgs a, i64 width, i64 chunks, const u32* __restrict__ row,
-                                                           const float* __restrict__ part, O* __restrict__ out) {
+__global__ void __launch_bounds__(kSumThreads) k_join_rows(const SumArgs a, i64 width, i64 chunks,
+                                                           const u64* __restrict__ sorted, const float* __restrict__ part,
+                                                           O* __restrict__ out) {
   const i64 column = (i64)blockIdx.y * kSumThreads + threadIdx.x;
   for (i64 c = blockIdx.x; c + 1 < chunks; c += gridDim.x) {
     const i64 begin = c * a.chunk, end = begin + a.chunk;
-    const u32 r = row[end - 1];
-    if (r >= a.num_rows || row[end] != r || (begin > 0 && row[begin - 1] == r)) continue;
+    const u32 row = pair_key(sorted[end - 1]);
+    if (row >= a.num_rows || pair_key(sorted[end]) != row || (begin > 0 && pair_key(sorted[begin - 1]) == row)) continue;
     if (column >= width) continue;
     float sum = part[(2 * c + 1) * width + column];
-    for (i64 next = c + 1; next < chunks && row[next * a.chunk] == r; ++next) sum += part[2 * next * width + column];
-    out[(i64)r * width + column] = from_float<O>(sum * a.scale);
-  }
-}
-
-// The sorted keys' ranks among the distinct ones.
-constexpr int kHeadThreads = 1024;
-
-__device__ __forceinline__ bool is_head(const u32* key, i64 i, i64 n, u32 num_keys) {
-  return i < n && key[i] < num_keys && (i == 0 || key[i - 1] != key[i]);
-}
-
-__global__ void __launch_bounds__(kHeadThreads) k_head_count(const u32* __restrict__ key, i64 n, u32 num_keys,
-                                                             u32* __restrict__ count) {
-  const i64 i = (i64)blockIdx.x * kHeadThreads + threadIdx.x;
-  const int heads = __syncthreads_count(is_head(key, i, n, num_keys));
-  if (threadIdx.x == 0) count[blockIdx.x] = heads;
-}
-
-__global__ void __launch_bounds__(kHeadThreads) k_head_rank(const u32* __restrict__ key, i64 n, u32 num_keys,
-                                                            const u32* __restrict__ count, u32* __restrict__ rank,
-                                                            i64* __restrict__ ids, i64* __restrict__ total, Mail mail,
-                                                            const i64* counters) {
-  __shared__ i64 s_scan[33];
-  i64 before = 0;
-  for (int t = threadIdx.x; t < (int)blockIdx.x; t += kHeadThreads) before += count[t];
-  i64 base;
-  block_exclusive_scan<kHeadThreads>(before, s_scan, &base);
-  const i64 i = (i64)blockIdx.x * kHeadThreads + threadIdx.x;
-  const bool head = is_head(key, i, n, num_keys);
-  i64 heads;
-  const i64 excl = block_exclusive_scan<kHeadThreads>((i64)head, s_scan, &heads);
-  const i64 mine = base + excl + (head ? 1 : 0) - 1;  // of the latest head up to here
-  if (i < n) rank[i] = key[i] < num_keys ? (u32)mine : kNoRow;
-  if (head) ids[mine] = key[i];
-  if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) {
-    total[0] = base + heads;
-    mail_post(mail, 0, base + heads, counters);
+    for (i64 next = c + 1; next < chunks && pair_key(sorted[next * a.chunk]) == row; ++next)
+      sum += part[2 * next * width + column];
+    out[(i64)row * width + column] = from_float<O>(sum * a.scale);
   }
 }
 
@@ -193,15 +162,13 @@ static GradPlan grad_plan(i64 n, i64 num_rows, i64 row_len) {
   Pieces p(nullptr);
   p.take<char>(g.sort_bytes);
   p.take<float>((size_t)g.chunks * 2 * (size_t)row_len);
-  p.take<u32>((size_t)(n + kHeadThreads - 1) / kHeadThreads);
-  p.take<i64>(1);
   g.total_bytes = p.used;
   return g;
 }
 
 template <class T, class O, int BYTES>
 static void launch_sum(cudaStream_t stream, SumArgs a, i64 chunks, const void* grad, i64 stride_bytes, i64 row_bytes,
-                       const SortedKeys& sorted, const u32* row, void* out, float* part) {
+                       const u64* sorted, void* out, float* part) {
   a.units = row_bytes / BYTES;
   a.stride = stride_bytes / BYTES;
   a.lanes = 1;
@@ -209,7 +176,7 @@ static void launch_sum(cudaStream_t stream, SumArgs a, i64 chunks, const void* g
   auto go = [&](auto steps) {
     constexpr int S = decltype(steps)::value;
     const dim3 grid(grid_for(chunks * a.lanes, kSumThreads), grid_for(a.units, a.lanes * S));
-    k_sum_rows<T, O, BYTES, S><<<grid, kSumThreads, 0, stream>>>(a, (const Unit<T, BYTES>*)grad, sorted.at, row, (O*)out, part);
+    k_sum_rows<T, O, BYTES, S><<<grid, kSumThreads, 0, stream>>>(a, (const Unit<T, BYTES>*)grad, sorted, (O*)out, part);
   };
   if (a.units <= 32) go(std::integral_constant<int, 1>{});
   else if (a.units <= 64) go(std::integral_constant<int, 2>{});
@@ -225,9 +192,9 @@ struct GradCall {
   int out_dtype;
 };
 
-// Sums of the sorted rows into out[row[j], :].
-static int sum_sorted(gsb_ctx* ctx, cudaStream_t stream, const GradCall& c, const GradPlan& plan, const SortedKeys& sorted,
-                      const u32* row, i64 n, i64 num_rows, float* part) {
+// Sums of the rows at the sorted positions, into the rows of `out` that the pairs name.
+static int sum_sorted(gsb_ctx* ctx, cudaStream_t stream, const GradCall& c, const GradPlan& plan, const u64* sorted, i64 n,
+                      i64 num_rows, float* part) {
   const int size = value_bytes(c.dtype), out_size = value_bytes(c.out_dtype);
   const i64 row_bytes = c.row_len * size, stride_bytes = c.grad_stride * size;
   int unit = unit_bytes(row_bytes, (u64)(uintptr_t)c.grad | (u64)stride_bytes);
@@ -238,16 +205,16 @@ static int sum_sorted(gsb_ctx* ctx, cudaStream_t stream, const GradCall& c, cons
     typedef decltype(value) T;
     constexpr int kBytes = decltype(bytes)::value;
     if (c.out_dtype == c.dtype)
-      launch_sum<T, T, kBytes>(stream, a, plan.chunks, c.grad, stride_bytes, row_bytes, sorted, row, c.out, part);
+      launch_sum<T, T, kBytes>(stream, a, plan.chunks, c.grad, stride_bytes, row_bytes, sorted, c.out, part);
     else
-      launch_sum<T, float, kBytes>(stream, a, plan.chunks, c.grad, stride_bytes, row_bytes, sorted, row, c.out, part);
+      launch_sum<T, float, kBytes>(stream, a, plan.chunks, c.grad, stride_bytes, row_bytes, sorted, c.out, part);
   });
   GSB_LAUNCH_OK();
   if (plan.chunks > 1) {
     const dim3 grid((unsigned)min(plan.chunks - 1, (i64)kNumSMs * 16), grid_for(c.row_len, kSumThreads));
-    if (c.out_dtype == GSB_F32) k_join_rows<float><<<grid, kSumThreads, 0, stream>>>(a, c.row_len, plan.chunks, row, part, (float*)c.out);
-    else if (c.out_dtype == GSB_F16) k_join_rows<__half><<<grid, kSumThreads, 0, stream>>>(a, c.row_len, plan.chunks, row, part, (__half*)c.out);
-    else k_join_rows<__nv_bfloat16><<<grid, kSumThreads, 0, stream>>>(a, c.row_len, plan.chunks, row, part, (__nv_bfloat16*)c.out);
+    if (c.out_dtype == GSB_F32) k_join_rows<float><<<grid, kSumThreads, 0, stream>>>(a, c.row_len, plan.chunks, sorted, part, (float*)c.out);
+    else if (c.out_dtype == GSB_F16) k_join_rows<__half><<<grid, kSumThreads, 0, stream>>>(a, c.row_len, plan.chunks, sorted, part, (__half*)c.out);
+    else k_join_rows<__nv_bfloat16><<<grid, kSumThreads, 0, stream>>>(a, c.row_len, plan.chunks, sorted, part, (__nv_bfloat16*)c.out);
     GSB_LAUNCH_OK();
     ctx_count_launches(ctx, 1);
   }
@@ -319,23 +286,28 @@ extern "C" int gsb_embedding_grad(gsb_ctx* ctx, void* stream_, const void* grad,
   if (num_rows == 0 && n == 0) return GSB_OK;
   GSB_REQUIRE(out || num_rows == 0, GSB_ERR_INVALID_ARGUMENT);
   cudaStream_t stream = (cudaStream_t)stream_;
-  if (num_rows > 0)
-    GSB_CUDA_OK(cudaMemsetAsync(out, 0, (size_t)num_rows * (size_t)row_len * value_bytes(out_dtype), stream));
-  if (n == 0) return GSB_OK;
+  const size_t out_bytes = (size_t)num_rows * (size_t)row_len * value_bytes(out_dtype);
+  if (n == 0) {
+    GSB_CUDA_OK(cudaMemsetAsync(out, 0, out_bytes, stream));
+    return GSB_OK;
+  }
   const GradPlan plan = grad_plan(n, num_rows, row_len);
   GSB_REQUIRE(grad && ids && workspace, GSB_ERR_INVALID_ARGUMENT);
   GSB_REQUIRE(workspace_bytes >= (int64_t)plan.total_bytes, GSB_ERR_CAPACITY);
-  SortedKeys sorted;
+  const u64* sorted;
   {
     ScopedKernelTimer timer(ctx, KID_KEY_SORT, stream);
-    st = key_sort(ctx, stream, KeySource{ids, n, num_rows, has_padding != 0, padding_id, ctx_counters(ctx)}, workspace, &sorted);
+    SortCall call{KeySource{ids, n, num_rows, has_padding != 0, padding_id, ctx_counters(ctx)}, SORT_PAIRS};
+    call.zero = out;
+    call.zero_bytes = out_bytes;
+    st = key_sort(ctx, stream, call, workspace, &sorted);
   }
   if (st != GSB_OK) return st;
   Pieces p(workspace);
   p.take<char>(plan.sort_bytes);
   float* part = p.take<float>((size_t)plan.chunks * 2 * (size_t)row_len);
-  return sum_sorted(ctx, stream, GradCall{grad, dtype, row_len, grad_stride, scale, out, out_dtype}, plan, sorted, sorted.key, n,
-                    num_rows, part);
+  return sum_sorted(ctx, stream, GradCall{grad, dtype, row_len, grad_stride, scale, out, out_dtype}, plan, sorted, n, num_rows,
+                    part);
 }
 
 extern "C" int gsb_embedding_grad_rows(gsb_ctx* ctx, void* stream_, const void* grad, int dtype, int64_t row_len,
@@ -360,26 +332,20 @@ extern "C" int gsb_embedding_grad_rows(gsb_ctx* ctx, void* stream_, const void* 
   const GradPlan plan = grad_plan(n, num_rows, row_len);
   GSB_REQUIRE(grad && ids && out_ids && out_rows && workspace, GSB_ERR_INVALID_ARGUMENT);
   GSB_REQUIRE(workspace_bytes >= (int64_t)plan.total_bytes, GSB_ERR_CAPACITY);
-  SortedKeys sorted;
-  const Mail mail = count_host ? ctx_mail(ctx) : Mail{nullptr, 0};
-  const int tiles = grid_for(n, kHeadThreads);
   Pieces p(workspace);
   p.take<char>(plan.sort_bytes);
   float* part = p.take<float>((size_t)plan.chunks * 2 * (size_t)row_len);
-  u32* count = p.take<u32>((size_t)tiles);
+  const u64* sorted;
+  SortCall call{KeySource{ids, n, num_rows, has_padding != 0, padding_id, ctx_counters(ctx)}, SORT_RANKS};
+  call.distinct = out_ids;
+  call.number = out_count;
+  if (count_host) call.mail = ctx_mail(ctx);
   {
     ScopedKernelTimer timer(ctx, KID_KEY_SORT, stream);
-    st = key_sort(ctx, stream, KeySource{ids, n, num_rows, has_padding != 0, padding_id, ctx_counters(ctx)}, workspace, &sorted);
-    if (st != GSB_OK) return st;
-    k_head_count<<<tiles, kHeadThreads, 0, stream>>>(sorted.key, n, (u32)num_rows, count);
-    GSB_LAUNCH_OK();
-    k_head_rank<<<tiles, kHeadThreads, 0, stream>>>(sorted.key, n, (u32)num_rows, count, sorted.spare, out_ids, out_count, mail,
-                                                    ctx_counters(ctx));
-    GSB_LAUNCH_OK();
-    ctx_count_launches(ctx, 2);
+    st = key_sort(ctx, stream, call, workspace, &sorted);
   }
-  st = sum_sorted(ctx, stream, GradCall{grad, dtype, row_len, grad_stride, scale, out_rows, out_dtype}, plan, sorted,
-                  sorted.spare, n, n, part);
+  if (st != GSB_OK) return st;
+  st = sum_sorted(ctx, stream, GradCall{grad, dtype, row_len, grad_stride, scale, out_rows, out_dtype}, plan, sorted, n, n, part);
   if (st != GSB_OK || !count_host) return st;
-  return ctx_mail_result(ctx, stream, mail, 1, count_host);
+  return ctx_mail_result(ctx, stream, call.mail, 1, count_host);
 }

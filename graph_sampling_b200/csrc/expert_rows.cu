@@ -15,20 +15,6 @@
 namespace gsb {
 
 constexpr int kRowThreads = 256;
-constexpr int kOrderThreads = 256;
-
-__global__ void __launch_bounds__(kOrderThreads) k_order_out(const u32* __restrict__ key, const u32* __restrict__ at, i64 n,
-                                                             i64 experts, i64* __restrict__ offsets,
-                                                             i64* __restrict__ source, i64* __restrict__ place) {
-  const i64 j = (i64)blockIdx.x * kOrderThreads + threadIdx.x;
-  if (j >= n) return;
-  const i64 e = key[j], before = j > 0 ? (i64)key[j - 1] : -1;
-  source[j] = at[j];
-  place[at[j]] = e < experts ? j : ~j;
-  for (i64 q = before + 1; q <= e; ++q) offsets[q] = j;
-  if (j == n - 1)
-    for (i64 q = e + 1; q <= experts; ++q) offsets[q] = n;
-}
 
 // Weights of type float or of the rows' type, or none (all 1).
 struct Weights {
@@ -190,14 +176,12 @@ extern "C" int gsb_expert_order(gsb_ctx* ctx, void* stream_, const int64_t* expe
   }
   GSB_REQUIRE(experts && out_source && out_place && workspace, GSB_ERR_INVALID_ARGUMENT);
   GSB_REQUIRE(workspace_bytes >= need, GSB_ERR_CAPACITY);
-  SortedKeys sorted;
+  SortCall call{KeySource{experts, n, num_experts, true, -1, ctx_counters(ctx)}, SORT_ORDER};
+  call.offsets = out_offsets;
+  call.order_source = out_source;
+  call.place = out_place;
   ScopedKernelTimer timer(ctx, KID_KEY_SORT, stream);
-  const int st = key_sort(ctx, stream, KeySource{experts, n, num_experts, true, -1, ctx_counters(ctx)}, workspace, &sorted);
-  if (st != GSB_OK) return st;
-  k_order_out<<<grid_for(n, kOrderThreads), kOrderThreads, 0, stream>>>(sorted.key, sorted.at, n, num_experts, out_offsets,
-                                                                       out_source, out_place);
-  GSB_LAUNCH_OK();
-  return GSB_OK;
+  return key_sort(ctx, stream, call, workspace, nullptr);
 }
 
 extern "C" int gsb_expert_spread(gsb_ctx* ctx, void* stream_, const void* x, int dtype, int64_t tokens, int64_t per_token,

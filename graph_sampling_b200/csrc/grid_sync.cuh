@@ -55,17 +55,17 @@ __device__ __forceinline__ void grid_share(i64 n, F f) {
 // in the weighted sampler, 10 000 columns with replacement 217 -> 259 us).
 //
 // grid_barrier_arrive and grid_barrier_wait are its halves, for work in between that needs nothing from other CTAs; a CTA waits
-// before it arrives at the next barrier.
+// before it arrives at the next barrier.  `ctas`: how many CTAs meet, where the grid has others that never come.
 __device__ __forceinline__ void grid_barrier_arrive(const GridSync& g) {
   __syncthreads();
   if (threadIdx.x == 0) asm volatile("red.release.gpu.global.add.u64 [%0], 1;" ::"l"(g.word) : "memory");
 }
 
 template <class F>
-__device__ __forceinline__ void grid_barrier_wait(const GridSync& g, u32 index, F give_up) {
+__device__ __forceinline__ void grid_barrier_wait(const GridSync& g, u32 index, F give_up, u32 ctas = gridDim.x) {
   bool ok = true;
   if (threadIdx.x == 0) {
-    const u64 target = g.base + (u64)index * gridDim.x;
+    const u64 target = g.base + (u64)index * ctas;
     int polls = 0;
     for (;;) {
       const u64 seen = ld_acquire_u64(g.word);
@@ -87,9 +87,9 @@ __device__ __forceinline__ void grid_barrier_wait(const GridSync& g, u32 index, 
 }
 
 template <class F>
-__device__ __forceinline__ void grid_barrier(const GridSync& g, u32 index, F give_up) {
+__device__ __forceinline__ void grid_barrier(const GridSync& g, u32 index, F give_up, u32 ctas = gridDim.x) {
   grid_barrier_arrive(g);
-  grid_barrier_wait(g, index, give_up);
+  grid_barrier_wait(g, index, give_up, ctas);
 }
 
 // CTAs of a kernel that are resident at once on the context's device (0: cooperative launches are not available).  The

@@ -1,140 +1,456 @@
+// One launch sorts: CTAs own equal stretches of the positions and go through the digits of the key, least significant first.
+// Per digit a CTA counts its stretch, all counts become visible behind a barrier, every CTA adds up for itself what lies before
+// its own (G CTAs x bins words from L2, in place of a scan with a barrier of its own), and puts its positions where they
+// belong, tile by tile through shared memory so that neighbouring threads write neighbouring words.  Nothing depends on the
+// order in which CTAs run.
+//
+// Up to 8 CTAs (32 768 positions) are one cluster: its barrier is the hardware's, needs no word in memory and no bound.  More
+// are launched cooperatively and meet at a word in the workspace (grid_sync.cuh).  Digits are as wide as keeps the number of
+// passes small: 11 bits where few CTAs have to read each other's counts, 9 where up to 148 do.
+//
+// The launch may also clear memory (the rows of a dense gradient that no position has): CTAs beyond the sorting ones do that
+// at the same time, the sort being bound by latency and the clearing by HBM.
 #include "key_sort.cuh"
 
+#include "grid_sync.cuh"
 #include "scan.cuh"
 
 namespace gsb {
 
-constexpr int kThreads = 256;
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
 constexpr int kRounds = 8;
 constexpr int kTile = kThreads * kRounds;
-constexpr int kBins = 256;
-constexpr int kScanThreads = 1024;
+constexpr int kClusterCtas = 8;
+constexpr int kClusterBits = 11, kGridBits = 9;
+constexpr int kMaxBins = 1 << kClusterBits;
+constexpr size_t kZeroPiece = 1 << 16;
 
-__device__ u32 checked_key_of(const KeySource& s, i64 i) {
+struct SortArgs {
+  SortCall call;
+  u64 *from, *to;  // [key : 32 | position : 32], exchanged after every pass
+  u32* counts;     // CTAs x bins
+  int ctas;        // that sort; the others clear
+  int bits, passes, digit;
+  i64 stretch;     // positions per CTA, a multiple of kTile
+  u64* next_piece;   // of the memory to clear (cooperative launches); null: pieces by CTA number
+  GridSync sync;
+};
+
+__device__ __forceinline__ u32 key_of(const KeySource& s, i64 i, bool check) {
   const i64 id = __ldg(s.ids + i);
   if (s.has_dropped && id == s.dropped) return (u32)s.num_keys;
   if ((u64)id < (u64)s.num_keys) return (u32)id;
-  raise_error(s.counters, GSB_ERR_INDEX_RANGE, i);
+  if (check) raise_error(s.counters, GSB_ERR_INDEX_RANGE, i);
   return (u32)s.num_keys;
 }
 
-template <bool FIRST>
-__global__ void __launch_bounds__(kThreads) k_key_count(const KeySource source, const u32* __restrict__ keys, i64 n, int shift,
-                                                        u32* __restrict__ count, int tiles) {
-  __shared__ u32 s_count[kBins];
-  s_count[threadIdx.x] = 0;
-  __syncthreads();
-  const i64 base = (i64)blockIdx.x * kTile;
-#pragma unroll
-  for (int r = 0; r < kRounds; ++r) {
-    const i64 i = base + r * kThreads + threadIdx.x;
-    if (i < n) atomicAdd(&s_count[((FIRST ? checked_key_of(source, i) : keys[i]) >> shift) & (kBins - 1)], 1u);
-  }
-  __syncthreads();
-  count[(i64)threadIdx.x * tiles + blockIdx.x] = s_count[threadIdx.x];
+__device__ __forceinline__ void clear_piece(char* p, size_t bytes) {
+  const size_t head = min(bytes, (size_t)(0 - (uintptr_t)p & 15));
+  for (size_t q = threadIdx.x; q < head; q += kThreads) p[q] = 0;
+  uint4* w = (uint4*)(p + head);
+  const size_t words = (bytes - head) / 16;
+  for (size_t q = threadIdx.x; q < words; q += kThreads) __stcs(w + q, make_uint4(0, 0, 0, 0));
+  for (size_t q = head + words * 16 + threadIdx.x; q < bytes; q += kThreads) p[q] = 0;
 }
 
-// Exclusive scan of all tiles' counts by one CTA.
-__global__ void __launch_bounds__(kScanThreads) k_key_scan(u32* __restrict__ count, i64 n) {
-  __shared__ i64 s_scan[33];
-  i64 before = 0;
-  for (i64 base = 0; base < n; base += kScanThreads) {
-    const i64 i = base + threadIdx.x;
-    const u32 mine = i < n ? count[i] : 0;
-    i64 total;
-    const i64 excl = block_exclusive_scan<kScanThreads>((i64)mine, s_scan, &total);
-    if (i < n) count[i] = (u32)(before + excl);
-    before += total;
+__device__ __forceinline__ size_t pieces_of(const SortCall& c) { return (c.zero_bytes + kZeroPiece - 1) / kZeroPiece; }
+
+__device__ void clear_by_number(const SortCall& c, size_t number, size_t of) {
+  for (size_t q = number; q < pieces_of(c); q += of)
+    clear_piece((char*)c.zero + q * kZeroPiece, min(kZeroPiece, c.zero_bytes - q * kZeroPiece));
+}
+
+__device__ void clear_rest(const SortCall& c, u64* next) {
+  __shared__ u64 s_piece;
+  for (;;) {
+    __syncthreads();
+    if (threadIdx.x == 0) s_piece = atomicAdd((unsigned long long*)next, 1ull);
+    __syncthreads();
+    const size_t q = (size_t)s_piece;
+    if (q >= pieces_of(c)) return;
+    clear_piece((char*)c.zero + q * kZeroPiece, min(kZeroPiece, c.zero_bytes - q * kZeroPiece));
   }
 }
 
-template <bool FIRST>
-__global__ void __launch_bounds__(kThreads) k_key_place(const KeySource source, const u32* __restrict__ keys,
-                                                        const u32* __restrict__ at, i64 n, int shift,
-                                                        const u32* __restrict__ start, int tiles, u32* __restrict__ out_keys,
-                                                        u32* __restrict__ out_at) {
-  constexpr int kWarps = kThreads / 32;
-  __shared__ u32 s_count[kWarps][kBins];
+// Exclusive scan of bins values, kMaxBins / kThreads per thread at most; returns the total through s_scan.
+__device__ __forceinline__ u32 scan_threads(u32 v, u32* s_scan) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int q = threadIdx.x; q < kWarps * kBins; q += kThreads) (&s_count[0][0])[q] = 0;
-  __syncthreads();
-  const i64 base = (i64)blockIdx.x * kTile + warp * (kRounds * 32);
-  u32 key[kRounds], rank[kRounds];
+  u32 inc = v;
 #pragma unroll
-  for (int r = 0; r < kRounds; ++r) {
-    const i64 i = base + r * 32 + lane;
-    const bool valid = i < n;
-    key[r] = valid ? (FIRST ? key_of(source, i) : keys[i]) : 0;
-    const u32 digit = valid ? (key[r] >> shift) & (kBins - 1) : kBins;
-    const u32 peers = __match_any_sync(0xffffffffu, digit);
-    const u32 before = __popc(peers & ((1u << lane) - 1u));
-    u32 found = 0;
-    if (valid) found = s_count[warp][digit];
-    __syncwarp();
-    if (valid && before == 0) s_count[warp][digit] = found + __popc(peers);
-    __syncwarp();
-    rank[r] = found + before;
+  for (int o = 1; o < 32; o <<= 1) {
+    const u32 t = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += t;
   }
+  __syncthreads();  // s_scan may still be read
+  if (lane == 31) s_scan[warp] = inc;
   __syncthreads();
-  {
-    u32 run = start[(i64)threadIdx.x * tiles + blockIdx.x];  // kThreads == kBins
+  u32 before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    const u32 t = s_scan[w];
+    if (w < warp) before += t;
+    all += t;
+  }
+  if (threadIdx.x == 0) s_scan[kWarps] = all;
+  return before + inc - v;
+}
+
+template <bool CLUSTER>
+struct Barrier {
+  const SortArgs& a;
+  u32 index = 0;
+  template <class F>
+  __device__ __forceinline__ void operator()(F give_up) {
+    ++index;
+    if constexpr (CLUSTER) {
+      __threadfence();
+      asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    } else {
+      grid_barrier(a.sync, index, give_up, (u32)a.ctas);
+    }
+  }
+};
+
+struct Tile {
+  u64 item[kRounds];
+  u32 rank[kRounds];
+};
+
+template <bool CLUSTER>
+__global__ void __launch_bounds__(kThreads) k_sort_keys(const SortArgs a) {
+  extern __shared__ __align__(16) char smem[];
+  __shared__ u32 s_scan[kWarps + 1];
+  const SortCall& c = a.call;
+  const int cta = blockIdx.x;
+  if (cta >= a.ctas) {
+    if (!CLUSTER) clear_rest(c, a.next_piece);
+    else if (cta >= kClusterCtas) clear_by_number(c, cta - kClusterCtas, gridDim.x - kClusterCtas);
+    return;
+  }
+  const i64 n = c.source.n;
+  const int bins = 1 << a.digit;
+  u64* s_items = (u64*)smem;                           // kTile, also the partial sums of the counts
+  u32* s_base = (u32*)(s_items + kTile);               // where the next item of a digit goes
+  u32* s_tile = s_base + bins;                         // where a digit starts in the tile
+  unsigned short* s_count = (unsigned short*)(s_tile + bins);  // kWarps x bins
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const i64 lo = (i64)cta * a.stretch, hi = min(lo + a.stretch, n);
+  const bool single = a.stretch == kTile;
+  Barrier<CLUSTER> barrier{a};
+  auto give_up = [&] {
+    if (c.result == SORT_RANKS) c.number[0] = 0;
+    if (c.result == SORT_ORDER)
+      for (i64 q = cta; q < max(n, c.source.num_keys + 1); q += a.ctas) {
+        if (q <= c.source.num_keys) c.offsets[q] = 0;
+        if (q < n) c.order_source[q] = q, c.place[q] = ~q;
+      }
+  };
+  const u64* from = a.from;
+  u64* to = a.to;
+  Tile t;
+
+  auto item_at = [&](i64 i, int pass, bool check) {
+    return pass == 0 ? (u64)key_of(c.source, i, check) << 32 | (u64)i : __ldcg(from + i);
+  };
+  // Ranks of a tile's items among those of the same digit in their warp; s_count = the warps' counts.
+  auto rank_tile = [&](i64 base, int pass, int shift, bool check) {
+    for (int q = threadIdx.x; q < kWarps * bins / 2; q += kThreads) ((u32*)s_count)[q] = 0;
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+      const i64 i = base + warp * (kRounds * 32) + r * 32 + lane;
+      t.item[r] = i < hi ? item_at(i, pass, check) : ~0ull;
+    }
+    __syncthreads();
+    unsigned short* mine = s_count + warp * bins;
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+      const bool valid = base + warp * (kRounds * 32) + r * 32 + lane < hi;
+      const u32 digit = valid ? (pair_key(t.item[r]) >> shift) & (bins - 1) : (u32)bins;
+      const u32 peers = __match_any_sync(0xffffffffu, digit);
+      const u32 before = __popc(peers & ((1u << lane) - 1u));
+      const u32 found = valid ? mine[digit] : 0;
+      __syncwarp();
+      if (valid && before == 0) mine[digit] = (unsigned short)(found + __popc(peers));
+      __syncwarp();
+      t.rank[r] = found + before;
+    }
+    __syncthreads();
+  };
+  // Warps' counts become starts within the digit; returns the digit's count in the tile.
+  auto warp_starts = [&](int digit) {
+    u32 run = 0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const u32 c = s_count[w][threadIdx.x];
-      s_count[w][threadIdx.x] = run;
-      run += c;
+      const u32 k = s_count[w * bins + digit];
+      s_count[w * bins + digit] = (unsigned short)run;
+      run += k;
     }
-  }
-  __syncthreads();
+    return run;
+  };
+
+  for (int pass = 0; pass < a.passes; ++pass) {
+    const int shift = pass * a.digit;
+    const bool last = pass == a.passes - 1;
+    // counts of the stretch
+    u32* row = a.counts + (size_t)cta * bins;
+    if (single) {
+      rank_tile(lo, pass, shift, true);
+      for (int d = threadIdx.x; d < bins; d += kThreads) row[d] = s_tile[d] = warp_starts(d);
+    } else {
+      for (int d = threadIdx.x; d < bins; d += kThreads) s_tile[d] = 0;
+      __syncthreads();
+      for (i64 i = lo + threadIdx.x; i < hi; i += kThreads)
+        atomicAdd(&s_tile[(pair_key(item_at(i, pass, true)) >> shift) & (bins - 1)], 1u);
+      __syncthreads();
+      for (int d = threadIdx.x; d < bins; d += kThreads) row[d] = s_tile[d];
+    }
+    barrier(give_up);
+    // all counts: of each digit, and of each digit in the CTAs before this one; `groups` groups of threads share the rows
+    {
+      const int per_row = min(bins / 4, kThreads), groups = kThreads / per_row, group = threadIdx.x / per_row;
+      const int d = (threadIdx.x % per_row) * 4;
+      u32* s_total = (u32*)s_items;                    // groups x bins
+      u32* s_before = s_total + groups * bins;
+      uint4 total = make_uint4(0, 0, 0, 0), before = total;
+#pragma unroll 4
+      for (int g = group; g < a.ctas; g += groups) {
+        const uint4 v = __ldcg((const uint4*)(a.counts + (size_t)g * bins + d));
+        total.x += v.x, total.y += v.y, total.z += v.z, total.w += v.w;
+        if (g < cta) before.x += v.x, before.y += v.y, before.z += v.z, before.w += v.w;
+      }
+      *(uint4*)(s_total + group * bins + d) = total;
+      *(uint4*)(s_before + group * bins + d) = before;
+      __syncthreads();
+      const int per = (bins + kThreads - 1) / kThreads;  // digits per thread, 1 .. 4
+      u32 sum = 0;
+      for (int q = 0; q < per; ++q) {
+        const int e = threadIdx.x * per + q;
+        if (e < bins)
+          for (int g = 0; g < groups; ++g) sum += s_total[g * bins + e];
+      }
+      u32 start = scan_threads(sum, s_scan);
+      for (int q = 0; q < per; ++q) {
+        const int e = threadIdx.x * per + q;
+        if (e >= bins) break;
+        u32 all = 0, mine = 0;
+        for (int g = 0; g < groups; ++g) all += s_total[g * bins + e], mine += s_before[g * bins + e];
+        s_base[e] = start + mine;
+        if (c.result == SORT_ORDER && a.passes == 1 && cta == 0 && e <= c.source.num_keys) c.offsets[e] = start;
+        start += all;
+      }
+      __syncthreads();
+    }
+    // to their places
+    for (i64 base = lo; base < hi; base += kTile) {
+      if (!single) {
+        rank_tile(base, pass, shift, false);
+        for (int d = threadIdx.x; d < bins; d += kThreads) s_tile[d] = warp_starts(d);
+      }
+      __syncthreads();
+      // s_tile: counts -> starts in the tile; s_base: where the tile's first item of a digit goes, less its place in the tile
+      const int per = (bins + kThreads - 1) / kThreads;
+      u32 count[kMaxBins / kThreads], sum = 0;
 #pragma unroll
-  for (int r = 0; r < kRounds; ++r) {
-    const i64 i = base + r * 32 + lane;
-    if (i < n) {
-      const u32 to = s_count[warp][(key[r] >> shift) & (kBins - 1)] + rank[r];
-      out_keys[to] = key[r];
-      out_at[to] = FIRST ? (u32)i : at[i];
+      for (int q = 0; q < kMaxBins / kThreads; ++q) {
+        const int e = threadIdx.x * per + q;
+        count[q] = q < per && e < bins ? s_tile[e] : 0;
+        sum += count[q];
+      }
+      u32 start = scan_threads(sum, s_scan);
+#pragma unroll
+      for (int q = 0; q < kMaxBins / kThreads; ++q) {
+        const int e = threadIdx.x * per + q;
+        if (q >= per || e >= bins) break;
+        s_tile[e] = start;
+        s_base[e] -= start;
+        start += count[q];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int r = 0; r < kRounds; ++r) {
+        const i64 i = base + warp * (kRounds * 32) + r * 32 + lane;
+        if (i < hi) {
+          const u32 digit = (pair_key(t.item[r]) >> shift) & (bins - 1);
+          const u32 at = s_tile[digit] + s_count[warp * bins + digit] + t.rank[r];
+          s_items[at] = t.item[r];
+          if (c.result == SORT_ORDER && last) {
+            const i64 row_of = (i64)(s_base[digit] + at);
+            if (row_of >= n || pair_at(t.item[r]) >= n) continue;  // never, unless memory was overwritten
+            c.place[pair_at(t.item[r])] = pair_key(t.item[r]) < c.source.num_keys ? row_of : ~row_of;
+          }
+        }
+      }
+      __syncthreads();
+      const int items = (int)min((i64)kTile, hi - base);
+      for (int j = threadIdx.x; j < items; j += kThreads) {
+        const u64 item = s_items[j];
+        const i64 at = (i64)(u32)(s_base[(pair_key(item) >> shift) & (bins - 1)] + (u32)j);
+        if (at >= n) continue;  // as above
+        if (c.result == SORT_ORDER && last) c.order_source[at] = pair_at(item);
+        if (c.result != SORT_ORDER || a.passes > 1) to[at] = item;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int q = 0; q < kMaxBins / kThreads; ++q) {
+        const int e = threadIdx.x * per + q;
+        if (q < per && e < bins) s_base[e] += s_tile[e] + count[q];
+      }
+    }
+    u64* free = const_cast<u64*>(from);
+    from = to;
+    to = free;
+    if (!last || c.result == SORT_RANKS || (c.result == SORT_ORDER && a.passes > 1)) barrier(give_up);
+  }
+
+  if (c.result == SORT_ORDER && a.passes > 1) {
+    const i64 experts = c.source.num_keys;
+    for (i64 j = lo + threadIdx.x; j < hi; j += kThreads) {
+      const i64 e = pair_key(__ldcg(from + j)), before = j > 0 ? (i64)pair_key(__ldcg(from + j - 1)) : -1;
+      for (i64 q = before + 1; q <= e; ++q) c.offsets[q] = j;
+      if (j == n - 1)
+        for (i64 q = e + 1; q <= experts; ++q) c.offsets[q] = n;
     }
   }
+  if (c.result == SORT_RANKS) {
+    const u32 none = (u32)c.source.num_keys;
+    auto is_head = [&](i64 i, u32 key) { return key < none && (i == 0 || pair_key(__ldcg(from + i - 1)) != key); };
+    u32 heads = 0;
+    for (i64 i = lo + threadIdx.x; i < hi; i += kThreads) heads += is_head(i, pair_key(__ldcg(from + i)));
+    scan_threads(heads, s_scan);
+    __syncthreads();
+    if (threadIdx.x == 0) a.counts[cta] = s_scan[kWarps];
+    barrier(give_up);
+    u32 mine = 0;
+    for (int g = threadIdx.x; g < cta; g += kThreads) mine += __ldcg(a.counts + g);
+    scan_threads(mine, s_scan);
+    __syncthreads();
+    u32 before = s_scan[kWarps];
+    for (i64 base = lo; base < hi; base += kThreads) {
+      const i64 i = base + threadIdx.x;
+      const u64 item = i < hi ? __ldcg(from + i) : 0;
+      const bool head = i < hi && is_head(i, pair_key(item));
+      const u32 rank = before + scan_threads(head, s_scan) + (head ? 1u : 0u) - 1u;  // of the latest head up to here
+      if (head) c.distinct[rank] = pair_key(item);
+      if (i < hi) to[i] = (u64)(pair_key(item) < none ? rank : kNoRow) << 32 | pair_at(item);
+      __syncthreads();
+      before += s_scan[kWarps];
+    }
+    if (cta == a.ctas - 1 && threadIdx.x == 0) {
+      c.number[0] = before;
+      mail_post(c.mail, 0, before, c.source.counters);
+    }
+  }
+  if (!CLUSTER && c.zero_bytes > 0) clear_rest(c, a.next_piece);
 }
 
-static int key_bits(i64 num_keys) {
+int key_bits(i64 num_keys) {  // of the largest key, num_keys itself
   int bits = 1;
   while (bits < 32 && (num_keys >> bits) != 0) ++bits;
   return bits;
 }
 
-size_t key_sort_bytes(i64 n, i64 num_keys) {
-  (void)num_keys;
+struct Plan {
+  bool cluster;
+  int ctas, bits, passes, digit;
+  i64 stretch;
+  size_t smem() const {
+    const size_t bins = (size_t)1 << digit;
+    return kTile * 8 + bins * 8 + kWarps * bins * 2;
+  }
+};
+
+Plan plan_of(i64 n, i64 num_keys) {
+  Plan p;
   const i64 tiles = (n + kTile - 1) / kTile;
-  Pieces p(nullptr);
-  for (int q = 0; q < 4; ++q) p.take<u32>((size_t)n);
-  p.take<u32>((size_t)(tiles * kBins));
-  return p.used;
+  p.cluster = tiles <= kClusterCtas;
+  const i64 per = p.cluster ? 1 : (tiles + kNumSMs - 1) / kNumSMs;
+  p.stretch = per * kTile;
+  p.ctas = (int)((tiles + per - 1) / per);
+  p.bits = key_bits(num_keys);
+  const int most = p.ctas <= 2 * kClusterCtas ? kClusterBits : kGridBits;
+  p.passes = (p.bits + most - 1) / most;
+  p.digit = (p.bits + p.passes - 1) / p.passes;
+  if (p.digit < 5) p.digit = 5;  // a row of counts is read in pieces of 16 bytes
+  return p;
 }
 
-int key_sort(gsb_ctx* ctx, cudaStream_t stream, const KeySource& source, void* workspace, SortedKeys* out) {
-  const i64 n = source.n;
-  const int tiles = grid_for(n, kTile);
-  Pieces p(workspace);
-  u32 *keys = p.take<u32>((size_t)n), *at = p.take<u32>((size_t)n), *keys_out = p.take<u32>((size_t)n),
-      *at_out = p.take<u32>((size_t)n);
-  u32* count = p.take<u32>((size_t)tiles * kBins);
-  const int bits = key_bits(source.num_keys);
-  for (int shift = 0; shift < bits; shift += 8) {
-    if (shift == 0) k_key_count<true><<<tiles, kThreads, 0, stream>>>(source, nullptr, n, shift, count, tiles);
-    else k_key_count<false><<<tiles, kThreads, 0, stream>>>(source, keys, n, shift, count, tiles);
-    GSB_LAUNCH_OK();
-    k_key_scan<<<1, kScanThreads, 0, stream>>>(count, (i64)tiles * kBins);
-    GSB_LAUNCH_OK();
-    if (shift == 0) k_key_place<true><<<tiles, kThreads, 0, stream>>>(source, nullptr, nullptr, n, shift, count, tiles, keys_out, at_out);
-    else k_key_place<false><<<tiles, kThreads, 0, stream>>>(source, keys, at, n, shift, count, tiles, keys_out, at_out);
-    GSB_LAUNCH_OK();
-    ctx_count_launches(ctx, 3);
-    u32* t = keys; keys = keys_out; keys_out = t;
-    t = at; at = at_out; at_out = t;
+template <bool CLUSTER>
+int launch(gsb_ctx* ctx, cudaStream_t stream, SortArgs& a, int grid, size_t smem) {
+  const void* kernel = (const void*)k_sort_keys<CLUSTER>;
+  static bool known[64] = {};
+  const int device = ctx_device(ctx);
+  if (device < 0 || device >= 64 || !known[device]) {
+    const size_t most = kTile * 8 + (size_t)kMaxBins * (8 + kWarps * 2);
+    GSB_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
+    if (device >= 0 && device < 64) known[device] = true;
   }
-  *out = SortedKeys{keys, at, keys_out};
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  if (CLUSTER) {
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = kClusterCtas;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  } else {
+    attr.id = cudaLaunchAttributeCooperative;
+    attr.val.cooperative = 1;
+  }
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  void* args[] = {&a};
+  GSB_CUDA_OK(cudaLaunchKernelExC(&cfg, kernel, args));
   return GSB_OK;
+}
+
+}  // namespace
+
+size_t key_sort_bytes(i64 n, i64 num_keys) {
+  if (n <= 0) return 256;
+  const Plan p = plan_of(n, num_keys);
+  Pieces w(nullptr);
+  w.take<u64>(32);
+  w.take<u32>((size_t)p.ctas << p.digit);
+  w.take<u64>((size_t)n);
+  w.take<u64>((size_t)n);
+  return w.used;
+}
+
+int key_sort(gsb_ctx* ctx, cudaStream_t stream, const SortCall& call, void* workspace, const u64** pairs) {
+  const i64 n = call.source.n;
+  const Plan p = plan_of(n, call.source.num_keys);
+  Pieces w(workspace);
+  u64* words = w.take<u64>(32);
+  SortArgs a;
+  a.call = call;
+  a.counts = w.take<u32>((size_t)p.ctas << p.digit);
+  a.from = w.take<u64>((size_t)n);
+  a.to = w.take<u64>((size_t)n);
+  a.ctas = p.ctas;
+  a.bits = p.bits;
+  a.passes = p.passes;
+  a.digit = p.digit;
+  a.stretch = p.stretch;
+  a.next_piece = words + 16;
+  int barriers = 2 * p.passes - 1;
+  if (call.result == SORT_RANKS) barriers += 2;
+  if (call.result == SORT_ORDER && p.passes > 1) barriers += 1;
+  a.sync = GridSync{words, 0, (u32)barriers, call.source.counters, (int)ctx_option(ctx, GSB_OPT_MAX_POLLS)};
+  if (pairs) *pairs = ((p.passes + (call.result == SORT_RANKS ? 1 : 0)) & 1) ? a.to : a.from;
+  const i64 pieces = (i64)((call.zero_bytes + kZeroPiece - 1) / kZeroPiece);
+  if (p.cluster) {
+    // CTAs that clear come in clusters too
+    const i64 more = min((pieces + kClusterCtas - 1) / kClusterCtas, (i64)(kNumSMs / kClusterCtas - 1)) * kClusterCtas;
+    return launch<true>(ctx, stream, a, (int)(kClusterCtas + more), p.smem());
+  }
+  GSB_CUDA_OK(cudaMemsetAsync(words, 0, 32 * sizeof(u64), stream));
+  const i64 more = min(pieces, (i64)kNumSMs - p.ctas);
+  return launch<false>(ctx, stream, a, (int)(p.ctas + more), p.smem());
 }
 
 }  // namespace gsb

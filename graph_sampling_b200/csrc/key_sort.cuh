@@ -10,29 +10,44 @@ namespace gsb {
 
 struct KeySource {
   const i64* ids;
-  i64 n;
+  i64 n;         // 1 .. 2^31 - 1
   i64 num_keys;  // below 2^32 - 1
   bool has_dropped;
   i64 dropped;
   i64* counters;
 };
 
-__device__ __forceinline__ u32 key_of(const KeySource& s, i64 i) {
-  const i64 id = __ldg(s.ids + i);
-  return (u64)id < (u64)s.num_keys && !(s.has_dropped && id == s.dropped) ? (u32)id : (u32)s.num_keys;
-}
-// The same, and an id out of range is recorded.
-__device__ u32 checked_key_of(const KeySource& s, i64 i);
+// A sorted position: [key, or what stands for it : 32 | position : 32].
+__host__ __device__ inline u32 pair_key(u64 p) { return (u32)(p >> 32); }
+__host__ __device__ inline u32 pair_at(u64 p) { return (u32)p; }
 
-// Sorted: position at[j] has the j-th smallest key, equal keys in the order of their positions.
-struct SortedKeys {
-  u32* key;
-  u32* at;
-  u32* spare;  // n words that the sort needs no longer
+constexpr u32 kNoRow = 0xffffffffu;
+
+// What a sort leaves behind.
+enum SortResult {
+  SORT_PAIRS,  // [key, position] in order
+  SORT_RANKS,  // [rank of the key among the distinct ones, kNoRow for num_keys; position], the distinct keys, their number
+  SORT_ORDER   // source, place and offsets of expert_rows.cu
+};
+
+struct SortCall {
+  KeySource source;
+  int result;
+  // bytes set to zero on the way: the rows of a dense gradient
+  void* zero = nullptr;
+  size_t zero_bytes = 0;
+  // SORT_RANKS
+  i64* distinct = nullptr;
+  i64* number = nullptr;
+  Mail mail = Mail{nullptr, 0};
+  // SORT_ORDER
+  i64 *offsets = nullptr, *order_source = nullptr, *place = nullptr;
 };
 
 size_t key_sort_bytes(i64 n, i64 num_keys);
-int key_sort(gsb_ctx* ctx, cudaStream_t stream, const KeySource& source, void* workspace, SortedKeys* out);
+// *pairs: the sorted pairs in `workspace` (SORT_PAIRS, SORT_RANKS).  A sort that is given up (a bounded wait ran out) leaves
+// anything at all there: what reads them checks both halves.
+int key_sort(gsb_ctx* ctx, cudaStream_t stream, const SortCall& call, void* workspace, const u64** pairs);
 
 // A caller's memory in pieces that start on 256-byte boundaries.
 struct Pieces {
