@@ -34,7 +34,9 @@ struct SortArgs {
   u32* counts;     // CTAs x bins
   int ctas;        // that sort; the others clear
   int bits, passes, digit;
-  i64 stretch;     // positions per CTA, a multiple of kTile
+  i64 stretch;     // positions per CTA
+  int rounds;      // of a tile: kThreads positions each
+  bool single;     // a stretch is one tile, which stays in registers between counting and placing
   u64* next_piece;   // of the memory to clear (cooperative launches); null: pieces by CTA number
   GridSync sync;
 };
@@ -106,7 +108,6 @@ struct Barrier {
   __device__ __forceinline__ void operator()(F give_up) {
     ++index;
     if constexpr (CLUSTER) {
-      __threadfence();
       asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     } else {
       grid_barrier(a.sync, index, give_up, (u32)a.ctas);
@@ -138,7 +139,8 @@ __global__ void __launch_bounds__(kThreads) k_sort_keys(const SortArgs a) {
   unsigned short* s_count = (unsigned short*)(s_tile + bins);  // kWarps x bins
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const i64 lo = (i64)cta * a.stretch, hi = min(lo + a.stretch, n);
-  const bool single = a.stretch == kTile;
+  const bool single = a.single;
+  const int rounds = a.rounds, tile = rounds * kThreads;
   Barrier<CLUSTER> barrier{a};
   auto give_up = [&] {
     if (c.result == SORT_RANKS) c.number[0] = 0;
@@ -155,25 +157,41 @@ __global__ void __launch_bounds__(kThreads) k_sort_keys(const SortArgs a) {
   auto item_at = [&](i64 i, int pass, bool check) {
     return pass == 0 ? (u64)key_of(c.source, i, check) << 32 | (u64)i : __ldcg(from + i);
   };
-  // Ranks of a tile's items among those of the same digit in their warp; s_count = the warps' counts.
-  auto rank_tile = [&](i64 base, int pass, int shift, bool check) {
-    for (int q = threadIdx.x; q < kWarps * bins / 2; q += kThreads) ((u32*)s_count)[q] = 0;
+  auto load_tile = [&](i64 base, int pass, bool check) {
 #pragma unroll
     for (int r = 0; r < kRounds; ++r) {
-      const i64 i = base + warp * (kRounds * 32) + r * 32 + lane;
-      t.item[r] = i < hi ? item_at(i, pass, check) : ~0ull;
+      const i64 i = base + warp * (rounds * 32) + r * 32 + lane;
+      t.item[r] = r < rounds && i < hi ? item_at(i, pass, check) : ~0ull;
+    }
+  };
+  // Ranks of a tile's items among those of the same digit in their warp; s_count = the warps' counts.  Lanes with the same digit
+  // are found bit by bit (a vote each; the match instruction takes as long as there are different digits: 6 us for eight
+  // rounds of 16 warps, where all votes of 9 bits take 2).
+  auto rank_tile = [&](i64 base, int shift) {
+    for (int q = threadIdx.x; q < kWarps * bins / 8; q += kThreads) ((uint4*)s_count)[q] = make_uint4(0, 0, 0, 0);
+    u32 peers[kRounds];
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r)
+      peers[r] = __ballot_sync(0xffffffffu, r < rounds && base + warp * (rounds * 32) + r * 32 + lane < hi);
+    for (int b = 0; b < a.digit; ++b) {
+#pragma unroll
+      for (int r = 0; r < kRounds; ++r) {
+        const bool bit = (pair_key(t.item[r]) >> (shift + b)) & 1u;
+        const u32 with = __ballot_sync(0xffffffffu, bit);
+        peers[r] &= bit ? with : ~with;
+      }
     }
     __syncthreads();
     unsigned short* mine = s_count + warp * bins;
 #pragma unroll
     for (int r = 0; r < kRounds; ++r) {
-      const bool valid = base + warp * (kRounds * 32) + r * 32 + lane < hi;
-      const u32 digit = valid ? (pair_key(t.item[r]) >> shift) & (bins - 1) : (u32)bins;
-      const u32 peers = __match_any_sync(0xffffffffu, digit);
-      const u32 before = __popc(peers & ((1u << lane) - 1u));
+      if (r >= rounds) break;
+      const bool valid = base + warp * (rounds * 32) + r * 32 + lane < hi;
+      const u32 digit = (pair_key(t.item[r]) >> shift) & (bins - 1);
+      const u32 before = __popc(peers[r] & ((1u << lane) - 1u));
       const u32 found = valid ? mine[digit] : 0;
       __syncwarp();
-      if (valid && before == 0) mine[digit] = (unsigned short)(found + __popc(peers));
+      if (valid && before == 0) mine[digit] = (unsigned short)(found + __popc(peers[r]));
       __syncwarp();
       t.rank[r] = found + before;
     }
@@ -181,12 +199,13 @@ __global__ void __launch_bounds__(kThreads) k_sort_keys(const SortArgs a) {
   };
   // Warps' counts become starts within the digit; returns the digit's count in the tile.
   auto warp_starts = [&](int digit) {
-    u32 run = 0;
+    u32 k[kWarps], run = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) k[w] = s_count[w * bins + digit];
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const u32 k = s_count[w * bins + digit];
       s_count[w * bins + digit] = (unsigned short)run;
-      run += k;
+      run += k[w];
     }
     return run;
   };
@@ -197,25 +216,34 @@ __global__ void __launch_bounds__(kThreads) k_sort_keys(const SortArgs a) {
     // counts of the stretch
     u32* row = a.counts + (size_t)cta * bins;
     if (single) {
-      rank_tile(lo, pass, shift, true);
+      load_tile(lo, pass, true);
+      rank_tile(lo, shift);
       for (int d = threadIdx.x; d < bins; d += kThreads) row[d] = s_tile[d] = warp_starts(d);
     } else {
       for (int d = threadIdx.x; d < bins; d += kThreads) s_tile[d] = 0;
       __syncthreads();
-      for (i64 i = lo + threadIdx.x; i < hi; i += kThreads)
-        atomicAdd(&s_tile[(pair_key(item_at(i, pass, true)) >> shift) & (bins - 1)], 1u);
+      for (i64 i = lo + threadIdx.x; i < hi; i += 4 * kThreads) {
+        u64 item[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (i + q * kThreads < hi) item[q] = item_at(i + q * kThreads, pass, true);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (i + q * kThreads < hi) atomicAdd(&s_tile[(pair_key(item[q]) >> shift) & (bins - 1)], 1u);
+      }
       __syncthreads();
       for (int d = threadIdx.x; d < bins; d += kThreads) row[d] = s_tile[d];
     }
     barrier(give_up);
     // all counts: of each digit, and of each digit in the CTAs before this one; `groups` groups of threads share the rows
     {
-      const int per_row = min(bins / 4, kThreads), groups = kThreads / per_row, group = threadIdx.x / per_row;
+      const int per_row = min(bins / 4, kThreads), groups = min(min(kThreads / per_row, a.ctas), 16), group = threadIdx.x / per_row;
       const int d = (threadIdx.x % per_row) * 4;
       u32* s_total = (u32*)s_items;                    // groups x bins
       u32* s_before = s_total + groups * bins;
       uint4 total = make_uint4(0, 0, 0, 0), before = total;
-#pragma unroll 4
+      if (group < groups) {
+#pragma unroll 8
       for (int g = group; g < a.ctas; g += groups) {
         const uint4 v = __ldcg((const uint4*)(a.counts + (size_t)g * bins + d));
         total.x += v.x, total.y += v.y, total.z += v.z, total.w += v.w;
@@ -223,6 +251,7 @@ __global__ void __launch_bounds__(kThreads) k_sort_keys(const SortArgs a) {
       }
       *(uint4*)(s_total + group * bins + d) = total;
       *(uint4*)(s_before + group * bins + d) = before;
+      }
       __syncthreads();
       const int per = (bins + kThreads - 1) / kThreads;  // digits per thread, 1 .. 4
       u32 sum = 0;
@@ -244,9 +273,10 @@ __global__ void __launch_bounds__(kThreads) k_sort_keys(const SortArgs a) {
       __syncthreads();
     }
     // to their places
-    for (i64 base = lo; base < hi; base += kTile) {
+    if (!single) load_tile(lo, pass, false);
+    for (i64 base = lo; base < hi; base += tile) {
       if (!single) {
-        rank_tile(base, pass, shift, false);
+        rank_tile(base, shift);
         for (int d = threadIdx.x; d < bins; d += kThreads) s_tile[d] = warp_starts(d);
       }
       __syncthreads();
@@ -271,8 +301,8 @@ __global__ void __launch_bounds__(kThreads) k_sort_keys(const SortArgs a) {
       __syncthreads();
 #pragma unroll
       for (int r = 0; r < kRounds; ++r) {
-        const i64 i = base + warp * (kRounds * 32) + r * 32 + lane;
-        if (i < hi) {
+        const i64 i = base + warp * (rounds * 32) + r * 32 + lane;
+        if (r < rounds && i < hi) {
           const u32 digit = (pair_key(t.item[r]) >> shift) & (bins - 1);
           const u32 at = s_tile[digit] + s_count[warp * bins + digit] + t.rank[r];
           s_items[at] = t.item[r];
@@ -283,8 +313,9 @@ __global__ void __launch_bounds__(kThreads) k_sort_keys(const SortArgs a) {
           }
         }
       }
+      if (base + tile < hi) load_tile(base + tile, pass, false);  // on its way while this tile is written
       __syncthreads();
-      const int items = (int)min((i64)kTile, hi - base);
+      const int items = (int)min((i64)tile, hi - base);
       for (int j = threadIdx.x; j < items; j += kThreads) {
         const u64 item = s_items[j];
         const i64 at = (i64)(u32)(s_base[(pair_key(item) >> shift) & (bins - 1)] + (u32)j);
@@ -316,25 +347,52 @@ __global__ void __launch_bounds__(kThreads) k_sort_keys(const SortArgs a) {
   }
   if (c.result == SORT_RANKS) {
     const u32 none = (u32)c.source.num_keys;
-    auto is_head = [&](i64 i, u32 key) { return key < none && (i == 0 || pair_key(__ldcg(from + i - 1)) != key); };
-    u32 heads = 0;
-    for (i64 i = lo + threadIdx.x; i < hi; i += kThreads) heads += is_head(i, pair_key(__ldcg(from + i)));
-    scan_threads(heads, s_scan);
+    // the tile's items, and which of them are the first of their key; returns how many of the warp's are
+    u32 first[kRounds];
+    auto find_heads = [&](i64 base) {
+      const i64 begin = base + warp * (rounds * 32);
+      u32 before = begin > 0 && begin < hi ? pair_key(__ldcg(from + begin - 1)) : kNoRow, all = 0;
+#pragma unroll
+      for (int r = 0; r < kRounds; ++r) {
+        const i64 i = begin + r * 32 + lane;
+        t.item[r] = r < rounds && i < hi ? __ldcg(from + i) : (u64)kNoRow << 32;
+      }
+#pragma unroll
+      for (int r = 0; r < kRounds; ++r) {
+        const u32 key = pair_key(t.item[r]);
+        u32 left = __shfl_up_sync(0xffffffffu, key, 1);
+        if (lane == 0) left = before;
+        before = __shfl_sync(0xffffffffu, key, 31);
+        first[r] = __ballot_sync(0xffffffffu, key < none && key != left);
+        all += __popc(first[r]);
+      }
+      return all;
+    };
+    u32 mine = 0, heads = 0;
+    for (i64 base = lo; base < hi; base += tile) mine += heads = find_heads(base);
+    scan_threads(lane == 0 ? mine : 0, s_scan);
     __syncthreads();
     if (threadIdx.x == 0) a.counts[cta] = s_scan[kWarps];
     barrier(give_up);
-    u32 mine = 0;
-    for (int g = threadIdx.x; g < cta; g += kThreads) mine += __ldcg(a.counts + g);
-    scan_threads(mine, s_scan);
+    u32 others = 0;
+    for (int g = threadIdx.x; g < cta; g += kThreads) others += __ldcg(a.counts + g);
+    scan_threads(others, s_scan);
     __syncthreads();
     u32 before = s_scan[kWarps];
-    for (i64 base = lo; base < hi; base += kThreads) {
-      const i64 i = base + threadIdx.x;
-      const u64 item = i < hi ? __ldcg(from + i) : 0;
-      const bool head = i < hi && is_head(i, pair_key(item));
-      const u32 rank = before + scan_threads(head, s_scan) + (head ? 1u : 0u) - 1u;  // of the latest head up to here
-      if (head) c.distinct[rank] = pair_key(item);
-      if (i < hi) to[i] = (u64)(pair_key(item) < none ? rank : kNoRow) << 32 | pair_at(item);
+    for (i64 base = lo; base < hi; base += tile) {
+      if (!single) heads = find_heads(base);
+      u32 rank = before + scan_threads(lane == 0 ? heads : 0, s_scan);
+      rank = __shfl_sync(0xffffffffu, rank, 0);
+#pragma unroll
+      for (int r = 0; r < kRounds; ++r) {
+        const i64 i = base + warp * (rounds * 32) + r * 32 + lane;
+        const u32 key = pair_key(t.item[r]), my = rank + __popc(first[r] & (2u << lane) - 1u) - 1u;  // of the latest head up to here
+        if (r < rounds && i < hi) {
+          if (first[r] >> lane & 1u) c.distinct[my] = key;
+          to[i] = (u64)(key < none ? my : kNoRow) << 32 | pair_at(t.item[r]);
+        }
+        rank += __popc(first[r]);
+      }
       __syncthreads();
       before += s_scan[kWarps];
     }
@@ -354,7 +412,8 @@ int key_bits(i64 num_keys) {  // of the largest key, num_keys itself
 
 struct Plan {
   bool cluster;
-  int ctas, bits, passes, digit;
+  int ctas, bits, passes, digit, rounds;
+  bool single;
   i64 stretch;
   size_t smem() const {
     const size_t bins = (size_t)1 << digit;
@@ -362,15 +421,18 @@ struct Plan {
   }
 };
 
-Plan plan_of(i64 n, i64 num_keys) {
+// With memory to clear, half of the SMs sort and the others clear.
+Plan plan_of(i64 n, i64 num_keys, bool clears) {
   Plan p;
-  const i64 tiles = (n + kTile - 1) / kTile;
-  p.cluster = tiles <= kClusterCtas;
-  const i64 per = p.cluster ? 1 : (tiles + kNumSMs - 1) / kNumSMs;
-  p.stretch = per * kTile;
-  p.ctas = (int)((tiles + per - 1) / per);
+  p.cluster = n <= (i64)kClusterCtas * kTile;
+  const i64 most_ctas = p.cluster ? kClusterCtas : clears ? kNumSMs / 2 : kNumSMs;
+  const i64 shares = (n + kThreads - 1) / kThreads, per = (shares + most_ctas - 1) / most_ctas;
+  p.stretch = per * kThreads;
+  p.ctas = (int)((shares + per - 1) / per);
+  p.single = per <= kRounds;
+  p.rounds = p.single ? (int)per : kRounds;
   p.bits = key_bits(num_keys);
-  const int most = p.ctas <= 2 * kClusterCtas ? kClusterBits : kGridBits;
+  const int most = p.cluster ? kClusterBits : kGridBits;
   p.passes = (p.bits + most - 1) / most;
   p.digit = (p.bits + p.passes - 1) / p.passes;
   if (p.digit < 5) p.digit = 5;  // a row of counts is read in pieces of 16 bytes
@@ -412,7 +474,7 @@ int launch(gsb_ctx* ctx, cudaStream_t stream, SortArgs& a, int grid, size_t smem
 
 size_t key_sort_bytes(i64 n, i64 num_keys) {
   if (n <= 0) return 256;
-  const Plan p = plan_of(n, num_keys);
+  const Plan p = plan_of(n, num_keys, false);  // the larger of the two
   Pieces w(nullptr);
   w.take<u64>(32);
   w.take<u32>((size_t)p.ctas << p.digit);
@@ -423,7 +485,7 @@ size_t key_sort_bytes(i64 n, i64 num_keys) {
 
 int key_sort(gsb_ctx* ctx, cudaStream_t stream, const SortCall& call, void* workspace, const u64** pairs) {
   const i64 n = call.source.n;
-  const Plan p = plan_of(n, call.source.num_keys);
+  const Plan p = plan_of(n, call.source.num_keys, call.zero_bytes > 0);
   Pieces w(workspace);
   u64* words = w.take<u64>(32);
   SortArgs a;
@@ -436,6 +498,8 @@ int key_sort(gsb_ctx* ctx, cudaStream_t stream, const SortCall& call, void* work
   a.passes = p.passes;
   a.digit = p.digit;
   a.stretch = p.stretch;
+  a.rounds = p.rounds;
+  a.single = p.single;
   a.next_piece = words + 16;
   int barriers = 2 * p.passes - 1;
   if (call.result == SORT_RANKS) barriers += 2;
