@@ -94,11 +94,11 @@ __global__ void __launch_bounds__(kSumThreads) k_sum_rows(const SumArgs a, const
       for (int q = 0; q < N; ++q) sum[s][q] = 0.f;
     }
   };
-  for (i64 j = begin; j < end; j += kAhead) {
-    u64 p[kAhead + 1];
-    Unit<T, BYTES> v[kAhead][STEPS];
+  u64 p[kAhead + 1], next[kAhead + 1];
 #pragma unroll
-    for (int u = 0; u <= kAhead; ++u) p[u] = j + u < a.n ? sorted[j + u] : ~0ull;
+  for (int u = 0; u <= kAhead; ++u) p[u] = begin + u < a.n ? __ldg(sorted + begin + u) : ~0ull;
+  for (i64 j = begin; j < end; j += kAhead) {
+    Unit<T, BYTES> v[kAhead][STEPS];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       if (j + u >= end || !usable(a, p[u])) continue;
@@ -107,6 +107,9 @@ __global__ void __launch_bounds__(kSumThreads) k_sum_rows(const SumArgs a, const
       for (int s = 0; s < STEPS; ++s)
         if (first + s * a.lanes < a.units) v[u][s] = load_unit_once(from + first + s * a.lanes);
     }
+    next[0] = p[kAhead];
+#pragma unroll
+    for (int u = 1; u <= kAhead; ++u) next[u] = j + kAhead + u < a.n ? __ldg(sorted + j + kAhead + u) : ~0ull;
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       if (j + u >= end || !usable(a, p[u])) return;  // the sorted list ends with the positions that belong to no row
@@ -121,31 +124,104 @@ __global__ void __launch_bounds__(kSumThreads) k_sum_rows(const SumArgs a, const
       else if (ends || j + u + 1 == end) put(part + (2 * chunk + (head ? 0 : 1)) * width, 1.f);
       if (ends) head = false;
     }
+#pragma unroll
+    for (int u = 0; u <= kAhead; ++u) p[u] = next[u];
   }
 }
 
-// Where the last sum of a chunk began there and goes on: its part and those of the chunks behind, in their order.
+// Where the last sum of a chunk began there and goes on: its part and those of the chunks behind.  A CTA looks at kJoinSpan
+// chunks and kJoinColumns columns.  A warp adds up to kJoinShort parts in their order, with the next ones on their way; longer
+// runs (a hub's, a frequent token's) are shared by the CTA's warps, whose sums are added in the warps' order.
+constexpr int kJoinThreads = 512, kJoinWarps = kJoinThreads / 32, kJoinSpan = 64, kJoinSteps = 4, kJoinColumns = 32 * kJoinSteps;
+constexpr int kJoinShort = 32;
+
 template <class O>
-__global__ void __launch_bounds__(kSumThreads) k_join_rows(const SumArgs a, i64 width, i64 chunks,
-                                                           const u64* __restrict__ sorted, const float* __restrict__ part,
-                                                           O* __restrict__ out) {
-  const i64 column = (i64)blockIdx.y * kSumThreads + threadIdx.x;
-  for (i64 c = blockIdx.x; c + 1 < chunks; c += gridDim.x) {
-    const i64 begin = c * a.chunk, end = begin + a.chunk;
-    const u32 row = pair_key(sorted[end - 1]);
-    if (row >= a.num_rows || pair_key(sorted[end]) != row || (begin > 0 && pair_key(sorted[begin - 1]) == row)) continue;
-    if (column >= width) continue;
-    float sum = part[(2 * c + 1) * width + column];
-    for (i64 next = c + 1; next < chunks && pair_key(sorted[next * a.chunk]) == row; ++next)
-      sum += part[2 * next * width + column];
-    out[(i64)row * width + column] = from_float<O>(sum * a.scale);
+__global__ void __launch_bounds__(kJoinThreads) k_join_rows(const SumArgs a, i64 width, i64 chunks,
+                                                            const u64* __restrict__ sorted, const float* __restrict__ part,
+                                                            O* __restrict__ out) {
+  __shared__ int s_found, s_long, s_chunk[kJoinSpan], s_run[kJoinSpan];
+  __shared__ float s_sum[kJoinWarps][kJoinColumns];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const i64 first = (i64)blockIdx.x * kJoinSpan, column = (i64)blockIdx.y * kJoinColumns + lane;
+  if (threadIdx.x == 0) s_found = s_long = 0;
+  __syncthreads();
+  if (threadIdx.x < kJoinSpan) {
+    const i64 c = first + threadIdx.x, begin = c * a.chunk, end = begin + a.chunk;
+    if (c + 1 < chunks) {
+      const u32 row = pair_key(__ldg(sorted + end - 1));
+      if (row < a.num_rows && pair_key(__ldg(sorted + end)) == row && (begin == 0 || pair_key(__ldg(sorted + begin - 1)) != row))
+        s_chunk[atomicAdd(&s_found, 1)] = threadIdx.x;
+    }
+  }
+  __syncthreads();
+  float sum[kJoinSteps];
+  auto add = [&](i64 from, i64 n, i64 step) {  // head parts of n chunks, `step` apart
+#pragma unroll 8
+    for (i64 q = 0; q < n; ++q) {
+      const float* row = part + 2 * (from + q * step) * width;
+#pragma unroll
+      for (int s = 0; s < kJoinSteps; ++s)
+        if (column + 32 * s < width) sum[s] += __ldg(row + column + 32 * s);
+    }
+  };
+  for (int f = warp; f < s_found; f += kJoinWarps) {
+    const i64 c = first + s_chunk[f];
+    const u32 row = pair_key(__ldg(sorted + (c + 1) * a.chunk));
+    i64 run = 0;  // chunks behind that go on with it
+    for (;;) {
+      const i64 next = c + 1 + run + lane;
+      const u32 with = __ballot_sync(0xffffffffu, next < chunks && pair_key(__ldg(sorted + next * a.chunk)) == row);
+      run += with == 0xffffffffu ? 32 : __ffs(~with) - 1;
+      if (with != 0xffffffffu) break;
+    }
+    if (run > kJoinShort) {
+      if (lane == 0) {
+        const int at = atomicAdd(&s_long, 1);
+        s_run[at] = (int)(c - first);
+      }
+      continue;
+    }
+#pragma unroll
+    for (int s = 0; s < kJoinSteps; ++s) sum[s] = column + 32 * s < width ? __ldg(part + (2 * c + 1) * width + column + 32 * s) : 0.f;
+    add(c + 1, run, 1);
+#pragma unroll
+    for (int s = 0; s < kJoinSteps; ++s)
+      if (column + 32 * s < width) out[(i64)row * width + column + 32 * s] = from_float<O>(sum[s] * a.scale);
+  }
+  __syncthreads();
+  for (int f = 0; f < s_long; ++f) {
+    const i64 c = first + s_run[f];
+    const u32 row = pair_key(__ldg(sorted + (c + 1) * a.chunk));
+    i64 run = 0;
+    for (;;) {  // every warp for itself
+      const i64 next = c + 1 + run + lane;
+      const u32 with = __ballot_sync(0xffffffffu, next < chunks && pair_key(__ldg(sorted + next * a.chunk)) == row);
+      run += with == 0xffffffffu ? 32 : __ffs(~with) - 1;
+      if (with != 0xffffffffu) break;
+    }
+#pragma unroll
+    for (int s = 0; s < kJoinSteps; ++s)
+      sum[s] = warp == 0 && column + 32 * s < width ? __ldg(part + (2 * c + 1) * width + column + 32 * s) : 0.f;
+    add(c + 1 + warp, run > warp ? (run - warp + kJoinWarps - 1) / kJoinWarps : 0, kJoinWarps);
+#pragma unroll
+    for (int s = 0; s < kJoinSteps; ++s) s_sum[warp][lane + 32 * s] = sum[s];
+    __syncthreads();
+    if (threadIdx.x < kJoinColumns && (i64)blockIdx.y * kJoinColumns + threadIdx.x < width) {
+      float all = 0.f;
+#pragma unroll
+      for (int w = 0; w < kJoinWarps; ++w) all += s_sum[w][threadIdx.x];
+      out[(i64)row * width + (i64)blockIdx.y * kJoinColumns + threadIdx.x] = from_float<O>(all * a.scale);
+    }
+    __syncthreads();
   }
 }
 
-// Chunks: long enough that their ends are few beside what is read, short enough that there are many of them.
-static int sum_chunk(i64 n) {
-  i64 c = (n / 16384 + 31) / 32 * 32;
-  return (int)(c < 32 ? 32 : c);
+// Positions per chunk: enough warps for all SMs where there are few positions, else so many that the ends of a chunk, whose
+// sums are written and read once more, are few beside what it reads.
+static int sum_chunk(i64 n, i64 row_len) {
+  const i64 warps_a_position = max((i64)1, row_len / 512);
+  i64 c = n * warps_a_position / (kNumSMs * 32);
+  return (int)(c < 4 ? 4 : c > 128 ? 128 : c);
 }
 
 struct GradPlan {
@@ -156,7 +232,7 @@ struct GradPlan {
 
 static GradPlan grad_plan(i64 n, i64 num_rows, i64 row_len) {
   GradPlan g;
-  g.chunk = sum_chunk(n);
+  g.chunk = sum_chunk(n, row_len);
   g.chunks = (n + g.chunk - 1) / g.chunk;
   g.sort_bytes = key_sort_bytes(n, num_rows);
   Pieces p(nullptr);
@@ -211,10 +287,10 @@ static int sum_sorted(gsb_ctx* ctx, cudaStream_t stream, const GradCall& c, cons
   });
   GSB_LAUNCH_OK();
   if (plan.chunks > 1) {
-    const dim3 grid((unsigned)min(plan.chunks - 1, (i64)kNumSMs * 16), grid_for(c.row_len, kSumThreads));
-    if (c.out_dtype == GSB_F32) k_join_rows<float><<<grid, kSumThreads, 0, stream>>>(a, c.row_len, plan.chunks, sorted, part, (float*)c.out);
-    else if (c.out_dtype == GSB_F16) k_join_rows<__half><<<grid, kSumThreads, 0, stream>>>(a, c.row_len, plan.chunks, sorted, part, (__half*)c.out);
-    else k_join_rows<__nv_bfloat16><<<grid, kSumThreads, 0, stream>>>(a, c.row_len, plan.chunks, sorted, part, (__nv_bfloat16*)c.out);
+    const dim3 grid(grid_for(plan.chunks - 1, kJoinSpan), grid_for(c.row_len, kJoinColumns));
+    if (c.out_dtype == GSB_F32) k_join_rows<float><<<grid, kJoinThreads, 0, stream>>>(a, c.row_len, plan.chunks, sorted, part, (float*)c.out);
+    else if (c.out_dtype == GSB_F16) k_join_rows<__half><<<grid, kJoinThreads, 0, stream>>>(a, c.row_len, plan.chunks, sorted, part, (__half*)c.out);
+    else k_join_rows<__nv_bfloat16><<<grid, kJoinThreads, 0, stream>>>(a, c.row_len, plan.chunks, sorted, part, (__nv_bfloat16*)c.out);
     GSB_LAUNCH_OK();
     ctx_count_launches(ctx, 1);
   }
@@ -224,7 +300,7 @@ static int sum_sorted(gsb_ctx* ctx, cudaStream_t stream, const GradCall& c, cons
 // What the calls that sum gradients ask of their arguments.
 static int check_grad(i64 n, i64 num_rows, i64 row_len, i64 grad_stride, int dtype, int out_dtype) {
   GSB_REQUIRE(n >= 0 && n < ((i64)1 << 31) && num_rows >= 0 && num_rows < 0xffffffffll, GSB_ERR_INVALID_ARGUMENT);
-  GSB_REQUIRE(row_len >= 1 && row_len <= ((i64)1 << 31) && grad_stride >= 0, GSB_ERR_INVALID_ARGUMENT);
+  GSB_REQUIRE(row_len >= 1 && row_len <= GSB_MAX_ROW_LEN && grad_stride >= 0, GSB_ERR_INVALID_ARGUMENT);
   GSB_REQUIRE(value_bytes(dtype) != 0 && (out_dtype == dtype || out_dtype == GSB_F32), GSB_ERR_INVALID_ARGUMENT);
   return GSB_OK;
 }
@@ -237,7 +313,7 @@ extern "C" int gsb_embedding_lookup(gsb_ctx* ctx, void* stream_, const void* tab
                                     int64_t row_len, int64_t row_stride, const int64_t* ids, int64_t n, float scale,
                                     int has_padding, int64_t padding_id, void* out) {
   GSB_ENTER(ctx);
-  GSB_REQUIRE(num_rows >= 0 && row_len >= 1 && row_stride >= 0 && n >= 0 && value_bytes(dtype) != 0, GSB_ERR_INVALID_ARGUMENT);
+  GSB_REQUIRE(num_rows >= 0 && row_len >= 1 && row_len <= GSB_MAX_ROW_LEN && row_stride >= 0 && n >= 0 && value_bytes(dtype) != 0, GSB_ERR_INVALID_ARGUMENT);
   if (n == 0) return GSB_OK;
   GSB_REQUIRE((table || num_rows == 0) && ids && out, GSB_ERR_INVALID_ARGUMENT);
   const void* from = nullptr;

@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(kRowThreads) k_combine_grad(const RowArgs a, c
 
 static int check_rows(i64 tokens, i64 per_token, i64 row_len, int dtype, i64 stride, const void* place, const void* weights,
                       int weights_dtype) {
-  GSB_REQUIRE(tokens >= 0 && per_token >= 1 && per_token < ((i64)1 << 31) && row_len >= 1 && row_len <= ((i64)1 << 31) &&
+  GSB_REQUIRE(tokens >= 0 && per_token >= 1 && per_token < ((i64)1 << 31) && row_len >= 1 && row_len <= GSB_MAX_ROW_LEN &&
                   stride >= 0 && value_bytes(dtype) != 0,
               GSB_ERR_INVALID_ARGUMENT);
   GSB_REQUIRE(tokens == 0 || place, GSB_ERR_INVALID_ARGUMENT);
