@@ -9,6 +9,7 @@
 #include <type_traits>
 
 #include "key_sort.cuh"
+#include "launch.cuh"
 #include "row_values.cuh"
 #include "scan.cuh"
 
@@ -16,30 +17,50 @@ namespace gsb {
 
 constexpr int kLookupThreads = 256;
 
-template <class T, int BYTES>
+// A group of lanes takes ROWS neighbouring rows of the result at a time: all reads of a tile of them are on their way before
+// anything is written.
+template <class T, int BYTES, int STEPS>
 __global__ void __launch_bounds__(kLookupThreads) k_lookup_rows(const Unit<T, BYTES>* __restrict__ table, i64 num_rows,
                                                                 i64 stride, i64 units, const i64* __restrict__ ids, i64 n,
                                                                 float scale, bool has_padding, i64 padding, int lanes,
                                                                 Unit<T, BYTES>* __restrict__ out, i64* counters) {
+  constexpr int kRows = STEPS == 1 ? 4 : 2, N = Unit<T, BYTES>::N;
+  await_previous();
   const int lane = threadIdx.x & (lanes - 1);
-  const i64 groups = (i64)gridDim.x * (kLookupThreads / lanes);
-  for (i64 i = ((i64)blockIdx.x * kLookupThreads + threadIdx.x) / lanes; i < n; i += groups) {
-    i64 row = __ldg(ids + i);
-    if ((u64)row >= (u64)num_rows || (has_padding && row == padding)) {
-      if (lane == 0 && !(has_padding && row == padding)) raise_error(counters, GSB_ERR_INDEX_RANGE, i);
-      row = -1;
-    }
-    for (i64 j = lane; j < units; j += lanes) {
-      Unit<T, BYTES> v;
-      if (row >= 0) {
-        v = load_unit(table + row * stride + j);
+  const i64 step = (i64)gridDim.x * (kLookupThreads / lanes) * kRows;
+  for (i64 i = ((i64)blockIdx.x * kLookupThreads + threadIdx.x) / lanes * kRows; i < n; i += step) {
+    i64 row[kRows];
 #pragma unroll
-        for (int q = 0; q < v.N; ++q) v.v[q] = from_float<T>(to_float(v.v[q]) * scale);
-      } else {
-#pragma unroll
-        for (int q = 0; q < v.N; ++q) v.v[q] = from_float<T>(0.f);
+    for (int r = 0; r < kRows; ++r) {
+      row[r] = i + r < n ? __ldg(ids + i + r) : -1;
+      const bool padded = has_padding && row[r] == padding;
+      if ((u64)row[r] >= (u64)num_rows || padded) {
+        if (lane == 0 && !padded && i + r < n) raise_error(counters, GSB_ERR_INDEX_RANGE, i + r);
+        row[r] = -1;
       }
-      store_unit(out + i * units + j, v);
+    }
+    for (i64 j = lane; j < units; j += lanes * STEPS) {
+      Unit<T, BYTES> v[kRows][STEPS];
+#pragma unroll
+      for (int r = 0; r < kRows; ++r)
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+          v[r][s].clear();
+          if (row[r] >= 0 && j + s * lanes < units) v[r][s] = load_unit(table + row[r] * stride + j + s * lanes);
+        }
+#pragma unroll
+      for (int r = 0; r < kRows; ++r)
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+          if (scale != 1.f && row[r] >= 0) {
+            float f[N];
+            v[r][s].get(f);
+#pragma unroll
+            for (int q = 0; q < N; ++q) f[q] *= scale;
+            v[r][s].set(f);
+          }
+          if (i + r < n && j + s * lanes < units) store_unit(out + (i + r) * units + j + s * lanes, v[r][s]);
+        }
     }
   }
 }
@@ -50,9 +71,11 @@ __device__ __forceinline__ void store_values(O* to, const float* v, float scale)
   constexpr int kBytes = N * (int)sizeof(O), kUnit = kBytes > 16 ? 16 : kBytes, kPer = kUnit / (int)sizeof(O);
 #pragma unroll
   for (int p = 0; p < N / kPer; ++p) {
-    Unit<O, kUnit> u;
+    float f[kPer];
 #pragma unroll
-    for (int q = 0; q < kPer; ++q) u.v[q] = from_float<O>(v[p * kPer + q] * scale);
+    for (int q = 0; q < kPer; ++q) f[q] = v[p * kPer + q] * scale;
+    Unit<O, kUnit> u;
+    u.set(f);
     store_unit((Unit<O, kUnit>*)(to + p * kPer), u);
   }
 }
@@ -77,7 +100,8 @@ template <class T, class O, int BYTES, int STEPS>
 __global__ void __launch_bounds__(kSumThreads) k_sum_rows(const SumArgs a, const Unit<T, BYTES>* __restrict__ grad,
                                                           const u64* __restrict__ sorted, O* __restrict__ out,
                                                           float* __restrict__ part) {
-  constexpr int N = Unit<T, BYTES>::N, kAhead = STEPS >= 4 ? 2 : 4;
+  constexpr int N = Unit<T, BYTES>::N, kAhead = STEPS >= 3 ? 2 : 4;
+  await_previous();
   const i64 chunk = ((i64)blockIdx.x * kSumThreads + threadIdx.x) / a.lanes;
   const i64 begin = chunk * a.chunk, end = min(begin + a.chunk, a.n);
   const i64 first = (i64)blockIdx.y * a.lanes * STEPS + (threadIdx.x & (a.lanes - 1));
@@ -115,9 +139,12 @@ __global__ void __launch_bounds__(kSumThreads) k_sum_rows(const SumArgs a, const
       if (j + u >= end || !usable(a, p[u])) return;  // the sorted list ends with the positions that belong to no row
 #pragma unroll
       for (int s = 0; s < STEPS; ++s)
-        if (first + s * a.lanes < a.units)
+        if (first + s * a.lanes < a.units) {
+          float f[N];
+          v[u][s].get(f);
 #pragma unroll
-          for (int q = 0; q < N; ++q) sum[s][q] += to_float(v[u][s].v[q]);
+          for (int q = 0; q < N; ++q) sum[s][q] += f[q];
+        }
       const u32 row = pair_key(p[u]);
       const bool ends = pair_key(p[u + 1]) != row;
       if (ends && !head) put(out + (i64)row * width, a.scale);
@@ -141,6 +168,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_join_rows(const SumArgs a, i64
                                                             O* __restrict__ out) {
   __shared__ int s_found, s_long, s_chunk[kJoinSpan], s_run[kJoinSpan];
   __shared__ float s_sum[kJoinWarps][kJoinColumns];
+  await_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const i64 first = (i64)blockIdx.x * kJoinSpan, column = (i64)blockIdx.y * kJoinColumns + lane;
   if (threadIdx.x == 0) s_found = s_long = 0;
@@ -216,11 +244,11 @@ __global__ void __launch_bounds__(kJoinThreads) k_join_rows(const SumArgs a, i64
   }
 }
 
-// Positions per chunk: enough warps for all SMs where there are few positions, else so many that the ends of a chunk, whose
-// sums are written and read once more, are few beside what it reads.
+// Positions per chunk: enough groups of lanes for two full sets of warps where there are few positions, else so many that the
+// ends of a chunk, whose sums are written and read once more, are few beside what it reads.
 static int sum_chunk(i64 n, i64 row_len) {
-  const i64 warps_a_position = max((i64)1, row_len / 512);
-  i64 c = n * warps_a_position / (kNumSMs * 32);
+  const i64 lanes = row_len >= 128 ? 32 : row_len >= 64 ? 16 : 8, tiles = (row_len + 511) / 512;
+  const i64 c = n * tiles * lanes / 32 / (kNumSMs * 128);
   return (int)(c < 4 ? 4 : c > 128 ? 128 : c);
 }
 
@@ -247,16 +275,13 @@ static void launch_sum(cudaStream_t stream, SumArgs a, i64 chunks, const void* g
                        const u64* sorted, void* out, float* part) {
   a.units = row_bytes / BYTES;
   a.stride = stride_bytes / BYTES;
-  a.lanes = 1;
-  while (a.lanes < 32 && a.lanes < a.units) a.lanes *= 2;
-  auto go = [&](auto steps) {
+  const RowShape shape = row_shape(a.units);
+  a.lanes = shape.lanes;
+  with_steps(shape.steps, [&](auto steps) {
     constexpr int S = decltype(steps)::value;
     const dim3 grid(grid_for(chunks * a.lanes, kSumThreads), grid_for(a.units, a.lanes * S));
-    k_sum_rows<T, O, BYTES, S><<<grid, kSumThreads, 0, stream>>>(a, (const Unit<T, BYTES>*)grad, sorted, (O*)out, part);
-  };
-  if (a.units <= 32) go(std::integral_constant<int, 1>{});
-  else if (a.units <= 64) go(std::integral_constant<int, 2>{});
-  else go(std::integral_constant<int, 4>{});
+    launch_behind(stream, k_sum_rows<T, O, BYTES, S>, grid, kSumThreads, a, (const Unit<T, BYTES>*)grad, sorted, (O*)out, part);
+  });
 }
 
 struct GradCall {
@@ -288,9 +313,9 @@ static int sum_sorted(gsb_ctx* ctx, cudaStream_t stream, const GradCall& c, cons
   GSB_LAUNCH_OK();
   if (plan.chunks > 1) {
     const dim3 grid(grid_for(plan.chunks - 1, kJoinSpan), grid_for(c.row_len, kJoinColumns));
-    if (c.out_dtype == GSB_F32) k_join_rows<float><<<grid, kJoinThreads, 0, stream>>>(a, c.row_len, plan.chunks, sorted, part, (float*)c.out);
-    else if (c.out_dtype == GSB_F16) k_join_rows<__half><<<grid, kJoinThreads, 0, stream>>>(a, c.row_len, plan.chunks, sorted, part, (__half*)c.out);
-    else k_join_rows<__nv_bfloat16><<<grid, kJoinThreads, 0, stream>>>(a, c.row_len, plan.chunks, sorted, part, (__nv_bfloat16*)c.out);
+    if (c.out_dtype == GSB_F32) launch_behind(stream, k_join_rows<float>, grid, kJoinThreads, a, c.row_len, plan.chunks, sorted, part, (float*)c.out);
+    else if (c.out_dtype == GSB_F16) launch_behind(stream, k_join_rows<__half>, grid, kJoinThreads, a, c.row_len, plan.chunks, sorted, part, (__half*)c.out);
+    else launch_behind(stream, k_join_rows<__nv_bfloat16>, grid, kJoinThreads, a, c.row_len, plan.chunks, sorted, part, (__nv_bfloat16*)c.out);
     GSB_LAUNCH_OK();
     ctx_count_launches(ctx, 1);
   }
@@ -334,13 +359,14 @@ extern "C" int gsb_embedding_lookup(gsb_ctx* ctx, void* stream_, const void* tab
       typedef decltype(value) T;
       constexpr int kBytes = decltype(bytes)::value;
       const i64 units = row_len * size / kBytes;
-      int lanes = 1;
-      while (lanes < 32 && lanes < units) lanes *= 2;
-      const int grid = (int)min((i64)kNumSMs * 32, (i64)grid_for(n * lanes, kLookupThreads));
-      k_lookup_rows<T, kBytes><<<grid, kLookupThreads, 0, stream>>>((const Unit<T, kBytes>*)from, num_rows,
-                                                                   row_stride * size / kBytes, units, ids, n, scale,
-                                                                   has_padding != 0, padding_id, lanes,
-                                                                   (Unit<T, kBytes>*)out, ctx_counters(ctx));
+      const RowShape shape = row_shape(units);
+      with_steps(shape.steps, [&](auto steps) {
+        constexpr int kRows = decltype(steps)::value == 1 ? 4 : 2;
+        const int grid = (int)min((i64)kNumSMs * 32, (i64)grid_for((n + kRows - 1) / kRows * shape.lanes, kLookupThreads));
+        launch_behind(stream, k_lookup_rows<T, kBytes, decltype(steps)::value>, grid, kLookupThreads,
+                      (const Unit<T, kBytes>*)from, num_rows, row_stride * size / kBytes, units, ids, n, scale,
+                      has_padding != 0, padding_id, shape.lanes, (Unit<T, kBytes>*)out, ctx_counters(ctx));
+      });
     });
   }
   GSB_LAUNCH_OK();

@@ -9,6 +9,7 @@
 #include <type_traits>
 
 #include "key_sort.cuh"
+#include "launch.cuh"
 #include "row_values.cuh"
 #include "scan.cuh"
 
@@ -47,48 +48,115 @@ __device__ __forceinline__ i64 place_of(const RowArgs& a, i64 slot, bool report)
   return kNowhere;
 }
 
-template <class T, int BYTES>
+// A group of lanes takes kTokens tokens at a time.
+template <class T, int BYTES, int STEPS>
 __global__ void __launch_bounds__(kRowThreads) k_spread_rows(const RowArgs a, const Unit<T, BYTES>* __restrict__ x,
                                                              Unit<T, BYTES>* __restrict__ rows) {
+  constexpr int kTokens = STEPS == 1 ? 4 : 2, N = Unit<T, BYTES>::N;
+  await_previous();
   const int lane = threadIdx.x & (a.lanes - 1);
-  const i64 groups = (i64)gridDim.x * (kRowThreads / a.lanes);
-  for (i64 t = ((i64)blockIdx.x * kRowThreads + threadIdx.x) / a.lanes; t < a.tokens; t += groups) {
-    for (i64 j = lane; j < a.units; j += a.lanes) {
-      const Unit<T, BYTES> v = load_unit_once(x + t * a.token_stride + j);
-      for (int k = 0; k < a.per_token; ++k) {
-        const i64 slot = t * a.per_token + k, p = place_of(a, slot, j == 0);
-        if (p == kNowhere) continue;
-        const float w = weight_of(a.weights, slot);
-        Unit<T, BYTES> u;
+  const i64 j = (i64)blockIdx.y * a.lanes * STEPS + lane;
+  const i64 step = (i64)gridDim.x * (kRowThreads / a.lanes) * kTokens;
+  for (i64 t = ((i64)blockIdx.x * kRowThreads + threadIdx.x) / a.lanes * kTokens; t < a.tokens; t += step) {
+    Unit<T, BYTES> v[kTokens][STEPS];
 #pragma unroll
-        for (int q = 0; q < u.N; ++q) u.v[q] = p < 0 ? from_float<T>(0.f) : from_float<T>(to_float(v.v[q]) * w);
-        store_unit(rows + (p < 0 ? ~p : p) * a.units + j, u);
+    for (int r = 0; r < kTokens; ++r)
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s)
+        if (t + r < a.tokens && j + s * a.lanes < a.units) v[r][s] = load_unit_once(x + (t + r) * a.token_stride + j + s * a.lanes);
+    for (int k = 0; k < a.per_token; ++k) {
+      i64 p[kTokens];
+      float w[kTokens];
+#pragma unroll
+      for (int r = 0; r < kTokens; ++r) {
+        const i64 slot = (t + r) * a.per_token + k;
+        p[r] = t + r < a.tokens ? place_of(a, slot, j == 0) : kNowhere;
+        w[r] = p[r] >= 0 && p[r] != kNowhere ? weight_of(a.weights, slot) : 0.f;
+      }
+#pragma unroll
+      for (int r = 0; r < kTokens; ++r) {
+        if (p[r] == kNowhere) continue;
+        Unit<T, BYTES>* to = rows + (p[r] < 0 ? ~p[r] : p[r]) * a.units + j;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+          Unit<T, BYTES> u = v[r][s];
+          if (p[r] < 0) {
+            u.clear();
+          } else if (a.weights.p) {
+            float f[N];
+            u.get(f);
+#pragma unroll
+            for (int q = 0; q < N; ++q) f[q] *= w[r];
+            u.set(f);
+          }
+          if (j + s * a.lanes < a.units) store_unit(to + s * a.lanes, u);
+        }
       }
     }
   }
 }
 
-template <class T, int BYTES>
-__global__ void __launch_bounds__(kRowThreads) k_combine_rows(const RowArgs a, const Unit<T, BYTES>* __restrict__ rows,
+// A group of lanes goes through the slots of its run of tokens, with the rows of the next kAhead slots on their way whatever
+// token they belong to.
+template <class T, int BYTES, int STEPS>
+__global__ void __launch_bounds__(kRowThreads) k_combine_rows(const RowArgs a, i64 run, const Unit<T, BYTES>* __restrict__ rows,
                                                               Unit<T, BYTES>* __restrict__ out) {
+  constexpr int N = Unit<T, BYTES>::N, kAhead = STEPS == 1 ? 4 : 2;
+  await_previous();
   const int lane = threadIdx.x & (a.lanes - 1);
-  const i64 groups = (i64)gridDim.x * (kRowThreads / a.lanes);
-  for (i64 t = ((i64)blockIdx.x * kRowThreads + threadIdx.x) / a.lanes; t < a.tokens; t += groups) {
-    for (i64 j = lane; j < a.units; j += a.lanes) {
-      float sum[Unit<T, BYTES>::N] = {};
-#pragma unroll 4
-      for (int k = 0; k < a.per_token; ++k) {
-        const i64 slot = t * a.per_token + k, p = place_of(a, slot, j == 0);
-        if (p < 0 || p == kNowhere) continue;
-        const float w = weight_of(a.weights, slot);
-        const Unit<T, BYTES> v = load_unit_once(rows + p * a.row_stride + j);
+  const i64 j = (i64)blockIdx.y * a.lanes * STEPS + lane;
+  const i64 first = ((i64)blockIdx.x * kRowThreads + threadIdx.x) / a.lanes * run;
+  if (first >= a.tokens) return;
+  const i64 begin = first * a.per_token, end = min(first + run, a.tokens) * a.per_token;
+  Unit<T, BYTES>* to = out + first * a.units + j;
+  float sum[STEPS][N] = {};
+  int left = a.per_token;  // slots of the token that are still to come
+  i64 p[kAhead];
+  float w[kAhead];
+  auto look = [&](i64 slot) {
 #pragma unroll
-        for (int q = 0; q < v.N; ++q) sum[q] += to_float(v.v[q]) * w;
+    for (int u = 0; u < kAhead; ++u) {
+      p[u] = slot + u < end ? place_of(a, slot + u, j == 0) : -1;
+      if (p[u] == kNowhere) p[u] = -1;
+      w[u] = p[u] >= 0 ? weight_of(a.weights, slot + u) : 0.f;
+    }
+  };
+  look(begin);
+  for (i64 slot = begin; slot < end; slot += kAhead) {
+    Unit<T, BYTES> v[kAhead][STEPS];
+    float factor[kAhead];
+    bool there[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      there[u] = p[u] >= 0;
+      factor[u] = w[u];
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s)
+        if (there[u] && j + s * a.lanes < a.units) v[u][s] = load_unit_once(rows + p[u] * a.row_stride + j + s * a.lanes);
+    }
+    look(slot + kAhead);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (slot + u >= end) continue;
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s)
+        if (there[u] && j + s * a.lanes < a.units) {
+          float f[N];
+          v[u][s].get(f);
+#pragma unroll
+          for (int q = 0; q < N; ++q) sum[s][q] += f[q] * factor[u];
+        }
+      if (--left > 0) continue;
+      left = a.per_token;
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+        Unit<T, BYTES> r;
+        r.set(sum[s]);
+        if (j + s * a.lanes < a.units) store_unit(to + s * a.lanes, r);
+#pragma unroll
+        for (int q = 0; q < N; ++q) sum[s][q] = 0.f;
       }
-      Unit<T, BYTES> u;
-#pragma unroll
-      for (int q = 0; q < u.N; ++q) u.v[q] = from_float<T>(sum[q]);
-      store_unit(out + t * a.units + j, u);
+      to += a.units;
     }
   }
 }
@@ -98,43 +166,70 @@ __device__ __forceinline__ void store_weight(void* p, i64 slot, float v) {
   ((W*)p)[slot] = from_float<W>(v);
 }
 
-// A warp per slot.
-template <class T, int BYTES>
+// A group of lanes takes kSlots neighbouring slots at a time.  The gradient of a token's output is read once per slot, from L1 or L2
+// after the first time.
+template <class T, int BYTES, int STEPS>
 __global__ void __launch_bounds__(kRowThreads) k_combine_grad(const RowArgs a, const Unit<T, BYTES>* __restrict__ grad,
                                                               const Unit<T, BYTES>* __restrict__ rows,
                                                               Unit<T, BYTES>* __restrict__ grad_rows, void* grad_weights) {
-  const int lane = threadIdx.x & 31;
-  const i64 warps = (i64)gridDim.x * (kRowThreads / 32), slots = a.tokens * a.per_token;
-  for (i64 slot = ((i64)blockIdx.x * kRowThreads + threadIdx.x) / 32; slot < slots; slot += warps) {
-    const i64 t = slot / a.per_token, p = place_of(a, slot, lane == 0);
-    float dot = 0.f;
-    if (p != kNowhere) {
-      const float w = weight_of(a.weights, slot);
-      for (i64 j = lane; j < a.units; j += 32) {
-        Unit<T, BYTES> u;
-        if (p >= 0) {
-          const Unit<T, BYTES> g = load_unit(grad + t * a.token_stride + j);
-          if (grad_weights) {
-            const Unit<T, BYTES> v = load_unit_once(rows + p * a.row_stride + j);
+  constexpr int N = Unit<T, BYTES>::N, kSlots = 2;
+  await_previous();
+  const int lane = threadIdx.x & (a.lanes - 1);
+  const i64 step = (i64)gridDim.x * (kRowThreads / a.lanes) * kSlots, slots = a.tokens * a.per_token;
+  // all groups of a warp take part in the sums over lanes, also those that have run out of slots
+  const i64 warp_first = ((i64)blockIdx.x * kRowThreads + (threadIdx.x & ~31)) / a.lanes * kSlots;
+  const i64 offset = (threadIdx.x & 31) / a.lanes * kSlots;
+  for (i64 base = warp_first; base < slots; base += step) {
+    const i64 slot = base + offset;
+    i64 p[kSlots], t[kSlots];
+    float w[kSlots], dot[kSlots] = {};
 #pragma unroll
-            for (int q = 0; q < v.N; ++q) dot += to_float(v.v[q]) * to_float(g.v[q]);
-          }
+    for (int r = 0; r < kSlots; ++r) {
+      p[r] = slot + r < slots ? place_of(a, slot + r, lane == 0) : kNowhere;
+      t[r] = (slot + r) / a.per_token;
+      w[r] = p[r] >= 0 && p[r] != kNowhere ? weight_of(a.weights, slot + r) : 0.f;
+    }
+    for (i64 j = lane; j < a.units; j += a.lanes * STEPS) {
+      Unit<T, BYTES> g[kSlots][STEPS], v[kSlots][STEPS];
 #pragma unroll
-          for (int q = 0; q < u.N; ++q) u.v[q] = from_float<T>(to_float(g.v[q]) * w);
-        } else {
+      for (int r = 0; r < kSlots; ++r)
 #pragma unroll
-          for (int q = 0; q < u.N; ++q) u.v[q] = from_float<T>(0.f);
+        for (int s = 0; s < STEPS; ++s) {
+          if (p[r] < 0 || p[r] == kNowhere || j + s * a.lanes >= a.units) continue;
+          if (grad_weights) v[r][s] = load_unit_once(rows + p[r] * a.row_stride + j + s * a.lanes);
+          g[r][s] = load_unit(grad + t[r] * a.token_stride + j + s * a.lanes);
         }
-        if (grad_rows) store_unit(grad_rows + (p < 0 ? ~p : p) * a.units + j, u);
-      }
+#pragma unroll
+      for (int r = 0; r < kSlots; ++r)
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+          if (p[r] == kNowhere || j + s * a.lanes >= a.units) continue;
+          Unit<T, BYTES> u;
+          u.clear();
+          if (p[r] >= 0) {
+            float f[N], h[N];
+            g[r][s].get(f);
+            if (grad_weights) {
+              v[r][s].get(h);
+#pragma unroll
+              for (int q = 0; q < N; ++q) dot[r] += f[q] * h[q];
+            }
+#pragma unroll
+            for (int q = 0; q < N; ++q) f[q] *= w[r];
+            u.set(f);
+          }
+          if (grad_rows) store_unit(grad_rows + (p[r] < 0 ? ~p[r] : p[r]) * a.units + j + s * a.lanes, u);
+        }
     }
     if (!grad_weights) continue;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-    if (lane != 0) continue;
-    if (a.weights.dtype == GSB_F32) store_weight<float>(grad_weights, slot, dot);
-    else if (a.weights.dtype == GSB_F16) store_weight<__half>(grad_weights, slot, dot);
-    else store_weight<__nv_bfloat16>(grad_weights, slot, dot);
+    for (int r = 0; r < kSlots; ++r) {
+      for (int o = a.lanes / 2; o > 0; o >>= 1) dot[r] += __shfl_xor_sync(0xffffffffu, dot[r], o);
+      if (lane != 0 || slot + r >= slots) continue;
+      if (a.weights.dtype == GSB_F32) store_weight<float>(grad_weights, slot + r, dot[r]);
+      else if (a.weights.dtype == GSB_F16) store_weight<__half>(grad_weights, slot + r, dot[r]);
+      else store_weight<__nv_bfloat16>(grad_weights, slot + r, dot[r]);
+    }
   }
 }
 
@@ -146,12 +241,6 @@ static int check_rows(i64 tokens, i64 per_token, i64 row_len, int dtype, i64 str
   GSB_REQUIRE(tokens == 0 || place, GSB_ERR_INVALID_ARGUMENT);
   GSB_REQUIRE(!weights || weights_dtype == dtype || weights_dtype == GSB_F32, GSB_ERR_INVALID_ARGUMENT);
   return GSB_OK;
-}
-
-static int group_lanes(i64 units) {
-  int lanes = 1;
-  while (lanes < 32 && lanes < units) lanes *= 2;
-  return lanes;
 }
 
 }  // namespace gsb
@@ -200,10 +289,16 @@ extern "C" int gsb_expert_spread(gsb_ctx* ctx, void* stream_, const void* x, int
     typedef decltype(value) T;
     constexpr int B = decltype(bytes)::value;
     const i64 units = row_len * size / B;
-    const RowArgs a{tokens, tokens * per_token, (int)per_token, group_lanes(units), units, x_stride * size / B, units,
+    const RowShape shape = row_shape(units);
+    const RowArgs a{tokens, tokens * per_token, (int)per_token, shape.lanes, units, x_stride * size / B, units,
                     place, Weights{weights, weights_dtype}, ctx_counters(ctx)};
-    const int grid = (int)min((i64)kNumSMs * 32, (i64)grid_for(tokens * a.lanes, kRowThreads));
-    k_spread_rows<T, B><<<grid, kRowThreads, 0, stream>>>(a, (const Unit<T, B>*)x, (Unit<T, B>*)out_rows);
+    with_steps(shape.steps, [&](auto steps) {
+      constexpr int S = decltype(steps)::value, kTokens = S == 1 ? 4 : 2;
+      const dim3 grid((unsigned)min((i64)kNumSMs * 32, (i64)grid_for((tokens + kTokens - 1) / kTokens * a.lanes, kRowThreads)),
+                      grid_for(units, shape.lanes * S));
+      launch_behind(stream, k_spread_rows<T, B, S>, grid, kRowThreads, a, (const Unit<T, B>*)x,
+                    (Unit<T, B>*)out_rows);
+    });
   });
   GSB_LAUNCH_OK();
   return GSB_OK;
@@ -226,10 +321,17 @@ extern "C" int gsb_expert_combine(gsb_ctx* ctx, void* stream_, const void* rows,
     typedef decltype(value) T;
     constexpr int B = decltype(bytes)::value;
     const i64 units = row_len * size / B;
-    const RowArgs a{tokens, num_rows, (int)per_token, group_lanes(units), units, units, rows_stride * size / B,
+    const RowShape shape = row_shape(units);
+    const RowArgs a{tokens, num_rows, (int)per_token, shape.lanes, units, units, rows_stride * size / B,
                     place, Weights{weights, weights_dtype}, ctx_counters(ctx)};
-    const int grid = (int)min((i64)kNumSMs * 32, (i64)grid_for(tokens * a.lanes, kRowThreads));
-    k_combine_rows<T, B><<<grid, kRowThreads, 0, stream>>>(a, (const Unit<T, B>*)rows, (Unit<T, B>*)out);
+    with_steps(shape.steps, [&](auto steps) {
+      constexpr int S = decltype(steps)::value;
+      // tokens per group of lanes: one while there are SMs without work
+      const i64 tiles = grid_for(units, shape.lanes * S), run = tokens * tiles * shape.lanes / 32 / (kNumSMs * 128) + 1;
+      const dim3 grid(grid_for((tokens + run - 1) / run * a.lanes, kRowThreads), (unsigned)tiles);
+      launch_behind(stream, k_combine_rows<T, B, S>, grid, kRowThreads, a, run, (const Unit<T, B>*)rows,
+                    (Unit<T, B>*)out);
+    });
   });
   GSB_LAUNCH_OK();
   return GSB_OK;
@@ -255,11 +357,14 @@ extern "C" int gsb_expert_combine_grad(gsb_ctx* ctx, void* stream_, const void* 
     typedef decltype(value) T;
     constexpr int B = decltype(bytes)::value;
     const i64 units = row_len * size / B;
-    const RowArgs a{tokens, num_rows, (int)per_token, 32, units, grad_stride * size / B, rows_stride * size / B,
+    const RowShape shape = row_shape(units);
+    const RowArgs a{tokens, num_rows, (int)per_token, shape.lanes, units, grad_stride * size / B, rows_stride * size / B,
                     place, Weights{weights, weights_dtype}, ctx_counters(ctx)};
-    const int grid = (int)min((i64)kNumSMs * 32, (i64)grid_for(tokens * per_token * 32, kRowThreads));
-    k_combine_grad<T, B><<<grid, kRowThreads, 0, stream>>>(a, (const Unit<T, B>*)grad, (const Unit<T, B>*)rows,
-                                                           (Unit<T, B>*)out_grad_rows, out_grad_weights);
+    const int grid = (int)min((i64)kNumSMs * 32, (i64)grid_for((tokens * per_token + 1) / 2 * a.lanes, kRowThreads));
+    with_steps(shape.steps, [&](auto steps) {
+      launch_behind(stream, k_combine_grad<T, B, decltype(steps)::value>, grid, kRowThreads, a, (const Unit<T, B>*)grad,
+                    (const Unit<T, B>*)rows, (Unit<T, B>*)out_grad_rows, out_grad_weights);
+    });
   });
   GSB_LAUNCH_OK();
   return GSB_OK;

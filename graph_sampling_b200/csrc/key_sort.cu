@@ -14,6 +14,7 @@
 #include "key_sort.cuh"
 
 #include "grid_sync.cuh"
+#include "launch.cuh"
 #include "scan.cuh"
 
 namespace gsb {
@@ -123,6 +124,7 @@ __global__ void __launch_bounds__(CLUSTER ? kClusterThreads : kGridThreads, 1) k
   constexpr int kDigitsPerThread = (1 << (CLUSTER ? kClusterBits : kGridBits)) / kThreads > 0 ? (1 << (CLUSTER ? kClusterBits : kGridBits)) / kThreads : 1;
   extern __shared__ __align__(128) char smem[];
   __shared__ u32 s_scan[33];
+  if (CLUSTER) await_previous();
   const SortCall& c = a.call;
   const u32 cta = blockIdx.x;
   const int bins = 1 << a.digit;
@@ -492,17 +494,19 @@ int launch(gsb_ctx* ctx, cudaStream_t stream, SortArgs& a, int grid, size_t smem
   cfg.blockDim = dim3(CLUSTER ? kClusterThreads : kGridThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr;
+  cudaLaunchAttribute attr[2];
   if (CLUSTER) {
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = kClusterCtas;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = kClusterCtas;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
   } else {
-    attr.id = cudaLaunchAttributeCooperative;
-    attr.val.cooperative = 1;
+    attr[0].id = cudaLaunchAttributeCooperative;
+    attr[0].val.cooperative = 1;
   }
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = CLUSTER ? 2 : 1;
   void* args[] = {&a};
   GSB_CUDA_OK(cudaLaunchKernelExC(&cfg, kernel, args));
   return GSB_OK;

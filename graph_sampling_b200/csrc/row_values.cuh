@@ -3,13 +3,11 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace gsb {
-
-__device__ __forceinline__ float to_float(float v) { return v; }
-__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 
 template <class T>
 __device__ __forceinline__ T from_float(float v);
@@ -20,64 +18,91 @@ __device__ __forceinline__ __half from_float<__half>(float v) { return __float2h
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// BYTES of a row as N values: one access each way.
-template <class T, int BYTES>
-struct alignas(BYTES) Unit {
-  static constexpr int N = BYTES / (int)sizeof(T);
-  T v[N];
-};
-
 template <int BYTES>
-struct Word;
+struct WordOf;
 template <>
-struct Word<16> { typedef uint4 type; };
+struct WordOf<16> { typedef uint4 type; };
 template <>
-struct Word<8> { typedef uint2 type; };
+struct WordOf<8> { typedef uint2 type; };
 template <>
-struct Word<4> { typedef unsigned int type; };
+struct WordOf<4> { typedef u32 type; };
 template <>
-struct Word<2> { typedef unsigned short type; };
+struct WordOf<2> { typedef unsigned short type; };
+
+// BYTES of a row: one access each way.  Held as the words they are; the N values exist only where they are worked with (an
+// array of 16-bit values does not stay in registers).
+template <class T, int BYTES>
+struct Unit {
+  typedef typename WordOf<BYTES>::type Word;
+  static constexpr int N = BYTES / (int)sizeof(T);
+  Word w;
+
+  __device__ __forceinline__ void get(float (&f)[N]) const {
+    if constexpr (BYTES == 2) {
+      f[0] = std::is_same<T, __half>::value ? __half2float(__ushort_as_half(w)) : __uint_as_float((u32)w << 16);
+    } else {
+      u32 q[BYTES / 4];
+      words(q);
+#pragma unroll
+      for (int i = 0; i < BYTES / 4; ++i) {
+        if constexpr (sizeof(T) == 4) {
+          f[i] = __uint_as_float(q[i]);
+        } else if constexpr (std::is_same<T, __half>::value) {
+          f[2 * i] = __half2float(__ushort_as_half((unsigned short)q[i]));
+          f[2 * i + 1] = __half2float(__ushort_as_half((unsigned short)(q[i] >> 16)));
+        } else {
+          f[2 * i] = __uint_as_float(q[i] << 16);
+          f[2 * i + 1] = __uint_as_float(q[i] & 0xffff0000u);
+        }
+      }
+    }
+  }
+  // Rounds to nearest even.
+  __device__ __forceinline__ void set(const float (&f)[N]) {
+    if constexpr (BYTES == 2) {
+      w = bits(f[0]);
+    } else {
+      u32 q[BYTES / 4];
+#pragma unroll
+      for (int i = 0; i < BYTES / 4; ++i) {
+        if constexpr (sizeof(T) == 4) q[i] = __float_as_uint(f[i]);
+        else q[i] = (u32)bits(f[2 * i]) | (u32)bits(f[2 * i + 1]) << 16;
+      }
+      if constexpr (BYTES == 4) w = q[0];
+      else if constexpr (BYTES == 8) w = make_uint2(q[0], q[1]);
+      else w = make_uint4(q[0], q[1], q[2], q[3]);
+    }
+  }
+  __device__ __forceinline__ void clear() {
+    if constexpr (BYTES <= 4) w = 0;
+    else if constexpr (BYTES == 8) w = make_uint2(0, 0);
+    else w = make_uint4(0, 0, 0, 0);
+  }
+
+ private:
+  __device__ __forceinline__ void words(u32 (&q)[BYTES / 4 > 0 ? BYTES / 4 : 1]) const {
+    if constexpr (BYTES == 4) q[0] = w;
+    else if constexpr (BYTES == 8) q[0] = w.x, q[1] = w.y;
+    else q[0] = w.x, q[1] = w.y, q[2] = w.z, q[3] = w.w;
+  }
+  static __device__ __forceinline__ unsigned short bits(float f) {
+    if constexpr (std::is_same<T, __half>::value) return __half_as_ushort(__float2half_rn(f));
+    else return __bfloat16_as_ushort(__float2bfloat16_rn(f));
+  }
+};
 
 template <class T, int BYTES>
 __device__ __forceinline__ Unit<T, BYTES> load_unit(const Unit<T, BYTES>* p) {
-  typedef typename Word<BYTES>::type W;
-  union {
-    W w;
-    Unit<T, BYTES> u;
-  } x;
-  x.w = __ldg((const W*)p);
-  return x.u;
+  return Unit<T, BYTES>{__ldg((const typename WordOf<BYTES>::type*)p)};
 }
-// What is read once and not again soon, and what is written and not read soon.
+// What is read once and not again soon.
 template <class T, int BYTES>
 __device__ __forceinline__ Unit<T, BYTES> load_unit_once(const Unit<T, BYTES>* p) {
-  typedef typename Word<BYTES>::type W;
-  union {
-    W w;
-    Unit<T, BYTES> u;
-  } x;
-  x.w = __ldcs((const W*)p);
-  return x.u;
+  return Unit<T, BYTES>{__ldcs((const typename WordOf<BYTES>::type*)p)};
 }
 template <class T, int BYTES>
 __device__ __forceinline__ void store_unit(Unit<T, BYTES>* p, const Unit<T, BYTES>& u) {
-  typedef typename Word<BYTES>::type W;
-  union {
-    W w;
-    Unit<T, BYTES> u;
-  } x;
-  x.u = u;
-  *(W*)p = x.w;
-}
-template <class T, int BYTES>
-__device__ __forceinline__ void store_unit_once(Unit<T, BYTES>* p, const Unit<T, BYTES>& u) {
-  typedef typename Word<BYTES>::type W;
-  union {
-    W w;
-    Unit<T, BYTES> u;
-  } x;
-  x.u = u;
-  __stcs((W*)p, x.w);
+  *(typename WordOf<BYTES>::type*)p = u.w;
 }
 
 inline int value_bytes(int dtype) { return dtype == GSB_F32 ? 4 : dtype == GSB_F16 || dtype == GSB_BF16 ? 2 : 0; }
@@ -87,6 +112,33 @@ inline int value_bytes(int dtype) { return dtype == GSB_F32 ? 4 : dtype == GSB_F
 inline int unit_bytes(int64_t row_bytes, uint64_t addresses) {
   const uint64_t all = (uint64_t)row_bytes | addresses;
   return all % 16 == 0 ? 16 : all % 8 == 0 ? 8 : all % 4 == 0 ? 4 : 2;
+}
+
+// How a row is taken: by `lanes` neighbouring lanes (a power of two up to 32), `steps` units (1 .. 3) of each at a time.  Of the shapes
+// that take the row at once the one that leaves the fewest lanes idle, with the most lanes; rows of more than 96 units go
+// in tiles of 32 lanes with two units each.
+struct RowShape {
+  int lanes, steps;
+};
+inline RowShape row_shape(int64_t units) {
+  RowShape best{32, 2};
+  if (units > 96) return best;
+  int idle = 1 << 20;
+  for (int lanes = 32; lanes >= 1; lanes /= 2) {
+    const int steps = (int)((units + lanes - 1) / lanes);
+    if (steps <= 3 && lanes * steps - (int)units < idle) {
+      idle = lanes * steps - (int)units;
+      best = RowShape{lanes, steps};
+    }
+  }
+  return best;
+}
+template <class F>
+void with_steps(int steps, F f) {
+  using std::integral_constant;
+  if (steps == 1) f(integral_constant<int, 1>{});
+  else if (steps == 2) f(integral_constant<int, 2>{});
+  else f(integral_constant<int, 3>{});
 }
 
 // Calls f(T, integral_constant<int, BYTES>) for the value type and the unit.
