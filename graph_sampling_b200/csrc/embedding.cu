@@ -17,14 +17,14 @@ namespace gsb {
 
 constexpr int kLookupThreads = 256;
 
-// A group of lanes takes ROWS neighbouring rows of the result at a time: all reads of a tile of them are on their way before
+// A group of lanes takes neighbouring rows of the result, a tile of their columns at a time: all its reads are on their way before
 // anything is written.
 template <class T, int BYTES, int STEPS>
 __global__ void __launch_bounds__(kLookupThreads) k_lookup_rows(const Unit<T, BYTES>* __restrict__ table, i64 num_rows,
                                                                 i64 stride, i64 units, const i64* __restrict__ ids, i64 n,
                                                                 float scale, bool has_padding, i64 padding, int lanes,
                                                                 Unit<T, BYTES>* __restrict__ out, i64* counters) {
-  constexpr int kRows = STEPS == 1 ? 4 : 2, N = Unit<T, BYTES>::N;
+  constexpr int kRows = rows_ahead<BYTES, STEPS>(), N = Unit<T, BYTES>::N;
   await_previous();
   const int lane = threadIdx.x & (lanes - 1);
   const i64 step = (i64)gridDim.x * (kLookupThreads / lanes) * kRows;
@@ -100,7 +100,7 @@ template <class T, class O, int BYTES, int STEPS>
 __global__ void __launch_bounds__(kSumThreads) k_sum_rows(const SumArgs a, const Unit<T, BYTES>* __restrict__ grad,
                                                           const u64* __restrict__ sorted, O* __restrict__ out,
                                                           float* __restrict__ part) {
-  constexpr int N = Unit<T, BYTES>::N, kAhead = STEPS >= 3 ? 2 : 4;
+  constexpr int N = Unit<T, BYTES>::N, kAhead = rows_ahead<BYTES, STEPS>();
   await_previous();
   const i64 chunk = ((i64)blockIdx.x * kSumThreads + threadIdx.x) / a.lanes;
   const i64 begin = chunk * a.chunk, end = min(begin + a.chunk, a.n);
@@ -159,14 +159,16 @@ __global__ void __launch_bounds__(kSumThreads) k_sum_rows(const SumArgs a, const
 // Where the last sum of a chunk began there and goes on: its part and those of the chunks behind.  A CTA looks at kJoinSpan
 // chunks and kJoinColumns columns.  A warp adds up to kJoinShort parts in their order, with the next ones on their way; longer
 // runs (a hub's, a frequent token's) are shared by the CTA's warps, whose sums are added in the warps' order.
-constexpr int kJoinThreads = 512, kJoinWarps = kJoinThreads / 32, kJoinSpan = 64, kJoinSteps = 4, kJoinColumns = 32 * kJoinSteps;
+constexpr int kJoinThreads = 512, kJoinWarps = kJoinThreads / 32, kJoinSpan = kJoinWarps, kJoinSteps = 4, kJoinColumns = 32 * kJoinSteps;
 constexpr int kJoinShort = 32;
 
 template <class O>
 __global__ void __launch_bounds__(kJoinThreads) k_join_rows(const SumArgs a, i64 width, i64 chunks,
                                                             const u64* __restrict__ sorted, const float* __restrict__ part,
                                                             O* __restrict__ out) {
-  __shared__ int s_found, s_long, s_chunk[kJoinSpan], s_run[kJoinSpan];
+  __shared__ int s_found, s_long, s_chunk[kJoinSpan], s_longs[kJoinSpan];
+  __shared__ u32 s_row[kJoinSpan];
+  __shared__ i64 s_run[kJoinSpan];
   __shared__ float s_sum[kJoinWarps][kJoinColumns];
   await_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -176,9 +178,13 @@ __global__ void __launch_bounds__(kJoinThreads) k_join_rows(const SumArgs a, i64
   if (threadIdx.x < kJoinSpan) {
     const i64 c = first + threadIdx.x, begin = c * a.chunk, end = begin + a.chunk;
     if (c + 1 < chunks) {
-      const u32 row = pair_key(__ldg(sorted + end - 1));
-      if (row < a.num_rows && pair_key(__ldg(sorted + end)) == row && (begin == 0 || pair_key(__ldg(sorted + begin - 1)) != row))
-        s_chunk[atomicAdd(&s_found, 1)] = threadIdx.x;
+      const u32 row = pair_key(__ldg(sorted + end - 1)), behind = pair_key(__ldg(sorted + end)),
+                before = begin > 0 ? pair_key(__ldg(sorted + begin - 1)) : kNoRow;
+      if (row < a.num_rows && behind == row && before != row) {
+        const int at = atomicAdd(&s_found, 1);
+        s_chunk[at] = threadIdx.x;
+        s_row[at] = row;
+      }
     }
   }
   __syncthreads();
@@ -194,18 +200,27 @@ __global__ void __launch_bounds__(kJoinThreads) k_join_rows(const SumArgs a, i64
   };
   for (int f = warp; f < s_found; f += kJoinWarps) {
     const i64 c = first + s_chunk[f];
-    const u32 row = pair_key(__ldg(sorted + (c + 1) * a.chunk));
+    const u32 row = s_row[f];
     i64 run = 0;  // chunks behind that go on with it
-    for (;;) {
-      const i64 next = c + 1 + run + lane;
-      const u32 with = __ballot_sync(0xffffffffu, next < chunks && pair_key(__ldg(sorted + next * a.chunk)) == row);
-      run += with == 0xffffffffu ? 32 : __ffs(~with) - 1;
-      if (with != 0xffffffffu) break;
+    for (bool more = true; more;) {
+      u32 with[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const i64 next = c + 1 + run + q * 32 + lane;
+        with[q] = next < chunks ? pair_key(__ldg(sorted + next * a.chunk)) : kNoRow;
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (!more) continue;
+        const u32 not_row = __ballot_sync(0xffffffffu, with[q] != row);
+        run += not_row ? __ffs(not_row) - 1 : 32;
+        more = not_row == 0;
+      }
     }
     if (run > kJoinShort) {
       if (lane == 0) {
-        const int at = atomicAdd(&s_long, 1);
-        s_run[at] = (int)(c - first);
+        s_longs[atomicAdd(&s_long, 1)] = f;
+        s_run[f] = run;
       }
       continue;
     }
@@ -218,15 +233,8 @@ __global__ void __launch_bounds__(kJoinThreads) k_join_rows(const SumArgs a, i64
   }
   __syncthreads();
   for (int f = 0; f < s_long; ++f) {
-    const i64 c = first + s_run[f];
-    const u32 row = pair_key(__ldg(sorted + (c + 1) * a.chunk));
-    i64 run = 0;
-    for (;;) {  // every warp for itself
-      const i64 next = c + 1 + run + lane;
-      const u32 with = __ballot_sync(0xffffffffu, next < chunks && pair_key(__ldg(sorted + next * a.chunk)) == row);
-      run += with == 0xffffffffu ? 32 : __ffs(~with) - 1;
-      if (with != 0xffffffffu) break;
-    }
+    const i64 c = first + s_chunk[s_longs[f]], run = s_run[s_longs[f]];
+    const u32 row = s_row[s_longs[f]];
 #pragma unroll
     for (int s = 0; s < kJoinSteps; ++s)
       sum[s] = warp == 0 && column + 32 * s < width ? __ldg(part + (2 * c + 1) * width + column + 32 * s) : 0.f;
@@ -249,7 +257,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_join_rows(const SumArgs a, i64
 static int sum_chunk(i64 n, i64 row_len) {
   const i64 lanes = row_len >= 128 ? 32 : row_len >= 64 ? 16 : 8, tiles = (row_len + 511) / 512;
   const i64 c = n * tiles * lanes / 32 / (kNumSMs * 128);
-  return (int)(c < 4 ? 4 : c > 128 ? 128 : c);
+  return (int)(c < 8 ? 8 : c > 128 ? 128 : c);
 }
 
 struct GradPlan {
@@ -361,9 +369,9 @@ extern "C" int gsb_embedding_lookup(gsb_ctx* ctx, void* stream_, const void* tab
       const i64 units = row_len * size / kBytes;
       const RowShape shape = row_shape(units);
       with_steps(shape.steps, [&](auto steps) {
-        constexpr int kRows = decltype(steps)::value == 1 ? 4 : 2;
+        constexpr int S = decltype(steps)::value, kRows = rows_ahead<kBytes, S>();
         const int grid = (int)min((i64)kNumSMs * 32, (i64)grid_for((n + kRows - 1) / kRows * shape.lanes, kLookupThreads));
-        launch_behind(stream, k_lookup_rows<T, kBytes, decltype(steps)::value>, grid, kLookupThreads,
+        launch_behind(stream, k_lookup_rows<T, kBytes, S>, grid, kLookupThreads,
                       (const Unit<T, kBytes>*)from, num_rows, row_stride * size / kBytes, units, ids, n, scale,
                       has_padding != 0, padding_id, shape.lanes, (Unit<T, kBytes>*)out, ctx_counters(ctx));
       });

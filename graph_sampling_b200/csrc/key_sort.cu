@@ -25,11 +25,12 @@ namespace {
 constexpr int kClusterThreads = 512, kGridThreads = 1024;
 constexpr int kRounds = 8;
 constexpr int kClusterCtas = 8;
+constexpr int kClearingClusters = 15;  // beside the one that sorts: two per GPC are resident
 constexpr int kAloneShares = 4;  // up to 2 048 positions one CTA sorts for itself, in shared memory
 constexpr int kClusterBits = 11, kGridBits = 9;
 constexpr int kMaxBins = 1 << kClusterBits;
 constexpr int kPiece = 16384;      // bytes cleared by one bulk copy
-constexpr int kPiecesAtOnce = 12;  // started by a sorting CTA between two steps: about what its SM writes meanwhile
+constexpr int kPiecesAtOnce = 32;  // at most, started by a sorting CTA between two steps: about what its SM writes meanwhile
 constexpr u32 kAllLanes = 0xffffffffu;
 
 struct SortArgs {
@@ -42,6 +43,7 @@ struct SortArgs {
   int rounds;      // of a tile: a position per thread each
   bool single;     // a stretch is one tile, which stays in registers between counting and placing
   int room;        // bytes of shared memory for a tile's items
+  int pieces;      // to clear, that a sorting CTA starts at a time
   GridSync sync;
 };
 
@@ -254,7 +256,7 @@ __global__ void __launch_bounds__(CLUSTER ? kClusterThreads : kGridThreads, 1) k
     }
     if (!alone) {
       for (int d = threadIdx.x; d < bins; d += kThreads) row[d] = s_tile[d];
-      clearing.start(kPiecesAtOnce);
+      clearing.start(a.pieces);
       barrier();
     }
     // all counts: of each digit, and of each digit in the CTAs before this one
@@ -360,7 +362,7 @@ __global__ void __launch_bounds__(CLUSTER ? kClusterThreads : kGridThreads, 1) k
       if (base + tile < hi) load_tile(base + tile, source, false);  // on its way while this tile is written
       __syncthreads();
       if (alone && !last) continue;  // the items are where the next pass takes them from
-      clearing.start(kPiecesAtOnce);
+      clearing.start(a.pieces);
       const u32 items = min(tile, hi - base);
 #pragma unroll
       for (int r = 0; r < kRounds; ++r) {
@@ -549,8 +551,11 @@ int key_sort(gsb_ctx* ctx, cudaStream_t stream, const SortCall& call, void* work
   if (pairs) *pairs = ((p.passes + (call.result == SORT_RANKS ? 1 : 0)) & 1) ? a.to : a.from;
   const i64 pieces = (i64)((call.zero_bytes + kPiece - 1) / kPiece);
   const size_t smem = p.smem(pieces > 0);
-  if (p.cluster) {  // CTAs that clear come in clusters too
-    const i64 more = min((pieces + kClusterCtas - 1) / kClusterCtas, (i64)(kNumSMs / kClusterCtas - 1)) * kClusterCtas;
+  // a sorting CTA clears as it goes: its share of the pieces over the steps of its passes
+  const i64 steps = p.passes * (1 + ((i64)p.stretch + p.threads() * p.rounds - 1) / (p.threads() * p.rounds));
+  a.pieces = (int)min((i64)kPiecesAtOnce, (pieces / kNumSMs + steps - 1) / steps);
+  if (p.cluster) {  // CTAs that clear come in clusters too, as many as the GPU holds at once
+    const i64 more = min((pieces + kClusterCtas - 1) / kClusterCtas, (i64)kClearingClusters) * kClusterCtas;
     return launch<true>(ctx, stream, a, (int)(kClusterCtas + more), smem);
   }
   GSB_CUDA_OK(cudaMemsetAsync(word, 0, sizeof(u64), stream));

@@ -105,6 +105,12 @@ __device__ __forceinline__ void store_unit(Unit<T, BYTES>* p, const Unit<T, BYTE
   *(typename WordOf<BYTES>::type*)p = u.w;
 }
 
+// What is written and not read soon.
+template <class T, int BYTES>
+__device__ __forceinline__ void store_unit_once(Unit<T, BYTES>* p, const Unit<T, BYTES>& u) {
+  __stcs((typename WordOf<BYTES>::type*)p, u.w);
+}
+
 inline int value_bytes(int dtype) { return dtype == GSB_F32 ? 4 : dtype == GSB_F16 || dtype == GSB_BF16 ? 2 : 0; }
 
 // The largest unit that divides a row and every address a row can start at: `addresses` is the bitwise or of base pointers
@@ -132,6 +138,12 @@ inline RowShape row_shape(int64_t units) {
     }
   }
   return best;
+}
+// Rows that a group of lanes has on their way at once.  More of them cost warps: with twice as many combine took 45 us for 30,
+// spread 169 for 153, sums 104 for 83.
+template <int BYTES, int STEPS>
+constexpr int rows_ahead() {
+  return STEPS == 1 ? 4 : 2;
 }
 template <class F>
 void with_steps(int steps, F f) {

@@ -606,7 +606,7 @@ GSB_API int64_t gsb_expert_order_workspace(int64_t n, int64_t num_experts);
 GSB_API int gsb_expert_order(gsb_ctx* ctx, void* stream, const int64_t* experts, int64_t n, int64_t num_experts,
                              int64_t* out_offsets, int64_t* out_source, int64_t* out_place, void* workspace,
                              int64_t workspace_bytes);
-/* Slot t * per_token + k is the k-th of token t.  Spread: out_rows[place[t, k], :] = weights[t, k] * x[t, :], zeros in the rows of
+/* Slot t * per_token + k is the k-th of token t; tokens * per_token is below 2^31.  Spread: out_rows[place[t, k], :] = weights[t, k] * x[t, :], zeros in the rows of
  * slots without an expert; tokens * per_token rows.  Combine: out[t, :] = sum over k of weights[t, k] * rows[place[t, k], :],
  * slots without an expert left out; place as gsb_expert_order gives it, num_rows at most tokens * per_token (fewer where the
  * caller leaves rows of slots without an expert away).  weights: NULL (all 1), of type dtype or GSB_F32.  The gradient of spread without weights
