@@ -1,16 +1,16 @@
 // One launch sorts: CTAs own equal stretches of the positions and go through the digits of the key, least significant first.
 // Per digit a CTA counts its stretch, all counts become visible behind a barrier, every CTA adds up for itself what lies before
-// its own (CTAs x bins words from L2, in place of a scan with a barrier of its own), and puts its positions where they
-// belong, tile by tile through shared memory so that neighbouring threads write neighbouring words.  Nothing depends on the
+// its own (in place of a scan with a barrier of its own), and puts its positions where they belong.  Nothing depends on the
 // order in which CTAs run.
 //
-// Up to 8 CTAs (32 768 positions) are one cluster: its barrier is the hardware's, needs no word in memory and no bound.  More
-// are launched cooperatively and meet at a word in the workspace (grid_sync.cuh).  Digits are as wide as keeps the number of
-// passes small: 11 bits where few CTAs have to read each other's counts, 9 where up to 148 do.
+// Up to 32 768 positions are sorted by one cluster of 8 CTAs in its shared memory (k_sort_cluster): counts are read and positions
+// written from CTA to CTA, the barrier is the hardware's, and nothing waits for global memory between the ids and the result.
+// More go through global memory (k_sort_grid), tile by tile through shared memory so that neighbouring threads write
+// neighbouring words, by CTAs that are launched cooperatively and meet at a word in the workspace (grid_sync.cuh).  Digits are
+// as wide as keeps the number of passes small: 11 bits where few CTAs have to read each other's counts, 9 where up to 148 do.
 //
-// The launch may also clear memory (the rows of a dense gradient that no position has).  The sort is bound by latency and
-// instruction issue, so bulk copies of zeros from shared memory run beside it: the sorting CTAs start some between their steps,
-// the SMs without one clear all the time.
+// The launch may also clear memory (the rows of a dense gradient that no position has), with bulk copies of zeros from shared
+// memory: SMs without a sorting CTA clear all the time, the sorting CTAs of a large sort start some between their steps.
 #include "key_sort.cuh"
 
 #include "grid_sync.cuh"
@@ -120,13 +120,241 @@ __device__ __forceinline__ u32 scan_threads(u32 v, u32* s_scan) {
   return (warp == 0 ? 0 : before) + inc - v;
 }
 
-template <bool CLUSTER>
-__global__ void __launch_bounds__(CLUSTER ? kClusterThreads : kGridThreads, 1) k_sort_keys(const SortArgs a) {
-  constexpr int kThreads = CLUSTER ? kClusterThreads : kGridThreads, kWarps = kThreads / 32;
-  constexpr int kDigitsPerThread = (1 << (CLUSTER ? kClusterBits : kGridBits)) / kThreads > 0 ? (1 << (CLUSTER ? kClusterBits : kGridBits)) / kThreads : 1;
+// Ranks of the items that a warp holds (round by round, lane by lane) among those of the same digit; `counts`, cleared, becomes the
+// warp's counts.  Lanes with the same digit are found bit by bit, by a vote each (the match instruction takes as long as
+// there are different digits).  mine: the thread's first item, of `items`.
+template <int ROUNDS>
+__device__ __forceinline__ void rank_items(const u32 (&key)[ROUNDS], u32 (&rank)[ROUNDS], unsigned short* counts, int shift,
+                                           int bits, int rounds, u32 mine, u32 items) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r) {
+    if (r >= rounds) break;
+    const bool valid = mine + r * 32 < items;
+    const u32 digit = (key[r] >> shift) & ((1u << bits) - 1u);
+    u32 peers = __ballot_sync(kAllLanes, valid);
+    for (int b = 0; b < bits; ++b) {
+      const u32 bit = (digit >> b) & 1u;
+      peers &= __ballot_sync(kAllLanes, bit) ^ (bit - 1u);
+    }
+    const u32 before = __popc(peers & ((1u << lane) - 1u));
+    const u32 found = valid ? counts[digit] : 0;
+    __syncwarp();
+    if (valid && before == 0) counts[digit] = (unsigned short)(found + __popc(peers));
+    __syncwarp();
+    rank[r] = found + before;
+  }
+}
+
+// Warps' counts become starts within the digit, two digits at a time; the digits' counts in the tile go to s_tile.
+template <int THREADS>
+__device__ __forceinline__ void warp_starts(unsigned short* s_count, u32* s_tile, int bins) {
+  for (int d = threadIdx.x; d < bins / 2; d += THREADS) {
+    u32* column = (u32*)s_count + d;
+    u32 run = 0;
+#pragma unroll
+    for (int part = 0; part < THREADS / 512; ++part) {
+      u32 k[16];
+#pragma unroll
+      for (int w = 0; w < 16; ++w) k[w] = column[(part * 16 + w) * (bins / 2)];
+#pragma unroll
+      for (int w = 0; w < 16; ++w) {
+        column[(part * 16 + w) * (bins / 2)] = run;
+        run += k[w];  // both halves: a tile has fewer than 2^16 items
+      }
+    }
+    s_tile[2 * d] = run & 0xffffu;
+    s_tile[2 * d + 1] = run >> 16;
+  }
+  __syncthreads();
+}
+
+// Addresses in another CTA's shared memory.
+__device__ __forceinline__ u32 in_cta(const void* p, u32 cta) {
+  u32 there;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"((u32)__cvta_generic_to_shared(p)), "r"(cta));
+  return there;
+}
+__device__ __forceinline__ u32 load_far(u32 address) {
+  u32 v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(address) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint4 load_far4(u32 address) {
+  uint4 v;
+  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(address) : "memory");
+  return v;
+}
+__device__ __forceinline__ void store_far(u32 address, u64 v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(address), "l"(v) : "memory");
+}
+
+__global__ void __launch_bounds__(kClusterThreads, 1) k_sort_cluster(const SortArgs a) {
+  constexpr int kThreads = kClusterThreads, kWarps = kThreads / 32, kPer = (1 << kClusterBits) / kThreads;
+  extern __shared__ __align__(128) char smem[];
+  __shared__ u32 s_scan[33], s_heads;
+  await_previous();
+  const SortCall& c = a.call;
+  const u32 cta = blockIdx.x;
+  if (cta >= (u32)a.ctas) {
+    if (cta < kClusterCtas) return;
+    Clearing clearing(c, smem, cta - kClusterCtas, gridDim.x - kClusterCtas);
+    clearing.finish();
+    return;
+  }
+  const int bins = 1 << a.digit, rounds = a.rounds;
+  u64* s_items = (u64*)smem;                                   // the stretch: written by all CTAs
+  u32* s_tile = (u32*)(s_items + rounds * kThreads);           // its counts: read by all CTAs
+  u32* s_base = s_tile + bins;                                 // where the CTA's items of a digit begin
+  unsigned short* s_count = (unsigned short*)(s_base + bins);  // kWarps x bins
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const u32 n = (u32)c.source.n, lo = cta * a.stretch, items = min(a.stretch, n - lo);
+  const u32 mine = warp * (rounds * 32) + lane;                // the thread's first item of the stretch
+  const bool alone = a.ctas == 1;
+  u32 key[kRounds], at[kRounds], rank[kRounds];
+  auto barrier = [&] {
+    if (alone) __syncthreads();
+    else asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
+  };
+  auto load = [&](bool ids) {
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+      const u32 i = mine + r * 32;
+      key[r] = kNoRow;
+      if (r >= rounds || i >= items) continue;
+      if (ids) {
+        key[r] = key_of(c.source, lo + i, true);
+        at[r] = lo + i;
+      } else {
+        const u64 pair = s_items[i];
+        key[r] = pair_key(pair);
+        at[r] = pair_at(pair);
+      }
+    }
+  };
+
+  for (int pass = 0; pass < a.passes; ++pass) {
+    const int shift = pass * a.digit;
+    load(pass == 0);
+    for (int q = threadIdx.x; q < kWarps * bins / 8; q += kThreads) ((uint4*)s_count)[q] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    rank_items<kRounds>(key, rank, s_count + warp * bins, shift, a.digit, rounds, mine, items);
+    __syncthreads();
+    warp_starts<kThreads>(s_count, s_tile, bins);
+    barrier();
+    {
+      const int per = max(1, bins / kThreads);  // digits of a thread
+      static_assert(kPer == 4, "four digits are one access");
+      u32 all[kPer] = {}, before[kPer] = {};
+#pragma unroll
+      for (int g = 0; g < kClusterCtas; ++g) {
+        if (g >= a.ctas) continue;
+        u32 v[kPer] = {};
+        if (per == kPer) {
+          const uint4 w = load_far4(in_cta(s_tile + threadIdx.x * kPer, g));
+          v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
+        } else {
+#pragma unroll
+          for (int q = 0; q < 2; ++q)
+            if (q < per && threadIdx.x * per + q < bins) v[q] = load_far(in_cta(s_tile + threadIdx.x * per + q, g));
+        }
+#pragma unroll
+        for (int q = 0; q < kPer; ++q) all[q] += v[q], before[q] += g < (int)cta ? v[q] : 0;
+      }
+      const u32 sum = all[0] + all[1] + all[2] + all[3];
+      u32 start = scan_threads<kWarps>(sum, s_scan);
+#pragma unroll
+      for (int q = 0; q < kPer; ++q) {
+        const int e = threadIdx.x * per + q;
+        if (q >= per || e >= bins) continue;
+        s_base[e] = start + before[q];
+        if (c.result == SORT_ORDER && a.passes == 1 && cta == 0 && e <= c.source.num_keys) c.offsets[e] = start;
+        start += all[q];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+      if (r >= rounds || mine + r * 32 >= items) continue;
+      const u32 digit = (key[r] >> shift) & (bins - 1);
+      const u32 spot = s_base[digit] + s_count[warp * bins + digit] + rank[r], to = spot / a.stretch;
+      const u64 pair = (u64)key[r] << 32 | at[r];
+      if (spot >= n) continue;  // never, unless memory was overwritten
+      if (alone) s_items[spot] = pair;
+      else store_far(in_cta(s_items + (spot - to * a.stretch), to), pair);
+    }
+    barrier();
+  }
+
+  if (c.result == SORT_PAIRS) {
+    for (u32 i = threadIdx.x; i < items; i += kThreads) a.to[lo + i] = s_items[i];
+    return;  // nobody reads this CTA's memory any more
+  }
+  // the key before the CTA's first
+  u32 before = kNoRow;
+  if (cta > 0) before = load_far(in_cta((const u32*)(s_items + a.stretch - 1) + 1, cta - 1));
+  if (c.result == SORT_ORDER) {
+    const i64 experts = c.source.num_keys;
+    for (u32 i = threadIdx.x; i < items; i += kThreads) {
+      const u64 pair = s_items[i];
+      const i64 j = lo + i, e = pair_key(pair);
+      c.order_source[j] = pair_at(pair);
+      c.place[pair_at(pair)] = e < experts ? j : ~j;
+      if (a.passes == 1) continue;
+      for (i64 q = j == 0 ? 0 : (i64)(i > 0 ? pair_key(s_items[i - 1]) : before) + 1; q <= e; ++q) c.offsets[q] = j;
+      if (j == n - 1)
+        for (i64 q = e + 1; q <= experts; ++q) c.offsets[q] = n;
+    }
+    barrier();  // until everybody has read the key before his first
+    return;
+  }
+  // SORT_RANKS
+  const u32 none = (u32)c.source.num_keys;
+  load(false);
+  u32 heads[kRounds], of_warp = 0;
+  {
+    u32 left_key = warp == 0 ? before : mine - lane < items ? pair_key(s_items[mine - lane - 1]) : kNoRow;
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+      u32 left = __shfl_up_sync(kAllLanes, key[r], 1);
+      if (lane == 0) left = left_key;
+      left_key = __shfl_sync(kAllLanes, key[r], 31);
+      heads[r] = __ballot_sync(kAllLanes, key[r] < none && key[r] != left);
+      of_warp += __popc(heads[r]);
+    }
+  }
+  u32 next = scan_threads<kWarps>(lane == 0 ? of_warp : 0, s_scan);
+  __syncthreads();
+  const u32 of_cta = s_scan[32];
+  if (threadIdx.x == 0) s_heads = of_cta;
+  barrier();
+  u32 others = 0;
+  if (!alone)
+#pragma unroll
+    for (int g = 0; g < kClusterCtas; ++g)
+      if (g < (int)cta) others += load_far(in_cta(&s_heads, g));
+  next = __shfl_sync(kAllLanes, next, 0) + others;
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    const u32 i = mine + r * 32, my = next + __popc(heads[r] & ((2u << lane) - 1u)) - 1u;  // of the latest head up to here
+    if (r < rounds && i < items) {
+      if (heads[r] >> lane & 1u) c.distinct[my] = key[r];
+      a.to[lo + i] = (u64)(key[r] < none ? my : kNoRow) << 32 | at[r];
+    }
+    next += __popc(heads[r]);
+  }
+  if (cta == (u32)a.ctas - 1 && threadIdx.x == 0) {
+    c.number[0] = others + of_cta;
+    mail_post(c.mail, 0, others + of_cta, c.source.counters);
+  }
+  barrier();  // until everybody has read s_heads
+}
+
+__global__ void __launch_bounds__(kGridThreads, 1) k_sort_grid(const SortArgs a) {
+  constexpr int kThreads = kGridThreads, kWarps = kThreads / 32;
+  static_assert((1 << kGridBits) <= kThreads, "a digit per thread");
   extern __shared__ __align__(128) char smem[];
   __shared__ u32 s_scan[33];
-  if (CLUSTER) await_previous();
   const SortCall& c = a.call;
   const u32 cta = blockIdx.x;
   const int bins = 1 << a.digit;
@@ -135,17 +363,14 @@ __global__ void __launch_bounds__(CLUSTER ? kClusterThreads : kGridThreads, 1) k
   u32* s_base = (u32*)((char*)s_items + a.room);               // where the next item of a digit goes
   u32* s_tile = s_base + bins;                                 // where a digit starts in the tile
   unsigned short* s_count = (unsigned short*)(s_tile + bins);  // kWarps x bins
-  if (CLUSTER && cta >= (u32)a.ctas && cta < kClusterCtas) return;
-  // the sorting CTAs of a cluster leave the clearing to the others
-  const u32 first = CLUSTER ? kClusterCtas : 0;
-  Clearing clearing(c, s_zeros, cta >= first ? cta - first : (size_t)1 << 40, gridDim.x - first);
+  Clearing clearing(c, s_zeros, cta, gridDim.x);
   if (cta >= (u32)a.ctas) {
     clearing.finish();
     return;
   }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const u32 n = (u32)c.source.n, lo = cta * a.stretch, hi = min(lo + a.stretch, n);
-  const bool single = a.single, alone = CLUSTER && a.ctas == 1;
+  const bool single = a.single;
   const int rounds = a.rounds;
   const u32 tile = (u32)rounds * kThreads, mine = warp * (rounds * 32) + lane;  // the thread's first item of a tile
   const u64* from = a.from;
@@ -164,128 +389,58 @@ __global__ void __launch_bounds__(CLUSTER ? kClusterThreads : kGridThreads, 1) k
   u32 met = 0;
   auto barrier = [&] {
     ++met;
-    if (alone) __syncthreads();
-    else if constexpr (CLUSTER) asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
-    else grid_barrier(a.sync, met, give_up, (u32)a.ctas);
+    grid_barrier(a.sync, met, give_up, (u32)a.ctas);
   };
-  // `source`: 0 the ids, 1 pairs in memory, 2 those that a CTA alone keeps
-  auto load_tile = [&](u32 base, int source, bool check) {
+  auto load_tile = [&](u32 base, bool ids, bool check) {
 #pragma unroll
     for (int r = 0; r < kRounds; ++r) {
       const u32 i = base + mine + r * 32;
       key[r] = kNoRow;
       if (r >= rounds || i >= hi) continue;
-      if (source == 0) {
+      if (ids) {
         key[r] = key_of(c.source, i, check);
         at[r] = i;
       } else {
-        const u64 pair = source == 2 ? s_items[i] : __ldcg(from + i);
+        const u64 pair = __ldcg(from + i);
         key[r] = pair_key(pair);
         at[r] = pair_at(pair);
       }
     }
   };
-  // Ranks of a tile's items among those of the same digit in their warp; s_count = the warps' counts.  Lanes with the same digit
-  // are found bit by bit, by a vote each (the match instruction takes as long as there are different digits).
+  // Ranks of a tile's items, and the warps' starts.
   auto rank_tile = [&](u32 base, int shift) {
     for (int q = threadIdx.x; q < kWarps * bins / 8; q += kThreads) ((uint4*)s_count)[q] = make_uint4(0, 0, 0, 0);
-    const u32 left = hi - base;
     __syncthreads();
-    unsigned short* counts = s_count + warp * bins;
-#pragma unroll
-    for (int r = 0; r < kRounds; ++r) {
-      if (r >= rounds) break;
-      const bool valid = mine + r * 32 < left;
-      const u32 digit = (key[r] >> shift) & (bins - 1);
-      u32 peers = __ballot_sync(kAllLanes, valid);
-      for (int b = 0; b < a.digit; ++b) {
-        const u32 bit = (digit >> b) & 1u;
-        peers &= __ballot_sync(kAllLanes, bit) ^ (bit - 1u);
-      }
-      const u32 before = __popc(peers & ((1u << lane) - 1u));
-      const u32 found = valid ? counts[digit] : 0;
-      __syncwarp();
-      if (valid && before == 0) counts[digit] = (unsigned short)(found + __popc(peers));
-      __syncwarp();
-      rank[r] = found + before;
-    }
+    rank_items<kRounds>(key, rank, s_count + warp * bins, shift, a.digit, rounds, mine, hi - base);
     __syncthreads();
-  };
-  // Warps' counts become starts within the digit, two digits at a time; the digits' counts in the tile go to s_tile.
-  auto warp_starts = [&] {
-    for (int d = threadIdx.x; d < bins / 2; d += kThreads) {
-      u32* column = (u32*)s_count + d;
-      u32 run = 0;
-#pragma unroll
-      for (int part = 0; part < kWarps / 16; ++part) {
-        u32 k[16];
-#pragma unroll
-        for (int w = 0; w < 16; ++w) k[w] = column[(part * 16 + w) * (bins / 2)];
-#pragma unroll
-        for (int w = 0; w < 16; ++w) {
-          column[(part * 16 + w) * (bins / 2)] = run;
-          run += k[w];  // both halves: a tile has fewer than 2^16 items
-        }
-      }
-      s_tile[2 * d] = run & 0xffffu;
-      s_tile[2 * d + 1] = run >> 16;
-    }
-    __syncthreads();
+    warp_starts<kThreads>(s_count, s_tile, bins);
   };
 
   for (int pass = 0; pass < a.passes; ++pass) {
     const int shift = pass * a.digit;
-    const bool last = pass == a.passes - 1;
-    const int source = pass == 0 ? 0 : alone ? 2 : 1;
+    const bool ids = pass == 0, last = pass == a.passes - 1;
     // counts of the stretch
     u32* row = a.counts + (size_t)cta * bins;
     if (single) {
-      load_tile(lo, source, true);
+      load_tile(lo, ids, true);
       rank_tile(lo, shift);
-      warp_starts();
     } else {
       for (int d = threadIdx.x; d < bins; d += kThreads) s_tile[d] = 0;
       __syncthreads();
       for (u32 base = lo; base < hi; base += tile) {
-        load_tile(base, source, true);
+        load_tile(base, ids, true);
 #pragma unroll
         for (int r = 0; r < kRounds; ++r)
           if (base + mine + r * 32 < hi) atomicAdd(&s_tile[(key[r] >> shift) & (bins - 1)], 1u);
       }
       __syncthreads();
     }
-    if (!alone) {
-      for (int d = threadIdx.x; d < bins; d += kThreads) row[d] = s_tile[d];
-      clearing.start(a.pieces);
-      barrier();
-    }
-    // all counts: of each digit, and of each digit in the CTAs before this one
-    const int per = max(1, bins / kThreads);  // digits of a thread
-    u32 all[kDigitsPerThread] = {}, before[kDigitsPerThread] = {};
-    if (CLUSTER && !alone) {
-      if (per == 4) {
-#pragma unroll
-        for (int g = 0; g < kClusterCtas; ++g) {
-          if (g >= a.ctas) continue;
-          const uint4 v = __ldcg((const uint4*)(a.counts + (size_t)g * bins) + threadIdx.x);
-          const u32 w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-          for (int q = 0; q < kDigitsPerThread; ++q) all[q] += w[q], before[q] += g < (int)cta ? w[q] : 0;
-        }
-      } else {
-#pragma unroll
-        for (int g = 0; g < kClusterCtas; ++g) {
-#pragma unroll
-          for (int q = 0; q < kDigitsPerThread; ++q) {
-            const int e = threadIdx.x * per + q;
-            if (g >= a.ctas || q >= per || e >= bins) continue;
-            const u32 w = __ldcg(a.counts + (size_t)g * bins + e);
-            all[q] += w, before[q] += g < (int)cta ? w : 0;
-          }
-        }
-      }
-    }
-    if (!CLUSTER) {  // groups of threads share the rows
+    if ((int)threadIdx.x < bins) row[threadIdx.x] = s_tile[threadIdx.x];
+    clearing.start(a.pieces);
+    barrier();
+    // all counts: of each digit, and of each digit in the CTAs before this one; groups of threads share the rows
+    const int e = threadIdx.x;  // the thread's digit
+    {
       const int per_row = bins / 4, groups = min(min(kThreads / per_row, a.ctas), 16), group = threadIdx.x / per_row;
       const int d = (threadIdx.x % per_row) * 4;
       u32* s_total = (u32*)s_items;  // groups x bins
@@ -302,49 +457,27 @@ __global__ void __launch_bounds__(CLUSTER ? kClusterThreads : kGridThreads, 1) k
         *(uint4*)(s_before + group * bins + d) = less;
       }
       __syncthreads();
-      if ((int)threadIdx.x < bins)
-        for (int g = 0; g < groups; ++g) all[0] += s_total[g * bins + threadIdx.x], before[0] += s_before[g * bins + threadIdx.x];
-    }
-    if (!alone) {
-      u32 sum = 0;
-#pragma unroll
-      for (int q = 0; q < kDigitsPerThread; ++q) sum += all[q];
-      u32 start = scan_threads<kWarps>(sum, s_scan);
-#pragma unroll
-      for (int q = 0; q < kDigitsPerThread; ++q) {
-        const int e = threadIdx.x * per + q;
-        if (q >= per || e >= bins) continue;
-        s_base[e] = start + before[q];
+      u32 all = 0, before = 0;
+      if (e < bins)
+        for (int g = 0; g < groups; ++g) all += s_total[g * bins + e], before += s_before[g * bins + e];
+      const u32 start = scan_threads<kWarps>(all, s_scan);
+      if (e < bins) {
+        s_base[e] = start + before;
         if (c.result == SORT_ORDER && a.passes == 1 && cta == 0 && e <= c.source.num_keys) c.offsets[e] = start;
-        start += all[q];
       }
       __syncthreads();
     }
     // to their places
-    if (!single) load_tile(lo, source, false);
+    if (!single) load_tile(lo, ids, false);
     for (u32 base = lo; base < hi; base += tile) {
       if (!single) {
         rank_tile(base, shift);
-        warp_starts();
       }
       // s_tile: counts -> starts in the tile; s_base: where the tile's first item of a digit goes, less its place in the tile
-      u32 count[kDigitsPerThread], sum = 0;
-#pragma unroll
-      for (int q = 0; q < kDigitsPerThread; ++q) {
-        const int e = threadIdx.x * per + q;
-        count[q] = q < per && e < bins ? s_tile[e] : 0;
-        sum += count[q];
-      }
-      u32 start = scan_threads<kWarps>(sum, s_scan);
-#pragma unroll
-      for (int q = 0; q < kDigitsPerThread; ++q) {
-        const int e = threadIdx.x * per + q;
-        if (q >= per || e >= bins) continue;
+      const u32 count = e < bins ? s_tile[e] : 0, start = scan_threads<kWarps>(count, s_scan);
+      if (e < bins) {
         s_tile[e] = start;
-        if (alone) s_base[e] = 0;
-        else s_base[e] -= start;
-        if (alone && c.result == SORT_ORDER && last && e <= c.source.num_keys && a.passes == 1) c.offsets[e] = start;
-        start += count[q];
+        s_base[e] -= start;
       }
       __syncthreads();
 #pragma unroll
@@ -359,9 +492,8 @@ __global__ void __launch_bounds__(CLUSTER ? kClusterThreads : kGridThreads, 1) k
           c.place[at[r]] = key[r] < (u32)c.source.num_keys ? (i64)row_of : ~(i64)row_of;
         }
       }
-      if (base + tile < hi) load_tile(base + tile, source, false);  // on its way while this tile is written
+      if (base + tile < hi) load_tile(base + tile, ids, false);  // on its way while this tile is written
       __syncthreads();
-      if (alone && !last) continue;  // the items are where the next pass takes them from
       clearing.start(a.pieces);
       const u32 items = min(tile, hi - base);
 #pragma unroll
@@ -375,16 +507,12 @@ __global__ void __launch_bounds__(CLUSTER ? kClusterThreads : kGridThreads, 1) k
         if (c.result != SORT_ORDER || a.passes > 1) to[spot] = item;
       }
       __syncthreads();
-#pragma unroll
-      for (int q = 0; q < kDigitsPerThread; ++q) {
-        const int e = threadIdx.x * per + q;
-        if (q < per && e < bins) s_base[e] += s_tile[e] + count[q];
-      }
+      if (e < bins) s_base[e] += start + count;
     }
     u64* free = const_cast<u64*>(from);
     from = to;
     to = free;
-    if ((!last && !alone) || (last && (c.result == SORT_RANKS || (c.result == SORT_ORDER && a.passes > 1)))) barrier();
+    if (!last || c.result == SORT_RANKS || (c.result == SORT_ORDER && a.passes > 1)) barrier();
   }
 
   if (c.result == SORT_ORDER && a.passes > 1) {
@@ -401,7 +529,7 @@ __global__ void __launch_bounds__(CLUSTER ? kClusterThreads : kGridThreads, 1) k
     // the tile's items, and which of them are the first of their key; returns how many of the warp's are
     u32 (&heads)[kRounds] = rank;
     auto find_heads = [&](u32 base) {
-      load_tile(base, 1, false);
+      load_tile(base, false, false);
       const u32 begin = base + warp * (rounds * 32);
       u32 before = begin > 0 && begin < hi ? pair_key(__ldcg(from + begin - 1)) : kNoRow, all = 0;
 #pragma unroll
@@ -448,6 +576,10 @@ __global__ void __launch_bounds__(CLUSTER ? kClusterThreads : kGridThreads, 1) k
   clearing.finish();
 }
 
+// Of both kernels: a full tile, the widest digits, and zeros to copy.
+constexpr int kMostShared = kPiece + kGridThreads * kRounds * 8 + kMaxBins * (8 + kClusterThreads / 32 * 2);
+static_assert(kMostShared <= 227 * 1024, "");
+
 struct Plan {
   bool cluster, single;
   int ctas, passes, digit, rounds;
@@ -458,7 +590,8 @@ struct Plan {
     return max(rounds * threads() * 8, cluster ? 0 : 2 * 4 * min(16 * bins(), 4 * threads()));
   }
   size_t smem(bool clears) const {
-    return (size_t)((clears ? kPiece : 0) + room() + bins() * 8 + threads() / 32 * bins() * 2);
+    const int sort = room() + bins() * 8 + threads() / 32 * bins() * 2;
+    return (size_t)(cluster ? max(sort, clears ? kPiece : 0) : sort + (clears ? kPiece : 0));
   }
 };
 
@@ -481,23 +614,21 @@ Plan plan_of(i64 n, i64 num_keys) {
   return p;
 }
 
-template <bool CLUSTER>
-int launch(gsb_ctx* ctx, cudaStream_t stream, SortArgs& a, int grid, size_t smem) {
-  const void* kernel = (const void*)k_sort_keys<CLUSTER>;
-  static bool known[64] = {};
+int launch(gsb_ctx* ctx, cudaStream_t stream, SortArgs& a, bool cluster, int grid, size_t smem) {
+  const void* kernel = cluster ? (const void*)k_sort_cluster : (const void*)k_sort_grid;
+  static bool known[2][64] = {};
   const int device = ctx_device(ctx);
-  if (device < 0 || device >= 64 || !known[device]) {
-    const size_t most = kPiece + (size_t)kGridThreads * kRounds * 8 + (size_t)kMaxBins * (8 + kClusterThreads / 32 * 2);
-    GSB_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
-    if (device >= 0 && device < 64) known[device] = true;
+  if (device < 0 || device >= 64 || !known[cluster][device]) {
+    GSB_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared));
+    if (device >= 0 && device < 64) known[cluster][device] = true;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3(CLUSTER ? kClusterThreads : kGridThreads);
+  cfg.blockDim = dim3(cluster ? kClusterThreads : kGridThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
-  if (CLUSTER) {
+  if (cluster) {
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = kClusterCtas;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
@@ -508,7 +639,7 @@ int launch(gsb_ctx* ctx, cudaStream_t stream, SortArgs& a, int grid, size_t smem
     attr[0].val.cooperative = 1;
   }
   cfg.attrs = attr;
-  cfg.numAttrs = CLUSTER ? 2 : 1;
+  cfg.numAttrs = cluster ? 2 : 1;
   void* args[] = {&a};
   GSB_CUDA_OK(cudaLaunchKernelExC(&cfg, kernel, args));
   return GSB_OK;
@@ -548,7 +679,7 @@ int key_sort(gsb_ctx* ctx, cudaStream_t stream, const SortCall& call, void* work
   if (call.result == SORT_RANKS) barriers += 2;
   if (call.result == SORT_ORDER && p.passes > 1) barriers += 1;
   a.sync = GridSync{word, 0, (u32)barriers, call.source.counters, (int)ctx_option(ctx, GSB_OPT_MAX_POLLS)};
-  if (pairs) *pairs = ((p.passes + (call.result == SORT_RANKS ? 1 : 0)) & 1) ? a.to : a.from;
+  if (pairs) *pairs = p.cluster || ((p.passes + (call.result == SORT_RANKS ? 1 : 0)) & 1) ? a.to : a.from;
   const i64 pieces = (i64)((call.zero_bytes + kPiece - 1) / kPiece);
   const size_t smem = p.smem(pieces > 0);
   // a sorting CTA clears as it goes: its share of the pieces over the steps of its passes
@@ -556,10 +687,10 @@ int key_sort(gsb_ctx* ctx, cudaStream_t stream, const SortCall& call, void* work
   a.pieces = (int)min((i64)kPiecesAtOnce, (pieces / kNumSMs + steps - 1) / steps);
   if (p.cluster) {  // CTAs that clear come in clusters too, as many as the GPU holds at once
     const i64 more = min((pieces + kClusterCtas - 1) / kClusterCtas, (i64)kClearingClusters) * kClusterCtas;
-    return launch<true>(ctx, stream, a, (int)(kClusterCtas + more), smem);
+    return launch(ctx, stream, a, true, (int)(kClusterCtas + more), smem);
   }
   GSB_CUDA_OK(cudaMemsetAsync(word, 0, sizeof(u64), stream));
-  return launch<false>(ctx, stream, a, (int)(p.ctas + min(pieces, (i64)(kNumSMs - p.ctas))), smem);
+  return launch(ctx, stream, a, false, (int)(p.ctas + min(pieces, (i64)(kNumSMs - p.ctas))), smem);
 }
 
 }  // namespace gsb
