@@ -52,7 +52,7 @@ __device__ __forceinline__ i64 place_of(const RowArgs& a, i64 slot, bool report)
 template <class T, int BYTES, int STEPS>
 __global__ void __launch_bounds__(kRowThreads) k_spread_rows(const RowArgs a, const Unit<T, BYTES>* __restrict__ x,
                                                              Unit<T, BYTES>* __restrict__ rows) {
-  constexpr int kTokens = rows_ahead<BYTES, STEPS>(), N = Unit<T, BYTES>::N;
+  constexpr int kTokens = rows_ahead(STEPS), N = Unit<T, BYTES>::N;
   await_previous();
   const int lane = threadIdx.x & (a.lanes - 1);
   const i64 j = (i64)blockIdx.y * a.lanes * STEPS + lane;
@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(kRowThreads) k_spread_rows(const RowArgs a, co
 template <class T, int BYTES, int STEPS>
 __global__ void __launch_bounds__(kRowThreads) k_combine_rows(const RowArgs a, i64 run, const Unit<T, BYTES>* __restrict__ rows,
                                                               Unit<T, BYTES>* __restrict__ out) {
-  constexpr int N = Unit<T, BYTES>::N, kAhead = rows_ahead<BYTES, STEPS>();
+  constexpr int N = Unit<T, BYTES>::N, kAhead = rows_ahead(STEPS);
   await_previous();
   const int lane = threadIdx.x & (a.lanes - 1);
   const i64 j = (i64)blockIdx.y * a.lanes * STEPS + lane;
@@ -166,58 +166,74 @@ __device__ __forceinline__ void store_weight(void* p, i64 slot, float v) {
   ((W*)p)[slot] = from_float<W>(v);
 }
 
-// A group of lanes takes a slot at a time.  The gradient of a token's output is read once per slot, from L1 or L2 after the first
-// time; two slots at a time cost warps and took 62 us for 58.
+// A group of lanes takes neighbouring slots at a time: one of rows in units of 16 bytes (two cost warps: 62 us for 58), two of
+// narrower ones.  The gradient of a token's output is read once per slot, from L1 or L2 after the first time.
+template <class T, int BYTES>
+constexpr int grad_slots() { return BYTES == 16 ? 1 : 2; }
+
 template <class T, int BYTES, int STEPS>
 __global__ void __launch_bounds__(kRowThreads) k_combine_grad(const RowArgs a, const Unit<T, BYTES>* __restrict__ grad,
                                                               const Unit<T, BYTES>* __restrict__ rows,
                                                               Unit<T, BYTES>* __restrict__ grad_rows, void* grad_weights) {
-  constexpr int N = Unit<T, BYTES>::N;
+  constexpr int N = Unit<T, BYTES>::N, kSlots = grad_slots<T, BYTES>();
   await_previous();
   const int lane = threadIdx.x & (a.lanes - 1);
-  const i64 step = (i64)gridDim.x * (kRowThreads / a.lanes), slots = a.tokens * a.per_token;
+  const i64 step = (i64)gridDim.x * (kRowThreads / a.lanes) * kSlots, slots = a.tokens * a.per_token;
   // all groups of a warp take part in the sums over lanes, also those that have run out of slots
-  const i64 warp_first = ((i64)blockIdx.x * kRowThreads + (threadIdx.x & ~31)) / a.lanes;
+  const i64 warp_first = ((i64)blockIdx.x * kRowThreads + (threadIdx.x & ~31)) / a.lanes * kSlots;
   for (i64 base = warp_first; base < slots; base += step) {
-    const i64 slot = base + (threadIdx.x & 31) / a.lanes;
-    const i64 p = slot < slots ? place_of(a, slot, lane == 0) : kNowhere, t = (u32)slot / (u32)a.per_token;
-    const bool there = p >= 0 && p != kNowhere;
-    const float w = there ? weight_of(a.weights, slot) : 0.f;
-    float dot = 0.f;
+    const i64 slot = base + (threadIdx.x & 31) / a.lanes * kSlots;
+    i64 p[kSlots], t[kSlots];
+    bool there[kSlots];
+    float w[kSlots], dot[kSlots] = {};
+#pragma unroll
+    for (int r = 0; r < kSlots; ++r) {
+      p[r] = slot + r < slots ? place_of(a, slot + r, lane == 0) : kNowhere;
+      t[r] = (u32)(slot + r) / (u32)a.per_token;
+      there[r] = p[r] >= 0 && p[r] != kNowhere;
+      w[r] = there[r] ? weight_of(a.weights, slot + r) : 0.f;
+    }
     for (i64 j = lane; j < a.units; j += a.lanes * STEPS) {
-      Unit<T, BYTES> g[STEPS], v[STEPS];
+      Unit<T, BYTES> g[kSlots][STEPS], v[kSlots][STEPS];
 #pragma unroll
-      for (int s = 0; s < STEPS; ++s) {
-        if (!there || j + s * a.lanes >= a.units) continue;
-        if (grad_weights) v[s] = load_unit_once(rows + p * a.row_stride + j + s * a.lanes);
-        g[s] = load_unit(grad + t * a.token_stride + j + s * a.lanes);
-      }
+      for (int r = 0; r < kSlots; ++r)
 #pragma unroll
-      for (int s = 0; s < STEPS; ++s) {
-        if (p == kNowhere || j + s * a.lanes >= a.units) continue;
-        Unit<T, BYTES> u;
-        u.clear();
-        if (there) {
-          float f[N], h[N];
-          g[s].get(f);
-          if (grad_weights) {
-            v[s].get(h);
-#pragma unroll
-            for (int q = 0; q < N; ++q) dot += f[q] * h[q];
-          }
-#pragma unroll
-          for (int q = 0; q < N; ++q) f[q] *= w;
-          u.set(f);
+        for (int s = 0; s < STEPS; ++s) {
+          if (!there[r] || j + s * a.lanes >= a.units) continue;
+          if (grad_weights) v[r][s] = load_unit_once(rows + p[r] * a.row_stride + j + s * a.lanes);
+          g[r][s] = load_unit(grad + t[r] * a.token_stride + j + s * a.lanes);
         }
-        if (grad_rows) store_unit_once(grad_rows + (p < 0 ? ~p : p) * a.units + j + s * a.lanes, u);
-      }
+#pragma unroll
+      for (int r = 0; r < kSlots; ++r)
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+          if (p[r] == kNowhere || j + s * a.lanes >= a.units) continue;
+          Unit<T, BYTES> u;
+          u.clear();
+          if (there[r]) {
+            float f[N], h[N];
+            g[r][s].get(f);
+            if (grad_weights) {
+              v[r][s].get(h);
+#pragma unroll
+              for (int q = 0; q < N; ++q) dot[r] += f[q] * h[q];
+            }
+#pragma unroll
+            for (int q = 0; q < N; ++q) f[q] *= w[r];
+            u.set(f);
+          }
+          if (grad_rows) store_unit_once(grad_rows + (p[r] < 0 ? ~p[r] : p[r]) * a.units + j + s * a.lanes, u);
+        }
     }
     if (!grad_weights) continue;
-    for (int o = a.lanes / 2; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-    if (lane != 0 || slot >= slots) continue;
-    if (a.weights.dtype == GSB_F32) store_weight<float>(grad_weights, slot, dot);
-    else if (a.weights.dtype == GSB_F16) store_weight<__half>(grad_weights, slot, dot);
-    else store_weight<__nv_bfloat16>(grad_weights, slot, dot);
+#pragma unroll
+    for (int r = 0; r < kSlots; ++r) {
+      for (int o = a.lanes / 2; o > 0; o >>= 1) dot[r] += __shfl_xor_sync(0xffffffffu, dot[r], o);
+      if (lane != 0 || slot + r >= slots) continue;
+      if (a.weights.dtype == GSB_F32) store_weight<float>(grad_weights, slot + r, dot[r]);
+      else if (a.weights.dtype == GSB_F16) store_weight<__half>(grad_weights, slot + r, dot[r]);
+      else store_weight<__nv_bfloat16>(grad_weights, slot + r, dot[r]);
+    }
   }
 }
 
@@ -278,11 +294,11 @@ extern "C" int gsb_expert_spread(gsb_ctx* ctx, void* stream_, const void* x, int
     typedef decltype(value) T;
     constexpr int B = decltype(bytes)::value;
     const i64 units = row_len * size / B;
-    const RowShape shape = row_shape(units);
+    const RowShape shape = row_shape(units, copy_steps(B));
     const RowArgs a{tokens, tokens * per_token, (int)per_token, shape.lanes, units, x_stride * size / B, units,
                     place, Weights{weights, weights_dtype}, ctx_counters(ctx)};
     with_steps(shape.steps, [&](auto steps) {
-      constexpr int S = decltype(steps)::value, kTokens = rows_ahead<B, S>();
+      constexpr int S = decltype(steps)::value, kTokens = rows_ahead(S);
       const dim3 grid((unsigned)min((i64)kNumSMs * 32, (i64)grid_for((tokens + kTokens - 1) / kTokens * a.lanes, kRowThreads)),
                       grid_for(units, shape.lanes * S));
       launch_behind(stream, k_spread_rows<T, B, S>, grid, kRowThreads, a, (const Unit<T, B>*)x,
@@ -310,7 +326,7 @@ extern "C" int gsb_expert_combine(gsb_ctx* ctx, void* stream_, const void* rows,
     typedef decltype(value) T;
     constexpr int B = decltype(bytes)::value;
     const i64 units = row_len * size / B;
-    const RowShape shape = row_shape(units);
+    const RowShape shape = row_shape(units, copy_steps(B));
     const RowArgs a{tokens, num_rows, (int)per_token, shape.lanes, units, units, rows_stride * size / B,
                     place, Weights{weights, weights_dtype}, ctx_counters(ctx)};
     with_steps(shape.steps, [&](auto steps) {
@@ -346,12 +362,12 @@ extern "C" int gsb_expert_combine_grad(gsb_ctx* ctx, void* stream_, const void* 
     typedef decltype(value) T;
     constexpr int B = decltype(bytes)::value;
     const i64 units = row_len * size / B;
-    const RowShape shape = row_shape(units);
+    const RowShape shape = row_shape(units, copy_steps(B));
     const RowArgs a{tokens, num_rows, (int)per_token, shape.lanes, units, grad_stride * size / B, rows_stride * size / B,
                     place, Weights{weights, weights_dtype}, ctx_counters(ctx)};
     with_steps(shape.steps, [&](auto steps) {
-      constexpr int S = decltype(steps)::value;
-      const int grid = (int)min((i64)kNumSMs * 32, (i64)grid_for(tokens * per_token * a.lanes, kRowThreads));
+      constexpr int S = decltype(steps)::value, kSlots = grad_slots<T, B>();
+      const int grid = (int)min((i64)kNumSMs * 32, (i64)grid_for((tokens * per_token + kSlots - 1) / kSlots * a.lanes, kRowThreads));
       launch_behind(stream, k_combine_grad<T, B, S>, grid, kRowThreads, a, (const Unit<T, B>*)grad,
                     (const Unit<T, B>*)rows, (Unit<T, B>*)out_grad_rows, out_grad_weights);
     });

@@ -350,11 +350,18 @@ __global__ void __launch_bounds__(kClusterThreads, 1) k_sort_cluster(const SortA
   barrier();  // until everybody has read s_heads
 }
 
+// The word that the sorting CTAs meet at.
+__global__ void k_clear_word(u64* word) {
+  await_previous();
+  *word = 0;
+}
+
 __global__ void __launch_bounds__(kGridThreads, 1) k_sort_grid(const SortArgs a) {
   constexpr int kThreads = kGridThreads, kWarps = kThreads / 32;
   static_assert((1 << kGridBits) <= kThreads, "a digit per thread");
   extern __shared__ __align__(128) char smem[];
   __shared__ u32 s_scan[33];
+  await_previous();
   const SortCall& c = a.call;
   const u32 cta = blockIdx.x;
   const int bins = 1 << a.digit;
@@ -431,7 +438,7 @@ __global__ void __launch_bounds__(kGridThreads, 1) k_sort_grid(const SortArgs a)
         load_tile(base, ids, true);
 #pragma unroll
         for (int r = 0; r < kRounds; ++r)
-          if (base + mine + r * 32 < hi) atomicAdd(&s_tile[(key[r] >> shift) & (bins - 1)], 1u);
+          if (r < rounds && base + mine + r * 32 < hi) atomicAdd(&s_tile[(key[r] >> shift) & (bins - 1)], 1u);
       }
       __syncthreads();
     }
@@ -447,11 +454,19 @@ __global__ void __launch_bounds__(kGridThreads, 1) k_sort_grid(const SortArgs a)
       u32* s_before = s_total + groups * bins;
       if (group < groups) {
         uint4 total = make_uint4(0, 0, 0, 0), less = total;
-#pragma unroll 8
-        for (int g = group; g < a.ctas; g += groups) {
-          const uint4 v = __ldcg((const uint4*)(a.counts + (size_t)g * bins + d));
-          total.x += v.x, total.y += v.y, total.z += v.z, total.w += v.w;
-          if (g < (int)cta) less.x += v.x, less.y += v.y, less.z += v.z, less.w += v.w;
+        constexpr int kBatch = 6;  // rows on their way
+        for (int g0 = group; g0 < a.ctas; g0 += kBatch * groups) {
+          uint4 v[kBatch];
+#pragma unroll
+          for (int q = 0; q < kBatch; ++q) {
+            const int g = g0 + q * groups;
+            v[q] = g < a.ctas ? __ldcg((const uint4*)(a.counts + (size_t)g * bins + d)) : make_uint4(0, 0, 0, 0);
+          }
+#pragma unroll
+          for (int q = 0; q < kBatch; ++q) {
+            total.x += v[q].x, total.y += v[q].y, total.z += v[q].z, total.w += v[q].w;
+            if (g0 + q * groups < (int)cta) less.x += v[q].x, less.y += v[q].y, less.z += v[q].z, less.w += v[q].w;
+          }
         }
         *(uint4*)(s_total + group * bins + d) = total;
         *(uint4*)(s_before + group * bins + d) = less;
@@ -604,7 +619,8 @@ Plan plan_of(i64 n, i64 num_keys) {
   p.stretch = (u32)(per * threads);
   p.ctas = (int)((shares + per - 1) / per);
   p.single = per <= kRounds;
-  p.rounds = p.single ? (int)per : kRounds;
+  const i64 tiles = (per + kRounds - 1) / kRounds;  // of a stretch, about equal
+  p.rounds = (int)((per + tiles - 1) / tiles);
   int bits = 1;  // of the largest key, num_keys itself
   while (bits < 32 && (num_keys >> bits) != 0) ++bits;
   const int most = p.cluster ? kClusterBits : kGridBits;
@@ -632,14 +648,14 @@ int launch(gsb_ctx* ctx, cudaStream_t stream, SortArgs& a, bool cluster, int gri
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = kClusterCtas;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
   } else {
     attr[0].id = cudaLaunchAttributeCooperative;
     attr[0].val.cooperative = 1;
   }
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = cluster ? 2 : 1;
+  cfg.numAttrs = 2;
   void* args[] = {&a};
   GSB_CUDA_OK(cudaLaunchKernelExC(&cfg, kernel, args));
   return GSB_OK;
@@ -689,7 +705,8 @@ int key_sort(gsb_ctx* ctx, cudaStream_t stream, const SortCall& call, void* work
     const i64 more = min((pieces + kClusterCtas - 1) / kClusterCtas, (i64)kClearingClusters) * kClusterCtas;
     return launch(ctx, stream, a, true, (int)(kClusterCtas + more), smem);
   }
-  GSB_CUDA_OK(cudaMemsetAsync(word, 0, sizeof(u64), stream));
+  GSB_CUDA_OK(launch_behind(stream, k_clear_word, dim3(1), 1, word));
+  ctx_count_launches(ctx, 1);
   return launch(ctx, stream, a, false, (int)(p.ctas + min(pieces, (i64)(kNumSMs - p.ctas))), smem);
 }
 

@@ -120,37 +120,43 @@ inline int unit_bytes(int64_t row_bytes, uint64_t addresses) {
   return all % 16 == 0 ? 16 : all % 8 == 0 ? 8 : all % 4 == 0 ? 4 : 2;
 }
 
-// How a row is taken: by `lanes` neighbouring lanes (a power of two up to 32), `steps` units (1 .. 3) of each at a time.  Of the shapes
-// that take the row at once the one that leaves the fewest lanes idle, with the most lanes; rows of more than 96 units go
-// in tiles of 32 lanes with two units each.
+// How a row is taken: by `lanes` neighbouring lanes (a power of two up to 32), `steps` units (1 .. 4) of each at a time.  Of the shapes
+// that take the row at once the one that leaves the fewest lanes idle; among equals the one whose steps are nearest to
+// `wanted`.  Rows of more than 96 units go in tiles of 32 lanes with two units each.
 struct RowShape {
   int lanes, steps;
 };
-inline RowShape row_shape(int64_t units) {
+inline RowShape row_shape(int64_t units, int wanted) {
   RowShape best{32, 2};
   if (units > 96) return best;
-  int idle = 1 << 20;
+  int idle = 1 << 20, away = 0;
   for (int lanes = 32; lanes >= 1; lanes /= 2) {
-    const int steps = (int)((units + lanes - 1) / lanes);
-    if (steps <= 3 && lanes * steps - (int)units < idle) {
-      idle = lanes * steps - (int)units;
+    const int steps = (int)((units + lanes - 1) / lanes), rest = lanes * steps - (int)units;
+    const int off = steps > wanted ? steps - wanted : wanted - steps;
+    if (steps <= 4 && (rest < idle || (rest == idle && off < away))) {
+      idle = rest;
+      away = off;
       best = RowShape{lanes, steps};
     }
   }
   return best;
 }
+// What copies and combines rows does well with two units of 16 bytes a lane, or four smaller ones (rows of 256 bytes spread in 30
+// us, with one unit a lane in 49; rows of 200 bytes combined in 32 and 43); what sums them, which has more to do per row and
+// lane, with one of 16 bytes (rows of 256 bytes 83 us, with two 98).
+inline int copy_steps(int unit) { return unit == 16 ? 2 : 4; }
+inline int sum_steps(int unit) { return unit >= 16 ? 1 : unit == 8 ? 2 : 4; }
 // Rows that a group of lanes has on their way at once.  More of them cost warps: with twice as many combine took 45 us for 30,
 // spread 169 for 153, sums 104 for 83.
-template <int BYTES, int STEPS>
-constexpr int rows_ahead() {
-  return STEPS == 1 ? 4 : 2;
-}
+constexpr int rows_ahead(int steps) { return steps == 1 ? 4 : 2; }
+
 template <class F>
 void with_steps(int steps, F f) {
   using std::integral_constant;
   if (steps == 1) f(integral_constant<int, 1>{});
   else if (steps == 2) f(integral_constant<int, 2>{});
-  else f(integral_constant<int, 3>{});
+  else if (steps == 3) f(integral_constant<int, 3>{});
+  else f(integral_constant<int, 4>{});
 }
 
 // Calls f(T, integral_constant<int, BYTES>) for the value type and the unit.

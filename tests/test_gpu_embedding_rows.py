@@ -117,7 +117,9 @@ def test_offsets_beyond_32_bits(ops, rows, width):
 SHAPES = [(1, 1, 1, "same"), (2, 1, 7, "same"), (31, 7, 3, "uniform"), (33, 40, 16, "distinct"), (1000, 10, 64, "skewed"),
           (1024, 100_000, 100, "uniform"), (2049, 2049, 257, "distinct"), (20_000, 3, 33, "same"), (20_011, 5000, 602, "skewed"),
           (70_001, 70_000, 8, "uniform"), (300_007, 1_000_000, 4, "skewed"), (300_007, 4, 130, "skewed"), (4096, 300, 2056, "skewed"),
-          (600_000, 2, 1, "uniform")]
+          (600_000, 2, 1, "uniform"), (1_300_000, 9000, 3, "skewed"), (2_500_000, 300_000, 2, "uniform"),
+          # one CTA, a cluster, the grid: the last of the one and the first of the next
+          (2048, 500, 4, "uniform"), (2049, 500, 4, "uniform"), (32_768, 70_000, 4, "uniform"), (32_769, 70_000, 4, "uniform")]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -274,11 +276,12 @@ def test_second_derivative_is_refused(nn):
         grad.sum().backward()
 
 
-def test_capture_and_replay(nn, ops):
+@pytest.mark.parametrize("n", [700, 3000, 50_000])
+def test_capture_and_replay(nn, ops, n):
     g = generator(8)
     table = normal(g, 1000, 64).requires_grad_()
-    ids = draw_ids(g, 700, 1000, "skewed")
-    up = normal(g, 700, 64)
+    ids = draw_ids(g, n, 1000, "skewed")
+    up = normal(g, n, 64)
     streams = torch.cuda.Stream()
     streams.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(streams):
@@ -296,8 +299,8 @@ def test_capture_and_replay(nn, ops):
         graphs.append((graph, out.detach(), dense, rows))
         del out
     for turn in range(3):
-        ids.copy_(draw_ids(g, 700, 1000, "uniform" if turn else "same"))
-        up.copy_(normal(g, 700, 64))
+        ids.copy_(draw_ids(g, n, 1000, "uniform" if turn else "same"))
+        up.copy_(normal(g, n, 64))
         for graph, out, dense, (row_ids, rows, number) in graphs:
             graph.replay()
             want = exact.lookup(table.detach(), ids, 2.0, 5)
