@@ -17,79 +17,86 @@ namespace gsb {
 
 constexpr int kRowThreads = 256;
 
-// Weights of type float or of the rows' type, or none (all 1).
-struct Weights {
-  const void* p;
-  int dtype;
-};
-__device__ __forceinline__ float weight_of(const Weights& w, i64 slot) {
-  if (!w.p) return 1.f;
-  if (w.dtype == GSB_F32) return __ldg((const float*)w.p + slot);
-  if (w.dtype == GSB_F16) return __half2float(((const __half*)w.p)[slot]);
-  return __bfloat162float(((const __nv_bfloat16*)w.p)[slot]);
-}
+enum { WEIGHTS_NONE, WEIGHTS_FLOAT, WEIGHTS_OF_ROWS };
 
+// All counts are below 2^31: 32-bit arithmetic, of which there is more in these kernels than of the rows' values if one lets it.
 struct RowArgs {
-  i64 tokens, num_rows;
-  int per_token, lanes;
-  i64 units, token_stride, row_stride;  // in units
+  u32 tokens, per_token, slots, num_rows;
+  int lanes, units;                  // per group; per row
+  i64 token_stride, row_stride;      // in units
   const i64* place;
-  Weights weights;
+  const void* weights;
+  int weight_kind;
   i64* counters;
 };
 
+template <class T>
+__device__ __forceinline__ float weight_at(const RowArgs& a, u32 slot) {
+  if (a.weight_kind == WEIGHTS_NONE) return 1.f;
+  if (a.weight_kind == WEIGHTS_FLOAT) return __ldg((const float*)a.weights + slot);
+  float f[1];
+  load_unit((const Unit<T, (int)sizeof(T)>*)a.weights + slot).get(f);
+  return f[0];
+}
+
 // Row of a slot, or ~row for a slot without an expert.  kNowhere: out of range, which is recorded, unless it is the row of a
 // slot without an expert that a caller's shorter array does not have.
-constexpr i64 kNowhere = (i64)1 << 62;
-__device__ __forceinline__ i64 place_of(const RowArgs& a, i64 slot, bool report) {
+constexpr int kNowhere = (int)0x80000000;
+__device__ __forceinline__ int place_of(const RowArgs& a, u32 slot, bool report) {
   const i64 p = __ldg(a.place + slot);
-  if ((u64)(p < 0 ? ~p : p) < (u64)a.num_rows) return p;
-  if (report && (p >= 0 || ~p >= a.tokens * a.per_token)) raise_error(a.counters, GSB_ERR_INDEX_RANGE, slot);
+  const u64 row = (u64)(p < 0 ? ~p : p);
+  if (row < (u64)a.num_rows) return (int)p;
+  if (report && (p >= 0 || row >= (u64)a.slots)) raise_error(a.counters, GSB_ERR_INDEX_RANGE, slot);
   return kNowhere;
 }
 
-// A group of lanes takes kTokens tokens at a time.
+// A group of lanes takes kTokens tokens at a time, a tile of their columns (blockIdx.y).
 template <class T, int BYTES, int STEPS>
 __global__ void __launch_bounds__(kRowThreads) k_spread_rows(const RowArgs a, const Unit<T, BYTES>* __restrict__ x,
                                                              Unit<T, BYTES>* __restrict__ rows) {
   constexpr int kTokens = rows_ahead(STEPS), N = Unit<T, BYTES>::N;
   await_previous();
-  const int lane = threadIdx.x & (a.lanes - 1);
-  const i64 j = (i64)blockIdx.y * a.lanes * STEPS + lane;
-  const i64 step = (i64)gridDim.x * (kRowThreads / a.lanes) * kTokens;
-  for (i64 t = ((i64)blockIdx.x * kRowThreads + threadIdx.x) / a.lanes * kTokens; t < a.tokens; t += step) {
+  const int j = blockIdx.y * a.lanes * STEPS + (threadIdx.x & (a.lanes - 1));
+  const u32 step = gridDim.x * (kRowThreads / a.lanes) * kTokens;
+  bool in[STEPS];
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) in[s] = j + s * a.lanes < a.units;
+  x += j;
+  rows += j;
+  for (u32 t = (blockIdx.x * kRowThreads + threadIdx.x) / a.lanes * kTokens; t < a.tokens; t += step) {
     Unit<T, BYTES> v[kTokens][STEPS];
 #pragma unroll
     for (int r = 0; r < kTokens; ++r)
 #pragma unroll
       for (int s = 0; s < STEPS; ++s)
-        if (t + r < a.tokens && j + s * a.lanes < a.units) v[r][s] = load_unit_once(x + (t + r) * a.token_stride + j + s * a.lanes);
-    for (int k = 0; k < a.per_token; ++k) {
-      i64 p[kTokens];
-      float w[kTokens];
+        if (t + r < a.tokens && in[s]) v[r][s] = load_unit_once(x + (i64)(t + r) * a.token_stride + s * a.lanes);
+    for (u32 k = 0; k < a.per_token; ++k) {
+      int p[kTokens];
 #pragma unroll
-      for (int r = 0; r < kTokens; ++r) {
-        const i64 slot = (t + r) * a.per_token + k;
-        p[r] = t + r < a.tokens ? place_of(a, slot, j == 0) : kNowhere;
-        w[r] = p[r] >= 0 && p[r] != kNowhere ? weight_of(a.weights, slot) : 0.f;
-      }
+      for (int r = 0; r < kTokens; ++r) p[r] = t + r < a.tokens ? place_of(a, (t + r) * a.per_token + k, j == 0) : kNowhere;
 #pragma unroll
       for (int r = 0; r < kTokens; ++r) {
         if (p[r] == kNowhere) continue;
-        Unit<T, BYTES>* to = rows + (p[r] < 0 ? ~p[r] : p[r]) * a.units + j;
+        Unit<T, BYTES>* to = rows + (i64)(p[r] < 0 ? ~p[r] : p[r]) * a.units;
+        if (a.weight_kind == WEIGHTS_NONE && p[r] >= 0) {
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s) {
-          Unit<T, BYTES> u = v[r][s];
-          if (p[r] < 0) {
+          for (int s = 0; s < STEPS; ++s)
+            if (in[s]) store_unit_once(to + s * a.lanes, v[r][s]);
+        } else {
+          const float w = p[r] >= 0 ? weight_at<T>(a, (t + r) * a.per_token + k) : 0.f;
+#pragma unroll
+          for (int s = 0; s < STEPS; ++s) {
+            Unit<T, BYTES> u;
             u.clear();
-          } else if (a.weights.p) {
-            float f[N];
-            u.get(f);
+            if (p[r] >= 0) {
+              float f[N];
+              v[r][s].get(f);
 #pragma unroll
-            for (int q = 0; q < N; ++q) f[q] *= w[r];
-            u.set(f);
+              for (int q = 0; q < N; ++q) f[q] *= w;
+              u.set(f);
+            }
+            if (in[s]) store_unit_once(to + s * a.lanes, u);
           }
-          if (j + s * a.lanes < a.units) store_unit_once(to + s * a.lanes, u);
         }
       }
     }
@@ -99,30 +106,32 @@ __global__ void __launch_bounds__(kRowThreads) k_spread_rows(const RowArgs a, co
 // A group of lanes goes through the slots of its run of tokens, with the rows of the next kAhead slots on their way whatever
 // token they belong to.
 template <class T, int BYTES, int STEPS>
-__global__ void __launch_bounds__(kRowThreads) k_combine_rows(const RowArgs a, i64 run, const Unit<T, BYTES>* __restrict__ rows,
+__global__ void __launch_bounds__(kRowThreads) k_combine_rows(const RowArgs a, u32 run, const Unit<T, BYTES>* __restrict__ rows,
                                                               Unit<T, BYTES>* __restrict__ out) {
   constexpr int N = Unit<T, BYTES>::N, kAhead = rows_ahead(STEPS);
   await_previous();
-  const int lane = threadIdx.x & (a.lanes - 1);
-  const i64 j = (i64)blockIdx.y * a.lanes * STEPS + lane;
-  const i64 first = ((i64)blockIdx.x * kRowThreads + threadIdx.x) / a.lanes * run;
+  const int j = blockIdx.y * a.lanes * STEPS + (threadIdx.x & (a.lanes - 1));
+  const u32 first = (blockIdx.x * kRowThreads + threadIdx.x) / a.lanes * run;
   if (first >= a.tokens) return;
-  const i64 begin = first * a.per_token, end = min(first + run, a.tokens) * a.per_token;
-  Unit<T, BYTES>* to = out + first * a.units + j;
+  const u32 begin = first * a.per_token, end = min(first + run, a.tokens) * a.per_token;
+  bool in[STEPS];
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) in[s] = j + s * a.lanes < a.units;
+  rows += j;
+  out += (i64)first * a.units + j;
   float sum[STEPS][N] = {};
-  int left = a.per_token;  // slots of the token that are still to come
-  i64 p[kAhead];
+  u32 left = a.per_token;  // slots of the token that are still to come
+  int p[kAhead];
   float w[kAhead];
-  auto look = [&](i64 slot) {
+  auto look = [&](u32 slot) {
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       p[u] = slot + u < end ? place_of(a, slot + u, j == 0) : -1;
-      if (p[u] == kNowhere) p[u] = -1;
-      w[u] = p[u] >= 0 ? weight_of(a.weights, slot + u) : 0.f;
+      w[u] = p[u] >= 0 ? weight_at<T>(a, slot + u) : 0.f;
     }
   };
   look(begin);
-  for (i64 slot = begin; slot < end; slot += kAhead) {
+  for (u32 slot = begin; slot < end; slot += kAhead) {
     Unit<T, BYTES> v[kAhead][STEPS];
     float factor[kAhead];
     bool there[kAhead];
@@ -130,17 +139,18 @@ __global__ void __launch_bounds__(kRowThreads) k_combine_rows(const RowArgs a, i
     for (int u = 0; u < kAhead; ++u) {
       there[u] = p[u] >= 0;
       factor[u] = w[u];
+      if (there[u])
 #pragma unroll
-      for (int s = 0; s < STEPS; ++s)
-        if (there[u] && j + s * a.lanes < a.units) v[u][s] = load_unit_once(rows + p[u] * a.row_stride + j + s * a.lanes);
+        for (int s = 0; s < STEPS; ++s)
+          if (in[s]) v[u][s] = load_unit_once(rows + p[u] * a.row_stride + s * a.lanes);
     }
-    look(slot + kAhead);
+    if (slot + kAhead < end) look(slot + kAhead);
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       if (slot + u >= end) continue;
+      if (there[u])
 #pragma unroll
-      for (int s = 0; s < STEPS; ++s)
-        if (there[u] && j + s * a.lanes < a.units) {
+        for (int s = 0; s < STEPS; ++s) {
           float f[N];
           v[u][s].get(f);
 #pragma unroll
@@ -152,18 +162,13 @@ __global__ void __launch_bounds__(kRowThreads) k_combine_rows(const RowArgs a, i
       for (int s = 0; s < STEPS; ++s) {
         Unit<T, BYTES> r;
         r.set(sum[s]);
-        if (j + s * a.lanes < a.units) store_unit_once(to + s * a.lanes, r);
+        if (in[s]) store_unit_once(out + s * a.lanes, r);
 #pragma unroll
         for (int q = 0; q < N; ++q) sum[s][q] = 0.f;
       }
-      to += a.units;
+      out += a.units;
     }
   }
-}
-
-template <class W>
-__device__ __forceinline__ void store_weight(void* p, i64 slot, float v) {
-  ((W*)p)[slot] = from_float<W>(v);
 }
 
 // A group of lanes takes neighbouring slots at a time: one of rows in units of 16 bytes (two cost warps: 62 us for 58), two of
@@ -171,49 +176,50 @@ __device__ __forceinline__ void store_weight(void* p, i64 slot, float v) {
 template <class T, int BYTES>
 constexpr int grad_slots() { return BYTES == 16 ? 1 : 2; }
 
-template <class T, int BYTES, int STEPS>
+template <class T, int BYTES, int STEPS, bool DOTS>
 __global__ void __launch_bounds__(kRowThreads) k_combine_grad(const RowArgs a, const Unit<T, BYTES>* __restrict__ grad,
                                                               const Unit<T, BYTES>* __restrict__ rows,
                                                               Unit<T, BYTES>* __restrict__ grad_rows, void* grad_weights) {
   constexpr int N = Unit<T, BYTES>::N, kSlots = grad_slots<T, BYTES>();
   await_previous();
   const int lane = threadIdx.x & (a.lanes - 1);
-  const i64 step = (i64)gridDim.x * (kRowThreads / a.lanes) * kSlots, slots = a.tokens * a.per_token;
+  const u32 step = gridDim.x * (kRowThreads / a.lanes) * kSlots;
   // all groups of a warp take part in the sums over lanes, also those that have run out of slots
-  const i64 warp_first = ((i64)blockIdx.x * kRowThreads + (threadIdx.x & ~31)) / a.lanes * kSlots;
-  for (i64 base = warp_first; base < slots; base += step) {
-    const i64 slot = base + (threadIdx.x & 31) / a.lanes * kSlots;
-    i64 p[kSlots], t[kSlots];
-    bool there[kSlots];
+  for (u32 base = (blockIdx.x * kRowThreads + (threadIdx.x & ~31u)) / a.lanes * kSlots; base < a.slots; base += step) {
+    const u32 slot = base + (threadIdx.x & 31) / a.lanes * kSlots;
+    int p[kSlots];
     float w[kSlots], dot[kSlots] = {};
+    const Unit<T, BYTES>* g_of[kSlots];
 #pragma unroll
     for (int r = 0; r < kSlots; ++r) {
-      p[r] = slot + r < slots ? place_of(a, slot + r, lane == 0) : kNowhere;
-      t[r] = (u32)(slot + r) / (u32)a.per_token;
-      there[r] = p[r] >= 0 && p[r] != kNowhere;
-      w[r] = there[r] ? weight_of(a.weights, slot + r) : 0.f;
+      p[r] = slot + r < a.slots ? place_of(a, slot + r, lane == 0) : kNowhere;
+      w[r] = p[r] >= 0 ? weight_at<T>(a, slot + r) : 0.f;
+      g_of[r] = grad + (i64)((slot + r) / a.per_token) * a.token_stride;
     }
-    for (i64 j = lane; j < a.units; j += a.lanes * STEPS) {
+    for (int j = lane; j < a.units; j += a.lanes * STEPS) {
       Unit<T, BYTES> g[kSlots][STEPS], v[kSlots][STEPS];
 #pragma unroll
       for (int r = 0; r < kSlots; ++r)
+        if (p[r] >= 0)
+#pragma unroll
+          for (int s = 0; s < STEPS; ++s)
+            if (j + s * a.lanes < a.units) {
+              if (DOTS) v[r][s] = load_unit_once(rows + p[r] * a.row_stride + j + s * a.lanes);
+              g[r][s] = load_unit(g_of[r] + j + s * a.lanes);
+            }
+#pragma unroll
+      for (int r = 0; r < kSlots; ++r) {
+        if (p[r] == kNowhere) continue;
+        Unit<T, BYTES>* to = grad_rows + (i64)(p[r] < 0 ? ~p[r] : p[r]) * a.units + j;
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
-          if (!there[r] || j + s * a.lanes >= a.units) continue;
-          if (grad_weights) v[r][s] = load_unit_once(rows + p[r] * a.row_stride + j + s * a.lanes);
-          g[r][s] = load_unit(grad + t[r] * a.token_stride + j + s * a.lanes);
-        }
-#pragma unroll
-      for (int r = 0; r < kSlots; ++r)
-#pragma unroll
-        for (int s = 0; s < STEPS; ++s) {
-          if (p[r] == kNowhere || j + s * a.lanes >= a.units) continue;
+          if (j + s * a.lanes >= a.units) continue;
           Unit<T, BYTES> u;
           u.clear();
-          if (there[r]) {
+          if (p[r] >= 0) {
             float f[N], h[N];
             g[r][s].get(f);
-            if (grad_weights) {
+            if (DOTS) {
               v[r][s].get(h);
 #pragma unroll
               for (int q = 0; q < N; ++q) dot[r] += f[q] * h[q];
@@ -222,17 +228,17 @@ __global__ void __launch_bounds__(kRowThreads) k_combine_grad(const RowArgs a, c
             for (int q = 0; q < N; ++q) f[q] *= w[r];
             u.set(f);
           }
-          if (grad_rows) store_unit_once(grad_rows + (p[r] < 0 ? ~p[r] : p[r]) * a.units + j + s * a.lanes, u);
+          if (grad_rows) store_unit_once(to + s * a.lanes, u);
         }
+      }
     }
-    if (!grad_weights) continue;
+    if (!DOTS) continue;
 #pragma unroll
     for (int r = 0; r < kSlots; ++r) {
       for (int o = a.lanes / 2; o > 0; o >>= 1) dot[r] += __shfl_xor_sync(0xffffffffu, dot[r], o);
-      if (lane != 0 || slot + r >= slots) continue;
-      if (a.weights.dtype == GSB_F32) store_weight<float>(grad_weights, slot + r, dot[r]);
-      else if (a.weights.dtype == GSB_F16) store_weight<__half>(grad_weights, slot + r, dot[r]);
-      else store_weight<__nv_bfloat16>(grad_weights, slot + r, dot[r]);
+      if (lane != 0 || slot + r >= a.slots) continue;
+      if (a.weight_kind == WEIGHTS_FLOAT) ((float*)grad_weights)[slot + r] = dot[r];
+      else ((T*)grad_weights)[slot + r] = from_float<T>(dot[r]);
     }
   }
 }
@@ -246,6 +252,13 @@ static int check_rows(i64 tokens, i64 per_token, i64 row_len, int dtype, i64 str
   GSB_REQUIRE(tokens == 0 || place, GSB_ERR_INVALID_ARGUMENT);
   GSB_REQUIRE(!weights || weights_dtype == dtype || weights_dtype == GSB_F32, GSB_ERR_INVALID_ARGUMENT);
   return GSB_OK;
+}
+
+static RowArgs row_args(gsb_ctx* ctx, i64 tokens, i64 per_token, i64 num_rows, RowShape shape, i64 units, i64 token_stride,
+                        i64 row_stride, const int64_t* place, const void* weights, int weights_dtype) {
+  return RowArgs{(u32)tokens, (u32)per_token, (u32)(tokens * per_token), (u32)num_rows, shape.lanes, (int)units, token_stride,
+                 row_stride, place, weights,
+                 !weights ? WEIGHTS_NONE : weights_dtype == GSB_F32 ? WEIGHTS_FLOAT : WEIGHTS_OF_ROWS, ctx_counters(ctx)};
 }
 
 }  // namespace gsb
@@ -295,8 +308,8 @@ extern "C" int gsb_expert_spread(gsb_ctx* ctx, void* stream_, const void* x, int
     constexpr int B = decltype(bytes)::value;
     const i64 units = row_len * size / B;
     const RowShape shape = row_shape(units, copy_steps(B));
-    const RowArgs a{tokens, tokens * per_token, (int)per_token, shape.lanes, units, x_stride * size / B, units,
-                    place, Weights{weights, weights_dtype}, ctx_counters(ctx)};
+    const RowArgs a = row_args(ctx, tokens, per_token, tokens * per_token, shape, units, x_stride * size / B, units, place, weights,
+                               weights_dtype);
     with_steps(shape.steps, [&](auto steps) {
       constexpr int S = decltype(steps)::value, kTokens = rows_ahead(S);
       const dim3 grid((unsigned)min((i64)kNumSMs * 32, (i64)grid_for((tokens + kTokens - 1) / kTokens * a.lanes, kRowThreads)),
@@ -327,14 +340,14 @@ extern "C" int gsb_expert_combine(gsb_ctx* ctx, void* stream_, const void* rows,
     constexpr int B = decltype(bytes)::value;
     const i64 units = row_len * size / B;
     const RowShape shape = row_shape(units, copy_steps(B));
-    const RowArgs a{tokens, num_rows, (int)per_token, shape.lanes, units, units, rows_stride * size / B,
-                    place, Weights{weights, weights_dtype}, ctx_counters(ctx)};
+    const RowArgs a = row_args(ctx, tokens, per_token, num_rows, shape, units, units, rows_stride * size / B, place, weights,
+                               weights_dtype);
     with_steps(shape.steps, [&](auto steps) {
       constexpr int S = decltype(steps)::value;
       // tokens per group of lanes: one while there are SMs without work
       const i64 tiles = grid_for(units, shape.lanes * S), run = tokens * tiles * shape.lanes / 32 / (kNumSMs * 128) + 1;
       const dim3 grid(grid_for((tokens + run - 1) / run * a.lanes, kRowThreads), (unsigned)tiles);
-      launch_behind(stream, k_combine_rows<T, B, S>, grid, kRowThreads, a, run, (const Unit<T, B>*)rows,
+      launch_behind(stream, k_combine_rows<T, B, S>, grid, kRowThreads, a, (u32)run, (const Unit<T, B>*)rows,
                     (Unit<T, B>*)out);
     });
   });
@@ -363,13 +376,14 @@ extern "C" int gsb_expert_combine_grad(gsb_ctx* ctx, void* stream_, const void* 
     constexpr int B = decltype(bytes)::value;
     const i64 units = row_len * size / B;
     const RowShape shape = row_shape(units, copy_steps(B));
-    const RowArgs a{tokens, num_rows, (int)per_token, shape.lanes, units, grad_stride * size / B, rows_stride * size / B,
-                    place, Weights{weights, weights_dtype}, ctx_counters(ctx)};
+    const RowArgs a = row_args(ctx, tokens, per_token, num_rows, shape, units, grad_stride * size / B, rows_stride * size / B, place,
+                               weights, weights_dtype);
     with_steps(shape.steps, [&](auto steps) {
       constexpr int S = decltype(steps)::value, kSlots = grad_slots<T, B>();
       const int grid = (int)min((i64)kNumSMs * 32, (i64)grid_for((tokens * per_token + kSlots - 1) / kSlots * a.lanes, kRowThreads));
-      launch_behind(stream, k_combine_grad<T, B, S>, grid, kRowThreads, a, (const Unit<T, B>*)grad,
-                    (const Unit<T, B>*)rows, (Unit<T, B>*)out_grad_rows, out_grad_weights);
+      auto kernel = out_grad_weights ? k_combine_grad<T, B, S, true> : k_combine_grad<T, B, S, false>;
+      launch_behind(stream, kernel, grid, kRowThreads, a, (const Unit<T, B>*)grad, (const Unit<T, B>*)rows,
+                    (Unit<T, B>*)out_grad_rows, out_grad_weights);
     });
   });
   GSB_LAUNCH_OK();
