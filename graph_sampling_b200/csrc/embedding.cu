@@ -22,48 +22,63 @@ constexpr int lookup_rows(int unit, int steps) { return unit < 16 ? 4 : rows_ahe
 
 // A group of lanes takes neighbouring rows of the result, a tile of their columns at a time: all its reads are on their way before
 // anything is written.
+struct LookupArgs {
+  const i64* ids;
+  u32 n;
+  int units, lanes;
+  i64 num_rows, stride;  // stride in units
+  i64 padding;
+  bool has_padding;
+  float scale;
+  i64* counters;
+};
+
 template <class T, int BYTES, int STEPS>
-__global__ void __launch_bounds__(kLookupThreads) k_lookup_rows(const Unit<T, BYTES>* __restrict__ table, i64 num_rows,
-                                                                i64 stride, i64 units, const i64* __restrict__ ids, i64 n,
-                                                                float scale, bool has_padding, i64 padding, int lanes,
-                                                                Unit<T, BYTES>* __restrict__ out, i64* counters) {
+__global__ void __launch_bounds__(kLookupThreads) k_lookup_rows(const LookupArgs a, const Unit<T, BYTES>* __restrict__ table,
+                                                                Unit<T, BYTES>* __restrict__ out) {
   constexpr int kRows = lookup_rows(BYTES, STEPS), N = Unit<T, BYTES>::N;
   await_previous();
-  const int lane = threadIdx.x & (lanes - 1);
-  const i64 step = (i64)gridDim.x * (kLookupThreads / lanes) * kRows;
-  for (i64 i = ((i64)blockIdx.x * kLookupThreads + threadIdx.x) / lanes * kRows; i < n; i += step) {
-    i64 row[kRows];
+  const int lane = threadIdx.x & (a.lanes - 1), lanes = a.lanes;
+  const u32 step = gridDim.x * (kLookupThreads / lanes) * kRows;
+  for (u32 i = (blockIdx.x * kLookupThreads + threadIdx.x) / lanes * kRows; i < a.n; i += step) {
+    const Unit<T, BYTES>* from[kRows];  // null: zeros
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      row[r] = i + r < n ? __ldg(ids + i + r) : -1;
-      const bool padded = has_padding && row[r] == padding;
-      if ((u64)row[r] >= (u64)num_rows || padded) {
-        if (lane == 0 && blockIdx.y == 0 && !padded && i + r < n) raise_error(counters, GSB_ERR_INDEX_RANGE, i + r);
-        row[r] = -1;
-      }
+      from[r] = nullptr;
+      if (i + r >= a.n) continue;
+      const i64 id = __ldg(a.ids + i + r);
+      if (a.has_padding && id == a.padding) continue;
+      if ((u64)id < (u64)a.num_rows) from[r] = table + id * a.stride;
+      else if (lane == 0 && blockIdx.y == 0) raise_error(a.counters, GSB_ERR_INDEX_RANGE, i + r);
     }
-    for (i64 j = (i64)blockIdx.y * lanes * STEPS + lane; j < units; j += (i64)gridDim.y * lanes * STEPS) {
+    Unit<T, BYTES>* to = out + (i64)i * a.units;
+    for (int j = blockIdx.y * lanes * STEPS + lane; j < a.units; j += gridDim.y * lanes * STEPS) {
       Unit<T, BYTES> v[kRows][STEPS];
 #pragma unroll
       for (int r = 0; r < kRows; ++r)
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
           v[r][s].clear();
-          if (row[r] >= 0 && j + s * lanes < units) v[r][s] = load_unit(table + row[r] * stride + j + s * lanes);
+          if (from[r] && j + s * lanes < a.units) v[r][s] = load_unit(from[r] + j + s * lanes);
         }
+      if (a.scale != 1.f)
+#pragma unroll
+        for (int r = 0; r < kRows; ++r)
+          if (from[r])
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) {
+              float f[N];
+              v[r][s].get(f);
+#pragma unroll
+              for (int q = 0; q < N; ++q) f[q] *= a.scale;
+              v[r][s].set(f);
+            }
 #pragma unroll
       for (int r = 0; r < kRows; ++r)
+        if (i + r < a.n)
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s) {
-          if (scale != 1.f && row[r] >= 0) {
-            float f[N];
-            v[r][s].get(f);
-#pragma unroll
-            for (int q = 0; q < N; ++q) f[q] *= scale;
-            v[r][s].set(f);
-          }
-          if (i + r < n && j + s * lanes < units) store_unit(out + (i + r) * units + j + s * lanes, v[r][s]);
-        }
+          for (int s = 0; s < STEPS; ++s)
+            if (j + s * lanes < a.units) store_unit(to + (i64)r * a.units + j + s * lanes, v[r][s]);
     }
   }
 }
@@ -86,16 +101,16 @@ __device__ __forceinline__ void store_values(O* to, const float* v, float scale)
 constexpr int kSumThreads = 128;
 
 struct SumArgs {
-  i64 n;          // sorted positions
-  int chunk;      // positions per group of lanes
-  int lanes;      // per group, a power of two
-  u32 num_rows;   // of the result: a position whose row is not below that belongs to no sum
-  i64 units;      // per row
-  i64 stride;     // of `grad`, in units
+  u32 n;         // sorted positions
+  u32 chunk;     // positions per group of lanes
+  u32 num_rows;  // of the result: a position whose row is not below that belongs to no sum
+  int lanes;     // per group, a power of two
+  int units;     // per row
+  i64 stride;    // of `grad`, in units
   float scale;
 };
 __device__ __forceinline__ bool usable(const SumArgs& a, u64 pair) {
-  return pair_key(pair) < a.num_rows && pair_at(pair) < (u32)a.n;
+  return pair_key(pair) < a.num_rows && pair_at(pair) < a.n;
 }
 
 // One group of lanes per chunk and column tile (blockIdx.y) of lanes * STEPS units.
@@ -105,44 +120,52 @@ __global__ void __launch_bounds__(kSumThreads) k_sum_rows(const SumArgs a, const
                                                           float* __restrict__ part) {
   constexpr int N = Unit<T, BYTES>::N, kAhead = BYTES >= 8 && BYTES * STEPS <= 16 ? 4 : 2;
   await_previous();
-  const i64 chunk = ((i64)blockIdx.x * kSumThreads + threadIdx.x) / a.lanes;
-  const i64 begin = chunk * a.chunk, end = min(begin + a.chunk, a.n);
-  const i64 first = (i64)blockIdx.y * a.lanes * STEPS + (threadIdx.x & (a.lanes - 1));
-  if (begin >= a.n) return;
-  const i64 width = a.units * N;
+  const u32 chunk = (u32)(((u64)blockIdx.x * kSumThreads + threadIdx.x) / a.lanes);
+  const u64 at = (u64)chunk * a.chunk;
+  if (at >= a.n) return;
+  const u32 begin = (u32)at, end = min(begin + a.chunk, a.n);
+  const int first = blockIdx.y * a.lanes * STEPS + (threadIdx.x & (a.lanes - 1));
+  bool in[STEPS];
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) in[s] = first + s * a.lanes < a.units;
+  const i64 width = (i64)a.units * N;
+  grad += first;
+  out += (i64)first * N;
+  part += 2 * (i64)chunk * width + (i64)first * N;
   float sum[STEPS][N] = {};
-  bool head = begin > 0 && pair_key(sorted[begin - 1]) == pair_key(sorted[begin]);
   auto put = [&](auto* to, float scale) {
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
-      const i64 unit = first + s * a.lanes;
-      if (unit < a.units) store_values<std::remove_pointer_t<decltype(to)>, N>(to + unit * N, sum[s], scale);
+      if (in[s]) store_values<std::remove_pointer_t<decltype(to)>, N>(to + s * a.lanes * N, sum[s], scale);
 #pragma unroll
       for (int q = 0; q < N; ++q) sum[s][q] = 0.f;
     }
   };
+  sorted += begin;
+  const u32 left = a.n - begin, mine = end - begin;  // positions up to the list's end, and the chunk's
+  bool head = begin > 0 && pair_key(__ldg(sorted - 1)) == pair_key(__ldg(sorted));
   u64 p[kAhead + 1], next[kAhead + 1];
 #pragma unroll
-  for (int u = 0; u <= kAhead; ++u) p[u] = begin + u < a.n ? __ldg(sorted + begin + u) : ~0ull;
-  for (i64 j = begin; j < end; j += kAhead) {
+  for (int u = 0; u <= kAhead; ++u) p[u] = u < left ? __ldg(sorted + u) : ~0ull;
+  for (u32 j = 0; j < mine; j += kAhead) {
     Unit<T, BYTES> v[kAhead][STEPS];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      if (j + u >= end || !usable(a, p[u])) continue;
+      if (j + u >= mine || !usable(a, p[u])) continue;
       const Unit<T, BYTES>* from = grad + (i64)pair_at(p[u]) * a.stride;
 #pragma unroll
       for (int s = 0; s < STEPS; ++s)
-        if (first + s * a.lanes < a.units) v[u][s] = load_unit_once(from + first + s * a.lanes);
+        if (in[s]) v[u][s] = load_unit_once(from + s * a.lanes);
     }
     next[0] = p[kAhead];
 #pragma unroll
-    for (int u = 1; u <= kAhead; ++u) next[u] = j + kAhead + u < a.n ? __ldg(sorted + j + kAhead + u) : ~0ull;
+    for (int u = 1; u <= kAhead; ++u) next[u] = j + kAhead + u < left ? __ldg(sorted + j + kAhead + u) : ~0ull;
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      if (j + u >= end || !usable(a, p[u])) return;  // the sorted list ends with the positions that belong to no row
+      if (j + u >= mine || !usable(a, p[u])) return;  // the sorted list ends with the positions that belong to no row
 #pragma unroll
       for (int s = 0; s < STEPS; ++s)
-        if (first + s * a.lanes < a.units) {
+        if (in[s]) {
           float f[N];
           v[u][s].get(f);
 #pragma unroll
@@ -151,7 +174,7 @@ __global__ void __launch_bounds__(kSumThreads) k_sum_rows(const SumArgs a, const
       const u32 row = pair_key(p[u]);
       const bool ends = pair_key(p[u + 1]) != row;
       if (ends && !head) put(out + (i64)row * width, a.scale);
-      else if (ends || j + u + 1 == end) put(part + (2 * chunk + (head ? 0 : 1)) * width, 1.f);
+      else if (ends || j + u + 1 == mine) put(part + (head ? 0 : width), 1.f);
       if (ends) head = false;
     }
 #pragma unroll
@@ -190,7 +213,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_join_rows(const SumArgs a, i64
     }
   };
   // lane l: chunk c + l, and the first key of the chunk behind it; the lanes from kJoinSpan on only look ahead
-  const i64 c = ((i64)blockIdx.x * kJoinWarps + warp) * kJoinSpan + lane, end = (c + 1) * a.chunk;
+  const i64 c = ((i64)blockIdx.x * kJoinWarps + warp) * kJoinSpan + lane, end = (c + 1) * (i64)a.chunk;
   const bool inner = c + 1 < chunks;
   const u32 behind = inner ? pair_key(__ldg(sorted + end)) : kNoRow;
   u32 last = kNoRow, before = kNoRow;
@@ -207,7 +230,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_join_rows(const SumArgs a, i64
     i64 run = other ? __ffs(other) - 1 - l : 32 - l;  // chunks behind that go on with it
     for (bool more = other == 0; more;) {
       const i64 next = chunk + 1 + run + lane;
-      const u32 rest = __ballot_sync(0xffffffffu, next >= chunks || pair_key(__ldg(sorted + next * a.chunk)) != row);
+      const u32 rest = __ballot_sync(0xffffffffu, next >= chunks || pair_key(__ldg(sorted + next * (i64)a.chunk)) != row);
       run += rest ? __ffs(rest) - 1 : 32;
       more = rest == 0;
     }
@@ -276,7 +299,7 @@ static GradPlan grad_plan(i64 n, i64 num_rows, i64 row_len) {
 template <class T, class O, int BYTES>
 static void launch_sum(cudaStream_t stream, SumArgs a, i64 chunks, const void* grad, i64 stride_bytes, i64 row_bytes,
                        const u64* sorted, void* out, float* part) {
-  a.units = row_bytes / BYTES;
+  a.units = (int)(row_bytes / BYTES);
   a.stride = stride_bytes / BYTES;
   const RowShape shape = row_shape(a.units, sum_steps(BYTES));
   a.lanes = shape.lanes;
@@ -303,7 +326,7 @@ static int sum_sorted(gsb_ctx* ctx, cudaStream_t stream, const GradCall& c, cons
   const i64 row_bytes = c.row_len * size, stride_bytes = c.grad_stride * size;
   int unit = unit_bytes(row_bytes, (u64)(uintptr_t)c.grad | (u64)stride_bytes);
   while (unit > size && (uintptr_t)c.out % min(16, unit / size * out_size) != 0) unit /= 2;
-  SumArgs a{n, plan.chunk, 32, (u32)num_rows, 0, 0, c.scale};
+  const SumArgs a{(u32)n, (u32)plan.chunk, (u32)num_rows, 32, 0, 0, c.scale};
   ScopedKernelTimer timer(ctx, KID_EMBED_GRAD, stream);
   with_unit(c.dtype, unit, [&](auto value, auto bytes) {
     typedef decltype(value) T;
@@ -341,7 +364,8 @@ extern "C" int gsb_embedding_lookup(gsb_ctx* ctx, void* stream_, const void* tab
                                     int64_t row_len, int64_t row_stride, const int64_t* ids, int64_t n, float scale,
                                     int has_padding, int64_t padding_id, void* out) {
   GSB_ENTER(ctx);
-  GSB_REQUIRE(num_rows >= 0 && row_len >= 1 && row_len <= GSB_MAX_ROW_LEN && row_stride >= 0 && n >= 0 && value_bytes(dtype) != 0, GSB_ERR_INVALID_ARGUMENT);
+  GSB_REQUIRE(num_rows >= 0 && row_len >= 1 && row_len <= GSB_MAX_ROW_LEN && row_stride >= 0 && n >= 0 && n < ((i64)1 << 31) &&
+                  value_bytes(dtype) != 0, GSB_ERR_INVALID_ARGUMENT);
   if (n == 0) return GSB_OK;
   GSB_REQUIRE((table || num_rows == 0) && ids && out, GSB_ERR_INVALID_ARGUMENT);
   const void* from = nullptr;
@@ -368,9 +392,10 @@ extern "C" int gsb_embedding_lookup(gsb_ctx* ctx, void* stream_, const void* tab
         // a group goes through the tiles of its rows' columns, or shares them with others where there are few rows
         const i64 ctas = grid_for((n + kRows - 1) / kRows * shape.lanes, kLookupThreads), tiles = grid_for(units, shape.lanes * S);
         const dim3 grid((unsigned)min((i64)kNumSMs * 32, ctas), (unsigned)min(tiles, max((i64)1, kNumSMs * 8 / ctas)));
-        launch_behind(stream, k_lookup_rows<T, kBytes, S>, grid, kLookupThreads,
-                      (const Unit<T, kBytes>*)from, num_rows, row_stride * size / kBytes, units, ids, n, scale,
-                      has_padding != 0, padding_id, shape.lanes, (Unit<T, kBytes>*)out, ctx_counters(ctx));
+        const LookupArgs args{ids, (u32)n, (int)units, shape.lanes, num_rows, row_stride * size / kBytes, padding_id, has_padding != 0,
+                              scale, ctx_counters(ctx)};
+        launch_behind(stream, k_lookup_rows<T, kBytes, S>, grid, kLookupThreads, args, (const Unit<T, kBytes>*)from,
+                      (Unit<T, kBytes>*)out);
       });
     });
   }

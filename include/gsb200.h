@@ -579,7 +579,7 @@ GSB_API int gsb_sage_hop_sized(gsb_ctx* ctx, void* stream, const int64_t* indptr
 enum gsb_dtype { GSB_F32 = 0, GSB_F16 = 1, GSB_BF16 = 2 };
 
 /* out[i, :] = scale * table[ids[i], :]; zeros where ids[i] == padding_id (with has_padding; it may be any number, -1 for
- * instance) or ids[i] is outside [0, num_rows).  table: device memory, or page-locked host memory read in place. */
+ * instance) or ids[i] is outside [0, num_rows).  n below 2^31.  table: device memory, or page-locked host memory read in place. */
 GSB_API int gsb_embedding_lookup(gsb_ctx* ctx, void* stream, const void* table, int dtype, int64_t num_rows,
                                  int64_t row_len, int64_t row_stride, const int64_t* ids, int64_t n, float scale,
                                  int has_padding, int64_t padding_id, void* out);
