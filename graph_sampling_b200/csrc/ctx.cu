@@ -394,9 +394,16 @@ int ctx_check_device_error(gsb_ctx* ctx, cudaStream_t stream) {
 void ctx_count_launches(gsb_ctx* ctx, int n) { ctx->launches += n; }
 void ctx_count_id_bound_refusal(gsb_ctx* ctx) { ctx->id_bound_refusals += 1; }
 
+// An event recorded in a capture has no time: captured launches are only counted.
+static bool prof_records(gsb_ctx* ctx, cudaStream_t stream) {
+  if (!ctx->profiling) return false;
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  return cudaStreamIsCapturing(stream, &capture) == cudaSuccess && capture == cudaStreamCaptureStatusNone;
+}
+
 void ctx_prof_begin(gsb_ctx* ctx, int kid, cudaStream_t stream) {
   ctx->launches += 1;
-  if (!ctx->profiling) return;
+  if (!prof_records(ctx, stream)) return;
   if (ctx->ev_used == ctx->ev_begin->size()) {
     cudaEvent_t a, b;
     if (cudaEventCreate(&a) != cudaSuccess || cudaEventCreate(&b) != cudaSuccess) return;
@@ -410,7 +417,7 @@ void ctx_prof_begin(gsb_ctx* ctx, int kid, cudaStream_t stream) {
 
 void ctx_prof_end(gsb_ctx* ctx, int kid, cudaStream_t stream) {
   (void)kid;
-  if (!ctx->profiling || ctx->ev_used >= ctx->ev_begin->size()) return;
+  if (!prof_records(ctx, stream) || ctx->ev_used >= ctx->ev_begin->size()) return;
   cudaEventRecord((*ctx->ev_end)[ctx->ev_used], stream);
   ctx->ev_used += 1;
 }

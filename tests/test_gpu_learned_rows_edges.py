@@ -1,0 +1,184 @@
+"""Learned rows where calls meet other things: waits that run out, memory at odd addresses, other streams, timing in a capture."""
+import pytest
+import torch
+
+import learned_rows as exact
+
+pytestmark = pytest.mark.gpu
+TIMEOUT = -5
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from graph_sampling_b200 import ops as m
+    return m
+
+
+def generator(seed):
+    g = torch.Generator("cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+# ---- the sort of more than 32 768 positions meets at a word in memory --------------------------------------------------------
+@pytest.mark.parametrize("kind", ["dense", "rows", "order", "order of many"])
+def test_waits_that_run_out(ops, kind):
+    from graph_sampling_b200.cabi import GsbError
+    g = generator(1)
+    n, rows = 400_000, 30_000
+    ids = torch.randint(0, rows, (n,), generator=g, device="cuda")
+    grad = torch.randn(n, 8, generator=g, device="cuda")
+    ctx = ops.Context()
+
+    def call():
+        if kind == "dense":
+            return (ops.embedding_grad(grad, ids, rows, ctx=ctx),)
+        if kind == "rows":
+            return ops.embedding_grad_rows(grad, ids, rows, sync=False, ctx=ctx)
+        return ops.expert_order(ids if kind == "order of many" else ids % 50, rows if kind == "order of many" else 50, ctx=ctx)
+
+    want = call()
+    ctx.check_device()
+    usual, expired = ctx.get_option("max_polls"), 0
+    ctx.set_option("max_polls", 1)
+    for _ in range(100):
+        got = call()
+        try:
+            ctx.check_device()
+            number = int(got[2]) if kind == "rows" else None
+            for x, y in zip(got, want):
+                assert torch.equal(x[:number], y[:number])     # whoever gets through all the same is right
+        except GsbError as e:
+            assert e.status == TIMEOUT
+            expired += 1
+            if kind.startswith("order"):                       # what is left can be used as indexes
+                offsets, source, place = got
+                assert 0 <= int(offsets.min()) and int(offsets.max()) <= n and 0 <= int(source.min()) and int(source.max()) < n
+                assert -n <= int(place.min()) and int(place.max()) < n
+            if expired == 5:
+                break
+    assert expired > 0 or kind == "order"          # one barrier, to which all come at the same time
+    ctx.set_option("max_polls", usual)
+    for x, y in zip(call(), want):
+        number = int(want[2]) if kind == "rows" else None
+        assert torch.equal(x[:number], y[:number])
+    ctx.check_device()
+
+
+# ---- memory at odd addresses ---------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,code", [(torch.float32, 0), (torch.float16, 1), (torch.bfloat16, 2)])
+@pytest.mark.parametrize("n", [50, 40_000])
+@pytest.mark.parametrize("shift", [1, 2, 3, 5])
+def test_results_at_any_address(ops, dtype, code, n, shift):
+    """Tables, gradients and results that begin in the middle of a unit, with nothing written around them."""
+    g = generator(shift)
+    rows, width = 333, 24
+    ctx = ops.default_context()
+    ids = torch.randint(0, rows - 30, (n,), generator=g, device="cuda")
+    room = torch.randn(n * width + 16, generator=g, device="cuda").to(dtype)
+    grad = room[shift:shift + n * width].view(n, width)
+    guard = torch.full((rows * width + 32,), 7.0, dtype=dtype, device="cuda")
+    work = torch.empty(ctx.lib.gsb_embedding_grad_workspace(n, rows, width), dtype=torch.uint8, device="cuda")
+    out = guard[shift:shift + rows * width].view(rows, width)
+    assert ctx.lib.gsb_embedding_grad(ctx.handle, stream(), grad.data_ptr(), code, width, width, ids.data_ptr(), n, rows, 1.0, 0, 0,
+                                      out.data_ptr(), code, work.data_ptr(), work.numel()) == 0
+    exact.within(out, *exact.sums(grad, ids, rows, 1.0, None))
+    assert torch.all(guard[:shift] == 7) and torch.all(guard[shift + rows * width:] == 7)
+    wide = torch.full((rows * width + 32,), 7.0, device="cuda")
+    out = wide[shift:shift + rows * width].view(rows, width)
+    assert ctx.lib.gsb_embedding_grad(ctx.handle, stream(), grad.data_ptr(), code, width, width, ids.data_ptr(), n, rows, 1.0, 0, 0,
+                                      out.data_ptr(), 0, work.data_ptr(), work.numel()) == 0
+    exact.within(out, *exact.sums(grad, ids, rows, 1.0, None))
+    assert torch.all(wide[:shift] == 7) and torch.all(wide[shift + rows * width:] == 7)
+    guard = torch.full((n * width + 32,), 7.0, dtype=dtype, device="cuda")
+    out = guard[shift:shift + n * width].view(n, width)
+    assert ctx.lib.gsb_embedding_lookup(ctx.handle, stream(), grad.data_ptr(), code, n, width, width, ids.data_ptr(), n, 1.0, 0, 0,
+                                        out.data_ptr()) == 0
+    assert torch.all(guard[:shift] == 7) and torch.all(guard[shift + n * width:] == 7)
+    keep = ids < n                                             # ids beyond the n rows of this table are zeros, and recorded
+    assert torch.equal(out[keep], grad[ids[keep]]) and torch.all(out[~keep] == 0)
+    if not bool(keep.all()):
+        from graph_sampling_b200.cabi import GsbError
+        with pytest.raises(GsbError):
+            ctx.check_device()
+
+
+def test_no_rows_and_all_padding(ops):
+    from graph_sampling_b200.cabi import GsbError
+    ctx = ops.Context()
+    for n in (5, 50_000):
+        grad = torch.ones(n, 6, device="cuda")
+        ids = torch.zeros(n, dtype=torch.int64, device="cuda")
+        assert ops.embedding_grad(grad, ids, 0, 1.0, 0, ctx=ctx).shape == (0, 6)
+        assert int(torch.count_nonzero(ops.embedding_grad(grad, ids, 9, 1.0, 0, ctx=ctx))) == 0
+        assert ops.embedding_grad_rows(grad, ids, 9, 1.0, 0, ctx=ctx)[0].numel() == 0
+        ctx.check_device()
+        ops.embedding_grad(grad, ids, 0, ctx=ctx)
+        with pytest.raises(GsbError):
+            ctx.check_device()
+
+
+# ---- other streams ---------------------------------------------------------------------------------------------------------------
+def test_inputs_made_on_another_stream(ops):
+    """Kernels are set up before the one in front of them has ended: what an event orders still comes first."""
+    g = generator(3)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    table = torch.randn(5000, 128, generator=g, device="cuda")
+    other = torch.randn(40_000, 128, generator=g, device="cuda")
+    ids = torch.randint(0, 5000, (40_000,), generator=g, device="cuda")
+    filler = torch.randn(4096, 4096, device="cuda")
+    torch.cuda.synchronize()
+    for turn in range(10):
+        n = 20_000 if turn % 2 else 40_000
+        value = float(turn + 1)
+        with torch.cuda.stream(b):
+            ops.embedding_lookup(table, ids)                                  # something of ours in front
+        with torch.cuda.stream(a):
+            filler @ filler                                                   # long enough for b to get ahead
+            made = other[:n] * 0 + value
+            event = a.record_event()
+        with torch.cuda.stream(b):
+            b.wait_event(event)
+            made.record_stream(b)
+            grad = ops.embedding_grad(made, ids[:n], 5000)
+            back = ops.embedding_lookup(grad, ids[:n])
+        torch.cuda.synchronize()
+        count = torch.bincount(ids[:n], minlength=5000).float() * value
+        assert torch.equal(grad, count[:, None].expand(5000, 128)) and torch.equal(back, count[ids[:n], None].expand(n, 128))
+
+
+def test_results_used_on_the_spot_by_other_kernels(ops):
+    """Ours behind torch's and torch's behind ours, in one stream, many times over."""
+    g = generator(4)
+    table = torch.randn(300, 64, generator=g, device="cuda")
+    ids = torch.randint(0, 300, (1000,), generator=g, device="cuda")
+    for _ in range(50):
+        table.add_(1.0)
+        rows = ops.embedding_lookup(table, ids)
+        rows.mul_(2.0)
+        grad = ops.embedding_grad(rows, ids, 300, 0.5)
+        count = torch.bincount(ids, minlength=300).double()[:, None]
+        want = table.double() * count                      # 2 * 0.5: exact scalings, sums of equal values
+        assert torch.all((grad.double() - want).abs() <= (count + 2) * exact.U * want.abs() * 1.01)
+
+
+def test_profiling_does_not_enter_a_capture(ops):
+    ctx = ops.Context()
+    g = generator(5)
+    ids = torch.randint(0, 100, (500,), generator=g, device="cuda")
+    grad = torch.randn(500, 16, generator=g, device="cuda")
+    ops.embedding_grad(grad, ids, 100, ctx=ctx)
+    ctx.profile_enable(True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.embedding_grad(grad, ids, 100, ctx=ctx)
+    ops.embedding_grad(grad, ids, 100, ctx=ctx)
+    graph.replay()
+    times = ctx.profile_read()
+    ctx.profile_enable(False)
+    assert times["key_sort"][1] == 1 and times["embed_grad"][1] == 1 and times["key_sort"][0] > 0
+    exact.within(out, *exact.sums(grad, ids, 100, 1.0, None))
