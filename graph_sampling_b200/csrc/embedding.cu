@@ -17,8 +17,8 @@ namespace gsb {
 
 constexpr int kLookupThreads = 256;
 
-// Narrow units: more rows (1 000 000 rows of 602 bf16 482 us for 509, 1.3 M of 50 bf16 72 for 81).
-constexpr int lookup_rows(int unit, int steps) { return unit < 16 ? 4 : rows_ahead(steps); }
+// Narrow units: more rows (1 000 000 rows of 602 bf16 435 us for 474), but not with four units a lane (1.3 M of 50 bf16 53 for 56).
+constexpr int lookup_rows(int unit, int steps) { return unit < 16 && steps < 4 ? 4 : rows_ahead(steps); }
 
 // A group of lanes takes neighbouring rows of the result, a tile of their columns at a time: all its reads are on their way before
 // anything is written.
@@ -118,7 +118,8 @@ template <class T, class O, int BYTES, int STEPS>
 __global__ void __launch_bounds__(kSumThreads) k_sum_rows(const SumArgs a, const Unit<T, BYTES>* __restrict__ grad,
                                                           const u64* __restrict__ sorted, O* __restrict__ out,
                                                           float* __restrict__ part) {
-  constexpr int N = Unit<T, BYTES>::N, kAhead = BYTES >= 8 && BYTES * STEPS <= 16 ? 4 : 2;
+  constexpr int N = Unit<T, BYTES>::N;
+  constexpr int kAhead = 2;  // rows on their way; with four, rows of 200 bytes took 86 us for 82
   await_previous();
   const u32 chunk = (u32)(((u64)blockIdx.x * kSumThreads + threadIdx.x) / a.lanes);
   const u64 at = (u64)chunk * a.chunk;
@@ -228,12 +229,16 @@ __global__ void __launch_bounds__(kJoinThreads) k_join_rows(const SumArgs a, i64
     const i64 chunk = __shfl_sync(0xffffffffu, c, l);
     const u32 other = __ballot_sync(0xffffffffu, behind != row) & ~((1u << l) - 1u);  // lanes whose next chunk begins with another
     i64 run = other ? __ffs(other) - 1 - l : 32 - l;  // chunks behind that go on with it
-    for (bool more = other == 0; more;) {
-      const i64 next = chunk + 1 + run + lane;
-      const u32 rest = __ballot_sync(0xffffffffu, next >= chunks || pair_key(__ldg(sorted + next * (i64)a.chunk)) != row);
-      run += rest ? __ffs(rest) - 1 : 32;
-      more = rest == 0;
+    // beyond the lanes' view: the keys ascend, so 32 probes at a time narrow the end down to a 32nd
+    i64 lo = chunk + 1 + run, hi = other ? lo : chunks;  // chunks before lo go on with it, from hi on none does
+    while (lo < hi) {
+      const i64 step = (hi - lo + 31) / 32, probe = lo + lane * step;
+      const u32 not_row = __ballot_sync(0xffffffffu, probe >= hi || pair_key(__ldg(sorted + probe * (i64)a.chunk)) != row);
+      const int with = not_row ? __ffs(not_row) - 1 : 32;  // probes that go on with it
+      if (with < 32) hi = min(hi, lo + with * step);
+      if (with > 0) lo += (with - 1) * step + 1;
     }
+    run = lo - chunk - 1;
     if (run > kJoinShort) {
       if (lane == 0) {
         const int at = atomicAdd(&s_long, 1);
@@ -270,43 +275,46 @@ __global__ void __launch_bounds__(kJoinThreads) k_join_rows(const SumArgs a, i64
   }
 }
 
-// Positions per chunk: enough groups of lanes for two full sets of warps where there are few positions, else so many that the
-// ends of a chunk, whose sums are written and read once more, are few beside what it reads.
-static int sum_chunk(i64 n, i64 row_len) {
-  const i64 lanes = row_len >= 128 ? 32 : row_len >= 64 ? 16 : 8, tiles = (row_len + 511) / 512;
-  const i64 c = n * tiles * lanes / 32 / (kNumSMs * 128);
-  return (int)(c < 8 ? 8 : c > 128 ? 128 : c);
+// Positions per chunk: as many groups of lanes as make two waves of warps, so that hubs and frequent ids are shared by many, and no
+// more: each chunk's ends, two sums, are written and read once more (200 000 rows of 512 bf16 133 us, with half the chunk 141).
+static i64 sum_chunk(i64 n, int lanes, i64 tiles) {
+  const i64 c = n * tiles * max(lanes, 8) / 32 / (kNumSMs * 64);
+  return c < 8 ? 8 : c > 128 ? 128 : c;
 }
 
 struct GradPlan {
   size_t sort_bytes, total_bytes;
-  i64 chunks;
-  int chunk;
+  i64 most_chunks;  // that there is room for
 };
 
 static GradPlan grad_plan(i64 n, i64 num_rows, i64 row_len) {
   GradPlan g;
-  g.chunk = sum_chunk(n, row_len);
-  g.chunks = (n + g.chunk - 1) / g.chunk;
+  // what the units of the call, which are not known here, make of a row is at least this
+  const i64 chunk = sum_chunk(n, row_len >= 512 ? 32 : row_len >= 256 ? 16 : 8, (row_len + 511) / 512);
+  g.most_chunks = (n + chunk - 1) / chunk;
   g.sort_bytes = key_sort_bytes(n, num_rows);
   Pieces p(nullptr);
   p.take<char>(g.sort_bytes);
-  p.take<float>((size_t)g.chunks * 2 * (size_t)row_len);
+  p.take<float>((size_t)g.most_chunks * 2 * (size_t)row_len);
   g.total_bytes = p.used;
   return g;
 }
 
+// Leaves the shape and the chunks in `a`.
 template <class T, class O, int BYTES>
-static void launch_sum(cudaStream_t stream, SumArgs a, i64 chunks, const void* grad, i64 stride_bytes, i64 row_bytes,
+static void launch_sum(cudaStream_t stream, SumArgs& a, i64 most_chunks, const void* grad, i64 stride_bytes, i64 row_bytes,
                        const u64* sorted, void* out, float* part) {
   a.units = (int)(row_bytes / BYTES);
   a.stride = stride_bytes / BYTES;
   const RowShape shape = row_shape(a.units, sum_steps(BYTES));
   a.lanes = shape.lanes;
+  const int tiles = grid_for(a.units, shape.lanes * shape.steps);
+  const i64 n = a.n;
+  a.chunk = (u32)max(sum_chunk(n, shape.lanes, tiles), (n + most_chunks - 1) / most_chunks);
   with_steps(shape.steps, [&](auto steps) {
-    constexpr int S = decltype(steps)::value;
-    const dim3 grid(grid_for(chunks * a.lanes, kSumThreads), grid_for(a.units, a.lanes * S));
-    launch_behind(stream, k_sum_rows<T, O, BYTES, S>, grid, kSumThreads, a, (const Unit<T, BYTES>*)grad, sorted, (O*)out, part);
+    const dim3 grid(grid_for((n + a.chunk - 1) / a.chunk * a.lanes, kSumThreads), tiles);
+    launch_behind(stream, k_sum_rows<T, O, BYTES, decltype(steps)::value>, grid, kSumThreads, a, (const Unit<T, BYTES>*)grad, sorted,
+                  (O*)out, part);
   });
 }
 
@@ -326,22 +334,23 @@ static int sum_sorted(gsb_ctx* ctx, cudaStream_t stream, const GradCall& c, cons
   const i64 row_bytes = c.row_len * size, stride_bytes = c.grad_stride * size;
   int unit = unit_bytes(row_bytes, (u64)(uintptr_t)c.grad | (u64)stride_bytes);
   while (unit > size && (uintptr_t)c.out % min(16, unit / size * out_size) != 0) unit /= 2;
-  const SumArgs a{(u32)n, (u32)plan.chunk, (u32)num_rows, 32, 0, 0, c.scale};
+  SumArgs a{(u32)n, 0, (u32)num_rows, 0, 0, 0, c.scale};
   ScopedKernelTimer timer(ctx, KID_EMBED_GRAD, stream);
   with_unit(c.dtype, unit, [&](auto value, auto bytes) {
     typedef decltype(value) T;
     constexpr int kBytes = decltype(bytes)::value;
     if (c.out_dtype == c.dtype)
-      launch_sum<T, T, kBytes>(stream, a, plan.chunks, c.grad, stride_bytes, row_bytes, sorted, c.out, part);
+      launch_sum<T, T, kBytes>(stream, a, plan.most_chunks, c.grad, stride_bytes, row_bytes, sorted, c.out, part);
     else
-      launch_sum<T, float, kBytes>(stream, a, plan.chunks, c.grad, stride_bytes, row_bytes, sorted, c.out, part);
+      launch_sum<T, float, kBytes>(stream, a, plan.most_chunks, c.grad, stride_bytes, row_bytes, sorted, c.out, part);
   });
   GSB_LAUNCH_OK();
-  if (plan.chunks > 1) {
-    const dim3 grid(grid_for(plan.chunks - 1, kJoinWarps * kJoinSpan), grid_for(c.row_len, kJoinColumns));
-    if (c.out_dtype == GSB_F32) launch_behind(stream, k_join_rows<float>, grid, kJoinThreads, a, c.row_len, plan.chunks, sorted, part, (float*)c.out);
-    else if (c.out_dtype == GSB_F16) launch_behind(stream, k_join_rows<__half>, grid, kJoinThreads, a, c.row_len, plan.chunks, sorted, part, (__half*)c.out);
-    else launch_behind(stream, k_join_rows<__nv_bfloat16>, grid, kJoinThreads, a, c.row_len, plan.chunks, sorted, part, (__nv_bfloat16*)c.out);
+  const i64 chunks = (n + a.chunk - 1) / a.chunk;
+  if (chunks > 1) {
+    const dim3 grid(grid_for(chunks - 1, kJoinWarps * kJoinSpan), grid_for(c.row_len, kJoinColumns));
+    if (c.out_dtype == GSB_F32) launch_behind(stream, k_join_rows<float>, grid, kJoinThreads, a, c.row_len, chunks, sorted, part, (float*)c.out);
+    else if (c.out_dtype == GSB_F16) launch_behind(stream, k_join_rows<__half>, grid, kJoinThreads, a, c.row_len, chunks, sorted, part, (__half*)c.out);
+    else launch_behind(stream, k_join_rows<__nv_bfloat16>, grid, kJoinThreads, a, c.row_len, chunks, sorted, part, (__nv_bfloat16*)c.out);
     GSB_LAUNCH_OK();
     ctx_count_launches(ctx, 1);
   }
@@ -437,7 +446,7 @@ extern "C" int gsb_embedding_grad(gsb_ctx* ctx, void* stream_, const void* grad,
   if (st != GSB_OK) return st;
   Pieces p(workspace);
   p.take<char>(plan.sort_bytes);
-  float* part = p.take<float>((size_t)plan.chunks * 2 * (size_t)row_len);
+  float* part = p.take<float>((size_t)plan.most_chunks * 2 * (size_t)row_len);
   return sum_sorted(ctx, stream, GradCall{grad, dtype, row_len, grad_stride, scale, out, out_dtype}, plan, sorted, n, num_rows,
                     part);
 }
@@ -466,7 +475,7 @@ extern "C" int gsb_embedding_grad_rows(gsb_ctx* ctx, void* stream_, const void* 
   GSB_REQUIRE(workspace_bytes >= (int64_t)plan.total_bytes, GSB_ERR_CAPACITY);
   Pieces p(workspace);
   p.take<char>(plan.sort_bytes);
-  float* part = p.take<float>((size_t)plan.chunks * 2 * (size_t)row_len);
+  float* part = p.take<float>((size_t)plan.most_chunks * 2 * (size_t)row_len);
   const u64* sorted;
   SortCall call{KeySource{ids, n, num_rows, has_padding != 0, padding_id, ctx_counters(ctx)}, SORT_RANKS};
   call.distinct = out_ids;

@@ -171,75 +171,59 @@ __global__ void __launch_bounds__(kRowThreads) k_combine_rows(const RowArgs a, u
   }
 }
 
-// A group of lanes takes neighbouring slots at a time: one of rows in units of 16 bytes (two cost warps: 62 us for 58), two of
-// narrower ones.  The gradient of a token's output is read once per slot, from L1 or L2 after the first time.
-template <class T, int BYTES>
-constexpr int grad_slots() { return BYTES == 16 ? 1 : 2; }
-
+// A group of lanes takes a slot at a time (two cost warps: rows of 100 halves 34 us for 32).  The gradient of a token's output is
+// read once per slot, from L1 or L2 after the first time.
 template <class T, int BYTES, int STEPS, bool DOTS>
 __global__ void __launch_bounds__(kRowThreads) k_combine_grad(const RowArgs a, const Unit<T, BYTES>* __restrict__ grad,
                                                               const Unit<T, BYTES>* __restrict__ rows,
                                                               Unit<T, BYTES>* __restrict__ grad_rows, void* grad_weights) {
-  constexpr int N = Unit<T, BYTES>::N, kSlots = grad_slots<T, BYTES>();
+  constexpr int N = Unit<T, BYTES>::N;
   await_previous();
   const int lane = threadIdx.x & (a.lanes - 1);
-  const u32 step = gridDim.x * (kRowThreads / a.lanes) * kSlots;
+  const u32 step = gridDim.x * (kRowThreads / a.lanes);
   // all groups of a warp take part in the sums over lanes, also those that have run out of slots
-  for (u32 base = (blockIdx.x * kRowThreads + (threadIdx.x & ~31u)) / a.lanes * kSlots; base < a.slots; base += step) {
-    const u32 slot = base + (threadIdx.x & 31) / a.lanes * kSlots;
-    int p[kSlots];
-    float w[kSlots], dot[kSlots] = {};
-    const Unit<T, BYTES>* g_of[kSlots];
-#pragma unroll
-    for (int r = 0; r < kSlots; ++r) {
-      p[r] = slot + r < a.slots ? place_of(a, slot + r, lane == 0) : kNowhere;
-      w[r] = p[r] >= 0 ? weight_at<T>(a, slot + r) : 0.f;
-      g_of[r] = grad + (i64)((slot + r) / a.per_token) * a.token_stride;
-    }
+  for (u32 base = (blockIdx.x * kRowThreads + (threadIdx.x & ~31u)) / a.lanes; base < a.slots; base += step) {
+    const u32 slot = base + (threadIdx.x & 31) / a.lanes;
+    const int p = slot < a.slots ? place_of(a, slot, lane == 0) : kNowhere;
+    const float w = p >= 0 ? weight_at<T>(a, slot) : 0.f;
+    const Unit<T, BYTES>* g_of = grad + (i64)(slot / a.per_token) * a.token_stride;
+    const Unit<T, BYTES>* v_of = rows + (p >= 0 ? p : 0) * a.row_stride;
+    Unit<T, BYTES>* to = grad_rows + (i64)(p < 0 ? ~p : p) * a.units;
+    float dot = 0.f;
     for (int j = lane; j < a.units; j += a.lanes * STEPS) {
-      Unit<T, BYTES> g[kSlots][STEPS], v[kSlots][STEPS];
+      Unit<T, BYTES> g[STEPS], v[STEPS];
+      if (p >= 0)
 #pragma unroll
-      for (int r = 0; r < kSlots; ++r)
-        if (p[r] >= 0)
-#pragma unroll
-          for (int s = 0; s < STEPS; ++s)
-            if (j + s * a.lanes < a.units) {
-              if (DOTS) v[r][s] = load_unit_once(rows + p[r] * a.row_stride + j + s * a.lanes);
-              g[r][s] = load_unit(g_of[r] + j + s * a.lanes);
-            }
-#pragma unroll
-      for (int r = 0; r < kSlots; ++r) {
-        if (p[r] == kNowhere) continue;
-        Unit<T, BYTES>* to = grad_rows + (i64)(p[r] < 0 ? ~p[r] : p[r]) * a.units + j;
-#pragma unroll
-        for (int s = 0; s < STEPS; ++s) {
-          if (j + s * a.lanes >= a.units) continue;
-          Unit<T, BYTES> u;
-          u.clear();
-          if (p[r] >= 0) {
-            float f[N], h[N];
-            g[r][s].get(f);
-            if (DOTS) {
-              v[r][s].get(h);
-#pragma unroll
-              for (int q = 0; q < N; ++q) dot[r] += f[q] * h[q];
-            }
-#pragma unroll
-            for (int q = 0; q < N; ++q) f[q] *= w[r];
-            u.set(f);
+        for (int s = 0; s < STEPS; ++s)
+          if (j + s * a.lanes < a.units) {
+            if (DOTS) v[s] = load_unit_once(v_of + j + s * a.lanes);
+            g[s] = load_unit(g_of + j + s * a.lanes);
           }
-          if (grad_rows) store_unit_once(to + s * a.lanes, u);
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+        if (p == kNowhere || j + s * a.lanes >= a.units) continue;
+        Unit<T, BYTES> u;
+        u.clear();
+        if (p >= 0) {
+          float f[N], h[N];
+          g[s].get(f);
+          if (DOTS) {
+            v[s].get(h);
+#pragma unroll
+            for (int q = 0; q < N; ++q) dot += f[q] * h[q];
+          }
+#pragma unroll
+          for (int q = 0; q < N; ++q) f[q] *= w;
+          u.set(f);
         }
+        if (grad_rows) store_unit_once(to + j + s * a.lanes, u);
       }
     }
     if (!DOTS) continue;
-#pragma unroll
-    for (int r = 0; r < kSlots; ++r) {
-      for (int o = a.lanes / 2; o > 0; o >>= 1) dot[r] += __shfl_xor_sync(0xffffffffu, dot[r], o);
-      if (lane != 0 || slot + r >= a.slots) continue;
-      if (a.weight_kind == WEIGHTS_FLOAT) ((float*)grad_weights)[slot + r] = dot[r];
-      else ((T*)grad_weights)[slot + r] = from_float<T>(dot[r]);
-    }
+    for (int o = a.lanes / 2; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+    if (lane != 0 || slot >= a.slots) continue;
+    if (a.weight_kind == WEIGHTS_FLOAT) ((float*)grad_weights)[slot] = dot;
+    else ((T*)grad_weights)[slot] = from_float<T>(dot);
   }
 }
 
@@ -379,8 +363,8 @@ extern "C" int gsb_expert_combine_grad(gsb_ctx* ctx, void* stream_, const void* 
     const RowArgs a = row_args(ctx, tokens, per_token, num_rows, shape, units, grad_stride * size / B, rows_stride * size / B, place,
                                weights, weights_dtype);
     with_steps(shape.steps, [&](auto steps) {
-      constexpr int S = decltype(steps)::value, kSlots = grad_slots<T, B>();
-      const int grid = (int)min((i64)kNumSMs * 32, (i64)grid_for((tokens * per_token + kSlots - 1) / kSlots * a.lanes, kRowThreads));
+      constexpr int S = decltype(steps)::value;
+      const int grid = (int)min((i64)kNumSMs * 32, (i64)grid_for(tokens * per_token * a.lanes, kRowThreads));
       auto kernel = out_grad_weights ? k_combine_grad<T, B, S, true> : k_combine_grad<T, B, S, false>;
       launch_behind(stream, kernel, grid, kRowThreads, a, (const Unit<T, B>*)grad, (const Unit<T, B>*)rows,
                     (Unit<T, B>*)out_grad_rows, out_grad_weights);

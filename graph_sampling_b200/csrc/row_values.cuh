@@ -141,13 +141,14 @@ inline RowShape row_shape(int64_t units, int wanted) {
   }
   return best;
 }
-// What copies and combines rows does well with two units of 16 bytes a lane, or four smaller ones (rows of 256 bytes spread in 30
-// us, with one unit a lane in 49; rows of 200 bytes combined in 32 and 43); what sums them, which has more to do per row and
-// lane, with one of 16 bytes (rows of 256 bytes 83 us, with two 98).
+// What copies and combines rows does well with two units of 16 bytes a lane, or four smaller ones (65 528 rows of 2 KB combined in 28
+// us, with one unit a lane in 34; 314 602 rows of 200 bytes in 26, with two units of 8 bytes in 30); what sums them, which has
+// more to do per row and lane, with one of 16 bytes or four of 4 (1 000 003 rows of 256 bytes 81 us, with two units 96; 1.3 M
+// rows of 100 bytes 51, with one unit 83).
 inline int copy_steps(int unit) { return unit == 16 ? 2 : 4; }
 inline int sum_steps(int unit) { return unit >= 16 ? 1 : unit == 8 ? 2 : 4; }
-// Rows that a group of lanes has on their way at once.  More of them cost warps: with twice as many combine took 45 us for 30,
-// spread 169 for 153, sums 104 for 83.
+// Rows that a group of lanes has on their way at once.  More of them cost warps: with twice as many 65 528 rows of 2 KB were spread
+// in 29 us for 25, 314 602 of 200 bytes in 33 for 26.
 constexpr int rows_ahead(int steps) { return steps == 1 ? 4 : 2; }
 
 template <class F>
