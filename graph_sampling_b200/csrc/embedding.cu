@@ -20,8 +20,6 @@ constexpr int kLookupThreads = 256;
 // Narrow units: more rows (1 000 000 rows of 602 bf16 435 us for 474), but not with four units a lane (1.3 M of 50 bf16 53 for 56).
 constexpr int lookup_rows(int unit, int steps) { return unit < 16 && steps < 4 ? 4 : rows_ahead(steps); }
 
-// A group of lanes takes neighbouring rows of the result, a tile of their columns at a time: all its reads are on their way before
-// anything is written.
 struct LookupArgs {
   const i64* ids;
   u32 n;
@@ -33,6 +31,9 @@ struct LookupArgs {
   i64* counters;
 };
 
+// A group of lanes takes neighbouring rows of the result, a tile of their columns at a time: all its reads are on their way before
+// anything is written.  Bound by DRAM with rows in no order: 1 000 000 rows of 1 204 bytes out of 2.45 M in 452 us, 5.3 TB/s of what
+// is read and written.
 template <class T, int BYTES, int STEPS>
 __global__ void __launch_bounds__(kLookupThreads) k_lookup_rows(const LookupArgs a, const Unit<T, BYTES>* __restrict__ table,
                                                                 Unit<T, BYTES>* __restrict__ out) {
@@ -113,7 +114,8 @@ __device__ __forceinline__ bool usable(const SumArgs& a, u64 pair) {
   return pair_key(pair) < a.num_rows && pair_at(pair) < a.n;
 }
 
-// One group of lanes per chunk and column tile (blockIdx.y) of lanes * STEPS units.
+// One group of lanes per chunk and column tile (blockIdx.y) of lanes * STEPS units.  Bound by DRAM: 3.65 M rows of 512 bytes summed
+// into 1.3 M in 428 us, 5.9 TB/s; 900 000 rows of 256 bytes into 0.79 M in 80, 5.4 TB/s.
 template <class T, class O, int BYTES, int STEPS>
 __global__ void __launch_bounds__(kSumThreads) k_sum_rows(const SumArgs a, const Unit<T, BYTES>* __restrict__ grad,
                                                           const u64* __restrict__ sorted, O* __restrict__ out,

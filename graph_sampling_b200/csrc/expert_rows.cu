@@ -6,6 +6,9 @@
 // Combine: out[t, :] = sum over k of w[t, k] * rows[place[t, k], :], slots without an expert left out.
 // Combine's gradient: spread of the output's gradient for the rows, and for w[t, k] the product <grad[t, :], rows[place[t, k], :]>.
 // Spread's gradient is a combine.  Sums are in float, in the order of k; each result is rounded once.
+//
+// All are bound by DRAM: 500 000 rows of 1 KB spread in 151 us and combined in 158, 6.8 and 6.5 TB/s; 65 528 rows of 2 KB from and to
+// 8 191 tokens spread in 25 us (6.0), combined in 28 (4.9, rows in no order), both with the weights' gradients in 50 (5.4).
 #include <type_traits>
 
 #include "key_sort.cuh"
@@ -19,7 +22,8 @@ constexpr int kRowThreads = 256;
 
 enum { WEIGHTS_NONE, WEIGHTS_FLOAT, WEIGHTS_OF_ROWS };
 
-// All counts are below 2^31: 32-bit arithmetic, of which there is more in these kernels than of the rows' values if one lets it.
+// All counts are below 2^31: with 64-bit arithmetic there was more of that than of the rows' values (314 602 rows of 200 bytes spread in
+// 45 us for 26).
 struct RowArgs {
   u32 tokens, per_token, slots, num_rows;
   int lanes, units;                  // per group; per row

@@ -10,7 +10,11 @@
 // as wide as keeps the number of passes small: 11 bits where few CTAs have to read each other's counts, 9 where up to 148 do.
 //
 // The launch may also clear memory (the rows of a dense gradient that no position has), with bulk copies of zeros from shared
-// memory: SMs without a sorting CTA clear all the time, the sorting CTAs of a large sort start some between their steps.
+// memory: SMs without a sorting CTA clear all the time, the others between the steps of the sort or behind it.
+//
+// What bounds it: instruction issue and the latencies of a pass's steps, not memory (1 000 003 positions by 27 bits, three passes
+// and the ranks of the distinct keys: 64 us, DRAM at 2 % of its peak, half of the issue slots used).  Of a pass of 17 us ranking
+// takes 6, the counts of all CTAs 4, the placing 4, two barriers 3.
 #include "key_sort.cuh"
 
 #include "grid_sync.cuh"
@@ -26,11 +30,13 @@ constexpr int kClusterThreads = 512, kGridThreads = 1024;
 constexpr int kRounds = 8;
 constexpr int kClusterCtas = 8;
 constexpr int kClearingClusters = 15;  // beside the one that sorts: two per GPC are resident
-constexpr int kAloneShares = 4;  // up to 2 048 positions one CTA sorts for itself, in shared memory
+// Up to 1 024 positions one CTA sorts for itself: 17 bits of 1 024 in 6.5 us, shared by two CTAs in 7.2; of 2 048 in 8.6 and 8.2.
+constexpr int kAloneShares = 2;
 constexpr int kClusterBits = 11, kGridBits = 9;
+constexpr int kMinBits = 5;  // a row of counts is read in pieces of 16 bytes
 constexpr int kMaxBins = 1 << kClusterBits;
 constexpr int kPiece = 16384;      // bytes cleared by one bulk copy
-constexpr int kPiecesAtOnce = 32;  // at most, started by a sorting CTA between two steps: about what its SM writes meanwhile
+constexpr int kPiecesAtOnce = 32;  // at most, that a sorting CTA starts between two steps
 constexpr u32 kAllLanes = 0xffffffffu;
 
 struct SortArgs {
@@ -121,8 +127,8 @@ __device__ __forceinline__ u32 scan_threads(u32 v, u32* s_scan) {
 }
 
 // Ranks of the items that a warp holds (round by round, lane by lane) among those of the same digit; `counts`, cleared, becomes the
-// warp's counts.  Lanes with the same digit are found bit by bit, by a vote each (the match instruction takes as long as
-// there are different digits).  mine: the thread's first item, of `items`.
+// warp's counts.  Lanes with the same digit are found bit by bit, by a vote each: with the match instruction 1 000 003 positions
+// take 72 us for 64, 16 384 take 16.6 for 14.7.  mine: the thread's first item, of `items`.
 template <int ROUNDS>
 __device__ __forceinline__ void rank_items(const u32 (&key)[ROUNDS], u32 (&rank)[ROUNDS], unsigned short* counts, int shift,
                                            int bits, int rounds, u32 mine, u32 items) {
@@ -612,7 +618,11 @@ struct Plan {
 
 Plan plan_of(i64 n, i64 num_keys) {
   Plan p;
-  p.cluster = n <= (i64)kClusterCtas * kClusterThreads * kRounds;
+  int bits = 1;  // of the largest key, num_keys itself
+  while (bits < 32 && (num_keys >> bits) != 0) ++bits;
+  // The cluster's passes are short and may be fewer, the grid has more SMs to rank with: one pass over 32 768 positions takes 12.4
+  // us in the grid and 15.1 in the cluster, two take 20.6 and 20.9; over 16 384 two take 20.6 and 14.7.
+  p.cluster = n <= (i64)kClusterCtas * kClusterThreads * (bits <= kClusterBits ? kRounds / 2 : kRounds);
   const i64 threads = p.threads(), shares = (n + threads - 1) / threads;
   const i64 most_ctas = !p.cluster ? kNumSMs : shares <= kAloneShares ? 1 : kClusterCtas;
   const i64 per = (shares + most_ctas - 1) / most_ctas;
@@ -621,12 +631,10 @@ Plan plan_of(i64 n, i64 num_keys) {
   p.single = per <= kRounds;
   const i64 tiles = (per + kRounds - 1) / kRounds;  // of a stretch, about equal
   p.rounds = (int)((per + tiles - 1) / tiles);
-  int bits = 1;  // of the largest key, num_keys itself
-  while (bits < 32 && (num_keys >> bits) != 0) ++bits;
   const int most = p.cluster ? kClusterBits : kGridBits;
   p.passes = (bits + most - 1) / most;
   p.digit = (bits + p.passes - 1) / p.passes;
-  if (p.digit < 5) p.digit = 5;  // a row of counts is read in pieces of 16 bytes
+  if (p.digit < kMinBits) p.digit = kMinBits;
   return p;
 }
 
@@ -698,9 +706,11 @@ int key_sort(gsb_ctx* ctx, cudaStream_t stream, const SortCall& call, void* work
   if (pairs) *pairs = p.cluster || ((p.passes + (call.result == SORT_RANKS ? 1 : 0)) & 1) ? a.to : a.from;
   const i64 pieces = (i64)((call.zero_bytes + kPiece - 1) / kPiece);
   const size_t smem = p.smem(pieces > 0);
-  // a sorting CTA clears as it goes: its share of the pieces over the steps of its passes
-  const i64 steps = p.passes * (1 + ((i64)p.stretch + p.threads() * p.rounds - 1) / (p.threads() * p.rounds));
-  a.pieces = (int)min((i64)kPiecesAtOnce, (pieces / kNumSMs + steps - 1) / steps);
+  // A sorting CTA with one tile clears as it goes, its share of the pieces over the steps of its passes (500 000 positions and 256
+  // MB 73 us, with all of it behind the sort 76).  With more tiles the writes hold the sort up by as much as they take (4.05 M
+  // and 1.25 GB 382 us, 371 with all of it behind).
+  const i64 steps = p.passes * 2;
+  a.pieces = p.single ? (int)min((i64)kPiecesAtOnce, (pieces / kNumSMs + steps - 1) / steps) : 0;
   if (p.cluster) {  // CTAs that clear come in clusters too, as many as the GPU holds at once
     const i64 more = min((pieces + kClusterCtas - 1) / kClusterCtas, (i64)kClearingClusters) * kClusterCtas;
     return launch(ctx, stream, a, true, (int)(kClusterCtas + more), smem);

@@ -1,8 +1,9 @@
 // Launches that may overlap the end of the kernel before them in their stream.
 //
 // A kernel launched by `launch_behind` is set up while its predecessor still runs and waits at `await_previous`, its first
-// statement, until that one is complete and its writes are visible: the order of the stream, without the microseconds
-// between two kernels (2.5 instead of 4.1 us a kernel for those of up to 2 us).  Captured, it becomes a programmatic edge.
+// statement, until that one is complete and its writes are visible: the order of the stream, without the microseconds between
+// two kernels.  Kernels of 2.5 us, one behind the other, take 3.0 us each and 4.1 without; the six of a training step over 16 384
+// tokens 63 us for 70, the five of a step to 64 experts 142 for 152.  Captured, it becomes a programmatic edge.
 #pragma once
 #include <type_traits>
 

@@ -119,7 +119,7 @@ SHAPES = [(1, 1, 1, "same"), (2, 1, 7, "same"), (31, 7, 3, "uniform"), (33, 40, 
           (70_001, 70_000, 8, "uniform"), (300_007, 1_000_000, 4, "skewed"), (300_007, 4, 130, "skewed"), (4096, 300, 2056, "skewed"),
           (600_000, 2, 1, "uniform"), (1_300_000, 9000, 3, "skewed"), (2_500_000, 300_000, 2, "uniform"),
           # one CTA, a cluster, the grid: the last of the one and the first of the next
-          (2048, 500, 4, "uniform"), (2049, 500, 4, "uniform"), (32_768, 70_000, 4, "uniform"), (32_769, 70_000, 4, "uniform")]
+          (1024, 5000, 4, "uniform"), (1025, 5000, 4, "uniform"), (2048, 500, 4, "uniform"), (2049, 500, 4, "uniform"), (32_768, 70_000, 4, "uniform"), (32_769, 70_000, 4, "uniform")]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

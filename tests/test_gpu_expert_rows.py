@@ -44,7 +44,7 @@ def same_order(got, want):
 # ---- order -----------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("shape,experts", [((1,), 1), ((1, 1), 7), ((3, 2), 8), ((16, 2), 8), ((255,), 3), ((257, 8), 64), ((1000, 1), 256),
                                            ((2047, 4), 255), ((4097,), 1000), ((5000, 6), 2048), ((8191, 8), 64), ((40_000,), 5000), ((70_001,), 65_536),
-                                           ((300_000, 2), 4), ((2_000_000,), 12)])
+                                           ((300_000, 2), 4), ((2_000_000,), 12), ((1024,), 30), ((1025,), 30), ((16_384,), 100), ((16_385,), 100)])
 def test_order(ops, shape, experts):
     g = generator(experts)
     ids = draw(g, shape, experts)
