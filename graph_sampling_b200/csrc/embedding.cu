@@ -367,6 +367,12 @@ static int check_grad(i64 n, i64 num_rows, i64 row_len, i64 grad_stride, int dty
   return GSB_OK;
 }
 
+// What they ask of addresses.
+static bool aligned_grad(const void* grad, int dtype, const i64* ids, const void* out, int out_dtype, const void* workspace) {
+  return aligned_to(value_bytes(dtype), (const char*)grad) && aligned_to(8, ids) && aligned_to(value_bytes(out_dtype), (const char*)out) &&
+         aligned_to(256, (const char*)workspace);
+}
+
 }  // namespace gsb
 
 using namespace gsb;
@@ -379,6 +385,7 @@ extern "C" int gsb_embedding_lookup(gsb_ctx* ctx, void* stream_, const void* tab
                   value_bytes(dtype) != 0, GSB_ERR_INVALID_ARGUMENT);
   if (n == 0) return GSB_OK;
   GSB_REQUIRE((table || num_rows == 0) && ids && out, GSB_ERR_INVALID_ARGUMENT);
+  GSB_REQUIRE(aligned_to(value_bytes(dtype), (const char*)table, (const char*)out) && aligned_to(8, ids), GSB_ERR_INVALID_ARGUMENT);
   const void* from = nullptr;
   if (num_rows > 0) {  // device memory, or page-locked host memory by the address that the device uses for it
     cudaPointerAttributes attr;
@@ -427,7 +434,7 @@ extern "C" int gsb_embedding_grad(gsb_ctx* ctx, void* stream_, const void* grad,
   int st = check_grad(n, num_rows, row_len, grad_stride, dtype, out_dtype);
   if (st != GSB_OK) return st;
   if (num_rows == 0 && n == 0) return GSB_OK;
-  GSB_REQUIRE(out || num_rows == 0, GSB_ERR_INVALID_ARGUMENT);
+  GSB_REQUIRE((out || num_rows == 0) && aligned_grad(grad, dtype, ids, out, out_dtype, workspace), GSB_ERR_INVALID_ARGUMENT);
   cudaStream_t stream = (cudaStream_t)stream_;
   const size_t out_bytes = (size_t)num_rows * (size_t)row_len * value_bytes(out_dtype);
   if (n == 0) {
@@ -474,6 +481,8 @@ extern "C" int gsb_embedding_grad_rows(gsb_ctx* ctx, void* stream_, const void* 
   }
   const GradPlan plan = grad_plan(n, num_rows, row_len);
   GSB_REQUIRE(grad && ids && out_ids && out_rows && workspace, GSB_ERR_INVALID_ARGUMENT);
+  GSB_REQUIRE(aligned_grad(grad, dtype, ids, out_rows, out_dtype, workspace) && aligned_to(8, out_ids, out_count),
+              GSB_ERR_INVALID_ARGUMENT);
   GSB_REQUIRE(workspace_bytes >= (int64_t)plan.total_bytes, GSB_ERR_CAPACITY);
   Pieces p(workspace);
   p.take<char>(plan.sort_bytes);

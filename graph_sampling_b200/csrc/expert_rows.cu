@@ -239,6 +239,8 @@ static int check_rows(i64 tokens, i64 per_token, i64 row_len, int dtype, i64 str
               GSB_ERR_INVALID_ARGUMENT);
   GSB_REQUIRE(tokens == 0 || place, GSB_ERR_INVALID_ARGUMENT);
   GSB_REQUIRE(!weights || weights_dtype == dtype || weights_dtype == GSB_F32, GSB_ERR_INVALID_ARGUMENT);
+  GSB_REQUIRE(aligned_to(8, (const char*)place) && (!weights || aligned_to(value_bytes(weights_dtype), (const char*)weights)),
+              GSB_ERR_INVALID_ARGUMENT);
   return GSB_OK;
 }
 
@@ -270,6 +272,8 @@ extern "C" int gsb_expert_order(gsb_ctx* ctx, void* stream_, const int64_t* expe
     return GSB_OK;
   }
   GSB_REQUIRE(experts && out_source && out_place && workspace, GSB_ERR_INVALID_ARGUMENT);
+  GSB_REQUIRE(aligned_to(8, experts, out_offsets, out_source, out_place) && aligned_to(256, (const char*)workspace),
+              GSB_ERR_INVALID_ARGUMENT);
   GSB_REQUIRE(workspace_bytes >= need, GSB_ERR_CAPACITY);
   SortCall call{KeySource{experts, n, num_experts, true, -1, ctx_counters(ctx)}, SORT_ORDER};
   call.offsets = out_offsets;
@@ -286,9 +290,9 @@ extern "C" int gsb_expert_spread(gsb_ctx* ctx, void* stream_, const void* x, int
   const int st = check_rows(tokens, per_token, row_len, dtype, x_stride, place, weights, weights_dtype);
   if (st != GSB_OK) return st;
   if (tokens == 0) return GSB_OK;
-  GSB_REQUIRE(x && out_rows, GSB_ERR_INVALID_ARGUMENT);
-  cudaStream_t stream = (cudaStream_t)stream_;
   const int size = value_bytes(dtype);
+  GSB_REQUIRE(x && out_rows && aligned_to(size, (const char*)x, (const char*)out_rows), GSB_ERR_INVALID_ARGUMENT);
+  cudaStream_t stream = (cudaStream_t)stream_;
   const int unit = unit_bytes(row_len * size, (u64)(uintptr_t)x | (u64)(uintptr_t)out_rows | (u64)(x_stride * size));
   ScopedKernelTimer timer(ctx, KID_EXPERT_ROWS, stream);
   with_unit(dtype, unit, [&](auto value, auto bytes) {
@@ -318,9 +322,9 @@ extern "C" int gsb_expert_combine(gsb_ctx* ctx, void* stream_, const void* rows,
   if (st != GSB_OK) return st;
   GSB_REQUIRE(num_rows >= 0 && num_rows <= tokens * per_token, GSB_ERR_INVALID_ARGUMENT);
   if (tokens == 0) return GSB_OK;
-  GSB_REQUIRE((rows || num_rows == 0) && out, GSB_ERR_INVALID_ARGUMENT);
-  cudaStream_t stream = (cudaStream_t)stream_;
   const int size = value_bytes(dtype);
+  GSB_REQUIRE((rows || num_rows == 0) && out && aligned_to(size, (const char*)rows, (const char*)out), GSB_ERR_INVALID_ARGUMENT);
+  cudaStream_t stream = (cudaStream_t)stream_;
   const int unit = unit_bytes(row_len * size, (u64)(uintptr_t)rows | (u64)(uintptr_t)out | (u64)(rows_stride * size));
   ScopedKernelTimer timer(ctx, KID_EXPERT_ROWS, stream);
   with_unit(dtype, unit, [&](auto value, auto bytes) {
@@ -355,6 +359,9 @@ extern "C" int gsb_expert_combine_grad(gsb_ctx* ctx, void* stream_, const void* 
   GSB_REQUIRE(grad && (!out_grad_weights || (weights && (rows || num_rows == 0))), GSB_ERR_INVALID_ARGUMENT);
   cudaStream_t stream = (cudaStream_t)stream_;
   const int size = value_bytes(dtype);
+  GSB_REQUIRE(aligned_to(size, (const char*)grad, (const char*)rows, (const char*)out_grad_rows) &&
+                  (!out_grad_weights || aligned_to(value_bytes(weights_dtype), (const char*)out_grad_weights)),
+              GSB_ERR_INVALID_ARGUMENT);
   u64 addresses = (u64)(uintptr_t)grad | (u64)(uintptr_t)out_grad_rows | (u64)(grad_stride * size);
   if (out_grad_weights) addresses |= (u64)(uintptr_t)rows | (u64)(rows_stride * size);
   const int unit = unit_bytes(row_len * size, addresses);

@@ -13,6 +13,7 @@
 #include <torch/csrc/autograd/variable.h>
 
 #include <limits>
+#include <mutex>
 #include <optional>
 #include <utility>
 
@@ -37,6 +38,9 @@ struct Failed : std::runtime_error {  // a call of the C ABI
 void refuse_unless(bool ok, const char* what) {
   if (!ok) throw BadArgument(what);
 }
+void refuse_unless(bool ok, const char* name, const char* what) {
+  if (!ok) throw BadArgument(std::string(name) + what);
+}
 void done(gsb_ctx* ctx, int st, const char* where) {
   if (st != GSB_OK) throw Failed(st, where, gsb_last_error_message(ctx));
 }
@@ -60,22 +64,22 @@ struct Rows {
 Rows rows_of(const Tensor& t, const char* name, bool pinned_too = false) {
   Rows r;
   r.dtype = dtype_of(t, name);
-  refuse_unless(t.dim() == 2, (std::string(name) + " must have two dimensions").c_str());
-  refuse_unless(t.is_cuda() || (pinned_too && t.is_pinned()),
-                (std::string(name) + (pinned_too ? " must live on the GPU or in pinned host memory" : " must be a CUDA tensor")).c_str());
+  refuse_unless(t.dim() == 2, name, " must have two dimensions");
+  refuse_unless(t.is_cuda() || (pinned_too && t.is_pinned()), name,
+                pinned_too ? " must live on the GPU or in pinned host memory" : " must be a CUDA tensor");
   r.n = t.size(0);
   r.width = t.size(1);
   r.t = t;
   if (r.width > 1 && t.stride(1) != 1) {
-    refuse_unless(t.is_cuda(), (std::string(name) + ": rows of a pinned host tensor must be contiguous").c_str());
+    refuse_unless(t.is_cuda(), name, ": rows of a pinned host tensor must be contiguous");
     r.t = t.contiguous();
   }
   r.stride = r.n > 1 ? r.t.stride(0) : r.width;
   return r;
 }
 Tensor ids_of(const Tensor& t, const char* name) {
-  refuse_unless(t.scalar_type() == at::kLong, (std::string(name) + " must be int64").c_str());
-  refuse_unless(t.is_cuda(), (std::string(name) + " must be a CUDA tensor").c_str());
+  refuse_unless(t.scalar_type() == at::kLong, name, " must be int64");
+  refuse_unless(t.is_cuda(), name, " must be a CUDA tensor");
   return t.contiguous();
 }
 void same_device(const Tensor& a, const Tensor& b) {
@@ -165,10 +169,15 @@ std::vector<Tensor> grad_rows(gsb_ctx* ctx, const Tensor& grad_, const Tensor& i
   Tensor row_ids = empty(n, dev), rows = fresh({n, width}, g.out_type, dev), count = empty(1, dev);
   Tensor work = scratch(gsb_embedding_grad_workspace(n, num_rows, width), "gsb_embedding_grad_rows", dev);
   int64_t found = 0;
+  // the number comes back through the context, which the backward passes of several threads share
+  static std::mutex waiting;
+  std::unique_lock<std::mutex> lock(waiting, std::defer_lock);
+  if (sync) lock.lock();
   done(ctx, gsb_embedding_grad_rows(ctx, stream(), g.grad.data(), g.grad.dtype, width, g.grad.stride, ids_ptr(g.ids), n, num_rows,
                                     (float)scale, pad.given, pad.id, static_cast<int64_t*>(data(row_ids)), data(rows), g.out_dtype,
                                     static_cast<int64_t*>(data(count)), data(work), work.numel(), sync ? &found : nullptr),
        "gsb_embedding_grad_rows");
+  if (sync) lock.unlock();
   if (!sync) return {row_ids, rows, count};
   trim(row_ids, found);
   rows.unsafeGetTensorImpl()->set_sizes_contiguous({found, width});

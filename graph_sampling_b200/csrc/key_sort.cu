@@ -17,6 +17,7 @@
 // takes 6, the counts of all CTAs 4, the placing 4, two barriers 3.
 #include "key_sort.cuh"
 
+#include <atomic>
 #include <initializer_list>
 
 #include "grid_sync.cuh"
@@ -643,7 +644,7 @@ Plan plan_of(i64 n, i64 num_keys) {
 // B200, two per GPC but one): a cluster that clears and has to wait for the one that sorts comes behind it (16 384 positions and 134
 // MB in 38 us for 23).
 int prepare(gsb_ctx* ctx, int* clusters) {
-  static int known[64] = {};
+  static std::atomic<int> known[64];
   const int device = ctx_device(ctx);
   if (device >= 0 && device < 64 && known[device] > 0) {
     *clusters = known[device];

@@ -120,6 +120,12 @@ inline int unit_bytes(int64_t row_bytes, uint64_t addresses) {
   return all % 16 == 0 ? 16 : all % 8 == 0 ? 8 : all % 4 == 0 ? 4 : 2;
 }
 
+// Every address is a multiple of `bytes` (null is).
+template <class... P>
+bool aligned_to(int bytes, const P*... p) {
+  return (((uint64_t)(uintptr_t)p | ...) & (uint64_t)(bytes - 1)) == 0;
+}
+
 // How a row is taken: by `lanes` neighbouring lanes (a power of two up to 32), `steps` units (1 .. 4) of each at a time.  Of the shapes
 // that take the row at once the one that leaves the fewest lanes idle; among equals the one whose steps are nearest to
 // `wanted`.  Rows of more than 96 units go in tiles of 32 lanes with two units each.

@@ -33,7 +33,8 @@ def dispatch(x, place):
 
 
 def combine(rows, place, weights=None):
-    """Sum over k of weights[t, k] * rows[place[t, k]], with gradients for rows and weights."""
+    """Sum over k of weights[t, k] * rows[place[t, k]], with gradients for rows and weights.  `place` as in dispatch: no row of
+    two slots."""
     place = getattr(place, "place", place)
     ctx = ops._context_for(place)
     return ctx.native.nn_combine(ctx.address, rows, place, weights)

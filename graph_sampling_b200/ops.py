@@ -456,14 +456,15 @@ def expert_order(expert_ids, num_experts, ctx=None):
 
 def expert_dispatch(x, place, weights=None, ctx=None):
     """rows[place[t, k], :] = x[t, :], times weights[t, k] where given → one row per slot; zeros in the rows of slots without
-    an expert.  `place` as expert_order gives it."""
+    an expert.  `place` as expert_order gives it: no row of two slots."""
     ctx = _context_for(place, ctx)
     return ctx.native.expert_dispatch(ctx.address, x, place, weights)
 
 
 def expert_combine(rows, place, weights=None, ctx=None):
     """out[t, :] = sum over k of weights[t, k] * rows[place[t, k], :] (weights float32 or of the rows' dtype, None: all 1);
-    slots without an expert are left out.  `rows` may end with the last row that an expert has."""
+    slots without an expert are left out.  `place` as expert_order gives it; `rows` may end with the last row that an expert
+    has."""
     ctx = _context_for(place, ctx)
     return ctx.native.expert_combine(ctx.address, rows, place, weights)
 

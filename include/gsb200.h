@@ -570,11 +570,11 @@ GSB_API int gsb_sage_hop_sized(gsb_ctx* ctx, void* stream, const int64_t* indptr
 
 /* ---- rows that are learned ---------------------------------------------------------------------------------------
  * No counterpart in the reference, which ends at the loaded features.  Rows of float, half or bfloat16 values (gsb_dtype),
- * of at most GSB_MAX_ROW_LEN each, one after the other with `*_stride` values from one row's start to the next (values of a row are contiguous); arithmetic
- * in float, every result rounded once.  These calls use no scratch of the context: the caller provides it (at least the
+ * of at most GSB_MAX_ROW_LEN each, one after the other with `*_stride` values from one row's start to the next (values of a row are
+ * contiguous, and every address a multiple of its type's size); arithmetic in float, every result rounded once.  These calls use no scratch of the context: the caller provides it (at least the
  * bytes that the *_workspace function of the same sizes names, 256-byte aligned), so they may be captured into a CUDA graph
  * and queued on several streams at once, each call with a workspace of its own.  Ids, experts and places out of range are
- * never followed and record GSB_ERR_INDEX_RANGE. */
+ * never followed and record GSB_ERR_INDEX_RANGE.  Threads that use them at once have a context each. */
 #define GSB_MAX_ROW_LEN 1048576
 enum gsb_dtype { GSB_F32 = 0, GSB_F16 = 1, GSB_BF16 = 2 };
 
@@ -606,9 +606,10 @@ GSB_API int64_t gsb_expert_order_workspace(int64_t n, int64_t num_experts);
 GSB_API int gsb_expert_order(gsb_ctx* ctx, void* stream, const int64_t* experts, int64_t n, int64_t num_experts,
                              int64_t* out_offsets, int64_t* out_source, int64_t* out_place, void* workspace,
                              int64_t workspace_bytes);
-/* Slot t * per_token + k is the k-th of token t; tokens * per_token is below 2^31.  Spread: out_rows[place[t, k], :] = weights[t, k] * x[t, :], zeros in the rows of
- * slots without an expert; tokens * per_token rows.  Combine: out[t, :] = sum over k of weights[t, k] * rows[place[t, k], :],
- * slots without an expert left out; place as gsb_expert_order gives it, num_rows at most tokens * per_token (fewer where the
+/* Slot t * per_token + k is the k-th of token t; tokens * per_token is below 2^31.  place: as gsb_expert_order gives it, no row of
+ * two slots.  Spread: out_rows[place[t, k], :] = weights[t, k] * x[t, :], zeros in the rows of slots without an expert;
+ * tokens * per_token rows.  Combine: out[t, :] = sum over k of weights[t, k] * rows[place[t, k], :], slots without an expert left
+ * out; num_rows at most tokens * per_token (fewer where the
  * caller leaves rows of slots without an expert away).  weights: NULL (all 1), of type dtype or GSB_F32.  The gradient of spread without weights
  * is combine without weights; that of combine is out_grad_rows = spread of grad (NULL: not wanted) and
  * out_grad_weights[t, k] = <grad[t, :], rows[place[t, k], :]> (NULL: not wanted; else of the weights' type), 0 for slots without

@@ -182,3 +182,82 @@ def test_profiling_does_not_enter_a_capture(ops):
     ctx.profile_enable(False)
     assert times["key_sort"][1] == 1 and times["embed_grad"][1] == 1 and times["key_sort"][0] > 0
     exact.within(out, *exact.sums(grad, ids, 100, 1.0, None))
+
+
+def test_large_sorts_on_several_streams_at_once(ops):
+    """More than 32 768 positions each: launches of which every one wants the whole GPU."""
+    g = generator(6)
+    jobs = []
+    for i in range(4):
+        n, rows, width = 60_000 + 50_000 * i, 20_000, 24
+        jobs.append((torch.randint(0, rows, (n,), generator=g, device="cuda"), torch.randn(n, width, generator=g, device="cuda"), rows))
+    want = [exact.sums(grad, ids, rows, 1.0, None) for ids, grad, rows in jobs]
+    streams = [torch.cuda.Stream() for _ in jobs]
+    ctx = ops.Context()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        got = []
+        for s, (ids, grad, rows) in zip(streams, jobs):
+            with torch.cuda.stream(s):
+                got.append((ops.embedding_grad(grad, ids, rows, ctx=ctx), ops.expert_order(ids, rows, ctx=ctx)[1]))
+        torch.cuda.synchronize()
+        ctx.check_device()
+        for (out, source), (w, error), (ids, _, _) in zip(got, want, jobs):
+            exact.within(out, w, error)
+            assert torch.equal(source, torch.sort(ids, stable=True).indices)
+
+
+def test_threads_that_wait_for_numbers_at_once():
+    """Backward passes of several threads through one context, each with a number of rows of its own."""
+    import threading
+
+    import graph_sampling_b200.gs as gs
+    g = generator(7)
+    tables = [torch.randn(2000, 16, generator=g, device="cuda").requires_grad_() for _ in range(4)]
+    ids = [torch.randint(0, 100 * (i + 1), (3000,), generator=g, device="cuda") for i in range(4)]
+    gs.nn.embedding(tables[0], ids[0])
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(30):
+                grad, = torch.autograd.grad(gs.nn.embedding(tables[i], ids[i], sparse=True).sum(), tables[i])
+                if not torch.equal(grad.indices()[0], torch.unique(ids[i])):
+                    wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(120)
+    assert not any(t.is_alive() for t in threads) and not wrong
+
+
+@pytest.mark.parametrize("dtype,code", [(torch.float32, 0), (torch.bfloat16, 2)])
+def test_addresses_that_no_tensor_has_are_refused(ops, dtype, code):
+    """Nothing is launched for an address that is not a multiple of its type's size, or for a workspace off its boundary."""
+    ctx, refused = ops.default_context(), -1
+    lib, h, s = ctx.lib, ctx.handle, stream()
+    ids = torch.zeros(8, dtype=torch.int64, device="cuda")
+    rows = torch.zeros(16, 8, dtype=dtype, device="cuda")
+    out = torch.full((16, 8), 5.0, dtype=dtype, device="cuda")
+    long = torch.full((32,), 5, dtype=torch.int64, device="cuda")
+    work = torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
+    r, o, i, q, w, size = rows.data_ptr(), out.data_ptr(), ids.data_ptr(), long.data_ptr(), work.data_ptr(), 1 << 19
+    for a, b, c in ((1, 0, 0), (0, 1, 0), (0, 0, 4)):
+        assert lib.gsb_embedding_lookup(h, s, r + a, code, 8, 8, 8, i + c, 4, 1.0, 0, 0, o + b) == refused
+        assert lib.gsb_expert_spread(h, s, r + a, code, 4, 2, 8, 8, i + c, None, 0, o + b) == refused
+        assert lib.gsb_expert_combine(h, s, r + a, code, 8, 4, 2, 8, 8, i + c, None, 0, o + b) == refused
+        assert lib.gsb_expert_combine_grad(h, s, r + a, code, 4, 2, 8, 8, r, 8, 8, i + c, None, 0, o + b, None) == refused
+    for a, b, c, d in ((1, 0, 0, 0), (0, 1, 0, 0), (0, 0, 4, 0), (0, 0, 0, 16)):
+        assert lib.gsb_embedding_grad(h, s, r + a, code, 8, 8, i + c, 4, 8, 1.0, 0, 0, o + b, code, w + d, size) == refused
+        assert lib.gsb_embedding_grad_rows(h, s, r + a, code, 8, 8, i + c, 4, 8, 1.0, 0, 0, q, o + b, code, q + 128, w + d, size,
+                                           None) == refused
+    for a, d in ((4, 0), (0, 16)):
+        assert lib.gsb_expert_order(h, s, i + a, 4, 4, q, q + 64, q + 128, w + d, size) == refused
+    weights = r                                                       # of the rows' type, off by a byte
+    assert lib.gsb_expert_spread(h, s, r, code, 4, 2, 8, 8, i, weights + 1, code, o) == refused
+    assert lib.gsb_expert_combine_grad(h, s, r, code, 4, 2, 8, 8, r, 8, 8, i, weights, code, o, o + 1) == refused
+    assert torch.all(out == 5) and torch.all(long == 5)
+    ctx.check_device()
