@@ -5,7 +5,8 @@
 // positions within pieces that depend on sizes alone, so the same inputs give the same bits; one rounding.  The positions are
 // sorted by id (key_sort.cuh); the sorted list is cut into chunks of equal length whoever the ids are, so a frequent id is
 // shared by many groups of lanes.  A sum that begins and ends inside a chunk is written at once; what reaches over a chunk's
-// ends goes to `part` and is added up by k_join_rows.
+// ends goes to `part` and is added up by k_join_rows.  Rows without a sum are cleared beside the sort, or, where that would write
+// much twice, by k_join_rows.
 #include <type_traits>
 
 #include "key_sort.cuh"
@@ -109,6 +110,7 @@ struct SumArgs {
   int units;     // per row
   i64 stride;    // of `grad`, in units
   float scale;
+  u32* summed;  // a bit per row of the result: it has a sum; null: they are not asked for
 };
 __device__ __forceinline__ bool usable(const SumArgs& a, u64 pair) {
   return pair_key(pair) < a.num_rows && pair_at(pair) < a.n;
@@ -116,7 +118,8 @@ __device__ __forceinline__ bool usable(const SumArgs& a, u64 pair) {
 
 // One group of lanes per chunk and column tile (blockIdx.y) of lanes * STEPS units.  Bound by DRAM: 3.65 M rows of 512 bytes summed
 // into 1.3 M in 428 us, 5.9 TB/s; 900 000 rows of 256 bytes into 0.79 M in 80, 5.4 TB/s.
-template <class T, class O, int BYTES, int STEPS>
+// MARK: a.summed is wanted.
+template <class T, class O, int BYTES, int STEPS, bool MARK>
 __global__ void __launch_bounds__(kSumThreads) k_sum_rows(const SumArgs a, const Unit<T, BYTES>* __restrict__ grad,
                                                           const u64* __restrict__ sorted, O* __restrict__ out,
                                                           float* __restrict__ part) {
@@ -150,6 +153,7 @@ __global__ void __launch_bounds__(kSumThreads) k_sum_rows(const SumArgs a, const
   u64 p[kAhead + 1], next[kAhead + 1];
 #pragma unroll
   for (int u = 0; u <= kAhead; ++u) p[u] = u < left ? __ldg(sorted + u) : ~0ull;
+  u32 bits = 0;  // of the rows that ended and have the latest one's word
   for (u32 j = 0; j < mine; j += kAhead) {
     Unit<T, BYTES> v[kAhead][STEPS];
 #pragma unroll
@@ -179,6 +183,13 @@ __global__ void __launch_bounds__(kSumThreads) k_sum_rows(const SumArgs a, const
       if (ends && !head) put(out + (i64)row * width, a.scale);
       else if (ends || j + u + 1 == mine) put(part + (head ? 0 : width), 1.f);
       if (ends) head = false;
+      if (!MARK) continue;
+      const u32 after = pair_key(p[u + 1]);
+      if (ends) bits |= 1u << (row & 31);
+      if (bits != 0 && (j + u + 1 == mine || after >= a.num_rows || after >> 5 != row >> 5)) {
+        if (first == 0) atomicOr(a.summed + (row >> 5), bits);
+        bits = 0;
+      }
     }
 #pragma unroll
     for (int u = 0; u <= kAhead; ++u) p[u] = next[u];
@@ -192,8 +203,36 @@ __global__ void __launch_bounds__(kSumThreads) k_sum_rows(const SumArgs a, const
 constexpr int kJoinThreads = 512, kJoinWarps = kJoinThreads / 32, kJoinSpan = 4, kJoinSteps = 4, kJoinColumns = 32 * kJoinSteps;
 constexpr int kJoinShort = 32;
 
+// Rows without a sum, 16 bytes at a time, by warps: 32 rows each, or a piece of their columns.
+struct ClearArgs {
+  uint4* out;
+  u32 units;    // of 16 bytes, per row
+  u32 pieces;   // of kClearPiece units, per row
+  u32 per_row;  // 2^32 / units, rounded up
+};
+constexpr u32 kClearPiece = 1024;
+
+__device__ __forceinline__ void clear_rows(const ClearArgs& c, const u32* __restrict__ summed, u32 num_rows, i64 number, i64 of) {
+  const int lane = threadIdx.x & 31;
+  const i64 all = (i64)((num_rows - 1) / 32 + 1) * c.pieces;
+  for (i64 item = number; item < all; item += of) {
+    const u32 word = (u32)(c.pieces == 1 ? item : item / c.pieces), used = __ldg(summed + word), rows = min(32u, num_rows - word * 32);
+    if (used == 0xffffffffu) continue;
+    uint4* to = c.out + (i64)word * 32 * c.units;
+    if (c.units < 32) {  // several rows at a time
+      for (u32 q = lane; q < rows * c.units; q += 32)
+        if (!(used >> __umulhi(q, c.per_row) & 1u)) to[q] = make_uint4(0, 0, 0, 0);
+    } else {
+      const u32 begin = (u32)(item - (i64)word * c.pieces) * kClearPiece, end = min(c.units, begin + kClearPiece);
+      for (u32 r = 0; r < rows; ++r)
+        if (!(used >> r & 1u))
+          for (u32 q = begin + lane; q < end; q += 32) to[(i64)r * c.units + q] = make_uint4(0, 0, 0, 0);
+    }
+  }
+}
+
 template <class O>
-__global__ void __launch_bounds__(kJoinThreads) k_join_rows(const SumArgs a, i64 width, i64 chunks,
+__global__ void __launch_bounds__(kJoinThreads) k_join_rows(const SumArgs a, const ClearArgs clear, i64 width, i64 chunks,
                                                             const u64* __restrict__ sorted, const float* __restrict__ part,
                                                             O* __restrict__ out) {
   __shared__ int s_long;
@@ -205,6 +244,10 @@ __global__ void __launch_bounds__(kJoinThreads) k_join_rows(const SumArgs a, i64
   const i64 column = (i64)blockIdx.y * kJoinColumns + lane;
   if (threadIdx.x == 0) s_long = 0;
   __syncthreads();
+  if (a.summed) {
+    const i64 number = ((i64)blockIdx.y * gridDim.x + blockIdx.x) * kJoinWarps + warp, of = (i64)gridDim.x * gridDim.y * kJoinWarps;
+    clear_rows(clear, a.summed, a.num_rows, number, of);
+  }
   float sum[kJoinSteps];
   auto add = [&](i64 from, i64 n, i64 step) {  // head parts of n chunks, `step` apart
 #pragma unroll 8
@@ -287,7 +330,10 @@ static i64 sum_chunk(i64 n, int lanes, i64 tiles) {
 struct GradPlan {
   size_t sort_bytes, total_bytes;
   i64 most_chunks;  // that there is room for
+  size_t words;     // a bit per row of the result, where they may be wanted
 };
+
+static bool may_clear_behind(i64 n, i64 num_rows, i64 row_bytes) { return min(n, num_rows) * row_bytes >= 200000000; }
 
 static GradPlan grad_plan(i64 n, i64 num_rows, i64 row_len) {
   GradPlan g;
@@ -298,6 +344,8 @@ static GradPlan grad_plan(i64 n, i64 num_rows, i64 row_len) {
   Pieces p(nullptr);
   p.take<char>(g.sort_bytes);
   p.take<float>((size_t)g.most_chunks * 2 * (size_t)row_len);
+  g.words = may_clear_behind(n, num_rows, row_len * 4) ? ((size_t)num_rows + 31) / 32 : 0;
+  p.take<u32>(g.words);
   g.total_bytes = p.used;
   return g;
 }
@@ -315,8 +363,11 @@ static void launch_sum(cudaStream_t stream, SumArgs& a, i64 most_chunks, const v
   a.chunk = (u32)max(sum_chunk(n, shape.lanes, tiles), (n + most_chunks - 1) / most_chunks);
   with_steps(shape.steps, [&](auto steps) {
     const dim3 grid(grid_for((n + a.chunk - 1) / a.chunk * a.lanes, kSumThreads), tiles);
-    launch_behind(stream, k_sum_rows<T, O, BYTES, decltype(steps)::value>, grid, kSumThreads, a, (const Unit<T, BYTES>*)grad, sorted,
-                  (O*)out, part);
+    constexpr int S = decltype(steps)::value;
+    auto kernel = k_sum_rows<T, O, BYTES, S, false>;
+    if constexpr (BYTES == 16)
+      if (a.summed) kernel = k_sum_rows<T, O, BYTES, S, true>;
+    launch_behind(stream, kernel, grid, kSumThreads, a, (const Unit<T, BYTES>*)grad, sorted, (O*)out, part);
   });
 }
 
@@ -329,14 +380,31 @@ struct GradCall {
   int out_dtype;
 };
 
+// The gradient's rows are read and the result's written in units of this many bytes of the former.
+static int unit_of(const GradCall& c) {
+  const int size = value_bytes(c.dtype), out_size = value_bytes(c.out_dtype);
+  int unit = unit_bytes(c.row_len * size, (u64)(uintptr_t)c.grad | (u64)(c.grad_stride * size));
+  while (unit > size && (uintptr_t)c.out % min(16, unit / size * out_size) != 0) unit /= 2;
+  return unit;
+}
+
+// Whether the rows without a sum are cleared behind the sums, which mark the others; if not, the sort clears all rows on its way.
+// What is saved is at most min(n, num_rows) rows; lost is what the sort hides and, of a small table, what would have stayed in L2.
+// 4.05 M positions into 2.45 M rows of 512 bytes take 781 us for 931, 1 M into 2.5 M of 1 KB 0.85 of the time, into 1 M of 256 bytes
+// 0.93, but 100 000 into 250 000 of 1 KB up to 1.09. Rows that share lines of 128 bytes with others cost more to clear one by
+// one than together (1 M into 2.5 M of 400 bytes 1.07).
+static bool clears_behind(const GradCall& c, i64 n, i64 num_rows) {
+  const i64 row_bytes = c.row_len * value_bytes(c.out_dtype);
+  return row_bytes % 128 == 0 && (uintptr_t)c.out % 128 == 0 && unit_of(c) == 16 && may_clear_behind(n, num_rows, row_bytes);
+}
+
 // Sums of the rows at the sorted positions, into the rows of `out` that the pairs name.
 static int sum_sorted(gsb_ctx* ctx, cudaStream_t stream, const GradCall& c, const GradPlan& plan, const u64* sorted, i64 n,
-                      i64 num_rows, float* part) {
+                      i64 num_rows, float* part, u32* summed) {
   const int size = value_bytes(c.dtype), out_size = value_bytes(c.out_dtype);
   const i64 row_bytes = c.row_len * size, stride_bytes = c.grad_stride * size;
-  int unit = unit_bytes(row_bytes, (u64)(uintptr_t)c.grad | (u64)stride_bytes);
-  while (unit > size && (uintptr_t)c.out % min(16, unit / size * out_size) != 0) unit /= 2;
-  SumArgs a{(u32)n, 0, (u32)num_rows, 0, 0, 0, c.scale};
+  const int unit = unit_of(c);
+  SumArgs a{(u32)n, 0, (u32)num_rows, 0, 0, 0, c.scale, summed};
   ScopedKernelTimer timer(ctx, KID_EMBED_GRAD, stream);
   with_unit(c.dtype, unit, [&](auto value, auto bytes) {
     typedef decltype(value) T;
@@ -348,11 +416,18 @@ static int sum_sorted(gsb_ctx* ctx, cudaStream_t stream, const GradCall& c, cons
   });
   GSB_LAUNCH_OK();
   const i64 chunks = (n + a.chunk - 1) / a.chunk;
-  if (chunks > 1) {
-    const dim3 grid(grid_for(chunks - 1, kJoinWarps * kJoinSpan), grid_for(c.row_len, kJoinColumns));
-    if (c.out_dtype == GSB_F32) launch_behind(stream, k_join_rows<float>, grid, kJoinThreads, a, c.row_len, chunks, sorted, part, (float*)c.out);
-    else if (c.out_dtype == GSB_F16) launch_behind(stream, k_join_rows<__half>, grid, kJoinThreads, a, c.row_len, chunks, sorted, part, (__half*)c.out);
-    else launch_behind(stream, k_join_rows<__nv_bfloat16>, grid, kJoinThreads, a, c.row_len, chunks, sorted, part, (__nv_bfloat16*)c.out);
+  if (chunks > 1 || summed) {
+    dim3 grid(grid_for(chunks - 1, kJoinWarps * kJoinSpan), grid_for(c.row_len, kJoinColumns));
+    ClearArgs clear{(uint4*)c.out, 0, 0, 0};
+    if (summed) {
+      clear.units = (u32)(c.row_len * out_size / 16);
+      clear.pieces = (clear.units + kClearPiece - 1) / kClearPiece;
+      clear.per_row = (u32)(((1ull << 32) + clear.units - 1) / clear.units);
+      grid.x = max(grid.x, (unsigned)min(kNumSMs * 4, grid_for((i64)plan.words * clear.pieces, kJoinWarps)) / grid.y);
+    }
+    if (c.out_dtype == GSB_F32) launch_behind(stream, k_join_rows<float>, grid, kJoinThreads, a, clear, c.row_len, chunks, sorted, part, (float*)c.out);
+    else if (c.out_dtype == GSB_F16) launch_behind(stream, k_join_rows<__half>, grid, kJoinThreads, a, clear, c.row_len, chunks, sorted, part, (__half*)c.out);
+    else launch_behind(stream, k_join_rows<__nv_bfloat16>, grid, kJoinThreads, a, clear, c.row_len, chunks, sorted, part, (__nv_bfloat16*)c.out);
     GSB_LAUNCH_OK();
     ctx_count_launches(ctx, 1);
   }
@@ -444,20 +519,22 @@ extern "C" int gsb_embedding_grad(gsb_ctx* ctx, void* stream_, const void* grad,
   const GradPlan plan = grad_plan(n, num_rows, row_len);
   GSB_REQUIRE(grad && ids && workspace, GSB_ERR_INVALID_ARGUMENT);
   GSB_REQUIRE(workspace_bytes >= (int64_t)plan.total_bytes, GSB_ERR_CAPACITY);
+  Pieces p(workspace);
+  p.take<char>(plan.sort_bytes);
+  float* part = p.take<float>((size_t)plan.most_chunks * 2 * (size_t)row_len);
+  u32* summed = p.take<u32>(plan.words);
+  const GradCall c{grad, dtype, row_len, grad_stride, scale, out, out_dtype};
+  if (!clears_behind(c, n, num_rows)) summed = nullptr;
   const u64* sorted;
   {
     ScopedKernelTimer timer(ctx, KID_KEY_SORT, stream);
     SortCall call{KeySource{ids, n, num_rows, has_padding != 0, padding_id, ctx_counters(ctx)}, SORT_PAIRS};
-    call.zero = out;
-    call.zero_bytes = out_bytes;
+    call.zero = summed ? (void*)summed : out;
+    call.zero_bytes = summed ? plan.words * sizeof(u32) : out_bytes;
     st = key_sort(ctx, stream, call, workspace, &sorted);
   }
   if (st != GSB_OK) return st;
-  Pieces p(workspace);
-  p.take<char>(plan.sort_bytes);
-  float* part = p.take<float>((size_t)plan.most_chunks * 2 * (size_t)row_len);
-  return sum_sorted(ctx, stream, GradCall{grad, dtype, row_len, grad_stride, scale, out, out_dtype}, plan, sorted, n, num_rows,
-                    part);
+  return sum_sorted(ctx, stream, c, plan, sorted, n, num_rows, part, summed);
 }
 
 extern "C" int gsb_embedding_grad_rows(gsb_ctx* ctx, void* stream_, const void* grad, int dtype, int64_t row_len,
@@ -497,7 +574,7 @@ extern "C" int gsb_embedding_grad_rows(gsb_ctx* ctx, void* stream_, const void* 
     st = key_sort(ctx, stream, call, workspace, &sorted);
   }
   if (st != GSB_OK) return st;
-  st = sum_sorted(ctx, stream, GradCall{grad, dtype, row_len, grad_stride, scale, out_rows, out_dtype}, plan, sorted, n, n, part);
+  st = sum_sorted(ctx, stream, GradCall{grad, dtype, row_len, grad_stride, scale, out_rows, out_dtype}, plan, sorted, n, n, part, nullptr);
   if (st != GSB_OK || !count_host) return st;
   return ctx_mail_result(ctx, stream, call.mail, 1, count_host);
 }

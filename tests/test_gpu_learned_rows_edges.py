@@ -261,3 +261,34 @@ def test_addresses_that_no_tensor_has_are_refused(ops, dtype, code):
     assert lib.gsb_expert_combine_grad(h, s, r, code, 4, 2, 8, 8, r, 8, 8, i, weights, code, o, o + 1) == refused
     assert torch.all(out == 5) and torch.all(long == 5)
     ctx.check_device()
+
+
+@pytest.mark.parametrize("n,rows,width,dtype,kind", [
+    (500_000, 410_007, 128, torch.float32, "spread"), (1_700_000, 1_600_005, 32, torch.float32, "spread"),
+    (900_001, 2_000_000, 128, torch.bfloat16, "front"), (1500, 1700, 36_032, torch.float32, "spread"),
+    (600_000, 420_000, 192, torch.bfloat16, "hub"), (420_000, 420_000, 128, torch.float32, "last"),
+    (420_000, 420_000, 128, torch.float32, "none"), (100_000, 98_000, 2048, torch.float16, "front")])
+def test_rows_without_a_sum_in_large_gradients(ops, n, rows, width, dtype, kind):
+    """More than 200 MB of rows: zeros wherever no position is, whatever was in the memory before."""
+    g = generator(8)
+    ids = torch.randint(0, rows, (n,), generator=g, device="cuda")
+    if kind == "front":
+        ids //= 64
+    elif kind == "hub":
+        ids = torch.where(ids % 3 > 0, 77_777, ids)
+    elif kind == "last":
+        ids = torch.full_like(ids, rows - 1)
+    elif kind == "none":
+        ids = torch.full_like(ids, 5)
+    grad = torch.randint(-3, 4, (n, width), generator=g, device="cuda").to(dtype)
+    for scale, pad in ((1.0, 5), (0.5, None)):
+        before = torch.full((rows, width), float("nan"), dtype=dtype, device="cuda")
+        del before                                         # whose memory the result gets
+        out = ops.embedding_grad(grad, ids, rows, scale, pad)
+        keep = torch.ones_like(ids, dtype=torch.bool) if pad is None else ids != pad
+        want = torch.zeros(rows, width, device="cuda").index_add_(0, ids[keep], grad[keep].float()) * scale
+        assert torch.equal(out, want.to(dtype))            # sums of small integers: exact in float, one rounding
+        again = ops.embedding_grad(grad, ids, rows, scale, pad)
+        assert torch.equal(out, again)
+        del out, want, again
+    torch.cuda.empty_cache()
