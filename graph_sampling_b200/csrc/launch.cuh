@@ -17,10 +17,11 @@ __device__ __forceinline__ void await_previous() {
 }
 
 template <class... P, class... A>
-cudaError_t launch_behind(cudaStream_t stream, void (*kernel)(P...), dim3 grid, int threads, A... args) {
+cudaError_t launch_behind_with(cudaStream_t stream, size_t smem, void (*kernel)(P...), dim3 grid, int threads, A... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -28,6 +29,10 @@ cudaError_t launch_behind(cudaStream_t stream, void (*kernel)(P...), dim3 grid, 
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+template <class... P, class... A>
+cudaError_t launch_behind(cudaStream_t stream, void (*kernel)(P...), dim3 grid, int threads, A... args) {
+  return launch_behind_with(stream, 0, kernel, grid, threads, args...);
 }
 
 }  // namespace gsb

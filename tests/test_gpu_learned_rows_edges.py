@@ -292,3 +292,35 @@ def test_rows_without_a_sum_in_large_gradients(ops, n, rows, width, dtype, kind)
         assert torch.equal(out, again)
         del out, want, again
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("width,n", [(301, 40_000), (601, 20_000), (1433, 7000), (2047, 4999), (4095, 2100), (4097, 2100)])
+@pytest.mark.parametrize("shift,gap", [(0, 0), (1, 0), (3, 1), (5, 7)])
+def test_large_lookups_of_odd_rows(ops, dtype, width, n, shift, gap):
+    """16 MB and more of rows whose values are no whole words, from tables that begin and end anywhere; nothing is written around."""
+    g = generator(9)
+    rows, stride = 501, width + gap
+    ctx = ops.Context()
+    room = torch.randn(shift + rows * stride, generator=g, device="cuda").to(dtype)
+    table = room[shift:].as_strided((rows, width), (stride, 1))
+    ids = torch.randint(0, rows, (n,), generator=g, device="cuda")
+    ids[:4] = torch.tensor([0, rows - 1, -1, 0])
+    ids[-3:] = torch.tensor([rows - 1, 7, 0])
+    for scale, pad in ((1.0, None), (0.5, 7)):
+        guard = torch.full((n * width + 16,), 7.0, dtype=dtype, device="cuda")
+        out = guard[shift:shift + n * width].view(n, width)
+        code = 1 if dtype == torch.float16 else 2
+        assert ctx.lib.gsb_embedding_lookup(ctx.handle, stream(), table.data_ptr(), code, rows, width, stride, ids.data_ptr(), n, scale,
+                                            int(pad is not None), pad or 0, out.data_ptr()) == 0
+        want = table[ids.clamp(0)] * scale                     # exact: a power of two
+        want[ids < 0] = 0
+        if pad is not None:
+            want[ids == pad] = 0
+        assert torch.equal(out, want)
+        assert torch.all(guard[:shift] == 7) and torch.all(guard[shift + n * width:] == 7)
+        with pytest.raises(Exception):
+            ctx.check_device()                                 # id -1
+    out = ops.embedding_lookup(table, ids.clamp(0), ctx=ctx)
+    assert torch.equal(out, table[ids.clamp(0)])
+    ctx.check_device()
