@@ -7,14 +7,15 @@
 // written from CTA to CTA, the barrier is the hardware's, and nothing waits for global memory between the ids and the result.
 // More go through global memory (k_sort_grid), tile by tile through shared memory so that neighbouring threads write
 // neighbouring words, by CTAs that are launched cooperatively and meet at a word in the workspace (grid_sync.cuh).  Digits are
-// as wide as keeps the number of passes small: 11 bits where few CTAs have to read each other's counts, 9 where up to 148 do.
+// as wide as keeps the number of passes small: 11 bits where few CTAs have to read each other's counts, 10 or 9 where up to 148 do.
+// A kernel for each width: with the width as an argument passes took 5 to 15 % longer (500 000 by 64 experts 16.7 us for 15.1).
 //
 // The launch may also clear memory (the rows of a dense gradient that no position has), with bulk copies of zeros from shared
 // memory: SMs without a sorting CTA clear all the time, the others between the steps of the sort or behind it.
 //
 // What bounds it: instruction issue and the latencies of a pass's steps, not memory (1 000 003 positions by 27 bits, three passes
-// and the ranks of the distinct keys: 64 us, DRAM at 2 % of its peak, half of the issue slots used).  Of a pass of 17 us ranking
-// takes 6, the counts of all CTAs 4, the placing 4, two barriers 3.
+// and the ranks of the distinct keys: 64 us between two events, DRAM at 2 % of its peak, half of the issue slots used).  Ranking takes a
+// third of a pass, the counts of all CTAs and the placing a quarter each, two barriers the rest.
 #include "key_sort.cuh"
 
 #include <atomic>
@@ -34,7 +35,10 @@ constexpr int kRounds = 8;
 constexpr int kClusterCtas = 8;
 // Up to 1 024 positions one CTA sorts for itself: 17 bits of 1 024 in 6.5 us, shared by two CTAs in 7.2; of 2 048 in 8.6 and 8.2.
 constexpr int kAloneShares = 2;
-constexpr int kClusterBits = 11, kGridBits = 9;
+constexpr int kClusterBits = 11, kGridBits = 10;
+// Ten bits make one pass of two for up to 1 023 keys (a million positions 23.1 us for 37.5), or save a pass of few positions (200 000 by
+// 20 bits 45.4 for 47.6); of many, two wide passes cost more than three narrow ones (4 M by 20 bits 437 for 416, a million the same).
+constexpr i64 kFewPositions = 600000;
 constexpr int kMinBits = 5;  // a row of counts is read in pieces of 16 bytes
 constexpr int kMaxBins = 1 << kClusterBits;
 constexpr int kPiece = 16384;      // bytes cleared by one bulk copy
@@ -46,7 +50,7 @@ struct SortArgs {
   u64 *from, *to;  // [key : 32 | position : 32], exchanged after every pass
   u32* counts;     // CTAs x bins
   int ctas;        // that sort; the others clear
-  int passes, digit;
+  int passes;
   u32 stretch;     // positions per CTA
   int rounds;      // of a tile: a position per thread each
   bool single;     // a stretch is one tile, which stays in registers between counting and placing
@@ -130,18 +134,19 @@ __device__ __forceinline__ u32 scan_threads(u32 v, u32* s_scan) {
 
 // Ranks of the items that a warp holds (round by round, lane by lane) among those of the same digit; `counts`, cleared, becomes the
 // warp's counts.  Lanes with the same digit are found bit by bit, by a vote each: with the match instruction 1 000 003 positions
-// take 72 us for 64, 16 384 take 16.6 for 14.7.  mine: the thread's first item, of `items`.
-template <int ROUNDS>
+// take 75 us for 64, 4.05 M take 191 for 156.  mine: the thread's first item, of `items`.
+template <int ROUNDS, int BITS>
 __device__ __forceinline__ void rank_items(const u32 (&key)[ROUNDS], u32 (&rank)[ROUNDS], unsigned short* counts, int shift,
-                                           int bits, int rounds, u32 mine, u32 items) {
+                                           int rounds, u32 mine, u32 items) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int r = 0; r < ROUNDS; ++r) {
     if (r >= rounds) break;
     const bool valid = mine + r * 32 < items;
-    const u32 digit = (key[r] >> shift) & ((1u << bits) - 1u);
+    const u32 digit = (key[r] >> shift) & ((1u << BITS) - 1u);
     u32 peers = __ballot_sync(kAllLanes, valid);
-    for (int b = 0; b < bits; ++b) {
+#pragma unroll
+    for (int b = 0; b < BITS; ++b) {
       const u32 bit = (digit >> b) & 1u;
       peers &= __ballot_sync(kAllLanes, bit) ^ (bit - 1u);
     }
@@ -197,6 +202,7 @@ __device__ __forceinline__ void store_far(u32 address, u64 v) {
   asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(address), "l"(v) : "memory");
 }
 
+template <int DIGIT>
 __global__ void __launch_bounds__(kClusterThreads, 1) k_sort_cluster(const SortArgs a) {
   constexpr int kThreads = kClusterThreads, kWarps = kThreads / 32, kPer = (1 << kClusterBits) / kThreads;
   extern __shared__ __align__(128) char smem[];
@@ -210,7 +216,8 @@ __global__ void __launch_bounds__(kClusterThreads, 1) k_sort_cluster(const SortA
     clearing.finish();
     return;
   }
-  const int bins = 1 << a.digit, rounds = a.rounds;
+  constexpr int bins = 1 << DIGIT;
+  const int rounds = a.rounds;
   u64* s_items = (u64*)smem;                                   // the stretch: written by all CTAs
   u32* s_tile = (u32*)(s_items + rounds * kThreads);           // its counts: read by all CTAs
   u32* s_base = s_tile + bins;                                 // where the CTA's items of a digit begin
@@ -242,16 +249,16 @@ __global__ void __launch_bounds__(kClusterThreads, 1) k_sort_cluster(const SortA
   };
 
   for (int pass = 0; pass < a.passes; ++pass) {
-    const int shift = pass * a.digit;
+    const int shift = pass * DIGIT;
     load(pass == 0);
     for (int q = threadIdx.x; q < kWarps * bins / 8; q += kThreads) ((uint4*)s_count)[q] = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    rank_items<kRounds>(key, rank, s_count + warp * bins, shift, a.digit, rounds, mine, items);
+    rank_items<kRounds, DIGIT>(key, rank, s_count + warp * bins, shift, rounds, mine, items);
     __syncthreads();
     warp_starts<kThreads>(s_count, s_tile, bins);
     barrier();
     {
-      const int per = max(1, bins / kThreads);  // digits of a thread
+      constexpr int per = bins > kThreads ? bins / kThreads : 1;  // digits of a thread
       static_assert(kPer == 4, "four digits are one access");
       u32 all[kPer] = {}, before[kPer] = {};
 #pragma unroll
@@ -364,6 +371,7 @@ __global__ void k_clear_word(u64* word) {
   *word = 0;
 }
 
+template <int DIGIT>
 __global__ void __launch_bounds__(kGridThreads, 1) k_sort_grid(const SortArgs a) {
   constexpr int kThreads = kGridThreads, kWarps = kThreads / 32;
   static_assert((1 << kGridBits) <= kThreads, "a digit per thread");
@@ -372,7 +380,7 @@ __global__ void __launch_bounds__(kGridThreads, 1) k_sort_grid(const SortArgs a)
   await_previous();
   const SortCall& c = a.call;
   const u32 cta = blockIdx.x;
-  const int bins = 1 << a.digit;
+  constexpr int bins = 1 << DIGIT;
   char* s_zeros = smem;                                        // kPiece
   u64* s_items = (u64*)(smem + (c.zero_bytes > 0 ? kPiece : 0));  // a tile; also the partial sums of the counts
   u32* s_base = (u32*)((char*)s_items + a.room);               // where the next item of a digit goes
@@ -426,13 +434,13 @@ __global__ void __launch_bounds__(kGridThreads, 1) k_sort_grid(const SortArgs a)
   auto rank_tile = [&](u32 base, int shift) {
     for (int q = threadIdx.x; q < kWarps * bins / 8; q += kThreads) ((uint4*)s_count)[q] = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    rank_items<kRounds>(key, rank, s_count + warp * bins, shift, a.digit, rounds, mine, hi - base);
+    rank_items<kRounds, DIGIT>(key, rank, s_count + warp * bins, shift, rounds, mine, hi - base);
     __syncthreads();
     warp_starts<kThreads>(s_count, s_tile, bins);
   };
 
   for (int pass = 0; pass < a.passes; ++pass) {
-    const int shift = pass * a.digit;
+    const int shift = pass * DIGIT;
     const bool ids = pass == 0, last = pass == a.passes - 1;
     // counts of the stretch
     u32* row = a.counts + (size_t)cta * bins;
@@ -622,9 +630,10 @@ Plan plan_of(i64 n, i64 num_keys) {
   Plan p;
   int bits = 1;  // of the largest key, num_keys itself
   while (bits < 32 && (num_keys >> bits) != 0) ++bits;
-  // The cluster's passes are short and may be fewer, the grid has more SMs to rank with: one pass over 32 768 positions takes 12.4
-  // us in the grid and 15.1 in the cluster, two take 20.6 and 20.9; over 16 384 two take 20.6 and 14.7.
-  p.cluster = n <= (i64)kClusterCtas * kClusterThreads * (bits <= kClusterBits ? kRounds / 2 : kRounds);
+  // The cluster's passes are short and may be fewer, the grid has more SMs to rank with: one pass over 32 768 positions takes 11.0
+  // us in the grid and 14.7 in the cluster, over 16 384 12.4 and 12.4; two passes and the ranks over 32 768 31.3 and 29.5; and by 11
+  // bits, of which the grid makes two passes, 20.8 and 17.9.
+  p.cluster = n <= (i64)kClusterCtas * kClusterThreads * (bits <= kGridBits ? kRounds / 2 : kRounds);
   const i64 threads = p.threads(), shares = (n + threads - 1) / threads;
   const i64 most_ctas = !p.cluster ? kNumSMs : shares <= kAloneShares ? 1 : kClusterCtas;
   const i64 per = (shares + most_ctas - 1) / most_ctas;
@@ -633,11 +642,23 @@ Plan plan_of(i64 n, i64 num_keys) {
   p.single = per <= kRounds;
   const i64 tiles = (per + kRounds - 1) / kRounds;  // of a stretch, about equal
   p.rounds = (int)((per + tiles - 1) / tiles);
-  const int most = p.cluster ? kClusterBits : kGridBits;
+  const int most = p.cluster ? kClusterBits : bits <= kGridBits || n <= kFewPositions ? kGridBits : kGridBits - 1;
   p.passes = (bits + most - 1) / most;
   p.digit = (bits + p.passes - 1) / p.passes;
   if (p.digit < kMinBits) p.digit = kMinBits;
   return p;
+}
+
+// By the width of a digit; null where a kernel does not use it.
+const void* kernel_of(bool cluster, int digit) {
+  static const void* const in_cluster[] = {(const void*)k_sort_cluster<5>, (const void*)k_sort_cluster<6>, (const void*)k_sort_cluster<7>,
+                                           (const void*)k_sort_cluster<8>, (const void*)k_sort_cluster<9>, (const void*)k_sort_cluster<10>,
+                                           (const void*)k_sort_cluster<11>};
+  static const void* const in_grid[] = {(const void*)k_sort_grid<5>, (const void*)k_sort_grid<6>, (const void*)k_sort_grid<7>,
+                                        (const void*)k_sort_grid<8>, (const void*)k_sort_grid<9>, (const void*)k_sort_grid<10>};
+  static_assert(kMinBits == 5 && kClusterBits == 11 && kGridBits == 10, "the lists above");
+  if (digit < kMinBits || digit > (cluster ? kClusterBits : kGridBits)) return nullptr;
+  return cluster ? in_cluster[digit - kMinBits] : in_grid[digit - kMinBits];
 }
 
 // Once per device: the kernels may use as much shared memory as they need, and how many clusters are resident at once (15 on a
@@ -650,8 +671,10 @@ int prepare(gsb_ctx* ctx, int* clusters) {
     *clusters = known[device];
     return GSB_OK;
   }
-  for (const void* kernel : {(const void*)k_sort_cluster, (const void*)k_sort_grid})
-    GSB_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared));
+  for (int digit = kMinBits; digit <= kClusterBits + kGridBits; ++digit) {
+    const void* kernel = digit <= kClusterBits ? kernel_of(true, digit) : kernel_of(false, digit - kClusterBits);
+    if (kernel) GSB_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared));
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(kNumSMs / kClusterCtas * kClusterCtas);
   cfg.blockDim = dim3(kClusterThreads);
@@ -662,14 +685,14 @@ int prepare(gsb_ctx* ctx, int* clusters) {
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  GSB_CUDA_OK(cudaOccupancyMaxActiveClusters(clusters, k_sort_cluster, &cfg));
+  GSB_CUDA_OK(cudaOccupancyMaxActiveClusters(clusters, kernel_of(true, kClusterBits), &cfg));
   if (*clusters < 2) *clusters = 2;  // one that clears there has to be
   if (device >= 0 && device < 64) known[device] = *clusters;
   return GSB_OK;
 }
 
-int launch(gsb_ctx* ctx, cudaStream_t stream, SortArgs& a, bool cluster, int grid, size_t smem) {
-  const void* kernel = cluster ? (const void*)k_sort_cluster : (const void*)k_sort_grid;
+int launch(gsb_ctx* ctx, cudaStream_t stream, SortArgs& a, bool cluster, int digit, int grid, size_t smem) {
+  const void* kernel = kernel_of(cluster, digit);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid);
   cfg.blockDim = dim3(cluster ? kClusterThreads : kGridThreads);
@@ -718,7 +741,6 @@ int key_sort(gsb_ctx* ctx, cudaStream_t stream, const SortCall& call, void* work
   a.to = w.take<u64>((size_t)n);
   a.ctas = p.ctas;
   a.passes = p.passes;
-  a.digit = p.digit;
   a.stretch = p.stretch;
   a.rounds = p.rounds;
   a.single = p.single;
@@ -740,11 +762,11 @@ int key_sort(gsb_ctx* ctx, cudaStream_t stream, const SortCall& call, void* work
   if (st != GSB_OK) return st;
   if (p.cluster) {  // CTAs that clear come in clusters too, as many as the GPU holds beside the one that sorts
     const i64 more = min((pieces + kClusterCtas - 1) / kClusterCtas, (i64)(clusters - 1)) * kClusterCtas;
-    return launch(ctx, stream, a, true, (int)(kClusterCtas + more), smem);
+    return launch(ctx, stream, a, true, p.digit, (int)(kClusterCtas + more), smem);
   }
   GSB_CUDA_OK(launch_behind(stream, k_clear_word, dim3(1), 1, word));
   ctx_count_launches(ctx, 1);
-  return launch(ctx, stream, a, false, (int)(p.ctas + min(pieces, (i64)(kNumSMs - p.ctas))), smem);
+  return launch(ctx, stream, a, false, p.digit, (int)(p.ctas + min(pieces, (i64)(kNumSMs - p.ctas))), smem);
 }
 
 }  // namespace gsb
