@@ -324,3 +324,34 @@ def test_large_lookups_of_odd_rows(ops, dtype, width, n, shift, gap):
     out = ops.embedding_lookup(table, ids.clamp(0), ctx=ctx)
     assert torch.equal(out, table[ids.clamp(0)])
     ctx.check_device()
+
+
+@pytest.mark.parametrize("n,keys", [(16_384, 1023), (16_385, 1023), (16_385, 1024), (32_768, 1024), (32_769, 2047), (40_000, 511),
+                                    (40_000, 512), (40_000, 1023), (40_000, 1024), (40_000, 65_536), (600_000, 65_536), (600_001, 65_536),
+                                    (1_300_000, 1023)])
+def test_widths_of_digits(ops, n, keys):
+    """Both sides of where a sort takes another digit, another number of passes, or more than one tile; the largest key is `keys`."""
+    g = generator(10)
+    ids = torch.randint(-1, keys, (n,), generator=g, device="cuda")
+    ids[:2] = torch.tensor([keys - 1, -1])
+    offsets, source, place = ops.expert_order(ids, keys)
+    key = torch.where(ids < 0, keys, ids)
+    want = torch.sort(key, stable=True).indices
+    assert torch.equal(source, want) and torch.equal(offsets[1:], torch.bincount(key, minlength=keys + 1)[:keys].cumsum(0))
+    row = torch.empty_like(want)
+    row[want] = torch.arange(n, device="cuda")
+    assert int(offsets[0]) == 0 and torch.equal(place, torch.where(ids < 0, ~row, row))
+
+
+@pytest.mark.parametrize("n", [900, 30_000, 599_999, 600_001])
+@pytest.mark.parametrize("bits", [1, 10, 11, 19, 20, 21, 22, 28, 30, 32])
+def test_widths_of_ids(ops, n, bits):
+    g = generator(bits)
+    rows = min(2 ** bits, 2 ** 32 - 2) - (1 if bits < 32 else 0)
+    ids = torch.randint(0, rows, (n,), generator=g, device="cuda")
+    ids[:2] = torch.tensor([rows - 1, 0])
+    grad = torch.randint(-3, 4, (n, 2), generator=g, device="cuda").float()
+    row_ids, got = ops.embedding_grad_rows(grad, ids, rows)
+    unique, at = torch.unique(ids, return_inverse=True)
+    assert torch.equal(row_ids, unique)
+    assert torch.equal(got, torch.zeros_like(got).index_add_(0, at, grad))     # sums of small integers are exact
