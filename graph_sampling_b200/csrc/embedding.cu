@@ -32,15 +32,18 @@ struct LookupArgs {
   i64* counters;
 };
 
+// LANES: 32, or 0 for a.lanes.  Known, and with rows that are copied as they are apart, they pay where a unit is one value of 16 bits (a
+// million rows of 101 values 124 us for 180, of 251 255 for 321), but not where there are fewer to take (500 000 of 1 434 748 for 555).
+//
 // A group of lanes takes neighbouring rows of the result, a tile of their columns at a time: all its reads are on their way before
 // anything is written.  Bound by DRAM with rows in no order: 1 000 000 rows of 1 204 bytes out of 2.45 M in 452 us, 5.3 TB/s of what
 // is read and written.
-template <class T, int BYTES, int STEPS>
+template <class T, int BYTES, int STEPS, int LANES>
 __global__ void __launch_bounds__(kLookupThreads) k_lookup_rows(const LookupArgs a, const Unit<T, BYTES>* __restrict__ table,
                                                                 Unit<T, BYTES>* __restrict__ out) {
   constexpr int kRows = lookup_rows(BYTES, STEPS), N = Unit<T, BYTES>::N;
   await_previous();
-  const int lane = threadIdx.x & (a.lanes - 1), lanes = a.lanes;
+  const int lanes = LANES > 0 ? LANES : a.lanes, lane = threadIdx.x & (lanes - 1);
   const u32 step = gridDim.x * (kLookupThreads / lanes) * kRows;
   for (u32 i = (blockIdx.x * kLookupThreads + threadIdx.x) / lanes * kRows; i < a.n; i += step) {
     const Unit<T, BYTES>* from[kRows];  // null: zeros
@@ -54,6 +57,33 @@ __global__ void __launch_bounds__(kLookupThreads) k_lookup_rows(const LookupArgs
       else if (lane == 0 && blockIdx.y == 0) raise_error(a.counters, GSB_ERR_INDEX_RANGE, i + r);
     }
     Unit<T, BYTES>* to = out + (i64)i * a.units;
+    bool plain = LANES > 0 && a.scale == 1.f && i + kRows <= a.n;  // copied as they are
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) plain = plain && from[r];
+    if (plain) {
+      const Unit<T, BYTES>* p[kRows];
+      Unit<T, BYTES>* q[kRows];
+      int j = blockIdx.y * lanes * STEPS + lane;
+      const int stride = gridDim.y * lanes * STEPS;
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) p[r] = from[r] + j, q[r] = to + (i64)r * a.units + j;
+      for (; j < a.units; j += stride) {
+        Unit<T, BYTES> v[kRows][STEPS];
+#pragma unroll
+        for (int r = 0; r < kRows; ++r)
+#pragma unroll
+          for (int s = 0; s < STEPS; ++s)
+            if (j + s * lanes < a.units) v[r][s] = load_unit(p[r] + s * lanes);
+#pragma unroll
+        for (int r = 0; r < kRows; ++r)
+#pragma unroll
+          for (int s = 0; s < STEPS; ++s)
+            if (j + s * lanes < a.units) store_unit(q[r] + s * lanes, v[r][s]);
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) p[r] += stride, q[r] += stride;
+      }
+      continue;
+    }
     for (int j = blockIdx.y * lanes * STEPS + lane; j < a.units; j += gridDim.y * lanes * STEPS) {
       Unit<T, BYTES> v[kRows][STEPS];
 #pragma unroll
@@ -86,12 +116,12 @@ __global__ void __launch_bounds__(kLookupThreads) k_lookup_rows(const LookupArgs
 }
 
 // Rows of 16-bit values that begin off the 4-byte boundaries, where a unit is one value: a warp copies the next rows into shared
-// memory in units of 16 bytes, from the boundary before a row to the one behind it, and writes them out in words.  300 000 rows
-// of 1 433 values 334 us for 506, a million of 601 493 for 725; but a million of 251 357 for 319, each row's steps being the same, and
-// 4 000 of 1 433 take as long.  With two or four rows on their way instead of three, rows of 2 002 bytes take 305 or 277 us for 298,
-// of 6 002 696 or 883 for 644.  (Where units of 4 bytes fit, nothing is gained: 1 204 bytes 474 us for 455.)
+// memory in units of 16 bytes, from the boundary before a row to the one behind it, and writes whole units of the result, each out
+// of two that it straddles.  A short row's steps cost more than it gains: 500 000 of 601 values 243 us for 352, 100 000 of 1 433
+// 108 for 169, but 500 000 of 301 167 for 155 and 30 000 of 501 15 for 13.  (Where units of 4 bytes fit, little is gained: a million
+// rows of 1 204 bytes 479 us for 456, of 2 868 bytes 1 026 for 1 115.)
 constexpr int kStagedThreads = 128, kStages = 3;
-static bool staged(i64 row_bytes, i64 n) { return row_bytes >= 600 && row_bytes <= 8192 && n * row_bytes >= 16 << 20; }
+static bool staged(i64 row_bytes, i64 n) { return row_bytes >= 800 && row_bytes <= 8192 && n * row_bytes >= 32000000; }
 
 struct StagedArgs {
   const char* begin;  // of the table
@@ -102,7 +132,9 @@ struct StagedArgs {
 };
 
 template <class T>
-__global__ void __launch_bounds__(kStagedThreads) k_lookup_staged(const LookupArgs a, const StagedArgs s, Unit<T, 2>* __restrict__ out) {
+__global__ void __launch_bounds__(kStagedThreads) k_lookup_staged(const LookupArgs a, const StagedArgs s, T* __restrict__ out) {
+  typedef Unit<T, (int)sizeof(T)> Value;
+  typedef Unit<T, 16> Wide;
   extern __shared__ __align__(16) char smem[];
   await_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -120,7 +152,7 @@ __global__ void __launch_bounds__(kStagedThreads) k_lookup_staged(const LookupAr
   i64 now = look(lane), then = look(32 + lane);
   auto from_of = [&](u32 r, u32 base) {  // null: zeros
     const i64 id = __shfl_sync(0xffffffffu, r - base < 32 ? now : then, (int)(r & 31));
-    return id < 0 ? nullptr : s.begin + id * a.stride * 2;
+    return id < 0 ? nullptr : s.begin + id * a.stride;
   };
   auto start = [&](u32 r, u32 base) {
     const char* from = from_of(r, base);
@@ -154,9 +186,7 @@ __global__ void __launch_bounds__(kStagedThreads) k_lookup_staged(const LookupAr
     asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
     __syncwarp();
     const char* from = from_of(r, base);
-    // the row in words of its place in `out`, and a value in front of them and behind them
-    Unit<T, 2>* to = out + (i64)(first + r) * a.units;
-    const int head = (int)((uintptr_t)to >> 1 & 1), words = (a.units - head) / 2, behind = head + 2 * words;
+    T* to = out + (i64)(first + r) * a.units;
     const char* row = ring + (r % kStages) * s.stage + ((uintptr_t)from & 15);
     auto put = [&](auto u, auto* at) {
       if (from && a.scale != 1.f) {
@@ -168,13 +198,42 @@ __global__ void __launch_bounds__(kStagedThreads) k_lookup_staged(const LookupAr
       }
       store_unit(at, u);
     };
-    if (lane == 0 && head) put(Unit<T, 2>{from ? *(const unsigned short*)row : (unsigned short)0}, to);
-    if (lane == 1 && behind < a.units) put(Unit<T, 2>{from ? ((const unsigned short*)row)[behind] : (unsigned short)0}, to + behind);
-    const u32* of = (const u32*)((uintptr_t)(row + 2 * head) & ~(uintptr_t)3);
-    const u32 shift = (u32)((uintptr_t)(row + 2 * head) & 2) * 8;
-#pragma unroll 4
-    for (int j = lane; j < words; j += 32)
-      put(Unit<T, 4>{from ? __funnelshift_r(of[j], of[j + 1], shift) : 0u}, (Unit<T, 4>*)(to + head) + j);
+    // whole units of 16 bytes of the result, and the values in front of them and behind them
+    const int head = min(a.units, (int)((0 - (uintptr_t)to & 15) / sizeof(T))), wide = (a.units - head) / Wide::N, behind = head + wide * Wide::N;
+    const int one = lane < 16 ? (lane < head ? lane : -1) : behind + lane - 16 < a.units ? behind + lane - 16 : -1;
+    if (one >= 0) {
+      Value v;
+      v.clear();
+      if (from) v = ((const Value*)row)[one];
+      put(v, (Value*)to + one);
+    }
+    Wide* wide_to = (Wide*)(to + head);
+    row += head * sizeof(T);
+    if (!from) {
+      Wide zero;
+      zero.clear();
+      for (int j = lane; j < wide; j += 32) put(zero, wide_to + j);
+    } else {
+      const uint4* of = (const uint4*)((uintptr_t)row & ~(uintptr_t)15);
+      const u32 shift = (u32)((uintptr_t)row & 3) * 8;
+      auto go = [&](auto word) {  // a unit begins in this word of one of the row's units in shared memory
+        constexpr int W = decltype(word)::value;
+#pragma unroll 2
+        for (int j = lane; j < wide; j += 32) {
+          const uint4 x = of[j], y = of[j + 1];
+          const u32 w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+          Wide u;
+          u.w = make_uint4(__funnelshift_r(w[W], w[W + 1], shift), __funnelshift_r(w[W + 1], w[W + 2], shift),
+                           __funnelshift_r(w[W + 2], w[W + 3], shift), __funnelshift_r(w[W + 3], w[W + 4], shift));
+          put(u, wide_to + j);
+        }
+      };
+      const int word = (int)((uintptr_t)row >> 2 & 3);
+      if (word == 0) go(std::integral_constant<int, 0>{});
+      else if (word == 1) go(std::integral_constant<int, 1>{});
+      else if (word == 2) go(std::integral_constant<int, 2>{});
+      else go(std::integral_constant<int, 3>{});
+    }
     __syncwarp();  // before the stage is written again
   }
 }
@@ -587,13 +646,13 @@ extern "C" int gsb_embedding_lookup(gsb_ctx* ctx, void* stream_, const void* tab
           const size_t smem = (size_t)(kStagedThreads / 32) * kStages * s.stage;
           const i64 most = (i64)kNumSMs * min((i64)16, (i64)(227 * 1024 / (smem + 1024))) * (kStagedThreads / 32);
           s.per_warp = (u32)((n + most - 1) / most);
-          const LookupArgs args{ids, (u32)n, (int)units, 0, num_rows, row_stride * size / kBytes, padding_id, has_padding != 0, scale,
+          const LookupArgs args{ids, (u32)n, (int)row_len, 0, num_rows, row_stride * size, padding_id, has_padding != 0, scale,
                                 ctx_counters(ctx)};
           if (smem > 48 * 1024)
             failed = cudaFuncSetAttribute(k_lookup_staged<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
           if (failed == cudaSuccess)
             failed = launch_behind_with(stream, smem, k_lookup_staged<T>, grid_for((n + s.per_warp - 1) / s.per_warp, kStagedThreads / 32),
-                                        kStagedThreads, args, s, (Unit<T, 2>*)out);
+                                        kStagedThreads, args, s, (T*)out);
           return;
         }
       }
@@ -605,7 +664,10 @@ extern "C" int gsb_embedding_lookup(gsb_ctx* ctx, void* stream_, const void* tab
         const dim3 grid((unsigned)min((i64)kNumSMs * 32, ctas), (unsigned)min(tiles, max((i64)1, kNumSMs * 8 / ctas)));
         const LookupArgs args{ids, (u32)n, (int)units, shape.lanes, num_rows, row_stride * size / kBytes, padding_id, has_padding != 0,
                               scale, ctx_counters(ctx)};
-        launch_behind(stream, k_lookup_rows<T, kBytes, S>, grid, kLookupThreads, args, (const Unit<T, kBytes>*)from,
+        auto kernel = k_lookup_rows<T, kBytes, S, 0>;
+        if constexpr (kBytes == 2)
+          if (shape.lanes == 32) kernel = k_lookup_rows<T, kBytes, S, 32>;
+        launch_behind(stream, kernel, grid, kLookupThreads, args, (const Unit<T, kBytes>*)from,
                       (Unit<T, kBytes>*)out);
       });
     });

@@ -295,10 +295,11 @@ def test_rows_without_a_sum_in_large_gradients(ops, n, rows, width, dtype, kind)
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
-@pytest.mark.parametrize("width,n", [(301, 40_000), (601, 20_000), (1433, 7000), (2047, 4999), (4095, 2100), (4097, 2100)])
+@pytest.mark.parametrize("width,n", [(301, 40_000), (601, 20_000), (1433, 7000), (2047, 4999), (4095, 2100), (4097, 2100),
+                                     (401, 45_000), (601, 30_000), (1433, 12_001), (2047, 8000), (4095, 4000), (4097, 4000), (51, 3001), (131, 3001)])
 @pytest.mark.parametrize("shift,gap", [(0, 0), (1, 0), (3, 1), (5, 7)])
 def test_large_lookups_of_odd_rows(ops, dtype, width, n, shift, gap):
-    """16 MB and more of rows whose values are no whole words, from tables that begin and end anywhere; nothing is written around."""
+    """Short and long lists of rows whose values are no whole words, from tables that begin and end anywhere; nothing is written around."""
     g = generator(9)
     rows, stride = 501, width + gap
     ctx = ops.Context()
