@@ -571,8 +571,9 @@ GSB_API int gsb_sage_hop_sized(gsb_ctx* ctx, void* stream, const int64_t* indptr
 /* ---- rows that are learned ---------------------------------------------------------------------------------------
  * No counterpart in the reference, which ends at the loaded features.  Rows of float, half or bfloat16 values (gsb_dtype),
  * of at most GSB_MAX_ROW_LEN each, one after the other with `*_stride` values from one row's start to the next (values of a row are
- * contiguous, and every address a multiple of its type's size); arithmetic in float, every result rounded once.  These calls use no scratch of the context: the caller provides it (at least the
- * bytes that the *_workspace function of the same sizes names, 256-byte aligned), so they may be captured into a CUDA graph
+ * contiguous, and every address a multiple of its type's size); arithmetic in float, every result rounded once.  These calls use
+ * no scratch of the context: the caller provides it (at least the bytes that the *_workspace function of the same sizes names,
+ * 256-byte aligned), so they may be captured into a CUDA graph
  * and queued on several streams at once, each call with a workspace of its own.  Ids, experts and places out of range are
  * never followed and record GSB_ERR_INDEX_RANGE.  Threads that use them at once have a context each. */
 #define GSB_MAX_ROW_LEN 1048576

@@ -356,3 +356,33 @@ def test_widths_of_ids(ops, n, bits):
     unique, at = torch.unique(ids, return_inverse=True)
     assert torch.equal(row_ids, unique)
     assert torch.equal(got, torch.zeros_like(got).index_add_(0, at, grad))     # sums of small integers are exact
+
+
+def test_large_calls_captured_and_replayed(ops):
+    """A gradient whose rows without a sum are cleared behind the sums, and rows that are looked up through shared memory; two graphs
+    that share a pool."""
+    g = generator(11)
+    n, rows, width = 420_000, 420_003, 128
+    ids = torch.randint(0, rows, (n,), generator=g, device="cuda")
+    grad = torch.randint(-3, 4, (n, width), generator=g, device="cuda").float()
+    table = torch.randn(5000, 1433, generator=g, device="cuda").half()
+    few = torch.randint(0, 5000, (12_000,), generator=g, device="cuda")
+    for _ in range(2):
+        ops.embedding_grad(grad, ids, rows), ops.embedding_lookup(table, few, 0.5, 3)
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=graphs[0][0].pool() if graphs else None):
+            out = ops.embedding_grad(grad, ids, rows), ops.embedding_lookup(table, few, 0.5, 3)
+        graphs.append((graph, out))
+    for turn in range(3):
+        ids.copy_(torch.randint(0, rows if turn != 1 else 1000, (n,), generator=g, device="cuda"))
+        few.copy_(torch.randint(0, 5000, (12_000,), generator=g, device="cuda"))
+        want = torch.zeros(rows, width, device="cuda").index_add_(0, ids, grad)       # small integers: exact in any order
+        looked = table[few] * 0.5 * (few != 3)[:, None]
+        for graph, (dense, found) in graphs:
+            dense.fill_(float("nan"))
+            found.fill_(float("nan"))
+            graph.replay()
+            assert torch.equal(dense, want) and torch.equal(found, looked)
