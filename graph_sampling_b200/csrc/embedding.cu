@@ -18,7 +18,7 @@ namespace gsb {
 
 constexpr int kLookupThreads = 256;
 
-// Narrow units: more rows (1 000 000 rows of 602 bf16 435 us for 474), but not with four units a lane (1.3 M of 50 bf16 53 for 56).
+// Narrow units: more rows (by two units a lane a million rows of 602 bf16 435 us for 474), but not with four (1.3 M of 50 bf16 53 for 56).
 constexpr int lookup_rows(int unit, int steps) { return unit < 16 && steps < 4 ? 4 : rows_ahead(steps); }
 
 struct LookupArgs {
@@ -36,7 +36,7 @@ struct LookupArgs {
 // million rows of 101 values 124 us for 180, of 251 255 for 321), but not where there are fewer to take (500 000 of 1 434 748 for 555).
 //
 // A group of lanes takes neighbouring rows of the result, a tile of their columns at a time: all its reads are on their way before
-// anything is written.  Bound by DRAM with rows in no order: 1 000 000 rows of 1 204 bytes out of 2.45 M in 452 us, 5.3 TB/s of what
+// anything is written.  Bound by DRAM with rows in no order: 1 000 000 rows of 1 204 bytes out of 2.45 M in 422 us, 5.7 TB/s of what
 // is read and written.
 template <class T, int BYTES, int STEPS, int LANES>
 __global__ void __launch_bounds__(kLookupThreads) k_lookup_rows(const LookupArgs a, const Unit<T, BYTES>* __restrict__ table,
@@ -118,8 +118,8 @@ __global__ void __launch_bounds__(kLookupThreads) k_lookup_rows(const LookupArgs
 // Rows of 16-bit values that begin off the 4-byte boundaries, where a unit is one value: a warp copies the next rows into shared
 // memory in units of 16 bytes, from the boundary before a row to the one behind it, and writes whole units of the result, each out
 // of two that it straddles.  A short row's steps cost more than it gains: 500 000 of 601 values 243 us for 352, 100 000 of 1 433
-// 108 for 169, but 500 000 of 301 167 for 155 and 30 000 of 501 15 for 13.  (Where units of 4 bytes fit, little is gained: a million
-// rows of 1 204 bytes 479 us for 456, of 2 868 bytes 1 026 for 1 115.)
+// 108 for 169, but 500 000 of 301 167 for 155 and 30 000 of 501 15 for 13.  (Where units of 4 bytes fit, nothing is gained: a million
+// rows of 1 204 bytes 479 us for 422.)
 constexpr int kStagedThreads = 128, kStages = 3;
 static bool staged(i64 row_bytes, i64 n) { return row_bytes >= 800 && row_bytes <= 8192 && n * row_bytes >= 32000000; }
 
@@ -509,7 +509,7 @@ static void launch_sum(cudaStream_t stream, SumArgs& a, i64 most_chunks, const v
                        const u64* sorted, void* out, float* part) {
   a.units = (int)(row_bytes / BYTES);
   a.stride = stride_bytes / BYTES;
-  const RowShape shape = row_shape(a.units, sum_steps(BYTES));
+  const RowShape shape = row_shape(a.units, sum_steps(BYTES), sum_wide(BYTES));
   a.lanes = shape.lanes;
   const int tiles = grid_for(a.units, shape.lanes * shape.steps);
   const i64 n = a.n;
@@ -656,7 +656,7 @@ extern "C" int gsb_embedding_lookup(gsb_ctx* ctx, void* stream_, const void* tab
           return;
         }
       }
-      const RowShape shape = row_shape(units, copy_steps(kBytes));
+      const RowShape shape = row_shape(units, copy_steps(kBytes), copy_wide(kBytes));
       with_steps(shape.steps, [&](auto steps) {
         constexpr int S = decltype(steps)::value, kRows = lookup_rows(kBytes, S);
         // a group goes through the tiles of its rows' columns, or shares them with others where there are few rows

@@ -299,7 +299,7 @@ extern "C" int gsb_expert_spread(gsb_ctx* ctx, void* stream_, const void* x, int
     typedef decltype(value) T;
     constexpr int B = decltype(bytes)::value;
     const i64 units = row_len * size / B;
-    const RowShape shape = row_shape(units, copy_steps(B));
+    const RowShape shape = row_shape(units, copy_steps(B), copy_wide(B));
     const RowArgs a = row_args(ctx, tokens, per_token, tokens * per_token, shape, units, x_stride * size / B, units, place, weights,
                                weights_dtype);
     with_steps(shape.steps, [&](auto steps) {
@@ -331,7 +331,7 @@ extern "C" int gsb_expert_combine(gsb_ctx* ctx, void* stream_, const void* rows,
     typedef decltype(value) T;
     constexpr int B = decltype(bytes)::value;
     const i64 units = row_len * size / B;
-    const RowShape shape = row_shape(units, copy_steps(B));
+    const RowShape shape = row_shape(units, copy_steps(B), copy_wide(B));
     const RowArgs a = row_args(ctx, tokens, per_token, num_rows, shape, units, units, rows_stride * size / B, place, weights,
                                weights_dtype);
     with_steps(shape.steps, [&](auto steps) {
@@ -370,7 +370,7 @@ extern "C" int gsb_expert_combine_grad(gsb_ctx* ctx, void* stream_, const void* 
     typedef decltype(value) T;
     constexpr int B = decltype(bytes)::value;
     const i64 units = row_len * size / B;
-    const RowShape shape = row_shape(units, copy_steps(B));
+    const RowShape shape = row_shape(units, copy_steps(B), copy_wide(B));
     const RowArgs a = row_args(ctx, tokens, per_token, num_rows, shape, units, grad_stride * size / B, rows_stride * size / B, place,
                                weights, weights_dtype);
     with_steps(shape.steps, [&](auto steps) {

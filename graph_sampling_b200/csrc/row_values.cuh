@@ -128,12 +128,12 @@ bool aligned_to(int bytes, const P*... p) {
 
 // How a row is taken: by `lanes` neighbouring lanes (a power of two up to 32), `steps` units (1 .. 4) of each at a time.  Of the shapes
 // that take the row at once the one that leaves the fewest lanes idle; among equals the one whose steps are nearest to
-// `wanted`.  Rows of more than 96 units go in tiles of 32 lanes with two units each.
+// `wanted`.  Rows of more than 96 units go in tiles of 32 lanes with `wide` units each.
 struct RowShape {
   int lanes, steps;
 };
-inline RowShape row_shape(int64_t units, int wanted) {
-  RowShape best{32, 2};
+inline RowShape row_shape(int64_t units, int wanted, int wide) {
+  RowShape best{32, wide};
   if (units > 96) return best;
   int idle = 1 << 20, away = 0;
   for (int lanes = 32; lanes >= 1; lanes /= 2) {
@@ -153,6 +153,11 @@ inline RowShape row_shape(int64_t units, int wanted) {
 // rows of 100 bytes 51, with one unit 83).
 inline int copy_steps(int unit) { return unit == 16 ? 2 : 4; }
 inline int sum_steps(int unit) { return unit >= 16 ? 1 : unit == 8 ? 2 : 4; }
+// Of long rows: four narrow units, though the last tile leaves more lanes idle (50 000 tokens to 200 000 rows of 1 434 bf16: spread 209
+// us for 258, combined 207 for 252; 200 000 rows of 602 looked up 86 for 92, summed 150 for 168), but two of 16 bytes (200 000 rows
+// of 2 KB combined 89 us, with four 95), and of 8 where they are summed (few rows of 602 floats 131 us, with four 140).
+inline int copy_wide(int unit) { return unit == 16 ? 2 : 4; }
+inline int sum_wide(int unit) { return unit >= 8 ? 2 : 4; }
 // Rows that a group of lanes has on their way at once.  More of them cost warps: with twice as many 65 528 rows of 2 KB were spread
 // in 29 us for 25, 314 602 of 200 bytes in 33 for 26.
 constexpr int rows_ahead(int steps) { return steps == 1 ? 4 : 2; }
