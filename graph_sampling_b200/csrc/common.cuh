@@ -3,6 +3,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <mutex>
+
 #include "../../include/gsb200.h"
 
 typedef int64_t i64;
@@ -109,6 +111,10 @@ constexpr int kMailSlots = 8;
 constexpr int kMailErrorBit = 47;
 constexpr u64 kMailValueMask = (1ull << kMailErrorBit) - 1;
 
+// Who waits.  A backward pass runs on a thread of autograd's and goes through the same context as the calls of the thread that
+// samples meanwhile: the calls on learned rows that wait have a mailbox, a ticket and an event of their own.
+enum Waiter { WAIT_CALL, WAIT_ROWS, WAITER_NUM };
+
 // Context internals (defined in ctx.cu).
 // Scratch of the call that is about to queue work on `stream`.  It is the same memory for every call, which is why they are
 // ordered on one stream; a call on another stream than the last one's waits here until the device is done with that.
@@ -135,7 +141,7 @@ i64 ctx_option(gsb_ctx* ctx, int option);
 // GSB_OPT_DIRECT_TABLE_BUDGET (the caller then takes the hash path).
 int ctx_direct_tables(gsb_ctx* ctx, i64 count, i64 num_nodes, cudaStream_t stream, u64** out_table,
                       uint32_t* out_epoch);
-int ctx_check_device_error(gsb_ctx* ctx, cudaStream_t stream);
+int ctx_check_device_error(gsb_ctx* ctx, cudaStream_t stream, Waiter who = WAIT_CALL);
 // Epoch-tagged tables of the single-launch unique + relabel (fused_unique.cu): at least `bytes` bytes kept by the context,
 // never cleared between calls.  which = 0: hash table, 1: direct-address table.  *epoch (1 .. epochs - 1) is new for every
 // call; when the epochs are used up, and when the table grows, every byte is set to `fill`.  Bounded by the callers (64 MB
@@ -144,14 +150,14 @@ int ctx_epoch_table(gsb_ctx* ctx, int which, size_t bytes, int fill, uint32_t ep
                     uint32_t* epoch);
 // Waits until everything queued on `stream` so far is done and returns the `n` counters starting at `first` (a copy in
 // page-locked memory, written by a one-warp kernel that the host spins on).
-int ctx_fetch_counters(gsb_ctx* ctx, cudaStream_t stream, int first, int n, const i64** out);
-// A fresh mailbox for the call's kernels, and the wait for `n` of its slots.  A slot holds the value its kernel posted;
-// *error tells whether a device error was recorded by then (the caller then takes ctx_check_device_error, which waits
-// for the stream).  Outputs of the posting kernel are complete in stream order, as after any launch.
-Mail ctx_mail(gsb_ctx* ctx);
-int ctx_wait_mail(gsb_ctx* ctx, cudaStream_t stream, const Mail& mail, int n, i64* values, bool* error);
-// The usual end of a call that reports `n` posted values: waits, fills `values`, returns the device error if there is one.
-int ctx_mail_result(gsb_ctx* ctx, cudaStream_t stream, const Mail& mail, int n, i64* values);
+int ctx_fetch_counters(gsb_ctx* ctx, cudaStream_t stream, int first, int n, const i64** out, Waiter who = WAIT_CALL);
+// A fresh mailbox for the call's kernels, and the usual end of a call that reports `n` values posted there: waits, fills `values`,
+// returns the device error if one was recorded by then.  Outputs of the posting kernel are complete in stream order, as after any
+// launch.  Nothing posted although the stream is done is an error too, whoever has read the record of its cause.
+Mail ctx_mail(gsb_ctx* ctx, Waiter who = WAIT_CALL);
+int ctx_mail_result(gsb_ctx* ctx, cudaStream_t stream, const Mail& mail, int n, i64* values, Waiter who = WAIT_CALL);
+// Held from ctx_mail to ctx_mail_result by the waiter WAIT_ROWS.
+std::mutex& ctx_rows_wait(gsb_ctx* ctx);
 void ctx_count_launches(gsb_ctx* ctx, int n);
 void ctx_count_id_bound_refusal(gsb_ctx* ctx);
 // When profiling is enabled (gsb_profile_enable) these bracket a launch with CUDA events on the

@@ -4,12 +4,22 @@
 
 #include <atomic>
 #include <chrono>
+#include <mutex>
 #include <new>
 #include <vector>
 
 #include "common.cuh"
 #include "grid_sync.cuh"
 #include "scan.cuh"
+
+// What a call that waits for the device needs on the host.
+struct HostWait {
+  i64* pinned;         // page-locked host memory the device writes: CNT_NUM counters, kMailSlots result words, one ticket
+  u64 mail_tag;        // 1 .. 65535, of the last mailbox handed out
+  u64 ticket;          // of the last counter fetch
+  cudaEvent_t event;   // created on first use when GSB_OPT_BLOCKING_WAIT is set
+};
+constexpr int kPinnedWords = gsb::CNT_NUM + gsb::kMailSlots + 1;
 
 struct gsb_ctx {
   int device;
@@ -21,9 +31,8 @@ struct gsb_ctx {
   i64 tile_capacity;
   uint32_t epoch;
   i64* counters;  // device, CNT_NUM entries and the grid-barrier word
-  i64* pinned;    // page-locked host memory the device writes: CNT_NUM counters, kMailSlots result words, one ticket
-  u64 mail_tag;   // 1 .. 65535, of the last mailbox handed out
-  u64 ticket;     // of the last counter fetch
+  HostWait waits[gsb::WAITER_NUM];
+  std::mutex rows_wait;  // held by the call on learned rows that waits
   i64 launches;
   i64 id_bound_refusals;
   char message[512];
@@ -47,7 +56,6 @@ struct gsb_ctx {
   cudaStream_t stream;   // of the last call that used scratch
   bool stream_known;
   u64 barrier_arrivals;  // the barrier word itself is counters[CNT_NUM]
-  cudaEvent_t wait_event;  // created on first use when GSB_OPT_BLOCKING_WAIT is set
 };
 
 namespace gsb {
@@ -264,29 +272,30 @@ int launch_cooperative(gsb_ctx* ctx, cudaStream_t stream, const void* kernel, in
 
 i64* ctx_counters(gsb_ctx* ctx) { return ctx->counters; }
 int ctx_device(gsb_ctx* ctx) { return ctx->device; }
+std::mutex& ctx_rows_wait(gsb_ctx* ctx) { return ctx->rows_wait; }
 
 // Waits for `stream`.  By default with cudaStreamSynchronize (the calling thread may spin); with
 // GSB_OPT_BLOCKING_WAIT through an event created with cudaEventBlockingSync, which puts the thread to sleep — what a
 // host that runs several streams from several threads (or several processes per machine) wants.
-static int ctx_wait(gsb_ctx* ctx, cudaStream_t stream) {
+static int ctx_wait(gsb_ctx* ctx, cudaStream_t stream, HostWait& wait) {
   if (ctx->options[GSB_OPT_BLOCKING_WAIT] == 0) {
     GSB_CUDA_OK(cudaStreamSynchronize(stream));
     return GSB_OK;
   }
-  if (!ctx->wait_event)
-    GSB_CUDA_OK(cudaEventCreateWithFlags(&ctx->wait_event, cudaEventBlockingSync | cudaEventDisableTiming));
-  GSB_CUDA_OK(cudaEventRecord(ctx->wait_event, stream));
-  GSB_CUDA_OK(cudaEventSynchronize(ctx->wait_event));
+  if (!wait.event) GSB_CUDA_OK(cudaEventCreateWithFlags(&wait.event, cudaEventBlockingSync | cudaEventDisableTiming));
+  GSB_CUDA_OK(cudaEventRecord(wait.event, stream));
+  GSB_CUDA_OK(cudaEventSynchronize(wait.event));
   return GSB_OK;
 }
 
 // Spins until `*word & mask == want`.  The device normally answers within microseconds; from half a millisecond on the
 // stream's status is asked now and then, so that a failed launch or a stream that finished without writing the word
 // (*answered = false) ends the wait.
-static int ctx_spin(gsb_ctx* ctx, cudaStream_t stream, const volatile u64* word, u64 mask, u64 want, bool* answered) {
+static int ctx_spin(gsb_ctx* ctx, cudaStream_t stream, HostWait& wait, const volatile u64* word, u64 mask, u64 want,
+                    bool* answered) {
   *answered = true;
   if (ctx->options[GSB_OPT_BLOCKING_WAIT] != 0) {
-    int st = ctx_wait(ctx, stream);
+    int st = ctx_wait(ctx, stream, wait);
     if (st != GSB_OK) return st;
     *answered = (*word & mask) == want;
     return GSB_OK;
@@ -313,41 +322,43 @@ static int ctx_spin(gsb_ctx* ctx, cudaStream_t stream, const volatile u64* word,
   }
 }
 
-Mail ctx_mail(gsb_ctx* ctx) {
-  if (++ctx->mail_tag > 0xFFFF) {
+Mail ctx_mail(gsb_ctx* ctx, Waiter who) {
+  HostWait& wait = ctx->waits[who];
+  if (++wait.mail_tag > 0xFFFF) {
     // The tags start over, and a slot that few calls post may still hold what one of them left there under a tag that comes
     // again: no word is older than its round of tags.
-    volatile u64* slots = (volatile u64*)(ctx->pinned + CNT_NUM);
+    volatile u64* slots = (volatile u64*)(wait.pinned + CNT_NUM);
     for (int q = 0; q < kMailSlots; ++q) slots[q] = 0;
-    ctx->mail_tag = 1;
+    wait.mail_tag = 1;
   }
-  return Mail{(u64*)(ctx->pinned + CNT_NUM), ctx->mail_tag << 48};
+  return Mail{(u64*)(wait.pinned + CNT_NUM), wait.mail_tag << 48};
 }
 
-int ctx_wait_mail(gsb_ctx* ctx, cudaStream_t stream, const Mail& mail, int n, i64* values, bool* error) {
-  *error = false;
+int ctx_mail_result(gsb_ctx* ctx, cudaStream_t stream, const Mail& mail, int n, i64* values, Waiter who) {
+  bool error = false, posted = true;
   for (int q = 0; q < n; ++q) {
     const volatile u64* word = mail.word + q;
     bool answered;
-    int st = ctx_spin(ctx, stream, word, 0xFFFFull << 48, mail.tag, &answered);
+    int st = ctx_spin(ctx, stream, ctx->waits[who], word, 0xFFFFull << 48, mail.tag, &answered);
     if (st != GSB_OK) return st;
     if (!answered) {  // the stream is done and nothing was posted: only a kernel that gave up does that
-      *error = true;
+      posted = false;
       values[q] = 0;
       continue;
     }
     const u64 w = *word;
     values[q] = (i64)(w & kMailValueMask);
-    *error |= ((w >> kMailErrorBit) & 1ull) != 0;
+    error |= ((w >> kMailErrorBit) & 1ull) != 0;
+  }
+  if (error || !posted) {
+    const int st = ctx_check_device_error(ctx, stream, who);
+    if (st != GSB_OK) return st;
+  }
+  if (!posted) {  // the record of it has been read by another call
+    snprintf(ctx->message, sizeof(ctx->message), "the size that the call waits for was not posted");
+    return GSB_ERR_LOOKBACK_TIMEOUT;
   }
   return GSB_OK;
-}
-
-int ctx_mail_result(gsb_ctx* ctx, cudaStream_t stream, const Mail& mail, int n, i64* values) {
-  bool error;
-  int st = ctx_wait_mail(ctx, stream, mail, n, values, &error);
-  if (st != GSB_OK) return st;
-  return error ? ctx_check_device_error(ctx, stream) : GSB_OK;
 }
 
 // One warp: counters -> page-locked host memory, then the ticket the host spins on.
@@ -358,21 +369,22 @@ __global__ void k_publish_counters(const i64* __restrict__ counters, int first, 
   if (threadIdx.x == 0) st_volatile_u64((u64*)host + CNT_NUM + kMailSlots, ticket);
 }
 
-int ctx_fetch_counters(gsb_ctx* ctx, cudaStream_t stream, int first, int n, const i64** out) {
-  ctx->ticket += 1;
-  k_publish_counters<<<1, 32, 0, stream>>>(ctx->counters, first, n, ctx->pinned, ctx->ticket);
+int ctx_fetch_counters(gsb_ctx* ctx, cudaStream_t stream, int first, int n, const i64** out, Waiter who) {
+  HostWait& wait = ctx->waits[who];
+  wait.ticket += 1;
+  k_publish_counters<<<1, 32, 0, stream>>>(ctx->counters, first, n, wait.pinned, wait.ticket);
   GSB_LAUNCH_OK();
   bool answered;
-  int st = ctx_spin(ctx, stream, (const volatile u64*)ctx->pinned + CNT_NUM + kMailSlots, ~0ull, ctx->ticket, &answered);
+  int st = ctx_spin(ctx, stream, wait, (const volatile u64*)wait.pinned + CNT_NUM + kMailSlots, ~0ull, wait.ticket, &answered);
   if (st != GSB_OK) return st;
   if (!answered) return GSB_ERR_CUDA;
-  *out = ctx->pinned + first;
+  *out = wait.pinned + first;
   return GSB_OK;
 }
 
-int ctx_check_device_error(gsb_ctx* ctx, cudaStream_t stream) {
+int ctx_check_device_error(gsb_ctx* ctx, cudaStream_t stream, Waiter who) {
   const i64* c;
-  int st = ctx_fetch_counters(ctx, stream, CNT_ERROR, 2, &c);
+  int st = ctx_fetch_counters(ctx, stream, CNT_ERROR, 2, &c, who);
   if (st != GSB_OK) return st;
   if (c[0] != 0) {
     int code = (int)c[0];
@@ -380,10 +392,11 @@ int ctx_check_device_error(gsb_ctx* ctx, cudaStream_t stream) {
              gsb_status_string(code), (long long)c[1]);
     GSB_CUDA_OK(cudaMemsetAsync(ctx->counters + CNT_ERROR, 0, 2 * sizeof(i64), stream));
     GSB_CUDA_OK(cudaMemsetAsync(ctx->counters + CNT_LOST, 0, sizeof(i64), stream));
-    // the mark of a grid barrier that was given up, the top byte of its word (grid_sync.cuh)
-    GSB_CUDA_OK(cudaMemsetAsync((char*)(ctx->counters + CNT_NUM) + kBarrierCountBits / 8, 0, 1, stream));
+    // the mark of a grid barrier that was given up, the top byte of its word (grid_sync.cuh); calls on learned rows have words of
+    // their own, and a kernel of the context's thread may be between two looks at this one
+    if (who == WAIT_CALL) GSB_CUDA_OK(cudaMemsetAsync((char*)(ctx->counters + CNT_NUM) + kBarrierCountBits / 8, 0, 1, stream));
     {
-      int st2 = ctx_wait(ctx, stream);
+      int st2 = ctx_wait(ctx, stream, ctx->waits[who]);
       if (st2 != GSB_OK) return st2;
     }
     return code;
@@ -448,7 +461,6 @@ int gsb_ctx_create(int device, gsb_ctx** out_ctx) {
   if (e != cudaSuccess || device < 0 || device >= count) return e != cudaSuccess ? GSB_ERR_CUDA : GSB_ERR_INVALID_ARGUMENT;
   gsb_ctx* ctx = new (std::nothrow) gsb_ctx();
   if (!ctx) return GSB_ERR_OUT_OF_MEMORY;
-  memset(ctx, 0, sizeof(*ctx));
   ctx->device = device;
   ctx->ev_begin = new std::vector<cudaEvent_t>();
   ctx->ev_end = new std::vector<cudaEvent_t>();
@@ -464,13 +476,14 @@ int gsb_ctx_create(int device, gsb_ctx** out_ctx) {
     if ((e = cudaSetDevice(device)) != cudaSuccess) break;
     if ((e = cudaMalloc((void**)&ctx->counters, sizeof(i64) * (gsb::CNT_NUM + 1))) != cudaSuccess) break;
     if ((e = cudaMemset(ctx->counters, 0, sizeof(i64) * (gsb::CNT_NUM + 1))) != cudaSuccess) break;
-    if ((e = cudaMallocHost((void**)&ctx->pinned, sizeof(i64) * (gsb::CNT_NUM + gsb::kMailSlots + 1))) != cudaSuccess) break;
-    memset(ctx->pinned, 0, sizeof(i64) * (gsb::CNT_NUM + gsb::kMailSlots + 1));
+    i64* pinned = nullptr;
+    if ((e = cudaMallocHost((void**)&pinned, sizeof(i64) * kPinnedWords * gsb::WAITER_NUM)) != cudaSuccess) break;
+    memset(pinned, 0, sizeof(i64) * kPinnedWords * gsb::WAITER_NUM);
+    for (int w = 0; w < gsb::WAITER_NUM; ++w) ctx->waits[w].pinned = pinned + w * kPinnedWords;
   } while (0);
   if (e != cudaSuccess) {
     st = gsb::cuda_fail(nullptr, e, __FILE__, __LINE__);
     if (ctx->counters) cudaFree(ctx->counters);
-    if (ctx->pinned) cudaFreeHost(ctx->pinned);
     delete ctx->ev_begin;
     delete ctx->ev_end;
     delete ctx->ev_kid;
@@ -494,9 +507,10 @@ int gsb_ctx_destroy(gsb_ctx* ctx) {
   if (ctx->direct_tables) cudaFree(ctx->direct_tables);
   for (void* t : ctx->epoch_table)
     if (t) cudaFree(t);
-  if (ctx->wait_event) cudaEventDestroy(ctx->wait_event);
+  for (HostWait& wait : ctx->waits)
+    if (wait.event) cudaEventDestroy(wait.event);
   if (ctx->counters) cudaFree(ctx->counters);
-  if (ctx->pinned) cudaFreeHost(ctx->pinned);
+  if (ctx->waits[0].pinned) cudaFreeHost(ctx->waits[0].pinned);  // that of all waiters
   for (size_t i = 0; i < ctx->ev_begin->size(); ++i) {
     cudaEventDestroy((*ctx->ev_begin)[i]);
     cudaEventDestroy((*ctx->ev_end)[i]);

@@ -749,7 +749,11 @@ extern "C" int gsb_embedding_grad_rows(gsb_ctx* ctx, void* stream_, const void* 
   SortCall call{KeySource{ids, n, num_rows, has_padding != 0, padding_id, ctx_counters(ctx)}, SORT_RANKS};
   call.distinct = out_ids;
   call.number = out_count;
-  if (count_host) call.mail = ctx_mail(ctx);
+  std::unique_lock<std::mutex> waiting;
+  if (count_host) {
+    waiting = std::unique_lock<std::mutex>(ctx_rows_wait(ctx));
+    call.mail = ctx_mail(ctx, WAIT_ROWS);
+  }
   {
     ScopedKernelTimer timer(ctx, KID_KEY_SORT, stream);
     st = key_sort(ctx, stream, call, workspace, &sorted);
@@ -757,5 +761,5 @@ extern "C" int gsb_embedding_grad_rows(gsb_ctx* ctx, void* stream_, const void* 
   if (st != GSB_OK) return st;
   st = sum_sorted(ctx, stream, GradCall{grad, dtype, row_len, grad_stride, scale, out_rows, out_dtype}, plan, sorted, n, n, part, nullptr);
   if (st != GSB_OK || !count_host) return st;
-  return ctx_mail_result(ctx, stream, call.mail, 1, count_host);
+  return ctx_mail_result(ctx, stream, call.mail, 1, count_host, WAIT_ROWS);
 }

@@ -13,7 +13,6 @@
 #include <torch/csrc/autograd/variable.h>
 
 #include <limits>
-#include <mutex>
 #include <optional>
 #include <utility>
 
@@ -169,16 +168,12 @@ std::vector<Tensor> grad_rows(gsb_ctx* ctx, const Tensor& grad_, const Tensor& i
   Tensor row_ids = empty(n, dev), rows = fresh({n, width}, g.out_type, dev), count = empty(1, dev);
   Tensor work = scratch(gsb_embedding_grad_workspace(n, num_rows, width), "gsb_embedding_grad_rows", dev);
   int64_t found = 0;
-  // the number comes back through the context, which the backward passes of several threads share
-  static std::mutex waiting;
-  std::unique_lock<std::mutex> lock(waiting, std::defer_lock);
-  if (sync) lock.lock();
   done(ctx, gsb_embedding_grad_rows(ctx, stream(), g.grad.data(), g.grad.dtype, width, g.grad.stride, ids_ptr(g.ids), n, num_rows,
                                     (float)scale, pad.given, pad.id, static_cast<int64_t*>(data(row_ids)), data(rows), g.out_dtype,
                                     static_cast<int64_t*>(data(count)), data(work), work.numel(), sync ? &found : nullptr),
        "gsb_embedding_grad_rows");
-  if (sync) lock.unlock();
   if (!sync) return {row_ids, rows, count};
+  if (found < 0 || found > n) throw Failed(GSB_ERR_CUDA, "gsb_embedding_grad_rows", "a number of rows that cannot be");
   trim(row_ids, found);
   rows.unsafeGetTensorImpl()->set_sizes_contiguous({found, width});
   return {row_ids, rows};

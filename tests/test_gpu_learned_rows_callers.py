@@ -1,0 +1,95 @@
+"""Learned rows beside other callers and in calls that the documentation allows and few make: threads, kinds of tensors, addresses,
+waits that run out, values that are no numbers."""
+import ctypes
+import threading
+
+import pytest
+import torch
+
+import learned_rows as exact
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from graph_sampling_b200 import ops as m
+    return m
+
+
+@pytest.fixture(scope="module")
+def nn():
+    from graph_sampling_b200.gs import nn as m
+    return m
+
+
+def generator(seed):
+    g = torch.Generator("cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def stream():
+    return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def at_once(*jobs):
+    """Runs the jobs on threads, each on a stream of its own, and raises what one of them raised."""
+    raised = []
+    torch.cuda.synchronize()
+
+    def run(job):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                job()
+                torch.cuda.current_stream().synchronize()
+        except BaseException as e:
+            raised.append(e)
+
+    threads = [threading.Thread(target=run, args=(job,)) for job in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(240)
+    assert not any(t.is_alive() for t in threads)
+    if raised:
+        raise raised[0]
+
+
+# ---- several threads -----------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("blocking", [0, 1])
+def test_sparse_gradients_beside_a_thread_that_samples(ops, nn, blocking):
+    """Both wait for sizes through the default context, whatever each finds."""
+    import graph_sampling_b200.gs as gs
+    from graph_sampling_b200.synthetic import rmat_csc
+    g = generator(1)
+    indptr, indices = rmat_csc(3000, 40_000, seed=5, device="cpu")
+    A = gs.Matrix().load_csc(indptr.cuda(), indices.cuda())
+    seeds = [torch.arange(10 * (i + 1), device="cuda") for i in range(20)]
+    degree = indptr.diff().clamp(max=8).cuda()
+    tables = [torch.randn(2000, 16, generator=g, device="cuda").requires_grad_() for _ in range(2)]
+    ids = [torch.randint(0, 150 * (i + 1), (3000,), generator=g, device="cuda") for i in range(2)]
+    unique = [torch.unique(i) for i in ids]
+
+    def sampler():
+        for turn in range(300):
+            s = seeds[turn % len(seeds)]
+            sub = A._graph._CAPI_fused_columnwise_slicing_sampling(s, 8, False)
+            found = sub._CAPI_all_indices()
+            assert s.numel() <= found.numel() <= s.numel() + int(degree[s].sum()) and bool((found < 3000).all())
+
+    def trainer(i):
+        def work():
+            for _ in range(300):
+                grad, = torch.autograd.grad(nn.embedding(tables[i], ids[i], sparse=True).sum(), tables[i])
+                assert torch.equal(grad.indices()[0], unique[i]) and grad.values().shape == (unique[i].numel(), 16)
+        return work
+
+    ctx = ops.default_context()
+    usual = ctx.get_option("blocking_wait")
+    ctx.set_option("blocking_wait", blocking)
+    try:
+        at_once(sampler, trainer(0), trainer(1))
+    finally:
+        ctx.set_option("blocking_wait", usual)
+    ctx.check_device()
