@@ -7,6 +7,7 @@
 // shared by many groups of lanes.  A sum that begins and ends inside a chunk is written at once; what reaches over a chunk's
 // ends goes to `part` and is added up by k_join_rows.  Rows without a sum are cleared beside the sort, or, where that would write
 // much twice, by k_join_rows.
+#include <atomic>
 #include <type_traits>
 
 #include "key_sort.cuh"
@@ -121,7 +122,10 @@ __global__ void __launch_bounds__(kLookupThreads) k_lookup_rows(const LookupArgs
 // 108 for 169, but 500 000 of 301 167 for 155 and 30 000 of 501 15 for 13.  (Where units of 4 bytes fit, nothing is gained: a million
 // rows of 1 204 bytes 479 us for 422.)
 constexpr int kStagedThreads = 128, kStages = 3;
-static bool staged(i64 row_bytes, i64 n) { return row_bytes >= 800 && row_bytes <= 8192 && n * row_bytes >= 32000000; }
+constexpr i64 kMostStagedBytes = 8192;
+static bool staged(i64 row_bytes, i64 n) { return row_bytes >= 800 && row_bytes <= kMostStagedBytes && n * row_bytes >= 32000000; }
+static u32 stage_bytes(i64 row_bytes) { return (u32)((row_bytes + 15) / 16 * 16 + 16); }
+static size_t staged_smem(u32 stage) { return (size_t)(kStagedThreads / 32) * kStages * stage; }
 
 struct StagedArgs {
   const char* begin;  // of the table
@@ -236,6 +240,19 @@ __global__ void __launch_bounds__(kStagedThreads) k_lookup_staged(const LookupAr
     }
     __syncwarp();  // before the stage is written again
   }
+}
+
+// Once per device: the kernel may use as much shared memory as the longest rows need.  (The limit is the function's, not the launch's:
+// set call by call, one thread would lower it between another's setting and launch.)
+template <class T>
+static cudaError_t prepare_staged(gsb_ctx* ctx) {
+  static std::atomic<bool> known[64];
+  const int device = ctx_device(ctx);
+  if (device >= 0 && device < 64 && known[device]) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(k_lookup_staged<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             (int)staged_smem(stage_bytes(kMostStagedBytes)));
+  if (e == cudaSuccess && device >= 0 && device < 64) known[device] = true;
+  return e;
 }
 
 // N values of `to`, 16 bytes at a time where they are that many.
@@ -641,15 +658,14 @@ extern "C" int gsb_embedding_lookup(gsb_ctx* ctx, void* stream_, const void* tab
           StagedArgs s;
           s.begin = (const char*)from;
           s.end = s.begin + (num_rows - 1) * row_stride * size + row_bytes;
-          s.stage = (u32)((row_bytes + 15) / 16 * 16 + 16);
+          s.stage = stage_bytes(row_bytes);
           s.row_bytes = (int)row_bytes;
-          const size_t smem = (size_t)(kStagedThreads / 32) * kStages * s.stage;
+          const size_t smem = staged_smem(s.stage);
           const i64 most = (i64)kNumSMs * min((i64)16, (i64)(227 * 1024 / (smem + 1024))) * (kStagedThreads / 32);
           s.per_warp = (u32)((n + most - 1) / most);
           const LookupArgs args{ids, (u32)n, (int)row_len, 0, num_rows, row_stride * size, padding_id, has_padding != 0, scale,
                                 ctx_counters(ctx)};
-          if (smem > 48 * 1024)
-            failed = cudaFuncSetAttribute(k_lookup_staged<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+          failed = prepare_staged<T>(ctx);
           if (failed == cudaSuccess)
             failed = launch_behind_with(stream, smem, k_lookup_staged<T>, grid_for((n + s.per_warp - 1) / s.per_warp, kStagedThreads / 32),
                                         kStagedThreads, args, s, (T*)out);

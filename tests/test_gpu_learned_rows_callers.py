@@ -93,3 +93,22 @@ def test_sparse_gradients_beside_a_thread_that_samples(ops, nn, blocking):
     finally:
         ctx.set_option("blocking_wait", usual)
     ctx.check_device()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_long_odd_rows_of_two_widths_looked_up_by_two_threads(ops, dtype):
+    """Launches with much shared memory and with less, a context each: what one asks for is not taken back by the other."""
+    g = generator(2)
+
+    def job(width, n):
+        table = torch.randn(60, width, generator=g, device="cuda").to(dtype)
+        ids = torch.randint(0, 60, (n,), generator=g, device="cuda")
+        want, ctx = table[ids], ops.Context()
+
+        def work():
+            for _ in range(400):
+                out = ops.embedding_lookup(table, ids, ctx=ctx)
+            assert torch.equal(out, want)
+        return work
+
+    at_once(job(4095, 4000), job(2047, 8000))
