@@ -309,6 +309,12 @@ void refuse_foreign_accumulator(const Tensor& leaf) {
         "a graph of this leaf made outside the capture, on another stream, is still alive: drop its outputs before capturing");
 }
 
+// The kernels read memory and know nothing of forward-mode tangents: a result without one would pass for a constant.
+void refuse_tangents(const char* name, const Tensor& t) {
+  if (t.defined() && t._fw_grad(0).defined())
+    throw std::runtime_error(std::string(name) + " carries a forward-mode tangent; only reverse-mode gradients are implemented");
+}
+
 struct EmbeddingFunction : torch::autograd::Function<EmbeddingFunction> {
   static Tensor forward(AutogradContext* a, const Tensor& table, const Tensor& ids, int64_t handle, double scale, bool padded,
                         int64_t padding, bool sparse) {
@@ -325,6 +331,7 @@ struct EmbeddingFunction : torch::autograd::Function<EmbeddingFunction> {
   static tensor_list backward(AutogradContext* a, tensor_list grads) {
     tensor_list out(7);
     if (!grads[0].defined()) return out;
+    refuse_tangents("grad", grads[0]);
     gsb_ctx* ctx = kept(a->saved_data["handle"].toInt());
     const Tensor ids = a->get_saved_variables()[0];
     const Padding pad{a->saved_data["padded"].toBool(), a->saved_data["padding"].toInt()};
@@ -353,6 +360,7 @@ struct DispatchFunction : torch::autograd::Function<DispatchFunction> {
   static tensor_list backward(AutogradContext* a, tensor_list grads) {
     tensor_list out(3);
     if (!grads[0].defined()) return out;
+    refuse_tangents("grad", grads[0]);
     {
       const at::NoGradGuard no_grad;
       out[0] = combine(kept(a->saved_data["handle"].toInt()), grads[0], a->get_saved_variables()[0], Tensor());
@@ -373,6 +381,7 @@ struct GatherFunction : torch::autograd::Function<GatherFunction> {
   static tensor_list backward(AutogradContext* a, tensor_list grads) {
     tensor_list out(3);
     if (!grads[0].defined()) return out;
+    refuse_tangents("grad", grads[0]);
     const Tensor place = a->get_saved_variables()[0];
     {
       const at::NoGradGuard no_grad;
@@ -392,6 +401,7 @@ struct CombineFunction : torch::autograd::Function<CombineFunction> {
   static tensor_list backward(AutogradContext* a, tensor_list grads) {
     tensor_list out(4);
     if (!grads[0].defined()) return out;
+    refuse_tangents("grad", grads[0]);
     const auto saved = a->get_saved_variables();
     {
       const at::NoGradGuard no_grad;
@@ -529,6 +539,7 @@ FUNCTION(nn_embedding, 6) {  // (ctx, table, ids, scale, padding id | None, spar
   const Padding pad = padding(a[4]);
   const bool sparse = truth(a[5]);
   return wrap(without_gil([&] {
+    refuse_tangents("table", table);
     if (!follows(table)) return lookup(ctx, table, ids, scale, pad);
     rows_of(table, "table");
     refuse_foreign_accumulator(table);
@@ -540,6 +551,7 @@ FUNCTION(nn_dispatch, 3) {  // (ctx, x, place) -> rows
   gsb_ctx* ctx = context(a[0]);
   const Tensor &x = tensor(a[1], "x"), &place = tensor(a[2], "place");
   return wrap(without_gil([&] {
+    refuse_tangents("x", x);
     if (!follows(x)) return spread(ctx, x, place, Tensor());
     refuse_foreign_accumulator(x);
     return DispatchFunction::apply(x, place, keep(ctx));
@@ -551,6 +563,8 @@ FUNCTION(nn_combine, 4) {  // (ctx, rows, place, weights | None) -> out
   const Tensor &rows = tensor(a[1], "rows"), &place = tensor(a[2], "place");
   const Tensor weights = tensor_or_none(a[3], "weights");
   return wrap(without_gil([&] {
+    refuse_tangents("rows", rows);
+    refuse_tangents("weights", weights);
     if (!follows(rows) && !follows(weights)) return combine(ctx, rows, place, weights);
     refuse_foreign_accumulator(rows);
     refuse_foreign_accumulator(weights);

@@ -2,9 +2,9 @@
 
 `embedding` looks rows up by node or token id (a frontier, a random walk); `expert_order`, `dispatch` and `combine` sort rows
 by expert or node type, so that every product runs over a run of rows, and bring the results back.  Gradients follow through
-torch's autograd; they cannot be differentiated a second time.  All of it may be captured into a CUDA graph, where no graph of the
-same leaves made outside the capture may be alive (refused).  The GPU's default context records errors.  Several threads may use
-these functions at once, also beside one that samples.
+torch's autograd, in reverse mode only: they cannot be differentiated a second time, and forward-mode tangents are refused.  All
+of it may be captured into a CUDA graph, where no graph of the same leaves made outside the capture may be alive (refused).  The
+GPU's default context records errors.  Several threads may use these functions at once, also beside one that samples.
 """
 from collections import namedtuple
 

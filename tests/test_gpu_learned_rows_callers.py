@@ -112,3 +112,27 @@ def test_long_odd_rows_of_two_widths_looked_up_by_two_threads(ops, dtype):
         return work
 
     at_once(job(4095, 4000), job(2047, 8000))
+
+
+# ---- kinds of tensors ----------------------------------------------------------------------------------------------------------
+def test_forward_mode_is_refused(nn):
+    """Tangents of what goes in, and of the gradients that come back, are not dropped without a word."""
+    import torch.autograd.forward_ad as fw
+    g = generator(3)
+    table, y, w = (torch.randn(*shape, generator=g, device="cuda") for shape in ((10, 8), (6, 8), (3, 2)))
+    ids, order = torch.tensor([3, 1, 3], device="cuda"), nn.expert_order(torch.tensor([[0, 1], [1, -1], [0, 0]], device="cuda"), 2)
+    x = torch.randn(3, 8, generator=g, device="cuda")
+    calls = [(table, lambda t: nn.embedding(t, ids)), (table, lambda t: nn.embedding(t, ids, sparse=True)), (x, lambda t: nn.dispatch(t, order)),
+             (y, lambda t: nn.combine(t, order)), (y, lambda t: nn.combine(t, order, w)), (w, lambda t: nn.combine(y, order, t))]
+    with fw.dual_level():
+        for leaf, call in calls:
+            for primal in (leaf, leaf.clone().requires_grad_()):
+                with pytest.raises(RuntimeError):
+                    call(fw.make_dual(primal, torch.ones_like(leaf)))
+            back = leaf.clone().requires_grad_()
+            out = call(back)
+            with pytest.raises(RuntimeError):
+                torch.autograd.grad(out, back, fw.make_dual(torch.ones_like(out), torch.ones_like(out)))
+            assert torch.autograd.grad(call(back), back, torch.ones_like(out))[0] is not None
+    for leaf, call in calls:
+        call(leaf)
