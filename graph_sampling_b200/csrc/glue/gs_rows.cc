@@ -12,6 +12,7 @@
 #include <torch/csrc/autograd/grad_mode.h>
 #include <torch/csrc/autograd/variable.h>
 
+#include <initializer_list>
 #include <limits>
 #include <optional>
 #include <utility>
@@ -282,13 +283,16 @@ std::pair<Tensor, Tensor> combine_grad(gsb_ctx* ctx, const Tensor& grad_, const 
 gsb_ctx* kept(int64_t handle) { return reinterpret_cast<gsb_ctx*>(handle); }
 int64_t keep(gsb_ctx* ctx) { return reinterpret_cast<int64_t>(ctx); }
 
-// Gradients that are differentiated again say that they cannot be, instead of passing for constants.
-tensor_list only_once(tensor_list grads) {
+// Gradients that are differentiated again say that they cannot be, instead of passing for constants, whatever they are
+// differentiated for: the node that says so stands between them and all that they were made of.
+tensor_list only_once(tensor_list grads, std::initializer_list<Tensor> made_of) {
   if (!at::GradMode::is_enabled()) return grads;
   variable_list given;
   for (const Tensor& g : grads)
     if (g.defined()) given.push_back(g.detach().requires_grad_(true));
-  auto error = std::make_shared<torch::autograd::DelayedError>("this gradient cannot be differentiated again", (int)given.size());
+  given.insert(given.end(), made_of.begin(), made_of.end());
+  const auto count = (int)given.size();
+  auto error = std::make_shared<torch::autograd::DelayedError>("this gradient cannot be differentiated again", count);
   variable_list marked = (*error)(std::move(given));
   size_t next = 0;
   for (Tensor& g : grads)
@@ -346,7 +350,7 @@ struct EmbeddingFunction : torch::autograd::Function<EmbeddingFunction> {
         out[0] = dense_grad(ctx, grads[0], ids, rows, scale, pad, std::nullopt);
       }
     }
-    return only_once(std::move(out));
+    return only_once(std::move(out), {grads[0]});
   }
 };
 
@@ -365,7 +369,7 @@ struct DispatchFunction : torch::autograd::Function<DispatchFunction> {
       const at::NoGradGuard no_grad;
       out[0] = combine(kept(a->saved_data["handle"].toInt()), grads[0], a->get_saved_variables()[0], Tensor());
     }
-    return only_once(std::move(out));
+    return only_once(std::move(out), {grads[0]});
   }
 };
 
@@ -387,7 +391,7 @@ struct GatherFunction : torch::autograd::Function<GatherFunction> {
       const at::NoGradGuard no_grad;
       out[0] = spread(kept(a->saved_data["handle"].toInt()), grads[0], place, Tensor()).narrow(0, 0, a->saved_data["rows"].toInt());
     }
-    return only_once(std::move(out));
+    return only_once(std::move(out), {grads[0]});
   }
 };
 
@@ -408,7 +412,7 @@ struct CombineFunction : torch::autograd::Function<CombineFunction> {
       std::tie(out[0], out[2]) = combine_grad(kept(a->saved_data["handle"].toInt()), grads[0], saved[0], saved[1], saved[2],
                                               a->needs_input_grad(0), a->needs_input_grad(2));
     }
-    return only_once(std::move(out));
+    return only_once(std::move(out), {grads[0], saved[0], saved[2]});
   }
 };
 

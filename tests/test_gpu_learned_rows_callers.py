@@ -136,3 +136,25 @@ def test_forward_mode_is_refused(nn):
             assert torch.autograd.grad(call(back), back, torch.ones_like(out))[0] is not None
     for leaf, call in calls:
         call(leaf)
+
+
+def test_second_derivatives_are_refused_for_whatever_they_are_taken(nn):
+    """Not only where a backward pass meets the gradient: also towards the gradient that came in, or one operand alone."""
+    from torch.autograd import functional
+    g = generator(4)
+    table, y, w = (torch.randn(*shape, generator=g, device="cuda") for shape in ((10, 8), (6, 8), (3, 2)))
+    ids, order = torch.tensor([3, 1, 3], device="cuda"), nn.expert_order(torch.tensor([[0, 1], [1, -1], [0, 0]], device="cuda"), 2)
+    x = torch.randn(3, 8, generator=g, device="cuda")
+    for leaf, call in ((table, lambda t: nn.embedding(t, ids)), (x, lambda t: nn.dispatch(t, order)), (y, lambda t: nn.combine(t, order)),
+                       (y, lambda t: nn.combine(t, order, w)), (w, lambda t: nn.combine(y, order, t))):
+        for twice in (lambda: functional.jvp(call, leaf, torch.ones_like(leaf)),
+                      lambda: functional.hvp(lambda t: call(t).square().sum(), leaf, torch.ones_like(leaf)),
+                      lambda: functional.vhp(lambda t: call(t).square().sum(), leaf, torch.ones_like(leaf))):
+            with pytest.raises(RuntimeError, match="cannot be differentiated again"):
+                twice()
+        assert functional.vjp(call, leaf, torch.ones_like(call(leaf)))[1].shape == leaf.shape
+    rows, weights = y.clone().requires_grad_(), w.clone().requires_grad_()
+    of_rows, of_weights = torch.autograd.grad(nn.combine(rows, order, weights).sum(), (rows, weights), create_graph=True)
+    for grad, other in ((of_rows, weights), (of_weights, rows)):
+        with pytest.raises(RuntimeError, match="cannot be differentiated again"):
+            torch.autograd.grad(grad.sum(), other, allow_unused=True, retain_graph=True)
