@@ -2,7 +2,7 @@
 //
 // Lookup: out[i, :] = scale * table[ids[i], :], one rounding.
 // Gradient: total[v, :] = scale * (sum of grad[i, :] over the positions i with ids[i] == v), summed in float in the order of the
-// positions within pieces that depend on sizes alone, so the same inputs give the same bits; one rounding.  The positions are
+// positions within pieces that depend on sizes and types alone, so the same inputs give the same bits; one rounding.  The positions are
 // sorted by id (key_sort.cuh); the sorted list is cut into chunks of equal length whoever the ids are, so a frequent id is
 // shared by many groups of lanes.  A sum that begins and ends inside a chunk is written at once; what reaches over a chunk's
 // ends goes to `part` and is added up by k_join_rows.  Rows without a sum are cleared beside the sort, or, where that would write
@@ -520,6 +520,15 @@ static GradPlan grad_plan(i64 n, i64 num_rows, i64 row_len) {
   return g;
 }
 
+// Positions per chunk of a call: a matter of sizes and types, not of the addresses and strides that decide about the unit, since it
+// decides about the order of the sums.  That of the unit that fits rows at the best addresses.
+static u32 chunk_of(i64 n, i64 row_bytes, i64 most_chunks) {
+  const int unit = unit_bytes(row_bytes, 0);
+  const i64 units = row_bytes / unit;
+  const RowShape shape = row_shape(units, sum_steps(unit), sum_wide(unit));
+  return (u32)max(sum_chunk(n, shape.lanes, grid_for(units, shape.lanes * shape.steps)), (n + most_chunks - 1) / most_chunks);
+}
+
 // Leaves the shape and the chunks in `a`.
 template <class T, class O, int BYTES>
 static void launch_sum(cudaStream_t stream, SumArgs& a, i64 most_chunks, const void* grad, i64 stride_bytes, i64 row_bytes,
@@ -530,7 +539,7 @@ static void launch_sum(cudaStream_t stream, SumArgs& a, i64 most_chunks, const v
   a.lanes = shape.lanes;
   const int tiles = grid_for(a.units, shape.lanes * shape.steps);
   const i64 n = a.n;
-  a.chunk = (u32)max(sum_chunk(n, shape.lanes, tiles), (n + most_chunks - 1) / most_chunks);
+  a.chunk = chunk_of(n, row_bytes, most_chunks);
   with_steps(shape.steps, [&](auto steps) {
     const dim3 grid(grid_for((n + a.chunk - 1) / a.chunk * a.lanes, kSumThreads), tiles);
     constexpr int S = decltype(steps)::value;

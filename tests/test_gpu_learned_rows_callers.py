@@ -158,3 +158,29 @@ def test_second_derivatives_are_refused_for_whatever_they_are_taken(nn):
     for grad, other in ((of_rows, weights), (of_weights, rows)):
         with pytest.raises(RuntimeError, match="cannot be differentiated again"):
             torch.autograd.grad(grad.sum(), other, allow_unused=True, retain_graph=True)
+
+
+# ---- addresses and waits ----------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,code", [(torch.float32, 0), (torch.float16, 1), (torch.bfloat16, 2)])
+@pytest.mark.parametrize("n,rows,width", [(60_000, 40, 256), (300_007, 4, 130), (9000, 2, 1032), (200_000, 70, 24)])
+def test_the_same_bits_at_any_address_and_stride(ops, dtype, code, n, rows, width):
+    """Long sums, whose pieces decide about the last bits."""
+    g = generator(4)
+    ids = torch.randint(0, rows, (n,), generator=g, device="cuda")
+    grad = torch.randn(n, width, generator=g, device="cuda").to(dtype)
+    want = ops.embedding_grad(grad, ids, rows), ops.embedding_grad(grad, ids, rows, dtype=torch.float32)
+    for shift, gap in ((1, 0), (2, 0), (4, 0), (0, 1), (0, 2), (3, 5), (0, 8)):
+        room = torch.empty(shift + n * (width + gap), dtype=dtype, device="cuda")
+        there = room[shift:].as_strided((n, width), (width + gap, 1))
+        there.copy_(grad)
+        assert torch.equal(ops.embedding_grad(there, ids, rows), want[0])
+        assert torch.equal(ops.embedding_grad(there, ids, rows, dtype=torch.float32), want[1])
+        row_ids, some = ops.embedding_grad_rows(there, ids, rows)
+        assert torch.equal(some, want[0][row_ids])
+    ctx = ops.default_context()
+    work = torch.empty(ctx.lib.gsb_embedding_grad_workspace(n, rows, width), dtype=torch.uint8, device="cuda")
+    for shift in (1, 2, 4):
+        out = torch.empty(shift + rows * width, dtype=dtype, device="cuda")[shift:].view(rows, width)
+        assert ctx.lib.gsb_embedding_grad(ctx.handle, stream(), grad.data_ptr(), code, width, width, ids.data_ptr(), n, rows, 1.0, 0, 0,
+                                          out.data_ptr(), code, work.data_ptr(), work.numel()) == 0
+        assert torch.equal(out, want[0])
