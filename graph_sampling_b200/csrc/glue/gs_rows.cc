@@ -54,6 +54,9 @@ int dtype_of(const Tensor& t, const char* name) {
   }
 }
 
+// The tensor itself, or a copy where its memory holds the negative of its values (the imaginary part of a conjugate).
+Tensor as_stored(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+
 // A matrix whose rows are runs of memory, at any distance from each other; a copy where they are not.
 struct Rows {
   Tensor t;
@@ -65,14 +68,14 @@ Rows rows_of(const Tensor& t, const char* name, bool pinned_too = false) {
   Rows r;
   r.dtype = dtype_of(t, name);
   refuse_unless(t.dim() == 2, name, " must have two dimensions");
-  refuse_unless(t.is_cuda() || (pinned_too && t.is_pinned()), name,
+  r.t = as_stored(t);
+  refuse_unless(r.t.is_cuda() || (pinned_too && r.t.is_pinned()), name,
                 pinned_too ? " must live on the GPU or in pinned host memory" : " must be a CUDA tensor");
   r.n = t.size(0);
   r.width = t.size(1);
-  r.t = t;
-  if (r.width > 1 && t.stride(1) != 1) {
+  if (r.width > 1 && r.t.stride(1) != 1) {
     refuse_unless(t.is_cuda(), name, ": rows of a pinned host tensor must be contiguous");
-    r.t = t.contiguous();
+    r.t = r.t.contiguous();
   }
   r.stride = r.n > 1 ? r.t.stride(0) : r.width;
   return r;
@@ -80,7 +83,7 @@ Rows rows_of(const Tensor& t, const char* name, bool pinned_too = false) {
 Tensor ids_of(const Tensor& t, const char* name) {
   refuse_unless(t.scalar_type() == at::kLong, name, " must be int64");
   refuse_unless(t.is_cuda(), name, " must be a CUDA tensor");
-  return t.contiguous();
+  return as_stored(t).contiguous();
 }
 void same_device(const Tensor& a, const Tensor& b) {
   refuse_unless(a.device() == b.device(), "tensors of one call must live on the same device");
@@ -217,7 +220,7 @@ WeightsOf weights_of(const Tensor& w, const Tensor& place, const Rows& rows) {
   refuse_unless(w.sizes() == place.sizes(), "weights must have the shape of place");
   refuse_unless(w.is_cuda(), "weights must be a CUDA tensor");
   same_device(w, rows.t);
-  r.t = w.contiguous();
+  r.t = as_stored(w).contiguous();
   return r;
 }
 

@@ -160,6 +160,29 @@ def test_second_derivatives_are_refused_for_whatever_they_are_taken(nn):
             torch.autograd.grad(grad.sum(), other, allow_unused=True, retain_graph=True)
 
 
+@pytest.mark.parametrize("width", [1, 6])
+def test_views_that_stand_for_their_negative(ops, nn, width):
+    """The imaginary part of a conjugate shares its memory and differs in sign."""
+    g = generator(5)
+    negative = lambda n, w=width: torch.view_as_complex(torch.randn(n, w, 2, generator=g, device="cuda")).conj().imag
+    flat = lambda n, w=width: torch._neg_view(torch.randn(n, w, generator=g, device="cuda"))
+    ids = torch.randint(0, 9, (40,), generator=g, device="cuda")
+    order = ops.expert_order(torch.randint(0, 4, (20, 2), generator=g, device="cuda"), 4)[2]
+    for make in (negative, flat):
+        table, x, y, w, up, ups = make(9), make(20), make(40), make(20, 2), make(40), make(20)
+        assert table.is_neg() and w.is_neg()
+        plain = lambda t: t.resolve_neg().clone().contiguous()
+        assert torch.equal(ops.embedding_lookup(table, ids), plain(table)[ids])
+        assert torch.equal(ops.embedding_grad(up, ids, 9), ops.embedding_grad(plain(up), ids, 9))
+        assert torch.equal(ops.embedding_grad_rows(up, ids, 9)[1], ops.embedding_grad_rows(plain(up), ids, 9)[1])
+        assert torch.equal(ops.expert_dispatch(x, order, w), ops.expert_dispatch(plain(x), order, plain(w)))
+        assert torch.equal(ops.expert_combine(y, order, w), ops.expert_combine(plain(y), order, plain(w)))
+        for a, b in zip(ops.expert_combine_grad(ups, y, order, w), ops.expert_combine_grad(plain(ups), plain(y), order, plain(w))):
+            assert torch.equal(a, b)
+        leaf = plain(table).requires_grad_()
+        assert torch.equal(torch.autograd.grad(nn.embedding(leaf, ids), leaf, up)[0], ops.embedding_grad(plain(up), ids, 9))
+
+
 # ---- addresses and waits ----------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype,code", [(torch.float32, 0), (torch.float16, 1), (torch.bfloat16, 2)])
 @pytest.mark.parametrize("n,rows,width", [(60_000, 40, 256), (300_007, 4, 130), (9000, 2, 1032), (200_000, 70, 24)])
