@@ -9,6 +9,7 @@ import torch
 import learned_rows as exact
 
 pytestmark = pytest.mark.gpu
+TIMEOUT = -5
 
 
 @pytest.fixture(scope="module")
@@ -207,3 +208,105 @@ def test_the_same_bits_at_any_address_and_stride(ops, dtype, code, n, rows, widt
         assert ctx.lib.gsb_embedding_grad(ctx.handle, stream(), grad.data_ptr(), code, width, width, ids.data_ptr(), n, rows, 1.0, 0, 0,
                                           out.data_ptr(), code, work.data_ptr(), work.numel()) == 0
         assert torch.equal(out, want[0])
+
+
+@pytest.mark.parametrize("kind", ["dense", "rows", "order", "order of many"])
+def test_a_wait_that_does_run_out(ops, kind):
+    """Ids read in place from host memory: the sort's CTAs come to their barrier one after the other, and the first gives up."""
+    g = generator(6)
+    n, rows, width, pad = 400_000, 30_000, 8, 64
+    experts = rows if kind == "order of many" else 50
+    ids = torch.randint(0, experts if kind.startswith("order") else rows, (n,), generator=g, device="cuda")
+    there = ids.cpu().pin_memory()
+    grad = torch.randn(n, width, generator=g, device="cuda")
+    ctx = ops.Context()
+    lib, h, s = ctx.lib, ctx.handle, stream()
+    size = lib.gsb_expert_order_workspace(n, experts) if kind.startswith("order") else lib.gsb_embedding_grad_workspace(n, rows, width)
+    work = torch.empty(size, dtype=torch.uint8, device="cuda")
+
+    def room(count, dtype):
+        return torch.full((count + pad,), -7, dtype=dtype, device="cuda")
+
+    def call(count_host=None):
+        if kind == "dense":
+            out = [room(rows * width, torch.float32)]
+            st = lib.gsb_embedding_grad(h, s, grad.data_ptr(), 0, width, width, there.data_ptr(), n, rows, 1.0, 0, 0, out[0].data_ptr(), 0,
+                                        work.data_ptr(), size)
+        elif kind == "rows":
+            out = [room(n, torch.int64), room(n * width, torch.float32), room(1, torch.int64)]
+            st = lib.gsb_embedding_grad_rows(h, s, grad.data_ptr(), 0, width, width, there.data_ptr(), n, rows, 1.0, 0, 0, out[0].data_ptr(),
+                                             out[1].data_ptr(), 0, out[2].data_ptr(), work.data_ptr(), size, count_host)
+        else:
+            out = [room(experts + 1, torch.int64), room(n, torch.int64), room(n, torch.int64)]
+            st = lib.gsb_expert_order(h, s, there.data_ptr(), n, experts, *(t.data_ptr() for t in out), work.data_ptr(), size)
+        assert all(bool((t[-pad:] == -7).all()) for t in out)       # nothing is written behind a result, wait or no wait
+        return st, [t[:-pad] for t in out]
+
+    st, want = call()
+    assert st == 0 and lib.gsb_check_device_status(h, s) == 0
+    usual = ctx.get_option("max_polls")
+    ctx.set_option("max_polls", 1)
+    for _ in range(3):
+        st, got = call()
+        assert st == 0 and lib.gsb_check_device_status(h, s) == TIMEOUT
+        if kind == "dense":
+            continue                                                # anything at all
+        if kind == "rows":
+            assert int(got[2]) == 0
+            number = ctypes.c_int64(-1)
+            assert call(ctypes.byref(number))[0] == TIMEOUT and number.value == 0
+        else:
+            offsets, source, place = got
+            assert 0 <= int(offsets.min()) and int(offsets.max()) <= n and 0 <= int(source.min()) and int(source.max()) < n
+            assert -n <= int(place.min()) and int(place.max()) < n
+    ctx.set_option("max_polls", usual)
+    st, got = call()
+    assert st == 0 and lib.gsb_check_device_status(h, s) == 0
+    number = int(want[2]) if kind == "rows" else None
+    if kind == "rows":
+        got, want = [got[0][:number], got[1][:number * width], got[2]], [want[0][:number], want[1][:number * width], want[2]]
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+# ---- values -------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_infinities_and_nan_that_count(ops, dtype):
+    """They reach the sums that they belong to and no other, in short sums and in those that many chunks share."""
+    g = generator(8)
+    n, rows, width = 5000, 6, 40
+    ids = torch.randint(0, 3, (n,), generator=g, device="cuda") * 2
+    grad = torch.randn(n, width, generator=g, device="cuda").to(dtype)
+    grad[ids == 0] = 1.0
+    grad[int((ids == 0).nonzero()[7]), 3] = float("inf")
+    at = (ids == 2).nonzero().flatten()
+    grad[at[5], 4], grad[at[900], 4] = float("inf"), float("-inf")
+    grad[at[11], 5] = float("nan")
+    out = ops.embedding_grad(grad, ids, rows, 0.5)
+    want = torch.zeros(rows, width, dtype=torch.float64, device="cuda").index_add_(0, ids, grad.double()) * 0.5
+    assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out.isposinf(), want.isposinf()) and not out.isneginf().any()
+    assert out[0, 3] == float("inf") and out[2, 4].isnan() and out[2, 5].isnan()
+    row_ids, some = ops.embedding_grad_rows(grad, ids, rows, 0.5)
+    assert row_ids.tolist() == [0, 2, 4] and torch.equal(some.nan_to_num(3.0), out[::2].nan_to_num(3.0))
+    order = torch.tensor([[0, 2], [1, 3], [4, ~5]], device="cuda")
+    y = torch.ones(6, width, dtype=dtype, device="cuda")
+    y[0, 1], y[2, 1], y[3, 2], y[5] = float("inf"), float("-inf"), float("nan"), float("nan")
+    got = ops.expert_combine(y, order)
+    assert got[0, 1].isnan() and got[1, 2].isnan() and int(got.isnan().sum()) == 2 and torch.all(got[2] == 1)
+    grad_rows, grad_weights = ops.expert_combine_grad(torch.ones(3, width, dtype=dtype, device="cuda"), y, order,
+                                                      torch.tensor([[2.0, 1.0], [float("inf"), 1.0], [1.0, float("nan")]], device="cuda"))
+    assert grad_weights[0].tolist() == [float("inf"), float("-inf")] and grad_weights[1, 1].isnan() and grad_weights[2].tolist() == [width, 0]
+    assert torch.all(grad_rows[1].isposinf()) and torch.all(grad_rows[5] == 0) and torch.all(grad_rows[0] == 2)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("width,n", [(1, 500), (33, 3000), (101, 40_000), (601, 30_000), (4095, 4000)])
+def test_odd_rows_out_of_pinned_host_memory(ops, nn, dtype, width, n):
+    table = torch.randn(501, width).to(dtype).pin_memory()
+    g = generator(9)
+    ids = torch.randint(0, 501, (n,), generator=g, device="cuda")
+    there = table.cuda()
+    assert torch.equal(ops.embedding_lookup(table, ids), there[ids])
+    want = there[ids] * 0.5
+    want[ids == 7] = 0
+    assert torch.equal(ops.embedding_lookup(table, ids, 0.5, 7), want) and torch.equal(nn.embedding(table, ids, 0.5, 7), want)
+    assert torch.equal(ops.embedding_lookup(table[3:], ids.clamp(max=497)), there[3:][ids.clamp(max=497)])
