@@ -456,7 +456,8 @@ def expert_order(expert_ids, num_experts, ctx=None):
 
 def expert_dispatch(x, place, weights=None, ctx=None):
     """rows[place[t, k], :] = x[t, :], times weights[t, k] where given → one row per slot; zeros in the rows of slots without
-    an expert.  `place` as expert_order gives it: no row of two slots."""
+    an expert.  `place` as expert_order gives it: no row of two slots, and none left out (a row that no place names holds
+    anything)."""
     ctx = _context_for(place, ctx)
     return ctx.native.expert_dispatch(ctx.address, x, place, weights)
 
@@ -470,7 +471,7 @@ def expert_combine(rows, place, weights=None, ctx=None):
 
 
 def expert_combine_grad(grad, rows, place, weights=None, ctx=None):
-    """Gradients of `expert_combine` → (of rows, of weights or None)."""
+    """Gradients of `expert_combine` → (of rows, of weights or None).  A row that no place names holds anything."""
     ctx = _context_for(place, ctx)
     return ctx.native.expert_combine_grad(ctx.address, grad, rows, place, weights)
 

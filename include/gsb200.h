@@ -611,13 +611,13 @@ GSB_API int gsb_expert_order(gsb_ctx* ctx, void* stream, const int64_t* experts,
                              int64_t* out_offsets, int64_t* out_source, int64_t* out_place, void* workspace,
                              int64_t workspace_bytes);
 /* Slot t * per_token + k is the k-th of token t; tokens * per_token is below 2^31.  place: as gsb_expert_order gives it, no row of
- * two slots.  Spread: out_rows[place[t, k], :] = weights[t, k] * x[t, :], zeros in the rows of slots without an expert;
- * tokens * per_token rows.  Combine: out[t, :] = sum over k of weights[t, k] * rows[place[t, k], :], slots without an expert left
- * out; num_rows at most tokens * per_token (fewer where the
- * caller leaves rows of slots without an expert away).  weights: NULL (all 1), of type dtype or GSB_F32.  The gradient of spread without weights
- * is combine without weights; that of combine is out_grad_rows = spread of grad (NULL: not wanted) and
- * out_grad_weights[t, k] = <grad[t, :], rows[place[t, k], :]> (NULL: not wanted; else of the weights' type), 0 for slots without
- * an expert. */
+ * two slots, and none left out.  Spread: out_rows[place[t, k], :] = weights[t, k] * x[t, :], zeros in the rows of slots without an
+ * expert; tokens * per_token rows, of which those that no place names (others are out of range) are left as they are.  Combine:
+ * out[t, :] = sum over k of weights[t, k] * rows[place[t, k], :], slots without an expert left out; num_rows at most
+ * tokens * per_token (fewer where the caller leaves rows of slots without an expert away).  weights: NULL (all 1), of type dtype or
+ * GSB_F32.  The gradient of spread without weights is combine without weights; that of combine is out_grad_rows = spread of grad
+ * (NULL: not wanted) and out_grad_weights[t, k] = <grad[t, :], rows[place[t, k], :]> (NULL: not wanted; else of the weights' type),
+ * 0 for slots without an expert. */
 GSB_API int gsb_expert_spread(gsb_ctx* ctx, void* stream, const void* x, int dtype, int64_t tokens, int64_t per_token,
                               int64_t row_len, int64_t x_stride, const int64_t* place, const void* weights,
                               int weights_dtype, void* out_rows);

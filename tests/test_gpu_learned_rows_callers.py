@@ -268,6 +268,40 @@ def test_a_wait_that_does_run_out(ops, kind):
     assert all(torch.equal(x, y) for x, y in zip(got, want))
 
 
+def test_what_places_out_of_range_leave(ops):
+    """Rows that no place names are not written; the others are right; sums leave bad places out."""
+    g = generator(7)
+    ctx = ops.Context()
+    tokens, per_token, width = 50, 3, 20
+    slots = tokens * per_token
+    place = torch.randperm(slots, generator=g, device="cuda").view(tokens, per_token)
+    bad = torch.rand(tokens, per_token, generator=g, device="cuda") < 0.2
+    given = torch.where(bad, torch.where(torch.rand(tokens, per_token, generator=g, device="cuda") < 0.5, slots, -(1 << 40)), place)
+    x, y = torch.randn(tokens, width, generator=g, device="cuda"), torch.randn(slots, width, generator=g, device="cuda")
+    w = torch.rand(tokens, per_token, generator=g, device="cuda")
+    named = torch.zeros(slots, dtype=torch.bool, device="cuda")
+    named[place[~bad]] = True
+    lib, h, s = ctx.lib, ctx.handle, stream()
+    out = torch.full((slots, width), 7.0, device="cuda")
+    assert lib.gsb_expert_spread(h, s, x.data_ptr(), 0, tokens, per_token, width, width, given.data_ptr(), None, 0, out.data_ptr()) == 0
+    want = torch.full((slots, width), 7.0, device="cuda")
+    want[place.reshape(-1)] = x.repeat_interleave(per_token, 0)
+    want[~named] = 7.0
+    assert torch.equal(out, want) and lib.gsb_check_device_status(h, s) == -8
+    rows, weights = torch.full((slots, width), 7.0, device="cuda"), torch.full((tokens, per_token), 7.0, device="cuda")
+    up = torch.randn(tokens, width, generator=g, device="cuda")
+    assert lib.gsb_expert_combine_grad(h, s, up.data_ptr(), 0, tokens, per_token, width, width, y.data_ptr(), slots, width, given.data_ptr(),
+                                       w.data_ptr(), 0, rows.data_ptr(), weights.data_ptr()) == 0
+    assert bool((rows[~named] == 7).all()) and bool((weights[bad] == 0).all()) and lib.gsb_check_device_status(h, s) == -8
+    left_out = torch.where(bad, -1, place)
+    exact.within(rows[named], *(t[named] for t in exact.spread(up, place, w)))
+    exact.within(weights, *exact.weight_grads(up, y, left_out))
+    exact.within(ops.expert_combine(y, given, w, ctx=ctx), *exact.combine(y, left_out, w))
+    assert lib.gsb_check_device_status(h, s) == -8
+    assert torch.equal(ops.expert_dispatch(x, given, ctx=ctx)[named], want[named])
+    assert lib.gsb_check_device_status(h, s) == -8
+
+
 # ---- values -------------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
 def test_infinities_and_nan_that_count(ops, dtype):
