@@ -161,16 +161,17 @@ std::mutex& ctx_rows_wait(gsb_ctx* ctx);
 void ctx_count_launches(gsb_ctx* ctx, int n);
 void ctx_count_id_bound_refusal(gsb_ctx* ctx);
 // When profiling is enabled (gsb_profile_enable) these bracket a launch with CUDA events on the
-// launching stream; otherwise they only count the launch.
-void ctx_prof_begin(gsb_ctx* ctx, int kid, cudaStream_t stream);
-void ctx_prof_end(gsb_ctx* ctx, int kid, cudaStream_t stream);
+// launching stream; otherwise they only count the launch.  One thread at a time is between them; the first returns what the second
+// takes, -1 for a launch that is not timed.
+i64 ctx_prof_begin(gsb_ctx* ctx, int kid, cudaStream_t stream);
+void ctx_prof_end(gsb_ctx* ctx, i64 at, cudaStream_t stream);
 
 struct ScopedKernelTimer {
   gsb_ctx* ctx;
-  int kid;
   cudaStream_t stream;
-  ScopedKernelTimer(gsb_ctx* c, int k, cudaStream_t s) : ctx(c), kid(k), stream(s) { ctx_prof_begin(c, k, s); }
-  ~ScopedKernelTimer() { ctx_prof_end(ctx, kid, stream); }
+  i64 at;
+  ScopedKernelTimer(gsb_ctx* c, int k, cudaStream_t s) : ctx(c), stream(s), at(ctx_prof_begin(c, k, s)) {}
+  ~ScopedKernelTimer() { ctx_prof_end(ctx, at, stream); }
 };
 
 static inline int grid_for(i64 work_items, int per_block) {

@@ -33,10 +33,11 @@ struct gsb_ctx {
   i64* counters;  // device, CNT_NUM entries and the grid-barrier word
   HostWait waits[gsb::WAITER_NUM];
   std::mutex rows_wait;  // held by the call on learned rows that waits
-  i64 launches;
+  std::atomic<i64> launches;
   i64 id_bound_refusals;
   char message[512];
-  // per-kernel event timing (off by default)
+  // per-kernel event timing (off by default); `timing` is held from a launch's first event to its second
+  std::recursive_mutex timing;
   bool profiling;
   std::vector<cudaEvent_t>* ev_begin;
   std::vector<cudaEvent_t>* ev_end;
@@ -414,29 +415,33 @@ static bool prof_records(gsb_ctx* ctx, cudaStream_t stream) {
   return cudaStreamIsCapturing(stream, &capture) == cudaSuccess && capture == cudaStreamCaptureStatusNone;
 }
 
-void ctx_prof_begin(gsb_ctx* ctx, int kid, cudaStream_t stream) {
+i64 ctx_prof_begin(gsb_ctx* ctx, int kid, cudaStream_t stream) {
   ctx->launches += 1;
-  if (!prof_records(ctx, stream)) return;
+  if (!prof_records(ctx, stream)) return -1;
+  std::unique_lock<std::recursive_mutex> lock(ctx->timing);
   if (ctx->ev_used == ctx->ev_begin->size()) {
     cudaEvent_t a, b;
-    if (cudaEventCreate(&a) != cudaSuccess || cudaEventCreate(&b) != cudaSuccess) return;
+    if (cudaEventCreate(&a) != cudaSuccess || cudaEventCreate(&b) != cudaSuccess) return -1;
     ctx->ev_begin->push_back(a);
     ctx->ev_end->push_back(b);
     ctx->ev_kid->push_back(kid);
   }
-  (*ctx->ev_kid)[ctx->ev_used] = kid;
-  cudaEventRecord((*ctx->ev_begin)[ctx->ev_used], stream);
+  const size_t at = ctx->ev_used++;
+  (*ctx->ev_kid)[at] = kid;
+  cudaEventRecord((*ctx->ev_begin)[at], stream);
+  lock.release();
+  return (i64)at;
 }
 
-void ctx_prof_end(gsb_ctx* ctx, int kid, cudaStream_t stream) {
-  (void)kid;
-  if (!prof_records(ctx, stream) || ctx->ev_used >= ctx->ev_begin->size()) return;
-  cudaEventRecord((*ctx->ev_end)[ctx->ev_used], stream);
-  ctx->ev_used += 1;
+void ctx_prof_end(gsb_ctx* ctx, i64 at, cudaStream_t stream) {
+  if (at < 0) return;
+  cudaEventRecord((*ctx->ev_end)[at], stream);
+  ctx->timing.unlock();
 }
 
 // Folds the recorded event pairs into the per-kernel totals (waits for the events).
 static void prof_collect(gsb_ctx* ctx) {
+  const std::lock_guard<std::recursive_mutex> lock(ctx->timing);
   for (size_t i = 0; i < ctx->ev_used; ++i) {
     float ms = 0.f;
     if (cudaEventSynchronize((*ctx->ev_end)[i]) == cudaSuccess &&
@@ -579,7 +584,7 @@ int gsb_ctx_get_option(gsb_ctx* ctx, int option, int64_t* value_host) {
   return GSB_OK;
 }
 
-int64_t gsb_launch_count(gsb_ctx* ctx) { return ctx ? ctx->launches : 0; }
+int64_t gsb_launch_count(gsb_ctx* ctx) { return ctx ? ctx->launches.load() : 0; }
 
 int64_t gsb_id_bound_refusals(gsb_ctx* ctx) { return ctx ? ctx->id_bound_refusals : 0; }
 
@@ -595,6 +600,7 @@ int gsb_read_counts(gsb_ctx* ctx, void* stream, int64_t* nnz_host, int64_t* uniq
 
 int gsb_profile_enable(gsb_ctx* ctx, int on) {
   if (!ctx) return GSB_ERR_INVALID_ARGUMENT;
+  const std::lock_guard<std::recursive_mutex> lock(ctx->timing);
   if (!on && ctx->profiling) gsb::prof_collect(ctx);
   if (on) {
     // Events are created here, not at the first launches that need them: creating an event is a driver call that
@@ -614,6 +620,7 @@ int gsb_profile_enable(gsb_ctx* ctx, int on) {
 
 int gsb_profile_reset(gsb_ctx* ctx) {
   if (!ctx) return GSB_ERR_INVALID_ARGUMENT;
+  const std::lock_guard<std::recursive_mutex> lock(ctx->timing);
   gsb::prof_collect(ctx);
   for (int k = 0; k < gsb::KID_NUM; ++k) {
     ctx->prof_ms[k] = 0.0;
@@ -636,6 +643,7 @@ const char* gsb_profile_kernel_name(int kid) {
 
 int gsb_profile_read(gsb_ctx* ctx, int kid, double* total_ms, int64_t* launches) {
   if (!ctx || kid < 0 || kid >= gsb::KID_NUM) return GSB_ERR_INVALID_ARGUMENT;
+  const std::lock_guard<std::recursive_mutex> lock(ctx->timing);
   gsb::prof_collect(ctx);
   if (total_ms) *total_ms = ctx->prof_ms[kid];
   if (launches) *launches = ctx->prof_launches[kid];

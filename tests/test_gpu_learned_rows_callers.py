@@ -115,6 +115,31 @@ def test_long_odd_rows_of_two_widths_looked_up_by_two_threads(ops, dtype):
     at_once(job(4095, 4000), job(2047, 8000))
 
 
+def test_timers_and_counts_of_two_threads(ops):
+    """Every launch is counted and timed as what it is, whoever else launches through the context meanwhile."""
+    g = generator(10)
+    table = torch.randn(500, 64, generator=g, device="cuda")
+    ids = torch.randint(0, 500, (20_000,), generator=g, device="cuda")
+    grad = torch.randn(20_000, 64, generator=g, device="cuda")
+    ctx = ops.Context()
+    ops.embedding_lookup(table, ids, ctx=ctx), ops.embedding_grad(grad, ids, 500, ctx=ctx)
+    before = ctx.launch_count()
+    ops.embedding_lookup(table, ids, ctx=ctx)
+    of_lookup = ctx.launch_count() - before
+    ops.embedding_grad(grad, ids, 500, ctx=ctx)
+    of_grad = ctx.launch_count() - before - of_lookup
+    ctx.profile_enable(True)
+    ctx.profile_reset()
+    before = ctx.launch_count()
+    at_once(lambda: [ops.embedding_lookup(table, ids, ctx=ctx) for _ in range(600)],
+            lambda: [ops.embedding_grad(grad, ids, 500, ctx=ctx) for _ in range(400)])
+    times = ctx.profile_read()
+    ctx.profile_enable(False)
+    assert ctx.launch_count() - before == 600 * of_lookup + 400 * of_grad
+    assert {name: n for name, (ms, n) in times.items()} == {"embed_lookup": 600, "key_sort": 400, "embed_grad": 400}
+    assert all(ms > 0 for ms, n in times.values())
+
+
 # ---- kinds of tensors ----------------------------------------------------------------------------------------------------------
 def test_forward_mode_is_refused(nn):
     """Tangents of what goes in, and of the gradients that come back, are not dropped without a word."""
