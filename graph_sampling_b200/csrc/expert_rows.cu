@@ -260,9 +260,8 @@ extern "C" int64_t gsb_expert_order_workspace(int64_t n, int64_t num_experts) {
   return (int64_t)key_sort_bytes(n, num_experts);
 }
 
-extern "C" int gsb_expert_order(gsb_ctx* ctx, void* stream_, const int64_t* experts, int64_t n, int64_t num_experts,
-                                int64_t* out_offsets, int64_t* out_source, int64_t* out_place, void* workspace,
-                                int64_t workspace_bytes) {
+static int order(gsb_ctx* ctx, void* stream_, const int64_t* experts, int64_t n, int64_t num_experts, int most_ctas,
+                 int64_t* out_offsets, int64_t* out_source, int64_t* out_place, void* workspace, int64_t workspace_bytes) {
   GSB_ENTER(ctx);
   const int64_t need = gsb_expert_order_workspace(n, num_experts);
   GSB_REQUIRE(need >= 0 && out_offsets, GSB_ERR_INVALID_ARGUMENT);
@@ -279,8 +278,22 @@ extern "C" int gsb_expert_order(gsb_ctx* ctx, void* stream_, const int64_t* expe
   call.offsets = out_offsets;
   call.order_source = out_source;
   call.place = out_place;
+  call.most_ctas = most_ctas;
   ScopedKernelTimer timer(ctx, KID_KEY_SORT, stream);
   return key_sort(ctx, stream, call, workspace, nullptr);
+}
+
+extern "C" int gsb_expert_order(gsb_ctx* ctx, void* stream, const int64_t* experts, int64_t n, int64_t num_experts,
+                                int64_t* out_offsets, int64_t* out_source, int64_t* out_place, void* workspace,
+                                int64_t workspace_bytes) {
+  return order(ctx, stream, experts, n, num_experts, kNumSMs, out_offsets, out_source, out_place, workspace, workspace_bytes);
+}
+
+extern "C" int gsb_selftest_expert_order(gsb_ctx* ctx, void* stream, const int64_t* experts, int64_t n, int64_t num_experts,
+                                         int most_ctas, int64_t* out_offsets, int64_t* out_source, int64_t* out_place,
+                                         void* workspace, int64_t workspace_bytes) {
+  GSB_REQUIRE(most_ctas >= 1, GSB_ERR_INVALID_ARGUMENT);
+  return order(ctx, stream, experts, n, num_experts, most_ctas, out_offsets, out_source, out_place, workspace, workspace_bytes);
 }
 
 extern "C" int gsb_expert_spread(gsb_ctx* ctx, void* stream_, const void* x, int dtype, int64_t tokens, int64_t per_token,

@@ -626,7 +626,7 @@ struct Plan {
   }
 };
 
-Plan plan_of(i64 n, i64 num_keys) {
+Plan plan_of(i64 n, i64 num_keys, int most = kNumSMs) {  // most: CTAs of a large sort
   Plan p;
   int bits = 1;  // of the largest key, num_keys itself
   while (bits < 32 && (num_keys >> bits) != 0) ++bits;
@@ -635,15 +635,15 @@ Plan plan_of(i64 n, i64 num_keys) {
   // bits, of which the grid makes two passes, 20.8 and 17.9.
   p.cluster = n <= (i64)kClusterCtas * kClusterThreads * (bits <= kGridBits ? kRounds / 2 : kRounds);
   const i64 threads = p.threads(), shares = (n + threads - 1) / threads;
-  const i64 most_ctas = !p.cluster ? kNumSMs : shares <= kAloneShares ? 1 : kClusterCtas;
+  const i64 most_ctas = !p.cluster ? most : shares <= kAloneShares ? 1 : kClusterCtas;
   const i64 per = (shares + most_ctas - 1) / most_ctas;
   p.stretch = (u32)(per * threads);
   p.ctas = (int)((shares + per - 1) / per);
   p.single = per <= kRounds;
   const i64 tiles = (per + kRounds - 1) / kRounds;  // of a stretch, about equal
   p.rounds = (int)((per + tiles - 1) / tiles);
-  const int most = p.cluster ? kClusterBits : bits <= kGridBits || n <= kFewPositions ? kGridBits : kGridBits - 1;
-  p.passes = (bits + most - 1) / most;
+  const int widest = p.cluster ? kClusterBits : bits <= kGridBits || n <= kFewPositions ? kGridBits : kGridBits - 1;
+  p.passes = (bits + widest - 1) / widest;
   p.digit = (bits + p.passes - 1) / p.passes;
   if (p.digit < kMinBits) p.digit = kMinBits;
   return p;
@@ -731,7 +731,13 @@ size_t key_sort_bytes(i64 n, i64 num_keys) {
 
 int key_sort(gsb_ctx* ctx, cudaStream_t stream, const SortCall& call, void* workspace, const u64** pairs) {
   const i64 n = call.source.n;
-  const Plan p = plan_of(n, call.source.num_keys);
+  int clusters = 0;
+  const int st = prepare(ctx, &clusters);
+  if (st != GSB_OK) return st;
+  static int resident[64];
+  const int most = min(call.most_ctas, ctx_resident_ctas(ctx, kernel_of(false, kGridBits), kGridThreads, kMostShared, resident));
+  const Plan p = plan_of(n, call.source.num_keys, max(1, most));  // fewer CTAs need less of the workspace
+  GSB_REQUIRE(p.cluster || most > 0, GSB_ERR_UNSUPPORTED);
   Pieces w(workspace);
   u64* word = w.take<u64>(32);
   SortArgs a;
@@ -757,16 +763,13 @@ int key_sort(gsb_ctx* ctx, cudaStream_t stream, const SortCall& call, void* work
   // and 1.25 GB 382 us, 371 with all of it behind).
   const i64 steps = p.passes * 2;
   a.pieces = p.single ? (int)min((i64)kPiecesAtOnce, (pieces / kNumSMs + steps - 1) / steps) : 0;
-  int clusters = 0;
-  const int st = prepare(ctx, &clusters);
-  if (st != GSB_OK) return st;
   if (p.cluster) {  // CTAs that clear come in clusters too, as many as the GPU holds beside the one that sorts
     const i64 more = min((pieces + kClusterCtas - 1) / kClusterCtas, (i64)(clusters - 1)) * kClusterCtas;
     return launch(ctx, stream, a, true, p.digit, (int)(kClusterCtas + more), smem);
   }
   GSB_CUDA_OK(launch_behind(stream, k_clear_word, dim3(1), 1, word));
   ctx_count_launches(ctx, 1);
-  return launch(ctx, stream, a, false, p.digit, (int)(p.ctas + min(pieces, (i64)(kNumSMs - p.ctas))), smem);
+  return launch(ctx, stream, a, false, p.digit, (int)(p.ctas + min(pieces, (i64)(most - p.ctas))), smem);
 }
 
 }  // namespace gsb

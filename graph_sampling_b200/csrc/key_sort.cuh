@@ -36,6 +36,8 @@ struct SortCall {
   // bytes set to zero on the way: the rows of a dense gradient
   void* zero = nullptr;
   size_t zero_bytes = 0;
+  // CTAs of a large sort, at most; no more than are resident at once
+  int most_ctas = kNumSMs;
   // SORT_RANKS
   i64* distinct = nullptr;
   i64* number = nullptr;

@@ -610,6 +610,10 @@ GSB_API int64_t gsb_expert_order_workspace(int64_t n, int64_t num_experts);
 GSB_API int gsb_expert_order(gsb_ctx* ctx, void* stream, const int64_t* experts, int64_t n, int64_t num_experts,
                              int64_t* out_offsets, int64_t* out_source, int64_t* out_place, void* workspace,
                              int64_t workspace_bytes);
+/* Self-test: the same by at most `most_ctas` CTAs where it is more than one cluster's work, as on a GPU that holds fewer at once. */
+GSB_API int gsb_selftest_expert_order(gsb_ctx* ctx, void* stream, const int64_t* experts, int64_t n, int64_t num_experts,
+                                      int most_ctas, int64_t* out_offsets, int64_t* out_source, int64_t* out_place,
+                                      void* workspace, int64_t workspace_bytes);
 /* Slot t * per_token + k is the k-th of token t; tokens * per_token is below 2^31.  place: as gsb_expert_order gives it, no row of
  * two slots, and none left out.  Spread: out_rows[place[t, k], :] = weights[t, k] * x[t, :], zeros in the rows of slots without an
  * expert; tokens * per_token rows, of which those that no place names (others are out of range) are left as they are.  Combine:

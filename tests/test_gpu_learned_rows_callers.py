@@ -327,6 +327,26 @@ def test_what_places_out_of_range_leave(ops):
     assert lib.gsb_check_device_status(h, s) == -8
 
 
+@pytest.mark.parametrize("n,experts", [(20_000, 50), (40_001, 7), (300_000, 1000), (123_457, 60_000), (700_001, 2000)])
+@pytest.mark.parametrize("most", [1, 2, 7, 100, 147, 148, 1000])
+def test_orders_by_fewer_ctas(ops, n, experts, most):
+    """A GPU, or a part of one, that holds fewer CTAs at once than a B200."""
+    g = generator(11)
+    ids = torch.randint(-1, experts, (n,), generator=g, device="cuda")
+    ctx = ops.Context()
+    size = ctx.lib.gsb_expert_order_workspace(n, experts)
+    work = torch.full((size + 256,), 77, dtype=torch.uint8, device="cuda")
+    offsets, source, place = (torch.full((m + 8,), -7, dtype=torch.int64, device="cuda") for m in (experts + 1, n, n))
+    assert ctx.lib.gsb_selftest_expert_order(ctx.handle, stream(), ids.data_ptr(), n, experts, most, offsets.data_ptr(), source.data_ptr(),
+                                             place.data_ptr(), work.data_ptr(), size) == 0
+    for got, want in zip((offsets, source, place), exact.order(ids, experts)):
+        assert torch.equal(got[:-8], want) and bool((got[-8:] == -7).all())
+    assert bool((work[size:] == 77).all())
+    ctx.check_device()
+    assert ctx.lib.gsb_selftest_expert_order(ctx.handle, stream(), ids.data_ptr(), n, experts, 0, offsets.data_ptr(), source.data_ptr(),
+                                             place.data_ptr(), work.data_ptr(), size) == -1
+
+
 # ---- values -------------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
 def test_infinities_and_nan_that_count(ops, dtype):
