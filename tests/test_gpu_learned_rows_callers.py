@@ -347,6 +347,18 @@ def test_orders_by_fewer_ctas(ops, n, experts, most):
                                              place.data_ptr(), work.data_ptr(), size) == -1
 
 
+@pytest.mark.parametrize("n", [1, 5, 33, 1030, 4100, 32_768, 40_003])
+@pytest.mark.parametrize("experts", [3, 2048, 2055, 65_535, 65_536])
+def test_offsets_of_experts_without_slots(ops, n, experts):
+    """Runs of them of any length in front, in between and behind."""
+    g = generator(12)
+    few = torch.randint(0, experts, (n,), generator=g, device="cuda") // 9 * 9
+    for ids in (few, few.clamp(min=experts // 2), few.clamp(max=experts // 3), torch.full_like(few, experts - 1), torch.zeros_like(few),
+                torch.full_like(few, -1), torch.where(few % 2 == 0, experts // 2, -1)):
+        for got, want in zip(ops.expert_order(ids, experts), exact.order(ids, experts)):
+            assert torch.equal(got, want)
+
+
 # ---- values -------------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
 def test_infinities_and_nan_that_count(ops, dtype):
