@@ -118,12 +118,15 @@ __global__ void __launch_bounds__(kLookupThreads) k_lookup_rows(const LookupArgs
 
 // Rows of 16-bit values that begin off the 4-byte boundaries, where a unit is one value: a warp copies the next rows into shared
 // memory in units of 16 bytes, from the boundary before a row to the one behind it, and writes whole units of the result, each out
-// of two that it straddles.  A short row's steps cost more than it gains: 500 000 of 601 values 243 us for 352, 100 000 of 1 433
-// 108 for 169, but 500 000 of 301 167 for 155 and 30 000 of 501 15 for 13.  (Where units of 4 bytes fit, nothing is gained: a million
-// rows of 1 204 bytes 479 us for 422.)
+// of two that it straddles.  A short row's steps cost more than it gains, and so do few rows, which come out of L2 (rows in no order
+// out of twice as many, bf16): 500 000 of 601 values 243 us for 352, 80 000 of 401 57 for 64, 53 000 of 601 26 for 28, 11 000 of 1 433
+// 11 for 19, 8 000 of 2 047 11.4 for 11.7, but 106 000 of 301 74 for 62, 40 000 of 401 18 for 15, 27 000 of 601 14 for 12.  (Where units
+// of 4 bytes fit, nothing is gained: a million rows of 1 204 bytes 479 us for 422.)
 constexpr int kStagedThreads = 128, kStages = 3;
 constexpr i64 kMostStagedBytes = 8192;
-static bool staged(i64 row_bytes, i64 n) { return row_bytes >= 800 && row_bytes <= kMostStagedBytes && n * row_bytes >= 32000000; }
+static bool staged(i64 row_bytes, i64 n) {
+  return row_bytes >= 800 && row_bytes <= kMostStagedBytes && n * row_bytes >= (row_bytes < 1600 ? 64000000 : 32000000);
+}
 static u32 stage_bytes(i64 row_bytes) { return (u32)((row_bytes + 15) / 16 * 16 + 16); }
 static size_t staged_smem(u32 stage) { return (size_t)(kStagedThreads / 32) * kStages * stage; }
 

@@ -359,6 +359,20 @@ def test_offsets_of_experts_without_slots(ops, n, experts):
             assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("width,n", [(399, 82_000), (401, 79_000), (401, 80_001), (601, 60_000), (799, 40_000), (799, 41_003), (801, 19_000), (801, 21_001)])
+def test_odd_rows_on_both_sides_of_the_staged_lookup(ops, dtype, width, n):
+    g = generator(13)
+    room = torch.randn(3 + 700 * (width + 4), generator=g, device="cuda").to(dtype)
+    table = room[3:].as_strided((700, width), (width + 4, 1))
+    ids = torch.randint(0, 700, (n,), generator=g, device="cuda")
+    ids[:2] = torch.tensor([0, 699])
+    assert torch.equal(ops.embedding_lookup(table, ids), table[ids])
+    want = table[ids] * 0.5
+    want[ids == 7] = 0
+    assert torch.equal(ops.embedding_lookup(table, ids, 0.5, 7), want)
+
+
 # ---- values -------------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
 def test_infinities_and_nan_that_count(ops, dtype):
