@@ -278,9 +278,8 @@ static int order(gsb_ctx* ctx, void* stream_, const int64_t* experts, int64_t n,
   call.offsets = out_offsets;
   call.order_source = out_source;
   call.place = out_place;
-  call.most_ctas = most_ctas;
   ScopedKernelTimer timer(ctx, KID_KEY_SORT, stream);
-  return key_sort(ctx, stream, call, workspace, nullptr);
+  return key_sort(ctx, stream, call, workspace, nullptr, most_ctas);
 }
 
 extern "C" int gsb_expert_order(gsb_ctx* ctx, void* stream, const int64_t* experts, int64_t n, int64_t num_experts,

@@ -753,13 +753,13 @@ size_t key_sort_bytes(i64 n, i64 num_keys) {
   return w.used;
 }
 
-int key_sort(gsb_ctx* ctx, cudaStream_t stream, const SortCall& call, void* workspace, const u64** pairs) {
+int key_sort(gsb_ctx* ctx, cudaStream_t stream, const SortCall& call, void* workspace, const u64** pairs, int most_ctas) {
   const i64 n = call.source.n;
   int clusters = 0;
   const int st = prepare(ctx, &clusters);
   if (st != GSB_OK) return st;
   static int resident[64];
-  const int most = min(call.most_ctas, ctx_resident_ctas(ctx, kernel_of(false, kGridBits), kGridThreads, kMostShared, resident));
+  const int most = min(most_ctas, ctx_resident_ctas(ctx, kernel_of(false, kGridBits), kGridThreads, kMostShared, resident));
   const Plan p = plan_of(n, call.source.num_keys, max(1, most));  // fewer CTAs need less of the workspace
   GSB_REQUIRE(p.cluster || most > 0, GSB_ERR_UNSUPPORTED);
   Pieces w(workspace);

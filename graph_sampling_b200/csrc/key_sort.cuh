@@ -36,8 +36,6 @@ struct SortCall {
   // bytes set to zero on the way: the rows of a dense gradient
   void* zero = nullptr;
   size_t zero_bytes = 0;
-  // CTAs of a large sort, at most; no more than are resident at once
-  int most_ctas = kNumSMs;
   // SORT_RANKS
   i64* distinct = nullptr;
   i64* number = nullptr;
@@ -49,7 +47,8 @@ struct SortCall {
 size_t key_sort_bytes(i64 n, i64 num_keys);
 // *pairs: the sorted pairs in `workspace` (SORT_PAIRS, SORT_RANKS).  A sort that is given up (a bounded wait ran out) leaves
 // anything at all there: what reads them checks both halves.
-int key_sort(gsb_ctx* ctx, cudaStream_t stream, const SortCall& call, void* workspace, const u64** pairs);
+// most_ctas: of a large sort; no more than are resident at once.
+int key_sort(gsb_ctx* ctx, cudaStream_t stream, const SortCall& call, void* workspace, const u64** pairs, int most_ctas = kNumSMs);
 
 // A caller's memory in pieces that start on 256-byte boundaries.
 struct Pieces {
