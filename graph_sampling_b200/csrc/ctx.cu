@@ -57,6 +57,7 @@ struct gsb_ctx {
   cudaStream_t stream;   // of the last call that used scratch
   bool stream_known;
   u64 barrier_arrivals;  // the barrier word itself is counters[CNT_NUM]
+  std::atomic<bool> barrier_marked;  // its mark may still be there although the error has been read
 };
 
 namespace gsb {
@@ -251,6 +252,13 @@ GridSync ctx_grid_sync(gsb_ctx* ctx, int grid, int barriers) {
   return g;
 }
 
+// The mark of a grid barrier that was given up, the top byte of its word (grid_sync.cuh).
+static int clear_barrier_mark(gsb_ctx* ctx, cudaStream_t stream) {
+  ctx->barrier_marked = false;
+  GSB_CUDA_OK(cudaMemsetAsync((char*)(ctx->counters + CNT_NUM) + kBarrierCountBits / 8, 0, 1, stream));
+  return GSB_OK;
+}
+
 int launch_cooperative(gsb_ctx* ctx, cudaStream_t stream, const void* kernel, int grid, int threads, size_t smem,
                        void** args, const GridSync& sync) {
   cudaLaunchConfig_t cfg = {};
@@ -263,6 +271,13 @@ int launch_cooperative(gsb_ctx* ctx, cudaStream_t stream, const void* kernel, in
   attr.val.cooperative = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
+  if (ctx->barrier_marked) {
+    const int st = clear_barrier_mark(ctx, stream);
+    if (st != GSB_OK) {
+      ctx->barrier_arrivals = sync.base;
+      return st;
+    }
+  }
   const cudaError_t e = cudaLaunchKernelExC(&cfg, kernel, args);
   if (e != cudaSuccess) {
     ctx->barrier_arrivals = sync.base;  // nothing ran: the barrier word stands where it stood
@@ -393,9 +408,13 @@ int ctx_check_device_error(gsb_ctx* ctx, cudaStream_t stream, Waiter who) {
              gsb_status_string(code), (long long)c[1]);
     GSB_CUDA_OK(cudaMemsetAsync(ctx->counters + CNT_ERROR, 0, 2 * sizeof(i64), stream));
     GSB_CUDA_OK(cudaMemsetAsync(ctx->counters + CNT_LOST, 0, sizeof(i64), stream));
-    // the mark of a grid barrier that was given up, the top byte of its word (grid_sync.cuh); calls on learned rows have words of
-    // their own, and a kernel of the context's thread may be between two looks at this one
-    if (who == WAIT_CALL) GSB_CUDA_OK(cudaMemsetAsync((char*)(ctx->counters + CNT_NUM) + kBarrierCountBits / 8, 0, 1, stream));
+    // Calls on learned rows have barrier words of their own, and a kernel of the context's thread may be between two looks at the
+    // context's: that thread clears the mark itself before it launches the next.
+    if (who == WAIT_ROWS) ctx->barrier_marked = true;
+    else {
+      const int st2 = clear_barrier_mark(ctx, stream);
+      if (st2 != GSB_OK) return st2;
+    }
     {
       int st2 = ctx_wait(ctx, stream, ctx->waits[who]);
       if (st2 != GSB_OK) return st2;

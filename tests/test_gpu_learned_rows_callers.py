@@ -373,6 +373,37 @@ def test_odd_rows_on_both_sides_of_the_staged_lookup(ops, dtype, width, n):
     assert torch.equal(ops.embedding_lookup(table, ids, 0.5, 7), want)
 
 
+def test_a_wait_of_the_sampler_that_ran_out_is_read_by_a_call_on_rows(ops):
+    """The next cooperative call of the context works again, without anybody else reading the error."""
+    g = generator(14)
+    n, keys = 300_001, 1_000_000
+    key = torch.randint(0, keys, (n,), generator=g, device="cuda")
+    there, rows_in = key.cpu().pin_memory(), torch.arange(n, device="cuda")
+    ctx = ops.Context()
+    lib, h, s = ctx.lib, ctx.handle, stream()
+
+    def convert():
+        out = [torch.empty(m, dtype=torch.int64, device="cuda") for m in (keys + 1, n, n)]
+        assert lib.gsb_coo2csc(h, s, there.data_ptr(), rows_in.data_ptr(), n, keys, 0, *(t.data_ptr() for t in out)) == 0
+        return out
+
+    want = convert()
+    ctx.check_device()
+    usual = ctx.get_option("max_polls")
+    ids, grad = torch.tensor([3, 1, 3], device="cuda"), torch.ones(3, 4, device="cuda")
+    for _ in range(3):
+        ctx.set_option("max_polls", 1)
+        convert()
+        ctx.set_option("max_polls", usual)
+        torch.cuda.synchronize()
+        with pytest.raises(Exception) as e:
+            ops.embedding_grad_rows(grad, ids, 5, ctx=ctx)
+        assert e.value.status == TIMEOUT
+        assert ops.embedding_grad_rows(grad, ids, 5, ctx=ctx)[0].tolist() == [1, 3]
+        assert all(torch.equal(x, y) for x, y in zip(convert(), want))
+        ctx.check_device()
+
+
 # ---- values -------------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
 def test_infinities_and_nan_that_count(ops, dtype):
