@@ -91,7 +91,11 @@ inline uint64_t unsigned_integer(PyObject* o) {
   if (v == (unsigned long long)-1 && PyErr_Occurred()) throw PyErrorSet();
   return v;
 }
-inline bool truth(PyObject* o) { return PyObject_IsTrue(o) == 1; }
+inline bool truth(PyObject* o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw PyErrorSet();
+  return v == 1;
+}
 inline gsb_ctx* context(PyObject* o) { return reinterpret_cast<gsb_ctx*>(unsigned_integer(o)); }
 
 inline void* stream() { return static_cast<void*>(c10::cuda::getCurrentCUDAStream().stream()); }
