@@ -15,7 +15,8 @@ ExpertOrder = namedtuple("ExpertOrder", "offsets source place")
 
 def embedding(table, ids, scale=1.0, padding_id=None, sparse=False):
     """scale * table[ids], zeros where ids == padding_id, which takes no gradient.  The table's gradient is dense, or, with
-    sparse=True, a sparse tensor of the rows that occur, each once, ascending (the backward pass then waits for their number)."""
+    sparse=True, a sparse tensor of the rows that occur, each once, ascending (the backward pass then waits for their number, and
+    the rows keep storage for all positions of `ids`: clone a gradient that stays)."""
     ctx = ops._context_for(ids)
     return ctx.native.nn_embedding(ctx.address, table, ids, scale, padding_id, sparse)
 

@@ -419,7 +419,8 @@ def take(src, index):
 
 # ---- rows that are learned -------------------------------------------------------------------
 # Rows of float32, float16 or bfloat16 values on the GPU, arithmetic in float32, every result rounded once.  These operators
-# take no gradients themselves (graph_sampling_b200.gs.nn does); they may be captured into a CUDA graph.
+# take no gradients themselves (graph_sampling_b200.gs.nn does); they may be captured into a CUDA graph, and several threads may
+# make them through one context.
 def embedding_lookup(table, ids, scale=1.0, padding_id=None, ctx=None):
     """out[..., :] = scale * table[ids[...], :] → a tensor of the shape of `ids` and the rows' width, in the table's dtype.
     Positions that hold `padding_id` (any number, -1 for instance) get zeros; so do ids outside the table, which are
@@ -438,8 +439,8 @@ def embedding_grad(grad, ids, num_rows, scale=1.0, padding_id=None, dtype=None, 
 
 
 def embedding_grad_rows(grad, ids, num_rows, scale=1.0, padding_id=None, dtype=None, sync=True, ctx=None):
-    """The rows of `embedding_grad` that occur → (row_ids, rows), row_ids ascending.  With sync=False the call does not wait
-    for their number and returns (row_ids, rows, number): what lies behind the first `number` (a tensor on the GPU) is
+    """The rows of `embedding_grad` that occur → (row_ids, rows), row_ids ascending, in storage for all positions.  With sync=False the
+    call does not wait for their number and returns (row_ids, rows, number): what lies behind the first `number` (a tensor on the GPU) is
     left as it was."""
     ctx = _context_for(ids, ctx)
     return ctx.native.embedding_grad_rows(ctx.address, grad, ids, num_rows, scale, padding_id, dtype, sync)
