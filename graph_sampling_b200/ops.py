@@ -11,6 +11,7 @@ import ctypes
 import importlib.machinery
 import importlib.util
 import os
+import threading
 
 import torch
 
@@ -18,6 +19,7 @@ from . import cabi
 from .cabi import GsbError, c_i64, c_i64p, c_int, c_u64, c_vp
 
 _contexts = {}
+_contexts_lock = threading.Lock()
 _native = None
 
 
@@ -145,8 +147,10 @@ def default_context(device=None):
     idx = torch.cuda.current_device() if device is None else (torch.device(device).index or 0)
     ctx = _contexts.get(idx)
     if ctx is None:
-        ctx = Context(torch.device("cuda", idx))
-        _contexts[idx] = ctx
+        with _contexts_lock:            # several threads may come first: one context, which whoever has its address keeps
+            ctx = _contexts.get(idx)
+            if ctx is None:
+                ctx = _contexts[idx] = Context(torch.device("cuda", idx))
     return ctx
 
 
