@@ -5,6 +5,7 @@
 // throws C++ exceptions, and the Python functions translate.  Scratch comes from torch's allocator on the current stream, call
 // by call: calls on several streams, and captured ones, share nothing but the context's error counters.
 #include <ATen/Functions.h>
+#include <ATen/core/CachingHostAllocator.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -119,6 +120,10 @@ Tensor lookup(gsb_ctx* ctx, const Tensor& table_, const Tensor& ids_, double sca
   done(ctx, gsb_embedding_lookup(ctx, stream(), table.data(), table.dtype, table.n, table.width, table.stride, ids_ptr(ids),
                                  ids.numel(), (float)scale, pad.given, pad.id, data(out)),
        "gsb_embedding_lookup");
+  // memory of the host allocator is not given to another tensor before the kernel has read it (a captured one's has to outlive the graph)
+  if (!table.t.is_cuda() && c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None)
+    at::getHostAllocator(at::kCUDA)->record_event(const_cast<void*>(table.data()), table.t.storage().data_ptr().get_context(),
+                                                  c10::cuda::getCurrentCUDAStream().unwrap());
   return out;
 }
 

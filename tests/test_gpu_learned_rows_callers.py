@@ -446,3 +446,18 @@ def test_odd_rows_out_of_pinned_host_memory(ops, nn, dtype, width, n):
     want[ids == 7] = 0
     assert torch.equal(ops.embedding_lookup(table, ids, 0.5, 7), want) and torch.equal(nn.embedding(table, ids, 0.5, 7), want)
     assert torch.equal(ops.embedding_lookup(table[3:], ids.clamp(max=497)), there[3:][ids.clamp(max=497)])
+
+
+def test_pinned_tables_that_go_at_once(ops):
+    """A table may be dropped behind the call: its memory is not handed out again while the lookup is still to come."""
+    ids = torch.arange(2000, device="cuda")
+    filler = torch.randn(4096, 4096, device="cuda")
+    ops.embedding_lookup(torch.zeros(2000, 64).pin_memory(), ids)
+    torch.cuda.synchronize()
+    for turn in range(5):
+        for _ in range(20):
+            filler @ filler                                   # long enough for the host to get ahead
+        out = ops.embedding_lookup(torch.full((2001, 64), float(turn)).pin_memory()[1:], ids)
+        later = [torch.full((2001, 64), -1.0).pin_memory() for _ in range(4)]
+        assert bool((out == turn).all())
+        del later
