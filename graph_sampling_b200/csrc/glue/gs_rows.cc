@@ -9,6 +9,7 @@
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/grad_mode.h>
 #include <torch/csrc/autograd/variable.h>
@@ -16,6 +17,7 @@
 #include <initializer_list>
 #include <limits>
 #include <optional>
+#include <unordered_set>
 #include <utility>
 
 #include "native.h"
@@ -310,15 +312,42 @@ tensor_list only_once(tensor_list grads, std::initializer_list<Tensor> made_of) 
 
 // While an eager graph of a leaf is alive, a captured backward pass would add to the leaf's gradient through that graph's node,
 // on the stream that it was made on, which ends the capture, and with it the process.  Said here, where it can still be helped.
+bool capturing() { return c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None; }
+[[noreturn]] void refuse_capture(const char* whose) {
+  throw std::runtime_error(std::string("a graph of ") + whose +
+                           " made outside the capture, on another stream, is still alive: drop its outputs before capturing");
+}
 void refuse_foreign_accumulator(const Tensor& leaf) {
-  if (!leaf.defined() || !leaf.requires_grad() || leaf.grad_fn() || !leaf.is_cuda()) return;
-  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+  if (!leaf.defined() || !leaf.requires_grad() || leaf.grad_fn() || !leaf.is_cuda() || !capturing()) return;
   const auto node = torch::autograd::impl::try_get_grad_accumulator(leaf);
   if (!node) return;
   const auto of_node = node->stream();
-  if (of_node && *of_node != c10::cuda::getCurrentCUDAStream(leaf.get_device()).unwrap())
-    throw std::runtime_error(
-        "a graph of this leaf made outside the capture, on another stream, is still alive: drop its outputs before capturing");
+  if (of_node && *of_node != c10::cuda::getCurrentCUDAStream(leaf.get_device()).unwrap()) refuse_capture("this leaf");
+}
+
+// Whether behind an operand there is, by operations of the capture alone, a leaf whose node belongs to the default stream, which cannot
+// join a capture.  Only a captured backward pass would meet it, and refuses there.
+bool foreign_leaf_behind(const Tensor& t) {
+  if (!t.defined() || !t.requires_grad() || !t.grad_fn() || !t.is_cuda() || !capturing()) return false;
+  const auto here = c10::cuda::getCurrentCUDAStream(t.get_device()).unwrap();
+  const auto never = c10::cuda::getDefaultCUDAStream(t.get_device()).unwrap();
+  std::vector<torch::autograd::Node*> left{t.grad_fn().get()};
+  std::unordered_set<torch::autograd::Node*> seen(left.begin(), left.end());
+  while (!left.empty()) {
+    torch::autograd::Node* const node = left.back();
+    left.pop_back();
+    const auto of_node = node->stream();
+    if (dynamic_cast<torch::autograd::AccumulateGrad*>(node)) {
+      if (of_node && *of_node == never) return true;
+    } else if (!of_node || *of_node == here) {
+      for (const auto& edge : node->next_edges())
+        if (edge.function && seen.insert(edge.function.get()).second) left.push_back(edge.function.get());
+    }
+  }
+  return false;
+}
+void refuse_foreign_leaf(AutogradContext* a) {
+  if (a->saved_data["foreign"].toBool() && capturing()) refuse_capture("a leaf behind this operand");
 }
 
 // The kernels read memory and know nothing of forward-mode tangents: a result without one would pass for a constant.
@@ -329,10 +358,11 @@ void refuse_tangents(const char* name, const Tensor& t) {
 
 struct EmbeddingFunction : torch::autograd::Function<EmbeddingFunction> {
   static Tensor forward(AutogradContext* a, const Tensor& table, const Tensor& ids, int64_t handle, double scale, bool padded,
-                        int64_t padding, bool sparse) {
+                        int64_t padding, bool sparse, bool foreign) {
     a->save_for_backward({ids});
     a->set_materialize_grads(false);
     a->saved_data["handle"] = handle;
+    a->saved_data["foreign"] = foreign;
     a->saved_data["scale"] = scale;
     a->saved_data["padded"] = padded;
     a->saved_data["padding"] = padding;
@@ -341,9 +371,10 @@ struct EmbeddingFunction : torch::autograd::Function<EmbeddingFunction> {
     return lookup(kept(handle), table, ids, scale, {padded, padding});
   }
   static tensor_list backward(AutogradContext* a, tensor_list grads) {
-    tensor_list out(7);
+    tensor_list out(8);
     if (!grads[0].defined()) return out;
     refuse_tangents("grad", grads[0]);
+    refuse_foreign_leaf(a);
     gsb_ctx* ctx = kept(a->saved_data["handle"].toInt());
     const Tensor ids = a->get_saved_variables()[0];
     const Padding pad{a->saved_data["padded"].toBool(), a->saved_data["padding"].toInt()};
@@ -363,16 +394,18 @@ struct EmbeddingFunction : torch::autograd::Function<EmbeddingFunction> {
 };
 
 struct DispatchFunction : torch::autograd::Function<DispatchFunction> {
-  static Tensor forward(AutogradContext* a, const Tensor& x, const Tensor& place, int64_t handle) {
+  static Tensor forward(AutogradContext* a, const Tensor& x, const Tensor& place, int64_t handle, bool foreign) {
     a->save_for_backward({place});
     a->set_materialize_grads(false);
     a->saved_data["handle"] = handle;
+    a->saved_data["foreign"] = foreign;
     return spread(kept(handle), x, place, Tensor());
   }
   static tensor_list backward(AutogradContext* a, tensor_list grads) {
-    tensor_list out(3);
+    tensor_list out(4);
     if (!grads[0].defined()) return out;
     refuse_tangents("grad", grads[0]);
+    refuse_foreign_leaf(a);
     {
       const at::NoGradGuard no_grad;
       out[0] = combine(kept(a->saved_data["handle"].toInt()), grads[0], a->get_saved_variables()[0], Tensor());
@@ -383,17 +416,19 @@ struct DispatchFunction : torch::autograd::Function<DispatchFunction> {
 
 // Without weights (autograd functions take defined tensors only).
 struct GatherFunction : torch::autograd::Function<GatherFunction> {
-  static Tensor forward(AutogradContext* a, const Tensor& rows, const Tensor& place, int64_t handle) {
+  static Tensor forward(AutogradContext* a, const Tensor& rows, const Tensor& place, int64_t handle, bool foreign) {
     a->save_for_backward({place});
     a->set_materialize_grads(false);
     a->saved_data["handle"] = handle;
+    a->saved_data["foreign"] = foreign;
     a->saved_data["rows"] = rows.size(0);
     return combine(kept(handle), rows, place, Tensor());
   }
   static tensor_list backward(AutogradContext* a, tensor_list grads) {
-    tensor_list out(3);
+    tensor_list out(4);
     if (!grads[0].defined()) return out;
     refuse_tangents("grad", grads[0]);
+    refuse_foreign_leaf(a);
     const Tensor place = a->get_saved_variables()[0];
     {
       const at::NoGradGuard no_grad;
@@ -404,16 +439,18 @@ struct GatherFunction : torch::autograd::Function<GatherFunction> {
 };
 
 struct CombineFunction : torch::autograd::Function<CombineFunction> {
-  static Tensor forward(AutogradContext* a, const Tensor& rows, const Tensor& place, const Tensor& weights, int64_t handle) {
+  static Tensor forward(AutogradContext* a, const Tensor& rows, const Tensor& place, const Tensor& weights, int64_t handle, bool foreign) {
     a->save_for_backward({rows, place, weights});
     a->set_materialize_grads(false);
     a->saved_data["handle"] = handle;
+    a->saved_data["foreign"] = foreign;
     return combine(kept(handle), rows, place, weights);
   }
   static tensor_list backward(AutogradContext* a, tensor_list grads) {
-    tensor_list out(4);
+    tensor_list out(5);
     if (!grads[0].defined()) return out;
     refuse_tangents("grad", grads[0]);
+    refuse_foreign_leaf(a);
     const auto saved = a->get_saved_variables();
     {
       const at::NoGradGuard no_grad;
@@ -555,7 +592,7 @@ FUNCTION(nn_embedding, 6) {  // (ctx, table, ids, scale, padding id | None, spar
     if (!follows(table)) return lookup(ctx, table, ids, scale, pad);
     rows_of(table, "table");
     refuse_foreign_accumulator(table);
-    return EmbeddingFunction::apply(table, ids, keep(ctx), scale, pad.given, pad.id, sparse);
+    return EmbeddingFunction::apply(table, ids, keep(ctx), scale, pad.given, pad.id, sparse, foreign_leaf_behind(table));
   }));
 }
 
@@ -566,7 +603,7 @@ FUNCTION(nn_dispatch, 3) {  // (ctx, x, place) -> rows
     refuse_tangents("x", x);
     if (!follows(x)) return spread(ctx, x, place, Tensor());
     refuse_foreign_accumulator(x);
-    return DispatchFunction::apply(x, place, keep(ctx));
+    return DispatchFunction::apply(x, place, keep(ctx), foreign_leaf_behind(x));
   }));
 }
 
@@ -580,8 +617,9 @@ FUNCTION(nn_combine, 4) {  // (ctx, rows, place, weights | None) -> out
     if (!follows(rows) && !follows(weights)) return combine(ctx, rows, place, weights);
     refuse_foreign_accumulator(rows);
     refuse_foreign_accumulator(weights);
-    if (!weights.defined()) return GatherFunction::apply(rows, place, keep(ctx));
-    return CombineFunction::apply(rows, place, weights, keep(ctx));
+    const bool foreign = foreign_leaf_behind(rows) || foreign_leaf_behind(weights);
+    if (!weights.defined()) return GatherFunction::apply(rows, place, keep(ctx), foreign);
+    return CombineFunction::apply(rows, place, weights, keep(ctx), foreign);
   }));
 }
 

@@ -209,6 +209,39 @@ def test_views_that_stand_for_their_negative(ops, nn, width):
         assert torch.equal(torch.autograd.grad(nn.embedding(leaf, ids), leaf, up)[0], ops.embedding_grad(plain(up), ids, 9))
 
 
+def test_captured_backward_passes_to_leaves_behind_a_view(nn):
+    """With an eager graph of the leaf alive the backward pass is refused, the forward call is not; without one both are captured."""
+    g = generator(15)
+    ids, order = torch.tensor([3, 1, 3], device="cuda"), nn.expert_order(torch.tensor([[0, 1], [1, -1], [0, 0]], device="cuda"), 2)
+    y = torch.randn(6, 8, generator=g, device="cuda")
+    for shape, call in (((10, 8), lambda t: nn.embedding(t, ids)), ((3, 8), lambda t: nn.dispatch(t, order)),
+                        ((6, 8), lambda t: nn.combine(t, order)), ((3, 2), lambda t: nn.combine(y, order, t))):
+        leaf = torch.randn(*shape, generator=g, device="cuda").requires_grad_()
+        up = torch.randn_like(call(leaf.detach()))
+        alive = leaf * 1
+        with pytest.raises(RuntimeError, match="behind this operand.*still alive"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                out = call(leaf.view_as(leaf)[:] * 2)
+                torch.autograd.grad(out, leaf, up)
+        del out
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            kept = call(leaf * 2).detach()                    # no backward pass: nothing to refuse
+        graph.replay()
+        assert torch.equal(kept, call(leaf.detach() * 2))
+        del alive
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            torch.autograd.grad(call(leaf * 2), leaf, up)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            grad, = torch.autograd.grad(call(leaf * 2), leaf, up)
+        graph.replay()
+        assert torch.equal(grad, torch.autograd.grad(call(leaf * 2), leaf, up)[0])
+
+
 # ---- addresses and waits ----------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype,code", [(torch.float32, 0), (torch.float16, 1), (torch.bfloat16, 2)])
 @pytest.mark.parametrize("n,rows,width", [(60_000, 40, 256), (300_007, 4, 130), (9000, 2, 1032), (200_000, 70, 24)])
