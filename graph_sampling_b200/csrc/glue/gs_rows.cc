@@ -347,7 +347,7 @@ bool foreign_leaf_behind(const Tensor& t) {
   return false;
 }
 void refuse_foreign_leaf(AutogradContext* a) {
-  if (a->saved_data["foreign"].toBool() && capturing()) refuse_capture("a leaf behind this operand");
+  if (a->saved_data.count("foreign") != 0 && capturing()) refuse_capture("a leaf behind this operand");
 }
 
 // The kernels read memory and know nothing of forward-mode tangents: a result without one would pass for a constant.
@@ -362,7 +362,7 @@ struct EmbeddingFunction : torch::autograd::Function<EmbeddingFunction> {
     a->save_for_backward({ids});
     a->set_materialize_grads(false);
     a->saved_data["handle"] = handle;
-    a->saved_data["foreign"] = foreign;
+    if (foreign) a->saved_data["foreign"] = true;
     a->saved_data["scale"] = scale;
     a->saved_data["padded"] = padded;
     a->saved_data["padding"] = padding;
@@ -398,7 +398,7 @@ struct DispatchFunction : torch::autograd::Function<DispatchFunction> {
     a->save_for_backward({place});
     a->set_materialize_grads(false);
     a->saved_data["handle"] = handle;
-    a->saved_data["foreign"] = foreign;
+    if (foreign) a->saved_data["foreign"] = true;
     return spread(kept(handle), x, place, Tensor());
   }
   static tensor_list backward(AutogradContext* a, tensor_list grads) {
@@ -420,7 +420,7 @@ struct GatherFunction : torch::autograd::Function<GatherFunction> {
     a->save_for_backward({place});
     a->set_materialize_grads(false);
     a->saved_data["handle"] = handle;
-    a->saved_data["foreign"] = foreign;
+    if (foreign) a->saved_data["foreign"] = true;
     a->saved_data["rows"] = rows.size(0);
     return combine(kept(handle), rows, place, Tensor());
   }
@@ -443,7 +443,7 @@ struct CombineFunction : torch::autograd::Function<CombineFunction> {
     a->save_for_backward({rows, place, weights});
     a->set_materialize_grads(false);
     a->saved_data["handle"] = handle;
-    a->saved_data["foreign"] = foreign;
+    if (foreign) a->saved_data["foreign"] = true;
     return combine(kept(handle), rows, place, weights);
   }
   static tensor_list backward(AutogradContext* a, tensor_list grads) {
