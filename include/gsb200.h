@@ -575,10 +575,10 @@ GSB_API int gsb_sage_hop_sized(gsb_ctx* ctx, void* stream, const int64_t* indptr
  * no scratch of the context: the caller provides it (at least the bytes that the *_workspace function of the same sizes names,
  * 256-byte aligned), so they may be captured into a CUDA graph
  * and queued on several streams at once, each call with a workspace of its own.  Ids, experts and places out of range are
- * never followed and record GSB_ERR_INDEX_RANGE.  Several threads may make these calls through one context at once, also while its own
- * thread makes others (backward passes run on threads of their own); those that wait for a number wait in turn. The order of
- * more than 32 768 ids meets at bounded waits: one that runs out records GSB_ERR_LOOKBACK_TIMEOUT and leaves an order that can be
- * used as indexes, a number of rows of 0, and anything at all in the rows of a dense gradient. */
+ * never followed and record GSB_ERR_INDEX_RANGE.  Several threads may make these calls through one context at once, also while its
+ * own thread makes others (backward passes run on threads of their own); those that wait for a number wait in turn.  A sort of more
+ * than 16 384 ids may meet at bounded waits: one that runs out records GSB_ERR_LOOKBACK_TIMEOUT and leaves an order that can be used
+ * as indexes, a number of rows of 0, and anything at all in the rows of a dense gradient. */
 #define GSB_MAX_ROW_LEN 1048576
 enum gsb_dtype { GSB_F32 = 0, GSB_F16 = 1, GSB_BF16 = 2 };
 
