@@ -159,9 +159,10 @@ def _plain_grad_weights(x, grad, ends, experts):
 
 
 def _plain_int8(x, values, scales, ends):
-    """Rows in 8 bits with a scale each, products of whole numbers (exact in 64-bit floats), scaled back."""
+    """Rows in 8 bits with a scale each, max / 127; products of whole numbers (exact in 64-bit floats), scaled back."""
     x = x.float()
-    row_scale = x.abs().amax(1) / 127.0
+    top = x.abs().amax(1)
+    row_scale = top / torch.full_like(top, 127.0)         # a quotient: division by a number multiplies with its reciprocal
     q = torch.round(x / row_scale[:, None]).clamp(-127, 127)
     q = torch.where(row_scale[:, None] == 0, 0.0, q).double()
     out = torch.zeros((x.shape[0], values.shape[1]), device=x.device)
@@ -305,7 +306,7 @@ def exact(case, seed):
     rows_of = torch.split(x.double(), sizes)[:E]
     rest = sizes[-1]
     if case["op"] == "int8":
-        scale = x.float().abs().max(dim=1).values.div(127)
+        scale = x.float().abs().max(dim=1).values.double().div(127).float()
         parts = []
         for e in range(E):
             of_rows = scale[ends[e]:ends[e + 1], None].double()
