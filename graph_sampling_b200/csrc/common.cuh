@@ -94,6 +94,9 @@ enum KernelId {
   KID_EMBED_LOOKUP,
   KID_EMBED_GRAD,
   KID_EXPERT_ROWS,
+  KID_EXPERT_PRODUCT,
+  KID_QUANTIZE,
+  KID_DROPOUT,
   KID_OTHER,
   KID_NUM
 };

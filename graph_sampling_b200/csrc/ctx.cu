@@ -656,7 +656,7 @@ const char* gsb_profile_kernel_name(int kid) {
       "table_insert",   "first_compact", "relabel",       "random_walk",    "sddmm_dot",       "sddmm_generic",
       "segment",        "row_filter",   "list_sample",    "sort",           "format",          "partition_count",
       "partition_scatter", "bucket_resolve", "first_bits",  "rank_emit",      "key_sort",        "embed_lookup",
-      "embed_grad",     "expert_rows",  "other"};
+      "embed_grad",     "expert_rows",  "expert_product", "quantize",       "dropout",         "other"};
   return (kid >= 0 && kid < gsb::KID_NUM) ? names[kid] : "";
 }
 

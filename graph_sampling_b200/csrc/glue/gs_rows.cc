@@ -1,4 +1,4 @@
-// The functions of the extension module for rows that are learned: embedding lookup and gradient, rows by expert, plain
+// The functions of the extension module for rows that are learned: embedding lookup and gradient, rows by expert, their products, dropout, plain
 // (graph_sampling_b200.ops) and as autograd functions (graph_sampling_b200.gs.nn).
 //
 // A backward pass runs on a thread of the autograd engine that does not hold the GIL, so everything below the Python functions
@@ -289,6 +289,171 @@ std::pair<Tensor, Tensor> combine_grad(gsb_ctx* ctx, const Tensor& grad_, const 
   return {grad_rows, grad_weights};
 }
 
+// One matrix per expert, its rows or its columns runs of memory; a copy where neither are.
+struct Matrices {
+  Tensor t;
+  int64_t experts, k, n;
+};
+Matrices matrices_of(const Tensor& w, const Rows& rows) {
+  refuse_unless(dtype_of(w, "weights") == rows.dtype, "weights must have the rows' dtype");
+  refuse_unless(w.dim() == 3, "weights must have the shape [experts, k, n]");
+  refuse_unless(w.size(0) >= 1 && w.size(0) <= GSB_MAX_EXPERTS, "weights must hold between 1 and 65536 experts");
+  refuse_unless(w.size(1) == rows.width, "weights must have as many rows each as the rows have values");
+  refuse_unless(w.is_cuda(), "weights must be a CUDA tensor");
+  same_device(w, rows.t);
+  Tensor t = as_stored(w);
+  if (!(t.size(1) <= 1 || t.stride(1) == 1) && !(t.size(2) <= 1 || t.stride(2) == 1)) t = t.contiguous();
+  return {t, w.size(0), w.size(1), w.size(2)};
+}
+Tensor offsets_of(const Tensor& t, int64_t experts, const Tensor& beside) {
+  const Tensor offsets = ids_of(t, "offsets");
+  refuse_unless(t.dim() == 1 && t.numel() >= 2, "offsets must hold one entry per expert and one more");
+  refuse_unless(experts < 0 || t.numel() == experts + 1, "offsets must hold one entry per expert and one more");
+  refuse_unless(t.numel() - 1 <= GSB_MAX_EXPERTS, "offsets must be of at most 65536 experts");
+  same_device(offsets, beside);
+  return offsets;
+}
+
+Tensor product(gsb_ctx* ctx, const Tensor& rows_, const Tensor& weights_, const Tensor& offsets_) {
+  const Rows rows = rows_of(rows_, "rows");
+  const Matrices w = matrices_of(weights_, rows);
+  const Tensor offsets = offsets_of(offsets_, w.experts, rows.t);
+  const c10::Device dev = rows.t.device();
+  const c10::cuda::CUDAGuard guard(dev);
+  Tensor out = fresh({rows.n, w.n}, rows.t.scalar_type(), dev);
+  if (out.numel() == 0) return out;
+  if (w.k == 0) return out.zero_();
+  const void* matrices = w.t.const_data_ptr();
+  const int64_t of_expert = w.t.stride(0), of_k = w.t.stride(1), of_n = w.t.stride(2);
+  Tensor work = scratch(gsb_expert_product_workspace(rows.data(), rows.dtype, rows.n, w.k, rows.stride, matrices, of_expert, of_k, of_n, w.n, w.experts),
+                        "gsb_expert_product", dev);
+  done(ctx, gsb_expert_product(ctx, stream(), rows.data(), rows.dtype, rows.n, w.k, rows.stride, matrices, of_expert, of_k, of_n, w.n, ids_ptr(offsets),
+                               w.experts, data(out), data(work), work.numel()),
+       "gsb_expert_product");
+  return out;
+}
+
+Tensor product_grad(gsb_ctx* ctx, const Tensor& rows_, const Tensor& grad_, const Tensor& offsets_) {
+  const Rows rows = rows_of(rows_, "rows"), grad = rows_of(grad_, "grad");
+  refuse_unless(grad.dtype == rows.dtype && grad.n == rows.n, "grad must have as many rows as rows, of the same dtype");
+  same_device(grad.t, rows.t);
+  const Tensor offsets = offsets_of(offsets_, -1, rows.t);
+  const int64_t experts = offsets.numel() - 1;
+  const c10::Device dev = rows.t.device();
+  const c10::cuda::CUDAGuard guard(dev);
+  Tensor out = fresh({experts, rows.width, grad.width}, rows.t.scalar_type(), dev);
+  if (out.numel() == 0) return out;
+  Tensor work = scratch(gsb_expert_product_grad_workspace(rows.data(), rows.dtype, rows.n, rows.width, rows.stride, grad.data(), grad.width,
+                                                          grad.stride, experts),
+                        "gsb_expert_product_grad", dev);
+  done(ctx, gsb_expert_product_grad(ctx, stream(), rows.data(), rows.dtype, rows.n, rows.width, rows.stride, grad.data(), grad.width, grad.stride,
+                                    ids_ptr(offsets), experts, data(out), data(work), work.numel()),
+       "gsb_expert_product_grad");
+  return out;
+}
+
+// ---- 8 bits
+constexpr int64_t kLine = 16;  // bytes that a row in 8 bits begins on
+int64_t in_lines(int64_t width) { return (width + kLine - 1) / kLine * kLine; }
+std::pair<Tensor, Tensor> quantize(gsb_ctx* ctx, const Tensor& x_) {
+  dtype_of(x_, "x");
+  refuse_unless(x_.dim() >= 1, "x must have at least one dimension");
+  refuse_unless(x_.is_cuda(), "x must be a CUDA tensor");
+  const auto shape = x_.sizes().slice(0, x_.dim() - 1);
+  const int64_t width = x_.size(-1);
+  const c10::cuda::CUDAGuard guard(x_.device());
+  const Rows x = rows_of(x_.reshape({c10::multiply_integers(shape), width}), "x");
+  Tensor values = fresh(with_width(shape, in_lines(width)), at::kChar, x.t.device()).narrow(-1, 0, width);
+  Tensor scales = fresh(shape, at::kFloat, x.t.device());
+  if (x.n == 0) return {values, scales};
+  if (width == 0) return {values, scales.zero_()};
+  done(ctx, gsb_quantize_rows(ctx, stream(), x.data(), x.dtype, x.n, width, x.stride, static_cast<int8_t*>(data(values)), in_lines(width),
+                              static_cast<float*>(data(scales))),
+       "gsb_quantize_rows");
+  return {values, scales};
+}
+
+// Rows in 8 bits that begin on 16-byte boundaries; a copy where they do not.
+Tensor bytes_of(const Tensor& t, const char* name, int64_t dim) {
+  refuse_unless(t.scalar_type() == at::kChar, name, " must be int8");
+  refuse_unless(t.dim() == dim, name, dim == 2 ? " must have two dimensions" : " must have the shape [experts, n, k]");
+  refuse_unless(t.is_cuda(), name, " must be a CUDA tensor");
+  bool good = (t.size(-1) <= 1 || t.stride(-1) == 1) && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % kLine == 0;
+  for (int64_t d = 0; d + 1 < dim; ++d) good = good && (t.size(d) <= 1 || (t.stride(d) % kLine == 0 && t.stride(d) >= t.size(-1)));
+  if (good || t.numel() == 0) return t;
+  Tensor copy = fresh(with_width(t.sizes().slice(0, dim - 1), in_lines(t.size(-1))), at::kChar, t.device()).narrow(-1, 0, t.size(-1));
+  copy.copy_(t);
+  return copy;
+}
+// Distance between neighbours of a dimension; where there is one alone, what it would be.
+int64_t step_of(const Tensor& t, int64_t d, int64_t alone) { return t.size(d) > 1 ? t.stride(d) : alone; }
+Tensor scales_of(const Tensor& t, const char* name, const Tensor& of) {
+  refuse_unless(t.scalar_type() == at::kFloat, name, " must be float32");
+  refuse_unless(t.sizes() == of.sizes().slice(0, of.dim() - 1), name, " must hold one value per row");
+  refuse_unless(t.is_cuda(), name, " must be a CUDA tensor");
+  same_device(t, of);
+  return as_stored(t).contiguous();
+}
+
+Tensor product_int8(gsb_ctx* ctx, const Tensor& values_, const Tensor& scales_, const Tensor& weight_values_, const Tensor& weight_scales_,
+                    const Tensor& offsets_, at::ScalarType type) {
+  refuse_unless(type == at::kFloat || type == at::kHalf || type == at::kBFloat16, "the result's dtype is float32, float16 or bfloat16");
+  const Tensor values = bytes_of(values_, "values", 2), w = bytes_of(weight_values_, "weight_values", 3);
+  same_device(values, w);
+  const int64_t n = values.size(0), k = values.size(1), experts = w.size(0), width = w.size(1);
+  refuse_unless(w.size(2) == k, "weight_values must have as many values in a row as values");
+  refuse_unless(k <= GSB_MAX_INT8_ROW_LEN, "rows in 8 bits must hold at most 131071 values");
+  refuse_unless(experts >= 1 && experts <= GSB_MAX_EXPERTS, "weight_values must hold between 1 and 65536 experts");
+  const Tensor scales = scales_of(scales_, "scales", values), weight_scales = scales_of(weight_scales_, "weight_scales", w);
+  const Tensor offsets = offsets_of(offsets_, experts, values);
+  const c10::cuda::CUDAGuard guard(values.device());
+  Tensor out = fresh({n, width}, type, values.device());
+  if (out.numel() == 0) return out;
+  if (k == 0) return out.zero_();
+  const int64_t of_n = step_of(w, 1, in_lines(k)), of_expert = step_of(w, 0, of_n * width);
+  done(ctx, gsb_expert_product_int8(ctx, stream(), static_cast<const int8_t*>(values.const_data_ptr()), n, k, step_of(values, 0, in_lines(k)),
+                                    static_cast<const float*>(scales.const_data_ptr()), static_cast<const int8_t*>(w.const_data_ptr()), of_expert, of_n,
+                                    static_cast<const float*>(weight_scales.const_data_ptr()), width, ids_ptr(offsets), experts, data(out),
+                                    dtype_of(out, "out")),
+       "gsb_expert_product_int8");
+  return out;
+}
+
+// ---- dropout
+struct Seed {
+  uint64_t number = 0;
+  Tensor on_device;  // where defined, read in the place of the number
+};
+Tensor drop(gsb_ctx* ctx, const Tensor& x_, double p, const Seed& seed) {
+  const int dtype = dtype_of(x_, "x");
+  refuse_unless(x_.is_cuda(), "x must be a CUDA tensor");
+  refuse_unless(p >= 0.0 && p <= 1.0, "p must be between 0 and 1");
+  if (seed.on_device.defined()) {
+    refuse_unless(seed.on_device.scalar_type() == at::kLong && seed.on_device.numel() == 1, "a seed that is a tensor must hold one int64");
+    refuse_unless(seed.on_device.is_cuda(), "a seed that is a tensor must be a CUDA tensor");
+    refuse_unless(!seed.on_device.is_neg(), "a seed that is a tensor must not be a negated view");
+    same_device(seed.on_device, x_);
+  }
+  const c10::cuda::CUDAGuard guard(x_.device());
+  Tensor x = as_stored(x_);
+  int64_t rows = 1, width = x.numel(), stride = x.numel();
+  if (!x.is_contiguous()) {  // rows at one distance are read in place
+    if (x.dim() == 2 && x.stride(1) == 1) {
+      rows = x.size(0);
+      width = x.size(1);
+      stride = x.stride(0);
+    } else {
+      x = x.contiguous();
+    }
+  }
+  Tensor out = fresh(x.sizes(), x.scalar_type(), x.device());
+  if (out.numel() == 0) return out;
+  done(ctx, gsb_dropout(ctx, stream(), x.const_data_ptr(), dtype, rows, width, stride, p, seed.number,
+                        seed.on_device.defined() ? static_cast<const uint64_t*>(seed.on_device.const_data_ptr()) : nullptr, data(out)),
+       "gsb_dropout");
+  return out;
+}
+
 // ---- autograd --------------------------------------------------------------------------------------------------------------
 gsb_ctx* kept(int64_t handle) { return reinterpret_cast<gsb_ctx*>(handle); }
 int64_t keep(gsb_ctx* ctx) { return reinterpret_cast<int64_t>(ctx); }
@@ -461,6 +626,57 @@ struct CombineFunction : torch::autograd::Function<CombineFunction> {
   }
 };
 
+struct ProductFunction : torch::autograd::Function<ProductFunction> {
+  static Tensor forward(AutogradContext* a, const Tensor& rows, const Tensor& weights, const Tensor& offsets, int64_t handle, bool foreign) {
+    a->save_for_backward({rows, weights, offsets});
+    a->set_materialize_grads(false);
+    a->saved_data["handle"] = handle;
+    if (foreign) a->saved_data["foreign"] = true;
+    return product(kept(handle), rows, weights, offsets);
+  }
+  static tensor_list backward(AutogradContext* a, tensor_list grads) {
+    tensor_list out(5);
+    if (!grads[0].defined()) return out;
+    refuse_tangents("grad", grads[0]);
+    refuse_foreign_leaf(a);
+    const auto saved = a->get_saved_variables();
+    {
+      const at::NoGradGuard no_grad;
+      gsb_ctx* ctx = kept(a->saved_data["handle"].toInt());
+      if (a->needs_input_grad(0)) out[0] = product(ctx, grads[0], saved[1].transpose(1, 2), saved[2]);
+      if (a->needs_input_grad(1)) out[1] = product_grad(ctx, saved[0], grads[0], saved[2]);
+    }
+    return only_once(std::move(out), {grads[0], saved[0], saved[1]});
+  }
+};
+
+// Two kinds of seed: a number, which is remembered, and a tensor, which is saved (autograd notices when it is changed in place).
+struct DropoutFunction : torch::autograd::Function<DropoutFunction> {
+  static Tensor forward(AutogradContext* a, const Tensor& x, double p, int64_t number, const std::optional<Tensor>& on_device, int64_t handle,
+                        bool foreign) {
+    a->set_materialize_grads(false);
+    a->saved_data["handle"] = handle;
+    if (foreign) a->saved_data["foreign"] = true;
+    a->saved_data["p"] = p;
+    a->saved_data["number"] = number;
+    if (on_device) a->save_for_backward({*on_device});
+    return drop(kept(handle), x, p, {(uint64_t)number, on_device.value_or(Tensor())});
+  }
+  static tensor_list backward(AutogradContext* a, tensor_list grads) {
+    tensor_list out(6);
+    if (!grads[0].defined()) return out;
+    refuse_tangents("grad", grads[0]);
+    refuse_foreign_leaf(a);
+    const auto saved = a->get_saved_variables();
+    {
+      const at::NoGradGuard no_grad;
+      out[0] = drop(kept(a->saved_data["handle"].toInt()), grads[0], a->saved_data["p"].toDouble(),
+                    {(uint64_t)a->saved_data["number"].toInt(), saved.empty() ? Tensor() : saved[0]});
+    }
+    return only_once(std::move(out), {grads[0]});
+  }
+};
+
 bool follows(const Tensor& t) { return t.defined() && t.requires_grad() && at::GradMode::is_enabled(); }
 
 // ---- the Python functions ----------------------------------------------------------------------------------------------------
@@ -623,9 +839,89 @@ FUNCTION(nn_combine, 4) {  // (ctx, rows, place, weights | None) -> out
   }));
 }
 
+FUNCTION(expert_product, 4) {  // (ctx, rows, weights, offsets) -> out
+  gsb_ctx* ctx = context(a[0]);
+  const Tensor &rows = tensor(a[1], "rows"), &weights = tensor(a[2], "weights"), &offsets = tensor(a[3], "offsets");
+  return wrap(without_gil([&] {
+    const at::NoGradGuard no_grad;
+    return product(ctx, rows, weights, offsets);
+  }));
+}
+
+FUNCTION(expert_product_grad, 4) {  // (ctx, rows, grad, offsets) -> gradient of the weights
+  gsb_ctx* ctx = context(a[0]);
+  const Tensor &rows = tensor(a[1], "rows"), &grad = tensor(a[2], "grad"), &offsets = tensor(a[3], "offsets");
+  return wrap(without_gil([&] {
+    const at::NoGradGuard no_grad;
+    return product_grad(ctx, rows, grad, offsets);
+  }));
+}
+
+FUNCTION(quantize_rows, 2) {  // (ctx, x) -> (values, scales)
+  gsb_ctx* ctx = context(a[0]);
+  const Tensor& x = tensor(a[1], "x");
+  auto r = without_gil([&] {
+    const at::NoGradGuard no_grad;
+    return quantize(ctx, x);
+  });
+  return tuple_of(wrap(std::move(r.first)), wrap(std::move(r.second)));
+}
+
+FUNCTION(expert_product_int8, 7) {  // (ctx, values, scales, weight values, weight scales, offsets, dtype) -> out
+  gsb_ctx* ctx = context(a[0]);
+  const Tensor &values = tensor(a[1], "values"), &scales = tensor(a[2], "scales"), &weight_values = tensor(a[3], "weight_values");
+  const Tensor &weight_scales = tensor(a[4], "weight_scales"), &offsets = tensor(a[5], "offsets");
+  const auto dtype = dtype_or_none(a[6]);
+  if (!dtype) type_error("dtype must be a torch.dtype");
+  return wrap(without_gil([&] {
+    const at::NoGradGuard no_grad;
+    return product_int8(ctx, values, scales, weight_values, weight_scales, offsets, *dtype);
+  }));
+}
+
+FUNCTION(dropout, 5) {  // (ctx, x, p, seed, seed on the device | None) -> out
+  gsb_ctx* ctx = context(a[0]);
+  const Tensor& x = tensor(a[1], "x");
+  const double p = number(a[2]);
+  const Seed seed{unsigned_integer(a[3]), tensor_or_none(a[4], "seed")};
+  return wrap(without_gil([&] {
+    const at::NoGradGuard no_grad;
+    return drop(ctx, x, p, seed);
+  }));
+}
+
+FUNCTION(nn_product, 4) {  // (ctx, rows, weights, offsets) -> out
+  gsb_ctx* ctx = context(a[0]);
+  const Tensor &rows = tensor(a[1], "rows"), &weights = tensor(a[2], "weights"), &offsets = tensor(a[3], "offsets");
+  return wrap(without_gil([&] {
+    refuse_tangents("rows", rows);
+    refuse_tangents("weights", weights);
+    if (!follows(rows) && !follows(weights)) return product(ctx, rows, weights, offsets);
+    refuse_foreign_accumulator(rows);
+    refuse_foreign_accumulator(weights);
+    return ProductFunction::apply(rows, weights, offsets, keep(ctx), foreign_leaf_behind(rows) || foreign_leaf_behind(weights));
+  }));
+}
+
+FUNCTION(nn_dropout, 5) {  // (ctx, x, p, seed, seed on the device | None) -> out
+  gsb_ctx* ctx = context(a[0]);
+  const Tensor& x = tensor(a[1], "x");
+  const double p = number(a[2]);
+  const Seed seed{unsigned_integer(a[3]), tensor_or_none(a[4], "seed")};
+  return wrap(without_gil([&] {
+    refuse_tangents("x", x);
+    if (!follows(x)) return drop(ctx, x, p, seed);
+    refuse_foreign_accumulator(x);
+    return DropoutFunction::apply(x, p, (int64_t)seed.number, seed.on_device.defined() ? std::optional<Tensor>(seed.on_device) : std::nullopt, keep(ctx),
+                                  foreign_leaf_behind(x));
+  }));
+}
+
 }  // namespace
 
 PyMethodDef native::row_methods[] = {ENTRY(embedding_lookup), ENTRY(embedding_grad), ENTRY(embedding_grad_rows),
                                      ENTRY(expert_order),     ENTRY(expert_dispatch), ENTRY(expert_combine),
                                      ENTRY(expert_combine_grad), ENTRY(nn_embedding), ENTRY(nn_dispatch),
-                                     ENTRY(nn_combine),       {nullptr, nullptr, 0, nullptr}};
+                                     ENTRY(nn_combine),       ENTRY(expert_product), ENTRY(expert_product_grad),
+                                     ENTRY(quantize_rows),    ENTRY(expert_product_int8), ENTRY(dropout),
+                                     ENTRY(nn_product),       ENTRY(nn_dropout), {nullptr, nullptr, 0, nullptr}};

@@ -1,0 +1,92 @@
+// Which rows and which tile of the result a CTA takes, for products over rows sorted by expert: found on the device from the
+// experts' offsets, so that no call waits for them.
+#pragma once
+#include "scan.cuh"
+
+namespace gsb {
+
+// Experts of one launch: their table is held in shared memory.  Calls with more go in several launches.
+constexpr int kPlanExperts = 1024;
+
+struct Groups {
+  const i64* offsets;  // of the launch's first expert
+  int first, experts;  // this launch's share
+  int all;             // the call's experts
+  u32 num_rows;
+  i64* counters;
+};
+
+// begin[e] .. begin[e + 1]: rows of expert e; tile[e] .. tile[e + 1]: its row tiles.  Offsets that decrease or lie outside the rows are
+// brought into range, so that nothing out of range is read or written, and recorded.
+struct PlanTable {
+  u32 begin[kPlanExperts + 1];
+  u32 tile[kPlanExperts + 1];
+  u32 carry[33];
+};
+
+__device__ __forceinline__ u32 clamped_offset(const Groups& g, int e) {
+  const i64 at = __ldg(g.offsets + e);
+  return (u32)(at < 0 ? 0 : at > (i64)g.num_rows ? (i64)g.num_rows : at);
+}
+
+// All THREADS threads of the CTA; ends with a barrier.  An expert without rows gets `at_least` tiles.
+template <int THREADS>
+__device__ __forceinline__ void make_plan(PlanTable& plan, const Groups& g, u32 tile_rows, u32 at_least) {
+  static_assert(THREADS % 32 == 0 && THREADS <= 1024, "whole warps");
+  constexpr int kEach = (kPlanExperts + THREADS - 1) / THREADS;
+  const int t = threadIdx.x;
+  for (int e = t; e <= g.experts; e += THREADS) {
+    const i64 at = __ldg(g.offsets + e);
+    plan.begin[e] = clamped_offset(g, e);
+    const bool bad = at < 0 || at > (i64)g.num_rows || (e < g.experts && __ldg(g.offsets + e + 1) < at);
+    if (bad && blockIdx.x == 0) raise_error(g.counters, GSB_ERR_INDEX_RANGE, g.first + e);
+  }
+  __syncthreads();
+  u32 own[kEach], sum = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int e = t * kEach + i;
+    u32 tiles = 0;
+    if (e < g.experts) {
+      const u32 b = plan.begin[e], end = plan.begin[e + 1];
+      tiles = end > b ? (end - b + tile_rows - 1) / tile_rows : 0;
+      if (tiles < at_least) tiles = at_least;
+    }
+    own[i] = sum;
+    sum += tiles;
+  }
+  u32 scan = sum;
+  for (int o = 1; o < 32; o <<= 1) {
+    const u32 up = __shfl_up_sync(0xffffffffu, scan, o);
+    if ((t & 31) >= o) scan += up;
+  }
+  if ((t & 31) == 31) plan.carry[t >> 5] = scan;
+  __syncthreads();
+  u32 before = scan - sum;
+  for (int w = 0; w < (t >> 5); ++w) before += plan.carry[w];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int e = t * kEach + i;
+    if (e <= g.experts) plan.tile[e] = before + own[i];
+  }
+  if (t == THREADS - 1 && THREADS * kEach == g.experts) plan.tile[g.experts] = before + sum;
+  __syncthreads();
+}
+
+// The expert whose row tiles hold number `tile` (below plan.tile[experts]).
+__device__ __forceinline__ int expert_of_tile(const PlanTable& plan, int experts, u32 tile) {
+  int low = 0, high = experts;  // plan.tile[low] <= tile < plan.tile[high]
+  while (high - low > 1) {
+    const int mid = (low + high) >> 1;
+    if (plan.tile[mid] <= tile) low = mid;
+    else high = mid;
+  }
+  return low;
+}
+
+// Rows of an expert: none where the next one's offset is smaller.
+__device__ __forceinline__ u32 rows_end(const PlanTable& plan, int e) {
+  return plan.begin[e + 1] > plan.begin[e] ? plan.begin[e + 1] : plan.begin[e];
+}
+
+}  // namespace gsb

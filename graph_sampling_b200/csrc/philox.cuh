@@ -13,7 +13,8 @@ enum : uint32_t {
   STREAM_WEIGHTED = 2,
   STREAM_WALK = 3,
   STREAM_LIST = 4,
-  STREAM_LIST_WEIGHTED = 5
+  STREAM_LIST_WEIGHTED = 5,
+  STREAM_DROPOUT = 6
 };
 
 struct U32x4 {

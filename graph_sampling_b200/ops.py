@@ -481,6 +481,48 @@ def expert_combine_grad(grad, rows, place, weights=None, ctx=None):
     return ctx.native.expert_combine_grad(ctx.address, grad, rows, place, weights)
 
 
+def expert_product(rows, weights, offsets, ctx=None):
+    """out[r, :] = rows[r, :] @ weights[e] for the rows offsets[e] .. offsets[e + 1] of every expert e → [rows, n]; zeros for rows of
+    no expert.  weights: [experts, k, n], of the rows' dtype; a transposed view is read in place.  offsets: those of
+    expert_order, on the GPU: the call does not wait for them."""
+    ctx = _context_for(rows, ctx)
+    return ctx.native.expert_product(ctx.address, rows, weights, offsets)
+
+
+def expert_product_grad(rows, grad, offsets, ctx=None):
+    """Gradient of `expert_product` for the weights → [experts, k, n]: rows[of e].T @ grad[of e], zeros for an expert without rows.
+    (That for the rows is expert_product(grad, weights.transpose(1, 2), offsets).)  The same inputs give the same bits."""
+    ctx = _context_for(rows, ctx)
+    return ctx.native.expert_product_grad(ctx.address, rows, grad, offsets)
+
+
+def quantize_rows(x, ctx=None):
+    """Rows (the last dimension) in 8 bits → (values, scales): scales = max |x| / 127 in float32, values = x / scales rounded to the
+    nearest whole number, in storage whose rows begin on 16-byte boundaries.  A row of zeros has the scale 0, one that holds an
+    infinity or NaN a NaN for its scale and zeros for its values."""
+    ctx = _context_for(x, ctx)
+    return ctx.native.quantize_rows(ctx.address, x)
+
+
+def expert_product_int8(values, scales, weight_values, weight_scales, offsets, dtype=torch.bfloat16, ctx=None):
+    """`expert_product` of rows and weights that are held in 8 bits → [rows, n] in `dtype`: out[r, j] = scales[r] * weight_scales[e, j] *
+    sum over i of values[r, i] * weight_values[e, j, i], the sum exact.  values, scales: of quantize_rows(rows); weight_values
+    [experts, n, k] and weight_scales [experts, n]: of quantize_rows(weights.transpose(1, 2)), made once.  Operands whose rows do not
+    begin on 16-byte boundaries are copied."""
+    ctx = _context_for(values, ctx)
+    return ctx.native.expert_product_int8(ctx.address, values, scales, weight_values, weight_scales, offsets, dtype)
+
+
+def dropout(x, p, seed=None, ctx=None):
+    """x with every value dropped (0) with probability p, a multiple of 2^-16, and the others divided by 1 - p.  Which ones depends
+    on `seed` and a value's position alone, so that the gradient is dropout(grad, p, seed), and no mask is stored.  seed: a number, None
+    for the next one of set_seed's, or a tensor of one int64 on the GPU that is read when the kernel runs: a captured call
+    draws anew when the tensor has changed."""
+    ctx = _context_for(x, ctx)
+    tensor = isinstance(seed, torch.Tensor)
+    return ctx.native.dropout(ctx.address, x, p, 0 if tensor else next_seed(seed), seed if tensor else None)
+
+
 def index_search(origin_data, keys, ctx=None):
     """gs::IndexSearch (src/tensor_ops.cc:23-31): position of every key in origin_data, -1 if absent."""
     origin_data, keys = _i64(origin_data, "origin_data"), _i64(keys, "keys")

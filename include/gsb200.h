@@ -633,6 +633,48 @@ GSB_API int gsb_expert_combine_grad(gsb_ctx* ctx, void* stream, const void* grad
                                     int64_t num_rows, int64_t rows_stride, const int64_t* place, const void* weights,
                                     int weights_dtype, void* out_grad_rows, void* out_grad_weights);
 
+/* ---- products over rows sorted by expert, in float types and in 8 bits; dropout ------------------------------------------
+ * As the calls on learned rows above.  offsets[num_experts + 1] (DEVICE, as gsb_expert_order gives it): rows offsets[e] ..
+ * offsets[e + 1] are those of expert e; offsets that decrease or lie outside the rows are brought into range, with
+ * GSB_ERR_INDEX_RANGE recorded.  num_rows below 2^31; k and n between 1 and GSB_MAX_ROW_LEN.
+ * Product: out[r, :] = rows[r, :] W[e(r)], zeros for rows of no expert; W[e][i][j] = weights[e * weights_expert_stride +
+ * i * weights_k_stride + j * weights_n_stride] for i < k, j < n, so the transposed matrices are the same memory with two strides
+ * exchanged.  Sums are held in float.  Its gradient for the weights (product_grad): out[e, i, j] = sum over the rows r of e of
+ * rows[r, i] * grad[r, j], zeros for an expert without rows; out is contiguous, of the rows' type.  The same inputs give the
+ * same bits.  The *_workspace functions take the operands of the call itself. */
+GSB_API int64_t gsb_expert_product_workspace(const void* rows, int dtype, int64_t num_rows, int64_t k, int64_t rows_stride,
+                                             const void* weights, int64_t weights_expert_stride, int64_t weights_k_stride,
+                                             int64_t weights_n_stride, int64_t n, int64_t num_experts);
+GSB_API int gsb_expert_product(gsb_ctx* ctx, void* stream, const void* rows, int dtype, int64_t num_rows, int64_t k,
+                               int64_t rows_stride, const void* weights, int64_t weights_expert_stride,
+                               int64_t weights_k_stride, int64_t weights_n_stride, int64_t n, const int64_t* offsets,
+                               int64_t num_experts, void* out, void* workspace, int64_t workspace_bytes);
+GSB_API int64_t gsb_expert_product_grad_workspace(const void* rows, int dtype, int64_t num_rows, int64_t k, int64_t rows_stride,
+                                                  const void* grad, int64_t n, int64_t grad_stride, int64_t num_experts);
+GSB_API int gsb_expert_product_grad(gsb_ctx* ctx, void* stream, const void* rows, int dtype, int64_t num_rows, int64_t k,
+                                    int64_t rows_stride, const void* grad, int64_t n, int64_t grad_stride,
+                                    const int64_t* offsets, int64_t num_experts, void* out, void* workspace,
+                                    int64_t workspace_bytes);
+/* Rows in 8 bits: out_scales[r] = max |x[r, :]| / 127, out_values[r, :] = x[r, :] / out_scales[r] rounded to the nearest whole
+ * number, ties to even (both divisions in IEEE float).  A row of zeros has the scale 0; one that holds an infinity or NaN has a
+ * NaN for its scale and zeros for its values.  values_stride >= row_len: the product wants a multiple of 16. */
+GSB_API int gsb_quantize_rows(gsb_ctx* ctx, void* stream, const void* x, int dtype, int64_t num_rows, int64_t row_len,
+                              int64_t x_stride, int8_t* out_values, int64_t values_stride, float* out_scales);
+/* out[r, j] = scales[r] * weight_scales[e(r) * n + j] * sum over i of values[r, i] * weight_values[e(r)][j][i], zeros for rows of
+ * no expert; the sums are exact (32-bit integers; k at most GSB_MAX_INT8_ROW_LEN), the result is rounded to float after each
+ * product and then to out_dtype.  Both operands' rows begin on 16-byte boundaries (their strides are multiples of 16). */
+#define GSB_MAX_INT8_ROW_LEN 131071
+GSB_API int gsb_expert_product_int8(gsb_ctx* ctx, void* stream, const int8_t* values, int64_t num_rows, int64_t k,
+                                    int64_t values_stride, const float* scales, const int8_t* weight_values,
+                                    int64_t weight_expert_stride, int64_t weight_n_stride, const float* weight_scales,
+                                    int64_t n, const int64_t* offsets, int64_t num_experts, void* out, int out_dtype);
+/* Dropout without a stored mask: value i of x, counted row by row, is dropped (0) where the 16 bits number i % 8 of block i / 8 of
+ * the generator under `seed` (Philox4x32-10, counter (i / 8, 0, 6)) are below p * 65 536, rounded; the others are multiplied so that
+ * the mean stays.  The gradient is the same call on the gradient.  seed_device (DEVICE, one value): read in the place of `seed`
+ * when the kernel runs, NULL: not.  0 <= p <= 1; out is contiguous. */
+GSB_API int gsb_dropout(gsb_ctx* ctx, void* stream, const void* x, int dtype, int64_t num_rows, int64_t row_len,
+                        int64_t x_stride, double p, uint64_t seed, const uint64_t* seed_device, void* out);
+
 /* ---- unique + relabel without any allocation ----------------------------------------------------------
  * No counterpart in the reference.  For callers that must not allocate device memory while they
  * run (a host process whose memory budget is fixed up front, a plug-in running under a lock that
