@@ -3,112 +3,449 @@
 // Rows offsets[e] .. offsets[e + 1] are those of expert e.  Product: out[r, :] = rows[r, :] W[e(r)], zeros for rows of no expert.
 // Its gradient for the rows is the product of the output's gradient with the transposed matrices, the same kernel; that for the
 // matrices is grad_W[e] = sum over the rows r of e of rows[r, :]^T grad[r, :].
+//
+// All run on the tensor cores.  float32 operands are taken apart into three bfloat16 parts, a = a0 + a1 + a2 with |a1| <= 2^-8 |a| and
+// |a2| <= 2^-16 |a|, exactly (24 bits are 3 times 8), and a b is the sum of the six products a_i b_j with i + j <= 2: what is left out is
+// 2^-23 |a b| at the very most.
 #include <type_traits>
 
 #include "group_plan.cuh"
 #include "launch.cuh"
 #include "row_values.cuh"
-#include "scan.cuh"
+#include "tensor_tile.cuh"
 
 namespace gsb {
 
-constexpr int kTile = 64, kDepth = 16, kThreads = 256;
+// A pair of CTAs takes a tile of 256 rows of the result, 128 each, by `columns` (128 or 256); each holds half of the columns' operand.
+constexpr int kPairRows = 256, kTileThreads = 256, kMaxStages = 8;
+constexpr int kSumColumns = 512;                 // of tensor memory: two tiles' sums, so that one is written out while the next is made
+constexpr int kRowsOperand = 128 * kLineBytes;   // bytes of a CTA's rows in a stage
+constexpr int kAcross = 64 * kLineBytes;         // a block of 64 lines
 
-template <class T>
-__device__ __forceinline__ float as_float(T v) {
-  return (float)v;
-}
-
-// acc[4][4] += sum over l < depth of A(i, l) * B(l, j) for the tile's rows i < height and columns j < width.
-template <class T, class Acc>
-__device__ __forceinline__ void tile_product(Acc (&acc)[4][4], const T* a, i64 a_i, i64 a_l, u32 height, const T* b, i64 b_l, i64 b_j, u32 width,
-                                             i64 depth, Acc (&sa)[kDepth][kTile + 1], Acc (&sb)[kDepth][kTile + 1]) {
-  const int t = threadIdx.x, ti = t / 16, tj = t % 16;
-  for (i64 l0 = 0; l0 < depth; l0 += kDepth) {
-    __syncthreads();
-#pragma unroll
-    for (int s = 0; s < kTile * kDepth / kThreads; ++s) {
-      const int at = s * kThreads + t;
-      const int i = at / kDepth, l = at % kDepth;
-      sa[l][i] = (u32)i < height && l0 + l < depth ? (Acc)as_float(a[i * a_i + (l0 + l) * a_l]) : (Acc)0;
-      sb[l][i] = (u32)i < width && l0 + l < depth ? (Acc)as_float(b[i * b_j + (l0 + l) * b_l]) : (Acc)0;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int l = 0; l < kDepth; ++l)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] += sa[l][ti * 4 + i] * sb[l][tj * 4 + j];
-  }
-}
-
-struct ProductArgs {
+struct TileArgs {
   Groups groups;
-  const void *rows, *weights;
-  i64 rows_stride, w_expert, w_k, w_n;
-  u32 k, n;
+  u32 depth, n;              // reduced index of a product; columns of the result
+  u32 k;                     // rows of a gradient's result
+  u32 columns;               // of a tile
+  u32 chunk;                 // rows of an expert that one tile of a gradient sums, a multiple of 64
+  int stages;
+  int expert_step;           // 0: one matrix for all experts
+  const CUtensorMap* maps;   // gradient: each expert's rows and gradient rows
+  float* partial;            // gradient: sums of the chunks (null: one chunk per expert, written out)
   const float *row_scales, *weight_scales;  // of 8-bit operands
+  u32 how;
 };
 
-template <class T, class Out>
-__global__ void __launch_bounds__(kThreads) k_product(const ProductArgs a, Out* __restrict__ out) {
-  using Acc = std::conditional_t<std::is_same<T, signed char>::value, int, float>;
-  __shared__ PlanTable plan;
-  __shared__ Acc sa[kDepth][kTile + 1], sb[kDepth][kTile + 1];
-  await_previous();
-  const Groups& g = a.groups;
-  make_plan<kThreads>(plan, g, kTile, 0);
-  const u32 columns = (a.n + kTile - 1) / kTile;
-  const u64 tiles = (u64)plan.tile[g.experts] * columns;
-  const int ti = threadIdx.x / 16 * 4, tj = threadIdx.x % 16 * 4;
-  for (u64 t = blockIdx.x; t < tiles; t += gridDim.x) {
-    const u32 row_tile = (u32)(t / columns), n0 = (u32)(t % columns) * kTile;
-    const int e = expert_of_tile(plan, g.experts, row_tile);
-    const u32 r0 = plan.begin[e] + (row_tile - plan.tile[e]) * kTile, height = min((u32)kTile, rows_end(plan, e) - r0);
-    Acc acc[4][4] = {};
-    tile_product<T, Acc>(acc, (const T*)a.rows + (i64)r0 * a.rows_stride, a.rows_stride, 1, height,
-                         (const T*)a.weights + (i64)(g.first + e) * a.w_expert + (i64)n0 * a.w_n, a.w_k, a.w_n, min((u32)kTile, a.n - n0), a.k, sa, sb);
-    for (int i = 0; i < 4; ++i)
-      for (int j = 0; j < 4; ++j) {
-        if ((u32)(ti + i) >= height || n0 + tj + j >= a.n) continue;
-        const u32 r = r0 + ti + i, c = n0 + tj + j;
-        float v = (float)acc[i][j];
-        if (a.row_scales) v = v * a.row_scales[r] * a.weight_scales[(i64)(g.first + e) * a.n + c];
-        out[(i64)r * a.n + c] = from_float<Out>(v);
-      }
-  }
-  // rows of no expert
-  const i64 step = (i64)gridDim.x * kThreads, at = (i64)blockIdx.x * kThreads + threadIdx.x;
-  if (g.first == 0)
-    for (i64 i = at; i < (i64)plan.begin[0] * a.n; i += step) out[i] = from_float<Out>(0.f);
-  if (g.first + g.experts == g.all)
-    for (i64 i = (i64)plan.begin[g.experts] * a.n + at; i < (i64)g.num_rows * a.n; i += step) out[i] = from_float<Out>(0.f);
+struct Tile {
+  int e;
+  u32 row0, rows;  // product: of the tile; gradient: of the chunk, counted from the expert's first
+  u32 m0, n0;      // gradient: first row of the result; first column
+  u32 blocks;      // steps of the reduced index, a line each
+  u32 chunk;
+};
+
+template <bool GRAD, int PER_LINE>
+__device__ __forceinline__ u64 number_of_tiles(const TileArgs& a, const PlanTable& plan) {
+  const u32 across = (a.n + a.columns - 1) / a.columns, down = GRAD ? (a.k + kPairRows - 1) / kPairRows : 1;
+  return (u64)plan.tile[a.groups.experts] * across * down;
+}
+template <bool GRAD, int PER_LINE>
+__device__ __forceinline__ Tile tile_at(const TileArgs& a, const PlanTable& plan, u64 t) {
+  Tile r;
+  const u32 across = (a.n + a.columns - 1) / a.columns, down = GRAD ? (a.k + kPairRows - 1) / kPairRows : 1;
+  r.chunk = (u32)(t / (across * down));
+  const u32 rest = (u32)(t % (across * down));
+  r.n0 = rest % across * a.columns;
+  r.m0 = rest / across * kPairRows;
+  r.e = expert_of_tile(plan, a.groups.experts, r.chunk);
+  const u32 step = GRAD ? a.chunk : kPairRows, count = plan.begin[r.e + 1] - plan.begin[r.e], from = (r.chunk - plan.tile[r.e]) * step;
+  r.rows = min(step, count - from);
+  r.row0 = GRAD ? from : plan.begin[r.e] + from;
+  r.blocks = ((GRAD ? r.rows : a.depth) + PER_LINE - 1) / PER_LINE;
+  return r;
 }
 
 template <class T>
-__global__ void __launch_bounds__(kThreads) k_grad_weights(const Groups g, const T* __restrict__ rows, i64 rows_stride, u32 k,
-                                                           const T* __restrict__ grad, i64 grad_stride, u32 n, T* __restrict__ out) {
-  __shared__ float sa[kDepth][kTile + 1], sb[kDepth][kTile + 1];
-  await_previous();
-  const u32 columns = (n + kTile - 1) / kTile, heights = (k + kTile - 1) / kTile;
-  const u64 tiles = (u64)g.experts * columns * heights;
-  const int ti = threadIdx.x / 16 * 4, tj = threadIdx.x % 16 * 4;
-  for (u64 t = blockIdx.x; t < tiles; t += gridDim.x) {
-    const int e = (int)(t / ((u64)columns * heights));
-    const u32 rest = (u32)(t % ((u64)columns * heights)), k0 = rest / columns * kTile, n0 = rest % columns * kTile;
-    const i64 from = __ldg(g.offsets + e), to = __ldg(g.offsets + e + 1);
-    if ((from < 0 || to < from || to > (i64)g.num_rows) && threadIdx.x == 0 && rest == 0) raise_error(g.counters, GSB_ERR_INDEX_RANGE, g.first + e);
-    const u32 begin = clamped_offset(g, e), end = max(begin, clamped_offset(g, e + 1));
-    const u32 height = min((u32)kTile, k - k0), width = min((u32)kTile, n - n0);
-    float acc[4][4] = {};
-    tile_product<T, float>(acc, rows + (i64)begin * rows_stride + k0, 1, rows_stride, height, grad + (i64)begin * grad_stride + n0, grad_stride, 1,
-                           width, end - begin, sa, sb);
-    for (int i = 0; i < 4; ++i)
-      for (int j = 0; j < 4; ++j)
-        if ((u32)(ti + i) < height && (u32)(tj + j) < width)
-          out[(i64)(g.first + e) * k * n + (i64)(k0 + ti + i) * n + n0 + tj + j] = from_float<T>(acc[i][j]);
+__device__ __forceinline__ void store_columns(T* to, const float (&v)[32], u32 valid, bool whole) {
+  if (whole && valid >= 32) {
+    constexpr int N = 16 / sizeof(T);
+#pragma unroll
+    for (int u = 0; u < 32 / N; ++u) {
+      float f[N];
+#pragma unroll
+      for (int q = 0; q < N; ++q) f[q] = v[u * N + q];
+      Unit<T, 16> w;
+      w.set(f);
+      store_unit((Unit<T, 16>*)to + u, w);
+    }
+  } else {
+#pragma unroll
+    for (int q = 0; q < 32; ++q)
+      if ((u32)q < valid) to[q] = from_float<T>(v[q]);
   }
+}
+
+// Warp 0 of each CTA loads, warp 1 of the first one issues the matrix instructions, warps 4 to 7 write results out.
+// PARTS: 3 for float32, else 1.  ACROSS: the second operand's lines hold the reduced index across them (a gradient's both do).
+template <class T, bool WHOLE_NUMBERS, int PARTS, bool GRAD, bool ACROSS>
+__global__ void __launch_bounds__(kTileThreads, 1) k_tiles(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                                                           const TileArgs a, T* __restrict__ out) {
+  constexpr int kPerLine = kLineBytes / (WHOLE_NUMBERS ? 1 : 2);
+  // float32: sums leave tensor memory, where additions cut, after this many lines of the reduced index, and are added up in registers
+  constexpr u32 kDrain = PARTS > 1 ? 4 : 0xffffffffu;
+  extern __shared__ char raw[];
+  __shared__ PlanTable plan;
+  __shared__ __align__(8) u64 bars[2 * kMaxStages + 4];
+  __shared__ u32 sums_at;
+  __shared__ volatile int stop;
+  const u32 stages_at = (smem_address(raw) + 1023u) & ~1023u;
+  const u32 full = smem_address(bars), empty = full + 8 * kMaxStages, sums_full = full + 16 * kMaxStages, sums_empty = sums_full + 16;
+  const u32 rank = rank_in_pair();
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  const Groups& g = a.groups;
+  i64* const counters = g.counters;
+
+  if (threadIdx.x == 0) {
+    stop = 0;
+    for (int s = 0; s < kMaxStages; ++s) {
+      barrier_init(full + 8 * s, 1);
+      barrier_init(empty + 8 * s, 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      barrier_init(sums_full + 8 * s, 1);
+      barrier_init(sums_empty + 8 * s, 8);  // the warps that write out, of both CTAs
+    }
+    barriers_ready();
+    if (!GRAD) {
+      prefetch_map(&map_a);
+      prefetch_map(&map_b);
+    }
+  }
+  if (warp == 2) sums_alloc(smem_address(&sums_at), kSumColumns);
+  make_plan<kTileThreads>(plan, g, GRAD ? a.chunk : kPairRows, GRAD ? 1 : 0);
+  sums_fence_before();
+  cluster_barrier();
+  sums_fence_after();
+  const u32 sums = sums_at;
+  const u64 tiles = number_of_tiles<GRAD, kPerLine>(a, plan);
+  const u64 first = blockIdx.x / 2, step = gridDim.x / 2;
+  const u32 half = a.columns / 2, b_bytes = half * kLineBytes, stage_bytes = PARTS * (kRowsOperand + b_bytes);
+
+  if (warp == 0 && lane == 0) {
+    const u32 full_of_first = address_in(full, 0);
+    u32 stage = 0, turn = 0;
+    for (u64 t = first; t < tiles; t += step) {
+      const Tile tile = tile_at<GRAD, kPerLine>(a, plan, t);
+      const CUtensorMap *of_a = &map_a, *of_b = &map_b;
+      if (GRAD) {
+        of_a = a.maps + 2 * tile.e;
+        of_b = of_a + 1;
+        if (tile.blocks > 0) {
+          asm volatile("fence.proxy.tensormap::generic.acquire.gpu [%0], 128;" ::"l"(of_a) : "memory");
+          asm volatile("fence.proxy.tensormap::generic.acquire.gpu [%0], 128;" ::"l"(of_b) : "memory");
+        }
+      }
+      const int matrix = (g.first + tile.e) * a.expert_step;
+      for (u32 b = 0; b < tile.blocks; ++b) {
+        if (!barrier_wait(empty + 8 * stage, turn ^ 1, &stop, counters)) goto loaded;
+        if (rank == 0) barrier_expect(full + 8 * stage, 2 * stage_bytes);
+        const u32 at = stages_at + stage * stage_bytes, bar = full_of_first + 8 * stage;
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+          const u32 to_a = at + p * kRowsOperand, to_b = at + PARTS * kRowsOperand + p * b_bytes;
+          if (GRAD) {
+            for (int j = 0; j < 2; ++j) load_tile(to_a + j * kAcross, of_a, bar, (int)(tile.m0 + rank * 128 + j * 64), (int)(tile.row0 + b * 64), p);
+            for (u32 j = 0; j < half / 64; ++j)
+              load_tile(to_b + j * kAcross, of_b, bar, (int)(tile.n0 + rank * half + j * 64), (int)(tile.row0 + b * 64), p);
+          } else {
+            load_tile(to_a, of_a, bar, (int)(b * kPerLine), (int)(tile.row0 + rank * 128), p);
+            if (ACROSS)
+              for (u32 j = 0; j < half / 64; ++j)
+                load_tile(to_b + j * kAcross, of_b, bar, (int)(tile.n0 + rank * half + j * 64), (int)(b * kPerLine), matrix, p);
+            else
+              load_tile(to_b, of_b, bar, (int)(b * kPerLine), (int)(tile.n0 + rank * half), matrix, p);
+          }
+        }
+        if (++stage == (u32)a.stages) stage = 0, turn ^= 1;
+      }
+    }
+  loaded:;
+  } else if (warp == 1 && rank == 0 && lane == 0) {
+    constexpr bool A_ACROSS = GRAD, B_ACROSS = GRAD || ACROSS;
+    u32 stage = 0, turn = 0, made = 0;
+    for (u64 t = first; t < tiles; t += step) {
+      const Tile tile = tile_at<GRAD, kPerLine>(a, plan, t);
+      for (u32 b0 = 0; b0 < tile.blocks; b0 += min(kDrain, tile.blocks - b0), ++made) {
+        const u32 buffer = made & 1, to = sums + buffer * 256;
+        if (!barrier_wait(sums_empty + 8 * buffer, (made >> 1 & 1) ^ 1, &stop, counters)) goto issued;
+        sums_fence_after();
+        for (u32 b = b0; b < b0 + min(kDrain, tile.blocks - b0); ++b) {
+          if (!barrier_wait(full + 8 * stage, turn, &stop, counters)) goto issued;
+          sums_fence_after();
+          const u32 at = stages_at + stage * stage_bytes;
+          const u64 op_a = operand(at, kAcross), op_b = operand(at + PARTS * kRowsOperand, kAcross);
+#pragma unroll
+          for (int s = 0; s < 4; ++s) {
+            const u64 a_s = op_a + s * ((A_ACROSS ? 16 * kLineBytes : 32) >> 4), b_s = op_b + s * ((B_ACROSS ? 16 * kLineBytes : 32) >> 4);
+            const bool add = b > b0 || s > 0;
+            multiply<WHOLE_NUMBERS>(to, a_s, b_s, a.how, add);
+            if (PARTS == 3) {  // the five small products have sums of their own, 2^-8 the size
+              const u64 next_a = kRowsOperand >> 4, next_b = b_bytes >> 4;
+              multiply<false>(to + 128, a_s, b_s + next_b, a.how, add);
+              multiply<false>(to + 128, a_s + next_a, b_s, a.how, true);
+              multiply<false>(to + 128, a_s + next_a, b_s + next_b, a.how, true);
+              multiply<false>(to + 128, a_s, b_s + 2 * next_b, a.how, true);
+              multiply<false>(to + 128, a_s + 2 * next_a, b_s, a.how, true);
+            }
+          }
+          multiplied(empty + 8 * stage);
+          if (++stage == (u32)a.stages) stage = 0, turn ^= 1;
+        }
+        multiplied(sums_full + 8 * buffer);
+      }
+    }
+  issued:;
+  } else if (warp >= 4) {
+    const u32 quarter = (u32)(warp & 3) * 32, row = rank * 128 + quarter + lane;  // of the tile
+    const u32 sums_empty_of_first = address_in(sums_empty, 0);
+    const bool whole = (u64)a.n * sizeof(T) % 16 == 0 && (u64)(uintptr_t)out % 16 == 0, whole_partial = a.n % 4 == 0;
+    u32 made = 0;
+    for (u64 t = first; t < tiles; t += step) {
+      const Tile tile = tile_at<GRAD, kPerLine>(a, plan, t);
+      const bool mine = GRAD ? tile.m0 + row < a.k : row < tile.rows;
+      const i64 at = GRAD ? ((i64)(a.partial ? (i64)tile.chunk : (i64)(g.first + tile.e)) * a.k + tile.m0 + row) * a.n + tile.n0
+                          : (i64)(tile.row0 + row) * a.n + tile.n0;
+      auto store = [&](u32 c, const float(&v)[32]) {
+        if (!mine || tile.n0 + c >= a.n) return;
+        if (GRAD && a.partial) store_columns(a.partial + at + c, v, a.n - tile.n0 - c, whole_partial);
+        else store_columns(out + at + c, v, a.n - tile.n0 - c, whole);
+      };
+      if (tile.blocks == 0) {
+        const float zeros[32] = {};
+        for (u32 c = 0; c < a.columns; c += 32) store(c, zeros);
+        continue;
+      }
+      if constexpr (PARTS == 1) {
+        const u32 buffer = made & 1;
+        const bool there = barrier_wait(sums_full + 8 * buffer, made >> 1 & 1, &stop, counters);
+        if (!__all_sync(0xffffffffu, there)) break;
+        sums_fence_after();
+        const float of_row = WHOLE_NUMBERS && mine ? a.row_scales[tile.row0 + row] : 1.f;
+        for (u32 c = 0; c < a.columns; c += 32) {
+          u32 v[32];
+          read_sums(sums + (quarter << 16) + buffer * 256 + c, v);
+          sums_read();
+          if (c + 32 == a.columns) {
+            sums_fence_before();
+            __syncwarp();
+            if (lane == 0) barrier_arrive_at(sums_empty_of_first + 8 * buffer);
+          }
+          float f[32];
+#pragma unroll
+          for (int q = 0; q < 32; ++q) {
+            if constexpr (WHOLE_NUMBERS) {
+              const u32 column = tile.n0 + c + q;
+              f[q] = (float)(int)v[q] * of_row * (column < a.n ? __ldg(a.weight_scales + (i64)(g.first + tile.e) * a.n + column) : 0.f);
+            } else {
+              f[q] = __uint_as_float(v[q]);
+            }
+          }
+          store(c, f);
+        }
+        ++made;
+      } else {
+        float total[4][32] = {};
+        bool lost = false;
+        for (u32 b0 = 0; b0 < tile.blocks; b0 += min(kDrain, tile.blocks - b0), ++made) {
+          const u32 buffer = made & 1;
+          const bool there = barrier_wait(sums_full + 8 * buffer, made >> 1 & 1, &stop, counters);
+          if (!__all_sync(0xffffffffu, there)) {
+            lost = true;
+            break;
+          }
+          sums_fence_after();
+          const u32 from = sums + (quarter << 16) + buffer * 256;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            u32 large[32], small[32];
+            read_sums(from + c * 32, large);
+            read_sums(from + 128 + c * 32, small);
+            sums_read();
+#pragma unroll
+            for (int q = 0; q < 32; ++q) {
+              // an infinity's small products are infinity times 0: the large one has the answer
+              const float of_large = __uint_as_float(large[q]);
+              total[c][q] += fabsf(of_large) <= 3.402823466e38f ? of_large + __uint_as_float(small[q]) : of_large;
+            }
+          }
+          sums_fence_before();
+          __syncwarp();
+          if (lane == 0) barrier_arrive_at(sums_empty_of_first + 8 * buffer);
+        }
+        if (lost) break;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) store(c * 32, total[c]);
+      }
+    }
+    if (!GRAD) {  // rows of no expert
+      const i64 at = (i64)blockIdx.x * 128 + (threadIdx.x - 128), by = (i64)gridDim.x * 128;
+      auto clear = [&](i64 from, i64 to) {
+        if (whole) {
+          constexpr int N = 16 / sizeof(T);
+          for (i64 i = from / N + at; i < to / N; i += by) ((uint4*)out)[i] = make_uint4(0, 0, 0, 0);
+        } else {
+          for (i64 i = from + at; i < to; i += by) out[i] = from_float<T>(0.f);
+        }
+      };
+      if (g.first == 0) clear(0, (i64)plan.begin[0] * a.n);
+      if (g.first + g.experts == g.all) clear((i64)plan.begin[g.experts] * a.n, (i64)g.num_rows * a.n);
+    }
+  }
+  __syncwarp();
+  if (stop) {  // given up: what is still on its way into this CTA's memory gets a moment to arrive
+    const u64 since = nanoseconds();
+    while (nanoseconds() - since < 1000000) __nanosleep(1000);
+  }
+  __syncthreads();
+  sums_fence_before();
+  cluster_barrier();
+  sums_fence_after();
+  if (warp == 2) sums_free(sums, kSumColumns);
+}
+
+// Descriptions of each expert's rows and gradient rows: the same arrays, from its first row on and as long as it has rows, so that loads
+// fill the rest of a tile with zeros.  A warp per expert and array.
+constexpr int kMapWarps = 8;
+__global__ void __launch_bounds__(32 * kMapWarps) k_expert_maps(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                                                                const Groups g, const char* a, i64 a_row_bytes, const char* b, i64 b_row_bytes,
+                                                                CUtensorMap* __restrict__ maps) {
+  __shared__ PlanTable plan;
+  __shared__ __align__(128) CUtensorMap held[kMapWarps];
+  await_previous();
+  make_plan<32 * kMapWarps>(plan, g, 1, 0);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, which = blockIdx.x * kMapWarps + warp, e = which / 2;
+  if (e >= g.experts || plan.begin[e + 1] == plan.begin[e]) return;
+  const bool second = which & 1;
+  ((u32*)&held[warp])[lane] = ((const u32*)(second ? &map_b : &map_a))[lane];
+  __syncwarp();
+  const u32 at = smem_address(&held[warp]);
+  if (lane == 0) {
+    const u64 address = (u64)(uintptr_t)(second ? b + plan.begin[e] * b_row_bytes : a + plan.begin[e] * a_row_bytes);
+    asm volatile("tensormap.replace.tile.global_address.shared::cta.b1024.b64 [%0], %1;" ::"r"(at), "l"(address) : "memory");
+    asm volatile("tensormap.replace.tile.global_dim.shared::cta.b1024.b32 [%0], 1, %1;" ::"r"(at), "r"(plan.begin[e + 1] - plan.begin[e]) : "memory");
+  }
+  __syncwarp();
+  asm volatile("tensormap.cp_fenceproxy.global.shared::cta.tensormap::generic.release.gpu.sync.aligned [%0], [%1], 128;" ::"l"(maps + which), "r"(at)
+               : "memory");
+}
+
+// out[e] = the sum of the chunks of expert e, in their order.
+template <class T>
+__global__ void __launch_bounds__(kTileThreads) k_add_chunks(const Groups g, u32 chunk, i64 values, const float* __restrict__ partial,
+                                                             T* __restrict__ out) {
+  __shared__ PlanTable plan;
+  await_previous();
+  make_plan<kTileThreads>(plan, g, chunk, 1);
+  const i64 step = (i64)gridDim.x * kTileThreads;
+  for (i64 i = (i64)blockIdx.x * kTileThreads + threadIdx.x; i < values * g.experts; i += step) {
+    const int e = (int)(i / values);
+    const i64 at = i - e * values;
+    float sum = 0.f;
+    for (u32 c = plan.tile[e]; c < plan.tile[e + 1]; ++c) sum += partial[c * values + at];
+    out[(i64)g.first * values + i] = from_float<T>(sum);
+  }
+}
+
+// ---- operands brought into lines -------------------------------------------------------------------------------------------------
+// Matrices whose rows do not begin on 16-byte boundaries are copied to where they do; float32 is cut into its parts, one array each.
+template <class T, int PARTS>
+__global__ void __launch_bounds__(256) k_into_lines(const T* __restrict__ from, i64 matrices, i64 matrix_stride, u32 height, i64 stride, u32 width,
+                                                    u32 to_stride, unsigned short* __restrict__ to) {
+  await_previous();
+  const u32 pieces = to_stride / 8;
+  const i64 count = matrices * height * pieces, plane = matrices * height * (i64)to_stride;
+  for (i64 i = (i64)blockIdx.x * 256 + threadIdx.x; i < count; i += (i64)gridDim.x * 256) {
+    const i64 line = i / pieces;
+    const u32 x = (u32)(i - line * pieces) * 8;
+    const T* row = from + line / height * matrix_stride + line % height * stride;
+    unsigned short v[PARTS][8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      if constexpr (PARTS == 1) {
+        v[0][q] = x + q < width ? ((const unsigned short*)row)[x + q] : (unsigned short)0;
+      } else {
+        float rest = x + q < width ? row[x + q] : 0.f;
+        const bool finite = fabsf(rest) <= 3.402823466e38f;
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+          // to nearest, but the largest numbers downwards, where that would be infinity.  Infinities and NaN are all in the first part
+          const __nv_bfloat16 part = finite && fabsf(rest) > 3.38e38f ? __float2bfloat16_rz(rest) : __float2bfloat16_rn(rest);
+          v[p][q] = __bfloat16_as_ushort(part);
+          rest = finite ? rest - __bfloat162float(part) : 0.f;
+        }
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) {
+      uint4 w;
+      w.x = v[p][0] | (u32)v[p][1] << 16;
+      w.y = v[p][2] | (u32)v[p][3] << 16;
+      w.z = v[p][4] | (u32)v[p][5] << 16;
+      w.w = v[p][6] | (u32)v[p][7] << 16;
+      *(uint4*)(to + p * plane + line * to_stride + x) = w;
+    }
+  }
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------------------
+static i64 rounded(i64 bytes) { return (bytes + 255) / 256 * 256; }
+
+// An operand as the kernel reads it: `matrices` of `height` lines of `width` values, neighbours in memory.
+struct Lines {
+  const void* at;
+  i64 matrices, matrix_stride, height, stride, width;
+  int dtype;
+  bool copied() const {
+    const int size = value_bytes(dtype);
+    return dtype == GSB_F32 || !aligned_to(16, (const char*)at) || (height > 1 && (stride * size % 16 != 0 || stride == 0)) ||
+           (matrices > 1 && matrix_stride * size % 16 != 0);
+  }
+  i64 parts() const { return dtype == GSB_F32 ? 3 : 1; }
+  i64 to_stride() const { return (width + 7) / 8 * 8; }
+  i64 copies() const { return matrices > 1 && matrix_stride == 0 ? 1 : matrices; }  // one matrix for all is copied once
+  i64 bytes() const { return copied() ? rounded(parts() * copies() * height * to_stride() * 2) : 0; }
+};
+
+// The operand, copied first where it has to be; `room` moves on behind the copy.
+static int bring(gsb_ctx* ctx, cudaStream_t stream, Lines* x, char** room) {
+  if (!x->copied()) return GSB_OK;
+  unsigned short* to = (unsigned short*)*room;
+  *room += x->bytes();
+  const i64 count = x->copies() * x->height * (x->to_stride() / 8);
+  const int grid = (int)min((i64)kNumSMs * 16, (i64)grid_for(count, 256));
+  ScopedKernelTimer timer(ctx, KID_EXPERT_PRODUCT, stream);
+  if (x->dtype == GSB_F32)
+    launch_behind(stream, k_into_lines<float, 3>, grid, 256, (const float*)x->at, x->copies(), x->matrix_stride, (u32)x->height, x->stride, (u32)x->width,
+                  (u32)x->to_stride(), to);
+  else
+    launch_behind(stream, k_into_lines<unsigned short, 1>, grid, 256, (const unsigned short*)x->at, x->copies(), x->matrix_stride, (u32)x->height, x->stride,
+                  (u32)x->width, (u32)x->to_stride(), to);
+  GSB_LAUNCH_OK();
+  x->at = to;
+  x->matrix_stride = x->matrix_stride == 0 ? 0 : x->height * x->to_stride();
+  x->stride = x->to_stride();
+  return GSB_OK;
+}
+
+// Four extents: along a line, lines, matrices, parts.  A distance between things of which there is one is never used, but checked.
+static int describe(const Lines& x, int size, u32 box_along, u32 box_lines, bool matrices, CUtensorMap* map) {
+  const i64 lines = x.height > 1 ? x.stride * size : 16, step = x.copies() > 1 ? x.matrix_stride * size : 16;
+  const i64 part = x.parts() > 1 ? x.copies() * x.height * x.stride * size : 16;
+  const u64 dims4[4] = {(u64)x.width, (u64)x.height, (u64)x.copies(), (u64)x.parts()}, strides4[3] = {(u64)lines, (u64)step, (u64)part};
+  const u64 dims3[3] = {(u64)x.width, (u64)x.height, (u64)x.parts()}, strides3[2] = {(u64)lines, (u64)part};
+  const u32 box[4] = {box_along, box_lines, 1, 1};
+  if (lines >= (i64)1 << 40 || step >= (i64)1 << 40 || part >= (i64)1 << 40) return GSB_ERR_UNSUPPORTED;
+  return describe_array(map, x.at, size, matrices ? 4 : 3, matrices ? dims4 : dims3, matrices ? strides4 : strides3, box) ? GSB_OK : GSB_ERR_UNSUPPORTED;
 }
 
 static int check_product(i64 num_rows, i64 k, i64 n, i64 num_experts, i64 rows_stride, const int64_t* offsets) {
@@ -130,6 +467,62 @@ static int by_experts(gsb_ctx* ctx, i64 num_experts, i64 num_rows, const int64_t
   return GSB_OK;
 }
 
+// Launches pairs of CTAs: at most one CTA per SM.  In the order of the stream, with no overlap of its neighbours' ends and beginnings: with
+// overlap, hundreds of copies and products queued one behind the other came to a halt, waiting CTAs of one kernel beside clusters of another
+// that need SMs as a whole.
+template <class T, bool WHOLE_NUMBERS, int PARTS, bool GRAD, bool ACROSS>
+static int launch_tiles(gsb_ctx* ctx, cudaStream_t stream, const CUtensorMap& map_a, const CUtensorMap& map_b, TileArgs a, i64 most_tiles, T* out) {
+  auto kernel = k_tiles<T, WHOLE_NUMBERS, PARTS, GRAD, ACROSS>;
+  const int stage = PARTS * (kRowsOperand + (int)a.columns / 2 * kLineBytes);
+  a.stages = min(kMaxStages, 200 * 1024 / stage);
+  a.how = instruction(WHOLE_NUMBERS ? OPERAND_S8 : std::is_same<T, __half>::value ? OPERAND_F16 : OPERAND_BF16, GRAD, GRAD || ACROSS, kPairRows, a.columns);
+  const int smem = a.stages * stage + 1024;
+  GSB_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * max((i64)1, min((i64)kNumSMs / 2, most_tiles))));
+  cfg.blockDim = dim3(kTileThreads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = 2;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  ScopedKernelTimer timer(ctx, KID_EXPERT_PRODUCT, stream);
+  GSB_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, map_a, map_b, a, out));
+  return GSB_OK;
+}
+
+// Columns of a tile: narrow ones for narrow results (and for float32, whose parts need the room).
+static u32 tile_columns(i64 n, int dtype) { return dtype == GSB_F32 || n <= 128 ? 128 : 256; }
+
+static Lines rows_operand(const void* rows, int dtype, i64 num_rows, i64 width, i64 stride) { return Lines{rows, 1, 0, num_rows, stride, width, dtype}; }
+// The matrices with their rows (ACROSS) or their columns as lines, whichever are neighbours in memory.
+static bool rows_are_lines(i64 k, i64 n, i64 k_stride, i64 n_stride) { return n_stride == 1 || n == 1 ? !(k_stride == 1 && n == 1 && k > 1) : false; }
+static Lines matrices_operand(const void* w, int dtype, i64 experts, i64 expert_stride, i64 k, i64 k_stride, i64 n, i64 n_stride) {
+  if (rows_are_lines(k, n, k_stride, n_stride)) return Lines{w, experts, experts > 1 ? expert_stride : 0, k, k_stride, n, dtype};
+  return Lines{w, experts, experts > 1 ? expert_stride : 0, n, n_stride, k, dtype};
+}
+
+// Rows of an expert that one tile of the weights' gradient sums.  All of them, unless that leaves pairs of CTAs without work.
+static i64 chunk_rows(i64 num_rows, i64 k, i64 n, u32 columns, i64 num_experts) {
+  const i64 tiles = (k + kPairRows - 1) / kPairRows * ((n + columns - 1) / columns);
+  const i64 wanted = (3 * kNumSMs / 2 + tiles - 1) / tiles;  // chunks in all
+  i64 chunk = (num_rows + wanted - 1) / wanted;
+  if (num_experts >= wanted) chunk = num_rows;
+  chunk = max(chunk, (i64)512);
+  return min((chunk + 63) / 64 * 64, ((num_rows + 63) / 64) * 64);
+}
+static i64 most_chunks(i64 num_rows, i64 chunk, i64 num_experts) { return min(num_experts, (i64)kPlanExperts) + num_rows / max((i64)1, chunk); }
+
+template <class F>
+static int with_type(int dtype, F f) {
+  if (dtype == GSB_F32) return f(float{}, std::integral_constant<int, 3>{});
+  if (dtype == GSB_F16) return f(__half{}, std::integral_constant<int, 1>{});
+  return f(__nv_bfloat16{}, std::integral_constant<int, 1>{});
+}
+
 }  // namespace gsb
 
 using namespace gsb;
@@ -137,55 +530,114 @@ using namespace gsb;
 extern "C" int64_t gsb_expert_product_workspace(const void* rows, int dtype, int64_t num_rows, int64_t k, int64_t rows_stride, const void* weights,
                                                 int64_t weights_expert_stride, int64_t weights_k_stride, int64_t weights_n_stride, int64_t n,
                                                 int64_t num_experts) {
-  return 0;
+  if (value_bytes(dtype) == 0 || num_rows < 0 || num_rows >= ((i64)1 << 31) || k < 1 || k > GSB_MAX_ROW_LEN || n < 1 || n > GSB_MAX_ROW_LEN ||
+      num_experts < 1 || num_experts > GSB_MAX_EXPERTS)
+    return GSB_ERR_INVALID_ARGUMENT;
+  return rows_operand(rows, dtype, num_rows, k, rows_stride).bytes() +
+         matrices_operand(weights, dtype, num_experts, weights_expert_stride, k, weights_k_stride, n, weights_n_stride).bytes();
 }
 
 extern "C" int gsb_expert_product(gsb_ctx* ctx, void* stream_, const void* rows, int dtype, int64_t num_rows, int64_t k, int64_t rows_stride,
                                   const void* weights, int64_t weights_expert_stride, int64_t weights_k_stride, int64_t weights_n_stride, int64_t n,
                                   const int64_t* offsets, int64_t num_experts, void* out, void* workspace, int64_t workspace_bytes) {
   GSB_ENTER(ctx);
-  const int st = check_product(num_rows, k, n, num_experts, rows_stride, offsets);
+  int st = check_product(num_rows, k, n, num_experts, rows_stride, offsets);
   if (st != GSB_OK) return st;
   const int size = value_bytes(dtype);
   GSB_REQUIRE(size != 0 && weights_expert_stride >= 0 && weights_k_stride >= 0 && weights_n_stride >= 0, GSB_ERR_INVALID_ARGUMENT);
+  GSB_REQUIRE(weights_k_stride == 1 || weights_n_stride == 1 || k == 1 || n == 1, GSB_ERR_INVALID_ARGUMENT);
   if (num_rows == 0) return GSB_OK;
   GSB_REQUIRE(rows && weights && out && aligned_to(size, (const char*)rows, (const char*)weights, (const char*)out), GSB_ERR_INVALID_ARGUMENT);
+  const int64_t need = gsb_expert_product_workspace(rows, dtype, num_rows, k, rows_stride, weights, weights_expert_stride, weights_k_stride,
+                                                    weights_n_stride, n, num_experts);
+  GSB_REQUIRE(need >= 0 && (need == 0 || workspace) && aligned_to(256, (const char*)workspace), GSB_ERR_INVALID_ARGUMENT);
+  GSB_REQUIRE(workspace_bytes >= need, GSB_ERR_CAPACITY);
   cudaStream_t stream = (cudaStream_t)stream_;
+  const bool across = rows_are_lines(k, n, weights_k_stride, weights_n_stride);
+  Lines x = rows_operand(rows, dtype, num_rows, k, rows_stride);
+  Lines w = matrices_operand(weights, dtype, num_experts, weights_expert_stride, k, weights_k_stride, n, weights_n_stride);
+  char* room = (char*)workspace;
+  if ((st = bring(ctx, stream, &x, &room)) != GSB_OK || (st = bring(ctx, stream, &w, &room)) != GSB_OK) return st;
+  TileArgs a = {};
+  a.depth = (u32)k;
+  a.n = (u32)n;
+  a.columns = tile_columns(n, dtype);
+  a.expert_step = w.copies() > 1;
+  CUtensorMap map_x, map_w;
+  if ((st = describe(x, 2, 64, 128, false, &map_x)) != GSB_OK || (st = describe(w, 2, 64, across ? 64 : a.columns / 2, true, &map_w)) != GSB_OK) return st;
   return by_experts(ctx, num_experts, num_rows, offsets, [&](const Groups& g) {
-    ScopedKernelTimer timer(ctx, KID_EXPERT_PRODUCT, stream);
-    const ProductArgs a{g, rows, weights, rows_stride, weights_expert_stride, weights_k_stride, weights_n_stride, (u32)k, (u32)n, nullptr, nullptr};
-    if (dtype == GSB_F32) launch_behind(stream, k_product<float, float>, kNumSMs * 4, kThreads, a, (float*)out);
-    else if (dtype == GSB_F16) launch_behind(stream, k_product<__half, __half>, kNumSMs * 4, kThreads, a, (__half*)out);
-    else launch_behind(stream, k_product<__nv_bfloat16, __nv_bfloat16>, kNumSMs * 4, kThreads, a, (__nv_bfloat16*)out);
-    GSB_LAUNCH_OK();
-    return (int)GSB_OK;
+    a.groups = g;
+    const i64 tiles = (num_rows / kPairRows + g.experts) * ((n + a.columns - 1) / a.columns);
+    return with_type(dtype, [&](auto value, auto parts) {
+      typedef decltype(value) T;
+      constexpr int P = decltype(parts)::value;
+      if (across) return launch_tiles<T, false, P, false, true>(ctx, stream, map_x, map_w, a, tiles, (T*)out);
+      return launch_tiles<T, false, P, false, false>(ctx, stream, map_x, map_w, a, tiles, (T*)out);
+    });
   });
 }
 
 extern "C" int64_t gsb_expert_product_grad_workspace(const void* rows, int dtype, int64_t num_rows, int64_t k, int64_t rows_stride, const void* grad,
                                                      int64_t n, int64_t grad_stride, int64_t num_experts) {
-  return 0;
+  if (value_bytes(dtype) == 0 || num_rows < 0 || num_rows >= ((i64)1 << 31) || k < 1 || k > GSB_MAX_ROW_LEN || n < 1 || n > GSB_MAX_ROW_LEN ||
+      num_experts < 1 || num_experts > GSB_MAX_EXPERTS)
+    return GSB_ERR_INVALID_ARGUMENT;
+  const i64 chunk = chunk_rows(num_rows, k, n, tile_columns(n, dtype), num_experts);
+  return rounded(min(num_experts, (i64)kPlanExperts) * 2 * (i64)sizeof(CUtensorMap)) + rows_operand(rows, dtype, num_rows, k, rows_stride).bytes() +
+         rows_operand(grad, dtype, num_rows, n, grad_stride).bytes() + (chunk < num_rows ? rounded(most_chunks(num_rows, chunk, num_experts) * k * n * 4) : 0);
 }
 
 extern "C" int gsb_expert_product_grad(gsb_ctx* ctx, void* stream_, const void* rows, int dtype, int64_t num_rows, int64_t k, int64_t rows_stride,
                                        const void* grad, int64_t n, int64_t grad_stride, const int64_t* offsets, int64_t num_experts, void* out,
                                        void* workspace, int64_t workspace_bytes) {
   GSB_ENTER(ctx);
-  const int st = check_product(num_rows, k, n, num_experts, rows_stride, offsets);
+  int st = check_product(num_rows, k, n, num_experts, rows_stride, offsets);
   if (st != GSB_OK) return st;
   const int size = value_bytes(dtype);
   GSB_REQUIRE(size != 0 && grad_stride >= 0 && out && ((rows && grad) || num_rows == 0), GSB_ERR_INVALID_ARGUMENT);
   GSB_REQUIRE(aligned_to(size, (const char*)rows, (const char*)grad, (const char*)out), GSB_ERR_INVALID_ARGUMENT);
   cudaStream_t stream = (cudaStream_t)stream_;
-  return by_experts(ctx, num_experts, num_rows, offsets, [&](const Groups& g) {
-    ScopedKernelTimer timer(ctx, KID_EXPERT_PRODUCT, stream);
-    with_unit(dtype, size, [&](auto value, auto) {
+  if (num_rows == 0) {
+    GSB_CUDA_OK(cudaMemsetAsync(out, 0, (size_t)(num_experts * k * n * size), stream));
+    return GSB_OK;
+  }
+  const int64_t need = gsb_expert_product_grad_workspace(rows, dtype, num_rows, k, rows_stride, grad, n, grad_stride, num_experts);
+  GSB_REQUIRE(need >= 0 && workspace && aligned_to(256, (const char*)workspace), GSB_ERR_INVALID_ARGUMENT);
+  GSB_REQUIRE(workspace_bytes >= need, GSB_ERR_CAPACITY);
+  char* room = (char*)workspace;
+  CUtensorMap* maps = (CUtensorMap*)room;
+  room += rounded(min(num_experts, (i64)kPlanExperts) * 2 * (i64)sizeof(CUtensorMap));
+  Lines x = rows_operand(rows, dtype, num_rows, k, rows_stride), d = rows_operand(grad, dtype, num_rows, n, grad_stride);
+  if ((st = bring(ctx, stream, &x, &room)) != GSB_OK || (st = bring(ctx, stream, &d, &room)) != GSB_OK) return st;
+  TileArgs a = {};
+  a.k = (u32)k;
+  a.n = (u32)n;
+  a.columns = tile_columns(n, dtype);
+  const i64 chunk = chunk_rows(num_rows, k, n, a.columns, num_experts);
+  a.chunk = (u32)chunk;
+  a.maps = maps;
+  a.partial = chunk < num_rows ? (float*)room : nullptr;
+  CUtensorMap map_x, map_d;
+  if ((st = describe(x, 2, 64, 64, false, &map_x)) != GSB_OK || (st = describe(d, 2, 64, 64, false, &map_d)) != GSB_OK) return st;
+  return by_experts(ctx, num_experts, num_rows, offsets, [&](const Groups& g) -> int {
+    a.groups = g;
+    {
+      ScopedKernelTimer timer(ctx, KID_EXPERT_PRODUCT, stream);
+      launch_behind(stream, k_expert_maps, grid_for(2 * g.experts, kMapWarps), 32 * kMapWarps, map_x, map_d, g, (const char*)x.at, x.height > 1 ? x.stride * 2 : 0, (const char*)d.at,
+                    d.height > 1 ? d.stride * 2 : 0, maps);
+      GSB_LAUNCH_OK();
+    }
+    const i64 tiles = (num_rows / chunk + g.experts) * ((k + kPairRows - 1) / kPairRows) * ((n + a.columns - 1) / a.columns);
+    return with_type(dtype, [&](auto value, auto parts) -> int {
       typedef decltype(value) T;
-      launch_behind(stream, k_grad_weights<T>, kNumSMs * 4, kThreads, g, (const T*)rows, rows_stride, (u32)k, (const T*)grad, grad_stride, (u32)n,
-                    (T*)out);
+      const int launched = launch_tiles<T, false, decltype(parts)::value, true, true>(ctx, stream, map_x, map_d, a, tiles, (T*)out);
+      if (launched != GSB_OK || !a.partial) return launched;
+      ScopedKernelTimer timer(ctx, KID_EXPERT_PRODUCT, stream);
+      launch_behind(stream, k_add_chunks<T>, (int)min((i64)kNumSMs * 8, (i64)grid_for(k * n * g.experts, kTileThreads)), kTileThreads, g, a.chunk, k * n,
+                    (const float*)a.partial, (T*)out);
+      GSB_LAUNCH_OK();
+      return GSB_OK;
     });
-    GSB_LAUNCH_OK();
-    return (int)GSB_OK;
   });
 }
 
@@ -193,24 +645,32 @@ extern "C" int gsb_expert_product_int8(gsb_ctx* ctx, void* stream_, const int8_t
                                        const float* scales, const int8_t* weight_values, int64_t weight_expert_stride, int64_t weight_n_stride,
                                        const float* weight_scales, int64_t n, const int64_t* offsets, int64_t num_experts, void* out, int out_dtype) {
   GSB_ENTER(ctx);
-  const int st = check_product(num_rows, k, n, num_experts, values_stride, offsets);
+  int st = check_product(num_rows, k, n, num_experts, values_stride, offsets);
   if (st != GSB_OK) return st;
   const int size = value_bytes(out_dtype);
   GSB_REQUIRE(size != 0 && k <= GSB_MAX_INT8_ROW_LEN && weight_expert_stride >= 0 && weight_n_stride >= 0, GSB_ERR_INVALID_ARGUMENT);
-  GSB_REQUIRE(aligned_to(16, values, weight_values) && values_stride % 16 == 0 && weight_expert_stride % 16 == 0 && weight_n_stride % 16 == 0,
+  GSB_REQUIRE(aligned_to(16, values, weight_values) && (num_rows <= 1 || (values_stride > 0 && values_stride % 16 == 0)) &&
+                  (num_experts == 1 || (weight_expert_stride > 0 && weight_expert_stride % 16 == 0)) &&
+                  (n == 1 || (weight_n_stride > 0 && weight_n_stride % 16 == 0)),
               GSB_ERR_INVALID_ARGUMENT);
   if (num_rows == 0) return GSB_OK;
   GSB_REQUIRE(values && scales && weight_values && weight_scales && out && aligned_to(4, scales, weight_scales) && aligned_to(size, (const char*)out),
               GSB_ERR_INVALID_ARGUMENT);
   cudaStream_t stream = (cudaStream_t)stream_;
+  const Lines x{values, 1, 0, num_rows, values_stride, k, GSB_F16};
+  const Lines w{weight_values, num_experts, num_experts > 1 ? weight_expert_stride : 0, n, weight_n_stride, k, GSB_F16};
+  TileArgs a = {};
+  a.depth = (u32)k;
+  a.n = (u32)n;
+  a.columns = tile_columns(n, GSB_F16);
+  a.expert_step = num_experts > 1;
+  a.row_scales = scales;
+  a.weight_scales = weight_scales;
+  CUtensorMap map_x, map_w;
+  if ((st = describe(x, 1, 128, 128, false, &map_x)) != GSB_OK || (st = describe(w, 1, 128, a.columns / 2, true, &map_w)) != GSB_OK) return st;
   return by_experts(ctx, num_experts, num_rows, offsets, [&](const Groups& g) {
-    ScopedKernelTimer timer(ctx, KID_EXPERT_PRODUCT, stream);
-    const ProductArgs a{g, values, weight_values, values_stride, weight_expert_stride, 1, weight_n_stride, (u32)k, (u32)n, scales, weight_scales};
-    with_unit(out_dtype, size, [&](auto value, auto) {
-      typedef decltype(value) Out;
-      launch_behind(stream, k_product<signed char, Out>, kNumSMs * 4, kThreads, a, (Out*)out);
-    });
-    GSB_LAUNCH_OK();
-    return (int)GSB_OK;
+    a.groups = g;
+    const i64 tiles = (num_rows / kPairRows + g.experts) * ((n + a.columns - 1) / a.columns);
+    return with_type(out_dtype, [&](auto value, auto) { return launch_tiles<decltype(value), true, 1, false, false>(ctx, stream, map_x, map_w, a, tiles, (decltype(value)*)out); });
   });
 }

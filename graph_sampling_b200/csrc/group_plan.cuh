@@ -16,8 +16,8 @@ struct Groups {
   i64* counters;
 };
 
-// begin[e] .. begin[e + 1]: rows of expert e; tile[e] .. tile[e + 1]: its row tiles.  Offsets that decrease or lie outside the rows are
-// brought into range, so that nothing out of range is read or written, and recorded.
+// begin[e] .. begin[e + 1]: rows of expert e; tile[e] .. tile[e + 1]: its row tiles.  Offsets outside the rows are brought into range and
+// ones below an earlier one raised to it, so that no row is in two experts and nothing out of range is read or written; both are recorded.
 struct PlanTable {
   u32 begin[kPlanExperts + 1];
   u32 tile[kPlanExperts + 1];
@@ -42,14 +42,31 @@ __device__ __forceinline__ void make_plan(PlanTable& plan, const Groups& g, u32 
     if (bad && blockIdx.x == 0) raise_error(g.counters, GSB_ERR_INDEX_RANGE, g.first + e);
   }
   __syncthreads();
+  u32 most = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i)
+    if (t * kEach + i <= g.experts) most = max(most, plan.begin[t * kEach + i]);
+  for (int o = 1; o < 32; o <<= 1) {
+    const u32 up = __shfl_up_sync(0xffffffffu, most, o);
+    if ((t & 31) >= o) most = max(most, up);
+  }
+  if ((t & 31) == 31) plan.carry[t >> 5] = most;
+  most = __shfl_up_sync(0xffffffffu, most, 1);
+  if ((t & 31) == 0) most = 0;
+  __syncthreads();
+  for (int w = 0; w < (t >> 5); ++w) most = max(most, plan.carry[w]);
+#pragma unroll
+  for (int i = 0; i < kEach; ++i)
+    if (t * kEach + i <= g.experts) plan.begin[t * kEach + i] = most = max(most, plan.begin[t * kEach + i]);
+  if (t == THREADS - 1 && THREADS * kEach == g.experts) plan.begin[g.experts] = max(most, plan.begin[g.experts]);
+  __syncthreads();
   u32 own[kEach], sum = 0;
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
     const int e = t * kEach + i;
     u32 tiles = 0;
     if (e < g.experts) {
-      const u32 b = plan.begin[e], end = plan.begin[e + 1];
-      tiles = end > b ? (end - b + tile_rows - 1) / tile_rows : 0;
+      tiles = (plan.begin[e + 1] - plan.begin[e] + tile_rows - 1) / tile_rows;
       if (tiles < at_least) tiles = at_least;
     }
     own[i] = sum;
@@ -82,11 +99,6 @@ __device__ __forceinline__ int expert_of_tile(const PlanTable& plan, int experts
     else high = mid;
   }
   return low;
-}
-
-// Rows of an expert: none where the next one's offset is smaller.
-__device__ __forceinline__ u32 rows_end(const PlanTable& plan, int e) {
-  return plan.begin[e + 1] > plan.begin[e] ? plan.begin[e + 1] : plan.begin[e];
 }
 
 }  // namespace gsb

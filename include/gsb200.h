@@ -635,7 +635,7 @@ GSB_API int gsb_expert_combine_grad(gsb_ctx* ctx, void* stream, const void* grad
 
 /* ---- products over rows sorted by expert, in float types and in 8 bits; dropout ------------------------------------------
  * As the calls on learned rows above.  offsets[num_experts + 1] (DEVICE, as gsb_expert_order gives it): rows offsets[e] ..
- * offsets[e + 1] are those of expert e; offsets that decrease or lie outside the rows are brought into range, with
+ * offsets[e + 1] are those of expert e; offsets outside the rows are brought into range and ones below an earlier one raised to it, with
  * GSB_ERR_INDEX_RANGE recorded.  num_rows below 2^31; k and n between 1 and GSB_MAX_ROW_LEN.
  * Product: out[r, :] = rows[r, :] W[e(r)], zeros for rows of no expert; W[e][i][j] = weights[e * weights_expert_stride +
  * i * weights_k_stride + j * weights_n_stride] for i < k, j < n, so the transposed matrices are the same memory with two strides

@@ -10,9 +10,11 @@ MASK32 = 0xFFFFFFFF
 
 
 def bounds(offsets, num_rows):
-    """The experts' rows as the operators take them: offsets brought into range."""
-    at = [min(max(o, 0), num_rows) for o in offsets.tolist()]
-    return [(a, max(a, b)) for a, b in zip(at, at[1:])]
+    """The experts' rows as the operators take them: offsets brought into range, and none below an earlier one."""
+    at = []
+    for o in offsets.tolist():
+        at.append(max(at[-1:] + [min(max(o, 0), num_rows)]))
+    return list(zip(at, at[1:]))
 
 
 def product(rows, weights, offsets):

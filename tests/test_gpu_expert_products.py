@@ -145,7 +145,7 @@ def test_offsets_out_of_range(ops):
             with pytest.raises(GsbError):
                 ctx.check_device()
         offsets = torch.tensor([0, 60, 30, 100], device="cuda")               # decreasing: the middle one has no rows
-        assert ops.expert_product(rows, weights, offsets, ctx=ctx)[:30].isfinite().all()
+        within(ops.expert_product(rows, weights, offsets, ctx=ctx), *exact.product(rows, weights, offsets))
         with pytest.raises(GsbError):
             ctx.check_device()
         within(ops.expert_product_grad(rows, grad, offsets, ctx=ctx), *exact.grad_weights(rows, grad, offsets))
