@@ -17,10 +17,25 @@
 namespace gsb {
 
 // A pair of CTAs takes a tile of 256 rows of the result, 128 each, by `columns` (128 or 256); each holds half of the columns' operand.
-constexpr int kPairRows = 256, kTileThreads = 256, kMaxStages = 8;
+constexpr int kPairRows = 256, kMaxStages = 8;
 constexpr int kSumColumns = 512;                 // of tensor memory: two tiles' sums, so that one is written out while the next is made
 constexpr int kRowsOperand = 128 * kLineBytes;   // bytes of a CTA's rows in a stage
 constexpr int kAcross = 64 * kLineBytes;         // a block of 64 lines
+// Warps: 0 loads by TMA, 1 (of the first CTA) issues the matrix instructions, 4 to 11 write results out, 12 to 19 read what TMA cannot, and 3
+// hands over what they have read.
+constexpr int kWriters = 8, kFirstReader = 4 + kWriters, kReaders = 8;
+constexpr int tile_threads(bool read) { return 32 * (kFirstReader + (read ? kReaders : 0)); }
+
+// The widest access, of at most 16 bytes, that addresses with these bits allow.
+__device__ __forceinline__ int unit_of(u64 bits) { return bits % 16 == 0 ? 16 : bits % 8 == 0 ? 8 : bits % 4 == 0 ? 4 : 2; }
+
+// Rows as they lie in memory, for the warps that read them.
+struct RawRows {
+  const void* at;
+  i64 stride;   // in values
+  u32 width;
+  int unit;     // bytes that an access may have
+};
 
 struct TileArgs {
   Groups groups;
@@ -31,6 +46,7 @@ struct TileArgs {
   int stages;
   int expert_step;           // 0: one matrix for all experts
   const CUtensorMap* maps;   // gradient: each expert's rows and gradient rows
+  RawRows rows, grad;        // where they are read by warps
   float* partial;            // gradient: sums of the chunks (null: one chunk per expert, written out)
   const float *row_scales, *weight_scales;  // of 8-bit operands
   u32 how;
@@ -44,7 +60,7 @@ struct Tile {
   u32 chunk;
 };
 
-template <bool GRAD, int PER_LINE>
+template <bool GRAD>
 __device__ __forceinline__ u64 number_of_tiles(const TileArgs& a, const PlanTable& plan) {
   const u32 across = (a.n + a.columns - 1) / a.columns, down = GRAD ? (a.k + kPairRows - 1) / kPairRows : 1;
   return (u64)plan.tile[a.groups.experts] * across * down;
@@ -54,7 +70,7 @@ __device__ __forceinline__ Tile tile_at(const TileArgs& a, const PlanTable& plan
   Tile r;
   const u32 across = (a.n + a.columns - 1) / a.columns, down = GRAD ? (a.k + kPairRows - 1) / kPairRows : 1;
   r.chunk = (u32)(t / (across * down));
-  const u32 rest = (u32)(t % (across * down));
+  const u32 rest = (u32)(t - (u64)r.chunk * (across * down));
   r.n0 = rest % across * a.columns;
   r.m0 = rest / across * kPairRows;
   r.e = expert_of_tile(plan, a.groups.experts, r.chunk);
@@ -65,41 +81,189 @@ __device__ __forceinline__ Tile tile_at(const TileArgs& a, const PlanTable& plan
   return r;
 }
 
-template <class T>
-__device__ __forceinline__ void store_columns(T* to, const float (&v)[32], u32 valid, bool whole) {
-  if (whole && valid >= 32) {
-    constexpr int N = 16 / sizeof(T);
+// 64 bytes of each of 32 rows of the result, a row a lane, brought through shared memory so that neighbouring lanes write neighbours: the
+// rows go to `to`, `pitch` bytes apart, `bytes` of each, in accesses of `unit` bytes, which divide them.
+constexpr int kStoreBytes = 64;
+template <class Word>
+__device__ __forceinline__ void copy_rows_by(const char* room, int lane, char* to, i64 pitch, u32 rows, u32 bytes) {
+  constexpr int W = sizeof(Word), LANES = kStoreBytes / W;  // of a row
+#pragma unroll 4
+  for (int i = 0; i < LANES; ++i) {
+    const u32 at = i * 32 + lane, r = at / LANES, x = at % LANES * W;
+    if (r < rows && x < bytes) *(Word*)(to + r * pitch + x) = *(const Word*)(room + r * kStoreBytes + ((x >> 4 ^ (r >> 1 & 3)) << 4) + (x & 15));
+  }
+}
+static __device__ __noinline__ void copy_rows(const char* room, int lane, char* to, i64 pitch, u32 rows, u32 bytes, int unit) {
+  __syncwarp();
+  if (unit == 16) copy_rows_by<uint4>(room, lane, to, pitch, rows, bytes);
+  else if (unit == 8) copy_rows_by<uint2>(room, lane, to, pitch, rows, bytes);
+  else if (unit == 4) copy_rows_by<u32>(room, lane, to, pitch, rows, bytes);
+  else copy_rows_by<unsigned short>(room, lane, to, pitch, rows, bytes);
+  __syncwarp();
+}
+template <class U>
+__device__ __forceinline__ void write_rows(char* room, int lane, const float (&v)[kStoreBytes / sizeof(U)], U* to, i64 pitch, u32 rows, u32 columns, int unit) {
+  constexpr int PER = 16 / sizeof(U);
 #pragma unroll
-    for (int u = 0; u < 32 / N; ++u) {
-      float f[N];
+  for (int p = 0; p < 4; ++p) {
+    float f[PER];
 #pragma unroll
-      for (int q = 0; q < N; ++q) f[q] = v[u * N + q];
-      Unit<T, 16> w;
-      w.set(f);
-      store_unit((Unit<T, 16>*)to + u, w);
+    for (int q = 0; q < PER; ++q) f[q] = v[p * PER + q];
+    Unit<U, 16> w;
+    w.set(f);
+    *(uint4*)(room + lane * kStoreBytes + ((p ^ (lane >> 1 & 3)) << 4)) = w.w;
+  }
+  copy_rows(room, lane, (char*)to, pitch * (i64)sizeof(U), rows, columns * (u32)sizeof(U), unit);
+}
+
+// ---- rows read by warps: rows of any address and distance, and float32, which is taken apart on the way ----------------------------
+// 16-bit values: a warp copies a line at a time, two neighbouring values a lane, straight to where they belong; every eighth line of an
+// operand, `lines` of them with values, the others zeros.  `valid`: of the lane's two columns;
+// `some`: an address in the array, for what is not read.
+template <int LINES>
+__device__ __forceinline__ void copy_lines(u32 to, const unsigned short* from, i64 step, int lines, u32 valid, bool aligned, const void* some) {
+  if (aligned && valid != 1) {
+    const u32 bytes = 2 * valid;
+    if (valid == 0) lines = 0;
+#pragma unroll
+    for (int i = 0; i < LINES; ++i, from += step) {
+      const bool in = i < lines;
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + i * 8 * kLineBytes), "l"(in ? from : (const unsigned short*)some), "r"(in ? bytes : 0) : "memory");
     }
   } else {
 #pragma unroll
-    for (int q = 0; q < 32; ++q)
-      if ((u32)q < valid) to[q] = from_float<T>(v[q]);
+    for (int i0 = 0; i0 < LINES; i0 += 8) {
+      u32 w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i, from += step) {
+        const bool in = i0 + i < lines;
+        w[i] = in && valid > 0 ? __ldg(from) : 0;
+        w[i] |= in && valid > 1 ? (u32)__ldg(from + 1) << 16 : 0;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) asm volatile("st.shared.b32 [%0], %1;" ::"r"(to + (i0 + i) * 8 * kLineBytes), "r"(w[i]) : "memory");
+    }
+  }
+}
+__device__ __forceinline__ void write_line(u32 to, const u32 (&w)[4]) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+}
+
+// float32: a piece is 8 neighbouring values of a row, copied behind the thread's back into a place of its own in shared memory, in two
+// halves `kRing` bytes apart.  `valid`: how many of them there are; `some`: an address in the array, for pieces without any.
+constexpr int kRing = 32 * kReaders * 16;
+__device__ __forceinline__ void copy_piece(u32 to, const float* from, int valid, bool aligned, const void* some) {
+  if (valid <= 0 || (valid >= 8 && aligned)) {
+    const u32 bytes = valid > 0 ? 16 : 0;
+    const float* at = valid > 0 ? from : (const float*)some;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(at), "r"(bytes) : "memory");
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + kRing), "l"(at + bytes / 4), "r"(bytes) : "memory");
+  } else {
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + q / 4 * kRing + q % 4 * 4), "l"(q < valid ? from + q : from),
+                   "r"(q < valid ? 4 : 0)
+                   : "memory");
+  }
+}
+__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
+
+// The next part of a float32 value, and what is left of it.  To nearest, but the largest numbers downwards, where that would be infinity.
+// Infinities and NaN are all in the first part.
+__device__ __forceinline__ u32 next_part(float& rest) {
+  const bool finite = fabsf(rest) <= 3.402823466e38f;
+  const __nv_bfloat16 part = finite && fabsf(rest) > 3.38e38f ? __float2bfloat16_rz(rest) : __float2bfloat16_rn(rest);
+  rest = finite ? rest - __bfloat162float(part) : 0.f;
+  return __bfloat16_as_ushort(part);
+}
+// Two parts of neighbours in a word; what is left of them stays.
+__device__ __forceinline__ u32 next_parts(float& low, float& high) {
+  u32 w;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(high), "f"(low));
+  low -= __uint_as_float(w << 16);
+  high -= __uint_as_float(w & 0xffff0000u);
+  return w;
+}
+// Two copied pieces to their places, 32 lines apart, every part in an operand of its own, `apart` bytes from the one before.
+__device__ __forceinline__ void write_parts(u32 ring, u32 to, u32 apart) {
+  float rest[2][8];
+#pragma unroll
+  for (int h = 0; h < 4; ++h)
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(rest[h / 2][h % 2 * 4]), "=f"(rest[h / 2][h % 2 * 4 + 1]), "=f"(rest[h / 2][h % 2 * 4 + 2]), "=f"(rest[h / 2][h % 2 * 4 + 3])
+                 : "r"(ring + h * kRing)
+                 : "memory");
+  u32 w[2][4];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i / 4][i % 4] = next_parts(rest[i / 4][2 * (i % 4)], rest[i / 4][2 * (i % 4) + 1]);
+  // what is left of an infinity, of NaN and of what became an infinity is none of the numbers
+  float any = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) any += (rest[0][2 * i] + rest[0][2 * i + 1]) + (rest[1][2 * i] + rest[1][2 * i + 1]);
+  if (fabsf(any) <= 3.402823466e38f) {
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+      if (p > 0)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i / 4][i % 4] = next_parts(rest[i / 4][2 * (i % 4)], rest[i / 4][2 * (i % 4) + 1]);
+      write_line(to + p * apart, w[0]);
+      write_line(to + p * apart + 32 * kLineBytes, w[1]);
+    }
+  } else {
+#pragma unroll 1
+    for (int h = 0; h < 8; ++h) {
+      float two[2];
+      asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(two[0]), "=f"(two[1]) : "r"(ring + h / 2 * kRing + h % 2 * 8) : "memory");
+      for (int p = 0; p < 3; ++p) {
+        const u32 low = next_part(two[0]);
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(to + p * apart + h / 4 * 32 * kLineBytes + h % 4 * 4), "r"(low | next_part(two[1]) << 16) : "memory");
+      }
+    }
   }
 }
 
-// Warp 0 of each CTA loads, warp 1 of the first one issues the matrix instructions, warps 4 to 7 write results out.
-// PARTS: 3 for float32, else 1.  ACROSS: the second operand's lines hold the reduced index across them (a gradient's both do).
-template <class T, bool WHOLE_NUMBERS, int PARTS, bool GRAD, bool ACROSS>
-__global__ void __launch_bounds__(kTileThreads, 1) k_tiles(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                                                           const TileArgs a, T* __restrict__ out) {
+// The lines of the reduced index that a pair of CTAs goes through, tile by tile.
+template <bool GRAD, int PER_LINE>
+struct Walk {
+  u64 t;
+  u32 b;
+  Tile tile;
+  __device__ __forceinline__ void settle(const TileArgs& a, const PlanTable& plan, u64 tiles, u64 step) {  // to the next tile that has lines
+    while (t < tiles && (tile = tile_at<GRAD, PER_LINE>(a, plan, t)).blocks == 0) t += step;
+  }
+  __device__ __forceinline__ void next(const TileArgs& a, const PlanTable& plan, u64 tiles, u64 step) {
+    if (++b < tile.blocks) return;
+    b = 0;
+    t += step;
+    settle(a, plan, tiles, step);
+  }
+};
+
+// float32 pieces that a reader has on their way: three times two.
+constexpr int kPairsAhead = 3;
+constexpr int ring_bytes(int parts) { return parts == 3 ? kPairsAhead * 4 * kRing : 0; }
+
+// PARTS: 3 for float32, else 1.  ACROSS: the second operand's lines hold the reduced index across them (a gradient's both do).  READ: rows
+// (and a gradient's both operands) are read by warps, not by TMA.
+template <class T, bool WHOLE_NUMBERS, int PARTS, bool GRAD, bool ACROSS, bool READ>
+__global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                                                                 const TileArgs a, T* __restrict__ out) {
   constexpr int kPerLine = kLineBytes / (WHOLE_NUMBERS ? 1 : 2);
-  // float32: sums leave tensor memory, where additions cut, after this many lines of the reduced index, and are added up in registers
+  // float32: sums leave tensor memory, where additions cut, after this many lines of the reduced index, and are added up in registers.
+  // Over 16 instructions that is an error of 2.3e-7 of the sums (rms), over 32 4.7e-7
   constexpr u32 kDrain = PARTS > 1 ? 4 : 0xffffffffu;
   extern __shared__ char raw[];
   __shared__ PlanTable plan;
-  __shared__ __align__(8) u64 bars[2 * kMaxStages + 4];
+  __shared__ __align__(8) u64 bars[3 * kMaxStages + 4];
+  __shared__ float column_scales[WHOLE_NUMBERS ? kWriters : 1][128];
+  __shared__ __align__(16) char rooms[kWriters][32 * kStoreBytes];
   __shared__ u32 sums_at;
   __shared__ volatile int stop;
   const u32 stages_at = (smem_address(raw) + 1023u) & ~1023u;
-  const u32 full = smem_address(bars), empty = full + 8 * kMaxStages, sums_full = full + 16 * kMaxStages, sums_empty = sums_full + 16;
+  const u32 full = smem_address(bars), empty = full + 8 * kMaxStages, written = full + 16 * kMaxStages;
+  const u32 sums_full = full + 24 * kMaxStages, sums_empty = sums_full + 16;
   const u32 rank = rank_in_pair();
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   const Groups& g = a.groups;
@@ -108,31 +272,32 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_tiles(const __grid_constant
   if (threadIdx.x == 0) {
     stop = 0;
     for (int s = 0; s < kMaxStages; ++s) {
-      barrier_init(full + 8 * s, 1);
+      barrier_init(full + 8 * s, (READ && GRAD ? 0 : 1) + (READ ? 2 : 0));
+      barrier_init(written + 8 * s, kReaders);
       barrier_init(empty + 8 * s, 1);
     }
     for (int s = 0; s < 2; ++s) {
       barrier_init(sums_full + 8 * s, 1);
-      barrier_init(sums_empty + 8 * s, 8);  // the warps that write out, of both CTAs
+      barrier_init(sums_empty + 8 * s, 2 * kWriters);
     }
     barriers_ready();
     if (!GRAD) {
-      prefetch_map(&map_a);
+      if (!READ) prefetch_map(&map_a);
       prefetch_map(&map_b);
     }
   }
   if (warp == 2) sums_alloc(smem_address(&sums_at), kSumColumns);
-  make_plan<kTileThreads>(plan, g, GRAD ? a.chunk : kPairRows, GRAD ? 1 : 0);
+  make_plan<tile_threads(READ)>(plan, g, GRAD ? a.chunk : kPairRows, GRAD ? 1 : 0);
   sums_fence_before();
   cluster_barrier();
   sums_fence_after();
   const u32 sums = sums_at;
-  const u64 tiles = number_of_tiles<GRAD, kPerLine>(a, plan);
+  const u64 tiles = number_of_tiles<GRAD>(a, plan);
   const u64 first = blockIdx.x / 2, step = gridDim.x / 2;
   const u32 half = a.columns / 2, b_bytes = half * kLineBytes, stage_bytes = PARTS * (kRowsOperand + b_bytes);
 
-  if (warp == 0 && lane == 0) {
-    const u32 full_of_first = address_in(full, 0);
+  if (warp == 0 && lane == 0 && !(READ && GRAD)) {
+    const u32 full_of_first = address_in(full, 0), loaded_bytes = 2 * PARTS * ((READ ? 0 : kRowsOperand) + b_bytes);
     u32 stage = 0, turn = 0;
     for (u64 t = first; t < tiles; t += step) {
       const Tile tile = tile_at<GRAD, kPerLine>(a, plan, t);
@@ -148,7 +313,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_tiles(const __grid_constant
       const int matrix = (g.first + tile.e) * a.expert_step;
       for (u32 b = 0; b < tile.blocks; ++b) {
         if (!barrier_wait(empty + 8 * stage, turn ^ 1, &stop, counters)) goto loaded;
-        if (rank == 0) barrier_expect(full + 8 * stage, 2 * stage_bytes);
+        if (rank == 0) barrier_expect(full + 8 * stage, loaded_bytes);
         const u32 at = stages_at + stage * stage_bytes, bar = full_of_first + 8 * stage;
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) {
@@ -158,7 +323,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_tiles(const __grid_constant
             for (u32 j = 0; j < half / 64; ++j)
               load_tile(to_b + j * kAcross, of_b, bar, (int)(tile.n0 + rank * half + j * 64), (int)(tile.row0 + b * 64), p);
           } else {
-            load_tile(to_a, of_a, bar, (int)(b * kPerLine), (int)(tile.row0 + rank * 128), p);
+            if (!READ) load_tile(to_a, of_a, bar, (int)(b * kPerLine), (int)(tile.row0 + rank * 128), p);
             if (ACROSS)
               for (u32 j = 0; j < half / 64; ++j)
                 load_tile(to_b + j * kAcross, of_b, bar, (int)(tile.n0 + rank * half + j * 64), (int)(b * kPerLine), matrix, p);
@@ -174,12 +339,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_tiles(const __grid_constant
     constexpr bool A_ACROSS = GRAD, B_ACROSS = GRAD || ACROSS;
     u32 stage = 0, turn = 0, made = 0;
     for (u64 t = first; t < tiles; t += step) {
-      const Tile tile = tile_at<GRAD, kPerLine>(a, plan, t);
-      for (u32 b0 = 0; b0 < tile.blocks; b0 += min(kDrain, tile.blocks - b0), ++made) {
+      const u32 blocks = tile_at<GRAD, kPerLine>(a, plan, t).blocks;
+      for (u32 b0 = 0; b0 < blocks; b0 += min(kDrain, blocks - b0), ++made) {
         const u32 buffer = made & 1, to = sums + buffer * 256;
         if (!barrier_wait(sums_empty + 8 * buffer, (made >> 1 & 1) ^ 1, &stop, counters)) goto issued;
         sums_fence_after();
-        for (u32 b = b0; b < b0 + min(kDrain, tile.blocks - b0); ++b) {
+        for (u32 b = b0; b < b0 + min(kDrain, blocks - b0); ++b) {
           if (!barrier_wait(full + 8 * stage, turn, &stop, counters)) goto issued;
           sums_fence_after();
           const u32 at = stages_at + stage * stage_bytes;
@@ -205,37 +370,202 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_tiles(const __grid_constant
       }
     }
   issued:;
-  } else if (warp >= 4) {
-    const u32 quarter = (u32)(warp & 3) * 32, row = rank * 128 + quarter + lane;  // of the tile
+  } else if (READ && warp == 3 && lane == 0) {
+    // The readers' fence towards the tensor cores: theirs would wait for their copies that are on their way
+    const u32 full_of_first = address_in(full, 0);
+    u32 stage = 0, turn = 0;
+    for (u64 t = first; t < tiles; t += step) {
+      const u32 blocks = tile_at<GRAD, kPerLine>(a, plan, t).blocks;
+      for (u32 b = 0; b < blocks; ++b) {
+        if (!barrier_wait(written + 8 * stage, turn, &stop, counters)) goto handed_over;
+        written_for_tensor_cores();
+        barrier_arrive_at(full_of_first + 8 * stage);
+        if (++stage == (u32)a.stages) stage = 0, turn ^= 1;
+      }
+    }
+  handed_over:;
+  } else if (READ && warp >= kFirstReader) {
+    // All readers take a stage together; what comes next is on its way while they write
+    const u32 me = threadIdx.x - 32 * kFirstReader;
+    u32 stage = 0, turn = 0;
+    Walk<GRAD, kPerLine> now{first, 0, {}};
+    now.settle(a, plan, tiles, step);
+    // first of a tile's rows that the reduced index runs over (gradient), or of this CTA's (product)
+    auto first_row = [&](const Tile& tile) { return GRAD ? (i64)plan.begin[tile.e] + tile.row0 : (i64)tile.row0 + rank * 128; };
+    auto rows_here = [&](const Tile& tile) { return GRAD ? (int)tile.rows : (int)tile.rows - (int)rank * 128; };
+    if constexpr (PARTS == 3) {
+      // a thread has the 16 bytes `chunk` of lines segment, segment + 32 and so on of a stage; two lines at a time
+      constexpr int kPairs = GRAD ? 3 : 2;
+      const u32 chunk = me & 7, segment = me / 8, place = segment * kLineBytes + ((chunk ^ (segment & 7)) << 4);
+      const u32 ring = stages_at + a.stages * stage_bytes + me * 16;
+      const bool aligned = a.rows.unit == 16, grad_aligned = a.grad.unit == 16;
+      Walk<GRAD, kPerLine> ahead = now;
+      const float *from = nullptr, *from_grad = nullptr;
+      int columns = 0, grad_columns = 0, rows_left = 0, pair = 0;  // from this thread's first on
+      auto begin_tile = [&] {
+        if (ahead.t >= tiles) return;
+        const Tile& tile = ahead.tile;
+        const u32 c = (GRAD ? tile.m0 + rank * 128 : 0) + chunk * 8;
+        from = (const float*)a.rows.at + (first_row(tile) + segment) * a.rows.stride + c;
+        columns = (int)a.rows.width - (int)c;
+        rows_left = rows_here(tile) - (int)segment;
+        if (GRAD) {
+          const u32 d = tile.n0 + rank * half + chunk * 8;
+          from_grad = (const float*)a.grad.at + (first_row(tile) + segment) * a.grad.stride + d;
+          grad_columns = (int)a.grad.width - (int)d;
+        }
+      };
+      begin_tile();
+      auto copy = [&](u32 slot) {
+        if (ahead.t < tiles) {
+          const u32 to = ring + slot * 4 * kRing;
+          if (GRAD && pair == 2) {
+            copy_piece(to, from_grad, rows_left > 0 ? grad_columns : 0, grad_aligned, a.grad.at);
+            copy_piece(to + 2 * kRing, from_grad + 32 * a.grad.stride, rows_left > 32 ? grad_columns : 0, grad_aligned, a.grad.at);
+          } else {
+            const float* at = from + (GRAD ? (i64)pair * 64 : pair * 64 * a.rows.stride);
+            const int rows = rows_left - (GRAD ? 0 : pair * 64), width = columns - (GRAD ? pair * 64 : 0);
+            copy_piece(to, at, rows > 0 ? width : 0, aligned, a.rows.at);
+            copy_piece(to + 2 * kRing, at + 32 * a.rows.stride, rows > 32 ? width : 0, aligned, a.rows.at);
+          }
+          if (++pair == kPairs) {
+            pair = 0;
+            from += GRAD ? 64 * a.rows.stride : 64;
+            if (GRAD) from_grad += 64 * a.grad.stride, rows_left -= 64;
+            else columns -= 64;
+            ahead.next(a, plan, tiles, step);
+            if (ahead.b == 0) begin_tile();
+          }
+        }
+        copies_end();
+      };
+      for (u32 slot = 0; slot < kPairsAhead; ++slot) copy(slot);
+      u32 slot = 0;
+      while (now.t < tiles) {
+        const bool free = barrier_wait(empty + 8 * stage, turn ^ 1, &stop, counters);
+        if (!__all_sync(0xffffffffu, free)) break;
+        const u32 at = stages_at + stage * stage_bytes + place;
+#pragma unroll
+        for (int q = 0; q < kPairs; ++q) {
+          copies_wait<kPairsAhead - 1>();
+          const bool of_grad = GRAD && q == 2;
+          write_parts(ring + slot * 4 * kRing, at + (of_grad ? PARTS * kRowsOperand : q * 64 * kLineBytes), of_grad ? b_bytes : kRowsOperand);
+          copy(slot);
+          if (++slot == kPairsAhead) slot = 0;
+        }
+        __syncwarp();
+        if (lane == 0) barrier_arrive(written + 8 * stage);
+        now.next(a, plan, tiles, step);
+        if (++stage == (u32)a.stages) stage = 0, turn ^= 1;
+      }
+      copies_wait<0>();
+    } else {
+      // warp w has lines w, w + 8 and so on; copies of kLag stages are on their way before the first is handed over
+      constexpr u32 kLag = 3;
+      const u32 w = me / 32, place = w * kLineBytes + (((lane >> 2) ^ w) << 4) + (lane & 3) * 4;
+      u32 handed = 0, copied = 0;
+      auto hand_over = [&] {
+        __syncwarp();
+        if (lane == 0) barrier_arrive(written + 8 * handed);
+        if (++handed == (u32)a.stages) handed = 0;
+      };
+      auto lines_of = [&](int rows) { return rows > (int)w ? (rows - (int)w + kReaders - 1) / kReaders : 0; };
+      auto valid_of = [&](const RawRows& x, u32 c) { return c < x.width ? min(2u, x.width - c) : 0; };
+      bool lost = false;
+      while (now.t < tiles) {
+        const bool free = barrier_wait(empty + 8 * stage, turn ^ 1, &stop, counters);
+        if (!__all_sync(0xffffffffu, free)) {
+          lost = true;
+          break;
+        }
+        const u32 at = stages_at + stage * stage_bytes + place;
+        const Tile& tile = now.tile;
+        const bool aligned = a.rows.unit >= 4, grad_aligned = a.grad.unit >= 4;
+        if (GRAD) {
+          const i64 row = first_row(tile) + now.b * 64 + w;
+          const int lines = lines_of(rows_here(tile) - (int)now.b * 64);
+          const unsigned short* from = (const unsigned short*)a.rows.at + row * a.rows.stride;
+          const unsigned short* from_grad = (const unsigned short*)a.grad.at + row * a.grad.stride;
+          for (u32 j = 0; j < 128; j += 64) {
+            const u32 c = tile.m0 + rank * 128 + j + lane * 2;
+            copy_lines<8>(at + j * kLineBytes, from + c, kReaders * a.rows.stride, lines, valid_of(a.rows, c), aligned, a.rows.at);
+          }
+          for (u32 j = 0; j < half; j += 64) {
+            const u32 c = tile.n0 + rank * half + j + lane * 2;
+            copy_lines<8>(at + kRowsOperand + j * kLineBytes, from_grad + c, kReaders * a.grad.stride, lines, valid_of(a.grad, c), grad_aligned, a.grad.at);
+          }
+        } else {
+          const u32 c = now.b * 64 + lane * 2;
+          copy_lines<16>(at, (const unsigned short*)a.rows.at + (first_row(tile) + w) * a.rows.stride + c, kReaders * a.rows.stride,
+                         lines_of(rows_here(tile)), valid_of(a.rows, c), aligned, a.rows.at);
+        }
+        copies_end();
+        if (++copied > kLag) {
+          copies_wait<kLag>();
+          hand_over();
+        }
+        now.next(a, plan, tiles, step);
+        if (++stage == (u32)a.stages) stage = 0, turn ^= 1;
+      }
+      copies_wait<0>();
+      if (!lost)
+        for (u32 left = min(copied, kLag); left > 0; --left) hand_over();
+    }
+  } else if (warp >= 4 && warp < 4 + kWriters) {
+    const u32 quarter = (u32)(warp & 3) * 32;
+    const u32 c0 = (u32)(warp - 4) / 4 * half;                                     // this warp's half of the columns
     const u32 sums_empty_of_first = address_in(sums_empty, 0);
-    const bool whole = (u64)a.n * sizeof(T) % 16 == 0 && (u64)(uintptr_t)out % 16 == 0, whole_partial = a.n % 4 == 0;
+    const int unit = unit_of((u64)(uintptr_t)out | (u64)a.n * sizeof(T)), unit_partial = unit_of((u64)a.n * 4);
+    char* const room = rooms[warp - 4];
     u32 made = 0;
     for (u64 t = first; t < tiles; t += step) {
       const Tile tile = tile_at<GRAD, kPerLine>(a, plan, t);
-      const bool mine = GRAD ? tile.m0 + row < a.k : row < tile.rows;
-      const i64 at = GRAD ? ((i64)(a.partial ? (i64)tile.chunk : (i64)(g.first + tile.e)) * a.k + tile.m0 + row) * a.n + tile.n0
-                          : (i64)(tile.row0 + row) * a.n + tile.n0;
+      const u32 limit = GRAD ? a.k - tile.m0 : tile.rows, above = rank * 128 + quarter;
+      const u32 valid_rows = limit > above ? min(32u, limit - above) : 0;
+      const bool mine = (u32)lane < valid_rows;
+      const u32 n0 = tile.n0 + c0;
+      const i64 at = GRAD ? ((i64)(a.partial ? (i64)tile.chunk : (i64)(g.first + tile.e)) * a.k + tile.m0 + above) * a.n + n0
+                          : (i64)(tile.row0 + above) * a.n + n0;
+      // 32 values of each row, in as many steps as they are 64 bytes
       auto store = [&](u32 c, const float(&v)[32]) {
-        if (!mine || tile.n0 + c >= a.n) return;
-        if (GRAD && a.partial) store_columns(a.partial + at + c, v, a.n - tile.n0 - c, whole_partial);
-        else store_columns(out + at + c, v, a.n - tile.n0 - c, whole);
+        auto write = [&](auto* to, int width) {
+          typedef std::remove_pointer_t<decltype(to)> U;
+          constexpr int N = kStoreBytes / sizeof(U);
+#pragma unroll
+          for (int x = 0; x < 32; x += N) {
+            if (n0 + c + x >= a.n || valid_rows == 0) continue;
+            float f[N];
+#pragma unroll
+            for (int q = 0; q < N; ++q) f[q] = v[x + q];
+            write_rows(room, lane, f, to + at + c + x, a.n, valid_rows, a.n - n0 - c - x, width);
+          }
+        };
+        if (GRAD && a.partial) write(a.partial, unit_partial);
+        else write(out, unit);
       };
       if (tile.blocks == 0) {
         const float zeros[32] = {};
-        for (u32 c = 0; c < a.columns; c += 32) store(c, zeros);
+        for (u32 c = 0; c < half; c += 32) store(c, zeros);
         continue;
       }
       if constexpr (PARTS == 1) {
+        float of_row = 1.f;
+        if constexpr (WHOLE_NUMBERS) {
+          if (mine) of_row = a.row_scales[tile.row0 + above + lane];
+          __syncwarp();
+          for (u32 c = lane; c < half; c += 32)
+            column_scales[warp - 4][c] = n0 + c < a.n ? __ldg(a.weight_scales + (i64)(g.first + tile.e) * a.n + n0 + c) : 0.f;
+          __syncwarp();
+        }
         const u32 buffer = made & 1;
         const bool there = barrier_wait(sums_full + 8 * buffer, made >> 1 & 1, &stop, counters);
         if (!__all_sync(0xffffffffu, there)) break;
         sums_fence_after();
-        const float of_row = WHOLE_NUMBERS && mine ? a.row_scales[tile.row0 + row] : 1.f;
-        for (u32 c = 0; c < a.columns; c += 32) {
+        for (u32 c = 0; c < half; c += 32) {
           u32 v[32];
-          read_sums(sums + (quarter << 16) + buffer * 256 + c, v);
+          read_sums(sums + (quarter << 16) + buffer * 256 + c0 + c, v);
           sums_read();
-          if (c + 32 == a.columns) {
+          if (c + 32 == half) {
             sums_fence_before();
             __syncwarp();
             if (lane == 0) barrier_arrive_at(sums_empty_of_first + 8 * buffer);
@@ -243,18 +573,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_tiles(const __grid_constant
           float f[32];
 #pragma unroll
           for (int q = 0; q < 32; ++q) {
-            if constexpr (WHOLE_NUMBERS) {
-              const u32 column = tile.n0 + c + q;
-              f[q] = (float)(int)v[q] * of_row * (column < a.n ? __ldg(a.weight_scales + (i64)(g.first + tile.e) * a.n + column) : 0.f);
-            } else {
-              f[q] = __uint_as_float(v[q]);
-            }
+            if constexpr (WHOLE_NUMBERS) f[q] = (float)(int)v[q] * of_row * column_scales[warp - 4][c + q];
+            else f[q] = __uint_as_float(v[q]);
           }
           store(c, f);
         }
         ++made;
       } else {
-        float total[4][32] = {};
+        float total[2][32] = {};
         bool lost = false;
         for (u32 b0 = 0; b0 < tile.blocks; b0 += min(kDrain, tile.blocks - b0), ++made) {
           const u32 buffer = made & 1;
@@ -264,18 +590,20 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_tiles(const __grid_constant
             break;
           }
           sums_fence_after();
-          const u32 from = sums + (quarter << 16) + buffer * 256;
+          const u32 from = sums + (quarter << 16) + buffer * 256 + c0;
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            u32 large[32], small[32];
-            read_sums(from + c * 32, large);
-            read_sums(from + 128 + c * 32, small);
-            sums_read();
 #pragma unroll
-            for (int q = 0; q < 32; ++q) {
-              // an infinity's small products are infinity times 0: the large one has the answer
-              const float of_large = __uint_as_float(large[q]);
-              total[c][q] += fabsf(of_large) <= 3.402823466e38f ? of_large + __uint_as_float(small[q]) : of_large;
+            for (int kind = 0; kind < 2; ++kind) {
+              u32 v[16];
+              read_sums(from + kind * 128 + c * 16, v);
+              sums_read();
+#pragma unroll
+              for (int q = 0; q < 16; ++q) {
+                // an infinity's small products are infinity times 0: the large one has the answer
+                const float f = __uint_as_float(v[q]);
+                total[c / 2][c % 2 * 16 + q] += kind == 0 || fabsf(f) <= 3.402823466e38f ? f : 0.f;
+              }
             }
           }
           sums_fence_before();
@@ -284,13 +612,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_tiles(const __grid_constant
         }
         if (lost) break;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) store(c * 32, total[c]);
+        for (int c = 0; c < 2; ++c) store(c * 32, total[c]);
       }
     }
     if (!GRAD) {  // rows of no expert
-      const i64 at = (i64)blockIdx.x * 128 + (threadIdx.x - 128), by = (i64)gridDim.x * 128;
+      const i64 at = (i64)blockIdx.x * (32 * kWriters) + (threadIdx.x - 128), by = (i64)gridDim.x * (32 * kWriters);
       auto clear = [&](i64 from, i64 to) {
-        if (whole) {
+        if (unit == 16) {
           constexpr int N = 16 / sizeof(T);
           for (i64 i = from / N + at; i < to / N; i += by) ((uint4*)out)[i] = make_uint4(0, 0, 0, 0);
         } else {
@@ -340,18 +668,20 @@ __global__ void __launch_bounds__(32 * kMapWarps) k_expert_maps(const __grid_con
 }
 
 // out[e] = the sum of the chunks of expert e, in their order.
+constexpr int kAddThreads = 256;
 template <class T>
-__global__ void __launch_bounds__(kTileThreads) k_add_chunks(const Groups g, u32 chunk, i64 values, const float* __restrict__ partial,
+__global__ void __launch_bounds__(kAddThreads) k_add_chunks(const Groups g, u32 chunk, i64 values, const float* __restrict__ partial,
                                                              T* __restrict__ out) {
   __shared__ PlanTable plan;
   await_previous();
-  make_plan<kTileThreads>(plan, g, chunk, 1);
-  const i64 step = (i64)gridDim.x * kTileThreads;
-  for (i64 i = (i64)blockIdx.x * kTileThreads + threadIdx.x; i < values * g.experts; i += step) {
+  make_plan<kAddThreads>(plan, g, chunk, 1);
+  const i64 step = (i64)gridDim.x * kAddThreads;
+  for (i64 i = (i64)blockIdx.x * kAddThreads + threadIdx.x; i < values * g.experts; i += step) {
     const int e = (int)(i / values);
     const i64 at = i - e * values;
     float sum = 0.f;
-    for (u32 c = plan.tile[e]; c < plan.tile[e + 1]; ++c) sum += partial[c * values + at];
+#pragma unroll 8
+    for (u32 c = plan.tile[e]; c < plan.tile[e + 1]; ++c) sum += __ldcs(partial + c * values + at);
     out[(i64)g.first * values + i] = from_float<T>(sum);
   }
 }
@@ -375,14 +705,8 @@ __global__ void __launch_bounds__(256) k_into_lines(const T* __restrict__ from, 
         v[0][q] = x + q < width ? ((const unsigned short*)row)[x + q] : (unsigned short)0;
       } else {
         float rest = x + q < width ? row[x + q] : 0.f;
-        const bool finite = fabsf(rest) <= 3.402823466e38f;
 #pragma unroll
-        for (int p = 0; p < PARTS; ++p) {
-          // to nearest, but the largest numbers downwards, where that would be infinity.  Infinities and NaN are all in the first part
-          const __nv_bfloat16 part = finite && fabsf(rest) > 3.38e38f ? __float2bfloat16_rz(rest) : __float2bfloat16_rn(rest);
-          v[p][q] = __bfloat16_as_ushort(part);
-          rest = finite ? rest - __bfloat162float(part) : 0.f;
-        }
+        for (int p = 0; p < PARTS; ++p) v[p][q] = (unsigned short)next_part(rest);
       }
     }
 #pragma unroll
@@ -470,17 +794,17 @@ static int by_experts(gsb_ctx* ctx, i64 num_experts, i64 num_rows, const int64_t
 // Launches pairs of CTAs: at most one CTA per SM.  In the order of the stream, with no overlap of its neighbours' ends and beginnings: with
 // overlap, hundreds of copies and products queued one behind the other came to a halt, waiting CTAs of one kernel beside clusters of another
 // that need SMs as a whole.
-template <class T, bool WHOLE_NUMBERS, int PARTS, bool GRAD, bool ACROSS>
+template <class T, bool WHOLE_NUMBERS, int PARTS, bool GRAD, bool ACROSS, bool READ>
 static int launch_tiles(gsb_ctx* ctx, cudaStream_t stream, const CUtensorMap& map_a, const CUtensorMap& map_b, TileArgs a, i64 most_tiles, T* out) {
-  auto kernel = k_tiles<T, WHOLE_NUMBERS, PARTS, GRAD, ACROSS>;
+  auto kernel = k_tiles<T, WHOLE_NUMBERS, PARTS, GRAD, ACROSS, READ>;
   const int stage = PARTS * (kRowsOperand + (int)a.columns / 2 * kLineBytes);
   a.stages = min(kMaxStages, 200 * 1024 / stage);
   a.how = instruction(WHOLE_NUMBERS ? OPERAND_S8 : std::is_same<T, __half>::value ? OPERAND_F16 : OPERAND_BF16, GRAD, GRAD || ACROSS, kPairRows, a.columns);
-  const int smem = a.stages * stage + 1024;
+  const int smem = a.stages * stage + 1024 + ring_bytes(PARTS);
   GSB_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(2 * max((i64)1, min((i64)kNumSMs / 2, most_tiles))));
-  cfg.blockDim = dim3(kTileThreads);
+  cfg.blockDim = dim3(tile_threads(READ));
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr;
@@ -516,11 +840,21 @@ static i64 chunk_rows(i64 num_rows, i64 k, i64 n, u32 columns, i64 num_experts) 
 }
 static i64 most_chunks(i64 num_rows, i64 chunk, i64 num_experts) { return min(num_experts, (i64)kPlanExperts) + num_rows / max((i64)1, chunk); }
 
+// Calls f(T, PARTS, READ).
 template <class F>
-static int with_type(int dtype, F f) {
-  if (dtype == GSB_F32) return f(float{}, std::integral_constant<int, 3>{});
-  if (dtype == GSB_F16) return f(__half{}, std::integral_constant<int, 1>{});
-  return f(__nv_bfloat16{}, std::integral_constant<int, 1>{});
+static int with_type(int dtype, bool read, F f) {
+  using std::integral_constant;
+  using Yes = integral_constant<bool, true>;
+  using No = integral_constant<bool, false>;
+  if (dtype == GSB_F32) return f(float{}, integral_constant<int, 3>{}, Yes{});
+  if (dtype == GSB_F16) return read ? f(__half{}, integral_constant<int, 1>{}, Yes{}) : f(__half{}, integral_constant<int, 1>{}, No{});
+  return read ? f(__nv_bfloat16{}, integral_constant<int, 1>{}, Yes{}) : f(__nv_bfloat16{}, integral_constant<int, 1>{}, No{});
+}
+// Rows for the warps that read them.
+static RawRows raw_rows(const Lines& x) {
+  const int size = value_bytes(x.dtype);
+  const i64 stride = x.height > 1 ? x.stride : 0;
+  return RawRows{x.at, stride, (u32)x.width, unit_bytes(16, (u64)(uintptr_t)x.at | (u64)(stride * size))};
 }
 
 }  // namespace gsb
@@ -533,8 +867,7 @@ extern "C" int64_t gsb_expert_product_workspace(const void* rows, int dtype, int
   if (value_bytes(dtype) == 0 || num_rows < 0 || num_rows >= ((i64)1 << 31) || k < 1 || k > GSB_MAX_ROW_LEN || n < 1 || n > GSB_MAX_ROW_LEN ||
       num_experts < 1 || num_experts > GSB_MAX_EXPERTS)
     return GSB_ERR_INVALID_ARGUMENT;
-  return rows_operand(rows, dtype, num_rows, k, rows_stride).bytes() +
-         matrices_operand(weights, dtype, num_experts, weights_expert_stride, k, weights_k_stride, n, weights_n_stride).bytes();
+  return matrices_operand(weights, dtype, num_experts, weights_expert_stride, k, weights_k_stride, n, weights_n_stride).bytes();
 }
 
 extern "C" int gsb_expert_product(gsb_ctx* ctx, void* stream_, const void* rows, int dtype, int64_t num_rows, int64_t k, int64_t rows_stride,
@@ -557,22 +890,26 @@ extern "C" int gsb_expert_product(gsb_ctx* ctx, void* stream_, const void* rows,
   Lines x = rows_operand(rows, dtype, num_rows, k, rows_stride);
   Lines w = matrices_operand(weights, dtype, num_experts, weights_expert_stride, k, weights_k_stride, n, weights_n_stride);
   char* room = (char*)workspace;
-  if ((st = bring(ctx, stream, &x, &room)) != GSB_OK || (st = bring(ctx, stream, &w, &room)) != GSB_OK) return st;
+  if ((st = bring(ctx, stream, &w, &room)) != GSB_OK) return st;
   TileArgs a = {};
+  a.rows = raw_rows(x);
   a.depth = (u32)k;
   a.n = (u32)n;
   a.columns = tile_columns(n, dtype);
   a.expert_step = w.copies() > 1;
-  CUtensorMap map_x, map_w;
-  if ((st = describe(x, 2, 64, 128, false, &map_x)) != GSB_OK || (st = describe(w, 2, 64, across ? 64 : a.columns / 2, true, &map_w)) != GSB_OK) return st;
+  CUtensorMap map_x = {}, map_w;
+  const bool read = x.copied();
+  if (!read && (st = describe(x, 2, 64, 128, false, &map_x)) != GSB_OK) return st;
+  if ((st = describe(w, 2, 64, across ? 64 : a.columns / 2, true, &map_w)) != GSB_OK) return st;
   return by_experts(ctx, num_experts, num_rows, offsets, [&](const Groups& g) {
     a.groups = g;
     const i64 tiles = (num_rows / kPairRows + g.experts) * ((n + a.columns - 1) / a.columns);
-    return with_type(dtype, [&](auto value, auto parts) {
+    return with_type(dtype, read, [&](auto value, auto parts, auto reading) {
       typedef decltype(value) T;
       constexpr int P = decltype(parts)::value;
-      if (across) return launch_tiles<T, false, P, false, true>(ctx, stream, map_x, map_w, a, tiles, (T*)out);
-      return launch_tiles<T, false, P, false, false>(ctx, stream, map_x, map_w, a, tiles, (T*)out);
+      constexpr bool R = decltype(reading)::value;
+      if (across) return launch_tiles<T, false, P, false, true, R>(ctx, stream, map_x, map_w, a, tiles, (T*)out);
+      return launch_tiles<T, false, P, false, false, R>(ctx, stream, map_x, map_w, a, tiles, (T*)out);
     });
   });
 }
@@ -583,8 +920,7 @@ extern "C" int64_t gsb_expert_product_grad_workspace(const void* rows, int dtype
       num_experts < 1 || num_experts > GSB_MAX_EXPERTS)
     return GSB_ERR_INVALID_ARGUMENT;
   const i64 chunk = chunk_rows(num_rows, k, n, tile_columns(n, dtype), num_experts);
-  return rounded(min(num_experts, (i64)kPlanExperts) * 2 * (i64)sizeof(CUtensorMap)) + rows_operand(rows, dtype, num_rows, k, rows_stride).bytes() +
-         rows_operand(grad, dtype, num_rows, n, grad_stride).bytes() + (chunk < num_rows ? rounded(most_chunks(num_rows, chunk, num_experts) * k * n * 4) : 0);
+  return rounded(min(num_experts, (i64)kPlanExperts) * 2 * (i64)sizeof(CUtensorMap)) + (chunk < num_rows ? rounded(most_chunks(num_rows, chunk, num_experts) * k * n * 4) : 0);
 }
 
 extern "C" int gsb_expert_product_grad(gsb_ctx* ctx, void* stream_, const void* rows, int dtype, int64_t num_rows, int64_t k, int64_t rows_stride,
@@ -608,8 +944,9 @@ extern "C" int gsb_expert_product_grad(gsb_ctx* ctx, void* stream_, const void* 
   CUtensorMap* maps = (CUtensorMap*)room;
   room += rounded(min(num_experts, (i64)kPlanExperts) * 2 * (i64)sizeof(CUtensorMap));
   Lines x = rows_operand(rows, dtype, num_rows, k, rows_stride), d = rows_operand(grad, dtype, num_rows, n, grad_stride);
-  if ((st = bring(ctx, stream, &x, &room)) != GSB_OK || (st = bring(ctx, stream, &d, &room)) != GSB_OK) return st;
   TileArgs a = {};
+  a.rows = raw_rows(x);
+  a.grad = raw_rows(d);
   a.k = (u32)k;
   a.n = (u32)n;
   a.columns = tile_columns(n, dtype);
@@ -617,23 +954,24 @@ extern "C" int gsb_expert_product_grad(gsb_ctx* ctx, void* stream_, const void* 
   a.chunk = (u32)chunk;
   a.maps = maps;
   a.partial = chunk < num_rows ? (float*)room : nullptr;
-  CUtensorMap map_x, map_d;
-  if ((st = describe(x, 2, 64, 64, false, &map_x)) != GSB_OK || (st = describe(d, 2, 64, 64, false, &map_d)) != GSB_OK) return st;
+  CUtensorMap map_x = {}, map_d = {};
+  const bool read = x.copied() || d.copied();
+  if (!read && ((st = describe(x, 2, 64, 64, false, &map_x)) != GSB_OK || (st = describe(d, 2, 64, 64, false, &map_d)) != GSB_OK)) return st;
   return by_experts(ctx, num_experts, num_rows, offsets, [&](const Groups& g) -> int {
     a.groups = g;
-    {
+    if (!read) {
       ScopedKernelTimer timer(ctx, KID_EXPERT_PRODUCT, stream);
       launch_behind(stream, k_expert_maps, grid_for(2 * g.experts, kMapWarps), 32 * kMapWarps, map_x, map_d, g, (const char*)x.at, x.height > 1 ? x.stride * 2 : 0, (const char*)d.at,
                     d.height > 1 ? d.stride * 2 : 0, maps);
       GSB_LAUNCH_OK();
     }
     const i64 tiles = (num_rows / chunk + g.experts) * ((k + kPairRows - 1) / kPairRows) * ((n + a.columns - 1) / a.columns);
-    return with_type(dtype, [&](auto value, auto parts) -> int {
+    return with_type(dtype, read, [&](auto value, auto parts, auto reading) -> int {
       typedef decltype(value) T;
-      const int launched = launch_tiles<T, false, decltype(parts)::value, true, true>(ctx, stream, map_x, map_d, a, tiles, (T*)out);
+      const int launched = launch_tiles<T, false, decltype(parts)::value, true, true, decltype(reading)::value>(ctx, stream, map_x, map_d, a, tiles, (T*)out);
       if (launched != GSB_OK || !a.partial) return launched;
       ScopedKernelTimer timer(ctx, KID_EXPERT_PRODUCT, stream);
-      launch_behind(stream, k_add_chunks<T>, (int)min((i64)kNumSMs * 8, (i64)grid_for(k * n * g.experts, kTileThreads)), kTileThreads, g, a.chunk, k * n,
+      launch_behind(stream, k_add_chunks<T>, (int)min((i64)kNumSMs * 8, (i64)grid_for(k * n * g.experts, kAddThreads)), kAddThreads, g, a.chunk, k * n,
                     (const float*)a.partial, (T*)out);
       GSB_LAUNCH_OK();
       return GSB_OK;
@@ -671,6 +1009,8 @@ extern "C" int gsb_expert_product_int8(gsb_ctx* ctx, void* stream_, const int8_t
   return by_experts(ctx, num_experts, num_rows, offsets, [&](const Groups& g) {
     a.groups = g;
     const i64 tiles = (num_rows / kPairRows + g.experts) * ((n + a.columns - 1) / a.columns);
-    return with_type(out_dtype, [&](auto value, auto) { return launch_tiles<decltype(value), true, 1, false, false>(ctx, stream, map_x, map_w, a, tiles, (decltype(value)*)out); });
+    if (out_dtype == GSB_F32) return launch_tiles<float, true, 1, false, false, false>(ctx, stream, map_x, map_w, a, tiles, (float*)out);
+    if (out_dtype == GSB_F16) return launch_tiles<__half, true, 1, false, false, false>(ctx, stream, map_x, map_w, a, tiles, (__half*)out);
+    return launch_tiles<__nv_bfloat16, true, 1, false, false, false>(ctx, stream, map_x, map_w, a, tiles, (__nv_bfloat16*)out);
   });
 }

@@ -36,6 +36,7 @@ __device__ __forceinline__ void barriers_ready() { asm volatile("fence.mbarrier_
 __device__ __forceinline__ void barrier_expect(u32 bar, u32 bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ void barrier_arrive(u32 bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ void barrier_arrive_at(u32 cluster_bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
@@ -48,6 +49,9 @@ __device__ __forceinline__ bool barrier_try(u32 bar, u32 parity) {
       : "memory");
   return done != 0;
 }
+
+// What was written to shared memory before is seen by matrix instructions that are issued behind a barrier this thread arrives at next.
+__device__ __forceinline__ void written_for_tensor_cores() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // A wait that lasts for two seconds is given up: the CTA notes it in `stop`, its other waits end too, and the error is recorded.
 constexpr u64 kWaitLimit = 2000000000ull;
@@ -126,7 +130,13 @@ __device__ __forceinline__ void multiplied(u32 bar) {
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((unsigned short)3)
                : "memory");
 }
-// 32 columns of sums, of the row that the lane stands for.
+// 16 or 32 columns of sums, of the row that the lane stands for.
+__device__ __forceinline__ void read_sums(u32 at, u32 (&v)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
+                 "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+               : "r"(at));
+}
 __device__ __forceinline__ void read_sums(u32 at, u32 (&v)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, "
