@@ -47,6 +47,7 @@ struct TileArgs {
   int expert_step;           // 0: one matrix for all experts
   const CUtensorMap* maps;   // gradient: each expert's rows and gradient rows
   RawRows rows, grad;        // where they are read by warps
+  bool by_tma;               // results may leave by TMA
   float* partial;            // gradient: sums of the chunks (null: one chunk per expert, written out)
   const float *row_scales, *weight_scales;  // of 8-bit operands
   u32 how;
@@ -81,9 +82,9 @@ __device__ __forceinline__ Tile tile_at(const TileArgs& a, const PlanTable& plan
   return r;
 }
 
-// 64 bytes of each of 32 rows of the result, a row a lane, brought through shared memory so that neighbouring lanes write neighbours: the
-// rows go to `to`, `pitch` bytes apart, `bytes` of each, in accesses of `unit` bytes, which divide them.
-constexpr int kStoreBytes = 64;
+// 64 bytes of each of 32 rows of the result, a row a lane, leave through shared memory: by TMA where all 32 rows are wanted and begin on 16-byte
+// boundaries, else copied by neighbouring lanes, to `to`, `pitch` bytes apart, `bytes` of each, in accesses of `unit` bytes, which divide them.
+constexpr int kStoreBytes = 64, kRoom = 32 * kStoreBytes;
 template <class Word>
 __device__ __forceinline__ void copy_rows_by(const char* room, int lane, char* to, i64 pitch, u32 rows, u32 bytes) {
   constexpr int W = sizeof(Word), LANES = kStoreBytes / W;  // of a row
@@ -101,9 +102,19 @@ static __device__ __noinline__ void copy_rows(const char* room, int lane, char* 
   else copy_rows_by<unsigned short>(room, lane, to, pitch, rows, bytes);
   __syncwarp();
 }
+// A warp's way out: two rooms, taken in turn.
+struct Exit {
+  char* rooms;
+  u32 turn;
+};
 template <class U>
-__device__ __forceinline__ void write_rows(char* room, int lane, const float (&v)[kStoreBytes / sizeof(U)], U* to, i64 pitch, u32 rows, u32 columns, int unit) {
+__device__ __forceinline__ void write_rows(Exit& exit, int lane, const float (&v)[kStoreBytes / sizeof(U)], U* to, i64 pitch, u32 rows, u32 columns, int unit,
+                                           const CUtensorMap* map, i64 row, u32 column) {
   constexpr int PER = 16 / sizeof(U);
+  char* const room = exit.rooms + (exit.turn & 1) * kRoom;
+  ++exit.turn;
+  if (lane == 0) stores_read<1>();
+  __syncwarp();
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
     float f[PER];
@@ -113,7 +124,14 @@ __device__ __forceinline__ void write_rows(char* room, int lane, const float (&v
     w.set(f);
     *(uint4*)(room + lane * kStoreBytes + ((p ^ (lane >> 1 & 3)) << 4)) = w.w;
   }
-  copy_rows(room, lane, (char*)to, pitch * (i64)sizeof(U), rows, columns * (u32)sizeof(U), unit);
+  if (map && rows == 32) {
+    written_for_tensor_cores();
+    __syncwarp();
+    if (lane == 0) store_tile(map, smem_address(room), (int)column, (int)row);
+  } else {
+    copy_rows(room, lane, (char*)to, pitch * (i64)sizeof(U), rows, columns * (u32)sizeof(U), unit);
+    if (lane == 0) asm volatile("cp.async.bulk.commit_group;" ::: "memory");  // an empty turn
+  }
 }
 
 // ---- rows read by warps: rows of any address and distance, and float32, which is taken apart on the way ----------------------------
@@ -149,21 +167,15 @@ __device__ __forceinline__ void write_line(u32 to, const u32 (&w)[4]) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
 }
 
-// float32: a piece is 8 neighbouring values of a row, copied behind the thread's back into a place of its own in shared memory, in two
-// halves `kRing` bytes apart.  `valid`: how many of them there are; `some`: an address in the array, for pieces without any.
-constexpr int kRing = 32 * kReaders * 16;
-__device__ __forceinline__ void copy_piece(u32 to, const float* from, int valid, bool aligned, const void* some) {
-  if (valid <= 0 || (valid >= 8 && aligned)) {
-    const u32 bytes = valid > 0 ? 16 : 0;
-    const float* at = valid > 0 ? from : (const float*)some;
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(at), "r"(bytes) : "memory");
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + kRing), "l"(at + bytes / 4), "r"(bytes) : "memory");
+// float32: 4 neighbouring values of a row, copied behind the thread's back.  `valid`: how many of them there are; `some`: an address in the
+// array, where there are none.
+__device__ __forceinline__ void copy_four(u32 to, const float* from, int valid, bool aligned, const void* some) {
+  if (valid <= 0 || (valid >= 4 && aligned)) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(valid > 0 ? from : (const float*)some), "r"(valid > 0 ? 16 : 0) : "memory");
   } else {
 #pragma unroll
-    for (int q = 0; q < 8; ++q)
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + q / 4 * kRing + q % 4 * 4), "l"(q < valid ? from + q : from),
-                   "r"(q < valid ? 4 : 0)
-                   : "memory");
+    for (int q = 0; q < 4; ++q)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + q * 4), "l"(q < valid ? from + q : from), "r"(q < valid ? 4 : 0) : "memory");
   }
 }
 __device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -186,14 +198,18 @@ __device__ __forceinline__ u32 next_parts(float& low, float& high) {
   high -= __uint_as_float(w & 0xffff0000u);
   return w;
 }
-// Two copied pieces to their places, 32 lines apart, every part in an operand of its own, `apart` bytes from the one before.
+// A warp's room for float32 values on their way: 8 lines of 64 values, in steps of 4 lines.  A step holds the first four of each 8
+// values (512 bytes), then the other four, so that a lane reads its 8 values, and all lanes theirs, without meeting in a bank.
+constexpr int kStepBytes = 4 * 64 * 4, kPairBytes = 2 * kStepBytes;
+// 8 values of each of two lines to their places, 32 lines apart, every part in an operand of its own, `apart` bytes from the one before.
+// `ring`: of this lane's first 16 bytes.  All of the warp's values have been read when it returns.
 __device__ __forceinline__ void write_parts(u32 ring, u32 to, u32 apart) {
   float rest[2][8];
 #pragma unroll
   for (int h = 0; h < 4; ++h)
     asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
                  : "=f"(rest[h / 2][h % 2 * 4]), "=f"(rest[h / 2][h % 2 * 4 + 1]), "=f"(rest[h / 2][h % 2 * 4 + 2]), "=f"(rest[h / 2][h % 2 * 4 + 3])
-                 : "r"(ring + h * kRing)
+                 : "r"(ring + h * 512)
                  : "memory");
   u32 w[2][4];
 #pragma unroll
@@ -215,13 +231,14 @@ __device__ __forceinline__ void write_parts(u32 ring, u32 to, u32 apart) {
 #pragma unroll 1
     for (int h = 0; h < 8; ++h) {
       float two[2];
-      asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(two[0]), "=f"(two[1]) : "r"(ring + h / 2 * kRing + h % 2 * 8) : "memory");
+      asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(two[0]), "=f"(two[1]) : "r"(ring + h / 2 * 512 + h % 2 * 8) : "memory");
       for (int p = 0; p < 3; ++p) {
         const u32 low = next_part(two[0]);
         asm volatile("st.shared.b32 [%0], %1;" ::"r"(to + p * apart + h / 4 * 32 * kLineBytes + h % 4 * 4), "r"(low | next_part(two[1]) << 16) : "memory");
       }
     }
   }
+  __syncwarp();
 }
 
 // The lines of the reduced index that a pair of CTAs goes through, tile by tile.
@@ -241,15 +258,15 @@ struct Walk {
   }
 };
 
-// float32 pieces that a reader has on their way: three times two.
-constexpr int kPairsAhead = 3;
-constexpr int ring_bytes(int parts) { return parts == 3 ? kPairsAhead * 4 * kRing : 0; }
+// float32 values that a reading warp has on their way: twice 8 lines.
+constexpr int kPairsAhead = 2;
+constexpr int ring_bytes(int parts) { return parts == 3 ? kReaders * kPairsAhead * kPairBytes : 0; }
 
 // PARTS: 3 for float32, else 1.  ACROSS: the second operand's lines hold the reduced index across them (a gradient's both do).  READ: rows
 // (and a gradient's both operands) are read by warps, not by TMA.
 template <class T, bool WHOLE_NUMBERS, int PARTS, bool GRAD, bool ACROSS, bool READ>
 __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                                                                 const TileArgs a, T* __restrict__ out) {
+                                                                 const __grid_constant__ CUtensorMap map_out, const TileArgs a, T* __restrict__ out) {
   constexpr int kPerLine = kLineBytes / (WHOLE_NUMBERS ? 1 : 2);
   // float32: sums leave tensor memory, where additions cut, after this many lines of the reduced index, and are added up in registers.
   // Over 16 instructions that is an error of 2.3e-7 of the sums (rms), over 32 4.7e-7
@@ -258,7 +275,7 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
   __shared__ PlanTable plan;
   __shared__ __align__(8) u64 bars[3 * kMaxStages + 4];
   __shared__ float column_scales[WHOLE_NUMBERS ? kWriters : 1][128];
-  __shared__ __align__(16) char rooms[kWriters][32 * kStoreBytes];
+  __shared__ __align__(1024) char rooms[kWriters][2 * kRoom];
   __shared__ u32 sums_at;
   __shared__ volatile int stop;
   const u32 stages_at = (smem_address(raw) + 1023u) & ~1023u;
@@ -394,40 +411,58 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
     auto first_row = [&](const Tile& tile) { return GRAD ? (i64)plan.begin[tile.e] + tile.row0 : (i64)tile.row0 + rank * 128; };
     auto rows_here = [&](const Tile& tile) { return GRAD ? (int)tile.rows : (int)tile.rows - (int)rank * 128; };
     if constexpr (PARTS == 3) {
-      // a thread has the 16 bytes `chunk` of lines segment, segment + 32 and so on of a stage; two lines at a time
+      // A warp has lines 4 w to 4 w + 3 and those 32, 64 and 96 behind them, 8 at a time.  A lane copies four values of two lines each time
+      // (16 lanes to a line), and takes apart 8 values of one line
       constexpr int kPairs = GRAD ? 3 : 2;
-      const u32 chunk = me & 7, segment = me / 8, place = segment * kLineBytes + ((chunk ^ (segment & 7)) << 4);
-      const u32 ring = stages_at + a.stages * stage_bytes + me * 16;
+      const u32 w = me / 32, chunk = lane & 7, segment = w * 4 + lane / 8, place = segment * kLineBytes + ((chunk ^ (segment & 7)) << 4);
+      const u32 ring = stages_at + a.stages * stage_bytes + w * kPairsAhead * kPairBytes;
+      const u32 copies_to = ring + (lane & 1) * 512 + (lane / 16 * 8 + (lane & 15) / 2) * 16;  // of the first of two lines; the next two are 256 bytes on
+      const int copied_line = (int)w * 4 + lane / 16, copied_column = (lane & 15) * 4;
       const bool aligned = a.rows.unit == 16, grad_aligned = a.grad.unit == 16;
+      const bool simple = aligned && a.rows.width % 4 == 0, grad_simple = grad_aligned && a.grad.width % 4 == 0;
       Walk<GRAD, kPerLine> ahead = now;
       const float *from = nullptr, *from_grad = nullptr;
       int columns = 0, grad_columns = 0, rows_left = 0, pair = 0;  // from this thread's first on
       auto begin_tile = [&] {
         if (ahead.t >= tiles) return;
         const Tile& tile = ahead.tile;
-        const u32 c = (GRAD ? tile.m0 + rank * 128 : 0) + chunk * 8;
-        from = (const float*)a.rows.at + (first_row(tile) + segment) * a.rows.stride + c;
+        const u32 c = (GRAD ? tile.m0 + rank * 128 : 0) + copied_column;
+        from = (const float*)a.rows.at + (first_row(tile) + copied_line) * a.rows.stride + c;
         columns = (int)a.rows.width - (int)c;
-        rows_left = rows_here(tile) - (int)segment;
+        rows_left = rows_here(tile) - copied_line;
         if (GRAD) {
-          const u32 d = tile.n0 + rank * half + chunk * 8;
-          from_grad = (const float*)a.grad.at + (first_row(tile) + segment) * a.grad.stride + d;
+          const u32 d = tile.n0 + rank * half + copied_column;
+          from_grad = (const float*)a.grad.at + (first_row(tile) + copied_line) * a.grad.stride + d;
           grad_columns = (int)a.grad.width - (int)d;
         }
       };
       begin_tile();
+      auto copy_pair = [&](u32 to, const float* at, i64 stride, int rows, int width, bool simple, bool wide, const void* some) {
+        if (simple) {  // four values or none
+          if (width <= 0) rows = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int line = (i >> 1) * 32 + (i & 1) * 2;
+            const bool in = rows > line;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + (i >> 1) * kStepBytes + (i & 1) * 256), "l"(in ? at : (const float*)some),
+                         "r"(in ? 16 : 0)
+                         : "memory");
+            at += (i & 1 ? 30 : 2) * stride;
+          }
+        } else {
+#pragma unroll 1
+          for (int i = 0; i < 4; ++i) {
+            const int line = (i >> 1) * 32 + (i & 1) * 2;
+            copy_four(to + (i >> 1) * kStepBytes + (i & 1) * 256, at + line * stride, rows > line ? width : 0, wide, some);
+          }
+        }
+      };
       auto copy = [&](u32 slot) {
         if (ahead.t < tiles) {
-          const u32 to = ring + slot * 4 * kRing;
-          if (GRAD && pair == 2) {
-            copy_piece(to, from_grad, rows_left > 0 ? grad_columns : 0, grad_aligned, a.grad.at);
-            copy_piece(to + 2 * kRing, from_grad + 32 * a.grad.stride, rows_left > 32 ? grad_columns : 0, grad_aligned, a.grad.at);
-          } else {
-            const float* at = from + (GRAD ? (i64)pair * 64 : pair * 64 * a.rows.stride);
-            const int rows = rows_left - (GRAD ? 0 : pair * 64), width = columns - (GRAD ? pair * 64 : 0);
-            copy_piece(to, at, rows > 0 ? width : 0, aligned, a.rows.at);
-            copy_piece(to + 2 * kRing, at + 32 * a.rows.stride, rows > 32 ? width : 0, aligned, a.rows.at);
-          }
+          const u32 to = copies_to + slot * kPairBytes;
+          if (GRAD && pair == 2) copy_pair(to, from_grad, a.grad.stride, rows_left, grad_columns, grad_simple, grad_aligned, a.grad.at);
+          else if (GRAD) copy_pair(to, from + pair * 64, a.rows.stride, rows_left, columns - pair * 64, simple, aligned, a.rows.at);
+          else copy_pair(to, from + pair * 64 * a.rows.stride, a.rows.stride, rows_left - pair * 64, columns, simple, aligned, a.rows.at);
           if (++pair == kPairs) {
             pair = 0;
             from += GRAD ? 64 * a.rows.stride : 64;
@@ -448,8 +483,9 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
 #pragma unroll
         for (int q = 0; q < kPairs; ++q) {
           copies_wait<kPairsAhead - 1>();
+          __syncwarp();
           const bool of_grad = GRAD && q == 2;
-          write_parts(ring + slot * 4 * kRing, at + (of_grad ? PARTS * kRowsOperand : q * 64 * kLineBytes), of_grad ? b_bytes : kRowsOperand);
+          write_parts(ring + lane * 16 + slot * kPairBytes, at + (of_grad ? PARTS * kRowsOperand : q * 64 * kLineBytes), of_grad ? b_bytes : kRowsOperand);
           copy(slot);
           if (++slot == kPairsAhead) slot = 0;
         }
@@ -516,7 +552,7 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
     const u32 c0 = (u32)(warp - 4) / 4 * half;                                     // this warp's half of the columns
     const u32 sums_empty_of_first = address_in(sums_empty, 0);
     const int unit = unit_of((u64)(uintptr_t)out | (u64)a.n * sizeof(T)), unit_partial = unit_of((u64)a.n * 4);
-    char* const room = rooms[warp - 4];
+    Exit exit{rooms[warp - 4], 0};
     u32 made = 0;
     for (u64 t = first; t < tiles; t += step) {
       const Tile tile = tile_at<GRAD, kPerLine>(a, plan, t);
@@ -524,8 +560,8 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
       const u32 valid_rows = limit > above ? min(32u, limit - above) : 0;
       const bool mine = (u32)lane < valid_rows;
       const u32 n0 = tile.n0 + c0;
-      const i64 at = GRAD ? ((i64)(a.partial ? (i64)tile.chunk : (i64)(g.first + tile.e)) * a.k + tile.m0 + above) * a.n + n0
-                          : (i64)(tile.row0 + above) * a.n + n0;
+      const i64 out_row = GRAD ? (i64)(a.partial ? (i64)tile.chunk : (i64)(g.first + tile.e)) * a.k + tile.m0 + above : (i64)tile.row0 + above;
+      const i64 at = out_row * a.n + n0;
       // 32 values of each row, in as many steps as they are 64 bytes
       auto store = [&](u32 c, const float(&v)[32]) {
         auto write = [&](auto* to, int width) {
@@ -537,7 +573,7 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
             float f[N];
 #pragma unroll
             for (int q = 0; q < N; ++q) f[q] = v[x + q];
-            write_rows(room, lane, f, to + at + c + x, a.n, valid_rows, a.n - n0 - c - x, width);
+            write_rows(exit, lane, f, to + at + c + x, a.n, valid_rows, a.n - n0 - c - x, width, a.by_tma ? &map_out : nullptr, out_row, n0 + c + x);
           }
         };
         if (GRAD && a.partial) write(a.partial, unit_partial);
@@ -563,6 +599,7 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
         sums_fence_after();
         for (u32 c = 0; c < half; c += 32) {
           u32 v[32];
+          __syncwarp();
           read_sums(sums + (quarter << 16) + buffer * 256 + c0 + c, v);
           sums_read();
           if (c + 32 == half) {
@@ -596,6 +633,7 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
 #pragma unroll
             for (int kind = 0; kind < 2; ++kind) {
               u32 v[16];
+              __syncwarp();
               read_sums(from + kind * 128 + c * 16, v);
               sums_read();
 #pragma unroll
@@ -615,6 +653,7 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
         for (int c = 0; c < 2; ++c) store(c * 32, total[c]);
       }
     }
+    if (lane == 0) stores_done();
     if (!GRAD) {  // rows of no expert
       const i64 at = (i64)blockIdx.x * (32 * kWriters) + (threadIdx.x - 128), by = (i64)gridDim.x * (32 * kWriters);
       auto clear = [&](i64 from, i64 to) {
@@ -635,9 +674,11 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
     while (nanoseconds() - since < 1000000) __nanosleep(1000);
   }
   __syncthreads();
+  __syncwarp();
   sums_fence_before();
   cluster_barrier();
   sums_fence_after();
+  __syncwarp();
   if (warp == 2) sums_free(sums, kSumColumns);
 }
 
@@ -791,16 +832,22 @@ static int by_experts(gsb_ctx* ctx, i64 num_experts, i64 num_rows, const int64_t
   return GSB_OK;
 }
 
+// Shared memory for stages and the readers' copies: what the fixed part (the plan, the ways out) leaves.
+constexpr int kStagesRoom = (227 - 46) * 1024 - 1024;
 // Launches pairs of CTAs: at most one CTA per SM.  In the order of the stream, with no overlap of its neighbours' ends and beginnings: with
 // overlap, hundreds of copies and products queued one behind the other came to a halt, waiting CTAs of one kernel beside clusters of another
 // that need SMs as a whole.
 template <class T, bool WHOLE_NUMBERS, int PARTS, bool GRAD, bool ACROSS, bool READ>
-static int launch_tiles(gsb_ctx* ctx, cudaStream_t stream, const CUtensorMap& map_a, const CUtensorMap& map_b, TileArgs a, i64 most_tiles, T* out) {
+static int launch_tiles(gsb_ctx* ctx, cudaStream_t stream, const CUtensorMap& map_a, const CUtensorMap& map_b, TileArgs a, i64 most_tiles, i64 out_rows, T* out) {
   auto kernel = k_tiles<T, WHOLE_NUMBERS, PARTS, GRAD, ACROSS, READ>;
   const int stage = PARTS * (kRowsOperand + (int)a.columns / 2 * kLineBytes);
-  a.stages = min(kMaxStages, 200 * 1024 / stage);
+  a.stages = min(kMaxStages, (kStagesRoom - ring_bytes(PARTS)) / stage);
   a.how = instruction(WHOLE_NUMBERS ? OPERAND_S8 : std::is_same<T, __half>::value ? OPERAND_F16 : OPERAND_BF16, GRAD, GRAD || ACROSS, kPairRows, a.columns);
   const int smem = a.stages * stage + 1024 + ring_bytes(PARTS);
+  CUtensorMap map_out = {};
+  const int size = a.partial ? 4 : (int)sizeof(T);
+  void* const results = a.partial ? (void*)a.partial : (void*)out;
+  a.by_tma = (i64)a.n * size % 16 == 0 && aligned_to(16, (const char*)results) && out_rows < ((i64)1 << 31) && describe_rows(&map_out, results, size, a.n, (u64)out_rows);
   GSB_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(2 * max((i64)1, min((i64)kNumSMs / 2, most_tiles))));
@@ -814,7 +861,7 @@ static int launch_tiles(gsb_ctx* ctx, cudaStream_t stream, const CUtensorMap& ma
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   ScopedKernelTimer timer(ctx, KID_EXPERT_PRODUCT, stream);
-  GSB_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, map_a, map_b, a, out));
+  GSB_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, map_a, map_b, map_out, a, out));
   return GSB_OK;
 }
 
@@ -908,8 +955,8 @@ extern "C" int gsb_expert_product(gsb_ctx* ctx, void* stream_, const void* rows,
       typedef decltype(value) T;
       constexpr int P = decltype(parts)::value;
       constexpr bool R = decltype(reading)::value;
-      if (across) return launch_tiles<T, false, P, false, true, R>(ctx, stream, map_x, map_w, a, tiles, (T*)out);
-      return launch_tiles<T, false, P, false, false, R>(ctx, stream, map_x, map_w, a, tiles, (T*)out);
+      if (across) return launch_tiles<T, false, P, false, true, R>(ctx, stream, map_x, map_w, a, tiles, num_rows, (T*)out);
+      return launch_tiles<T, false, P, false, false, R>(ctx, stream, map_x, map_w, a, tiles, num_rows, (T*)out);
     });
   });
 }
@@ -968,7 +1015,7 @@ extern "C" int gsb_expert_product_grad(gsb_ctx* ctx, void* stream_, const void* 
     const i64 tiles = (num_rows / chunk + g.experts) * ((k + kPairRows - 1) / kPairRows) * ((n + a.columns - 1) / a.columns);
     return with_type(dtype, read, [&](auto value, auto parts, auto reading) -> int {
       typedef decltype(value) T;
-      const int launched = launch_tiles<T, false, decltype(parts)::value, true, true, decltype(reading)::value>(ctx, stream, map_x, map_d, a, tiles, (T*)out);
+      const int launched = launch_tiles<T, false, decltype(parts)::value, true, true, decltype(reading)::value>(ctx, stream, map_x, map_d, a, tiles, (a.partial ? num_rows / chunk + g.experts : num_experts) * k, (T*)out);
       if (launched != GSB_OK || !a.partial) return launched;
       ScopedKernelTimer timer(ctx, KID_EXPERT_PRODUCT, stream);
       launch_behind(stream, k_add_chunks<T>, (int)min((i64)kNumSMs * 8, (i64)grid_for(k * n * g.experts, kAddThreads)), kAddThreads, g, a.chunk, k * n,
@@ -1009,8 +1056,8 @@ extern "C" int gsb_expert_product_int8(gsb_ctx* ctx, void* stream_, const int8_t
   return by_experts(ctx, num_experts, num_rows, offsets, [&](const Groups& g) {
     a.groups = g;
     const i64 tiles = (num_rows / kPairRows + g.experts) * ((n + a.columns - 1) / a.columns);
-    if (out_dtype == GSB_F32) return launch_tiles<float, true, 1, false, false, false>(ctx, stream, map_x, map_w, a, tiles, (float*)out);
-    if (out_dtype == GSB_F16) return launch_tiles<__half, true, 1, false, false, false>(ctx, stream, map_x, map_w, a, tiles, (__half*)out);
-    return launch_tiles<__nv_bfloat16, true, 1, false, false, false>(ctx, stream, map_x, map_w, a, tiles, (__nv_bfloat16*)out);
+    if (out_dtype == GSB_F32) return launch_tiles<float, true, 1, false, false, false>(ctx, stream, map_x, map_w, a, tiles, num_rows, (float*)out);
+    if (out_dtype == GSB_F16) return launch_tiles<__half, true, 1, false, false, false>(ctx, stream, map_x, map_w, a, tiles, num_rows, (__half*)out);
+    return launch_tiles<__nv_bfloat16, true, 1, false, false, false>(ctx, stream, map_x, map_w, a, tiles, num_rows, (__nv_bfloat16*)out);
   });
 }

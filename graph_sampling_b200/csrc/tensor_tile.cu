@@ -34,4 +34,13 @@ bool describe_array(CUtensorMap* map, const void* base, int value_bytes, int ran
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool describe_rows(CUtensorMap* map, void* base, int value_bytes, u64 width, u64 rows) {
+  const EncodeTiled encode = encode_tiled();
+  if (!encode) return false;
+  const cuuint64_t extents[2] = {width, rows}, distance[1] = {width * (u64)value_bytes};
+  const cuuint32_t box[2] = {64u / (u32)value_bytes, 32}, ones[2] = {1, 1};
+  return encode(map, value_bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, extents, distance, box, ones,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 }  // namespace gsb

@@ -37,8 +37,11 @@ __device__ __forceinline__ void barrier_expect(u32 bar, u32 bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void barrier_arrive(u32 bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+// At a barrier of either CTA.  What it tells of is in this CTA's shared memory or in tensor memory, behind a fence of its own
+// (written_for_tensor_cores, sums_fence_before), so the arrival does not publish this thread's other writes to the cluster, which took 1 250
+// cycles each time.
 __device__ __forceinline__ void barrier_arrive_at(u32 cluster_bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
 __device__ __forceinline__ bool barrier_try(u32 bar, u32 parity) {
   u32 done;
@@ -90,6 +93,16 @@ __device__ __forceinline__ void load_tile(u32 to, const CUtensorMap* map, u32 cl
                "l"(map), "r"(cluster_bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
                : "memory");
 }
+// Rows of 64 bytes out of shared memory, 16-byte pieces of row i exchanged by i / 2 % 4 (the 64-byte swizzle).  What lies outside the array is
+// not written.
+__device__ __forceinline__ void store_tile(const CUtensorMap* map, u32 from, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(from), "r"(c0), "r"(c1) : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// All but the last LEFT stores of this thread have read what they write.
+template <int LEFT>
+__device__ __forceinline__ void stores_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(LEFT) : "memory"); }
+__device__ __forceinline__ void stores_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 
 // ---- matrix instructions ----
@@ -152,5 +165,7 @@ __device__ __forceinline__ void sums_read() { asm volatile("tcgen05.wait::ld.syn
 // `dims` extents, the first of neighbours in memory; strides in bytes of the others (multiples of 16, below 2^40).  False: it cannot be
 // described.
 bool describe_array(CUtensorMap* map, const void* base, int value_bytes, int rank, const u64* dims, const u64* strides, const u32* box);
+// Of stores: `rows` rows of `width` values, one behind the other; boxes of 32 rows by 64 bytes.
+bool describe_rows(CUtensorMap* map, void* base, int value_bytes, u64 width, u64 rows);
 
 }  // namespace gsb
