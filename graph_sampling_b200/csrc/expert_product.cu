@@ -7,6 +7,7 @@
 // All run on the tensor cores.  float32 operands are taken apart into three bfloat16 parts, a = a0 + a1 + a2 with |a1| <= 2^-8 |a| and
 // |a2| <= 2^-16 |a|, exactly (24 bits are 3 times 8), and a b is the sum of the six products a_i b_j with i + j <= 2: what is left out is
 // 2^-23 |a b| at the very most.
+#include <atomic>
 #include <type_traits>
 
 #include "group_plan.cuh"
@@ -848,7 +849,12 @@ static int launch_tiles(gsb_ctx* ctx, cudaStream_t stream, const CUtensorMap& ma
   const int size = a.partial ? 4 : (int)sizeof(T);
   void* const results = a.partial ? (void*)a.partial : (void*)out;
   a.by_tma = (i64)a.n * size % 16 == 0 && aligned_to(16, (const char*)results) && out_rows < ((i64)1 << 31) && describe_rows(&map_out, results, size, a.n, (u64)out_rows);
-  GSB_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  static std::atomic<bool> allowed[64];  // on which devices the kernel may have all the shared memory it can ask for
+  const int device = ctx_device(ctx);
+  if (device >= 64 || !allowed[device]) {
+    GSB_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kStagesRoom + 1024));
+    if (device < 64) allowed[device] = true;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(2 * max((i64)1, min((i64)kNumSMs / 2, most_tiles))));
   cfg.blockDim = dim3(tile_threads(READ));
