@@ -10,6 +10,7 @@
 #include <atomic>
 #include <type_traits>
 
+#include "few_rows.cuh"
 #include "group_plan.cuh"
 #include "launch.cuh"
 #include "row_values.cuh"
@@ -28,7 +29,7 @@ constexpr int kWriters = 8, kFirstReader = 4 + kWriters, kReaders = 8;
 constexpr int tile_threads(bool read) { return 32 * (kFirstReader + (read ? kReaders : 0)); }
 
 // The widest access, of at most 16 bytes, that addresses with these bits allow.
-__device__ __forceinline__ int unit_of(u64 bits) { return bits % 16 == 0 ? 16 : bits % 8 == 0 ? 8 : bits % 4 == 0 ? 4 : 2; }
+__host__ __device__ __forceinline__ int unit_of(u64 bits) { return bits % 16 == 0 ? 16 : bits % 8 == 0 ? 8 : bits % 4 == 0 ? 4 : 2; }
 
 // Rows as they lie in memory, for the warps that read them.
 struct RawRows {
@@ -168,15 +169,18 @@ __device__ __forceinline__ void write_line(u32 to, const u32 (&w)[4]) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
 }
 
-// float32: 4 neighbouring values of a row, copied behind the thread's back.  `valid`: how many of them there are; `some`: an address in the
-// array, where there are none.
-__device__ __forceinline__ void copy_four(u32 to, const float* from, int valid, bool aligned, const void* some) {
-  if (valid <= 0 || (valid >= 4 && aligned)) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(valid > 0 ? from : (const float*)some), "r"(valid > 0 ? 16 : 0) : "memory");
+// float32: 8 neighbouring values of a row, of which there are `valid`, in accesses of up to `unit` bytes.
+__device__ __forceinline__ void read_eight(const float* from, int valid, int unit, float (&v)[8]) {
+  if (valid >= 8 && unit == 32) {
+    asm volatile("ld.global.nc.L1::no_allocate.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+                 : "l"(from));
+  } else if (valid >= 8 && unit == 16) {
+    const float4 a = __ldg((const float4*)from), b = __ldg((const float4*)from + 1);
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
   } else {
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + q * 4), "l"(q < valid ? from + q : from), "r"(q < valid ? 4 : 0) : "memory");
+    for (int q = 0; q < 8; ++q) v[q] = q < valid ? __ldg(from + q) : 0.f;
   }
 }
 __device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -199,47 +203,37 @@ __device__ __forceinline__ u32 next_parts(float& low, float& high) {
   high -= __uint_as_float(w & 0xffff0000u);
   return w;
 }
-// A warp's room for float32 values on their way: 8 lines of 64 values, in steps of 4 lines.  A step holds the first four of each 8
-// values (512 bytes), then the other four, so that a lane reads its 8 values, and all lanes theirs, without meeting in a bank.
-constexpr int kStepBytes = 4 * 64 * 4, kPairBytes = 2 * kStepBytes;
-// 8 values of each of two lines to their places, 32 lines apart, every part in an operand of its own, `apart` bytes from the one before.
-// `ring`: of this lane's first 16 bytes.  All of the warp's values have been read when it returns.
-__device__ __forceinline__ void write_parts(u32 ring, u32 to, u32 apart) {
-  float rest[2][8];
+// 8 values to their place in a line, every part in an operand of its own, `apart` bytes from the one before.
+__device__ __forceinline__ void write_parts(float (&rest)[8], u32 to, u32 apart) {
+  u32 w[4];
+  float any = 0.f;  // what is left of an infinity, of NaN and of what became an infinity is none of the numbers
+  float kept[8];
 #pragma unroll
-  for (int h = 0; h < 4; ++h)
-    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                 : "=f"(rest[h / 2][h % 2 * 4]), "=f"(rest[h / 2][h % 2 * 4 + 1]), "=f"(rest[h / 2][h % 2 * 4 + 2]), "=f"(rest[h / 2][h % 2 * 4 + 3])
-                 : "r"(ring + h * 512)
-                 : "memory");
-  u32 w[2][4];
+  for (int q = 0; q < 8; ++q) kept[q] = rest[q];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) w[i / 4][i % 4] = next_parts(rest[i / 4][2 * (i % 4)], rest[i / 4][2 * (i % 4) + 1]);
-  // what is left of an infinity, of NaN and of what became an infinity is none of the numbers
-  float any = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) any += (rest[0][2 * i] + rest[0][2 * i + 1]) + (rest[1][2 * i] + rest[1][2 * i + 1]);
+  for (int q = 0; q < 4; ++q) {
+    w[q] = next_parts(rest[2 * q], rest[2 * q + 1]);
+    any += rest[2 * q] + rest[2 * q + 1];
+  }
   if (fabsf(any) <= 3.402823466e38f) {
 #pragma unroll
     for (int p = 0; p < 3; ++p) {
       if (p > 0)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w[i / 4][i % 4] = next_parts(rest[i / 4][2 * (i % 4)], rest[i / 4][2 * (i % 4) + 1]);
-      write_line(to + p * apart, w[0]);
-      write_line(to + p * apart + 32 * kLineBytes, w[1]);
+        for (int q = 0; q < 4; ++q) w[q] = next_parts(rest[2 * q], rest[2 * q + 1]);
+      write_line(to + p * apart, w);
     }
   } else {
 #pragma unroll 1
-    for (int h = 0; h < 8; ++h) {
-      float two[2];
-      asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(two[0]), "=f"(two[1]) : "r"(ring + h / 2 * 512 + h % 2 * 8) : "memory");
-      for (int p = 0; p < 3; ++p) {
-        const u32 low = next_part(two[0]);
-        asm volatile("st.shared.b32 [%0], %1;" ::"r"(to + p * apart + h / 4 * 32 * kLineBytes + h % 4 * 4), "r"(low | next_part(two[1]) << 16) : "memory");
+    for (int p = 0; p < 3; ++p) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const u32 low = next_part(kept[2 * q]);
+        w[q] = low | next_part(kept[2 * q + 1]) << 16;
       }
+      write_line(to + p * apart, w);
     }
   }
-  __syncwarp();
 }
 
 // The lines of the reduced index that a pair of CTAs goes through, tile by tile.
@@ -258,10 +252,6 @@ struct Walk {
     settle(a, plan, tiles, step);
   }
 };
-
-// float32 values that a reading warp has on their way: twice 8 lines.
-constexpr int kPairsAhead = 2;
-constexpr int ring_bytes(int parts) { return parts == 3 ? kReaders * kPairsAhead * kPairBytes : 0; }
 
 // PARTS: 3 for float32, else 1.  ACROSS: the second operand's lines hold the reduced index across them (a gradient's both do).  READ: rows
 // (and a gradient's both operands) are read by warps, not by TMA.
@@ -315,7 +305,7 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
   const u32 half = a.columns / 2, b_bytes = half * kLineBytes, stage_bytes = PARTS * (kRowsOperand + b_bytes);
 
   if (warp == 0 && lane == 0 && !(READ && GRAD)) {
-    const u32 full_of_first = address_in(full, 0), loaded_bytes = 2 * PARTS * ((READ ? 0 : kRowsOperand) + b_bytes);
+    const u32 full_of_first = address_in(full, 0);
     u32 stage = 0, turn = 0;
     for (u64 t = first; t < tiles; t += step) {
       const Tile tile = tile_at<GRAD, kPerLine>(a, plan, t);
@@ -329,6 +319,10 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
         }
       }
       const int matrix = (g.first + tile.e) * a.expert_step;
+      // The second CTA's rows only where there are any: what else lies in its shared memory makes sums that nobody reads.  (Boxes of the 32 rows
+      // that a step has were slower than one of 128: 15.7 us for 14.1.)
+      const bool both = tile.rows > 128, rows_here = rank == 0 || both;
+      const u32 loaded_bytes = PARTS * ((GRAD ? 2 : READ ? 0 : both ? 2 : 1) * kRowsOperand + 2 * b_bytes);
       for (u32 b = 0; b < tile.blocks; ++b) {
         if (!barrier_wait(empty + 8 * stage, turn ^ 1, &stop, counters)) goto loaded;
         if (rank == 0) barrier_expect(full + 8 * stage, loaded_bytes);
@@ -341,7 +335,7 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
             for (u32 j = 0; j < half / 64; ++j)
               load_tile(to_b + j * kAcross, of_b, bar, (int)(tile.n0 + rank * half + j * 64), (int)(tile.row0 + b * 64), p);
           } else {
-            if (!READ) load_tile(to_a, of_a, bar, (int)(b * kPerLine), (int)(tile.row0 + rank * 128), p);
+            if (!READ && rows_here) load_tile(to_a, of_a, bar, (int)(b * kPerLine), (int)(tile.row0 + rank * 128), p);
             if (ACROSS)
               for (u32 j = 0; j < half / 64; ++j)
                 load_tile(to_b + j * kAcross, of_b, bar, (int)(tile.n0 + rank * half + j * 64), (int)(b * kPerLine), matrix, p);
@@ -412,90 +406,62 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
     auto first_row = [&](const Tile& tile) { return GRAD ? (i64)plan.begin[tile.e] + tile.row0 : (i64)tile.row0 + rank * 128; };
     auto rows_here = [&](const Tile& tile) { return GRAD ? (int)tile.rows : (int)tile.rows - (int)rank * 128; };
     if constexpr (PARTS == 3) {
-      // A warp has lines 4 w to 4 w + 3 and those 32, 64 and 96 behind them, 8 at a time.  A lane copies four values of two lines each time
-      // (16 lanes to a line), and takes apart 8 values of one line
-      constexpr int kPairs = GRAD ? 3 : 2;
-      const u32 w = me / 32, chunk = lane & 7, segment = w * 4 + lane / 8, place = segment * kLineBytes + ((chunk ^ (segment & 7)) << 4);
-      const u32 ring = stages_at + a.stages * stage_bytes + w * kPairsAhead * kPairBytes;
-      const u32 copies_to = ring + (lane & 1) * 512 + (lane / 16 * 8 + (lane & 15) / 2) * 16;  // of the first of two lines; the next two are 256 bytes on
-      const int copied_line = (int)w * 4 + lane / 16, copied_column = (lane & 15) * 4;
-      const bool aligned = a.rows.unit == 16, grad_aligned = a.grad.unit == 16;
-      const bool simple = aligned && a.rows.width % 4 == 0, grad_simple = grad_aligned && a.grad.width % 4 == 0;
+      // A lane has the same 8 values' place in lines 4 w + lane / 8, 32 behind them and so on; those of the next stage are on their way while it
+      // takes this one's apart.  (Copied into shared memory meanwhile they met the matrix instructions' operands there: 460 us for 500 000
+      // rows of 256 to 256 values.)
+      constexpr int kPieces = GRAD ? 6 : 4;
+      const u32 chunk = lane & 7, segment = me / 32 * 4 + lane / 8, place = segment * kLineBytes + ((chunk ^ (segment & 7)) << 4);
       Walk<GRAD, kPerLine> ahead = now;
       const float *from = nullptr, *from_grad = nullptr;
-      int columns = 0, grad_columns = 0, rows_left = 0, pair = 0;  // from this thread's first on
+      int columns = 0, grad_columns = 0, rows_left = 0;  // from this lane's first on
       auto begin_tile = [&] {
         if (ahead.t >= tiles) return;
         const Tile& tile = ahead.tile;
-        const u32 c = (GRAD ? tile.m0 + rank * 128 : 0) + copied_column;
-        from = (const float*)a.rows.at + (first_row(tile) + copied_line) * a.rows.stride + c;
+        const u32 c = (GRAD ? tile.m0 + rank * 128 : 0) + chunk * 8;
+        from = (const float*)a.rows.at + (first_row(tile) + segment) * a.rows.stride + c;
         columns = (int)a.rows.width - (int)c;
-        rows_left = rows_here(tile) - copied_line;
+        rows_left = rows_here(tile) - (int)segment;
         if (GRAD) {
-          const u32 d = tile.n0 + rank * half + copied_column;
-          from_grad = (const float*)a.grad.at + (first_row(tile) + copied_line) * a.grad.stride + d;
+          const u32 d = tile.n0 + rank * half + chunk * 8;
+          from_grad = (const float*)a.grad.at + (first_row(tile) + segment) * a.grad.stride + d;
           grad_columns = (int)a.grad.width - (int)d;
         }
       };
       begin_tile();
-      auto copy_pair = [&](u32 to, const float* at, i64 stride, int rows, int width, bool simple, bool wide, const void* some) {
-        if (simple) {  // four values or none
-          if (width <= 0) rows = 0;
+      float v[kPieces][8];
+      auto read = [&](int j, float(&to)[8]) {  // piece j: of the rows, lines 32 j on (a gradient's second two: the next 64 columns); of a gradient's rows
+        if (ahead.t >= tiles) return;
+        if (GRAD && j >= 4) read_eight(from_grad + (j - 4) * 32 * a.grad.stride, rows_left > (j - 4) * 32 ? grad_columns : 0, a.grad.unit, to);
+        else if (GRAD) read_eight(from + (j & 1) * 32 * a.rows.stride + (j >> 1) * 64, rows_left > (j & 1) * 32 ? columns - (j >> 1) * 64 : 0, a.rows.unit, to);
+        else read_eight(from + j * 32 * a.rows.stride, rows_left > j * 32 ? columns : 0, a.rows.unit, to);
+      };
+      auto go_on = [&] {
+        if (ahead.t >= tiles) return;
+        from += GRAD ? 64 * a.rows.stride : 64;
+        if (GRAD) from_grad += 64 * a.grad.stride, rows_left -= 64;
+        else columns -= 64;
+        ahead.next(a, plan, tiles, step);
+        if (ahead.b == 0) begin_tile();
+      };
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int line = (i >> 1) * 32 + (i & 1) * 2;
-            const bool in = rows > line;
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + (i >> 1) * kStepBytes + (i & 1) * 256), "l"(in ? at : (const float*)some),
-                         "r"(in ? 16 : 0)
-                         : "memory");
-            at += (i & 1 ? 30 : 2) * stride;
-          }
-        } else {
-#pragma unroll 1
-          for (int i = 0; i < 4; ++i) {
-            const int line = (i >> 1) * 32 + (i & 1) * 2;
-            copy_four(to + (i >> 1) * kStepBytes + (i & 1) * 256, at + line * stride, rows > line ? width : 0, wide, some);
-          }
-        }
-      };
-      auto copy = [&](u32 slot) {
-        if (ahead.t < tiles) {
-          const u32 to = copies_to + slot * kPairBytes;
-          if (GRAD && pair == 2) copy_pair(to, from_grad, a.grad.stride, rows_left, grad_columns, grad_simple, grad_aligned, a.grad.at);
-          else if (GRAD) copy_pair(to, from + pair * 64, a.rows.stride, rows_left, columns - pair * 64, simple, aligned, a.rows.at);
-          else copy_pair(to, from + pair * 64 * a.rows.stride, a.rows.stride, rows_left - pair * 64, columns, simple, aligned, a.rows.at);
-          if (++pair == kPairs) {
-            pair = 0;
-            from += GRAD ? 64 * a.rows.stride : 64;
-            if (GRAD) from_grad += 64 * a.grad.stride, rows_left -= 64;
-            else columns -= 64;
-            ahead.next(a, plan, tiles, step);
-            if (ahead.b == 0) begin_tile();
-          }
-        }
-        copies_end();
-      };
-      for (u32 slot = 0; slot < kPairsAhead; ++slot) copy(slot);
-      u32 slot = 0;
+      for (int j = 0; j < kPieces; ++j) read(j, v[j]);
+      go_on();
       while (now.t < tiles) {
         const bool free = barrier_wait(empty + 8 * stage, turn ^ 1, &stop, counters);
         if (!__all_sync(0xffffffffu, free)) break;
         const u32 at = stages_at + stage * stage_bytes + place;
 #pragma unroll
-        for (int q = 0; q < kPairs; ++q) {
-          copies_wait<kPairsAhead - 1>();
-          __syncwarp();
-          const bool of_grad = GRAD && q == 2;
-          write_parts(ring + lane * 16 + slot * kPairBytes, at + (of_grad ? PARTS * kRowsOperand : q * 64 * kLineBytes), of_grad ? b_bytes : kRowsOperand);
-          copy(slot);
-          if (++slot == kPairsAhead) slot = 0;
+        for (int j = 0; j < kPieces; ++j) {
+          const bool of_grad = GRAD && j >= 4;
+          write_parts(v[j], at + (of_grad ? PARTS * kRowsOperand + (j - 4) * 32 * kLineBytes : j * 32 * kLineBytes), of_grad ? b_bytes : kRowsOperand);
+          read(j, v[j]);
         }
+        go_on();
         __syncwarp();
         if (lane == 0) barrier_arrive(written + 8 * stage);
         now.next(a, plan, tiles, step);
         if (++stage == (u32)a.stages) stage = 0, turn ^= 1;
       }
-      copies_wait<0>();
     } else {
       // warp w has lines w, w + 8 and so on; copies of kLag stages are on their way before the first is handed over
       constexpr u32 kLag = 3;
@@ -833,7 +799,7 @@ static int by_experts(gsb_ctx* ctx, i64 num_experts, i64 num_rows, const int64_t
   return GSB_OK;
 }
 
-// Shared memory for stages and the readers' copies: what the fixed part (the plan, the ways out) leaves.
+// Shared memory for stages: what the fixed part (the plan, the ways out) leaves.
 constexpr int kStagesRoom = (227 - 46) * 1024 - 1024;
 // Launches pairs of CTAs: at most one CTA per SM.  In the order of the stream, with no overlap of its neighbours' ends and beginnings: with
 // overlap, hundreds of copies and products queued one behind the other came to a halt, waiting CTAs of one kernel beside clusters of another
@@ -842,9 +808,9 @@ template <class T, bool WHOLE_NUMBERS, int PARTS, bool GRAD, bool ACROSS, bool R
 static int launch_tiles(gsb_ctx* ctx, cudaStream_t stream, const CUtensorMap& map_a, const CUtensorMap& map_b, TileArgs a, i64 most_tiles, i64 out_rows, T* out) {
   auto kernel = k_tiles<T, WHOLE_NUMBERS, PARTS, GRAD, ACROSS, READ>;
   const int stage = PARTS * (kRowsOperand + (int)a.columns / 2 * kLineBytes);
-  a.stages = min(kMaxStages, (kStagesRoom - ring_bytes(PARTS)) / stage);
+  a.stages = min(kMaxStages, kStagesRoom / stage);
   a.how = instruction(WHOLE_NUMBERS ? OPERAND_S8 : std::is_same<T, __half>::value ? OPERAND_F16 : OPERAND_BF16, GRAD, GRAD || ACROSS, kPairRows, a.columns);
-  const int smem = a.stages * stage + 1024 + ring_bytes(PARTS);
+  const int smem = a.stages * stage + 1024;
   CUtensorMap map_out = {};
   const int size = a.partial ? 4 : (int)sizeof(T);
   void* const results = a.partial ? (void*)a.partial : (void*)out;
@@ -882,6 +848,30 @@ static Lines matrices_operand(const void* w, int dtype, i64 experts, i64 expert_
   return Lines{w, experts, experts > 1 ? expert_stride : 0, n, n_stride, k, dtype};
 }
 
+// Whether a product is of little work, for which the kernels without tensor cores are sooner done: by what both take, in microseconds,
+// fitted to a sweep of 17 shapes with bfloat16 and float32 (1 to 16 384 rows, 1 to 200 experts, widths of 32 to 2 048).
+// Few rows: 4 for the launch, one per 300 CTAs, one per 350 of the reduced index, one per 2.4 M weights that pass a CTA (1 024 rows of 100 to 47 by
+// three experts: 5.4 for 13.4 by tiles; 4 096 of 64 to 64 by four: 10.3 for 7.1; 32 of 1 024 floats to 2 048 by eight: 18 for 87).  Tiles: 7, the
+// weights or the chain of stages, whichever is longer, and the copy of matrices that TMA cannot read.
+static double few_time(i64 num_rows, i64 k, i64 n, i64 num_experts) {
+  const double tiles = (double)(num_rows / kFewRows + min(num_rows, num_experts));
+  return 4. + tiles * (double)((n + kFewColumns - 1) / kFewColumns) / 300. + (double)k / 350. + tiles * (double)k * (double)n / 2.4e6;
+}
+static bool few_rows(i64 num_rows, i64 k, i64 n, i64 num_experts, int size, i64 copied_bytes) {
+  const double weights = (double)min(num_rows, num_experts) * (double)k * (double)n * size / 4.5e6, chain = (double)k * size / 128. * 0.35;
+  // the copy: read, written with its parts, and read again by the products
+  const double copy = copied_bytes > 0 ? 3. + (double)copied_bytes * (size == 4 ? 10. / 6. : 2.) / 2.6e6 : 0.;
+  return few_time(num_rows, k, n, num_experts) < 7. + (weights > chain ? weights : chain) + copy;
+}
+// The same of the weights' gradient.  Few rows: 3, one per 400 CTAs, and the rows that a CTA goes through (1 024 rows of 100 to 47 by three experts 7.5
+// us for 22; one row of 1 024 to 1 024 16 for 11.6; 4 096 of 64 to 64 by four 20 for 15, of floats 14 for 26).  Tiles: 9, or 15 with chunks, 8 more for float32.
+static bool few_grad(i64 num_rows, i64 k, i64 n, i64 num_experts, int size, bool chunks) {
+  const double ctas = (double)num_experts * (double)((k + kFewRows - 1) / kFewRows) * (double)((n + kFewColumns - 1) / kFewColumns);
+  const double few = 3. + ctas / 400. + (double)num_rows / (double)num_experts * 0.018;
+  return few < (chunks ? 15. : 9.) + (size == 4 ? 8. : 0.) + (double)num_experts * (double)k * (double)n * size / 3e6;
+}
+static int few_grid(i64 tiles) { return (int)max((i64)1, min((i64)kNumSMs * 6, tiles)); }
+
 // Rows of an expert that one tile of the weights' gradient sums.  All of them, unless that leaves pairs of CTAs without work.
 static i64 chunk_rows(i64 num_rows, i64 k, i64 n, u32 columns, i64 num_experts) {
   const i64 tiles = (k + kPairRows - 1) / kPairRows * ((n + columns - 1) / columns);
@@ -907,7 +897,8 @@ static int with_type(int dtype, bool read, F f) {
 static RawRows raw_rows(const Lines& x) {
   const int size = value_bytes(x.dtype);
   const i64 stride = x.height > 1 ? x.stride : 0;
-  return RawRows{x.at, stride, (u32)x.width, unit_bytes(16, (u64)(uintptr_t)x.at | (u64)(stride * size))};
+  const u64 bits = (u64)(uintptr_t)x.at | (u64)(stride * size);
+  return RawRows{x.at, stride, (u32)x.width, bits % 32 == 0 ? 32 : unit_of(bits)};
 }
 
 }  // namespace gsb
@@ -920,7 +911,8 @@ extern "C" int64_t gsb_expert_product_workspace(const void* rows, int dtype, int
   if (value_bytes(dtype) == 0 || num_rows < 0 || num_rows >= ((i64)1 << 31) || k < 1 || k > GSB_MAX_ROW_LEN || n < 1 || n > GSB_MAX_ROW_LEN ||
       num_experts < 1 || num_experts > GSB_MAX_EXPERTS)
     return GSB_ERR_INVALID_ARGUMENT;
-  return matrices_operand(weights, dtype, num_experts, weights_expert_stride, k, weights_k_stride, n, weights_n_stride).bytes();
+  const i64 copied = matrices_operand(weights, dtype, num_experts, weights_expert_stride, k, weights_k_stride, n, weights_n_stride).bytes();
+  return few_rows(num_rows, k, n, num_experts, value_bytes(dtype), copied) ? 0 : copied;
 }
 
 extern "C" int gsb_expert_product(gsb_ctx* ctx, void* stream_, const void* rows, int dtype, int64_t num_rows, int64_t k, int64_t rows_stride,
@@ -942,6 +934,21 @@ extern "C" int gsb_expert_product(gsb_ctx* ctx, void* stream_, const void* rows,
   const bool across = rows_are_lines(k, n, weights_k_stride, weights_n_stride);
   Lines x = rows_operand(rows, dtype, num_rows, k, rows_stride);
   Lines w = matrices_operand(weights, dtype, num_experts, weights_expert_stride, k, weights_k_stride, n, weights_n_stride);
+  if (few_rows(num_rows, k, n, num_experts, size, w.bytes()))
+    return by_experts(ctx, num_experts, num_rows, offsets, [&](const Groups& g) {
+      const i64 line = w.height > 1 ? w.stride : 0;
+      const FewArgs a{g, rows, weights, rows_stride, line, w.matrix_stride, (u32)k, (u32)n, nullptr, nullptr};
+      const bool wide = aligned_to(16, (const char*)weights) && line * size % 16 == 0 && w.matrix_stride * size % 16 == 0;
+      const int grid = few_grid((num_rows / kFewRows + min(num_rows, (i64)g.experts)) * ((n + kFewColumns - 1) / kFewColumns));
+      ScopedKernelTimer timer(ctx, KID_EXPERT_PRODUCT, stream);
+      with_unit(dtype, size, [&](auto value, auto) {
+        typedef decltype(value) T;
+        auto kernel = across ? (wide ? k_few_across<T, true> : k_few_across<T, false>) : (wide ? k_few_along<T, T, true> : k_few_along<T, T, false>);
+        launch_behind(stream, kernel, grid, kFewThreads, a, (T*)out);
+      });
+      GSB_LAUNCH_OK();
+      return (int)GSB_OK;
+    });
   char* room = (char*)workspace;
   if ((st = bring(ctx, stream, &w, &room)) != GSB_OK) return st;
   TileArgs a = {};
@@ -973,6 +980,7 @@ extern "C" int64_t gsb_expert_product_grad_workspace(const void* rows, int dtype
       num_experts < 1 || num_experts > GSB_MAX_EXPERTS)
     return GSB_ERR_INVALID_ARGUMENT;
   const i64 chunk = chunk_rows(num_rows, k, n, tile_columns(n, dtype), num_experts);
+  if (few_grad(num_rows, k, n, num_experts, value_bytes(dtype), chunk < num_rows)) return 0;
   return rounded(min(num_experts, (i64)kPlanExperts) * 2 * (i64)sizeof(CUtensorMap)) + (chunk < num_rows ? rounded(most_chunks(num_rows, chunk, num_experts) * k * n * 4) : 0);
 }
 
@@ -990,6 +998,19 @@ extern "C" int gsb_expert_product_grad(gsb_ctx* ctx, void* stream_, const void* 
     GSB_CUDA_OK(cudaMemsetAsync(out, 0, (size_t)(num_experts * k * n * size), stream));
     return GSB_OK;
   }
+  if (few_grad(num_rows, k, n, num_experts, size, chunk_rows(num_rows, k, n, tile_columns(n, dtype), num_experts) < num_rows))
+    return by_experts(ctx, num_experts, num_rows, offsets, [&](const Groups& g) {
+      const FewArgs a{g, rows, grad, rows_stride, grad_stride, 0, (u32)k, (u32)n, nullptr, nullptr};
+      const bool wide = aligned_to(16, (const char*)grad) && (num_rows == 1 || grad_stride * size % 16 == 0);
+      const int grid = few_grid(g.experts * ((k + kFewRows - 1) / kFewRows) * ((n + kFewColumns - 1) / kFewColumns));
+      ScopedKernelTimer timer(ctx, KID_EXPERT_PRODUCT, stream);
+      with_unit(dtype, size, [&](auto value, auto) {
+        typedef decltype(value) T;
+        launch_behind(stream, wide ? k_few_grad<T, true> : k_few_grad<T, false>, grid, kFewThreads, a, (T*)out);
+      });
+      GSB_LAUNCH_OK();
+      return (int)GSB_OK;
+    });
   const int64_t need = gsb_expert_product_grad_workspace(rows, dtype, num_rows, k, rows_stride, grad, n, grad_stride, num_experts);
   GSB_REQUIRE(need >= 0 && workspace && aligned_to(256, (const char*)workspace), GSB_ERR_INVALID_ARGUMENT);
   GSB_REQUIRE(workspace_bytes >= need, GSB_ERR_CAPACITY);
@@ -1048,6 +1069,18 @@ extern "C" int gsb_expert_product_int8(gsb_ctx* ctx, void* stream_, const int8_t
   GSB_REQUIRE(values && scales && weight_values && weight_scales && out && aligned_to(4, scales, weight_scales) && aligned_to(size, (const char*)out),
               GSB_ERR_INVALID_ARGUMENT);
   cudaStream_t stream = (cudaStream_t)stream_;
+  if (few_rows(num_rows, k, n, num_experts, 1, 0))
+    return by_experts(ctx, num_experts, num_rows, offsets, [&](const Groups& g) {
+      const FewArgs a{g, values, weight_values, values_stride, weight_n_stride, num_experts > 1 ? weight_expert_stride : 0, (u32)k, (u32)n, scales, weight_scales};
+      const int grid = few_grid((num_rows / kFewRows + min(num_rows, (i64)g.experts)) * ((n + kFewColumns - 1) / kFewColumns));
+      ScopedKernelTimer timer(ctx, KID_EXPERT_PRODUCT, stream);
+      with_unit(out_dtype, size, [&](auto value, auto) {
+        typedef decltype(value) Out;
+        launch_behind(stream, k_few_along<signed char, Out, true>, grid, kFewThreads, a, (Out*)out);
+      });
+      GSB_LAUNCH_OK();
+      return (int)GSB_OK;
+    });
   const Lines x{values, 1, 0, num_rows, values_stride, k, GSB_F16};
   const Lines w{weight_values, num_experts, num_experts > 1 ? weight_expert_stride : 0, n, weight_n_stride, k, GSB_F16};
   TileArgs a = {};
