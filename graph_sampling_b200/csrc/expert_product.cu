@@ -104,18 +104,21 @@ static __device__ __noinline__ void copy_rows(const char* room, int lane, char* 
   else copy_rows_by<unsigned short>(room, lane, to, pitch, rows, bytes);
   __syncwarp();
 }
-// A warp's way out: two rooms, taken in turn.
+// A warp's way out: one room or two, taken in turn.  float32 has two; 16-bit types do better with one and a stage more for their loads (65 536
+// rows of 2 048 to 2 048: 411 us for 433).
+constexpr int rooms_of(int parts) { return parts == 3 ? 2 : 1; }
+template <int ROOMS>
 struct Exit {
   char* rooms;
   u32 turn;
 };
-template <class U>
-__device__ __forceinline__ void write_rows(Exit& exit, int lane, const float (&v)[kStoreBytes / sizeof(U)], U* to, i64 pitch, u32 rows, u32 columns, int unit,
+template <class U, int ROOMS>
+__device__ __forceinline__ void write_rows(Exit<ROOMS>& exit, int lane, const float (&v)[kStoreBytes / sizeof(U)], U* to, i64 pitch, u32 rows, u32 columns, int unit,
                                            const CUtensorMap* map, i64 row, u32 column) {
   constexpr int PER = 16 / sizeof(U);
-  char* const room = exit.rooms + (exit.turn & 1) * kRoom;
+  char* const room = exit.rooms + exit.turn % ROOMS * kRoom;
   ++exit.turn;
-  if (lane == 0) stores_read<1>();
+  if (lane == 0) stores_read<ROOMS - 1>();
   __syncwarp();
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
@@ -266,7 +269,8 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
   __shared__ PlanTable plan;
   __shared__ __align__(8) u64 bars[3 * kMaxStages + 4];
   __shared__ float column_scales[WHOLE_NUMBERS ? kWriters : 1][128];
-  __shared__ __align__(1024) char rooms[kWriters][2 * kRoom];
+  constexpr int kRooms = rooms_of(PARTS);
+  __shared__ __align__(1024) char rooms[kWriters][kRooms * kRoom];
   __shared__ u32 sums_at;
   __shared__ volatile int stop;
   const u32 stages_at = (smem_address(raw) + 1023u) & ~1023u;
@@ -519,7 +523,7 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
     const u32 c0 = (u32)(warp - 4) / 4 * half;                                     // this warp's half of the columns
     const u32 sums_empty_of_first = address_in(sums_empty, 0);
     const int unit = unit_of((u64)(uintptr_t)out | (u64)a.n * sizeof(T)), unit_partial = unit_of((u64)a.n * 4);
-    Exit exit{rooms[warp - 4], 0};
+    Exit<kRooms> exit{rooms[warp - 4], 0};
     u32 made = 0;
     for (u64 t = first; t < tiles; t += step) {
       const Tile tile = tile_at<GRAD, kPerLine>(a, plan, t);
@@ -799,8 +803,8 @@ static int by_experts(gsb_ctx* ctx, i64 num_experts, i64 num_rows, const int64_t
   return GSB_OK;
 }
 
-// Shared memory for stages: what the fixed part (the plan, the ways out) leaves.
-constexpr int kStagesRoom = (227 - 46) * 1024 - 1024;
+// Shared memory for stages: what the fixed part (the plan, the scales, the ways out) leaves, and what is lost to their alignment.
+constexpr int stages_room(int parts) { return (227 - 14) * 1024 - rooms_of(parts) * kWriters * kRoom - 1024; }
 // Launches pairs of CTAs: at most one CTA per SM.  In the order of the stream, with no overlap of its neighbours' ends and beginnings: with
 // overlap, hundreds of copies and products queued one behind the other came to a halt, waiting CTAs of one kernel beside clusters of another
 // that need SMs as a whole.
@@ -808,7 +812,7 @@ template <class T, bool WHOLE_NUMBERS, int PARTS, bool GRAD, bool ACROSS, bool R
 static int launch_tiles(gsb_ctx* ctx, cudaStream_t stream, const CUtensorMap& map_a, const CUtensorMap& map_b, TileArgs a, i64 most_tiles, i64 out_rows, T* out) {
   auto kernel = k_tiles<T, WHOLE_NUMBERS, PARTS, GRAD, ACROSS, READ>;
   const int stage = PARTS * (kRowsOperand + (int)a.columns / 2 * kLineBytes);
-  a.stages = min(kMaxStages, kStagesRoom / stage);
+  a.stages = min(kMaxStages, stages_room(PARTS) / stage);
   a.how = instruction(WHOLE_NUMBERS ? OPERAND_S8 : std::is_same<T, __half>::value ? OPERAND_F16 : OPERAND_BF16, GRAD, GRAD || ACROSS, kPairRows, a.columns);
   const int smem = a.stages * stage + 1024;
   CUtensorMap map_out = {};
@@ -818,7 +822,7 @@ static int launch_tiles(gsb_ctx* ctx, cudaStream_t stream, const CUtensorMap& ma
   static std::atomic<bool> allowed[64];  // on which devices the kernel may have all the shared memory it can ask for
   const int device = ctx_device(ctx);
   if (device >= 64 || !allowed[device]) {
-    GSB_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kStagesRoom + 1024));
+    GSB_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, stages_room(PARTS) + 1024));
     if (device < 64) allowed[device] = true;
   }
   cudaLaunchConfig_t cfg = {};

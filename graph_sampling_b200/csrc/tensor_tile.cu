@@ -19,6 +19,15 @@ static EncodeTiled encode_tiled() {
   return found;
 }
 
+// The driver's call wants the device's context to be current on this thread, which only calls of the runtime make it: a thread of autograd's that
+// comes here first has none yet.
+template <class F>
+static bool encoded(F encode) {
+  if (encode() == CUDA_SUCCESS) return true;
+  int device;
+  return cudaGetDevice(&device) == cudaSuccess && cudaSetDevice(device) == cudaSuccess && encode() == CUDA_SUCCESS;
+}
+
 bool describe_array(CUtensorMap* map, const void* base, int value_bytes, int rank, const u64* dims, const u64* strides, const u32* box) {
   const EncodeTiled encode = encode_tiled();
   if (!encode) return false;
@@ -29,9 +38,11 @@ bool describe_array(CUtensorMap* map, const void* base, int value_bytes, int ran
     boxes[d] = box[d];
     if (d > 0) distances[d - 1] = strides[d - 1];
   }
-  return encode(map, value_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, const_cast<void*>(base), extents,
-                distances, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return encoded([&] {
+    return encode(map, value_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, const_cast<void*>(base), extents,
+                  distances, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  });
 }
 
 bool describe_rows(CUtensorMap* map, void* base, int value_bytes, u64 width, u64 rows) {
@@ -39,8 +50,10 @@ bool describe_rows(CUtensorMap* map, void* base, int value_bytes, u64 width, u64
   if (!encode) return false;
   const cuuint64_t extents[2] = {width, rows}, distance[1] = {width * (u64)value_bytes};
   const cuuint32_t box[2] = {64u / (u32)value_bytes, 32}, ones[2] = {1, 1};
-  return encode(map, value_bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, extents, distance, box, ones,
-                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return encoded([&] {
+    return encode(map, value_bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, extents, distance, box, ones,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  });
 }
 
 }  // namespace gsb

@@ -317,3 +317,28 @@ def test_product_int8_limits_and_layouts(ops):
                 (values, scales, weight_values[:, :40], weight_scales, offsets[:2])):
         with pytest.raises(TypeError):
             ops.expert_product_int8(*bad)
+
+
+def test_first_call_of_a_thread(ops, nn):
+    """A thread that has made no other call of CUDA's runtime yet (autograd's, a new one) has no context of the driver's."""
+    import threading
+    g = generator(21)
+    offsets = offsets_of([3000, 2000, 1000])
+    rows, weights = normal(g, 6000, 256, dtype=torch.bfloat16), normal(g, 3, 256, 256, dtype=torch.bfloat16)
+    want = ops.expert_product(rows, weights, offsets)
+    want_grad = ops.expert_product_grad(rows, want, offsets)
+    kept = [torch.empty_like(want) for _ in range(4)], [torch.empty_like(want_grad) for _ in range(4)]
+    torch.cuda.synchronize()
+    del kept                                                                    # memory that needs no call to be had
+    got = {}
+
+    def call(k):
+        got[k] = ops.expert_product_grad(rows, want, offsets) if k % 2 else ops.expert_product(rows, weights, offsets)
+    for k in range(4):
+        thread = threading.Thread(target=call, args=(k,))
+        thread.start()
+        thread.join()
+        assert torch.equal(got[k], want_grad if k % 2 else want)
+    leaf = rows.clone().requires_grad_()
+    back, = torch.autograd.grad(nn.product(leaf, weights, offsets), leaf, want)
+    assert torch.equal(back, ops.expert_product(want, weights.transpose(1, 2), offsets))
