@@ -206,35 +206,37 @@ __device__ __forceinline__ u32 next_parts(float& low, float& high) {
   high -= __uint_as_float(w & 0xffff0000u);
   return w;
 }
-// 8 values to their place in a line, every part in an operand of its own, `apart` bytes from the one before.
-__device__ __forceinline__ void write_parts(float (&rest)[8], u32 to, u32 apart) {
-  u32 w[4];
-  float any = 0.f;  // what is left of an infinity, of NaN and of what became an infinity is none of the numbers
-  float kept[8];
+// 8 values each of two lines, 32 apart, to their places, every part in an operand of its own, `apart` bytes from the one before.
+__device__ __forceinline__ void write_parts(const float (&x)[8], const float (&y)[8], u32 to, u32 apart) {
+  float rest[16], any = 0.f;  // what is left of an infinity, of NaN and of what became an infinity is none of the numbers
+  u32 w[2][4];
 #pragma unroll
-  for (int q = 0; q < 8; ++q) kept[q] = rest[q];
+  for (int q = 0; q < 8; ++q) rest[q] = x[q], rest[8 + q] = y[q];
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    w[q] = next_parts(rest[2 * q], rest[2 * q + 1]);
-    any += rest[2 * q] + rest[2 * q + 1];
-  }
+  for (int q = 0; q < 8; ++q) w[q / 4][q % 4] = next_parts(rest[2 * q], rest[2 * q + 1]);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) any += (rest[4 * q] + rest[4 * q + 1]) + (rest[4 * q + 2] + rest[4 * q + 3]);
   if (fabsf(any) <= 3.402823466e38f) {
 #pragma unroll
     for (int p = 0; p < 3; ++p) {
       if (p > 0)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) w[q] = next_parts(rest[2 * q], rest[2 * q + 1]);
-      write_line(to + p * apart, w);
+        for (int q = 0; q < 8; ++q) w[q / 4][q % 4] = next_parts(rest[2 * q], rest[2 * q + 1]);
+      write_line(to + p * apart, w[0]);
+      write_line(to + p * apart + 32 * kLineBytes, w[1]);
     }
   } else {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) rest[q] = x[q], rest[8 + q] = y[q];
 #pragma unroll 1
     for (int p = 0; p < 3; ++p) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const u32 low = next_part(kept[2 * q]);
-        w[q] = low | next_part(kept[2 * q + 1]) << 16;
+      for (int q = 0; q < 8; ++q) {
+        const u32 low = next_part(rest[2 * q]);
+        w[q / 4][q % 4] = low | next_part(rest[2 * q + 1]) << 16;
       }
-      write_line(to + p * apart, w);
+      write_line(to + p * apart, w[0]);
+      write_line(to + p * apart + 32 * kLineBytes, w[1]);
     }
   }
 }
@@ -455,10 +457,11 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
         if (!__all_sync(0xffffffffu, free)) break;
         const u32 at = stages_at + stage * stage_bytes + place;
 #pragma unroll
-        for (int j = 0; j < kPieces; ++j) {
+        for (int j = 0; j < kPieces; j += 2) {
           const bool of_grad = GRAD && j >= 4;
-          write_parts(v[j], at + (of_grad ? PARTS * kRowsOperand + (j - 4) * 32 * kLineBytes : j * 32 * kLineBytes), of_grad ? b_bytes : kRowsOperand);
+          write_parts(v[j], v[j + 1], at + (of_grad ? PARTS * kRowsOperand : j * 32 * kLineBytes), of_grad ? b_bytes : kRowsOperand);
           read(j, v[j]);
+          read(j + 1, v[j + 1]);
         }
         go_on();
         __syncwarp();
