@@ -52,6 +52,7 @@ struct TileArgs {
   bool by_tma;               // results may leave by TMA
   float* partial;            // gradient: sums of the chunks (null: one chunk per expert, written out)
   const float *row_scales, *weight_scales;  // of 8-bit operands
+  u64 wait_limit;            // ns
   u32 how;
 };
 
@@ -281,7 +282,7 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
   const u32 rank = rank_in_pair();
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   const Groups& g = a.groups;
-  i64* const counters = g.counters;
+  const Patience patience{a.wait_limit, &stop, g.counters};
 
   if (threadIdx.x == 0) {
     stop = 0;
@@ -330,7 +331,7 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
       const bool both = tile.rows > 128, rows_here = rank == 0 || both;
       const u32 loaded_bytes = PARTS * ((GRAD ? 2 : READ ? 0 : both ? 2 : 1) * kRowsOperand + 2 * b_bytes);
       for (u32 b = 0; b < tile.blocks; ++b) {
-        if (!barrier_wait(empty + 8 * stage, turn ^ 1, &stop, counters)) goto loaded;
+        if (!barrier_wait(empty + 8 * stage, turn ^ 1, patience)) goto loaded;
         if (rank == 0) barrier_expect(full + 8 * stage, loaded_bytes);
         const u32 at = stages_at + stage * stage_bytes, bar = full_of_first + 8 * stage;
 #pragma unroll
@@ -360,10 +361,10 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
       const u32 blocks = tile_at<GRAD, kPerLine>(a, plan, t).blocks;
       for (u32 b0 = 0; b0 < blocks; b0 += min(kDrain, blocks - b0), ++made) {
         const u32 buffer = made & 1, to = sums + buffer * 256;
-        if (!barrier_wait(sums_empty + 8 * buffer, (made >> 1 & 1) ^ 1, &stop, counters)) goto issued;
+        if (!barrier_wait(sums_empty + 8 * buffer, (made >> 1 & 1) ^ 1, patience)) goto issued;
         sums_fence_after();
         for (u32 b = b0; b < b0 + min(kDrain, blocks - b0); ++b) {
-          if (!barrier_wait(full + 8 * stage, turn, &stop, counters)) goto issued;
+          if (!barrier_wait(full + 8 * stage, turn, patience)) goto issued;
           sums_fence_after();
           const u32 at = stages_at + stage * stage_bytes;
           const u64 op_a = operand(at, kAcross), op_b = operand(at + PARTS * kRowsOperand, kAcross);
@@ -395,7 +396,7 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
     for (u64 t = first; t < tiles; t += step) {
       const u32 blocks = tile_at<GRAD, kPerLine>(a, plan, t).blocks;
       for (u32 b = 0; b < blocks; ++b) {
-        if (!barrier_wait(written + 8 * stage, turn, &stop, counters)) goto handed_over;
+        if (!barrier_wait(written + 8 * stage, turn, patience)) goto handed_over;
         written_for_tensor_cores();
         barrier_arrive_at(full_of_first + 8 * stage);
         if (++stage == (u32)a.stages) stage = 0, turn ^= 1;
@@ -453,7 +454,7 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
       for (int j = 0; j < kPieces; ++j) read(j, v[j]);
       go_on();
       while (now.t < tiles) {
-        const bool free = barrier_wait(empty + 8 * stage, turn ^ 1, &stop, counters);
+        const bool free = barrier_wait(empty + 8 * stage, turn ^ 1, patience);
         if (!__all_sync(0xffffffffu, free)) break;
         const u32 at = stages_at + stage * stage_bytes + place;
 #pragma unroll
@@ -483,7 +484,7 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
       auto valid_of = [&](const RawRows& x, u32 c) { return c < x.width ? min(2u, x.width - c) : 0; };
       bool lost = false;
       while (now.t < tiles) {
-        const bool free = barrier_wait(empty + 8 * stage, turn ^ 1, &stop, counters);
+        const bool free = barrier_wait(empty + 8 * stage, turn ^ 1, patience);
         if (!__all_sync(0xffffffffu, free)) {
           lost = true;
           break;
@@ -568,7 +569,7 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
           __syncwarp();
         }
         const u32 buffer = made & 1;
-        const bool there = barrier_wait(sums_full + 8 * buffer, made >> 1 & 1, &stop, counters);
+        const bool there = barrier_wait(sums_full + 8 * buffer, made >> 1 & 1, patience);
         if (!__all_sync(0xffffffffu, there)) break;
         sums_fence_after();
         for (u32 c = 0; c < half; c += 32) {
@@ -595,7 +596,7 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
         bool lost = false;
         for (u32 b0 = 0; b0 < tile.blocks; b0 += min(kDrain, tile.blocks - b0), ++made) {
           const u32 buffer = made & 1;
-          const bool there = barrier_wait(sums_full + 8 * buffer, made >> 1 & 1, &stop, counters);
+          const bool there = barrier_wait(sums_full + 8 * buffer, made >> 1 & 1, patience);
           if (!__all_sync(0xffffffffu, there)) {
             lost = true;
             break;
@@ -739,6 +740,8 @@ __global__ void __launch_bounds__(256) k_into_lines(const T* __restrict__ from, 
 // ---- host ------------------------------------------------------------------------------------------------------------------------
 static i64 rounded(i64 bytes) { return (bytes + 255) / 256 * 256; }
 
+constexpr i64 kMostStride = (i64)1 << 40;  // bytes that a description for TMA can hold
+
 // An operand as the kernel reads it: `matrices` of `height` lines of `width` values, neighbours in memory.
 struct Lines {
   const void* at;
@@ -747,7 +750,7 @@ struct Lines {
   bool copied() const {
     const int size = value_bytes(dtype);
     return dtype == GSB_F32 || !aligned_to(16, (const char*)at) || (height > 1 && (stride * size % 16 != 0 || stride == 0)) ||
-           (matrices > 1 && matrix_stride * size % 16 != 0);
+           (matrices > 1 && matrix_stride * size % 16 != 0) || (height > 1 && stride >= kMostStride / size) || (matrices > 1 && matrix_stride >= kMostStride / size);
   }
   i64 parts() const { return dtype == GSB_F32 ? 3 : 1; }
   i64 to_stride() const { return (width + 7) / 8 * 8; }
@@ -783,7 +786,7 @@ static int describe(const Lines& x, int size, u32 box_along, u32 box_lines, bool
   const u64 dims4[4] = {(u64)x.width, (u64)x.height, (u64)x.copies(), (u64)x.parts()}, strides4[3] = {(u64)lines, (u64)step, (u64)part};
   const u64 dims3[3] = {(u64)x.width, (u64)x.height, (u64)x.parts()}, strides3[2] = {(u64)lines, (u64)part};
   const u32 box[4] = {box_along, box_lines, 1, 1};
-  if (lines >= (i64)1 << 40 || step >= (i64)1 << 40 || part >= (i64)1 << 40) return GSB_ERR_UNSUPPORTED;
+  if (step >= kMostStride || part >= kMostStride) return GSB_ERR_UNSUPPORTED;
   return describe_array(map, x.at, size, matrices ? 4 : 3, matrices ? dims4 : dims3, matrices ? strides4 : strides3, box) ? GSB_OK : GSB_ERR_UNSUPPORTED;
 }
 
@@ -808,6 +811,8 @@ static int by_experts(gsb_ctx* ctx, i64 num_experts, i64 num_rows, const int64_t
 
 // Shared memory for stages: what the fixed part (the plan, the scales, the ways out) leaves, and what is lost to their alignment.
 constexpr int stages_room(int parts) { return (227 - 14) * 1024 - rooms_of(parts) * kWriters * kRoom - 1024; }
+// A wait is given up after GSB_OPT_MAX_POLLS of these: two seconds by default.
+constexpr u64 kNanosecondsPerPoll = 477;
 // Launches pairs of CTAs: at most one CTA per SM.  In the order of the stream, with no overlap of its neighbours' ends and beginnings: with
 // overlap, hundreds of copies and products queued one behind the other came to a halt, waiting CTAs of one kernel beside clusters of another
 // that need SMs as a whole.
@@ -817,6 +822,7 @@ static int launch_tiles(gsb_ctx* ctx, cudaStream_t stream, const CUtensorMap& ma
   const int stage = PARTS * (kRowsOperand + (int)a.columns / 2 * kLineBytes);
   a.stages = min(kMaxStages, stages_room(PARTS) / stage);
   a.how = instruction(WHOLE_NUMBERS ? OPERAND_S8 : std::is_same<T, __half>::value ? OPERAND_F16 : OPERAND_BF16, GRAD, GRAD || ACROSS, kPairRows, a.columns);
+  a.wait_limit = (u64)ctx_option(ctx, GSB_OPT_MAX_POLLS) * kNanosecondsPerPoll;
   const int smem = a.stages * stage + 1024;
   CUtensorMap map_out = {};
   const int size = a.partial ? 4 : (int)sizeof(T);
@@ -886,6 +892,10 @@ static i64 chunk_rows(i64 num_rows, i64 k, i64 n, u32 columns, i64 num_experts) 
   i64 chunk = (num_rows + wanted - 1) / wanted;
   if (num_experts >= wanted) chunk = num_rows;
   chunk = max(chunk, (i64)512);
+  // in tensor memory additions cut, by 2^-26 of the sum each: beyond so many rows a float16 would show it.  Where room for the chunks' sums
+  // is to be had; an expert of a million rows is 9e-4 off without
+  constexpr i64 kMostRows = 262144;
+  if (chunk > kMostRows && (min(num_experts, (i64)kPlanExperts) + num_rows / kMostRows) * k * n * 4 <= (i64)1 << 30) chunk = kMostRows;
   return min((chunk + 63) / 64 * 64, ((num_rows + 63) / 64) * 64);
 }
 static i64 most_chunks(i64 num_rows, i64 chunk, i64 num_experts) { return min(num_experts, (i64)kPlanExperts) + num_rows / max((i64)1, chunk); }

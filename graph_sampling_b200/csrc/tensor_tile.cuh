@@ -56,29 +56,34 @@ __device__ __forceinline__ bool barrier_try(u32 bar, u32 parity) {
 // What was written to shared memory before is seen by matrix instructions that are issued behind a barrier this thread arrives at next.
 __device__ __forceinline__ void written_for_tensor_cores() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// A wait that lasts for two seconds is given up: the CTA notes it in `stop`, its other waits end too, and the error is recorded.
-constexpr u64 kWaitLimit = 2000000000ull;
+// How long a wait may last, in nanoseconds, and what one that lasts longer does: the CTA notes it in `stop`, its other waits end too, and the
+// error is recorded.
+struct Patience {
+  u64 limit;
+  volatile int* stop;
+  i64* counters;
+};
 __device__ __forceinline__ u64 nanoseconds() {
   u64 t;
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
   return t;
 }
-static __device__ __noinline__ bool barrier_wait_long(u32 bar, u32 parity, volatile int* stop, i64* counters) {
+static __device__ __noinline__ bool barrier_wait_long(u32 bar, u32 parity, Patience p) {
   const u64 start = nanoseconds();
   while (!barrier_try(bar, parity)) {
-    if (*stop) return false;
-    if (nanoseconds() - start > kWaitLimit) {
-      *stop = 1;
-      raise_error(counters, GSB_ERR_LOOKBACK_TIMEOUT, blockIdx.x);
+    if (*p.stop) return false;
+    if (nanoseconds() - start > p.limit) {
+      *p.stop = 1;
+      raise_error(p.counters, GSB_ERR_LOOKBACK_TIMEOUT, blockIdx.x);
       return false;
     }
   }
   return true;
 }
-__device__ __forceinline__ bool barrier_wait(u32 bar, u32 parity, volatile int* stop, i64* counters) {
+__device__ __forceinline__ bool barrier_wait(u32 bar, u32 parity, const Patience& p) {
   for (int i = 0; i < 16; ++i)
     if (barrier_try(bar, parity)) return true;
-  return barrier_wait_long(bar, parity, stop, counters);
+  return barrier_wait_long(bar, parity, p);
 }
 
 // ---- tiles by TMA ----
