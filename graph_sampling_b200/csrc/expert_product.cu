@@ -141,33 +141,27 @@ __device__ __forceinline__ void write_rows(Exit<ROOMS>& exit, int lane, const fl
 }
 
 // ---- rows read by warps: rows of any address and distance, and float32, which is taken apart on the way ----------------------------
-// 16-bit values: a warp copies a line at a time, two neighbouring values a lane, straight to where they belong; every eighth line of an
-// operand, `lines` of them with values, the others zeros.  `valid`: of the lane's two columns;
-// `some`: an address in the array, for what is not read.
-template <int LINES>
-__device__ __forceinline__ void copy_lines(u32 to, const unsigned short* from, i64 step, int lines, u32 valid, bool aligned, const void* some) {
+// 16-bit values: a warp reads a line at a time, two neighbouring values a lane: every eighth line of an operand, `lines` of them with values, the
+// others zeros, into LINES words from FIRST on.  `valid`: of the lane's two columns; `aligned`: they are one word.
+template <int FIRST, int LINES, int WORDS>
+__device__ __forceinline__ void read_lines(u32 (&v)[WORDS], const unsigned short* from, i64 step, int lines, int valid, bool aligned) {
   if (aligned && valid != 1) {
-    const u32 bytes = 2 * valid;
-    if (valid == 0) lines = 0;
+    if (valid <= 0) lines = 0;
 #pragma unroll
-    for (int i = 0; i < LINES; ++i, from += step) {
-      const bool in = i < lines;
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + i * 8 * kLineBytes), "l"(in ? from : (const unsigned short*)some), "r"(in ? bytes : 0) : "memory");
-    }
+    for (int i = 0; i < LINES; ++i, from += step) v[FIRST + i] = i < lines ? __ldg((const u32*)from) : 0;
   } else {
 #pragma unroll
-    for (int i0 = 0; i0 < LINES; i0 += 8) {
-      u32 w[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i, from += step) {
-        const bool in = i0 + i < lines;
-        w[i] = in && valid > 0 ? __ldg(from) : 0;
-        w[i] |= in && valid > 1 ? (u32)__ldg(from + 1) << 16 : 0;
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) asm volatile("st.shared.b32 [%0], %1;" ::"r"(to + (i0 + i) * 8 * kLineBytes), "r"(w[i]) : "memory");
+    for (int i = 0; i < LINES; ++i, from += step) {
+      const u32 low = i < lines && valid > 0 ? __ldg(from) : 0, high = i < lines && valid > 1 ? __ldg(from + 1) : 0;
+      v[FIRST + i] = low | high << 16;
     }
   }
+}
+// To lines 8 apart.
+template <int FIRST, int LINES, int WORDS>
+__device__ __forceinline__ void write_lines(const u32 (&v)[WORDS], u32 to) {
+#pragma unroll
+  for (int i = 0; i < LINES; ++i) asm volatile("st.shared.b32 [%0], %1;" ::"r"(to + i * 8 * kLineBytes), "r"(v[FIRST + i]) : "memory");
 }
 __device__ __forceinline__ void write_line(u32 to, const u32 (&w)[4]) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
@@ -187,10 +181,6 @@ __device__ __forceinline__ void read_eight(const float* from, int valid, int uni
     for (int q = 0; q < 8; ++q) v[q] = q < valid ? __ldg(from + q) : 0.f;
   }
 }
-__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int LEFT>
-__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
-
 // The next part of a float32 value, and what is left of it.  To nearest, but the largest numbers downwards, where that would be infinity.
 // Infinities and NaN are all in the first part.
 __device__ __forceinline__ u32 next_part(float& rest) {
@@ -326,10 +316,10 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
         }
       }
       const int matrix = (g.first + tile.e) * a.expert_step;
-      // The second CTA's rows only where there are any: what else lies in its shared memory makes sums that nobody reads.  (Boxes of the 32 rows
-      // that a step has were slower than one of 128: 15.7 us for 14.1.)
-      const bool both = tile.rows > 128, rows_here = rank == 0 || both;
-      const u32 loaded_bytes = PARTS * ((GRAD ? 2 : READ ? 0 : both ? 2 : 1) * kRowsOperand + 2 * b_bytes);
+      // A second CTA without rows loads zeros from behind the array: no traffic, and products that cost the least power (1 to 2 % under the power
+      // limit).  (Boxes of the 32 rows that a step has were slower than one of 128: 15.7 us for 14.1.)
+      const int first_row = rank == 0 || tile.rows > 128 ? (int)(tile.row0 + rank * 128) : (int)g.num_rows;
+      const u32 loaded_bytes = 2 * PARTS * ((READ ? 0 : kRowsOperand) + b_bytes);
       for (u32 b = 0; b < tile.blocks; ++b) {
         if (!barrier_wait(empty + 8 * stage, turn ^ 1, patience)) goto loaded;
         if (rank == 0) barrier_expect(full + 8 * stage, loaded_bytes);
@@ -342,7 +332,7 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
             for (u32 j = 0; j < half / 64; ++j)
               load_tile(to_b + j * kAcross, of_b, bar, (int)(tile.n0 + rank * half + j * 64), (int)(tile.row0 + b * 64), p);
           } else {
-            if (!READ && rows_here) load_tile(to_a, of_a, bar, (int)(b * kPerLine), (int)(tile.row0 + rank * 128), p);
+            if (!READ) load_tile(to_a, of_a, bar, (int)(b * kPerLine), first_row, p);
             if (ACROSS)
               for (u32 j = 0; j < half / 64; ++j)
                 load_tile(to_b + j * kAcross, of_b, bar, (int)(tile.n0 + rank * half + j * 64), (int)(b * kPerLine), matrix, p);
@@ -471,56 +461,63 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
         if (++stage == (u32)a.stages) stage = 0, turn ^= 1;
       }
     } else {
-      // warp w has lines w, w + 8 and so on; copies of kLag stages are on their way before the first is handed over
-      constexpr u32 kLag = 3;
+      // Warp w has lines w, w + 8 and so on; those of the next stages are on their way while it writes this one's, two stages of a product's rows
+      // or one of both operands of a gradient.  (200 003 rows of 602 to 100 take 106 us; of 608, which TMA loads, 58.  Asynchronous copies of four
+      // bytes a lane, and twice as many warps, took 111 and 109: lines that begin between 128-byte boundaries are what costs.)
+      constexpr int kWords = GRAD ? 32 : 16;
       const u32 w = me / 32, place = w * kLineBytes + (((lane >> 2) ^ w) << 4) + (lane & 3) * 4;
-      u32 handed = 0, copied = 0;
-      auto hand_over = [&] {
-        __syncwarp();
-        if (lane == 0) barrier_arrive(written + 8 * handed);
-        if (++handed == (u32)a.stages) handed = 0;
-      };
+      const bool aligned = a.rows.unit >= 4, grad_aligned = a.grad.unit >= 4;
+      Walk<GRAD, kPerLine> ahead = now;
       auto lines_of = [&](int rows) { return rows > (int)w ? (rows - (int)w + kReaders - 1) / kReaders : 0; };
-      auto valid_of = [&](const RawRows& x, u32 c) { return c < x.width ? min(2u, x.width - c) : 0; };
-      bool lost = false;
-      while (now.t < tiles) {
-        const bool free = barrier_wait(empty + 8 * stage, turn ^ 1, patience);
-        if (!__all_sync(0xffffffffu, free)) {
-          lost = true;
-          break;
-        }
-        const u32 at = stages_at + stage * stage_bytes + place;
-        const Tile& tile = now.tile;
-        const bool aligned = a.rows.unit >= 4, grad_aligned = a.grad.unit >= 4;
-        if (GRAD) {
-          const i64 row = first_row(tile) + now.b * 64 + w;
-          const int lines = lines_of(rows_here(tile) - (int)now.b * 64);
-          const unsigned short* from = (const unsigned short*)a.rows.at + row * a.rows.stride;
-          const unsigned short* from_grad = (const unsigned short*)a.grad.at + row * a.grad.stride;
-          for (u32 j = 0; j < 128; j += 64) {
-            const u32 c = tile.m0 + rank * 128 + j + lane * 2;
-            copy_lines<8>(at + j * kLineBytes, from + c, kReaders * a.rows.stride, lines, valid_of(a.rows, c), aligned, a.rows.at);
-          }
-          for (u32 j = 0; j < half; j += 64) {
-            const u32 c = tile.n0 + rank * half + j + lane * 2;
-            copy_lines<8>(at + kRowsOperand + j * kLineBytes, from_grad + c, kReaders * a.grad.stride, lines, valid_of(a.grad, c), grad_aligned, a.grad.at);
-          }
+      auto fetch = [&](u32(&v)[kWords]) {
+        if (ahead.t >= tiles) return;
+        const Tile& tile = ahead.tile;
+        const i64 step_of_rows = kReaders * a.rows.stride;
+        if constexpr (GRAD) {
+          const i64 row = first_row(tile) + ahead.b * 64 + w;
+          const int lines = lines_of(rows_here(tile) - (int)ahead.b * 64);
+          const u32 c = tile.m0 + rank * 128 + lane * 2, d = tile.n0 + rank * half + lane * 2;
+          const unsigned short* from = (const unsigned short*)a.rows.at + row * a.rows.stride + c;
+          const unsigned short* from_grad = (const unsigned short*)a.grad.at + row * a.grad.stride + d;
+          read_lines<0, 8>(v, from, step_of_rows, lines, (int)a.rows.width - (int)c, aligned);
+          read_lines<8, 8>(v, from + 64, step_of_rows, lines, (int)a.rows.width - (int)c - 64, aligned);
+          read_lines<16, 8>(v, from_grad, kReaders * a.grad.stride, lines, (int)a.grad.width - (int)d, grad_aligned);
+          if (half > 64) read_lines<24, 8>(v, from_grad + 64, kReaders * a.grad.stride, lines, (int)a.grad.width - (int)d - 64, grad_aligned);
         } else {
-          const u32 c = now.b * 64 + lane * 2;
-          copy_lines<16>(at, (const unsigned short*)a.rows.at + (first_row(tile) + w) * a.rows.stride + c, kReaders * a.rows.stride,
-                         lines_of(rows_here(tile)), valid_of(a.rows, c), aligned, a.rows.at);
+          const u32 c = ahead.b * 64 + lane * 2;
+          const unsigned short* from = (const unsigned short*)a.rows.at + (first_row(tile) + w) * a.rows.stride + c;
+          read_lines<0, 16>(v, from, step_of_rows, lines_of(rows_here(tile)), (int)a.rows.width - (int)c, aligned);
         }
-        copies_end();
-        if (++copied > kLag) {
-          copies_wait<kLag>();
-          hand_over();
+        ahead.next(a, plan, tiles, step);
+      };
+      auto turn_over = [&](u32(&v)[kWords]) {  // false: nothing is left, or the wait was given up
+        if (now.t >= tiles) return false;
+        const bool free = barrier_wait(empty + 8 * stage, turn ^ 1, patience);
+        if (!__all_sync(0xffffffffu, free)) return false;
+        const u32 at = stages_at + stage * stage_bytes + place;
+        write_lines<0, 16>(v, at);
+        if constexpr (GRAD) {
+          write_lines<16, 8>(v, at + kRowsOperand);
+          if (half > 64) write_lines<24, 8>(v, at + kRowsOperand + kAcross);
         }
+        __syncwarp();
+        if (lane == 0) barrier_arrive(written + 8 * stage);
+        fetch(v);
         now.next(a, plan, tiles, step);
         if (++stage == (u32)a.stages) stage = 0, turn ^= 1;
+        return true;
+      };
+      u32 v[kWords];
+      fetch(v);
+      if constexpr (GRAD) {
+        while (turn_over(v)) {
+        }
+      } else {
+        u32 second[kWords];
+        fetch(second);
+        while (turn_over(v) && turn_over(second)) {
+        }
       }
-      copies_wait<0>();
-      if (!lost)
-        for (u32 left = min(copied, kLag); left > 0; --left) hand_over();
     }
   } else if (warp >= 4 && warp < 4 + kWriters) {
     const u32 quarter = (u32)(warp & 3) * 32;
