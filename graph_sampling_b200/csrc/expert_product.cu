@@ -317,7 +317,7 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
       }
       const int matrix = (g.first + tile.e) * a.expert_step;
       // A second CTA without rows loads zeros from behind the array: no traffic, and products that cost the least power (1 to 2 % under the power
-      // limit).  (Boxes of the 32 rows that a step has were slower than one of 128: 15.7 us for 14.1.)
+      // limit).  (Boxes of the 32 rows that a step has, which leave the rest as it was, were slower than one of 128: 15.3 us for 14.0.)
       const int first_row = rank == 0 || tile.rows > 128 ? (int)(tile.row0 + rank * 128) : (int)g.num_rows;
       const u32 loaded_bytes = 2 * PARTS * ((READ ? 0 : kRowsOperand) + b_bytes);
       for (u32 b = 0; b < tile.blocks; ++b) {
@@ -847,8 +847,11 @@ static int launch_tiles(gsb_ctx* ctx, cudaStream_t stream, const CUtensorMap& ma
   return GSB_OK;
 }
 
-// Columns of a tile: narrow ones for narrow results (and for float32, whose parts need the room).
-static u32 tile_columns(i64 n, int dtype) { return dtype == GSB_F32 || n <= 128 ? 128 : 256; }
+// Columns of a tile: narrow ones for narrow results, for float32, whose parts need the room, and where wide ones would leave half of the pairs of
+// CTAs without any (512 rows of 512 to 512 by eight experts 9.7 us for 12.6).  `row_tiles`: how many there are down the result.
+static u32 tile_columns(i64 n, int dtype, i64 row_tiles) { return dtype == GSB_F32 || n <= 128 || row_tiles * ((n + 255) / 256) <= kNumSMs / 4 ? 128 : 256; }
+static i64 row_tiles_of(i64 num_rows, i64 num_experts) { return num_rows / kPairRows + min(num_rows, num_experts); }
+static i64 row_tiles_of_grad(i64 k, i64 num_experts) { return (k + kPairRows - 1) / kPairRows * num_experts; }
 
 static Lines rows_operand(const void* rows, int dtype, i64 num_rows, i64 width, i64 stride) { return Lines{rows, 1, 0, num_rows, stride, width, dtype}; }
 // The matrices with their rows (ACROSS) or their columns as lines, whichever are neighbours in memory.
@@ -969,7 +972,7 @@ extern "C" int gsb_expert_product(gsb_ctx* ctx, void* stream_, const void* rows,
   a.rows = raw_rows(x);
   a.depth = (u32)k;
   a.n = (u32)n;
-  a.columns = tile_columns(n, dtype);
+  a.columns = tile_columns(n, dtype, row_tiles_of(num_rows, num_experts));
   a.expert_step = w.copies() > 1;
   CUtensorMap map_x = {}, map_w;
   const bool read = x.copied();
@@ -993,7 +996,7 @@ extern "C" int64_t gsb_expert_product_grad_workspace(const void* rows, int dtype
   if (value_bytes(dtype) == 0 || num_rows < 0 || num_rows >= ((i64)1 << 31) || k < 1 || k > GSB_MAX_ROW_LEN || n < 1 || n > GSB_MAX_ROW_LEN ||
       num_experts < 1 || num_experts > GSB_MAX_EXPERTS)
     return GSB_ERR_INVALID_ARGUMENT;
-  const i64 chunk = chunk_rows(num_rows, k, n, tile_columns(n, dtype), num_experts);
+  const i64 chunk = chunk_rows(num_rows, k, n, tile_columns(n, dtype, row_tiles_of_grad(k, num_experts)), num_experts);
   if (few_grad(num_rows, k, n, num_experts, value_bytes(dtype), chunk < num_rows)) return 0;
   return rounded(min(num_experts, (i64)kPlanExperts) * 2 * (i64)sizeof(CUtensorMap)) + (chunk < num_rows ? rounded(most_chunks(num_rows, chunk, num_experts) * k * n * 4) : 0);
 }
@@ -1012,7 +1015,7 @@ extern "C" int gsb_expert_product_grad(gsb_ctx* ctx, void* stream_, const void* 
     GSB_CUDA_OK(cudaMemsetAsync(out, 0, (size_t)(num_experts * k * n * size), stream));
     return GSB_OK;
   }
-  if (few_grad(num_rows, k, n, num_experts, size, chunk_rows(num_rows, k, n, tile_columns(n, dtype), num_experts) < num_rows))
+  if (few_grad(num_rows, k, n, num_experts, size, chunk_rows(num_rows, k, n, tile_columns(n, dtype, row_tiles_of_grad(k, num_experts)), num_experts) < num_rows))
     return by_experts(ctx, num_experts, num_rows, offsets, [&](const Groups& g) {
       const FewArgs a{g, rows, grad, rows_stride, grad_stride, 0, (u32)k, (u32)n, nullptr, nullptr};
       const bool wide = aligned_to(16, (const char*)grad) && (num_rows == 1 || grad_stride * size % 16 == 0);
@@ -1037,7 +1040,7 @@ extern "C" int gsb_expert_product_grad(gsb_ctx* ctx, void* stream_, const void* 
   a.grad = raw_rows(d);
   a.k = (u32)k;
   a.n = (u32)n;
-  a.columns = tile_columns(n, dtype);
+  a.columns = tile_columns(n, dtype, row_tiles_of_grad(k, num_experts));
   const i64 chunk = chunk_rows(num_rows, k, n, a.columns, num_experts);
   a.chunk = (u32)chunk;
   a.maps = maps;
@@ -1100,7 +1103,7 @@ extern "C" int gsb_expert_product_int8(gsb_ctx* ctx, void* stream_, const int8_t
   TileArgs a = {};
   a.depth = (u32)k;
   a.n = (u32)n;
-  a.columns = tile_columns(n, GSB_F16);
+  a.columns = tile_columns(n, GSB_F16, row_tiles_of(num_rows, num_experts));
   a.expert_step = num_experts > 1;
   a.row_scales = scales;
   a.weight_scales = weight_scales;
