@@ -117,19 +117,26 @@ template <class U, int ROOMS>
 __device__ __forceinline__ void write_rows(Exit<ROOMS>& exit, int lane, const float (&v)[kStoreBytes / sizeof(U)], U* to, i64 pitch, u32 rows, u32 columns, int unit,
                                            const CUtensorMap* map, i64 row, u32 column) {
   constexpr int PER = 16 / sizeof(U);
-  char* const room = exit.rooms + exit.turn % ROOMS * kRoom;
-  ++exit.turn;
-  if (lane == 0) stores_read<ROOMS - 1>();
-  __syncwarp();
+  Unit<U, 16> w[4];
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
     float f[PER];
 #pragma unroll
     for (int q = 0; q < PER; ++q) f[q] = v[p * PER + q];
-    Unit<U, 16> w;
-    w.set(f);
-    *(uint4*)(room + lane * kStoreBytes + ((p ^ (lane >> 1 & 3)) << 4)) = w.w;
+    w[p].set(f);
   }
+  if (rows < 32 && unit == 16 && columns >= kStoreBytes / sizeof(U)) {  // each lane its row: for a few of them that is sooner
+    if ((u32)lane < rows)
+#pragma unroll
+      for (int p = 0; p < 4; ++p) store_unit((Unit<U, 16>*)(to + lane * pitch) + p, w[p]);
+    return;
+  }
+  char* const room = exit.rooms + exit.turn % ROOMS * kRoom;
+  ++exit.turn;
+  if (lane == 0) stores_read<ROOMS - 1>();
+  __syncwarp();
+#pragma unroll
+  for (int p = 0; p < 4; ++p) *(uint4*)(room + lane * kStoreBytes + ((p ^ (lane >> 1 & 3)) << 4)) = w[p].w;
   if (map && rows == 32) {
     written_for_tensor_cores();
     __syncwarp();
@@ -317,7 +324,8 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
       }
       const int matrix = (g.first + tile.e) * a.expert_step;
       // A second CTA without rows loads zeros from behind the array: no traffic, and products that cost the least power (1 to 2 % under the power
-      // limit).  (Boxes of the 32 rows that a step has, which leave the rest as it was, were slower than one of 128: 15.3 us for 14.0.)
+      // limit).  (Boxes of the 32 rows that a step has, which leave the rest as it was, were slower than one of 128: 64 rows to 64 experts 30 us
+      // for 27.)
       const int first_row = rank == 0 || tile.rows > 128 ? (int)(tile.row0 + rank * 128) : (int)g.num_rows;
       const u32 loaded_bytes = 2 * PARTS * ((READ ? 0 : kRowsOperand) + b_bytes);
       for (u32 b = 0; b < tile.blocks; ++b) {
@@ -874,14 +882,14 @@ static bool few_rows(i64 num_rows, i64 k, i64 n, i64 num_experts, int size, i64 
   const double weights = (double)min(num_rows, num_experts) * (double)k * (double)n * size / 4.5e6, chain = (double)k * size / 128. * 0.35;
   // the copy: read, written with its parts, and read again by the products
   const double copy = copied_bytes > 0 ? 3. + (double)copied_bytes * (size == 4 ? 10. / 6. : 2.) / 2.6e6 : 0.;
-  return few_time(num_rows, k, n, num_experts) < 7. + (weights > chain ? weights : chain) + copy;
+  return few_time(num_rows, k, n, num_experts) < 6. + (weights > chain ? weights : chain) + copy;
 }
 // The same of the weights' gradient.  Few rows: 3, one per 400 CTAs, and the rows that a CTA goes through (1 024 rows of 100 to 47 by three experts 7.5
-// us for 22; one row of 1 024 to 1 024 16 for 11.6; 4 096 of 64 to 64 by four 20 for 15, of floats 14 for 26).  Tiles: 9, or 15 with chunks, 8 more for float32.
+// us for 22; one row of 1 024 to 1 024 16 for 11.6; 4 096 of 64 to 64 by four 20 for 15, of floats 14 for 26).  Tiles: 8, or 14 with chunks, 8 more for float32.
 static bool few_grad(i64 num_rows, i64 k, i64 n, i64 num_experts, int size, bool chunks) {
   const double ctas = (double)num_experts * (double)((k + kFewRows - 1) / kFewRows) * (double)((n + kFewColumns - 1) / kFewColumns);
   const double few = 3. + ctas / 400. + (double)num_rows / (double)num_experts * 0.018;
-  return few < (chunks ? 15. : 9.) + (size == 4 ? 8. : 0.) + (double)num_experts * (double)k * (double)n * size / 3e6;
+  return few < (chunks ? 14. : 8.) + (size == 4 ? 8. : 0.) + (double)num_experts * (double)k * (double)n * size / 3e6;
 }
 static int few_grid(i64 tiles) { return (int)max((i64)1, min((i64)kNumSMs * 6, tiles)); }
 
