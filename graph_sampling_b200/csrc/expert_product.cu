@@ -72,9 +72,9 @@ __device__ __forceinline__ u64 number_of_tiles(const TileArgs& a, const PlanTabl
 template <bool GRAD, int PER_LINE>
 __device__ __forceinline__ Tile tile_at(const TileArgs& a, const PlanTable& plan, u64 t) {
   Tile r;
-  const u32 across = (a.n + a.columns - 1) / a.columns, down = GRAD ? (a.k + kPairRows - 1) / kPairRows : 1;
-  r.chunk = (u32)(t / (across * down));
-  const u32 rest = (u32)(t - (u64)r.chunk * (across * down));
+  const u32 across = (a.n + a.columns - 1) / a.columns, down = GRAD ? (a.k + kPairRows - 1) / kPairRows : 1, each = across * down;
+  r.chunk = t >> 32 ? (u32)(t / each) : (u32)t / each;
+  const u32 rest = (u32)(t - (u64)r.chunk * each);
   r.n0 = rest % across * a.columns;
   r.m0 = rest / across * kPairRows;
   r.e = expert_of_tile(plan, a.groups.experts, r.chunk);
@@ -83,6 +83,13 @@ __device__ __forceinline__ Tile tile_at(const TileArgs& a, const PlanTable& plan
   r.row0 = GRAD ? from : plan.begin[r.e] + from;
   r.blocks = ((GRAD ? r.rows : a.depth) + PER_LINE - 1) / PER_LINE;
   return r;
+}
+
+// The steps of a tile alone: all of a product's have the same.
+template <bool GRAD, int PER_LINE>
+__device__ __forceinline__ u32 blocks_at(const TileArgs& a, const PlanTable& plan, u64 t) {
+  if constexpr (GRAD) return tile_at<GRAD, PER_LINE>(a, plan, t).blocks;
+  else return (a.depth + PER_LINE - 1) / PER_LINE;
 }
 
 // 64 bytes of each of 32 rows of the result, a row a lane, leave through shared memory: by TMA where all 32 rows are wanted and begin on 16-byte
@@ -155,11 +162,11 @@ __device__ __forceinline__ void read_lines(u32 (&v)[WORDS], const unsigned short
   if (aligned && valid != 1) {
     if (valid <= 0) lines = 0;
 #pragma unroll
-    for (int i = 0; i < LINES; ++i, from += step) v[FIRST + i] = i < lines ? __ldg((const u32*)from) : 0;
+    for (int i = 0; i < LINES; ++i) v[FIRST + i] = i < lines ? __ldg((const u32*)(from + i * step)) : 0;
   } else {
 #pragma unroll
-    for (int i = 0; i < LINES; ++i, from += step) {
-      const u32 low = i < lines && valid > 0 ? __ldg(from) : 0, high = i < lines && valid > 1 ? __ldg(from + 1) : 0;
+    for (int i = 0; i < LINES; ++i) {
+      const u32 low = i < lines && valid > 0 ? __ldg(from + i * step) : 0, high = i < lines && valid > 1 ? __ldg(from + i * step + 1) : 0;
       v[FIRST + i] = low | high << 16;
     }
   }
@@ -356,7 +363,7 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
     constexpr bool A_ACROSS = GRAD, B_ACROSS = GRAD || ACROSS;
     u32 stage = 0, turn = 0, made = 0;
     for (u64 t = first; t < tiles; t += step) {
-      const u32 blocks = tile_at<GRAD, kPerLine>(a, plan, t).blocks;
+      const u32 blocks = blocks_at<GRAD, kPerLine>(a, plan, t);
       for (u32 b0 = 0; b0 < blocks; b0 += min(kDrain, blocks - b0), ++made) {
         const u32 buffer = made & 1, to = sums + buffer * 256;
         if (!barrier_wait(sums_empty + 8 * buffer, (made >> 1 & 1) ^ 1, patience)) goto issued;
@@ -392,7 +399,7 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
     const u32 full_of_first = address_in(full, 0);
     u32 stage = 0, turn = 0;
     for (u64 t = first; t < tiles; t += step) {
-      const u32 blocks = tile_at<GRAD, kPerLine>(a, plan, t).blocks;
+      const u32 blocks = blocks_at<GRAD, kPerLine>(a, plan, t);
       for (u32 b = 0; b < blocks; ++b) {
         if (!barrier_wait(written + 8 * stage, turn, patience)) goto handed_over;
         written_for_tensor_cores();
@@ -405,8 +412,8 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
     // All readers take a stage together; what comes next is on its way while they write
     const u32 me = threadIdx.x - 32 * kFirstReader;
     u32 stage = 0, turn = 0;
-    Walk<GRAD, kPerLine> now{first, 0, {}};
-    now.settle(a, plan, tiles, step);
+    Walk<GRAD, kPerLine> ahead{first, 0, {}};  // what is read next
+    ahead.settle(a, plan, tiles, step);
     // first of a tile's rows that the reduced index runs over (gradient), or of this CTA's (product)
     auto first_row = [&](const Tile& tile) { return GRAD ? (i64)plan.begin[tile.e] + tile.row0 : (i64)tile.row0 + rank * 128; };
     auto rows_here = [&](const Tile& tile) { return GRAD ? (int)tile.rows : (int)tile.rows - (int)rank * 128; };
@@ -416,7 +423,6 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
       // rows of 256 to 256 values.)
       constexpr int kPieces = GRAD ? 6 : 4;
       const u32 chunk = lane & 7, segment = me / 32 * 4 + lane / 8, place = segment * kLineBytes + ((chunk ^ (segment & 7)) << 4);
-      Walk<GRAD, kPerLine> ahead = now;
       const float *from = nullptr, *from_grad = nullptr;
       int columns = 0, grad_columns = 0, rows_left = 0;  // from this lane's first on
       auto begin_tile = [&] {
@@ -450,8 +456,9 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
       };
 #pragma unroll
       for (int j = 0; j < kPieces; ++j) read(j, v[j]);
+      bool left = ahead.t < tiles;
       go_on();
-      while (now.t < tiles) {
+      while (left) {
         const bool free = barrier_wait(empty + 8 * stage, turn ^ 1, patience);
         if (!__all_sync(0xffffffffu, free)) break;
         const u32 at = stages_at + stage * stage_bytes + place;
@@ -462,44 +469,57 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
           read(j, v[j]);
           read(j + 1, v[j + 1]);
         }
-        go_on();
         __syncwarp();
         if (lane == 0) barrier_arrive(written + 8 * stage);
-        now.next(a, plan, tiles, step);
+        left = ahead.t < tiles;
+        go_on();
         if (++stage == (u32)a.stages) stage = 0, turn ^= 1;
       }
     } else {
       // Warp w has lines w, w + 8 and so on; those of the next stages are on their way while it writes this one's, two stages of a product's rows
       // or one of both operands of a gradient.  (200 003 rows of 602 to 100 take 106 us; of 608, which TMA loads, 58.  Asynchronous copies of four
-      // bytes a lane, and twice as many warps, took 111 and 109: lines that begin between 128-byte boundaries are what costs.)
+      // bytes a lane, and twice as many warps, took 111 and 109: two requests for each line that begins between 128-byte boundaries, of which
+      // L1 has so many on their way and no more.)
       constexpr int kWords = GRAD ? 32 : 16;
       const u32 w = me / 32, place = w * kLineBytes + (((lane >> 2) ^ w) << 4) + (lane & 3) * 4;
       const bool aligned = a.rows.unit >= 4, grad_aligned = a.grad.unit >= 4;
-      Walk<GRAD, kPerLine> ahead = now;
       auto lines_of = [&](int rows) { return rows > (int)w ? (rows - (int)w + kReaders - 1) / kReaders : 0; };
-      auto fetch = [&](u32(&v)[kWords]) {
-        if (ahead.t >= tiles) return;
-        const Tile& tile = ahead.tile;
-        const i64 step_of_rows = kReaders * a.rows.stride;
+      const i64 rows_step = kReaders * a.rows.stride, grad_step = kReaders * a.grad.stride;
+      const unsigned short *from = nullptr, *from_grad = nullptr;
+      int columns = 0, grad_columns = 0, rows_left = 0;  // from this lane's first on
+      auto fetch = [&](u32(&v)[kWords]) {                // whether there was anything left
+        if (ahead.t >= tiles) return false;
+        if (ahead.b == 0) {
+          const Tile& tile = ahead.tile;
+          const u32 c = (GRAD ? tile.m0 + rank * 128 : 0) + lane * 2;
+          from = (const unsigned short*)a.rows.at + (first_row(tile) + w) * a.rows.stride + c;
+          columns = (int)a.rows.width - (int)c;
+          rows_left = rows_here(tile);
+          if (GRAD) {
+            const u32 d = tile.n0 + rank * half + lane * 2;
+            from_grad = (const unsigned short*)a.grad.at + (first_row(tile) + w) * a.grad.stride + d;
+            grad_columns = (int)a.grad.width - (int)d;
+          }
+        }
+        const int lines = lines_of(rows_left);
         if constexpr (GRAD) {
-          const i64 row = first_row(tile) + ahead.b * 64 + w;
-          const int lines = lines_of(rows_here(tile) - (int)ahead.b * 64);
-          const u32 c = tile.m0 + rank * 128 + lane * 2, d = tile.n0 + rank * half + lane * 2;
-          const unsigned short* from = (const unsigned short*)a.rows.at + row * a.rows.stride + c;
-          const unsigned short* from_grad = (const unsigned short*)a.grad.at + row * a.grad.stride + d;
-          read_lines<0, 8>(v, from, step_of_rows, lines, (int)a.rows.width - (int)c, aligned);
-          read_lines<8, 8>(v, from + 64, step_of_rows, lines, (int)a.rows.width - (int)c - 64, aligned);
-          read_lines<16, 8>(v, from_grad, kReaders * a.grad.stride, lines, (int)a.grad.width - (int)d, grad_aligned);
-          if (half > 64) read_lines<24, 8>(v, from_grad + 64, kReaders * a.grad.stride, lines, (int)a.grad.width - (int)d - 64, grad_aligned);
+          read_lines<0, 8>(v, from, rows_step, lines, columns, aligned);
+          read_lines<8, 8>(v, from + 64, rows_step, lines, columns - 64, aligned);
+          read_lines<16, 8>(v, from_grad, grad_step, lines, grad_columns, grad_aligned);
+          if (half > 64) read_lines<24, 8>(v, from_grad + 64, grad_step, lines, grad_columns - 64, grad_aligned);
+          from += 8 * rows_step;
+          from_grad += 8 * grad_step;
+          rows_left -= 64;
         } else {
-          const u32 c = ahead.b * 64 + lane * 2;
-          const unsigned short* from = (const unsigned short*)a.rows.at + (first_row(tile) + w) * a.rows.stride + c;
-          read_lines<0, 16>(v, from, step_of_rows, lines_of(rows_here(tile)), (int)a.rows.width - (int)c, aligned);
+          read_lines<0, 16>(v, from, rows_step, lines, columns, aligned);
+          from += 64;
+          columns -= 64;
         }
         ahead.next(a, plan, tiles, step);
+        return true;
       };
-      auto turn_over = [&](u32(&v)[kWords]) {  // false: nothing is left, or the wait was given up
-        if (now.t >= tiles) return false;
+      auto turn_over = [&](u32(&v)[kWords], bool& there) {  // false: nothing is left, or the wait was given up
+        if (!there) return false;
         const bool free = barrier_wait(empty + 8 * stage, turn ^ 1, patience);
         if (!__all_sync(0xffffffffu, free)) return false;
         const u32 at = stages_at + stage * stage_bytes + place;
@@ -510,20 +530,19 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
         }
         __syncwarp();
         if (lane == 0) barrier_arrive(written + 8 * stage);
-        fetch(v);
-        now.next(a, plan, tiles, step);
+        there = fetch(v);
         if (++stage == (u32)a.stages) stage = 0, turn ^= 1;
         return true;
       };
       u32 v[kWords];
-      fetch(v);
+      bool there = fetch(v);
       if constexpr (GRAD) {
-        while (turn_over(v)) {
+        while (turn_over(v, there)) {
         }
       } else {
         u32 second[kWords];
-        fetch(second);
-        while (turn_over(v) && turn_over(second)) {
+        bool second_there = fetch(second);
+        while (turn_over(v, there) && turn_over(second, second_there)) {
         }
       }
     }
