@@ -49,21 +49,84 @@ struct Largest {
       for (int i = 0; i < Unit<T, BYTES>::N; ++i) bits = max(bits, __float_as_uint(f[i]) & 0x7fffffffu);
     }
   }
-  // of all lanes; NaN where one is an infinity or NaN
-  __device__ __forceinline__ float of_warp() {
-    u32 most = bits;
+  // of all lanes, or of `lanes` neighbouring ones; NaN where one is an infinity or NaN
+  __device__ __forceinline__ float of_warp() const { return checked(__reduce_max_sync(0xffffffffu, as_float())); }
+  __device__ __forceinline__ float of_lanes(int lanes) const {
+    u32 most = as_float();
+    for (int o = lanes / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+    return checked(most);
+  }
+
+ private:
+  __device__ __forceinline__ u32 as_float() const {
     if constexpr (kWords) {
       const u32 half = max(bits & 0xffffu, bits >> 16);
-      most = __float_as_uint(std::is_same<T, __half>::value ? __half2float(__ushort_as_half((unsigned short)half)) : __uint_as_float(half << 16));
+      return __float_as_uint(std::is_same<T, __half>::value ? __half2float(__ushort_as_half((unsigned short)half)) : __uint_as_float(half << 16)) & 0x7fffffffu;
+    } else {
+      return bits;
     }
-    most = __reduce_max_sync(0xffffffffu, most & 0x7fffffffu);
-    return __uint_as_float(most >= 0x7f800000u ? 0x7fffffffu : most);
   }
+  static __device__ __forceinline__ float checked(u32 most) { return __uint_as_float(most >= 0x7f800000u ? 0x7fffffffu : most); }
 };
+
+__device__ __forceinline__ float inverse_of(float scale) { return scale > 1e-30f ? __fdiv_rn(1.f, scale) : __int_as_float(0x7fffffff); }
+// PACKED: the N values of a unit are written as one word.
+template <bool PACKED, class T, int BYTES>
+__device__ __forceinline__ void put(const Unit<T, BYTES>& unit, int8_t* to, float scale, float inverse) {
+  constexpr int N = Unit<T, BYTES>::N;
+  float f[N];
+  int q[N];
+  unit.get(f);
+  quantized(f, scale, inverse, q);
+  if constexpr (PACKED && N == 2) {
+    __stcs((unsigned short*)to, (unsigned short)__byte_perm(q[0], q[1], 0x0040));
+  } else if constexpr (PACKED) {
+    u32 w[N / 4];
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i)
+      w[i] = __byte_perm(__byte_perm(q[4 * i], q[4 * i + 1], 0x0040), __byte_perm(q[4 * i + 2], q[4 * i + 3], 0x0040), 0x5410);
+    if constexpr (N == 8) __stcs((uint2*)to, make_uint2(w[0], w[1]));
+    else __stcs((u32*)to, w[0]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) to[i] = (int8_t)q[i];
+  }
+}
+
+// Short rows: `lanes` neighbouring lanes (a power of two) take a row, kSteps units each, and kRows rows at a time.
+constexpr int kShortRows = 4, kShortSteps = 2;
+template <class T, int BYTES, bool PACKED>
+__global__ void __launch_bounds__(kQuantThreads) k_quantize_short(const Unit<T, BYTES>* __restrict__ x, i64 x_stride, int units, int lanes, u32 num_rows,
+                                                                  int8_t* __restrict__ values, i64 values_stride, float* __restrict__ scales) {
+  constexpr int N = Unit<T, BYTES>::N;
+  await_previous();
+  const int lane = threadIdx.x & (lanes - 1);
+  const u32 groups = kQuantThreads / lanes, first = blockIdx.x * groups * kShortRows + threadIdx.x / lanes;
+  Unit<T, BYTES> v[kShortRows][kShortSteps];
+#pragma unroll
+  for (int r = 0; r < kShortRows; ++r)
+#pragma unroll
+    for (int s = 0; s < kShortSteps; ++s) {
+      v[r][s].clear();
+      if (first + r * groups < num_rows && lane + s * lanes < units) v[r][s] = load_unit_once(x + (i64)(first + r * groups) * x_stride + lane + s * lanes);
+    }
+#pragma unroll
+  for (int r = 0; r < kShortRows; ++r) {
+    const u32 row = first + r * groups;
+    Largest<T, BYTES> largest;
+#pragma unroll
+    for (int s = 0; s < kShortSteps; ++s) largest.look(v[r][s]);
+    const float scale = __fdiv_rn(largest.of_lanes(lanes), 127.f), inverse = inverse_of(scale);
+    if (row >= num_rows) continue;
+    if (lane == 0) scales[row] = scale;
+#pragma unroll
+    for (int s = 0; s < kShortSteps; ++s)
+      if (lane + s * lanes < units) put<PACKED>(v[r][s], values + (i64)row * values_stride + (i64)(lane + s * lanes) * N, scale, inverse);
+  }
+}
 
 // A warp takes a row.  Its first kHeld units stay in shared memory between the search for the largest value and the division (in registers
 // the unrolled divisions were more code than the instruction cache holds: 65 536 rows of 2 048 bf16 took 184 us).
-// PACKED: the N values of a unit are written as one word.
 constexpr int kHeld = 256;
 template <class T, int BYTES, bool PACKED>
 __global__ void __launch_bounds__(kQuantThreads) k_quantize_rows(const Unit<T, BYTES>* __restrict__ x, i64 x_stride, int units, u32 num_rows,
@@ -92,7 +155,7 @@ __global__ void __launch_bounds__(kQuantThreads) k_quantize_rows(const Unit<T, B
       }
     }
     const float scale = __fdiv_rn(largest.of_warp(), 127.f);
-    const float inverse = scale > 1e-30f ? __fdiv_rn(1.f, scale) : __int_as_float(0x7fffffff);
+    const float inverse = inverse_of(scale);
     if (lane == 0) scales[r] = scale;
     int8_t* const to_row = values + (i64)r * values_stride;
 #pragma unroll 2
@@ -100,22 +163,7 @@ __global__ void __launch_bounds__(kQuantThreads) k_quantize_rows(const Unit<T, B
       U unit;
       if (j < kHeld) unit.w = held[j];
       else unit = load_unit(row + j);
-      float f[N];
-      int q[N];
-      unit.get(f);
-      quantized(f, scale, inverse, q);
-      int8_t* to = to_row + (i64)j * N;
-      if constexpr (PACKED) {
-        u32 w[N / 4];
-#pragma unroll
-        for (int i = 0; i < N / 4; ++i)
-          w[i] = __byte_perm(__byte_perm(q[4 * i], q[4 * i + 1], 0x0040), __byte_perm(q[4 * i + 2], q[4 * i + 3], 0x0040), 0x5410);
-        if constexpr (N == 8) __stcs((uint2*)to, make_uint2(w[0], w[1]));
-        else __stcs((u32*)to, w[0]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) to[i] = (int8_t)q[i];
-      }
+      put<PACKED>(unit, to_row + (i64)j * N, scale, inverse);
     }
   }
 }
@@ -139,12 +187,19 @@ extern "C" int gsb_quantize_rows(gsb_ctx* ctx, void* stream_, const void* x, int
   with_unit(dtype, unit, [&](auto value, auto bytes) {
     typedef decltype(value) T;
     constexpr int B = decltype(bytes)::value;
-    const int grid = grid_for(num_rows, kQuantThreads / 32);
     constexpr int N = B / (int)sizeof(T);
-    constexpr bool can = N == 4 || N == 8;
-    auto kernel = can && aligned_to(N, out_values) && values_stride % N == 0 ? k_quantize_rows<T, B, can> : k_quantize_rows<T, B, false>;
-    launch_behind(stream, kernel, grid, kQuantThreads, (const Unit<T, B>*)x, x_stride * size / B, (int)(row_len * size / B), (u32)num_rows,
-                  out_values, values_stride, out_scales);
+    constexpr bool can = N == 2 || N == 4 || N == 8;
+    const bool packed = can && aligned_to(N, out_values) && values_stride % N == 0;
+    const i64 units = row_len * size / B, stride = x_stride * size / B;
+    if (units <= 32 * kShortSteps) {  // 459 844 rows of 100 bf16 53 us, a warp a row 112; 500 000 of 64 floats 27 and 139
+      int lanes = 1;
+      while (lanes * kShortSteps < units) lanes *= 2;
+      launch_behind(stream, packed ? k_quantize_short<T, B, can> : k_quantize_short<T, B, false>, grid_for(num_rows, kQuantThreads / lanes * kShortRows),
+                    kQuantThreads, (const Unit<T, B>*)x, stride, (int)units, lanes, (u32)num_rows, out_values, values_stride, out_scales);
+    } else {
+      launch_behind(stream, packed ? k_quantize_rows<T, B, can> : k_quantize_rows<T, B, false>, grid_for(num_rows, kQuantThreads / 32), kQuantThreads,
+                    (const Unit<T, B>*)x, stride, (int)units, (u32)num_rows, out_values, values_stride, out_scales);
+    }
   });
   GSB_LAUNCH_OK();
   return GSB_OK;
