@@ -8,6 +8,7 @@
 // |a2| <= 2^-16 |a|, exactly (24 bits are 3 times 8), and a b is the sum of the six products a_i b_j with i + j <= 2: what is left out is
 // 2^-23 |a b| at the very most.
 #include <atomic>
+#include <initializer_list>
 #include <type_traits>
 
 #include "few_rows.cuh"
@@ -730,7 +731,7 @@ __global__ void __launch_bounds__(kAddThreads) k_add_chunks(const Groups g, u32 
 // Matrices whose rows do not begin on 16-byte boundaries are copied to where they do; float32 is cut into its parts, one array each.
 template <class T, int PARTS>
 __global__ void __launch_bounds__(256) k_into_lines(const T* __restrict__ from, i64 matrices, i64 matrix_stride, u32 height, i64 stride, u32 width,
-                                                    u32 to_stride, unsigned short* __restrict__ to) {
+                                                    u32 to_stride, int unit, unsigned short* __restrict__ to) {
   await_previous();
   const u32 pieces = to_stride / 8;
   const i64 count = matrices * height * pieces, plane = matrices * height * (i64)to_stride;
@@ -738,6 +739,18 @@ __global__ void __launch_bounds__(256) k_into_lines(const T* __restrict__ from, 
     const i64 line = i / pieces;
     const u32 x = (u32)(i - line * pieces) * 8;
     const T* row = from + line / height * matrix_stride + line % height * stride;
+    if (PARTS == 1 && unit >= 4 && x + 8 <= width) {
+      const u32* words = (const u32*)(row + x);
+      uint4 w;
+      if (unit >= 8) {
+        const uint2 low = __ldg((const uint2*)words), high = __ldg((const uint2*)words + 1);
+        w = make_uint4(low.x, low.y, high.x, high.y);
+      } else {
+        w = make_uint4(__ldg(words), __ldg(words + 1), __ldg(words + 2), __ldg(words + 3));
+      }
+      *(uint4*)(to + line * to_stride + x) = w;
+      continue;
+    }
     unsigned short v[PARTS][8];
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
@@ -789,13 +802,16 @@ static int bring(gsb_ctx* ctx, cudaStream_t stream, Lines* x, char** room) {
   *room += x->bytes();
   const i64 count = x->copies() * x->height * (x->to_stride() / 8);
   const int grid = (int)min((i64)kNumSMs * 16, (i64)grid_for(count, 256));
+  const int size = value_bytes(x->dtype);
+  const u64 strides = (u64)((x->height > 1 ? x->stride : 0) | (x->copies() > 1 ? x->matrix_stride : 0));
+  const int unit = unit_of((u64)(uintptr_t)x->at | strides * (u64)size);
   ScopedKernelTimer timer(ctx, KID_EXPERT_PRODUCT, stream);
   if (x->dtype == GSB_F32)
     launch_behind(stream, k_into_lines<float, 3>, grid, 256, (const float*)x->at, x->copies(), x->matrix_stride, (u32)x->height, x->stride, (u32)x->width,
-                  (u32)x->to_stride(), to);
+                  (u32)x->to_stride(), unit, to);
   else
     launch_behind(stream, k_into_lines<unsigned short, 1>, grid, 256, (const unsigned short*)x->at, x->copies(), x->matrix_stride, (u32)x->height, x->stride,
-                  (u32)x->width, (u32)x->to_stride(), to);
+                  (u32)x->width, (u32)x->to_stride(), unit, to);
   GSB_LAUNCH_OK();
   x->at = to;
   x->matrix_stride = x->matrix_stride == 0 ? 0 : x->height * x->to_stride();
@@ -890,18 +906,22 @@ static Lines matrices_operand(const void* w, int dtype, i64 experts, i64 expert_
 
 // Whether a product is of little work, for which the kernels without tensor cores are sooner done: by what both take, in microseconds,
 // fitted to a sweep of 17 shapes with bfloat16 and float32 (1 to 16 384 rows, 1 to 200 experts, widths of 32 to 2 048).
-// Few rows: 4 for the launch, one per 300 CTAs, one per 350 of the reduced index, one per 2.4 M weights that pass a CTA (1 024 rows of 100 to 47 by
+// Few rows: 4 for the launch, one per 300 CTAs, one per 350 of the reduced index, one per 2.4 M weights that pass a CTA, 1.2 M of floats whose columns
+// are runs (1 024 rows of 100 to 47 by
 // three experts: 5.4 for 13.4 by tiles; 4 096 of 64 to 64 by four: 10.3 for 7.1; 32 of 1 024 floats to 2 048 by eight: 18 for 87).  Tiles: 7, the
 // weights or the chain of stages, whichever is longer, and the copy of matrices that TMA cannot read.
-static double few_time(i64 num_rows, i64 k, i64 n, i64 num_experts) {
+static double few_time(i64 num_rows, i64 k, i64 n, i64 num_experts, bool slow) {
   const double tiles = (double)(num_rows / kFewRows + min(num_rows, num_experts));
-  return 4. + tiles * (double)((n + kFewColumns - 1) / kFewColumns) / 300. + (double)k / 350. + tiles * (double)k * (double)n / 2.4e6;
+  return 4. + tiles * (double)((n + kFewColumns - 1) / kFewColumns) / 300. + (double)k / 350. + tiles * (double)k * (double)n / (slow ? 1.2e6 : 2.4e6);
 }
-static bool few_rows(i64 num_rows, i64 k, i64 n, i64 num_experts, int size, i64 copied_bytes) {
-  const double weights = (double)min(num_rows, num_experts) * (double)k * (double)n * size / 4.5e6, chain = (double)k * size / 128. * 0.35;
+static bool few_rows(i64 num_rows, i64 k, i64 n, i64 num_experts, int size, bool across, i64 copied_bytes) {
+  const double weights = (double)min(num_rows, num_experts) * (double)k * (double)n * size / 4.5e6;
+  // steps one behind the other, of all tiles that a pair of CTAs takes: 0.35 us each, of float32 1.4
+  const double waves = (double)(num_rows / kPairRows + min(num_rows, num_experts)) * (double)((n + 255) / 256) / (kNumSMs / 2);
+  const double chain = (waves > 1. ? waves : 1.) * (double)k * size / 128. * (size == 4 ? 0.7 : 0.35);
   // the copy: read, written with its parts, and read again by the products
   const double copy = copied_bytes > 0 ? 3. + (double)copied_bytes * (size == 4 ? 10. / 6. : 2.) / 2.6e6 : 0.;
-  return few_time(num_rows, k, n, num_experts) < 6. + (weights > chain ? weights : chain) + copy;
+  return few_time(num_rows, k, n, num_experts, !across && size > 1) < 6. + (weights > chain ? weights : chain) + copy;
 }
 // The same of the weights' gradient.  Few rows: 3, one per 400 CTAs, and the rows that a CTA goes through (1 024 rows of 100 to 47 by three experts 7.5
 // us for 22; one row of 1 024 to 1 024 16 for 11.6; 4 096 of 64 to 64 by four 20 for 15, of floats 14 for 26).  Tiles: 8, or 14 with chunks, 8 more for float32.
@@ -937,6 +957,18 @@ static int with_type(int dtype, bool read, F f) {
   if (dtype == GSB_F16) return read ? f(__half{}, integral_constant<int, 1>{}, Yes{}) : f(__half{}, integral_constant<int, 1>{}, No{});
   return read ? f(__nv_bfloat16{}, integral_constant<int, 1>{}, Yes{}) : f(__nv_bfloat16{}, integral_constant<int, 1>{}, No{});
 }
+// 16-bit rows that TMA cannot load are read by warps where every tile reads them once, and copied into lines where several tiles of columns would
+// read them again (a product of 210 395 rows of 602 to 602 by 33 experts with both gradients 950 us for 1 190; 100 000 of 601 to 601 by four
+// 660 for 2 125).  Rows that begin on odd values, which are read value by value, are copied for a gradient (300 000 of 101 and 101 127 us for 254) and, where
+// they are long, for a product (200 003 of 601 to 100 162 us for 295, of 101 58 for 48).
+static bool rows_are_copied(const Lines& x, i64 readers, bool grad) {
+  if (x.dtype == GSB_F32 || !x.copied()) return false;
+  const bool odd = (((u64)(uintptr_t)x.at | (u64)(x.height > 1 ? x.stride * 2 : 0)) & 3) != 0;
+  return readers > 1 || (odd && (grad || x.width > 256));
+}
+static i64 grad_readers(i64 k, i64 n, u32 columns) { return (k + kPairRows - 1) / kPairRows * ((n + columns - 1) / columns); }
+static i64 tiles_across(i64 n, u32 columns) { return (n + columns - 1) / columns; }
+
 // Rows for the warps that read them.
 static RawRows raw_rows(const Lines& x) {
   const int size = value_bytes(x.dtype);
@@ -956,7 +988,10 @@ extern "C" int64_t gsb_expert_product_workspace(const void* rows, int dtype, int
       num_experts < 1 || num_experts > GSB_MAX_EXPERTS)
     return GSB_ERR_INVALID_ARGUMENT;
   const i64 copied = matrices_operand(weights, dtype, num_experts, weights_expert_stride, k, weights_k_stride, n, weights_n_stride).bytes();
-  return few_rows(num_rows, k, n, num_experts, value_bytes(dtype), copied) ? 0 : copied;
+  if (few_rows(num_rows, k, n, num_experts, value_bytes(dtype), rows_are_lines(k, n, weights_k_stride, weights_n_stride), copied)) return 0;
+  const Lines x = rows_operand(rows, dtype, num_rows, k, rows_stride);
+  const i64 across = tiles_across(n, tile_columns(n, dtype, row_tiles_of(num_rows, num_experts)));
+  return copied + (rows_are_copied(x, across, false) ? x.bytes() : 0);
 }
 
 extern "C" int gsb_expert_product(gsb_ctx* ctx, void* stream_, const void* rows, int dtype, int64_t num_rows, int64_t k, int64_t rows_stride,
@@ -978,7 +1013,7 @@ extern "C" int gsb_expert_product(gsb_ctx* ctx, void* stream_, const void* rows,
   const bool across = rows_are_lines(k, n, weights_k_stride, weights_n_stride);
   Lines x = rows_operand(rows, dtype, num_rows, k, rows_stride);
   Lines w = matrices_operand(weights, dtype, num_experts, weights_expert_stride, k, weights_k_stride, n, weights_n_stride);
-  if (few_rows(num_rows, k, n, num_experts, size, w.bytes()))
+  if (few_rows(num_rows, k, n, num_experts, size, across, w.bytes()))
     return by_experts(ctx, num_experts, num_rows, offsets, [&](const Groups& g) {
       const i64 line = w.height > 1 ? w.stride : 0;
       const FewArgs a{g, rows, weights, rows_stride, line, w.matrix_stride, (u32)k, (u32)n, nullptr, nullptr};
@@ -994,12 +1029,13 @@ extern "C" int gsb_expert_product(gsb_ctx* ctx, void* stream_, const void* rows,
       return (int)GSB_OK;
     });
   char* room = (char*)workspace;
-  if ((st = bring(ctx, stream, &w, &room)) != GSB_OK) return st;
   TileArgs a = {};
+  a.columns = tile_columns(n, dtype, row_tiles_of(num_rows, num_experts));
+  if ((st = bring(ctx, stream, &w, &room)) != GSB_OK) return st;
+  if (rows_are_copied(x, tiles_across(n, a.columns), false) && (st = bring(ctx, stream, &x, &room)) != GSB_OK) return st;
   a.rows = raw_rows(x);
   a.depth = (u32)k;
   a.n = (u32)n;
-  a.columns = tile_columns(n, dtype, row_tiles_of(num_rows, num_experts));
   a.expert_step = w.copies() > 1;
   CUtensorMap map_x = {}, map_w;
   const bool read = x.copied();
@@ -1025,7 +1061,10 @@ extern "C" int64_t gsb_expert_product_grad_workspace(const void* rows, int dtype
     return GSB_ERR_INVALID_ARGUMENT;
   const i64 chunk = chunk_rows(num_rows, k, n, tile_columns(n, dtype, row_tiles_of_grad(k, num_experts)), num_experts);
   if (few_grad(num_rows, k, n, num_experts, value_bytes(dtype), chunk < num_rows)) return 0;
-  return rounded(min(num_experts, (i64)kPlanExperts) * 2 * (i64)sizeof(CUtensorMap)) + (chunk < num_rows ? rounded(most_chunks(num_rows, chunk, num_experts) * k * n * 4) : 0);
+  const Lines x = rows_operand(rows, dtype, num_rows, k, rows_stride), d = rows_operand(grad, dtype, num_rows, n, grad_stride);
+  const i64 readers = grad_readers(k, n, tile_columns(n, dtype, row_tiles_of_grad(k, num_experts)));
+  return rounded(min(num_experts, (i64)kPlanExperts) * 2 * (i64)sizeof(CUtensorMap)) + (rows_are_copied(x, readers, true) ? x.bytes() : 0) +
+         (rows_are_copied(d, readers, true) ? d.bytes() : 0) + (chunk < num_rows ? rounded(most_chunks(num_rows, chunk, num_experts) * k * n * 4) : 0);
 }
 
 extern "C" int gsb_expert_product_grad(gsb_ctx* ctx, void* stream_, const void* rows, int dtype, int64_t num_rows, int64_t k, int64_t rows_stride,
@@ -1063,11 +1102,13 @@ extern "C" int gsb_expert_product_grad(gsb_ctx* ctx, void* stream_, const void* 
   room += rounded(min(num_experts, (i64)kPlanExperts) * 2 * (i64)sizeof(CUtensorMap));
   Lines x = rows_operand(rows, dtype, num_rows, k, rows_stride), d = rows_operand(grad, dtype, num_rows, n, grad_stride);
   TileArgs a = {};
+  a.columns = tile_columns(n, dtype, row_tiles_of_grad(k, num_experts));
+  for (Lines* some : {&x, &d})
+    if (rows_are_copied(*some, grad_readers(k, n, a.columns), true) && (st = bring(ctx, stream, some, &room)) != GSB_OK) return st;
   a.rows = raw_rows(x);
   a.grad = raw_rows(d);
   a.k = (u32)k;
   a.n = (u32)n;
-  a.columns = tile_columns(n, dtype, row_tiles_of_grad(k, num_experts));
   const i64 chunk = chunk_rows(num_rows, k, n, a.columns, num_experts);
   a.chunk = (u32)chunk;
   a.maps = maps;
@@ -1113,7 +1154,7 @@ extern "C" int gsb_expert_product_int8(gsb_ctx* ctx, void* stream_, const int8_t
   GSB_REQUIRE(values && scales && weight_values && weight_scales && out && aligned_to(4, scales, weight_scales) && aligned_to(size, (const char*)out),
               GSB_ERR_INVALID_ARGUMENT);
   cudaStream_t stream = (cudaStream_t)stream_;
-  if (few_rows(num_rows, k, n, num_experts, 1, 0))
+  if (few_rows(num_rows, k, n, num_experts, 1, false, 0))
     return by_experts(ctx, num_experts, num_rows, offsets, [&](const Groups& g) {
       const FewArgs a{g, values, weight_values, values_stride, weight_n_stride, num_experts > 1 ? weight_expert_stride : 0, (u32)k, (u32)n, scales, weight_scales};
       const int grid = few_grid((num_rows / kFewRows + min(num_rows, (i64)g.experts)) * ((n + kFewColumns - 1) / kFewColumns));
