@@ -54,6 +54,15 @@ def test_strides_and_addresses(ops, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_widths_of_an_access(ops, dtype):
+    """Rows and runs that begin on 32-byte boundaries, on 16-byte ones, and end a block after the last whole access."""
+    big = normal(generator(12), 303, 128, dtype=dtype)
+    for x in (big[:, 16:80], big[:, 16:88], big[:, 8:72], big.view(-1)[16:], big.view(-1)[8:], big.view(-1)[4:], big.view(-1)[:24], big.view(-1)[:2000 * 8 + 8],
+              big.view(-1)[16:16 + 4096 * 8 + 13], big[::2, :64], big[1::2, 64:]):
+        within(ops.dropout(x, 0.3, 98), *exact.dropout(x, 0.3, 98))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_dropped_values_do_not_count(ops, nn, dtype):
     stay, _ = exact.kept(3, 0, 5000, 0.4)
     for value in (float("nan"), float("inf"), -float("inf")):
