@@ -238,6 +238,24 @@ def test_addresses(ops, dtype, n, k, m):
     ctx.check_device()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("width", [65, 72, 129, 257, 264, 602, 1319, 3057, 3064, 3065, 3066])
+def test_quantize_from_and_to_any_address(ops, dtype, width):
+    """Rows that begin at every value of a line, written to bytes at every distance, with what is around them left as it was."""
+    ctx, code = ops.default_context(), CODES[dtype]
+    n, flat = 19, normal(generator(width), 20 * (width + 9) + 16, dtype=dtype)
+    for start in range(8):
+        for more, out_more in ((0, 0), (1, 3), (8, 1), (3, 2)):
+            rows = flat[start:start + n * (width + more)].view(n, width + more)[:, :width]
+            wide = width + out_more
+            values, scales = torch.full((n * wide + 64,), 9, dtype=torch.int8, device="cuda"), torch.full((n + 2,), -1.0, device="cuda")
+            assert ctx.lib.gsb_quantize_rows(ctx.handle, stream(), rows.data_ptr(), code, n, width, width + more, values.data_ptr() + start, wide,
+                                             scales.data_ptr() + 4) == 0
+            want, got = exact.quantized(rows), values[start:start + n * wide].view(n, wide)
+            assert torch.equal(got[:, :width], want[0]) and torch.equal(scales[1:-1], want[1]) and scales[0] == scales[-1] == -1
+            assert torch.all(values[:start] == 9) and torch.all(values[start + n * wide:] == 9) and torch.all(got[:, width:] == 9)
+
+
 def test_arguments_that_the_c_interface_refuses(ops):
     ctx = ops.default_context()
     lib, x = ctx.lib, torch.zeros(4096, device="cuda")
