@@ -32,6 +32,20 @@ constexpr int tile_threads(bool read) { return 32 * (kFirstReader + (read ? kRea
 // The widest access, of at most 16 bytes, that addresses with these bits allow.
 __host__ __device__ __forceinline__ int unit_of(u64 bits) { return bits % 16 == 0 ? 16 : bits % 8 == 0 ? 8 : bits % 4 == 0 ? 4 : 2; }
 
+// How rows come: by TMA; by warps, from memory; by TMA as they lie in memory, from where warps bring them into their lines.
+enum { BY_TMA, BY_WARPS, SHIFTED };
+// Rows that do not begin on 16-byte boundaries, for TMA: their distance in bytes times `classes` (2, 4 or 8) is a multiple of 16, so the rows number
+// c, c + classes and so on are an array whose lines begin on 16-byte boundaries, the row some values behind.  A slot of shared memory holds 128
+// rows, class by class, and of each the 128 bytes of two lines and those that the row may begin behind the boundary.  A box costs TMA some 140 cycles
+// and a row of it 9, so two lines at a time (200 003 rows of 602, 601 and 604 fp16 to 100: 77, 82 and 75 us) do better than one (95, 128 and 80) and, for
+// want of slots, than three (85, 88 and 83); two slots of two 86, four with two stages 81.  Of 608, which need none of this, 61 us.
+constexpr int kMostClasses = 8, kSlots = 3, kSlotBlocks = 2, kSlotLine = kSlotBlocks * kLineBytes + 16, kSlotBytes = 128 * kSlotLine;
+struct ShiftedMaps {
+  CUtensorMap of_class[kMostClasses];
+};
+template <int READ>
+using RowMaps = std::conditional_t<READ == SHIFTED, ShiftedMaps, CUtensorMap>;
+
 // Rows as they lie in memory, for the warps that read them.
 struct RawRows {
   const void* at;
@@ -50,6 +64,7 @@ struct TileArgs {
   int expert_step;           // 0: one matrix for all experts
   const CUtensorMap* maps;   // gradient: each expert's rows and gradient rows
   RawRows rows, grad;        // where they are read by warps
+  u32 classes;               // of shifted rows
   bool by_tma;               // results may leave by TMA
   float* partial;            // gradient: sums of the chunks (null: one chunk per expert, written out)
   const float *row_scales, *weight_scales;  // of 8-bit operands
@@ -264,10 +279,10 @@ struct Walk {
   }
 };
 
-// PARTS: 3 for float32, else 1.  ACROSS: the second operand's lines hold the reduced index across them (a gradient's both do).  READ: rows
-// (and a gradient's both operands) are read by warps, not by TMA.
-template <class T, bool WHOLE_NUMBERS, int PARTS, bool GRAD, bool ACROSS, bool READ>
-__global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+// PARTS: 3 for float32, else 1.  ACROSS: the second operand's lines hold the reduced index across them (a gradient's both do).  READ: how rows
+// (and a gradient's both operands) come.
+template <class T, bool WHOLE_NUMBERS, int PARTS, bool GRAD, bool ACROSS, int READ>
+__global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_constant__ RowMaps<READ> map_a, const __grid_constant__ CUtensorMap map_b,
                                                                  const __grid_constant__ CUtensorMap map_out, const TileArgs a, T* __restrict__ out) {
   constexpr int kPerLine = kLineBytes / (WHOLE_NUMBERS ? 1 : 2);
   // float32: sums leave tensor memory, where additions cut, after this many lines of the reduced index, and are added up in registers.
@@ -275,7 +290,8 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
   constexpr u32 kDrain = PARTS > 1 ? 4 : 0xffffffffu;
   extern __shared__ char raw[];
   __shared__ PlanTable plan;
-  __shared__ __align__(8) u64 bars[3 * kMaxStages + 4];
+  static_assert(READ != SHIFTED || (PARTS == 1 && !GRAD && !WHOLE_NUMBERS), "a product's rows of 16-bit values");
+  __shared__ __align__(8) u64 bars[3 * kMaxStages + 4 + 2 * kSlots];
   __shared__ float column_scales[WHOLE_NUMBERS ? kWriters : 1][128];
   constexpr int kRooms = rooms_of(PARTS);
   __shared__ __align__(1024) char rooms[kWriters][kRooms * kRoom];
@@ -284,6 +300,7 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
   const u32 stages_at = (smem_address(raw) + 1023u) & ~1023u;
   const u32 full = smem_address(bars), empty = full + 8 * kMaxStages, written = full + 16 * kMaxStages;
   const u32 sums_full = full + 24 * kMaxStages, sums_empty = sums_full + 16;
+  const u32 slot_full = sums_empty + 16, slot_empty = slot_full + 8 * kSlots;
   const u32 rank = rank_in_pair();
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   const Groups& g = a.groups;
@@ -300,9 +317,13 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
       barrier_init(sums_full + 8 * s, 1);
       barrier_init(sums_empty + 8 * s, 2 * kWriters);
     }
+    for (int s = 0; s < kSlots; ++s) {
+      barrier_init(slot_full + 8 * s, 1);
+      barrier_init(slot_empty + 8 * s, kReaders);
+    }
     barriers_ready();
     if (!GRAD) {
-      if (!READ) prefetch_map(&map_a);
+      if (!READ) prefetch_map((const CUtensorMap*)&map_a);
       prefetch_map(&map_b);
     }
   }
@@ -315,13 +336,14 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
   const u64 tiles = number_of_tiles<GRAD>(a, plan);
   const u64 first = blockIdx.x / 2, step = gridDim.x / 2;
   const u32 half = a.columns / 2, b_bytes = half * kLineBytes, stage_bytes = PARTS * (kRowsOperand + b_bytes);
+  const u32 slots_at = stages_at + a.stages * stage_bytes;  // of shifted rows
 
   if (warp == 0 && lane == 0 && !(READ && GRAD)) {
     const u32 full_of_first = address_in(full, 0);
     u32 stage = 0, turn = 0;
     for (u64 t = first; t < tiles; t += step) {
       const Tile tile = tile_at<GRAD, kPerLine>(a, plan, t);
-      const CUtensorMap *of_a = &map_a, *of_b = &map_b;
+      const CUtensorMap *of_a = (const CUtensorMap*)&map_a, *of_b = &map_b;
       if (GRAD) {
         of_a = a.maps + 2 * tile.e;
         of_b = of_a + 1;
@@ -395,6 +417,23 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
       }
     }
   issued:;
+  } else if (READ == SHIFTED && warp == 2 && lane == 0) {
+    u32 slot = 0, turn = 0;
+    for (u64 t = first; t < tiles; t += step) {
+      const Tile tile = tile_at<GRAD, kPerLine>(a, plan, t);
+      const u32 first_row = rank == 0 || tile.rows > 128 ? tile.row0 + rank * 128 : g.num_rows;  // from behind the array: zeros
+      for (u32 b = 0; b < tile.blocks; b += kSlotBlocks) {
+        if (!barrier_wait(slot_empty + 8 * slot, turn ^ 1, patience)) goto brought;
+        barrier_expect(slot_full + 8 * slot, kSlotBytes);
+        for (u32 c = 0; c < a.classes; ++c) {
+          const u32 row = first_row + ((c - first_row) & (a.classes - 1));
+          load_own_tile(slots_at + slot * kSlotBytes + c * (kSlotBytes / a.classes), (const CUtensorMap*)&map_a + c, slot_full + 8 * slot, (int)(b * 64),
+                        (int)(row / a.classes));
+        }
+        if (++slot == kSlots) slot = 0, turn ^= 1;
+      }
+    }
+  brought:;
   } else if (READ && warp == 3 && lane == 0) {
     // The readers' fence towards the tensor cores: theirs would wait for their copies that are on their way
     const u32 full_of_first = address_in(full, 0);
@@ -476,6 +515,41 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
         go_on();
         if (++stage == (u32)a.stages) stage = 0, turn ^= 1;
       }
+    } else if constexpr (READ == SHIFTED) {
+      // Warp w has lines w, w + 8 and so on, all of one class
+      const u32 w = me / 32, to = stages_at + w * kLineBytes + (((lane >> 2) ^ w) << 4) + (lane & 3) * 4, class_bytes = kSlotBytes / a.classes;
+      u32 slot = 0, slot_turn = 0;
+      for (u64 t = first; t < tiles; t += step) {
+        const Tile tile = tile_at<GRAD, kPerLine>(a, plan, t);
+        const u32 c = (tile.row0 + rank * 128 + w) & (a.classes - 1), behind = c * (u32)a.rows.stride & 7;  // values behind the boundary
+        const u32 from = slots_at + c * class_bytes + w / a.classes * kSlotLine + behind / 2 * 4 + lane * 4, by = 8 / a.classes * kSlotLine;
+        for (u32 b = 0; b < tile.blocks; ++b) {
+          const u32 block = b % kSlotBlocks;
+          if (block == 0 && !__all_sync(0xffffffffu, barrier_wait(slot_full + 8 * slot, slot_turn, patience))) goto shifted;
+          u32 v[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const u32 at = from + slot * kSlotBytes + block * kLineBytes + i * by;
+            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v[i]) : "r"(at) : "memory");
+            if (behind & 1) {
+              u32 next;
+              asm volatile("ld.shared.b32 %0, [%1];" : "=r"(next) : "r"(at + 4) : "memory");
+              v[i] = __funnelshift_r(v[i], next, 16);
+            }
+          }
+          if (!__all_sync(0xffffffffu, barrier_wait(empty + 8 * stage, turn ^ 1, patience))) goto shifted;
+          write_lines<0, 16>(v, to + stage * stage_bytes);
+          __syncwarp();
+          const bool last = block + 1 == kSlotBlocks || b + 1 == tile.blocks;
+          if (lane == 0) {
+            if (last) barrier_arrive(slot_empty + 8 * slot);
+            barrier_arrive(written + 8 * stage);
+          }
+          if (last && ++slot == kSlots) slot = 0, slot_turn ^= 1;
+          if (++stage == (u32)a.stages) stage = 0, turn ^= 1;
+        }
+      }
+    shifted:;
     } else {
       // Warp w has lines w, w + 8 and so on; those of the next stages are on their way while it writes this one's, two stages of a product's rows
       // or one of both operands of a gradient.  (200 003 rows of 602 to 100 take 106 us; of 608, which TMA loads, 58.  Asynchronous copies of four
@@ -789,6 +863,12 @@ struct Lines {
     return dtype == GSB_F32 || !aligned_to(16, (const char*)at) || (height > 1 && (stride * size % 16 != 0 || stride == 0)) ||
            (matrices > 1 && matrix_stride * size % 16 != 0) || (height > 1 && stride >= kMostStride / size) || (matrices > 1 && matrix_stride >= kMostStride / size);
   }
+  // TMA can load its lines class by class
+  bool shifted() const {
+    return dtype != GSB_F32 && height >= kMostClasses && matrices == 1 && aligned_to(16, (const char*)at) && stride % 8 != 0 && stride >= width &&
+           stride < kMostStride / (2 * kMostClasses);
+  }
+  u32 classes() const { return stride % 2 ? 8 : stride % 4 ? 4 : 2; }
   i64 parts() const { return dtype == GSB_F32 ? 3 : 1; }
   i64 to_stride() const { return (width + 7) / 8 * 8; }
   i64 copies() const { return matrices > 1 && matrix_stride == 0 ? 1 : matrices; }  // one matrix for all is copied once
@@ -830,6 +910,17 @@ static int describe(const Lines& x, int size, u32 box_along, u32 box_lines, bool
   return describe_array(map, x.at, size, matrices ? 4 : 3, matrices ? dims4 : dims3, matrices ? strides4 : strides3, box) ? GSB_OK : GSB_ERR_UNSUPPORTED;
 }
 
+static int describe_shifted(const Lines& x, ShiftedMaps* maps) {
+  const u32 classes = x.classes();
+  for (u32 c = 0; c < classes; ++c) {
+    const u32 behind = (u32)(c * x.stride % 8);
+    const u64 dims[3] = {(u64)(x.width + behind), (u64)((x.height - c + classes - 1) / classes), 1}, strides[2] = {(u64)(x.stride * 2 * classes), 16};
+    const u32 box[3] = {kSlotLine / 2, 128 / classes, 1};
+    if (!describe_array(&maps->of_class[c], (const unsigned short*)x.at + c * x.stride - behind, 2, 3, dims, strides, box, false)) return GSB_ERR_UNSUPPORTED;
+  }
+  return GSB_OK;
+}
+
 static int check_product(i64 num_rows, i64 k, i64 n, i64 num_experts, i64 rows_stride, const int64_t* offsets) {
   GSB_REQUIRE(num_rows >= 0 && num_rows < ((i64)1 << 31) && k >= 1 && k <= GSB_MAX_ROW_LEN && n >= 1 && n <= GSB_MAX_ROW_LEN && num_experts >= 1 &&
                   num_experts <= GSB_MAX_EXPERTS && rows_stride >= 0,
@@ -856,14 +947,15 @@ constexpr u64 kNanosecondsPerPoll = 477;
 // Launches pairs of CTAs: at most one CTA per SM.  In the order of the stream, with no overlap of its neighbours' ends and beginnings: with
 // overlap, hundreds of copies and products queued one behind the other came to a halt, waiting CTAs of one kernel beside clusters of another
 // that need SMs as a whole.
-template <class T, bool WHOLE_NUMBERS, int PARTS, bool GRAD, bool ACROSS, bool READ>
-static int launch_tiles(gsb_ctx* ctx, cudaStream_t stream, const CUtensorMap& map_a, const CUtensorMap& map_b, TileArgs a, i64 most_tiles, i64 out_rows, T* out) {
+template <class T, bool WHOLE_NUMBERS, int PARTS, bool GRAD, bool ACROSS, int READ>
+static int launch_tiles(gsb_ctx* ctx, cudaStream_t stream, const RowMaps<READ>& map_a, const CUtensorMap& map_b, TileArgs a, i64 most_tiles, i64 out_rows, T* out) {
   auto kernel = k_tiles<T, WHOLE_NUMBERS, PARTS, GRAD, ACROSS, READ>;
   const int stage = PARTS * (kRowsOperand + (int)a.columns / 2 * kLineBytes);
-  a.stages = min(kMaxStages, stages_room(PARTS) / stage);
+  constexpr int kSlotsRoom = READ == SHIFTED ? kSlots * kSlotBytes : 0;
+  a.stages = min(kMaxStages, (stages_room(PARTS) - kSlotsRoom) / stage);
   a.how = instruction(WHOLE_NUMBERS ? OPERAND_S8 : std::is_same<T, __half>::value ? OPERAND_F16 : OPERAND_BF16, GRAD, GRAD || ACROSS, kPairRows, a.columns);
   a.wait_limit = (u64)ctx_option(ctx, GSB_OPT_MAX_POLLS) * kNanosecondsPerPoll;
-  const int smem = a.stages * stage + 1024;
+  const int smem = a.stages * stage + kSlotsRoom + 1024;
   CUtensorMap map_out = {};
   const int size = a.partial ? 4 : (int)sizeof(T);
   void* const results = a.partial ? (void*)a.partial : (void*)out;
@@ -949,20 +1041,24 @@ static i64 most_chunks(i64 num_rows, i64 chunk, i64 num_experts) { return min(nu
 
 // Calls f(T, PARTS, READ).
 template <class F>
-static int with_type(int dtype, bool read, F f) {
+static int with_type(int dtype, int read, F f) {
   using std::integral_constant;
-  using Yes = integral_constant<bool, true>;
-  using No = integral_constant<bool, false>;
-  if (dtype == GSB_F32) return f(float{}, integral_constant<int, 3>{}, Yes{});
-  if (dtype == GSB_F16) return read ? f(__half{}, integral_constant<int, 1>{}, Yes{}) : f(__half{}, integral_constant<int, 1>{}, No{});
-  return read ? f(__nv_bfloat16{}, integral_constant<int, 1>{}, Yes{}) : f(__nv_bfloat16{}, integral_constant<int, 1>{}, No{});
+  if (dtype == GSB_F32) return f(float{}, integral_constant<int, 3>{}, integral_constant<int, BY_WARPS>{});
+  auto by_type = [&](auto reading) {
+    return dtype == GSB_F16 ? f(__half{}, integral_constant<int, 1>{}, reading) : f(__nv_bfloat16{}, integral_constant<int, 1>{}, reading);
+  };
+  if (read == SHIFTED) return by_type(integral_constant<int, SHIFTED>{});
+  return read == BY_WARPS ? by_type(integral_constant<int, BY_WARPS>{}) : by_type(integral_constant<int, BY_TMA>{});
 }
-// 16-bit rows that TMA cannot load are read by warps where every tile reads them once, and copied into lines where several tiles of columns would
-// read them again (a product of 210 395 rows of 602 to 602 by 33 experts with both gradients 950 us for 1 190; 100 000 of 601 to 601 by four
-// 660 for 2 125).  Rows that begin on odd values, which are read value by value, are copied for a gradient (300 000 of 101 and 101 127 us for 254) and, where
-// they are long, for a product (200 003 of 601 to 100 162 us for 295, of 101 58 for 48).
+// A product's 16-bit rows that TMA cannot load line by line come class by class (shifted).  Of the others (from an address off 16-byte boundaries, all one row,
+// fewer than eight) and of a gradient's, for which rows of several classes would meet in one line of the reduced index, those are read by warps
+// that every tile reads once, and copied into lines those that several tiles of columns would read again (a product of 210 395 rows of 602 to 602 by 33
+// experts with both gradients 950 us for 1 190).  Rows that begin on odd values, which are read value by value, are copied for a gradient (300 000 of
+// 101 and 101 127 us for 254) and, where they are long, for a product.  Shifted against copied, products of 200 003 rows of 602 to 602 235 us for
+// 264, of 601 240 for 283, of 602 to 2 048 591 for 548; of 100 000 of 102 to 512 42 for 62.
 static bool rows_are_copied(const Lines& x, i64 readers, bool grad) {
   if (x.dtype == GSB_F32 || !x.copied()) return false;
+  if (!grad && x.shifted()) return false;
   const bool odd = (((u64)(uintptr_t)x.at | (u64)(x.height > 1 ? x.stride * 2 : 0)) & 3) != 0;
   return readers > 1 || (odd && (grad || x.width > 256));
 }
@@ -1038,8 +1134,11 @@ extern "C" int gsb_expert_product(gsb_ctx* ctx, void* stream_, const void* rows,
   a.n = (u32)n;
   a.expert_step = w.copies() > 1;
   CUtensorMap map_x = {}, map_w;
-  const bool read = x.copied();
-  if (!read && (st = describe(x, 2, 64, 128, false, &map_x)) != GSB_OK) return st;
+  ShiftedMaps shifted_x = {};
+  const int read = !x.copied() ? BY_TMA : x.shifted() ? SHIFTED : BY_WARPS;
+  if (read == BY_TMA && (st = describe(x, 2, 64, 128, false, &map_x)) != GSB_OK) return st;
+  if (read == SHIFTED && (st = describe_shifted(x, &shifted_x)) != GSB_OK) return st;
+  a.classes = read == SHIFTED ? x.classes() : 0;
   if ((st = describe(w, 2, 64, across ? 64 : a.columns / 2, true, &map_w)) != GSB_OK) return st;
   return by_experts(ctx, num_experts, num_rows, offsets, [&](const Groups& g) {
     a.groups = g;
@@ -1047,9 +1146,13 @@ extern "C" int gsb_expert_product(gsb_ctx* ctx, void* stream_, const void* rows,
     return with_type(dtype, read, [&](auto value, auto parts, auto reading) {
       typedef decltype(value) T;
       constexpr int P = decltype(parts)::value;
-      constexpr bool R = decltype(reading)::value;
-      if (across) return launch_tiles<T, false, P, false, true, R>(ctx, stream, map_x, map_w, a, tiles, num_rows, (T*)out);
-      return launch_tiles<T, false, P, false, false, R>(ctx, stream, map_x, map_w, a, tiles, num_rows, (T*)out);
+      constexpr int R = decltype(reading)::value;
+      auto launch = [&](const RowMaps<R>& map) {
+        if (across) return launch_tiles<T, false, P, false, true, R>(ctx, stream, map, map_w, a, tiles, num_rows, (T*)out);
+        return launch_tiles<T, false, P, false, false, R>(ctx, stream, map, map_w, a, tiles, num_rows, (T*)out);
+      };
+      if constexpr (R == SHIFTED) return launch(shifted_x);
+      else return launch(map_x);
     });
   });
 }
@@ -1114,7 +1217,7 @@ extern "C" int gsb_expert_product_grad(gsb_ctx* ctx, void* stream_, const void* 
   a.maps = maps;
   a.partial = chunk < num_rows ? (float*)room : nullptr;
   CUtensorMap map_x = {}, map_d = {};
-  const bool read = x.copied() || d.copied();
+  const int read = x.copied() || d.copied() ? BY_WARPS : BY_TMA;
   if (!read && ((st = describe(x, 2, 64, 64, false, &map_x)) != GSB_OK || (st = describe(d, 2, 64, 64, false, &map_d)) != GSB_OK)) return st;
   return by_experts(ctx, num_experts, num_rows, offsets, [&](const Groups& g) -> int {
     a.groups = g;
@@ -1127,7 +1230,8 @@ extern "C" int gsb_expert_product_grad(gsb_ctx* ctx, void* stream_, const void* 
     const i64 tiles = (num_rows / chunk + g.experts) * ((k + kPairRows - 1) / kPairRows) * ((n + a.columns - 1) / a.columns);
     return with_type(dtype, read, [&](auto value, auto parts, auto reading) -> int {
       typedef decltype(value) T;
-      const int launched = launch_tiles<T, false, decltype(parts)::value, true, true, decltype(reading)::value>(ctx, stream, map_x, map_d, a, tiles, (a.partial ? num_rows / chunk + g.experts : num_experts) * k, (T*)out);
+      constexpr int R = decltype(reading)::value == BY_TMA ? BY_TMA : BY_WARPS;
+      const int launched = launch_tiles<T, false, decltype(parts)::value, true, true, R>(ctx, stream, map_x, map_d, a, tiles, (a.partial ? num_rows / chunk + g.experts : num_experts) * k, (T*)out);
       if (launched != GSB_OK || !a.partial) return launched;
       ScopedKernelTimer timer(ctx, KID_EXPERT_PRODUCT, stream);
       launch_behind(stream, k_add_chunks<T>, (int)min((i64)kNumSMs * 8, (i64)grid_for(k * n * g.experts, kAddThreads)), kAddThreads, g, a.chunk, k * n,
@@ -1180,8 +1284,8 @@ extern "C" int gsb_expert_product_int8(gsb_ctx* ctx, void* stream_, const int8_t
   return by_experts(ctx, num_experts, num_rows, offsets, [&](const Groups& g) {
     a.groups = g;
     const i64 tiles = (num_rows / kPairRows + g.experts) * ((n + a.columns - 1) / a.columns);
-    if (out_dtype == GSB_F32) return launch_tiles<float, true, 1, false, false, false>(ctx, stream, map_x, map_w, a, tiles, num_rows, (float*)out);
-    if (out_dtype == GSB_F16) return launch_tiles<__half, true, 1, false, false, false>(ctx, stream, map_x, map_w, a, tiles, num_rows, (__half*)out);
-    return launch_tiles<__nv_bfloat16, true, 1, false, false, false>(ctx, stream, map_x, map_w, a, tiles, num_rows, (__nv_bfloat16*)out);
+    if (out_dtype == GSB_F32) return launch_tiles<float, true, 1, false, false, BY_TMA>(ctx, stream, map_x, map_w, a, tiles, num_rows, (float*)out);
+    if (out_dtype == GSB_F16) return launch_tiles<__half, true, 1, false, false, BY_TMA>(ctx, stream, map_x, map_w, a, tiles, num_rows, (__half*)out);
+    return launch_tiles<__nv_bfloat16, true, 1, false, false, BY_TMA>(ctx, stream, map_x, map_w, a, tiles, num_rows, (__nv_bfloat16*)out);
   });
 }

@@ -28,7 +28,8 @@ static bool encoded(F encode) {
   return cudaGetDevice(&device) == cudaSuccess && cudaSetDevice(device) == cudaSuccess && encode() == CUDA_SUCCESS;
 }
 
-bool describe_array(CUtensorMap* map, const void* base, int value_bytes, int rank, const u64* dims, const u64* strides, const u32* box) {
+bool describe_array(CUtensorMap* map, const void* base, int value_bytes, int rank, const u64* dims, const u64* strides, const u32* box,
+                    bool swizzled) {
   const EncodeTiled encode = encode_tiled();
   if (!encode) return false;
   cuuint64_t extents[5], distances[4];
@@ -40,7 +41,7 @@ bool describe_array(CUtensorMap* map, const void* base, int value_bytes, int ran
   }
   return encoded([&] {
     return encode(map, value_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, const_cast<void*>(base), extents,
-                  distances, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  distances, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzled ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   });
 }

@@ -98,6 +98,12 @@ __device__ __forceinline__ void load_tile(u32 to, const CUtensorMap* map, u32 cl
                "l"(map), "r"(cluster_bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
                : "memory");
 }
+// Lines one behind the other, not exchanged, with the arrival at a barrier of this CTA's.
+__device__ __forceinline__ void load_own_tile(u32 to, const CUtensorMap* map, u32 bar, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(to), "l"(map),
+               "r"(bar), "r"(c0), "r"(c1), "r"(0)
+               : "memory");
+}
 // Rows of 64 bytes out of shared memory, 16-byte pieces of row i exchanged by i / 2 % 4 (the 64-byte swizzle).  What lies outside the array is
 // not written.
 __device__ __forceinline__ void store_tile(const CUtensorMap* map, u32 from, int c0, int c1) {
@@ -168,8 +174,9 @@ __device__ __forceinline__ void sums_read() { asm volatile("tcgen05.wait::ld.syn
 
 // ---- host: what a TMA load is told of an array ----
 // `dims` extents, the first of neighbours in memory; strides in bytes of the others (multiples of 16, below 2^40).  False: it cannot be
-// described.
-bool describe_array(CUtensorMap* map, const void* base, int value_bytes, int rank, const u64* dims, const u64* strides, const u32* box);
+// described.  Swizzled: 16-byte pieces of line i of a box are exchanged by i % 8 (the 128-byte swizzle).
+bool describe_array(CUtensorMap* map, const void* base, int value_bytes, int rank, const u64* dims, const u64* strides, const u32* box,
+                    bool swizzled = true);
 // Of stores: `rows` rows of `width` values, one behind the other; boxes of 32 rows by 64 bytes.
 bool describe_rows(CUtensorMap* map, void* base, int value_bytes, u64 width, u64 rows);
 

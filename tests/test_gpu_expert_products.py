@@ -240,6 +240,26 @@ def test_changed_operands_are_noticed(nn):
         out.sum().backward()
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("width,stride", [(602, 602), (601, 601), (604, 604), (64, 66), (1, 3), (7, 7), (65, 67), (130, 132), (191, 193), (9, 1201), (100, 100)])
+def test_rows_at_distances_that_no_line_has(ops, dtype, width, stride):
+    """Rows 2, 4 and 8 of which begin a 16-byte line: few and many, experts that begin at any of them, NaN and infinities in the row before and behind."""
+    for rows in (7, 8, 9, 127, 129, 300, 1111, 5000):
+        g = generator(rows + width)
+        x = normal(g, rows * stride, dtype=dtype).view(rows, stride)[:, :width]
+        offsets = torch.tensor([0, rows // 3, rows // 3, rows // 2 + 1, rows - rows // 7], device="cuda")
+        for n in (100, 300):
+            w = normal(g, 4, width, n, dtype=dtype)
+            want = exact.product(x, w, offsets)
+            within(ops.expert_product(x, w, offsets), *want)
+        spoiled = x.clone()                                 # contiguous: its distances are the width
+        spoiled[rows // 2 - 1, -1], spoiled[rows // 2 + 1, 0] = float("nan"), float("inf")
+        out, clean = ops.expert_product(spoiled, w, offsets), ops.expert_product(x.contiguous(), w, offsets)
+        other = torch.ones(rows, dtype=torch.bool, device="cuda")
+        other[rows // 2 - 1] = other[rows // 2 + 1] = False
+        assert torch.equal(out[other], clean[other])
+
+
 # ---- 8 bits ----------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,width", [(1, 1), (3, 5), (33, 1024), (200, 100), (65, 602), (70, 2048), (40, 2056), (9, 4099), (1000, 16), (2, 70_000)])
