@@ -161,6 +161,8 @@ __global__ void __launch_bounds__(kQuantThreads) k_quantize_short(const Unit<T, 
 // the unrolled divisions were more code than the instruction cache holds: 65 536 rows of 2 048 bf16 took 184 us).  They take 71 (5.7 TB/s), 200 000
 // rows of 608 take 90: the instructions of a row bound it, so one of up to 128 units is asked for by 4 to a lane at once, not 8 (90 and 101 us).
 constexpr int kHeld = 256;
+// Counted in warps: threads of 2^27 rows are more than 32 bits hold.
+__device__ __forceinline__ u32 row_of_warp() { return blockIdx.x * (kQuantThreads / 32) + threadIdx.x / 32; }
 template <class T, int BYTES, bool PACKED, int kAhead>
 __global__ void __launch_bounds__(kQuantThreads) k_quantize_rows(const Unit<T, BYTES>* __restrict__ x, i64 x_stride, int units, u32 num_rows,
                                                                  int8_t* __restrict__ values, i64 values_stride, float* __restrict__ scales) {
@@ -171,7 +173,7 @@ __global__ void __launch_bounds__(kQuantThreads) k_quantize_rows(const Unit<T, B
   await_previous();
   const int lane = threadIdx.x & 31;
   Word* const held = room[threadIdx.x / 32];
-  for (u32 r = (blockIdx.x * kQuantThreads + threadIdx.x) / 32; r < num_rows; r += gridDim.x * (kQuantThreads / 32)) {
+  for (u32 r = row_of_warp(); r < num_rows; r += gridDim.x * (kQuantThreads / 32)) {
     const U* row = x + (i64)r * x_stride;
     Largest<T, BYTES> largest;
     for (int j0 = lane; j0 < units; j0 += 32 * kAhead) {
@@ -213,7 +215,7 @@ __global__ void __launch_bounds__(kQuantThreads, 6) k_quantize_shifted(const T* 
   await_previous();
   const int lane = threadIdx.x & 31;
   uint4* const held = rooms + threadIdx.x / 32 * room;
-  for (u32 r = (blockIdx.x * kQuantThreads + threadIdx.x) / 32; r < num_rows; r += gridDim.x * (kQuantThreads / 32)) {
+  for (u32 r = row_of_warp(); r < num_rows; r += gridDim.x * (kQuantThreads / 32)) {
     const T* row = x + (i64)r * x_stride;
     const int lead = (int)((u64)(uintptr_t)row & 15) / 2, end = lead + row_len, first = lead ? 1 : 0, last = end / 8;
     const Unit<T, 16>* lines = (const Unit<T, 16>*)(row - lead);
