@@ -374,10 +374,11 @@ std::pair<Tensor, Tensor> quantize(gsb_ctx* ctx, const Tensor& x_) {
 }
 
 // Rows in 8 bits that begin on 16-byte boundaries; a copy where they do not.
-Tensor bytes_of(const Tensor& t, const char* name, int64_t dim) {
-  refuse_unless(t.scalar_type() == at::kChar, name, " must be int8");
-  refuse_unless(t.dim() == dim, name, dim == 2 ? " must have two dimensions" : " must have the shape [experts, n, k]");
-  refuse_unless(t.is_cuda(), name, " must be a CUDA tensor");
+Tensor bytes_of(const Tensor& t_, const char* name, int64_t dim) {
+  refuse_unless(t_.scalar_type() == at::kChar, name, " must be int8");
+  refuse_unless(t_.dim() == dim, name, dim == 2 ? " must have two dimensions" : " must have the shape [experts, n, k]");
+  refuse_unless(t_.is_cuda(), name, " must be a CUDA tensor");
+  const Tensor t = as_stored(t_);
   bool good = (t.size(-1) <= 1 || t.stride(-1) == 1) && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % kLine == 0;
   for (int64_t d = 0; d + 1 < dim; ++d) good = good && (t.size(d) <= 1 || (t.stride(d) % kLine == 0 && t.stride(d) >= t.size(-1)));
   if (good || t.numel() == 0) return t;

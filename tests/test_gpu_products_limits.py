@@ -48,3 +48,17 @@ def test_more_rows_than_32_bits_count_lanes_of(ops, dtype, width):
     assert torch.all(scales == want_scale)
     for first in range(0, n, 1 << 23):
         assert torch.all(values[first:first + (1 << 23)] == want), first
+
+
+def test_negated_views_in_8_bits(ops):
+    """Rows and weights that lie on 16-byte boundaries and are read in place, and some that do not and are copied."""
+    g = generator(2)
+    offsets = torch.tensor([0, 20, 50], device="cuda")
+    scales, weight_scales = torch.rand(50, generator=g, device="cuda"), torch.rand(2, 40, generator=g, device="cuda")
+    for k in (32, 27):
+        values = torch.randint(-127, 128, (50, k), generator=g, device="cuda").to(torch.int8)
+        weight_values = torch.randint(-127, 128, (2, 40, k), generator=g, device="cuda").to(torch.int8)
+        minus = ops.expert_product_int8(-values, scales, weight_values, weight_scales, offsets)
+        assert torch.count_nonzero(minus) > 0
+        assert torch.equal(ops.expert_product_int8(torch._neg_view(values), scales, weight_values, weight_scales, offsets), minus)
+        assert torch.equal(ops.expert_product_int8(values, scales, torch._neg_view(weight_values), weight_scales, offsets), minus)
