@@ -329,6 +329,7 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
   }
   if (warp == 2) sums_alloc(smem_address(&sums_at), kSumColumns);
   make_plan<tile_threads(READ)>(plan, g, GRAD ? a.chunk : kPairRows, GRAD ? 1 : 0);
+  leave_end(plan, g);
   sums_fence_before();
   cluster_barrier();
   sums_fence_after();
@@ -929,15 +930,23 @@ static int check_product(i64 num_rows, i64 k, i64 n, i64 num_experts, i64 rows_s
   return GSB_OK;
 }
 
-// One launch per kPlanExperts experts.
+// One launch per kPlanExperts experts, in order.  `ends`: a word for each, or null.
 template <class F>
-static int by_experts(gsb_ctx* ctx, i64 num_experts, i64 num_rows, const int64_t* offsets, F launch) {
+static int by_experts(gsb_ctx* ctx, i64 num_experts, i64 num_rows, const int64_t* offsets, u32* ends, F launch) {
   for (i64 first = 0; first < num_experts; first += kPlanExperts) {
     const int some = (int)min((i64)kPlanExperts, num_experts - first);
-    const int st = launch(Groups{offsets + first, (int)first, some, (int)num_experts, (u32)num_rows, ctx_counters(ctx)});
+    const int st = launch(Groups{offsets + first, (int)first, some, (int)num_experts, (u32)num_rows, ctx_counters(ctx), ends ? ends + first / kPlanExperts : nullptr});
     if (st != GSB_OK) return st;
   }
   return GSB_OK;
+}
+// Room for the ends of all launches, where there are several, and one word behind the last.  It is the first of a workspace.
+static i64 ends_bytes(i64 num_experts) { return num_experts > kPlanExperts ? rounded((num_experts + kPlanExperts - 1) / kPlanExperts * 4 + 4) : 0; }
+static u32* take_ends(i64 num_experts, char** room) {
+  const i64 bytes = ends_bytes(num_experts);
+  u32* const ends = bytes > 0 ? (u32*)*room : nullptr;
+  *room += bytes;
+  return ends;
 }
 
 // Shared memory for stages: what the fixed part (the plan, the scales, the ways out) leaves, and what is lost to their alignment.
@@ -1084,10 +1093,10 @@ extern "C" int64_t gsb_expert_product_workspace(const void* rows, int dtype, int
       num_experts < 1 || num_experts > GSB_MAX_EXPERTS)
     return GSB_ERR_INVALID_ARGUMENT;
   const i64 copied = matrices_operand(weights, dtype, num_experts, weights_expert_stride, k, weights_k_stride, n, weights_n_stride).bytes();
-  if (few_rows(num_rows, k, n, num_experts, value_bytes(dtype), rows_are_lines(k, n, weights_k_stride, weights_n_stride), copied)) return 0;
+  if (few_rows(num_rows, k, n, num_experts, value_bytes(dtype), rows_are_lines(k, n, weights_k_stride, weights_n_stride), copied)) return ends_bytes(num_experts);
   const Lines x = rows_operand(rows, dtype, num_rows, k, rows_stride);
   const i64 across = tiles_across(n, tile_columns(n, dtype, row_tiles_of(num_rows, num_experts)));
-  return copied + (rows_are_copied(x, across, false) ? x.bytes() : 0);
+  return ends_bytes(num_experts) + copied + (rows_are_copied(x, across, false) ? x.bytes() : 0);
 }
 
 extern "C" int gsb_expert_product(gsb_ctx* ctx, void* stream_, const void* rows, int dtype, int64_t num_rows, int64_t k, int64_t rows_stride,
@@ -1109,8 +1118,10 @@ extern "C" int gsb_expert_product(gsb_ctx* ctx, void* stream_, const void* rows,
   const bool across = rows_are_lines(k, n, weights_k_stride, weights_n_stride);
   Lines x = rows_operand(rows, dtype, num_rows, k, rows_stride);
   Lines w = matrices_operand(weights, dtype, num_experts, weights_expert_stride, k, weights_k_stride, n, weights_n_stride);
+  char* room = (char*)workspace;
+  u32* const ends = take_ends(num_experts, &room);
   if (few_rows(num_rows, k, n, num_experts, size, across, w.bytes()))
-    return by_experts(ctx, num_experts, num_rows, offsets, [&](const Groups& g) {
+    return by_experts(ctx, num_experts, num_rows, offsets, ends, [&](const Groups& g) {
       const i64 line = w.height > 1 ? w.stride : 0;
       const FewArgs a{g, rows, weights, rows_stride, line, w.matrix_stride, (u32)k, (u32)n, nullptr, nullptr};
       const bool wide = aligned_to(16, (const char*)weights) && line * size % 16 == 0 && w.matrix_stride * size % 16 == 0;
@@ -1124,7 +1135,6 @@ extern "C" int gsb_expert_product(gsb_ctx* ctx, void* stream_, const void* rows,
       GSB_LAUNCH_OK();
       return (int)GSB_OK;
     });
-  char* room = (char*)workspace;
   TileArgs a = {};
   a.columns = tile_columns(n, dtype, row_tiles_of(num_rows, num_experts));
   if ((st = bring(ctx, stream, &w, &room)) != GSB_OK) return st;
@@ -1140,7 +1150,7 @@ extern "C" int gsb_expert_product(gsb_ctx* ctx, void* stream_, const void* rows,
   if (read == SHIFTED && (st = describe_shifted(x, &shifted_x)) != GSB_OK) return st;
   a.classes = read == SHIFTED ? x.classes() : 0;
   if ((st = describe(w, 2, 64, across ? 64 : a.columns / 2, true, &map_w)) != GSB_OK) return st;
-  return by_experts(ctx, num_experts, num_rows, offsets, [&](const Groups& g) {
+  return by_experts(ctx, num_experts, num_rows, offsets, ends, [&](const Groups& g) {
     a.groups = g;
     const i64 tiles = (num_rows / kPairRows + g.experts) * ((n + a.columns - 1) / a.columns);
     return with_type(dtype, read, [&](auto value, auto parts, auto reading) {
@@ -1163,10 +1173,10 @@ extern "C" int64_t gsb_expert_product_grad_workspace(const void* rows, int dtype
       num_experts < 1 || num_experts > GSB_MAX_EXPERTS)
     return GSB_ERR_INVALID_ARGUMENT;
   const i64 chunk = chunk_rows(num_rows, k, n, tile_columns(n, dtype, row_tiles_of_grad(k, num_experts)), num_experts);
-  if (few_grad(num_rows, k, n, num_experts, value_bytes(dtype), chunk < num_rows)) return 0;
+  if (few_grad(num_rows, k, n, num_experts, value_bytes(dtype), chunk < num_rows)) return ends_bytes(num_experts);
   const Lines x = rows_operand(rows, dtype, num_rows, k, rows_stride), d = rows_operand(grad, dtype, num_rows, n, grad_stride);
   const i64 readers = grad_readers(k, n, tile_columns(n, dtype, row_tiles_of_grad(k, num_experts)));
-  return rounded(min(num_experts, (i64)kPlanExperts) * 2 * (i64)sizeof(CUtensorMap)) + (rows_are_copied(x, readers, true) ? x.bytes() : 0) +
+  return ends_bytes(num_experts) + rounded(min(num_experts, (i64)kPlanExperts) * 2 * (i64)sizeof(CUtensorMap)) + (rows_are_copied(x, readers, true) ? x.bytes() : 0) +
          (rows_are_copied(d, readers, true) ? d.bytes() : 0) + (chunk < num_rows ? rounded(most_chunks(num_rows, chunk, num_experts) * k * n * 4) : 0);
 }
 
@@ -1184,8 +1194,13 @@ extern "C" int gsb_expert_product_grad(gsb_ctx* ctx, void* stream_, const void* 
     GSB_CUDA_OK(cudaMemsetAsync(out, 0, (size_t)(num_experts * k * n * size), stream));
     return GSB_OK;
   }
+  const int64_t need = gsb_expert_product_grad_workspace(rows, dtype, num_rows, k, rows_stride, grad, n, grad_stride, num_experts);
+  GSB_REQUIRE(need >= 0 && (need == 0 || workspace) && aligned_to(256, (const char*)workspace), GSB_ERR_INVALID_ARGUMENT);
+  GSB_REQUIRE(workspace_bytes >= need, GSB_ERR_CAPACITY);
+  char* room = (char*)workspace;
+  u32* const ends = take_ends(num_experts, &room);
   if (few_grad(num_rows, k, n, num_experts, size, chunk_rows(num_rows, k, n, tile_columns(n, dtype, row_tiles_of_grad(k, num_experts)), num_experts) < num_rows))
-    return by_experts(ctx, num_experts, num_rows, offsets, [&](const Groups& g) {
+    return by_experts(ctx, num_experts, num_rows, offsets, ends, [&](const Groups& g) {
       const FewArgs a{g, rows, grad, rows_stride, grad_stride, 0, (u32)k, (u32)n, nullptr, nullptr};
       const bool wide = aligned_to(16, (const char*)grad) && (num_rows == 1 || grad_stride * size % 16 == 0);
       const int grid = few_grid(g.experts * ((k + kFewRows - 1) / kFewRows) * ((n + kFewColumns - 1) / kFewColumns));
@@ -1197,10 +1212,6 @@ extern "C" int gsb_expert_product_grad(gsb_ctx* ctx, void* stream_, const void* 
       GSB_LAUNCH_OK();
       return (int)GSB_OK;
     });
-  const int64_t need = gsb_expert_product_grad_workspace(rows, dtype, num_rows, k, rows_stride, grad, n, grad_stride, num_experts);
-  GSB_REQUIRE(need >= 0 && workspace && aligned_to(256, (const char*)workspace), GSB_ERR_INVALID_ARGUMENT);
-  GSB_REQUIRE(workspace_bytes >= need, GSB_ERR_CAPACITY);
-  char* room = (char*)workspace;
   CUtensorMap* maps = (CUtensorMap*)room;
   room += rounded(min(num_experts, (i64)kPlanExperts) * 2 * (i64)sizeof(CUtensorMap));
   Lines x = rows_operand(rows, dtype, num_rows, k, rows_stride), d = rows_operand(grad, dtype, num_rows, n, grad_stride);
@@ -1219,7 +1230,7 @@ extern "C" int gsb_expert_product_grad(gsb_ctx* ctx, void* stream_, const void* 
   CUtensorMap map_x = {}, map_d = {};
   const int read = x.copied() || d.copied() ? BY_WARPS : BY_TMA;
   if (!read && ((st = describe(x, 2, 64, 64, false, &map_x)) != GSB_OK || (st = describe(d, 2, 64, 64, false, &map_d)) != GSB_OK)) return st;
-  return by_experts(ctx, num_experts, num_rows, offsets, [&](const Groups& g) -> int {
+  return by_experts(ctx, num_experts, num_rows, offsets, ends, [&](const Groups& g) -> int {
     a.groups = g;
     if (!read) {
       ScopedKernelTimer timer(ctx, KID_EXPERT_PRODUCT, stream);
@@ -1259,7 +1270,7 @@ extern "C" int gsb_expert_product_int8(gsb_ctx* ctx, void* stream_, const int8_t
               GSB_ERR_INVALID_ARGUMENT);
   cudaStream_t stream = (cudaStream_t)stream_;
   if (few_rows(num_rows, k, n, num_experts, 1, false, 0))
-    return by_experts(ctx, num_experts, num_rows, offsets, [&](const Groups& g) {
+    return by_experts(ctx, num_experts, num_rows, offsets, nullptr, [&](const Groups& g) {
       const FewArgs a{g, values, weight_values, values_stride, weight_n_stride, num_experts > 1 ? weight_expert_stride : 0, (u32)k, (u32)n, scales, weight_scales};
       const int grid = few_grid((num_rows / kFewRows + min(num_rows, (i64)g.experts)) * ((n + kFewColumns - 1) / kFewColumns));
       ScopedKernelTimer timer(ctx, KID_EXPERT_PRODUCT, stream);
@@ -1281,7 +1292,7 @@ extern "C" int gsb_expert_product_int8(gsb_ctx* ctx, void* stream_, const int8_t
   a.weight_scales = weight_scales;
   CUtensorMap map_x, map_w;
   if ((st = describe(x, 1, 128, 128, false, &map_x)) != GSB_OK || (st = describe(w, 1, 128, a.columns / 2, true, &map_w)) != GSB_OK) return st;
-  return by_experts(ctx, num_experts, num_rows, offsets, [&](const Groups& g) {
+  return by_experts(ctx, num_experts, num_rows, offsets, nullptr, [&](const Groups& g) {
     a.groups = g;
     const i64 tiles = (num_rows / kPairRows + g.experts) * ((n + a.columns - 1) / a.columns);
     if (out_dtype == GSB_F32) return launch_tiles<float, true, 1, false, false, BY_TMA>(ctx, stream, map_x, map_w, a, tiles, num_rows, (float*)out);

@@ -80,6 +80,7 @@ __global__ void __launch_bounds__(kFewThreads) k_few_across(const FewArgs a, T* 
   await_previous();
   const Groups& g = a.groups;
   make_plan<kFewThreads>(plan, g, kFewRows, 0);
+  leave_end(plan, g);
   const u32 across = (a.n + kFewColumns - 1) / kFewColumns;
   const u64 tiles = (u64)plan.tile[g.experts] * across;
   const u32 part = threadIdx.x / 8, column = threadIdx.x % 8 * 8;
@@ -135,6 +136,7 @@ __global__ void __launch_bounds__(kFewThreads) k_few_along(const FewArgs a, Out*
   await_previous();
   const Groups& g = a.groups;
   make_plan<kFewThreads>(plan, g, kFewRows, 0);
+  leave_end(plan, g);
   const u32 across = (a.n + kFewColumns - 1) / kFewColumns;
   const u64 tiles = (u64)plan.tile[g.experts] * across;
   const int lane = threadIdx.x & 31;
@@ -226,6 +228,7 @@ __global__ void __launch_bounds__(kFewThreads) k_few_grad(const FewArgs a, T* __
   await_previous();
   const Groups& g = a.groups;
   make_plan<kFewThreads>(plan, g, 1, 0);
+  leave_end(plan, g);
   const u32 across = (a.n + kFewColumns - 1) / kFewColumns, down = (a.k + kFewRows - 1) / kFewRows;
   const u64 tiles = (u64)g.experts * across * down;
   const u32 part = threadIdx.x / 8, column = threadIdx.x % 8 * 8;

@@ -62,3 +62,59 @@ def test_negated_views_in_8_bits(ops):
         assert torch.count_nonzero(minus) > 0
         assert torch.equal(ops.expert_product_int8(torch._neg_view(values), scales, weight_values, weight_scales, offsets), minus)
         assert torch.equal(ops.expert_product_int8(values, scales, torch._neg_view(weight_values), weight_scales, offsets), minus)
+
+
+@pytest.mark.parametrize("rows_of_all,k,n", [(6_000, 24, 16), (40_000, 256, 128), (40_001, 250, 99)])
+def test_offsets_that_fall_from_one_launch_to_the_next(ops, rows_of_all, k, n):
+    """A launch takes 1 024 experts.  An offset below one of an earlier launch is raised to it as it is within a launch: no row is in two experts, and those
+    behind the last expert's are zeros."""
+    from graph_sampling_b200.cabi import GsbError
+    g, ctx, experts = generator(k), ops.Context(), 2500
+    good = torch.randint(0, rows_of_all + 1, (experts + 1,), generator=g, device="cuda").sort().values
+    falls = good.clone()
+    falls[500], falls[1024] = good[1100], good[3]                                # the second launch's first is below
+    far = good.clone()
+    far[10], far[1025:2049] = good[2300], good[1025:2049] // 2                   # the third's are below one of the first
+    end = good.clone()
+    end[-1] = end[2049] = 5                                                      # the last launch ends below where an earlier one does
+    for dtype in DTYPES:
+        rows, grad, weights = normal(g, rows_of_all, k, dtype=dtype), normal(g, rows_of_all, n, dtype=dtype), normal(g, experts, k, n, dtype=dtype)
+        values, scales = ops.quantize_rows(rows)
+        weight_values, weight_scales = ops.quantize_rows(weights.transpose(1, 2))
+        for offsets in (good, falls, far, end):
+            for call in (lambda: within(ops.expert_product(rows, weights, offsets, ctx=ctx), *exact.product(rows, weights, offsets)),
+                         lambda: within(ops.expert_product(grad, weights.transpose(1, 2), offsets, ctx=ctx),
+                                        *exact.product(grad, weights.transpose(1, 2), offsets)),
+                         lambda: within(ops.expert_product_grad(rows, grad, offsets, ctx=ctx), *exact.grad_weights(rows, grad, offsets)),
+                         lambda: within(ops.expert_product_int8(values, scales, weight_values, weight_scales, offsets, dtype, ctx=ctx),
+                                        *exact.product_int8(values, scales, weight_values, weight_scales, offsets))):
+                call()
+                if offsets is good:
+                    ctx.check_device()
+                else:
+                    with pytest.raises(GsbError) as e:
+                        ctx.check_device()
+                    assert e.value.status == -8
+
+
+def test_workspace_of_many_experts(ops):
+    """More than 1 024 experts want room for where each launch ends, whatever kernels the call goes to."""
+    ctx, g = ops.default_context(), generator(4)
+    rows, grad, weights = normal(g, 1500, 8), normal(g, 1500, 8), normal(g, 1500, 8, 8)
+    offsets = torch.arange(1501, device="cuda")
+    need = ctx.lib.gsb_expert_product_workspace(rows.data_ptr(), 0, 1500, 8, 8, weights.data_ptr(), 64, 8, 1, 8, 1500)
+    need_grad = ctx.lib.gsb_expert_product_grad_workspace(rows.data_ptr(), 0, 1500, 8, 8, grad.data_ptr(), 8, 8, 1500)
+    assert need > 0 and need_grad > 0
+    work, out, out_grad = torch.empty(max(need, need_grad), dtype=torch.uint8, device="cuda"), torch.empty_like(rows), torch.empty_like(weights)
+
+    def product(room, size):
+        return ctx.lib.gsb_expert_product(ctx.handle, stream(), rows.data_ptr(), 0, 1500, 8, 8, weights.data_ptr(), 64, 8, 1, 8, offsets.data_ptr(), 1500,
+                                          out.data_ptr(), room, size)
+
+    def product_grad(room, size):
+        return ctx.lib.gsb_expert_product_grad(ctx.handle, stream(), rows.data_ptr(), 0, 1500, 8, 8, grad.data_ptr(), 8, 8, offsets.data_ptr(), 1500,
+                                               out_grad.data_ptr(), room, size)
+    for call, size in ((product, need), (product_grad, need_grad)):
+        assert call(None, 0) == -1 and call(work.data_ptr(), size - 1) == -4 and call(work.data_ptr(), size) == 0
+    within(out, *exact.product(rows, weights, offsets))
+    within(out_grad, *exact.grad_weights(rows, grad, offsets))
