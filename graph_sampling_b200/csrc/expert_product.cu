@@ -25,7 +25,7 @@ constexpr int kSumColumns = 512;                 // of tensor memory: two tiles'
 constexpr int kRowsOperand = 128 * kLineBytes;   // bytes of a CTA's rows in a stage
 constexpr int kAcross = 64 * kLineBytes;         // a block of 64 lines
 // Warps: 0 loads by TMA, 1 (of the first CTA) issues the matrix instructions, 4 to 11 write results out, 12 to 19 read what TMA cannot, and 3
-// hands over what they have read.
+// hands over what they have read, or, of a gradient that TMA loads, the lines that an expert's rows end in.
 constexpr int kWriters = 8, kFirstReader = 4 + kWriters, kReaders = 8;
 constexpr int tile_threads(bool read) { return 32 * (kFirstReader + (read ? kReaders : 0)); }
 
@@ -62,7 +62,6 @@ struct TileArgs {
   u32 chunk;                 // rows of an expert that one tile of a gradient sums, a multiple of 64
   int stages;
   int expert_step;           // 0: one matrix for all experts
-  const CUtensorMap* maps;   // gradient: each expert's rows and gradient rows
   RawRows rows, grad;        // where they are read by warps
   u32 classes;               // of shifted rows
   bool by_tma;               // results may leave by TMA
@@ -309,8 +308,8 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
   if (threadIdx.x == 0) {
     stop = 0;
     for (int s = 0; s < kMaxStages; ++s) {
-      barrier_init(full + 8 * s, (READ && GRAD ? 0 : 1) + (READ ? 2 : 0));
-      barrier_init(written + 8 * s, kReaders);
+      barrier_init(full + 8 * s, (READ && GRAD ? 0 : 1) + (READ || GRAD ? 2 : 0));
+      barrier_init(written + 8 * s, READ ? kReaders : 1);
       barrier_init(empty + 8 * s, 1);
     }
     for (int s = 0; s < 2; ++s) {
@@ -322,10 +321,8 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
       barrier_init(slot_empty + 8 * s, kReaders);
     }
     barriers_ready();
-    if (!GRAD) {
-      if (!READ) prefetch_map((const CUtensorMap*)&map_a);
-      prefetch_map(&map_b);
-    }
+    if (!READ) prefetch_map((const CUtensorMap*)&map_a);
+    if (!READ || !GRAD) prefetch_map(&map_b);
   }
   if (warp == 2) sums_alloc(smem_address(&sums_at), kSumColumns);
   make_plan<tile_threads(READ)>(plan, g, GRAD ? a.chunk : kPairRows, GRAD ? 1 : 0);
@@ -345,14 +342,6 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
     for (u64 t = first; t < tiles; t += step) {
       const Tile tile = tile_at<GRAD, kPerLine>(a, plan, t);
       const CUtensorMap *of_a = (const CUtensorMap*)&map_a, *of_b = &map_b;
-      if (GRAD) {
-        of_a = a.maps + 2 * tile.e;
-        of_b = of_a + 1;
-        if (tile.blocks > 0) {
-          asm volatile("fence.proxy.tensormap::generic.acquire.gpu [%0], 128;" ::"l"(of_a) : "memory");
-          asm volatile("fence.proxy.tensormap::generic.acquire.gpu [%0], 128;" ::"l"(of_b) : "memory");
-        }
-      }
       const int matrix = (g.first + tile.e) * a.expert_step;
       // A second CTA without rows loads zeros from behind the array: no traffic, and products that cost the least power (1 to 2 % under the power
       // limit).  (Boxes of the 32 rows that a step has, which leave the rest as it was, were slower than one of 128: 64 rows to 64 experts 30 us
@@ -361,15 +350,23 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
       const u32 loaded_bytes = 2 * PARTS * ((READ ? 0 : kRowsOperand) + b_bytes);
       for (u32 b = 0; b < tile.blocks; ++b) {
         if (!barrier_wait(empty + 8 * stage, turn ^ 1, patience)) goto loaded;
-        if (rank == 0) barrier_expect(full + 8 * stage, loaded_bytes);
-        const u32 at = stages_at + stage * stage_bytes, bar = full_of_first + 8 * stage;
+        const u32 at = stages_at + stage * stage_bytes;
+        u32 bar = full_of_first + 8 * stage;
+        if (GRAD && b + 1 == tile.blocks && tile.rows % 64 != 0) {  // warp 3 hands it over
+          if (rank == 0) barrier_arrive(full + 8 * stage);
+          barrier_expect(written + 8 * stage, loaded_bytes / 2);
+          bar = address_in(written, rank) + 8 * stage;
+        } else {
+          if (rank == 0) barrier_expect(full + 8 * stage, loaded_bytes);
+          if (GRAD) barrier_arrive_at(bar);
+        }
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) {
           const u32 to_a = at + p * kRowsOperand, to_b = at + PARTS * kRowsOperand + p * b_bytes;
           if (GRAD) {
-            for (int j = 0; j < 2; ++j) load_tile(to_a + j * kAcross, of_a, bar, (int)(tile.m0 + rank * 128 + j * 64), (int)(tile.row0 + b * 64), p);
-            for (u32 j = 0; j < half / 64; ++j)
-              load_tile(to_b + j * kAcross, of_b, bar, (int)(tile.n0 + rank * half + j * 64), (int)(tile.row0 + b * 64), p);
+            const int row = (int)(plan.begin[tile.e] + tile.row0 + b * 64);
+            for (int j = 0; j < 2; ++j) load_tile(to_a + j * kAcross, of_a, bar, (int)(tile.m0 + rank * 128 + j * 64), row, p);
+            for (u32 j = 0; j < half / 64; ++j) load_tile(to_b + j * kAcross, of_b, bar, (int)(tile.n0 + rank * half + j * 64), row, p);
           } else {
             if (!READ) load_tile(to_a, of_a, bar, (int)(b * kPerLine), first_row, p);
             if (ACROSS)
@@ -435,6 +432,27 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
       }
     }
   brought:;
+  } else if (GRAD && !READ && warp == 3) {
+    // Behind an expert's last row are the next one's: where a line of the reduced index is none of its own, both operands are zeros.  (Descriptions
+    // that end where the expert's rows do, made on the device from the array's, are no way: TMA sends what is out of range to somewhere in the array
+    // as it was first described, which from a later beginning is behind its end, up to 32 KB, and faults where memory ends there too.)
+    const u32 full_of_first = address_in(full, 0);
+    u32 stage = 0, turns = 0;  // of which stages the next turn is an odd one
+    for (u64 t = first; t < tiles; t += step) {
+      const Tile tile = tile_at<GRAD, kPerLine>(a, plan, t);
+      const u32 lines = tile.rows % 64, last = (stage + tile.blocks - 1) % a.stages;
+      stage = (stage + tile.blocks) % a.stages;
+      if (lines == 0) continue;
+      const bool there = barrier_wait(written + 8 * last, turns >> last & 1, patience);
+      if (!__all_sync(0xffffffffu, there)) break;
+      turns ^= 1u << last;
+      const u32 zeros[4] = {}, at = stages_at + last * stage_bytes;
+      for (u32 j = 0; j < 2 + half / 64; ++j)  // the blocks of both operands
+        for (u32 piece = lines * (kLineBytes / 16) + lane; piece < 64 * (kLineBytes / 16); piece += 32) write_line(at + j * kAcross + piece * 16, zeros);
+      written_for_tensor_cores();
+      __syncwarp();
+      if (lane == 0) barrier_arrive_at(full_of_first + 8 * last);
+    }
   } else if (READ && warp == 3 && lane == 0) {
     // The readers' fence towards the tensor cores: theirs would wait for their copies that are on their way
     const u32 full_of_first = address_in(full, 0);
@@ -755,32 +773,6 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
   sums_fence_after();
   __syncwarp();
   if (warp == 2) sums_free(sums, kSumColumns);
-}
-
-// Descriptions of each expert's rows and gradient rows: the same arrays, from its first row on and as long as it has rows, so that loads
-// fill the rest of a tile with zeros.  A warp per expert and array.
-constexpr int kMapWarps = 8;
-__global__ void __launch_bounds__(32 * kMapWarps) k_expert_maps(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                                                                const Groups g, const char* a, i64 a_row_bytes, const char* b, i64 b_row_bytes,
-                                                                CUtensorMap* __restrict__ maps) {
-  __shared__ PlanTable plan;
-  __shared__ __align__(128) CUtensorMap held[kMapWarps];
-  await_previous();
-  make_plan<32 * kMapWarps>(plan, g, 1, 0);
-  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, which = blockIdx.x * kMapWarps + warp, e = which / 2;
-  if (e >= g.experts || plan.begin[e + 1] == plan.begin[e]) return;
-  const bool second = which & 1;
-  ((u32*)&held[warp])[lane] = ((const u32*)(second ? &map_b : &map_a))[lane];
-  __syncwarp();
-  const u32 at = smem_address(&held[warp]);
-  if (lane == 0) {
-    const u64 address = (u64)(uintptr_t)(second ? b + plan.begin[e] * b_row_bytes : a + plan.begin[e] * a_row_bytes);
-    asm volatile("tensormap.replace.tile.global_address.shared::cta.b1024.b64 [%0], %1;" ::"r"(at), "l"(address) : "memory");
-    asm volatile("tensormap.replace.tile.global_dim.shared::cta.b1024.b32 [%0], 1, %1;" ::"r"(at), "r"(plan.begin[e + 1] - plan.begin[e]) : "memory");
-  }
-  __syncwarp();
-  asm volatile("tensormap.cp_fenceproxy.global.shared::cta.tensormap::generic.release.gpu.sync.aligned [%0], [%1], 128;" ::"l"(maps + which), "r"(at)
-               : "memory");
 }
 
 // out[e] = the sum of the chunks of expert e, in their order.
@@ -1176,7 +1168,7 @@ extern "C" int64_t gsb_expert_product_grad_workspace(const void* rows, int dtype
   if (few_grad(num_rows, k, n, num_experts, value_bytes(dtype), chunk < num_rows)) return ends_bytes(num_experts);
   const Lines x = rows_operand(rows, dtype, num_rows, k, rows_stride), d = rows_operand(grad, dtype, num_rows, n, grad_stride);
   const i64 readers = grad_readers(k, n, tile_columns(n, dtype, row_tiles_of_grad(k, num_experts)));
-  return ends_bytes(num_experts) + rounded(min(num_experts, (i64)kPlanExperts) * 2 * (i64)sizeof(CUtensorMap)) + (rows_are_copied(x, readers, true) ? x.bytes() : 0) +
+  return ends_bytes(num_experts) + (rows_are_copied(x, readers, true) ? x.bytes() : 0) +
          (rows_are_copied(d, readers, true) ? d.bytes() : 0) + (chunk < num_rows ? rounded(most_chunks(num_rows, chunk, num_experts) * k * n * 4) : 0);
 }
 
@@ -1212,8 +1204,6 @@ extern "C" int gsb_expert_product_grad(gsb_ctx* ctx, void* stream_, const void* 
       GSB_LAUNCH_OK();
       return (int)GSB_OK;
     });
-  CUtensorMap* maps = (CUtensorMap*)room;
-  room += rounded(min(num_experts, (i64)kPlanExperts) * 2 * (i64)sizeof(CUtensorMap));
   Lines x = rows_operand(rows, dtype, num_rows, k, rows_stride), d = rows_operand(grad, dtype, num_rows, n, grad_stride);
   TileArgs a = {};
   a.columns = tile_columns(n, dtype, row_tiles_of_grad(k, num_experts));
@@ -1225,19 +1215,12 @@ extern "C" int gsb_expert_product_grad(gsb_ctx* ctx, void* stream_, const void* 
   a.n = (u32)n;
   const i64 chunk = chunk_rows(num_rows, k, n, a.columns, num_experts);
   a.chunk = (u32)chunk;
-  a.maps = maps;
   a.partial = chunk < num_rows ? (float*)room : nullptr;
   CUtensorMap map_x = {}, map_d = {};
   const int read = x.copied() || d.copied() ? BY_WARPS : BY_TMA;
   if (!read && ((st = describe(x, 2, 64, 64, false, &map_x)) != GSB_OK || (st = describe(d, 2, 64, 64, false, &map_d)) != GSB_OK)) return st;
   return by_experts(ctx, num_experts, num_rows, offsets, ends, [&](const Groups& g) -> int {
     a.groups = g;
-    if (!read) {
-      ScopedKernelTimer timer(ctx, KID_EXPERT_PRODUCT, stream);
-      launch_behind(stream, k_expert_maps, grid_for(2 * g.experts, kMapWarps), 32 * kMapWarps, map_x, map_d, g, (const char*)x.at, x.height > 1 ? x.stride * 2 : 0, (const char*)d.at,
-                    d.height > 1 ? d.stride * 2 : 0, maps);
-      GSB_LAUNCH_OK();
-    }
     const i64 tiles = (num_rows / chunk + g.experts) * ((k + kPairRows - 1) / kPairRows) * ((n + a.columns - 1) / a.columns);
     return with_type(dtype, read, [&](auto value, auto parts, auto reading) -> int {
       typedef decltype(value) T;

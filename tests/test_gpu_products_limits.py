@@ -118,3 +118,87 @@ def test_workspace_of_many_experts(ops):
         assert call(None, 0) == -1 and call(work.data_ptr(), size - 1) == -4 and call(work.data_ptr(), size) == 0
     within(out, *exact.product(rows, weights, offsets))
     within(out_grad, *exact.grad_weights(rows, grad, offsets))
+
+
+class MappedMemory:
+    """`size` bytes (a multiple of 2 MiB) with nothing mapped behind them, as a tensor of bytes."""
+    GRANULE = 2 << 20
+
+    def __init__(self, size):
+        self.cuda, self.size, self.address = ctypes.CDLL("libcuda.so.1"), size, ctypes.c_uint64(0)
+        self.handle = ctypes.c_uint64(0)
+        # CUmemAllocationProp: pinned memory of the current device; CUmemAccessDesc: to be read and written by it
+        device = torch.cuda.current_device()
+        prop, access = (ctypes.c_int32 * 8)(1, 0, 1, device, 0, 0, 0, 0), (ctypes.c_int32 * 3)(1, device, 3)
+        self.do("cuMemAddressReserve", ctypes.byref(self.address), ctypes.c_size_t(size + self.GRANULE), ctypes.c_size_t(0), ctypes.c_uint64(0), ctypes.c_uint64(0))
+        self.do("cuMemCreate", ctypes.byref(self.handle), ctypes.c_size_t(size), ctypes.byref(prop), ctypes.c_uint64(0))
+        self.do("cuMemMap", self.address, ctypes.c_size_t(size), ctypes.c_size_t(0), self.handle, ctypes.c_uint64(0))
+        self.do("cuMemSetAccess", self.address, ctypes.c_size_t(size), ctypes.byref(access), ctypes.c_size_t(1))
+        self.__cuda_array_interface__ = {"shape": (size,), "typestr": "|u1", "data": (self.address.value, False), "version": 3}
+        self.bytes = torch.as_tensor(self, device="cuda")
+        assert self.bytes.data_ptr() == self.address.value
+
+    def do(self, name, *args):
+        status = getattr(self.cuda, name)(*args)
+        assert status == 0, (name, status)
+
+    def last(self, rows, width, dtype):
+        """A matrix that ends where the memory does."""
+        size = torch.empty(0, dtype=dtype).element_size()
+        return self.bytes[self.size - rows * width * size:].view(dtype).view(rows, width)
+
+    def free(self):
+        torch.cuda.synchronize()
+        del self.bytes
+        self.do("cuMemUnmap", self.address, ctypes.c_size_t(self.size))
+        self.do("cuMemRelease", self.handle)
+        self.do("cuMemAddressFree", self.address, ctypes.c_size_t(self.size + self.GRANULE))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("k,n,counts", [(64, 64, [1] * 16384), (256, 320, [5000, 0, 3191]), (128, 64, [64] * 128 + [8191]), (512, 512, [2, 63, 65, 3966])])
+def test_rows_that_end_where_memory_does(ops, dtype, k, n, counts):
+    """Nothing is mapped behind the rows and the gradient's rows of an expert that ends inside a tile."""
+    g, offsets, rows = generator(k), torch.tensor([0] + counts, device="cuda").cumsum(0), sum(counts)
+    size = [(rows * width * 2 + (4 << 20) - 1) // (2 << 20) * (2 << 20) for width in (k, n)]
+    memory, other = MappedMemory(size[0]), MappedMemory(size[1])
+    x, d = memory.last(rows, k, dtype), other.last(rows, n, dtype)
+    x.copy_(normal(g, rows, k, dtype=dtype))
+    d.copy_(normal(g, rows, n, dtype=dtype))
+    got = ops.expert_product_grad(x, d, offsets)
+    out = ops.expert_product(x, normal(generator(1), len(counts), k, n, dtype=dtype), offsets)
+    torch.cuda.synchronize()
+    want = torch.zeros(got.shape, dtype=torch.float64, device="cuda")
+    error = torch.zeros_like(want)
+    if len(counts) == rows:  # one row each
+        want = x.double()[:, :, None] * d.double()[:, None, :]
+        error = 18 * exact.U * want.abs()
+    else:
+        want, error = exact.grad_weights(x, d, offsets)
+    within(got, want, error)
+    some = slice(0, offsets.numel() - 1) if len(counts) < 200 else slice(len(counts) - 50, len(counts))
+    weights = normal(generator(1), len(counts), k, n, dtype=dtype)
+    first, part = int(offsets[some.start]), offsets[some.start:some.stop + 1] - offsets[some.start]
+    within(out[first:], *exact.product(x[first:], weights[some], part))
+    x = d = None
+    memory.free()
+    other.free()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gradients_of_experts_that_end_inside_a_tile(ops, dtype):
+    """The next expert's rows, infinities and NaN among them, are none of an expert's, wherever in a line of 64 rows it ends."""
+    g = generator(6)
+    counts = [64 * (i % 3) + i for i in range(1, 64)] + [0, 64, 128, 1, 700, 3000]
+    offsets, n = torch.tensor([5] + counts, device="cuda").cumsum(0), sum(counts) + 5 + 70
+    for k, m in ((64, 64), (200, 136), (264, 520)):
+        rows, grad = normal(g, n, k, dtype=dtype), normal(g, n, m, dtype=dtype)
+        want, error = exact.grad_weights(rows, grad, offsets)
+        within(ops.expert_product_grad(rows, grad, offsets), want, error)
+        spoiled, spoiled_grad = rows.clone(), grad.clone()
+        for e in range(1, len(counts), 2):
+            spoiled[offsets[e]:offsets[e + 1]] = float("nan")
+            spoiled_grad[offsets[e]:offsets[e + 1]] = float("inf")
+        for at in (slice(0, 5), slice(int(offsets[-1]), n)):
+            spoiled[at], spoiled_grad[at] = float("inf"), float("nan")
+        within(ops.expert_product_grad(spoiled, spoiled_grad, offsets)[::2], want[::2], error[::2])
