@@ -106,6 +106,9 @@ __device__ __forceinline__ u32 blocks_at(const TileArgs& a, const PlanTable& pla
   if constexpr (GRAD) return tile_at<GRAD, PER_LINE>(a, plan, t).blocks;
   else return (a.depth + PER_LINE - 1) / PER_LINE;
 }
+// Lines of the reduced index that a matrix instruction takes.  A gradient's last block has as many instructions as its rows need, and only
+// in the last of them may there be lines that are none of the expert's.
+constexpr u32 kStepLines = 16;
 
 // 64 bytes of each of 32 rows of the result, a row a lane, leave through shared memory: by TMA where all 32 rows are wanted and begin on 16-byte
 // boundaries, else copied by neighbouring lanes, to `to`, `pitch` bytes apart, `bytes` of each, in accesses of `unit` bytes, which divide them.
@@ -290,7 +293,7 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
   extern __shared__ char raw[];
   __shared__ PlanTable plan;
   static_assert(READ != SHIFTED || (PARTS == 1 && !GRAD && !WHOLE_NUMBERS), "a product's rows of 16-bit values");
-  __shared__ __align__(8) u64 bars[3 * kMaxStages + 4 + 2 * kSlots];
+  __shared__ __align__(8) u64 bars[4 * kMaxStages + 4 + 2 * kSlots];
   __shared__ float column_scales[WHOLE_NUMBERS ? kWriters : 1][128];
   constexpr int kRooms = rooms_of(PARTS);
   __shared__ __align__(1024) char rooms[kWriters][kRooms * kRoom];
@@ -299,7 +302,7 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
   const u32 stages_at = (smem_address(raw) + 1023u) & ~1023u;
   const u32 full = smem_address(bars), empty = full + 8 * kMaxStages, written = full + 16 * kMaxStages;
   const u32 sums_full = full + 24 * kMaxStages, sums_empty = sums_full + 16;
-  const u32 slot_full = sums_empty + 16, slot_empty = slot_full + 8 * kSlots;
+  const u32 slot_full = sums_empty + 16, slot_empty = slot_full + 8 * kSlots, cut = slot_empty + 8 * kSlots;
   const u32 rank = rank_in_pair();
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   const Groups& g = a.groups;
@@ -308,8 +311,9 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
   if (threadIdx.x == 0) {
     stop = 0;
     for (int s = 0; s < kMaxStages; ++s) {
-      barrier_init(full + 8 * s, (READ && GRAD ? 0 : 1) + (READ || GRAD ? 2 : 0));
+      barrier_init(full + 8 * s, (READ && GRAD ? 0 : 1) + (READ ? 2 : 0));
       barrier_init(written + 8 * s, READ ? kReaders : 1);
+      barrier_init(cut + 8 * s, 2);
       barrier_init(empty + 8 * s, 1);
     }
     for (int s = 0; s < 2; ++s) {
@@ -352,13 +356,11 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
         if (!barrier_wait(empty + 8 * stage, turn ^ 1, patience)) goto loaded;
         const u32 at = stages_at + stage * stage_bytes;
         u32 bar = full_of_first + 8 * stage;
-        if (GRAD && b + 1 == tile.blocks && tile.rows % 64 != 0) {  // warp 3 hands it over
-          if (rank == 0) barrier_arrive(full + 8 * stage);
+        if (GRAD && b + 1 == tile.blocks && tile.rows % kStepLines != 0) {  // warp 3 hands it over
           barrier_expect(written + 8 * stage, loaded_bytes / 2);
           bar = address_in(written, rank) + 8 * stage;
-        } else {
-          if (rank == 0) barrier_expect(full + 8 * stage, loaded_bytes);
-          if (GRAD) barrier_arrive_at(bar);
+        } else if (rank == 0) {
+          barrier_expect(full + 8 * stage, loaded_bytes);
         }
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) {
@@ -382,20 +384,37 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
   loaded:;
   } else if (warp == 1 && rank == 0 && lane == 0) {
     constexpr bool A_ACROSS = GRAD, B_ACROSS = GRAD || ACROSS;
-    u32 stage = 0, turn = 0, made = 0;
+    u32 stage = 0, turn = 0, made = 0, full_turns = 0, cut_turns = 0;
     for (u64 t = first; t < tiles; t += step) {
-      const u32 blocks = blocks_at<GRAD, kPerLine>(a, plan, t);
+      u32 blocks, last_steps = 4;
+      bool last_cut = false;
+      if constexpr (GRAD && !READ) {
+        const Tile tile = tile_at<GRAD, kPerLine>(a, plan, t);
+        blocks = tile.blocks;
+        last_steps = ((tile.rows + 63) % 64 + kStepLines) / kStepLines;
+        last_cut = tile.rows % kStepLines != 0;
+      } else {
+        blocks = blocks_at<GRAD, kPerLine>(a, plan, t);
+      }
       for (u32 b0 = 0; b0 < blocks; b0 += min(kDrain, blocks - b0), ++made) {
         const u32 buffer = made & 1, to = sums + buffer * 256;
         if (!barrier_wait(sums_empty + 8 * buffer, (made >> 1 & 1) ^ 1, patience)) goto issued;
         sums_fence_after();
         for (u32 b = b0; b < b0 + min(kDrain, blocks - b0); ++b) {
-          if (!barrier_wait(full + 8 * stage, turn, patience)) goto issued;
+          if constexpr (GRAD && !READ) {
+            const bool from_cut = last_cut && b + 1 == blocks;
+            u32& turns = from_cut ? cut_turns : full_turns;
+            if (!barrier_wait((from_cut ? cut : full) + 8 * stage, turns >> stage & 1, patience)) goto issued;
+            turns ^= 1u << stage;
+          } else {
+            if (!barrier_wait(full + 8 * stage, turn, patience)) goto issued;
+          }
           sums_fence_after();
           const u32 at = stages_at + stage * stage_bytes;
           const u64 op_a = operand(at, kAcross), op_b = operand(at + PARTS * kRowsOperand, kAcross);
 #pragma unroll
           for (int s = 0; s < 4; ++s) {
+            if (GRAD && !READ && b + 1 == blocks && s >= (int)last_steps) break;
             const u64 a_s = op_a + s * ((A_ACROSS ? 16 * kLineBytes : 32) >> 4), b_s = op_b + s * ((B_ACROSS ? 16 * kLineBytes : 32) >> 4);
             const bool add = b > b0 || s > 0;
             multiply<WHOLE_NUMBERS>(to, a_s, b_s, a.how, add);
@@ -433,25 +452,26 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
     }
   brought:;
   } else if (GRAD && !READ && warp == 3) {
-    // Behind an expert's last row are the next one's: where a line of the reduced index is none of its own, both operands are zeros.  (Descriptions
+    // Behind an expert's last row are the next one's: where an instruction takes lines that are none of its own, both operands get zeros.  (Descriptions
     // that end where the expert's rows do, made on the device from the array's, are no way: TMA sends what is out of range to somewhere in the array
-    // as it was first described, which from a later beginning is behind its end, up to 32 KB, and faults where memory ends there too.)
-    const u32 full_of_first = address_in(full, 0);
+    // as it was first described, which from a later beginning is behind its end, up to 32 KB, and faults where memory ends there too.)  64 experts of
+    // 1 009 rows, 1 024 to 1 024, take 129.7 us, of 1 008, which need none of this, 128.7.
+    const u32 cut_of_first = address_in(cut, 0);
     u32 stage = 0, turns = 0;  // of which stages the next turn is an odd one
     for (u64 t = first; t < tiles; t += step) {
       const Tile tile = tile_at<GRAD, kPerLine>(a, plan, t);
-      const u32 lines = tile.rows % 64, last = (stage + tile.blocks - 1) % a.stages;
+      const u32 lines = tile.rows % 64, none = (kStepLines - lines % kStepLines) % kStepLines, last = (stage + tile.blocks - 1) % a.stages;
       stage = (stage + tile.blocks) % a.stages;
-      if (lines == 0) continue;
+      if (none == 0) continue;
+      const u32 zeros[4] = {}, at = stages_at + last * stage_bytes + lines * kLineBytes;
       const bool there = barrier_wait(written + 8 * last, turns >> last & 1, patience);
       if (!__all_sync(0xffffffffu, there)) break;
       turns ^= 1u << last;
-      const u32 zeros[4] = {}, at = stages_at + last * stage_bytes;
       for (u32 j = 0; j < 2 + half / 64; ++j)  // the blocks of both operands
-        for (u32 piece = lines * (kLineBytes / 16) + lane; piece < 64 * (kLineBytes / 16); piece += 32) write_line(at + j * kAcross + piece * 16, zeros);
+        for (u32 piece = lane; piece < none * (kLineBytes / 16); piece += 32) write_line(at + j * kAcross + piece * 16, zeros);
       written_for_tensor_cores();
       __syncwarp();
-      if (lane == 0) barrier_arrive_at(full_of_first + 8 * last);
+      if (lane == 0) barrier_arrive_at(cut_of_first + 8 * last);
     }
   } else if (READ && warp == 3 && lane == 0) {
     // The readers' fence towards the tensor cores: theirs would wait for their copies that are on their way
