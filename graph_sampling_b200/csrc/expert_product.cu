@@ -4,9 +4,10 @@
 // Its gradient for the rows is the product of the output's gradient with the transposed matrices, the same kernel; that for the
 // matrices is grad_W[e] = sum over the rows r of e of rows[r, :]^T grad[r, :].
 //
-// All run on the tensor cores.  float32 operands are taken apart into three bfloat16 parts, a = a0 + a1 + a2 with |a1| <= 2^-8 |a| and
-// |a2| <= 2^-16 |a|, exactly (24 bits are 3 times 8), and a b is the sum of the six products a_i b_j with i + j <= 2: what is left out is
-// 2^-23 |a b| at the very most.
+// All run on the tensor cores.  float32 operands are taken apart into three bfloat16 parts, a = a0 + a1 + a2 with |a1| < 2^-7 |a| and
+// |a2| <= 2^-16 |a|, and a b is the sum of the six products a_i b_j with i + j <= 2: what is left out is 2^-22 |a b| at the very most.  a0 is a
+// towards zero, so that a0 b0 leaves the range of float only where a b does; a1 and a2 are to nearest.  That is exact (24 bits are 3 times 8)
+// but for numbers below 2^-100, of which the parts that bfloat16 has no numbers for are lost.
 #include <atomic>
 #include <initializer_list>
 #include <type_traits>
@@ -213,30 +214,31 @@ __device__ __forceinline__ void read_eight(const float* from, int valid, int uni
     for (int q = 0; q < 8; ++q) v[q] = q < valid ? __ldg(from + q) : 0.f;
   }
 }
-// The next part of a float32 value, and what is left of it.  To nearest, but the largest numbers downwards, where that would be infinity.
-// Infinities and NaN are all in the first part.
-__device__ __forceinline__ u32 next_part(float& rest) {
-  const bool finite = fabsf(rest) <= 3.402823466e38f;
-  const __nv_bfloat16 part = finite && fabsf(rest) > 3.38e38f ? __float2bfloat16_rz(rest) : __float2bfloat16_rn(rest);
-  rest = finite ? rest - __bfloat162float(part) : 0.f;
+// The next part of a float32 value, and what is left of it: the first towards zero, the others to nearest.  Infinities and NaN are all in the
+// first part.
+__device__ __forceinline__ u32 next_part(float& rest, bool is_first) {
+  const __nv_bfloat16 part = is_first ? __float2bfloat16_rz(rest) : __float2bfloat16_rn(rest);
+  rest = fabsf(rest) <= 3.402823466e38f ? rest - __bfloat162float(part) : 0.f;
   return __bfloat16_as_ushort(part);
 }
-// Two parts of neighbours in a word; what is left of them stays.
+// Two parts of neighbours in a word; what is left of them stays.  Towards zero a part is the upper half.
+template <bool IS_FIRST>
 __device__ __forceinline__ u32 next_parts(float& low, float& high) {
   u32 w;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(high), "f"(low));
+  if constexpr (IS_FIRST) w = __byte_perm(__float_as_uint(low), __float_as_uint(high), 0x7632);
+  else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(high), "f"(low));
   low -= __uint_as_float(w << 16);
   high -= __uint_as_float(w & 0xffff0000u);
   return w;
 }
 // 8 values each of two lines, 32 apart, to their places, every part in an operand of its own, `apart` bytes from the one before.
 __device__ __forceinline__ void write_parts(const float (&x)[8], const float (&y)[8], u32 to, u32 apart) {
-  float rest[16], any = 0.f;  // what is left of an infinity, of NaN and of what became an infinity is none of the numbers
+  float rest[16], any = 0.f;  // what is left of an infinity and of NaN is none of the numbers
   u32 w[2][4];
 #pragma unroll
   for (int q = 0; q < 8; ++q) rest[q] = x[q], rest[8 + q] = y[q];
 #pragma unroll
-  for (int q = 0; q < 8; ++q) w[q / 4][q % 4] = next_parts(rest[2 * q], rest[2 * q + 1]);
+  for (int q = 0; q < 8; ++q) w[q / 4][q % 4] = next_parts<true>(rest[2 * q], rest[2 * q + 1]);
 #pragma unroll
   for (int q = 0; q < 4; ++q) any += (rest[4 * q] + rest[4 * q + 1]) + (rest[4 * q + 2] + rest[4 * q + 3]);
   if (fabsf(any) <= 3.402823466e38f) {
@@ -244,7 +246,7 @@ __device__ __forceinline__ void write_parts(const float (&x)[8], const float (&y
     for (int p = 0; p < 3; ++p) {
       if (p > 0)
 #pragma unroll
-        for (int q = 0; q < 8; ++q) w[q / 4][q % 4] = next_parts(rest[2 * q], rest[2 * q + 1]);
+        for (int q = 0; q < 8; ++q) w[q / 4][q % 4] = next_parts<false>(rest[2 * q], rest[2 * q + 1]);
       write_line(to + p * apart, w[0]);
       write_line(to + p * apart + 32 * kLineBytes, w[1]);
     }
@@ -255,8 +257,8 @@ __device__ __forceinline__ void write_parts(const float (&x)[8], const float (&y
     for (int p = 0; p < 3; ++p) {
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
-        const u32 low = next_part(rest[2 * q]);
-        w[q / 4][q % 4] = low | next_part(rest[2 * q + 1]) << 16;
+        const u32 low = next_part(rest[2 * q], p == 0);
+        w[q / 4][q % 4] = low | next_part(rest[2 * q + 1], p == 0) << 16;
       }
       write_line(to + p * apart, w[0]);
       write_line(to + p * apart + 32 * kLineBytes, w[1]);
@@ -418,7 +420,7 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
             const u64 a_s = op_a + s * ((A_ACROSS ? 16 * kLineBytes : 32) >> 4), b_s = op_b + s * ((B_ACROSS ? 16 * kLineBytes : 32) >> 4);
             const bool add = b > b0 || s > 0;
             multiply<WHOLE_NUMBERS>(to, a_s, b_s, a.how, add);
-            if (PARTS == 3) {  // the five small products have sums of their own, 2^-8 the size
+            if (PARTS == 3) {  // the five small products have sums of their own, 2^-7 the size
               const u64 next_a = kRowsOperand >> 4, next_b = b_bytes >> 4;
               multiply<false>(to + 128, a_s, b_s + next_b, a.how, add);
               multiply<false>(to + 128, a_s + next_a, b_s, a.how, true);
@@ -846,7 +848,7 @@ __global__ void __launch_bounds__(256) k_into_lines(const T* __restrict__ from, 
       } else {
         float rest = x + q < width ? row[x + q] : 0.f;
 #pragma unroll
-        for (int p = 0; p < PARTS; ++p) v[p][q] = (unsigned short)next_part(rest);
+        for (int p = 0; p < PARTS; ++p) v[p][q] = (unsigned short)next_part(rest, p == 0);
       }
     }
 #pragma unroll

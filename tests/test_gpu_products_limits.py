@@ -202,3 +202,116 @@ def test_gradients_of_experts_that_end_inside_a_tile(ops, dtype):
         for at in (slice(0, 5), slice(int(offsets[-1]), n)):
             spoiled[at], spoiled_grad[at] = float("inf"), float("nan")
         within(ops.expert_product_grad(spoiled, spoiled_grad, offsets)[::2], want[::2], error[::2])
+
+
+# ---- float32 on the tensor cores -------------------------------------------------------------------------------------------------------
+# Operands are taken apart into three parts, a = a0 + a1 + a2 exactly, the first towards zero: |a1| < 2^-7 |a|, |a2| <= 2^-16 |a|.  Left out are a1 b2,
+# a2 b1 and a2 b2, below 2^-22 (1 + 2^-10) |a b| together.  Where a sum has one product that is not zero, a0 b0 is exact, the five others, 2^-6 of it in
+# size, are added in five additions that cut less than 2^-23 of them each, and the two sums meet in one rounding of 2^-24.
+ONE_PRODUCT = 2.0 ** -22 + 2.0 ** -24 + 2.0 ** -26
+ROWS, K, N = 3000, 520, 512
+ENDS = [0, 1100, 1100, 2990]
+
+
+def by_tiles(ops, rows, weights, grad):
+    """All three calls of these operands go to the tensor cores: of float32 they want room for the weights' parts and for the rows' descriptions."""
+    lib, (n, k), (experts, _, m) = ops.default_context().lib, rows.shape, weights.shape
+    forward = lib.gsb_expert_product_workspace(rows.data_ptr(), 0, n, k, k, weights.data_ptr(), k * m, m, 1, m, experts)
+    back = lib.gsb_expert_product_workspace(grad.data_ptr(), 0, n, m, m, weights.data_ptr(), k * m, 1, m, k, experts)
+    return min(forward, back, lib.gsb_expert_product_grad_workspace(rows.data_ptr(), 0, n, k, k, grad.data_ptr(), m, m, experts)) > 0
+
+
+def one_product_each(g, near):
+    """Rows, weights and gradient rows of which every sum of a product, of the rows' gradient and of the weights' has one product that is not zero.  `near`:
+    all of those within 2^-9 of the largest number, above it none; else numbers of 24 bits around 1."""
+    def number(*shape):
+        x = 1 + torch.rand(*shape, generator=g, device="cuda") * (2 ** -10 if near else 1)
+        return x * torch.where(torch.rand(*shape, generator=g, device="cuda") < 0.5, -1.0, 1.0)
+    top = torch.finfo(torch.float32).max
+    low, high = (2.0 ** 63 * (1.25 + 0.75 / 128), 0.0) if near else (1.0, 1.0)  # to nearest in 8 bits both are larger
+    if near:  # (1 + 2^-10)^2 (1 + 2^-20) low high is the largest number
+        high = top / (low * (1 + 2 ** -10) ** 2 * (1 + 2 ** -20))
+    weights = number(3, K, N) * low
+    rows, grad = torch.zeros(ROWS, K, device="cuda"), torch.zeros(ROWS, N, device="cuda")
+    at = torch.arange(ROWS, device="cuda")
+    rows[at, at * 7 % K] = number(ROWS) * high
+    grad[at, at * 5 % N] = number(ROWS) * high
+    # of the weights' gradient: one row of each expert with numbers, the others zeros
+    alone, alone_grad = torch.zeros(ROWS, K, device="cuda"), torch.zeros(ROWS, N, device="cuda")
+    for a, b in ((0, 1100), (1100, 2990)):
+        alone[(a + 2 * b) // 3], alone_grad[(a + 2 * b) // 3] = number(K) * high, number(N) * low
+    return rows, weights, grad, alone, alone_grad
+
+
+def all_close(got, want, relative):
+    assert want.float().isfinite().all() and got.isfinite().all()
+    assert ((got.double() - want).abs() - relative * want.abs()).max().item() <= 0
+
+
+@pytest.mark.parametrize("near", [False, True])
+def test_float32_products_of_24_bits(ops, near):
+    """Every part of both operands counts: losing a product of a third part, or of two second ones, would be off by up to 2^-16 and 2^-14.  And a product that is
+    not infinite is none, however near the largest number it and its factors' first parts are."""
+    g, offsets = generator(11 + near), torch.tensor(ENDS, device="cuda")
+    rows, weights, grad, alone, alone_grad = one_product_each(g, near)
+    assert by_tiles(ops, rows, weights, grad)
+    all_close(ops.expert_product(rows, weights, offsets), exact.product(rows, weights, offsets)[0], ONE_PRODUCT)
+    turned = weights.transpose(1, 2)
+    all_close(ops.expert_product(grad, turned, offsets), exact.product(grad, turned, offsets)[0], ONE_PRODUCT)
+    all_close(ops.expert_product_grad(alone, alone_grad, offsets), exact.grad_weights(alone, alone_grad, offsets)[0], ONE_PRODUCT)
+
+
+def same_numbers(got, want, error):
+    """NaN and infinities where the definition in 64 bits has them, and numbers within the bound."""
+    narrow = want.float()
+    assert torch.equal(got.isnan(), narrow.isnan()) and torch.equal(got == float("inf"), narrow == float("inf"))
+    assert torch.equal(got == -float("inf"), narrow == -float("inf"))
+    fine = narrow.isfinite()
+    within(got[fine], want[fine], error[fine])
+
+
+def test_float32_infinities_and_nan(ops):
+    """In rows, weights and gradient rows, by ones and by whole rows, of some experts and of rows of none."""
+    g, offsets, inf, nan = generator(13), torch.tensor(ENDS, device="cuda"), float("inf"), float("nan")
+    rows, weights, grad = normal(g, ROWS, K), normal(g, 3, K, N), normal(g, ROWS, N)
+    assert by_tiles(ops, rows, weights, grad)
+    clean = rows.clone(), weights.clone(), grad.clone()
+
+    def all_three(rows, weights, grad):
+        for got, (want, _), (_, error) in ((ops.expert_product(rows, weights, offsets), exact.product(rows, weights, offsets), exact.product(clean[0], clean[1], offsets)),
+                                           (ops.expert_product(grad, weights.transpose(1, 2), offsets), exact.product(grad, weights.transpose(1, 2), offsets),
+                                            exact.product(clean[2], clean[1].transpose(1, 2), offsets)),
+                                           (ops.expert_product_grad(rows, grad, offsets), exact.grad_weights(rows, grad, offsets),
+                                            exact.grad_weights(clean[0], clean[2], offsets))):
+            same_numbers(got, want, error)
+    all_three(*clean)
+    for x, width in ((rows, K), (grad, N)):
+        x[7, 3], x[8, width - 1], x[130, 64], x[131, 63] = inf, -inf, nan, inf
+        x[1500, 5], x[1500, 6] = inf, -inf
+        x[2000], x[2995] = 0, nan
+        x[2000, 9] = inf
+    all_three(rows, clean[1], clean[2])
+    all_three(clean[0], clean[1], grad)
+    weights[0, 5, 7], weights[0, :, 100], weights[2, K - 1, N - 1], weights[2, 64, 64], weights[1] = inf, 0, -inf, nan, nan
+    all_three(clean[0], weights, clean[2])
+    all_three(rows, weights, grad)
+    weights[0, 5, 7] = weights[2, K - 1, N - 1] = torch.finfo(torch.float32).max  # and next to it the largest number alone
+    weights[2, 64, 64] = 0
+    rows[:, 5], rows[:, K - 1], grad[:, 7], grad[:, N - 1] = 0.5, -0.25, 0.125, 0.5
+    got, want = ops.expert_product(rows, weights, offsets), exact.product(rows, weights, offsets)[0]
+    assert torch.equal(got.isfinite(), want.float().isfinite())
+    got, want = ops.expert_product(grad, weights.transpose(1, 2), offsets), exact.product(grad, weights.transpose(1, 2), offsets)[0]
+    assert torch.equal(got.isfinite(), want.float().isfinite())
+
+
+def test_float32_root_mean_square(ops):
+    """What the documents say of the error of sums: 3e-7 of the result (rms).  Each of the six products of parts that are summed is above it."""
+    g, offsets = generator(14), torch.tensor(ENDS, device="cuda")
+    rows, weights, grad = normal(g, ROWS, K), normal(g, 3, K, N), normal(g, ROWS, N)
+    assert by_tiles(ops, rows, weights, grad)
+    for got, (want, _) in ((ops.expert_product(rows, weights, offsets), exact.product(rows, weights, offsets)),
+                           (ops.expert_product(grad, weights.transpose(1, 2), offsets), exact.product(grad, weights.transpose(1, 2), offsets)),
+                           (ops.expert_product_grad(rows, grad, offsets), exact.grad_weights(rows, grad, offsets))):
+        assert ((got.double() - want).pow(2).mean().sqrt() / want.pow(2).mean().sqrt()).item() < 6e-7
+
+
