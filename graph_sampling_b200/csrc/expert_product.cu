@@ -67,6 +67,7 @@ struct TileArgs {
   u32 classes;               // of shifted rows
   bool by_tma;               // results may leave by TMA
   float* partial;            // gradient: sums of the chunks (null: one chunk per expert, written out)
+  float* held;               // of 16-bit types: room for the sums that leave tensor memory before the last (null: none does)
   const float *row_scales, *weight_scales;  // of 8-bit operands
   u64 wait_limit;            // ns
   u32 how;
@@ -110,6 +111,10 @@ __device__ __forceinline__ u32 blocks_at(const TileArgs& a, const PlanTable& pla
 // Lines of the reduced index that a matrix instruction takes.  A gradient's last block has as many instructions as its rows need, and only
 // in the last of them may there be lines that are none of the expert's.
 constexpr u32 kStepLines = 16;
+// An addition to a sum in tensor memory cuts what is left of its 16 products below the sum's last bits: of positive numbers 6.4e-9 of the result
+// for each value that is summed (1 024 to 262 144 of them), 1.7e-3 over 262 144, where a float16 is rounded by 4.9e-4.  Longer sums of 16-bit types
+// than 16 384 values leave tensor memory after so many, and are added in float: 1.1e-4 (2 048 rows of 65 536 to 2 048 412 us for 399).
+constexpr u32 kHeldLines = 256, kHeldValues = 64 * kHeldLines;
 
 // 64 bytes of each of 32 rows of the result, a row a lane, leave through shared memory: by TMA where all 32 rows are wanted and begin on 16-byte
 // boundaries, else copied by neighbouring lanes, to `to`, `pitch` bytes apart, `bytes` of each, in accesses of `unit` bytes, which divide them.
@@ -289,9 +294,11 @@ template <class T, bool WHOLE_NUMBERS, int PARTS, bool GRAD, bool ACROSS, int RE
 __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_constant__ RowMaps<READ> map_a, const __grid_constant__ CUtensorMap map_b,
                                                                  const __grid_constant__ CUtensorMap map_out, const TileArgs a, T* __restrict__ out) {
   constexpr int kPerLine = kLineBytes / (WHOLE_NUMBERS ? 1 : 2);
-  // float32: sums leave tensor memory, where additions cut, after this many lines of the reduced index, and are added up in registers.
-  // Over 16 instructions that is an error of 2.3e-7 of the sums (rms), over 32 4.7e-7
-  constexpr u32 kDrain = PARTS > 1 ? 4 : 0xffffffffu;
+  // Sums leave tensor memory, where additions cut, after this many lines of the reduced index.  float32: over 16 instructions that is an error
+  // of 2.3e-7 of the sums (rms), over 32 4.7e-7, and they are added up in registers.  16-bit types: kHeldLines where there are more
+  u32 drain = PARTS > 1 ? 4 : 0xffffffffu;
+  if constexpr (PARTS == 1 && !WHOLE_NUMBERS)
+    if (a.held) drain = kHeldLines;
   extern __shared__ char raw[];
   __shared__ PlanTable plan;
   static_assert(READ != SHIFTED || (PARTS == 1 && !GRAD && !WHOLE_NUMBERS), "a product's rows of 16-bit values");
@@ -398,11 +405,11 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
       } else {
         blocks = blocks_at<GRAD, kPerLine>(a, plan, t);
       }
-      for (u32 b0 = 0; b0 < blocks; b0 += min(kDrain, blocks - b0), ++made) {
+      for (u32 b0 = 0; b0 < blocks; b0 += min(drain, blocks - b0), ++made) {
         const u32 buffer = made & 1, to = sums + buffer * 256;
         if (!barrier_wait(sums_empty + 8 * buffer, (made >> 1 & 1) ^ 1, patience)) goto issued;
         sums_fence_after();
-        for (u32 b = b0; b < b0 + min(kDrain, blocks - b0); ++b) {
+        for (u32 b = b0; b < b0 + min(drain, blocks - b0); ++b) {
           if constexpr (GRAD && !READ) {
             const bool from_cut = last_cut && b + 1 == blocks;
             u32& turns = from_cut ? cut_turns : full_turns;
@@ -708,33 +715,56 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
             column_scales[warp - 4][c] = n0 + c < a.n ? __ldg(a.weight_scales + (i64)(g.first + tile.e) * a.n + n0 + c) : 0.f;
           __syncwarp();
         }
-        const u32 buffer = made & 1;
-        const bool there = barrier_wait(sums_full + 8 * buffer, made >> 1 & 1, patience);
-        if (!__all_sync(0xffffffffu, there)) break;
-        sums_fence_after();
-        for (u32 c = 0; c < half; c += 32) {
-          u32 v[32];
-          __syncwarp();
-          read_sums(sums + (quarter << 16) + buffer * 256 + c0 + c, v);
-          sums_read();
-          if (c + 32 == half) {
-            sums_fence_before();
+        constexpr int kAtOnce = READ ? 8 : 32;  // that there are registers for
+        float* const held = a.held + (i64)(blockIdx.x * kWriters + warp - 4) * half * 32 + lane;  // read by the lane that wrote it
+        bool lost = false;
+        for (u32 b0 = 0; b0 < tile.blocks; b0 += min(drain, tile.blocks - b0), ++made) {
+          const u32 buffer = made & 1;
+          const bool there = barrier_wait(sums_full + 8 * buffer, made >> 1 & 1, patience);
+          if (!__all_sync(0xffffffffu, there)) {
+            lost = true;
+            break;
+          }
+          sums_fence_after();
+          const bool last = tile.blocks - b0 <= drain;
+          for (u32 c = 0; c < half; c += 32) {
+            u32 v[32];
             __syncwarp();
-            if (lane == 0) barrier_arrive_at(sums_empty_of_first + 8 * buffer);
-          }
-          float f[32];
+            read_sums(sums + (quarter << 16) + buffer * 256 + c0 + c, v);
+            sums_read();
+            if (c + 32 == half) {
+              sums_fence_before();
+              __syncwarp();
+              if (lane == 0) barrier_arrive_at(sums_empty_of_first + 8 * buffer);
+            }
+            float f[32];
 #pragma unroll
-          for (int q = 0; q < 32; ++q) {
-            if constexpr (WHOLE_NUMBERS) f[q] = (float)(int)v[q] * of_row * column_scales[warp - 4][c + q];
-            else f[q] = __uint_as_float(v[q]);
+            for (int q = 0; q < 32; ++q) {
+              if constexpr (WHOLE_NUMBERS) f[q] = (float)(int)v[q] * of_row * column_scales[warp - 4][c + q];
+              else f[q] = __uint_as_float(v[q]);
+            }
+            if constexpr (!WHOLE_NUMBERS) {
+              if (b0 > 0 || !last)
+#pragma unroll
+                for (int q = 0; q < 32; q += kAtOnce) {
+                  float* const at = held + (c + q) * 32;
+                  if (b0 > 0)
+#pragma unroll
+                    for (int i = 0; i < kAtOnce; ++i) f[q + i] += at[i * 32];
+                  if (!last)
+#pragma unroll
+                    for (int i = 0; i < kAtOnce; ++i) at[i * 32] = f[q + i];
+                  __syncwarp();
+                }
+            }
+            if (last) store(c, f);
           }
-          store(c, f);
         }
-        ++made;
+        if (lost) break;
       } else {
         float total[2][32] = {};
         bool lost = false;
-        for (u32 b0 = 0; b0 < tile.blocks; b0 += min(kDrain, tile.blocks - b0), ++made) {
+        for (u32 b0 = 0; b0 < tile.blocks; b0 += min(drain, tile.blocks - b0), ++made) {
           const u32 buffer = made & 1;
           const bool there = barrier_wait(sums_full + 8 * buffer, made >> 1 & 1, patience);
           if (!__all_sync(0xffffffffu, there)) {
@@ -1005,6 +1035,17 @@ static int launch_tiles(gsb_ctx* ctx, cudaStream_t stream, const RowMaps<READ>& 
   return GSB_OK;
 }
 
+// Room for the sums of 16-bit types that leave tensor memory before the last, of all CTAs; it follows the launches' ends in a workspace.
+static i64 held_bytes(i64 depth, int dtype, u32 columns) {
+  return dtype != GSB_F32 && depth > kHeldValues ? (i64)kNumSMs * kWriters * 32 * (columns / 2) * 4 : 0;
+}
+static float* take_held(i64 depth, int dtype, u32 columns, char** room) {
+  const i64 bytes = held_bytes(depth, dtype, columns);
+  float* const held = bytes > 0 ? (float*)*room : nullptr;
+  *room += bytes;
+  return held;
+}
+
 // Columns of a tile: narrow ones for narrow results, for float32, whose parts need the room, and where wide ones would leave half of the pairs of
 // CTAs without any (512 rows of 512 to 512 by eight experts 9.7 us for 12.6).  `row_tiles`: how many there are down the result.
 static u32 tile_columns(i64 n, int dtype, i64 row_tiles) { return dtype == GSB_F32 || n <= 128 || row_tiles * ((n + 255) / 256) <= kNumSMs / 4 ? 128 : 256; }
@@ -1054,8 +1095,8 @@ static i64 chunk_rows(i64 num_rows, i64 k, i64 n, u32 columns, i64 num_experts) 
   i64 chunk = (num_rows + wanted - 1) / wanted;
   if (num_experts >= wanted) chunk = num_rows;
   chunk = max(chunk, (i64)512);
-  // in tensor memory additions cut, by 2^-26 of the sum each: beyond so many rows a float16 would show it.  Where room for the chunks' sums
-  // is to be had; an expert of a million rows is 9e-4 off without
+  // Of more rows than this an expert is cut however many experts there are, where room for the chunks' sums is to be had: 600 000 rows of 256 to 256
+  // values, nearly all of one of 300 experts, take 1.6 ms for 3.5 without, of experts that are even 195 us for 116
   constexpr i64 kMostRows = 262144;
   if (chunk > kMostRows && (min(num_experts, (i64)kPlanExperts) + num_rows / kMostRows) * k * n * 4 <= (i64)1 << 30) chunk = kMostRows;
   return min((chunk + 63) / 64 * 64, ((num_rows + 63) / 64) * 64);
@@ -1109,8 +1150,8 @@ extern "C" int64_t gsb_expert_product_workspace(const void* rows, int dtype, int
   const i64 copied = matrices_operand(weights, dtype, num_experts, weights_expert_stride, k, weights_k_stride, n, weights_n_stride).bytes();
   if (few_rows(num_rows, k, n, num_experts, value_bytes(dtype), rows_are_lines(k, n, weights_k_stride, weights_n_stride), copied)) return ends_bytes(num_experts);
   const Lines x = rows_operand(rows, dtype, num_rows, k, rows_stride);
-  const i64 across = tiles_across(n, tile_columns(n, dtype, row_tiles_of(num_rows, num_experts)));
-  return ends_bytes(num_experts) + copied + (rows_are_copied(x, across, false) ? x.bytes() : 0);
+  const u32 columns = tile_columns(n, dtype, row_tiles_of(num_rows, num_experts));
+  return ends_bytes(num_experts) + held_bytes(k, dtype, columns) + copied + (rows_are_copied(x, tiles_across(n, columns), false) ? x.bytes() : 0);
 }
 
 extern "C" int gsb_expert_product(gsb_ctx* ctx, void* stream_, const void* rows, int dtype, int64_t num_rows, int64_t k, int64_t rows_stride,
@@ -1151,6 +1192,7 @@ extern "C" int gsb_expert_product(gsb_ctx* ctx, void* stream_, const void* rows,
     });
   TileArgs a = {};
   a.columns = tile_columns(n, dtype, row_tiles_of(num_rows, num_experts));
+  a.held = take_held(k, dtype, a.columns, &room);
   if ((st = bring(ctx, stream, &w, &room)) != GSB_OK) return st;
   if (rows_are_copied(x, tiles_across(n, a.columns), false) && (st = bring(ctx, stream, &x, &room)) != GSB_OK) return st;
   a.rows = raw_rows(x);
@@ -1186,11 +1228,12 @@ extern "C" int64_t gsb_expert_product_grad_workspace(const void* rows, int dtype
   if (value_bytes(dtype) == 0 || num_rows < 0 || num_rows >= ((i64)1 << 31) || k < 1 || k > GSB_MAX_ROW_LEN || n < 1 || n > GSB_MAX_ROW_LEN ||
       num_experts < 1 || num_experts > GSB_MAX_EXPERTS)
     return GSB_ERR_INVALID_ARGUMENT;
-  const i64 chunk = chunk_rows(num_rows, k, n, tile_columns(n, dtype, row_tiles_of_grad(k, num_experts)), num_experts);
+  const u32 columns = tile_columns(n, dtype, row_tiles_of_grad(k, num_experts));
+  const i64 chunk = chunk_rows(num_rows, k, n, columns, num_experts);
   if (few_grad(num_rows, k, n, num_experts, value_bytes(dtype), chunk < num_rows)) return ends_bytes(num_experts);
   const Lines x = rows_operand(rows, dtype, num_rows, k, rows_stride), d = rows_operand(grad, dtype, num_rows, n, grad_stride);
-  const i64 readers = grad_readers(k, n, tile_columns(n, dtype, row_tiles_of_grad(k, num_experts)));
-  return ends_bytes(num_experts) + (rows_are_copied(x, readers, true) ? x.bytes() : 0) +
+  const i64 readers = grad_readers(k, n, columns);
+  return ends_bytes(num_experts) + held_bytes(chunk, dtype, columns) + (rows_are_copied(x, readers, true) ? x.bytes() : 0) +
          (rows_are_copied(d, readers, true) ? d.bytes() : 0) + (chunk < num_rows ? rounded(most_chunks(num_rows, chunk, num_experts) * k * n * 4) : 0);
 }
 
@@ -1229,13 +1272,14 @@ extern "C" int gsb_expert_product_grad(gsb_ctx* ctx, void* stream_, const void* 
   Lines x = rows_operand(rows, dtype, num_rows, k, rows_stride), d = rows_operand(grad, dtype, num_rows, n, grad_stride);
   TileArgs a = {};
   a.columns = tile_columns(n, dtype, row_tiles_of_grad(k, num_experts));
+  const i64 chunk = chunk_rows(num_rows, k, n, a.columns, num_experts);
+  a.held = take_held(chunk, dtype, a.columns, &room);
   for (Lines* some : {&x, &d})
     if (rows_are_copied(*some, grad_readers(k, n, a.columns), true) && (st = bring(ctx, stream, some, &room)) != GSB_OK) return st;
   a.rows = raw_rows(x);
   a.grad = raw_rows(d);
   a.k = (u32)k;
   a.n = (u32)n;
-  const i64 chunk = chunk_rows(num_rows, k, n, a.columns, num_experts);
   a.chunk = (u32)chunk;
   a.partial = chunk < num_rows ? (float*)room : nullptr;
   CUtensorMap map_x = {}, map_d = {};

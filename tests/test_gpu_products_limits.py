@@ -315,3 +315,48 @@ def test_float32_root_mean_square(ops):
         assert ((got.double() - want).pow(2).mean().sqrt() / want.pow(2).mean().sqrt()).item() < 6e-7
 
 
+
+
+# ---- long sums of 16-bit types -----------------------------------------------------------------------------------------------------------
+# Tensor memory cuts what an addition of 16 products leaves below the sum's last bits.  By what was measured an instruction's products are held with two bits
+# more than the sum, whose last is 2^-23 of it at most: 16 products cut by 2^-25 and the sum by 2^-23 are 5 * 2^-23 of the running sum at the very most, half of that on average,
+# and of the final one, where all are positive, half again.  Sums leave it after 16 384 values, 1 024 instructions: 1 024 * 5 / 4 * 2^-23 = 1.5e-4 of the result
+# (1.1e-4 was measured).  The float additions of 62 such sums to a million values are below 62 / 2 * 2^-24 < 2^-19.
+LONG = 1024 * 5 / 4 * 2.0 ** -23 + 2.0 ** -19
+
+
+def positive(g, dtype, *shape):
+    return (torch.rand(*shape, generator=g, device="cuda") * 0.03 + 0.001).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("k,first", [(300_032, 0), (1_000_000, 0), (999_996, 0), (999_001, 0), (600_000, 1), (600_000, 2)])
+def test_products_over_long_rows(ops, dtype, k, first):
+    """By TMA, by TMA class by class, copied and read by warps (`first`: values in front of the first row, off 16-byte boundaries)."""
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB")
+    g = generator(k)
+    rows = positive(g, dtype, 500 * k + 8)[first:first + 500 * k].view(500, k)
+    offsets = torch.tensor([0, 150, 150, 490], device="cuda")
+    for n, turned in ((120, False), (250, True)):
+        weights = positive(g, dtype, 3, n, k).transpose(1, 2) if turned else positive(g, dtype, 3, k, n)
+        out = ops.expert_product(rows, weights, offsets)
+        want = exact.product(rows, weights, offsets)[0]
+        within(out, want, want.abs() * LONG)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("width", [512, 508])
+def test_gradients_over_long_experts(ops, dtype, width):
+    """So many matrices that there is no room for sums of chunks: an expert's million rows are summed in one."""
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB")
+    g, n, experts = generator(width), 1_000_000, 1040
+    rows, grad = positive(g, dtype, n, width), positive(g, dtype, n, width)
+    offsets = torch.full((experts + 1,), n - 3, dtype=torch.long, device="cuda")
+    offsets[:3] = torch.tensor([0, 0, 990_001], device="cuda")
+    out = ops.expert_product_grad(rows, grad, offsets)
+    for e, a, b in ((1, 0, 990_001), (2, 990_001, n - 3)):
+        want = sum(rows[i:min(i + 100_000, b)].double().t() @ grad[i:min(i + 100_000, b)].double() for i in range(a, b, 100_000))
+        within(out[e], want, want.abs() * LONG)
+    assert not out[0].any() and not out[3:].any()
