@@ -220,13 +220,18 @@ __device__ __forceinline__ void read_eight(const float* from, int valid, int uni
   }
 }
 // The next part of a float32 value, and what is left of it: the first towards zero, the others to nearest.  Infinities and NaN are all in the
-// first part.
+// first part.  OF_WEIGHT: it is 0 for zeros alone, so that infinity times a weight is NaN for them alone.
+template <bool OF_WEIGHT>
 __device__ __forceinline__ u32 next_part(float& rest, bool is_first) {
-  const __nv_bfloat16 part = is_first ? __float2bfloat16_rz(rest) : __float2bfloat16_rn(rest);
+  __nv_bfloat16 part = is_first ? __float2bfloat16_rz(rest) : __float2bfloat16_rn(rest);
+  if constexpr (OF_WEIGHT)
+    if (is_first && __bfloat162float(part) == 0.f && rest != 0.f) part = __ushort_as_bfloat16(rest < 0.f ? 0x8001 : 1);
   rest = fabsf(rest) <= 3.402823466e38f ? rest - __bfloat162float(part) : 0.f;
   return __bfloat16_as_ushort(part);
 }
-// Two parts of neighbours in a word; what is left of them stays.  Towards zero a part is the upper half.
+// Two parts of neighbours in a word; what is left of them stays.  Towards zero a part is the upper half, also where that is 0 and the number is
+// not: looking for such numbers, of no weight but in a product with infinity, cost products 3 to 11 % (500 000 rows of 256 to 256 403 us for
+// 393, their gradient 473 for 426).
 template <bool IS_FIRST>
 __device__ __forceinline__ u32 next_parts(float& low, float& high) {
   u32 w;
@@ -262,8 +267,8 @@ __device__ __forceinline__ void write_parts(const float (&x)[8], const float (&y
     for (int p = 0; p < 3; ++p) {
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
-        const u32 low = next_part(rest[2 * q], p == 0);
-        w[q / 4][q % 4] = low | next_part(rest[2 * q + 1], p == 0) << 16;
+        const u32 low = next_part<false>(rest[2 * q], p == 0);
+        w[q / 4][q % 4] = low | next_part<false>(rest[2 * q + 1], p == 0) << 16;
       }
       write_line(to + p * apart, w[0]);
       write_line(to + p * apart + 32 * kLineBytes, w[1]);
@@ -878,7 +883,7 @@ __global__ void __launch_bounds__(256) k_into_lines(const T* __restrict__ from, 
       } else {
         float rest = x + q < width ? row[x + q] : 0.f;
 #pragma unroll
-        for (int p = 0; p < PARTS; ++p) v[p][q] = (unsigned short)next_part(rest, p == 0);
+        for (int p = 0; p < PARTS; ++p) v[p][q] = (unsigned short)next_part<true>(rest, p == 0);
       }
     }
 #pragma unroll

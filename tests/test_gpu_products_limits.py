@@ -317,6 +317,23 @@ def test_float32_root_mean_square(ops):
 
 
 
+@pytest.mark.parametrize("exponent", [-149, -142, -134, -133, -130, -126])
+def test_float32_infinity_times_the_smallest_weights(ops, exponent):
+    """Infinity times a weight is NaN where the weight is 0, and else infinity, however small it is."""
+    g, offsets, inf = generator(15), torch.tensor(ENDS, device="cuda"), float("inf")
+    rows, weights, grad = torch.zeros(ROWS, K, device="cuda"), torch.zeros(3, K, N, device="cuda"), torch.zeros(ROWS, N, device="cuda")
+    sign = torch.where(torch.rand(3, 64, 64, generator=g, device="cuda") < 0.5, -1.0, 1.0)
+    weights[:, :64, :64] = (sign.double() * torch.randint(1, 3, (3, 64, 64), generator=g, device="cuda") * 2.0 ** exponent).float()
+    at = torch.arange(ROWS, device="cuda")
+    rows[at, at % 64] = grad[at, at % 64] = inf
+    assert by_tiles(ops, rows, weights, grad)
+    turned = weights.transpose(1, 2)
+    for got, want in ((ops.expert_product(rows, weights, offsets), exact.product(rows, weights, offsets)[0]),
+                      (ops.expert_product(grad, turned, offsets), exact.product(grad, turned, offsets)[0])):
+        assert (want == inf).any() and (want == -inf).any() and want.isnan().any()
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got == inf, want == inf) and torch.equal(got == -inf, want == -inf)
+
+
 # ---- long sums of 16-bit types -----------------------------------------------------------------------------------------------------------
 # Tensor memory cuts what an addition of 16 products leaves below the sum's last bits.  By what was measured an instruction's products are held with two bits
 # more than the sum, whose last is 2^-23 of it at most: 16 products cut by 2^-25 and the sum by 2^-23 are 5 * 2^-23 of the running sum at the very most, half of that on average,
