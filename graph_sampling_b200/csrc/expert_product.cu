@@ -108,8 +108,7 @@ __device__ __forceinline__ u32 blocks_at(const TileArgs& a, const PlanTable& pla
   if constexpr (GRAD) return tile_at<GRAD, PER_LINE>(a, plan, t).blocks;
   else return (a.depth + PER_LINE - 1) / PER_LINE;
 }
-// Lines of the reduced index that a matrix instruction takes.  A gradient's last block has as many instructions as its rows need, and only
-// in the last of them may there be lines that are none of the expert's.
+// Lines of the reduced index that a matrix instruction takes.
 constexpr u32 kStepLines = 16;
 // An addition to a sum in tensor memory cuts what is left of its 16 products below the sum's last bits: of positive numbers 6.4e-9 of the result
 // for each value that is summed (1 024 to 262 144 of them), 1.7e-3 over 262 144, where a float16 is rounded by 4.9e-4.  Longer sums of 16-bit types
@@ -366,21 +365,15 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
       // for 27.)
       const int first_row = rank == 0 || tile.rows > 128 ? (int)(tile.row0 + rank * 128) : (int)g.num_rows;
       const u32 loaded_bytes = 2 * PARTS * ((READ ? 0 : kRowsOperand) + b_bytes);
-      for (u32 b = 0; b < tile.blocks; ++b) {
-        if (!barrier_wait(empty + 8 * stage, turn ^ 1, patience)) goto loaded;
+      const u32 cut_blocks = GRAD && tile.rows % 64 != 0 ? 1 : 0;  // the last, which warp 3 hands over
+      const int grad_row = GRAD ? (int)(plan.begin[tile.e] + tile.row0) : 0;
+      auto load = [&](u32 b, u32 bar) {
         const u32 at = stages_at + stage * stage_bytes;
-        u32 bar = full_of_first + 8 * stage;
-        if (GRAD && b + 1 == tile.blocks && tile.rows % kStepLines != 0) {  // warp 3 hands it over
-          barrier_expect(written + 8 * stage, loaded_bytes / 2);
-          bar = address_in(written, rank) + 8 * stage;
-        } else if (rank == 0) {
-          barrier_expect(full + 8 * stage, loaded_bytes);
-        }
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) {
           const u32 to_a = at + p * kRowsOperand, to_b = at + PARTS * kRowsOperand + p * b_bytes;
           if (GRAD) {
-            const int row = (int)(plan.begin[tile.e] + tile.row0 + b * 64);
+            const int row = grad_row + (int)(b * 64);
             for (int j = 0; j < 2; ++j) load_tile(to_a + j * kAcross, of_a, bar, (int)(tile.m0 + rank * 128 + j * 64), row, p);
             for (u32 j = 0; j < half / 64; ++j) load_tile(to_b + j * kAcross, of_b, bar, (int)(tile.n0 + rank * half + j * 64), row, p);
           } else {
@@ -393,20 +386,29 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
           }
         }
         if (++stage == (u32)a.stages) stage = 0, turn ^= 1;
+      };
+      for (u32 b = 0; b + cut_blocks < tile.blocks; ++b) {
+        if (!barrier_wait(empty + 8 * stage, turn ^ 1, patience)) goto loaded;
+        if (rank == 0) barrier_expect(full + 8 * stage, loaded_bytes);
+        load(b, full_of_first + 8 * stage);
+      }
+      if (GRAD && cut_blocks) {
+        if (!barrier_wait(empty + 8 * stage, turn ^ 1, patience)) goto loaded;
+        if (rank == 0) barrier_arrive(full + 8 * stage);  // a turn like any other
+        barrier_expect(written + 8 * stage, loaded_bytes / 2);
+        load(tile.blocks - 1, address_in(written, rank) + 8 * stage);
       }
     }
   loaded:;
   } else if (warp == 1 && rank == 0 && lane == 0) {
     constexpr bool A_ACROSS = GRAD, B_ACROSS = GRAD || ACROSS;
-    u32 stage = 0, turn = 0, made = 0, full_turns = 0, cut_turns = 0;
+    u32 stage = 0, turn = 0, made = 0, cut_turns = 0;
     for (u64 t = first; t < tiles; t += step) {
-      u32 blocks, last_steps = 4;
-      bool last_cut = false;
+      u32 blocks, cut_lines = 0;
       if constexpr (GRAD && !READ) {
         const Tile tile = tile_at<GRAD, kPerLine>(a, plan, t);
         blocks = tile.blocks;
-        last_steps = ((tile.rows + 63) % 64 + kStepLines) / kStepLines;
-        last_cut = tile.rows % kStepLines != 0;
+        cut_lines = tile.rows % 64;
       } else {
         blocks = blocks_at<GRAD, kPerLine>(a, plan, t);
       }
@@ -414,23 +416,14 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
         const u32 buffer = made & 1, to = sums + buffer * 256;
         if (!barrier_wait(sums_empty + 8 * buffer, (made >> 1 & 1) ^ 1, patience)) goto issued;
         sums_fence_after();
-        for (u32 b = b0; b < b0 + min(drain, blocks - b0); ++b) {
-          if constexpr (GRAD && !READ) {
-            const bool from_cut = last_cut && b + 1 == blocks;
-            u32& turns = from_cut ? cut_turns : full_turns;
-            if (!barrier_wait((from_cut ? cut : full) + 8 * stage, turns >> stage & 1, patience)) goto issued;
-            turns ^= 1u << stage;
-          } else {
-            if (!barrier_wait(full + 8 * stage, turn, patience)) goto issued;
-          }
-          sums_fence_after();
+        auto issue = [&](bool onto, u32 steps) {  // the stage's block, onto what the sums are or as the first of them
           const u32 at = stages_at + stage * stage_bytes;
           const u64 op_a = operand(at, kAcross), op_b = operand(at + PARTS * kRowsOperand, kAcross);
 #pragma unroll
-          for (int s = 0; s < 4; ++s) {
-            if (GRAD && !READ && b + 1 == blocks && s >= (int)last_steps) break;
+          for (u32 s = 0; s < 4; ++s) {
+            if (s >= steps) break;
             const u64 a_s = op_a + s * ((A_ACROSS ? 16 * kLineBytes : 32) >> 4), b_s = op_b + s * ((B_ACROSS ? 16 * kLineBytes : 32) >> 4);
-            const bool add = b > b0 || s > 0;
+            const bool add = onto || s > 0;
             multiply<WHOLE_NUMBERS>(to, a_s, b_s, a.how, add);
             if (PARTS == 3) {  // the five small products have sums of their own, 2^-7 the size
               const u64 next_a = kRowsOperand >> 4, next_b = b_bytes >> 4;
@@ -443,7 +436,20 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
           }
           multiplied(empty + 8 * stage);
           if (++stage == (u32)a.stages) stage = 0, turn ^= 1;
+        };
+        const u32 end = b0 + min(drain, blocks - b0), whole_end = cut_lines > 0 && end == blocks ? end - 1 : end;
+        for (u32 b = b0; b < whole_end; ++b) {
+          if (!barrier_wait(full + 8 * stage, turn, patience)) goto issued;
+          sums_fence_after();
+          issue(b > b0, 4);
         }
+        if constexpr (GRAD && !READ)
+          if (whole_end < end) {  // as many instructions as have lines of the expert's
+            if (!barrier_wait(cut + 8 * stage, cut_turns >> stage & 1, patience)) goto issued;
+            cut_turns ^= 1u << stage;
+            sums_fence_after();
+            issue(whole_end > b0, (cut_lines + kStepLines - 1) / kStepLines);
+          }
         multiplied(sums_full + 8 * buffer);
       }
     }
@@ -469,14 +475,14 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
     // Behind an expert's last row are the next one's: where an instruction takes lines that are none of its own, both operands get zeros.  (Descriptions
     // that end where the expert's rows do, made on the device from the array's, are no way: TMA sends what is out of range to somewhere in the array
     // as it was first described, which from a later beginning is behind its end, up to 32 KB, and faults where memory ends there too.)  64 experts of
-    // 1 009 rows, 1 024 to 1 024, take 129.7 us, of 1 008, which need none of this, 128.7.
+    // 497 rows, 1 024 to 1 024, take 72.7 us, of 512, which need none of this, 72.2.
     const u32 cut_of_first = address_in(cut, 0);
     u32 stage = 0, turns = 0;  // of which stages the next turn is an odd one
     for (u64 t = first; t < tiles; t += step) {
       const Tile tile = tile_at<GRAD, kPerLine>(a, plan, t);
       const u32 lines = tile.rows % 64, none = (kStepLines - lines % kStepLines) % kStepLines, last = (stage + tile.blocks - 1) % a.stages;
       stage = (stage + tile.blocks) % a.stages;
-      if (none == 0) continue;
+      if (lines == 0) continue;
       const u32 zeros[4] = {}, at = stages_at + last * stage_bytes + lines * kLineBytes;
       const bool there = barrier_wait(written + 8 * last, turns >> last & 1, patience);
       if (!__all_sync(0xffffffffu, there)) break;
