@@ -293,16 +293,15 @@ struct Walk {
 };
 
 // PARTS: 3 for float32, else 1.  ACROSS: the second operand's lines hold the reduced index across them (a gradient's both do).  READ: how rows
-// (and a gradient's both operands) come.
-template <class T, bool WHOLE_NUMBERS, int PARTS, bool GRAD, bool ACROSS, int READ>
+// (and a gradient's both operands) come.  LONG: 16-bit types' sums may be longer than kHeldValues; what holds them would cost short calls 0.4 of 14 us.
+template <class T, bool WHOLE_NUMBERS, int PARTS, bool GRAD, bool ACROSS, int READ, bool LONG>
 __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_constant__ RowMaps<READ> map_a, const __grid_constant__ CUtensorMap map_b,
                                                                  const __grid_constant__ CUtensorMap map_out, const TileArgs a, T* __restrict__ out) {
   constexpr int kPerLine = kLineBytes / (WHOLE_NUMBERS ? 1 : 2);
+  static_assert(!LONG || (PARTS == 1 && !WHOLE_NUMBERS), "of 16-bit types");
   // Sums leave tensor memory, where additions cut, after this many lines of the reduced index.  float32: over 16 instructions that is an error
-  // of 2.3e-7 of the sums (rms), over 32 4.7e-7, and they are added up in registers.  16-bit types: kHeldLines where there are more
-  u32 drain = PARTS > 1 ? 4 : 0xffffffffu;
-  if constexpr (PARTS == 1 && !WHOLE_NUMBERS)
-    if (a.held) drain = kHeldLines;
+  // of 2.3e-7 of the sums (rms), over 32 4.7e-7, and they are added up in registers
+  constexpr u32 kDrain = PARTS > 1 ? 4 : LONG ? kHeldLines : 0xffffffffu;
   extern __shared__ char raw[];
   __shared__ PlanTable plan;
   static_assert(READ != SHIFTED || (PARTS == 1 && !GRAD && !WHOLE_NUMBERS), "a product's rows of 16-bit values");
@@ -326,7 +325,7 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
     for (int s = 0; s < kMaxStages; ++s) {
       barrier_init(full + 8 * s, (READ && GRAD ? 0 : 1) + (READ ? 2 : 0));
       barrier_init(written + 8 * s, READ ? kReaders : 1);
-      barrier_init(cut + 8 * s, 2);
+      if (GRAD && !READ) barrier_init(cut + 8 * s, 2);
       barrier_init(empty + 8 * s, 1);
     }
     for (int s = 0; s < 2; ++s) {
@@ -412,7 +411,7 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
       } else {
         blocks = blocks_at<GRAD, kPerLine>(a, plan, t);
       }
-      for (u32 b0 = 0; b0 < blocks; b0 += min(drain, blocks - b0), ++made) {
+      for (u32 b0 = 0; b0 < blocks; b0 += min(kDrain, blocks - b0), ++made) {
         const u32 buffer = made & 1, to = sums + buffer * 256;
         if (!barrier_wait(sums_empty + 8 * buffer, (made >> 1 & 1) ^ 1, patience)) goto issued;
         sums_fence_after();
@@ -437,7 +436,7 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
           multiplied(empty + 8 * stage);
           if (++stage == (u32)a.stages) stage = 0, turn ^= 1;
         };
-        const u32 end = b0 + min(drain, blocks - b0), whole_end = cut_lines > 0 && end == blocks ? end - 1 : end;
+        const u32 end = b0 + min(kDrain, blocks - b0), whole_end = cut_lines > 0 && end == blocks ? end - 1 : end;
         for (u32 b = b0; b < whole_end; ++b) {
           if (!barrier_wait(full + 8 * stage, turn, patience)) goto issued;
           sums_fence_after();
@@ -729,7 +728,7 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
         constexpr int kAtOnce = READ ? 8 : 32;  // that there are registers for
         float* const held = a.held + (i64)(blockIdx.x * kWriters + warp - 4) * half * 32 + lane;  // read by the lane that wrote it
         bool lost = false;
-        for (u32 b0 = 0; b0 < tile.blocks; b0 += min(drain, tile.blocks - b0), ++made) {
+        for (u32 b0 = 0; b0 < tile.blocks; b0 += min(kDrain, tile.blocks - b0), ++made) {
           const u32 buffer = made & 1;
           const bool there = barrier_wait(sums_full + 8 * buffer, made >> 1 & 1, patience);
           if (!__all_sync(0xffffffffu, there)) {
@@ -737,7 +736,7 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
             break;
           }
           sums_fence_after();
-          const bool last = tile.blocks - b0 <= drain;
+          const bool last = tile.blocks - b0 <= kDrain;
           for (u32 c = 0; c < half; c += 32) {
             u32 v[32];
             __syncwarp();
@@ -754,7 +753,7 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
               if constexpr (WHOLE_NUMBERS) f[q] = (float)(int)v[q] * of_row * column_scales[warp - 4][c + q];
               else f[q] = __uint_as_float(v[q]);
             }
-            if constexpr (!WHOLE_NUMBERS) {
+            if constexpr (LONG) {
               if (b0 > 0 || !last)
 #pragma unroll
                 for (int q = 0; q < 32; q += kAtOnce) {
@@ -775,7 +774,7 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
       } else {
         float total[2][32] = {};
         bool lost = false;
-        for (u32 b0 = 0; b0 < tile.blocks; b0 += min(drain, tile.blocks - b0), ++made) {
+        for (u32 b0 = 0; b0 < tile.blocks; b0 += min(kDrain, tile.blocks - b0), ++made) {
           const u32 buffer = made & 1;
           const bool there = barrier_wait(sums_full + 8 * buffer, made >> 1 & 1, patience);
           if (!__all_sync(0xffffffffu, there)) {
@@ -1009,11 +1008,15 @@ constexpr int stages_room(int parts) { return (227 - 14) * 1024 - rooms_of(parts
 // A wait is given up after GSB_OPT_MAX_POLLS of these: two seconds by default.
 constexpr u64 kNanosecondsPerPoll = 477;
 // Launches pairs of CTAs: at most one CTA per SM.  In the order of the stream, with no overlap of its neighbours' ends and beginnings: with
-// overlap, hundreds of copies and products queued one behind the other came to a halt, waiting CTAs of one kernel beside clusters of another
-// that need SMs as a whole.
+// overlap, hundreds of copies and products queued one behind the other once came to a halt.  Why is not known.  A successor is set up only when all CTAs
+// of its predecessor have begun, so it was not CTAs that wait beside pairs which have no room yet; at that time the writers also went from stores that some
+// lanes made alone to warp-wide reads of tensor memory without converging, which is mended.
 template <class T, bool WHOLE_NUMBERS, int PARTS, bool GRAD, bool ACROSS, int READ>
 static int launch_tiles(gsb_ctx* ctx, cudaStream_t stream, const RowMaps<READ>& map_a, const CUtensorMap& map_b, TileArgs a, i64 most_tiles, i64 out_rows, T* out) {
-  auto kernel = k_tiles<T, WHOLE_NUMBERS, PARTS, GRAD, ACROSS, READ>;
+  constexpr bool kHalves = PARTS == 1 && !WHOLE_NUMBERS;
+  const bool is_long = kHalves && a.held;
+  auto kernel = k_tiles<T, WHOLE_NUMBERS, PARTS, GRAD, ACROSS, READ, false>;
+  if (is_long) kernel = k_tiles<T, WHOLE_NUMBERS, PARTS, GRAD, ACROSS, READ, kHalves>;
   const int stage = PARTS * (kRowsOperand + (int)a.columns / 2 * kLineBytes);
   constexpr int kSlotsRoom = READ == SHIFTED ? kSlots * kSlotBytes : 0;
   a.stages = min(kMaxStages, (stages_room(PARTS) - kSlotsRoom) / stage);
@@ -1024,11 +1027,11 @@ static int launch_tiles(gsb_ctx* ctx, cudaStream_t stream, const RowMaps<READ>& 
   const int size = a.partial ? 4 : (int)sizeof(T);
   void* const results = a.partial ? (void*)a.partial : (void*)out;
   a.by_tma = (i64)a.n * size % 16 == 0 && aligned_to(16, (const char*)results) && out_rows < ((i64)1 << 31) && describe_rows(&map_out, results, size, a.n, (u64)out_rows);
-  static std::atomic<bool> allowed[64];  // on which devices the kernel may have all the shared memory it can ask for
+  static std::atomic<bool> allowed[2][64];  // on which devices the kernel may have all the shared memory it can ask for
   const int device = ctx_device(ctx);
-  if (device >= 64 || !allowed[device]) {
+  if (device >= 64 || !allowed[is_long][device]) {
     GSB_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, stages_room(PARTS) + 1024));
-    if (device < 64) allowed[device] = true;
+    if (device < 64) allowed[is_long][device] = true;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(2 * max((i64)1, min((i64)kNumSMs / 2, most_tiles))));
@@ -1126,7 +1129,7 @@ static int with_type(int dtype, int read, F f) {
   return read == BY_WARPS ? by_type(integral_constant<int, BY_WARPS>{}) : by_type(integral_constant<int, BY_TMA>{});
 }
 // A product's 16-bit rows that TMA cannot load line by line come class by class (shifted).  Of the others (from an address off 16-byte boundaries, all one row,
-// fewer than eight) and of a gradient's, for which rows of several classes would meet in one line of the reduced index, those are read by warps
+// fewer than eight) and of a gradient's, for which classes are not built (a line of its operands is one row, and so of one class, too), those are read by warps
 // that every tile reads once, and copied into lines those that several tiles of columns would read again (a product of 210 395 rows of 602 to 602 by 33
 // experts with both gradients 950 us for 1 190).  Rows that begin on odd values, which are read value by value, are copied for a gradient (300 000 of
 // 101 and 101 127 us for 254) and, where they are long, for a product.  Shifted against copied, products of 200 003 rows of 602 to 602 235 us for
