@@ -359,9 +359,9 @@ __global__ void __launch_bounds__(tile_threads(READ), 1) k_tiles(const __grid_co
       const Tile tile = tile_at<GRAD, kPerLine>(a, plan, t);
       const CUtensorMap *of_a = (const CUtensorMap*)&map_a, *of_b = &map_b;
       const int matrix = (g.first + tile.e) * a.expert_step;
-      // A second CTA without rows loads zeros from behind the array: no traffic, and products that cost the least power (1 to 2 % under the power
-      // limit).  (Boxes of the 32 rows that a step has, which leave the rest as it was, were slower than one of 128: 64 rows to 64 experts 30 us
-      // for 27.)
+      // A second CTA without rows loads zeros from behind the array: products that cost the least power (1 to 2 % under the power limit).  (Not the
+      // least traffic: for what is out of range TMA reads as many sectors somewhere in the array.  Boxes of the 32 rows that a step has, which leave the
+      // rest as it was, were slower than one of 128: 64 rows to 64 experts 30 us for 27.)
       const int first_row = rank == 0 || tile.rows > 128 ? (int)(tile.row0 + rank * 128) : (int)g.num_rows;
       const u32 loaded_bytes = 2 * PARTS * ((READ ? 0 : kRowsOperand) + b_bytes);
       const u32 cut_blocks = GRAD && tile.rows % 64 != 0 ? 1 : 0;  // the last, which warp 3 hands over
