@@ -660,7 +660,8 @@ GSB_API int gsb_expert_product_grad(gsb_ctx* ctx, void* stream, const void* rows
                                     const int64_t* offsets, int64_t num_experts, void* out, void* workspace,
                                     int64_t workspace_bytes);
 /* Rows in 8 bits: out_scales[r] = max |x[r, :]| / 127, out_values[r, :] = x[r, :] / out_scales[r] rounded to the nearest whole
- * number, ties to even (both divisions in IEEE float).  A row of zeros has the scale 0; one that holds an infinity or NaN has a
+ * number, ties to even (both divisions in IEEE float), and no further from 0 than 127, which only a scale below the normal numbers lets
+ * them exceed.  A row of zeros has the scale 0; one that holds an infinity or NaN has a
  * NaN for its scale and zeros for its values.  values_stride >= row_len: the product wants a multiple of 16. */
 GSB_API int gsb_quantize_rows(gsb_ctx* ctx, void* stream, const void* x, int dtype, int64_t num_rows, int64_t row_len,
                               int64_t x_stride, int8_t* out_values, int64_t values_stride, float* out_scales);
